@@ -49,6 +49,9 @@ extern "C" {
 #define JB200_STATUS_LSF_LOAD 0x31u
 #define JB200_STATUS_PEER_BARRIER 0x41u
 #define JB200_STATUS_STEP_CLUSTER 0x51u
+#define JB200_STATUS_HEAD_LOAD 0x61u
+#define JB200_STATUS_HEAD_MMA 0x62u
+#define JB200_STATUS_HEAD_EPILOGUE 0x63u
 #define JB200_STATUS_SELFTEST_WAIT 0x7Fu
 
 /* ---- library ----------------------------------------------------------------------- */
@@ -390,6 +393,55 @@ int jb200_forward_layers_prepared(const jb200_layer* layers, int n_layers, const
  * loss: f32 [1]. */
 int jb200_cross_entropy(const void* logits, int ld, int n_rows, int V, const int64_t* targets, float* row_loss,
                         const float* aux_a, int stride_a, const float* aux_b, int n_aux, float* loss, void* stream);
+
+/* ---- losses of the head from hidden rows, without the logits, and their gradients ------------------------ */
+
+/* lm_head and the loss on its logits (jarvis_engine/jarvis_model.py:535-540) as one operator: the N x V logits z = x w^T are never
+ * stored.  Cross entropy when `targets` is given, distillation from a teacher's top logits when `ids` is, or both of the same rows:
+ *   ce[n] = log sum_v exp(z[n][v]) - z[n][targets[n]]
+ *   kd[n] = t^2 * sum_k q[n][k] (log q[n][k] - log softmax(z[n] / t)[id[n][k]]),   t the temperature
+ * The losses and their statistics are f32; products accumulate in f32 from bf16 operands. */
+typedef struct jb200_head {
+  int N, V, C;                /* rows, vocabulary, channels (a multiple of 8, at least 64) */
+  const void* x;              /* bf16 [N][C], 16-byte aligned */
+  const void* w;              /* bf16 [V][C], 16-byte aligned */
+  const int64_t* targets;     /* [N] or NULL; -100: the row has none, its loss is 0; otherwise outside [0, V): its loss is NaN */
+  float* lse;                 /* [2][N], with targets: r and s with sum exp(z) = 2^r s, left by the forward call, read by the backward one */
+  int K;                      /* entries of a teacher's row, 1 to 256 */
+  const int32_t* ids;         /* [K][N] or NULL: what jb200_teacher_rows leaves */
+  const float* q;             /* [K][N] */
+  const float* neg_entropy;   /* [N] */
+  float temperature;
+  float* lse_t;               /* [2][N], with a teacher: the same of sum exp(z / temperature) */
+} jb200_head;
+
+/* Teacher rows (ids i64 [N][K], logits f32 or bf16 [N][K]) -> entries in ascending order of id with q = softmax(logits / temperature)
+ * over the row's entries, transposed, and sum q log q (+inf for a row without any, whose loss is 0; NaN where an id is >= V).  A
+ * negative id is no entry, whatever its logit.  An id may come twice: its probabilities add. */
+int jb200_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, int32_t* ids_sorted,
+                       float* q, float* neg_entropy, void* stream);
+
+/* ce, kd: f32 [N], where asked for.  means: NULL or f32 [4]: mean of ce over the rows with a target (NaN without any), their number, then
+ * the same of kd.  Without rows both means are NaN of 0.
+ * scratch: jb200_head_loss_scratch_bytes (ce, kd: whether asked for). */
+size_t jb200_head_loss_scratch_bytes(int N, int V, int ce, int kd);
+int jb200_head_loss(const jb200_head* h, float* ce, float* kd, float* means, void* scratch, void* stream);
+
+/* Gradients of sum_n g_ce[n] ce[n] / *n_ce + g_kd[n] kd[n] / *n_kd: dx [N][C] and dw [V][C] (dtype 0: f32, 1: bf16), overwritten, NULL
+ * where not wanted.  g_ce, g_kd: device f32, stride 0 (one value for all rows) or 1; n_ce, n_kd: device f32 or NULL (1).  The gradients of the logits are
+ * rounded to bf16, a piece of the vocabulary at a time.  A row without target and teacher has a gradient of 0 and no part in dw,
+ * whatever it holds.  dw 32-byte, scratch 256-byte aligned; sums are formed in a fixed order. */
+size_t jb200_head_loss_backward_scratch_bytes(int N, int V, int C);
+int jb200_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_stride, const float* n_ce, const float* g_kd, int g_kd_stride,
+                             const float* n_kd, void* dx, int dx_dtype, void* dw, int dw_dtype, void* scratch, void* stream);
+/* How such a pass is cut on a device with `sms` SMs: columns of a piece, pieces, slabs of dx. */
+int jb200_host_head_plan(int N, int V, int C, int sms, int32_t* out3);
+
+/* Gradient of jb200_rmsnorm: dx (x's dtype) and dw f32 [C], both overwritten; statistics are formed anew from x.  C a multiple of 8, at
+ * most 4096.  dw is summed in f32 in a fixed order. */
+size_t jb200_rmsnorm_backward_scratch_bytes(int n_rows, int C);
+int jb200_rmsnorm_backward(const void* x, int x_dtype, const float* w, float eps, const void* dy, int dy_dtype, int n_rows, int C, void* dx,
+                           float* dw, void* scratch, void* stream);
 
 /* ---- expert parallelism over peer memory (no counterpart: the reference is single-GPU) ------------------- */
 

@@ -195,7 +195,7 @@ extern "C" {
 
 const char* jb200_last_error(void) { return g_err; }
 
-int jb200_abi_version(void) { return 14; }
+int jb200_abi_version(void) { return 15; }
 
 long long jb200_kernel_launches(int reset) {
   return reset ? g_launches.exchange(0) : g_launches.load();
@@ -466,6 +466,27 @@ int jb200_cross_entropy(const void* logits, int ld, int n_rows, int V, const int
                         const float* aux_a, int stride_a, const float* aux_b, int n_aux, float* loss, void* stream) {
   return launch_cross_entropy(logits, ld, n_rows, V, targets, row_loss, aux_a, stride_a, aux_b, n_aux, loss,
                               static_cast<cudaStream_t>(stream));
+}
+
+int jb200_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, int32_t* ids_sorted,
+                       float* q, float* neg_entropy, void* stream) {
+  return launch_teacher_rows(ids, logits, logits_dtype, N, K, V, temperature, ids_sorted, q, neg_entropy, static_cast<cudaStream_t>(stream));
+}
+size_t jb200_head_loss_scratch_bytes(int N, int V, int ce, int kd) { return N < 1 || V < 1 ? 0 : head_loss_scratch_bytes(N, V, ce, kd); }
+int jb200_head_loss(const jb200_head* h, float* ce, float* kd, float* means, void* scratch, void* stream) {
+  return launch_head_loss(h, ce, kd, means, scratch, static_cast<cudaStream_t>(stream));
+}
+size_t jb200_head_loss_backward_scratch_bytes(int N, int V, int C) { return head_loss_backward_scratch_bytes(N, V, C); }
+int jb200_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_stride, const float* n_ce, const float* g_kd, int g_kd_stride,
+                             const float* n_kd, void* dx, int dx_dtype, void* dw, int dw_dtype, void* scratch, void* stream) {
+  return launch_head_loss_backward(h, g_ce, g_ce_stride, n_ce, g_kd, g_kd_stride, n_kd, dx, dx_dtype, dw, dw_dtype, scratch,
+                                   static_cast<cudaStream_t>(stream));
+}
+int jb200_host_head_plan(int N, int V, int C, int sms, int32_t* out3) { return head_plan_host(N, V, C, sms, out3); }
+size_t jb200_rmsnorm_backward_scratch_bytes(int n_rows, int C) { return rmsnorm_backward_scratch_bytes(n_rows, C); }
+int jb200_rmsnorm_backward(const void* x, int x_dtype, const float* w, float eps, const void* dy, int dy_dtype, int n_rows, int C, void* dx,
+                           float* dw, void* scratch, void* stream) {
+  return launch_rmsnorm_backward(x, x_dtype, w, eps, dy, dy_dtype, n_rows, C, dx, dw, scratch, static_cast<cudaStream_t>(stream));
 }
 
 int jb200_prepare_weights(const uint8_t* packed, size_t n_bytes, uint8_t* prepared, void* stream) {

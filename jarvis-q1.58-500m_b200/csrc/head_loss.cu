@@ -1,0 +1,860 @@
+// Losses of the language-model head straight from hidden rows and head weight: cross entropy, and distillation from a teacher's top
+// logits, with their gradients.  The reference computes logits = lm_head(x) and F.cross_entropy on them
+// (jarvis_engine/jarvis_model.py:535-540); here the N x V logits exist only in tensor memory.
+//
+//   z[n][v] = x[n] . w[v]                                        bf16 operands, f32 accumulation
+//   ce[n]   = log sum_v exp(z) - z[target]
+//   kd[n]   = tau^2 (sum_k q log q + log sum_v exp(z / tau) - sum_k q[k] z[id_k] / tau),   q = softmax_k(teacher / tau)
+//   dz      = g_ce (softmax(z) - 1[target]) + g_kd tau (softmax(z / tau) - sum_k q[k] 1[id_k])
+//
+// Forward: a product kernel whose epilogue keeps, per row of a 256 x 256 tile, the maximum, the sum of exponentials and the logits that
+// the target and the teacher ask for; a second kernel joins the tiles.  Backward: the same product again, whose epilogue writes dz
+// of a piece of the vocabulary as bf16 (the operand type of the products dx += dz W and dW = dz^T x that follow, head_grad.cu), so
+// that the workspace stays bounded whatever the vocabulary: 8 N V C operations for a training step, where 6 N V C would need the
+// logits kept.
+//
+// Exponentials are base 2 with a whole number as the reference point: 2^(z k - r), k the f32 value next to log2(e), has one rounding in its
+// argument and rescaling by 2^(r - r') has none.  A row's sum travels as the pair (r, sum 2^(z k - r)), and logarithms are divided by
+// that very k, so that logits of any size keep their differences.
+#include <float.h>
+#include <limits.h>
+
+#include "head_loss.cuh"
+#include "launchers.h"
+
+namespace jb {
+
+namespace {
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr int TEACHER_MAX = 256;
+constexpr size_t PIECE_BYTES = size_t(256) << 20;      // bf16 gradients of the logits kept at a time
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---------------------------------------------------------------------------
+// The teacher's rows: entries sorted by id (a tile's epilogue walks them in step with its columns) with their probabilities.
+// ---------------------------------------------------------------------------
+constexpr int TEACHER_ROWS = 32, TEACHER_WARPS = 8;
+
+template <typename T> __device__ __forceinline__ float teacher_value(const T* p);
+template <> __device__ __forceinline__ float teacher_value<float>(const float* p) { return *p; }
+template <> __device__ __forceinline__ float teacher_value<__nv_bfloat16>(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+
+// One warp takes a row at a time; [K][32 rows] tiles leave through shared memory, since the consumers' lanes are rows.
+// neg_entropy: sum q log q; +inf for a row without entries, NaN for one with an id beyond the vocabulary.
+template <typename T>
+__global__ void __launch_bounds__(32 * TEACHER_WARPS)
+teacher_rows_kernel(const int64_t* __restrict__ ids, const T* __restrict__ logits, int N, int K, int V, float inv_tau,
+                    int* __restrict__ ids_out, float* __restrict__ q_out, float* __restrict__ neg_entropy) {
+  pdl_wait();
+  pdl_trigger();
+  extern __shared__ int s_teacher[];
+  int* t_id = s_teacher;                                       // [K][33]
+  float* t_q = reinterpret_cast<float*>(t_id + K * 33);        // [K][33]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* w_id = t_id + 2 * K * 33 + warp * K;                    // [warps][K]: the row as it came
+  const int row0 = blockIdx.x * TEACHER_ROWS;
+  for (int r = warp; r < TEACHER_ROWS; r += TEACHER_WARPS) {
+    const int row = row0 + r;
+    if (row >= N) break;
+    constexpr int PER = TEACHER_MAX / 32;
+    float v[PER];
+    int id[PER];
+    bool bad = false;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int k = i * 32 + lane;
+      v[i] = -INFINITY;
+      id[i] = INT_MAX;
+      if (k < K) {
+        const long long y = ids[size_t(row) * K + k];
+        if (y >= 0) {
+          v[i] = teacher_value(logits + size_t(row) * K + k) * inv_tau;
+          if (y >= V) bad = true; else id[i] = int(y);
+        }
+        w_id[k] = id[i];
+        top = fmaxf(top, v[i]);
+      }
+    }
+    bad = __any_sync(0xffffffffu, bad);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // a row whose kept values are all -inf has no probabilities either (a NaN among them: NaN)
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float e = top == -INFINITY && v[i] == -INFINITY ? 0.f : expf(v[i] - (top == -INFINITY ? 0.f : top));
+      v[i] -= top;
+      sum += id[i] == INT_MAX ? 0.f : e;
+    }
+    sum = warp_sum(sum);
+    const float inv = 1.0f / sum, log_sum = logf(sum);
+    const bool none = sum == 0.f && !bad;
+    float ent = 0.f;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int k = i * 32 + lane;
+      if (k >= K) break;
+      float q = 0.f;
+      if (id[i] != INT_MAX && !none) {
+        if (v[i] != -INFINITY) {
+          q = expf(v[i]) * inv;
+          ent += q * (v[i] - log_sum);
+        }
+      }
+      int at = 0;                                              // its place: how many come before it
+      for (int j = 0; j < K; ++j) {
+        const int other = w_id[j];
+        at += other < id[i] || (other == id[i] && j < k);
+      }
+      t_id[at * 33 + r] = none ? INT_MAX : id[i];
+      t_q[at * 33 + r] = q;
+    }
+    ent = warp_sum(ent);
+    if (lane == 0) neg_entropy[row] = bad ? __int_as_float(0x7fc00000) : none ? INFINITY : ent;
+    __syncwarp();
+  }
+  __syncthreads();
+  const int rows = min(TEACHER_ROWS, N - row0);
+  for (int i = threadIdx.x; i < K * TEACHER_ROWS; i += 32 * TEACHER_WARPS) {
+    const int k = i >> 5, r = i & 31;
+    if (r < rows) {
+      ids_out[size_t(k) * N + row0 + r] = t_id[k * 33 + r];
+      q_out[size_t(k) * N + row0 + r] = t_q[k * 33 + r];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Logits of 256 rows x 256 vocabulary columns per CTA pair.
+// ---------------------------------------------------------------------------
+struct HeadLogits {
+  int N, V, C;
+  int v0, cols;              // vocabulary columns [v0, v0 + cols) of this launch
+  const int64_t* targets;    // CE
+  const int* ids;            // KD: [K][N], ascending in every row
+  const float* q;
+  int K;
+  float inv_tau;
+  float* part;               // statistics: [2 tiles + half][values][N]
+  float* z_target;           // [N]
+  // gradient, [3][N] each: the sum's reference point, the row's factor, and the factor over the sum
+  const float *r_ce, *r_kd;
+  __nv_bfloat16* g;          // gradient: [N][ldg]
+  int ldg;
+  unsigned int* status;
+};
+
+// Tiles of the same columns run side by side, so that a weight tile comes from HBM once; beyond 64 row tiles (32 MB of rows at 1024
+// channels) in groups, so that the group's rows stay in L2.
+constexpr int HEAD_GROUP = 64;
+__device__ __forceinline__ void head_tile(int t, int tm, int tv, int* m, int* v) {
+  const int g = t / (HEAD_GROUP * tv), base = g * HEAD_GROUP, size = min(HEAD_GROUP, tm - base);
+  const int r = t - base * tv;
+  *v = r / size;
+  *m = base + r - *v * size;
+}
+
+__device__ __forceinline__ float pick32(const uint32_t (&v)[32], int j) {
+  uint32_t a[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) a[i] = j & 16 ? v[i + 16] : v[i];
+#pragma unroll
+  for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+    for (int i = 0; i < w; ++i) a[i] = j & w ? a[i + w] : a[i];
+  return __uint_as_float(a[0]);
+}
+
+// Sum of 2^(z k) relative to 2^ref, ref a whole number.
+struct RunningSum {
+  float ref = -INFINITY, sum = 0.f;
+  __device__ __forceinline__ void add(const uint32_t (&v)[32], float top, float k) {
+    const float to = fmaxf(ref, rintf(top * k));
+    const float r = to == -INFINITY ? 0.f : to;                // nothing but -inf so far: all terms are 0 (or NaN)
+    float s0 = ref == -INFINITY ? sum : sum * ex2(ref - r), s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      s0 += ex2(fmaf(__uint_as_float(v[j]), k, -r));
+      s1 += ex2(fmaf(__uint_as_float(v[j + 1]), k, -r));
+      s2 += ex2(fmaf(__uint_as_float(v[j + 2]), k, -r));
+      s3 += ex2(fmaf(__uint_as_float(v[j + 3]), k, -r));
+    }
+    sum = (s0 + s1) + (s2 + s3);
+    ref = to;
+  }
+};
+
+constexpr int head_values(bool ce, bool kd) { return (ce ? 2 : 0) + (kd ? 3 : 0); }
+
+// A lane of an epilogue warp is a row, its registers are 32 consecutive columns.  Bound by the tensor pipe: a tile is 8 C / 64 x 512
+// cycles of MMA against about 1200 issue cycles of epilogue.
+template <bool CE, bool KD, bool GRAD>
+__global__ void __launch_bounds__(HEAD_THREADS, 1)
+head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
+                   const __grid_constant__ HeadLogits p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  const uint32_t a_base = base, b_base = base + HEAD_STAGES * HEAD_OPERAND;
+  HeadRing* ctl = reinterpret_cast<HeadRing*>(smem_raw + (base - raw_addr) + 2 * HEAD_STAGES * HEAD_OPERAND);
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int rank = int(cluster_rank());
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmap_x);
+    tma_prefetch_desc(&tmap_w);
+  }
+  pair_ring_init(ctl, warp);
+  pdl_wait();
+  pdl_trigger();
+  const uint32_t tmem = ctl->tmem_base;
+  volatile uint32_t* abort_flag = &ctl->abort_flag;
+  const int pair = int(blockIdx.x >> 1), n_pairs = int(gridDim.x >> 1);
+  const int tm = (p.N + HEAD_TILE - 1) / HEAD_TILE, tv = (p.cols + HEAD_TILE - 1) / HEAD_TILE, total = tm * tv;
+  const int n_kb = (p.C + HEAD_BK - 1) / HEAD_BK;
+
+  if (warp == 0) {
+    // ---------------- TMA: this CTA's rows and its half of the columns ----------------
+    int s = 0;
+    uint32_t ph = 1u;
+    bool ok = true;
+    for (int t = pair; ok && t < total; t += n_pairs) {
+      int m, v;
+      head_tile(t, tm, tv, &m, &v);
+      const int row = m * HEAD_TILE + rank * (HEAD_TILE / 2), col = p.v0 + v * HEAD_TILE + rank * (HEAD_TILE / 2);
+#pragma unroll 1
+      for (int kb = 0; kb < n_kb; ++kb) {
+        if (!mbar_wait(smem_u32(&ctl->empty[s]), ph, abort_flag, p.status, JB200_STATUS_HEAD_LOAD)) { ok = false; break; }
+        const uint32_t full = cluster_map(smem_u32(&ctl->full[s]), 0u);
+        if (elect_one()) {
+          if (rank == 0) mbar_arrive_expect_tx(smem_u32(&ctl->full[s]), 4 * HEAD_OPERAND);       // of both CTAs
+          pair_tma_load_2d(a_base + uint32_t(s) * HEAD_OPERAND, &tmap_x, kb * HEAD_BK, row, full);
+          pair_tma_load_2d(b_base + uint32_t(s) * HEAD_OPERAND, &tmap_w, kb * HEAD_BK, col, full);
+        }
+        __syncwarp();
+        if (++s == HEAD_STAGES) { s = 0; ph ^= 1u; }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA: the leader's, for both CTAs ----------------
+    if (rank == 0) {
+      const uint64_t ad0 = umma_desc_k_sw128(a_base), bd0 = umma_desc_k_sw128(b_base);
+      constexpr uint32_t idesc = umma_idesc_bf16(HEAD_TILE, HEAD_TILE);
+      int s = 0;
+      uint32_t ph = 0u, tile = 0u;
+      bool ok = true;
+      for (int t = pair; ok && t < total; t += n_pairs, ++tile) {
+        const uint32_t acc = tile & 1u;
+        if (!cluster_mbar_wait(smem_u32(&ctl->acc_empty[acc]), ((tile >> 1) & 1u) ^ 1u, abort_flag, p.status, JB200_STATUS_HEAD_MMA)) break;
+        tc_fence_after_sync();
+        const uint32_t d = tmem + acc * HEAD_TILE;
+#pragma unroll 1
+        for (int kb = 0; kb < n_kb; ++kb) {
+          if (!cluster_mbar_wait(smem_u32(&ctl->full[s]), ph, abort_flag, p.status, JB200_STATUS_HEAD_MMA)) { ok = false; break; }
+          tc_fence_after_sync();
+          if (elect_one()) {
+            const uint64_t ad = ad0 + uint64_t(s * (HEAD_OPERAND >> 4)), bd = bd0 + uint64_t(s * (HEAD_OPERAND >> 4));
+#pragma unroll
+            for (int kk = 0; kk < HEAD_BK / 16; ++kk)
+              pair_umma(d, ad + uint64_t(kk * 2), bd + uint64_t(kk * 2), idesc, (kb | kk) != 0 ? 1u : 0u);
+            pair_commit(smem_u32(&ctl->empty[s]));
+            if (kb + 1 == n_kb) pair_commit(smem_u32(&ctl->acc_full[acc]));
+          }
+          __syncwarp();
+          if (++s == HEAD_STAGES) { s = 0; ph ^= 1u; }
+        }
+      }
+    }
+  } else {
+    // ---------------- epilogue ----------------
+    const int quarter = warp & 3;                              // TMEM lanes this warp may read
+    const int half = (warp - HEAD_EPI_WARP0) >> 2;             // which of the alternating 32-column chunks
+    const float k1 = LOG2E, k2 = LOG2E * p.inv_tau;
+    uint32_t tile = 0u;
+    for (int t = pair; t < total; t += n_pairs, ++tile) {
+      const uint32_t acc = tile & 1u;
+      int m, v;
+      head_tile(t, tm, tv, &m, &v);
+      const int f0 = p.v0 + v * HEAD_TILE;                     // first vocabulary column, and the first beyond the launch's
+      const int f_end = min(f0 + HEAD_TILE, p.v0 + p.cols);
+      const int row = m * HEAD_TILE + rank * (HEAD_TILE / 2) + quarter * 32 + lane;
+      const bool on = row < p.N;
+      int target = -1;
+      if (CE && on) {
+        const long long y = p.targets[row];
+        if (y >= f0 && y < f_end) target = int(y) - f0;
+      }
+      // the row's first entry in this tile
+      int at = p.K, next = INT_MAX;
+      const int* ids = p.ids + row;
+      const float* q = p.q + row;
+      if (KD && on) {
+        int lo = 0, hi = p.K;
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (__ldg(ids + size_t(mid) * p.N) < f0) lo = mid + 1; else hi = mid;
+        }
+        at = lo;
+        if (at < p.K) next = __ldg(ids + size_t(at) * p.N);
+      }
+      float l1 = 0.f, l2 = 0.f, g1 = 0.f, g2 = 0.f, p1 = 0.f, p2 = 0.f;
+      if (GRAD && on) {
+        if (CE) { l1 = p.r_ce[row]; g1 = p.r_ce[size_t(p.N) + row]; p1 = p.r_ce[2 * size_t(p.N) + row]; }
+        if (KD) { l2 = p.r_kd[row]; g2 = p.r_kd[size_t(p.N) + row]; p2 = p.r_kd[2 * size_t(p.N) + row]; }
+      }
+      RunningSum s1, s2;
+      float dot = 0.f;
+      if (!mbar_wait(smem_u32(&ctl->acc_full[acc]), (tile >> 1) & 1u, abort_flag, p.status, JB200_STATUS_HEAD_EPILOGUE)) break;
+      tc_fence_after_sync();
+      __syncwarp();
+      const uint32_t t_lane = tmem + (uint32_t(quarter * 32) << 16) + acc * HEAD_TILE;
+      for (int c0 = half * 32; c0 < HEAD_TILE; c0 += 64) {
+        const int col = f0 + c0;
+        if (!GRAD && col >= f_end) break;
+        uint32_t z[32];
+        tmem_ld_32x32(t_lane + c0, z);
+        tmem_ld_wait();
+        if constexpr (GRAD) {
+          float g[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float x = __uint_as_float(z[j]);
+            float y = 0.f;
+            if (CE) y = p1 * ex2(fmaf(x, k1, -l1));
+            if (KD) y = fmaf(p2, ex2(fmaf(x, k2, -l2)), y);
+            g[j] = y;
+          }
+          if (CE && __any_sync(0xffffffffu, unsigned(target - c0) < 32u)) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (target - c0 == j) g[j] -= g1;
+          }
+          if (KD) {
+            while (__any_sync(0xffffffffu, next < col + 32)) {
+              if (next < col + 32) {
+                const int j0 = next - col;                     // below 0: the other half's
+                const float d = j0 < 0 ? 0.f : g2 * __ldg(q + size_t(at) * p.N);
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (j0 == j) g[j] -= d;
+                ++at;
+                next = at < p.K ? __ldg(ids + size_t(at) * p.N) : INT_MAX;
+              }
+              __syncwarp();
+            }
+          }
+          if (col + 32 > f_end) {                              // columns past the vocabulary: the products read zeros
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col + j >= f_end) g[j] = 0.f;
+          }
+          if (on) {
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(g[2 * j], g[2 * j + 1]);
+            __nv_bfloat16* d = p.g + size_t(row) * p.ldg + (col - p.v0);
+            st_global_256(d, w);
+            st_global_256(d + 16, w + 8);
+          }
+        } else {
+          if (CE && __any_sync(0xffffffffu, unsigned(target - c0) < 32u)) {
+            const float x = pick32(z, target - c0);
+            if (unsigned(target - c0) < 32u) p.z_target[row] = x;
+          }
+          if (KD) {
+            while (__any_sync(0xffffffffu, next < col + 32)) {
+              if (next < col + 32) {
+                const int j0 = next - col;
+                if (j0 >= 0) {
+                  const float w = __ldg(q + size_t(at) * p.N);
+                  if (w != 0.f) dot = fmaf(w, pick32(z, j0), dot);
+                }
+                ++at;
+                next = at < p.K ? __ldg(ids + size_t(at) * p.N) : INT_MAX;
+              }
+              __syncwarp();
+            }
+          }
+          if (col + 32 > f_end) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col + j >= f_end) z[j] = 0xff800000u;        // -inf
+          }
+          float top = __uint_as_float(z[0]);
+#pragma unroll
+          for (int j = 1; j < 32; ++j) top = fmaxf(top, __uint_as_float(z[j]));
+          if (CE) s1.add(z, top, k1);
+          if (KD) s2.add(z, top, k2);
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) cluster_mbar_arrive(cluster_map(smem_u32(&ctl->acc_empty[acc]), 0u));
+      if (!GRAD && on) {
+        constexpr int F = head_values(CE, KD);
+        float* o = p.part + size_t(2 * v + half) * F * p.N + row;
+        if (CE) { o[0] = s1.ref; o[p.N] = s1.sum; o += 2 * size_t(p.N); }
+        if (KD) { o[0] = s2.ref; o[p.N] = s2.sum; o[2 * size_t(p.N)] = dot; }
+      }
+    }
+  }
+  pair_ring_close(tmem, warp);
+}
+
+// ---------------------------------------------------------------------------
+// Statistics of the tiles -> losses of the rows (and, from a single CTA, their means).
+// ---------------------------------------------------------------------------
+struct HeadRowsOut {
+  const int64_t* targets;
+  const float* neg_entropy;
+  const float* part;
+  const float* z_target;
+  float *lse, *ce, *lse_t, *kd;
+  float* means;              // mean and number of the rows with a target, then of those with a teacher; null: not wanted
+  int N, V, parts;
+  float inv_tau, tau;
+};
+
+__device__ __forceinline__ void join(float& ref, float& sum, float r, float s) {
+  const float to = fmaxf(ref, r);
+  sum = to == -INFINITY ? sum + s : (ref == -INFINITY ? sum : sum * ex2(ref - to)) + (r == -INFINITY ? s : s * ex2(r - to));
+  ref = to;
+}
+
+constexpr int JOIN_GROUPS = 32;      // warps of a CTA: each takes every 32nd part of the CTA's 32 rows
+
+template <bool CE, bool KD>
+__global__ void __launch_bounds__(32 * JOIN_GROUPS) head_join_kernel(const __grid_constant__ HeadRowsOut p) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int F = head_values(CE, KD);
+  __shared__ float s_v[JOIN_GROUPS][F][33];
+  const int g = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * 32 + lane;
+  float r1 = -INFINITY, s1 = 0.f, r2 = -INFINITY, s2 = 0.f, dot = 0.f;
+  if (row < p.N) {
+#pragma unroll 4
+    for (int i = g; i < p.parts; i += JOIN_GROUPS) {
+      const float* v = p.part + size_t(i) * F * p.N + row;
+      if (CE) { join(r1, s1, v[0], v[p.N]); v += 2 * size_t(p.N); }
+      if (KD) { join(r2, s2, v[0], v[p.N]); dot += v[2 * size_t(p.N)]; }
+    }
+  }
+  if (CE) { s_v[g][0][lane] = r1; s_v[g][1][lane] = s1; }
+  if (KD) { s_v[g][F - 3][lane] = r2; s_v[g][F - 2][lane] = s2; s_v[g][F - 1][lane] = dot; }
+  __syncthreads();
+  if (g != 0 || row >= p.N) return;
+  for (int i = 1; i < JOIN_GROUPS; ++i) {
+    if (CE) join(r1, s1, s_v[i][0][lane], s_v[i][1][lane]);
+    if (KD) { join(r2, s2, s_v[i][F - 3][lane], s_v[i][F - 2][lane]); dot += s_v[i][F - 1][lane]; }
+  }
+  const float nan = __int_as_float(0x7fc00000);
+  if (CE) {
+    const double l = (double(r1) + log2(double(s1))) / double(LOG2E);
+    const long long y = p.targets[row];
+    p.lse[row] = r1;
+    p.lse[size_t(p.N) + row] = s1;
+    p.ce[row] = y == -100 ? 0.f : y >= 0 && y < p.V ? float(l - double(p.z_target[row])) : nan;
+  }
+  if (KD) {
+    const double l = (double(r2) + log2(double(s2))) / double(LOG2E * p.inv_tau);      // tau times the logarithm of sum exp(z / tau)
+    const float e = p.neg_entropy[row];
+    p.lse_t[row] = r2;
+    p.lse_t[size_t(p.N) + row] = s2;
+    p.kd[row] = e == INFINITY ? 0.f : float(double(p.tau) * (double(p.tau) * double(e) + (l - double(dot))));
+  }
+}
+
+// Means over the rows that count, in a fixed order: thread, warp, warps.
+template <bool CE, bool KD>
+__global__ void __launch_bounds__(1024) head_mean_kernel(const __grid_constant__ HeadRowsOut p) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ double s_sum[2][32];
+  __shared__ int s_cnt[2][32];
+  double sum[2] = {0.0, 0.0};
+  int cnt[2] = {0, 0};
+  for (int r = threadIdx.x; r < p.N; r += 1024) {
+    if (CE) { sum[0] += double(p.ce[r]); cnt[0] += p.targets[r] != -100; }
+    if (KD) { sum[1] += double(p.kd[r]); cnt[1] += p.neg_entropy[r] != INFINITY; }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+      cnt[i] += __shfl_xor_sync(0xffffffffu, cnt[i], o);
+    }
+    if ((threadIdx.x & 31) == 0) { s_sum[i][threadIdx.x >> 5] = sum[i]; s_cnt[i][threadIdx.x >> 5] = cnt[i]; }
+  }
+  __syncthreads();
+  if (threadIdx.x < 2 && (threadIdx.x == 0 ? CE : KD)) {
+    const int i = threadIdx.x;
+    double a = 0.0;
+    int n = 0;
+    for (int w = 0; w < 32; ++w) { a += s_sum[i][w]; n += s_cnt[i][w]; }
+    p.means[2 * i] = float(a / double(n));             // no row that counts: 0 / 0 = NaN, as the mean of the logits' loss has it
+    p.means[2 * i + 1] = float(n);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Backward: the rows' factors, and the rows that have a gradient at all.
+// ---------------------------------------------------------------------------
+struct HeadRowsIn {
+  const __nv_bfloat16* x;
+  const int64_t* targets;
+  const float* neg_entropy;
+  const float *lse_in, *lse_t_in;
+  const float *g_ce, *g_kd;               // gradients of the rows' losses (stride 0: the same for all)
+  int g_ce_stride, g_kd_stride;
+  const float *n_ce, *n_kd;               // divisors (the means' row counts) or null
+  __nv_bfloat16* xs;
+  float *r_ce, *r_kd;                     // [3][N], as HeadLogits has them
+  float* scale;                           // [1]
+  int N, V, C;
+  float tau;
+};
+
+// The gradients of the logits are kept relative to one factor of the whole call, which the products apply to their f32 sums: rows of a
+// mean then have the factor 1, and a target of small probability -1, which bf16 holds.  (With 1 / rows in them that entry, half of a
+// row's gradient, had the same rounding in every row: an error of up to 2^-8 of dx and dW, and no noise that averages out.)
+__device__ __forceinline__ float common_factor(float ce, float kd) {
+  const bool by_ce = ce > 0.f && ce <= FLT_MAX && !(kd > ce * 1e18f);
+  const float s = by_ce ? ce : kd;
+  return s > 0.f && s <= FLT_MAX ? s : 1.f;
+}
+__device__ __forceinline__ float row_factor(const float* g, int stride, const float* n, int row) {
+  const float c = g[size_t(row) * stride];
+  return n ? c / *n : c;
+}
+
+// Losses of the rows: the largest finite factor of each kind.
+__global__ void __launch_bounds__(1024) head_scale_kernel(const __grid_constant__ HeadRowsIn p) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float s_top[2][32];
+  float ce = 0.f, kd = 0.f;
+  for (int r = threadIdx.x; r < p.N; r += 1024) {
+    if (p.targets && p.targets[r] != -100) {
+      const float c = fabsf(row_factor(p.g_ce, p.g_ce_stride, p.n_ce, r));
+      if (c <= FLT_MAX) ce = fmaxf(ce, c);
+    }
+    if (p.neg_entropy && p.neg_entropy[r] != INFINITY) {
+      const float c = fabsf(row_factor(p.g_kd, p.g_kd_stride, p.n_kd, r)) * p.tau;
+      if (c <= FLT_MAX) kd = fmaxf(kd, c);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ce = fmaxf(ce, __shfl_xor_sync(0xffffffffu, ce, o));
+    kd = fmaxf(kd, __shfl_xor_sync(0xffffffffu, kd, o));
+  }
+  if ((threadIdx.x & 31) == 0) { s_top[0][threadIdx.x >> 5] = ce; s_top[1][threadIdx.x >> 5] = kd; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; ++w) { ce = fmaxf(ce, s_top[0][w]); kd = fmaxf(kd, s_top[1][w]); }
+    *p.scale = common_factor(ce, kd);
+  }
+}
+
+// A row without target and teacher takes part in nothing: it becomes a row of zeros with factors of 0, so that a NaN or
+// an infinity in it reaches neither its own gradient nor the weight's.
+__global__ void __launch_bounds__(256) head_rows_kernel(const __grid_constant__ HeadRowsIn p) {
+  pdl_wait();
+  pdl_trigger();
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= p.N) return;
+  const float nan = __int_as_float(0x7fc00000);
+  const bool same = p.g_ce_stride == 0 && p.g_kd_stride == 0;      // else the scale is there already
+  float c1 = p.targets ? row_factor(p.g_ce, p.g_ce_stride, p.n_ce, row) : 0.f;
+  float c2 = p.neg_entropy ? row_factor(p.g_kd, p.g_kd_stride, p.n_kd, row) * p.tau : 0.f;
+  const float scale = same ? common_factor(fabsf(c1), fabsf(c2)) : *p.scale;
+  if (same && row == 0 && lane == 0) *p.scale = scale;
+  bool live = false;
+  if (p.targets) {
+    const long long y = p.targets[row];
+    const bool on = y != -100;
+    live |= on;
+    c1 = !on ? 0.f : y < 0 || y >= p.V ? nan : c1 / scale;
+  }
+  if (p.neg_entropy) {
+    const float e = p.neg_entropy[row];
+    const bool on = e != INFINITY;
+    live |= on;
+    c2 = !on ? 0.f : e != e ? nan : c2 / scale;
+  }
+  if (lane == 0) {
+    const size_t N = size_t(p.N);
+    if (p.targets) { p.r_ce[row] = live ? p.lse_in[row] : 0.f; p.r_ce[N + row] = c1; p.r_ce[2 * N + row] = live ? c1 / p.lse_in[N + row] : 0.f; }
+    if (p.neg_entropy) { p.r_kd[row] = live ? p.lse_t_in[row] : 0.f; p.r_kd[N + row] = c2; p.r_kd[2 * N + row] = live ? c2 / p.lse_t_in[N + row] : 0.f; }
+  }
+  const uint4* src = reinterpret_cast<const uint4*>(p.x + size_t(row) * p.C);
+  uint4* dst = reinterpret_cast<uint4*>(p.xs + size_t(row) * p.C);
+  for (int c = lane; c < p.C / 8; c += 32) dst[c] = live ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+}
+
+// Sum of the slabs in their order -> dx.
+template <bool BF16_OUT>
+__global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ slabs, int n_slabs, size_t n, void* __restrict__ dx) {
+  pdl_wait();
+  pdl_trigger();
+  const size_t i = (size_t(blockIdx.x) * 256 + threadIdx.x) * 8;
+  if (i >= n) return;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+#pragma unroll 4
+  for (int s = 0; s < n_slabs; ++s) {
+    const float4* v = reinterpret_cast<const float4*>(slabs + size_t(s) * n + i);
+    const float4 x = __ldcs(v), y = __ldcs(v + 1);
+    a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+    b.x += y.x; b.y += y.y; b.z += y.z; b.w += y.w;
+  }
+  if constexpr (BF16_OUT) {
+    reinterpret_cast<uint4*>(dx)[i / 8] = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
+  } else {
+    reinterpret_cast<float4*>(dx)[i / 4] = a;
+    reinterpret_cast<float4*>(dx)[i / 4 + 1] = b;
+  }
+}
+
+template <bool CE, bool KD, bool GRAD>
+int launch_logits(const CUtensorMap& tx, const CUtensorMap& tw, const HeadLogits& p, int sms, cudaStream_t stream) {
+  const long long tiles = (long long)((p.N + HEAD_TILE - 1) / HEAD_TILE) * ((p.cols + HEAD_TILE - 1) / HEAD_TILE);
+  const int pairs = sms / 2;
+  auto kernel = head_logits_kernel<CE, KD, GRAD>;
+  JB_MAX_SMEM(kernel, HEAD_SMEM);
+  launch_dep_cluster(kernel, dim3(2 * unsigned(tiles < pairs ? tiles : pairs)), dim3(HEAD_THREADS), HEAD_SMEM, 2, stream, tx, tw, p);
+  JB_LAUNCH_CHECK("head_logits_kernel");
+  return JB200_OK;
+}
+template <bool GRAD>
+int launch_logits(bool ce, bool kd, const CUtensorMap& tx, const CUtensorMap& tw, const HeadLogits& p, int sms, cudaStream_t stream) {
+  if (ce && kd) return launch_logits<true, true, GRAD>(tx, tw, p, sms, stream);
+  return ce ? launch_logits<true, false, GRAD>(tx, tw, p, sms, stream) : launch_logits<false, true, GRAD>(tx, tw, p, sms, stream);
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Everything about the arguments that both directions share.
+int check_head(const jb200_head* h, const char* what) {
+  JB_REQUIRE(h, "%s: null pointer", what);
+  JB_REQUIRE(h->N >= 0 && h->V >= 1 && h->C >= 64 && h->C % 8 == 0,
+             "%s: bad shape (%d rows, vocabulary %d, %d channels; channels must be a multiple of 8 and at least 64)", what, h->N, h->V, h->C);
+  const long long tiles = (long long)((h->N + HEAD_TILE - 1) / HEAD_TILE) * ((h->V + HEAD_TILE - 1) / HEAD_TILE);
+  JB_REQUIRE(tiles < INT_MAX / 4 && h->V <= INT_MAX - HEAD_TILE && h->N <= INT_MAX - HEAD_TILE, "%s: too many logits (%d x %d)", what, h->N, h->V);
+  JB_REQUIRE(h->N == 0 || (h->x && h->w), "%s: null pointer", what);
+  JB_REQUIRE(aligned16(h->x) && aligned16(h->w), "%s: rows and weight must be 16-byte aligned", what);
+  JB_REQUIRE(h->N == 0 || h->targets || h->ids, "%s: neither targets nor a teacher", what);
+  JB_REQUIRE(h->N == 0 || !h->targets || h->lse, "%s: lse is needed with targets", what);
+  if (h->ids) {
+    JB_REQUIRE(h->K >= 1 && h->K <= TEACHER_MAX, "%s: a teacher has 1 to %d entries a row, got %d", what, TEACHER_MAX, h->K);
+    JB_REQUIRE(h->q && h->neg_entropy && h->lse_t, "%s: null pointer (teacher)", what);
+    JB_REQUIRE(h->temperature > 0.f && h->temperature <= FLT_MAX && 1.0f / h->temperature <= FLT_MAX, "%s: temperature must be positive and finite", what);
+  }
+  return JB200_OK;
+}
+
+}  // namespace
+
+int encode_head_map(CUtensorMap* tm, const void* ptr, long long cols, long long rows, int box_rows, const char* what) {
+  const cuuint64_t dim[2] = {cuuint64_t(cols), cuuint64_t(rows)};
+  const cuuint64_t stride[1] = {cuuint64_t(cols) * 2};
+  const cuuint32_t box[2] = {HEAD_BK, cuuint32_t(box_rows)};
+  return encode_tiled(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dim, stride, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, what);
+}
+
+HeadPlan head_plan(int N, int V, int C, int pairs) {
+  HeadPlan pl;
+  const long long tv = (V + HEAD_TILE - 1) / HEAD_TILE, tm = (N + HEAD_TILE - 1) / HEAD_TILE, tc = (C + HEAD_TILE - 1) / HEAD_TILE;
+  long long most = (long long)(PIECE_BYTES / (size_t(N > 0 ? N : 1) * HEAD_TILE * 2));
+  if (most < 1) most = 1;
+  pl.pieces = int((tv + most - 1) / most);
+  const long long per = (tv + pl.pieces - 1) / pl.pieces;      // tiles of a piece
+  pl.pieces = int((tv + per - 1) / per);
+  pl.cols = int(per) * HEAD_TILE;
+  // dx: tm * tc items of per * 4 K-blocks, beside per * tc items of dW.  Few of them would outlast the others: cut.
+  const long long kb = per * (HEAD_TILE / HEAD_BK), work = tm * tc * kb + per * tc * ((N + HEAD_BK - 1) / HEAD_BK);
+  const long long share = (work + pairs - 1) / pairs;          // K-blocks of a pair, were all alike
+  long long s = (kb + share - 1) / (share > 0 ? share : 1);
+  if (s > kb / 8) s = kb / 8;                                  // at least eight K-blocks each
+  if (s > 64) s = 64;
+  pl.slabs = int(s < 1 ? 1 : s);
+  return pl;
+}
+
+int launch_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, int* ids_out,
+                        float* q_out, float* neg_entropy, cudaStream_t stream) {
+  JB_REQUIRE(N >= 0 && V >= 1, "teacher_rows: bad shape");
+  JB_REQUIRE(K >= 1 && K <= TEACHER_MAX, "teacher_rows: a teacher has 1 to %d entries a row, got %d", TEACHER_MAX, K);
+  JB_REQUIRE(logits_dtype == 0 || logits_dtype == 1, "teacher_rows: dtype must be 0 (f32) or 1 (bf16)");
+  JB_REQUIRE(temperature > 0.f && temperature <= FLT_MAX && 1.0f / temperature <= FLT_MAX, "teacher_rows: temperature must be positive and finite");
+  if (N == 0) return JB200_OK;
+  JB_REQUIRE(ids && logits && ids_out && q_out && neg_entropy, "teacher_rows: null pointer");
+  const size_t smem = size_t(K) * (2 * 33 + TEACHER_WARPS) * 4;
+  const dim3 grid((N + TEACHER_ROWS - 1) / TEACHER_ROWS), block(32 * TEACHER_WARPS);
+  const size_t most = size_t(TEACHER_MAX) * (2 * 33 + TEACHER_WARPS) * 4;
+  if (logits_dtype == 0) {
+    JB_MAX_SMEM(teacher_rows_kernel<float>, most);
+    launch_dep(teacher_rows_kernel<float>, grid, block, smem, stream, ids, static_cast<const float*>(logits), N, K, V, 1.0f / temperature,
+               ids_out, q_out, neg_entropy);
+  } else {
+    JB_MAX_SMEM(teacher_rows_kernel<__nv_bfloat16>, most);
+    launch_dep(teacher_rows_kernel<__nv_bfloat16>, grid, block, smem, stream, ids, static_cast<const __nv_bfloat16*>(logits), N, K, V,
+               1.0f / temperature, ids_out, q_out, neg_entropy);
+  }
+  JB_LAUNCH_CHECK("teacher_rows_kernel");
+  return JB200_OK;
+}
+
+size_t head_loss_scratch_bytes(int N, int V, int ce, int kd) {
+  const size_t parts = 2 * ((size_t(V) + HEAD_TILE - 1) / HEAD_TILE);
+  return (parts * head_values(ce != 0, kd != 0) + 1) * size_t(N) * 4;
+}
+
+int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* means, void* scratch, cudaStream_t stream) {
+  int rc = check_head(h, "head_loss");
+  if (rc != JB200_OK) return rc;
+  JB_REQUIRE(h->N == 0 || scratch, "head_loss: null pointer (scratch)");
+  JB_REQUIRE(h->N == 0 || ((!h->targets || ce) && (!h->ids || kd)), "head_loss: null pointer (losses)");
+  const bool has_ce = h->targets != nullptr, has_kd = h->ids != nullptr;
+  if (h->N == 0 && !means) return JB200_OK;
+  HeadRowsOut o{};
+  o.targets = h->targets; o.neg_entropy = h->neg_entropy;
+  o.lse = h->lse; o.ce = ce; o.lse_t = h->lse_t; o.kd = kd; o.means = means;
+  o.N = h->N; o.V = h->V;
+  o.tau = has_kd ? h->temperature : 1.f;
+  o.inv_tau = 1.0f / o.tau;
+  o.parts = 2 * ((h->V + HEAD_TILE - 1) / HEAD_TILE);
+  if (h->N > 0) {
+    const int sms = sm_count();
+    if (sms < 2) return JB200_ERR_CUDA;
+    HeadLogits p{};
+    p.N = h->N; p.V = h->V; p.C = h->C; p.v0 = 0; p.cols = h->V;
+    p.targets = h->targets; p.ids = h->ids; p.q = h->q; p.K = h->K; p.inv_tau = o.inv_tau;
+    p.part = static_cast<float*>(scratch);
+    p.z_target = p.part + size_t(o.parts) * head_values(has_ce, has_kd) * h->N;
+    p.status = device_status_ptr();
+    if (!p.status) return JB200_ERR_CUDA;
+    o.part = p.part; o.z_target = p.z_target;
+    CUtensorMap tx, tw;
+    if ((rc = encode_head_map(&tx, h->x, h->C, h->N, HEAD_TILE / 2, "head_loss (rows)")) != JB200_OK) return rc;
+    if ((rc = encode_head_map(&tw, h->w, h->C, h->V, HEAD_TILE / 2, "head_loss (weight)")) != JB200_OK) return rc;
+    if ((rc = launch_logits<false>(has_ce, has_kd, tx, tw, p, sms, stream)) != JB200_OK) return rc;
+    auto join = has_ce && has_kd ? head_join_kernel<true, true> : has_ce ? head_join_kernel<true, false> : head_join_kernel<false, true>;
+    launch_dep(join, (h->N + 31) / 32, 32 * JOIN_GROUPS, 0, stream, o);
+    JB_LAUNCH_CHECK("head_join_kernel");
+  }
+  if (means) {
+    // (without rows both means are written: nothing says which was asked for)
+    auto mean = (has_ce && has_kd) || h->N == 0 ? head_mean_kernel<true, true> : has_ce ? head_mean_kernel<true, false> : head_mean_kernel<false, true>;
+    launch_dep(mean, 1, 1024, 0, stream, o);
+    JB_LAUNCH_CHECK("head_mean_kernel");
+  }
+  return JB200_OK;
+}
+
+namespace {
+struct BackwardScratch {
+  size_t xs, rows, g, slabs, total;
+};
+BackwardScratch backward_scratch(int N, int C, const HeadPlan& pl) {
+  BackwardScratch s;
+  s.xs = 0;
+  s.rows = up256(size_t(N) * C * 2);
+  s.g = s.rows + up256((size_t(N) * 6 + 1) * 4);
+  s.slabs = s.g + up256(size_t(N) * pl.cols * 2);
+  s.total = s.slabs + up256(size_t(pl.slabs) * N * C * 4);
+  return s;
+}
+}  // namespace
+
+size_t head_loss_backward_scratch_bytes(int N, int V, int C) {
+  const int sms = sm_count();
+  if (N < 1 || V < 1 || C < 1 || sms < 2) return 0;
+  return backward_scratch(N, C, head_plan(N, V, C, sms / 2)).total;
+}
+
+int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_stride, const float* n_ce, const float* g_kd, int g_kd_stride,
+                              const float* n_kd, void* dx, int dx_dtype, void* dw, int dw_dtype, void* scratch, cudaStream_t stream) {
+  int rc = check_head(h, "head_loss_backward");
+  if (rc != JB200_OK) return rc;
+  JB_REQUIRE((dx_dtype == 0 || dx_dtype == 1) && (dw_dtype == 0 || dw_dtype == 1), "head_loss_backward: dtype must be 0 (f32) or 1 (bf16)");
+  JB_REQUIRE((reinterpret_cast<uintptr_t>(dw) & 31u) == 0, "head_loss_backward: dw must be 32-byte aligned");
+  if (!dx && !dw) return JB200_OK;
+  if (h->N == 0) {
+    if (dw) JB_CUDA(cudaMemsetAsync(dw, 0, size_t(h->V) * h->C * (dw_dtype ? 2 : 4), stream));
+    return JB200_OK;
+  }
+  JB_REQUIRE(aligned16(dx) && scratch && (reinterpret_cast<uintptr_t>(scratch) & 255u) == 0,
+             "head_loss_backward: dx must be 16-byte, scratch 256-byte aligned");
+  JB_REQUIRE((!h->targets || g_ce) && (!h->ids || g_kd), "head_loss_backward: null pointer (gradients of the losses)");
+  JB_REQUIRE((g_ce_stride == 0 || g_ce_stride == 1) && (g_kd_stride == 0 || g_kd_stride == 1), "head_loss_backward: strides must be 0 or 1");
+  const int sms = sm_count();
+  if (sms < 2) return JB200_ERR_CUDA;
+  const HeadPlan pl = head_plan(h->N, h->V, h->C, sms / 2);
+  const BackwardScratch at = backward_scratch(h->N, h->C, pl);
+  uint8_t* base = static_cast<uint8_t*>(scratch);
+  float* rows = reinterpret_cast<float*>(base + at.rows);
+  const size_t N = size_t(h->N);
+
+  HeadRowsIn r{};
+  r.x = static_cast<const __nv_bfloat16*>(h->x);
+  r.targets = h->targets; r.neg_entropy = h->ids ? h->neg_entropy : nullptr;
+  r.lse_in = h->lse; r.lse_t_in = h->lse_t;
+  r.g_ce = g_ce; r.g_kd = g_kd; r.g_ce_stride = g_ce_stride; r.g_kd_stride = g_kd_stride; r.n_ce = n_ce; r.n_kd = n_kd;
+  r.xs = reinterpret_cast<__nv_bfloat16*>(base + at.xs);
+  r.r_ce = rows; r.r_kd = rows + 3 * N;
+  r.N = h->N; r.V = h->V; r.C = h->C;
+  r.tau = h->ids ? h->temperature : 1.f;
+  r.scale = rows + 6 * N;
+  if (g_ce_stride != 0 || g_kd_stride != 0) {
+    launch_dep(head_scale_kernel, 1, 1024, 0, stream, r);
+    JB_LAUNCH_CHECK("head_scale_kernel");
+  }
+  launch_dep(head_rows_kernel, (h->N + 7) / 8, 256, 0, stream, r);
+  JB_LAUNCH_CHECK("head_rows_kernel");
+
+  HeadLogits p{};
+  p.N = h->N; p.V = h->V; p.C = h->C;
+  p.targets = h->targets; p.ids = h->ids; p.q = h->q; p.K = h->K; p.inv_tau = 1.0f / r.tau;
+  p.r_ce = r.r_ce; p.r_kd = r.r_kd;
+  p.g = reinterpret_cast<__nv_bfloat16*>(base + at.g);
+  p.ldg = pl.cols;
+  p.status = device_status_ptr();
+  if (!p.status) return JB200_ERR_CUDA;
+  CUtensorMap tx, tw;
+  if ((rc = encode_head_map(&tx, r.xs, h->C, h->N, HEAD_TILE / 2, "head_loss_backward (rows)")) != JB200_OK) return rc;
+  if ((rc = encode_head_map(&tw, h->w, h->C, h->V, HEAD_TILE / 2, "head_loss_backward (weight)")) != JB200_OK) return rc;
+  // one slab in f32 is the result itself
+  const bool direct = dx_dtype == 0 && pl.slabs == 1 && (reinterpret_cast<uintptr_t>(dx) & 31u) == 0;
+  float* slabs = !dx ? nullptr : direct ? static_cast<float*>(dx) : reinterpret_cast<float*>(base + at.slabs);
+  for (int i = 0; i < pl.pieces; ++i) {
+    p.v0 = i * pl.cols;
+    p.cols = h->V - p.v0 < pl.cols ? h->V - p.v0 : pl.cols;
+    if ((rc = launch_logits<true>(h->targets != nullptr, h->ids != nullptr, tx, tw, p, sms, stream)) != JB200_OK) return rc;
+    rc = launch_head_products(p.g, pl.cols, p.cols, r.xs, h->w, h->N, h->V, h->C, p.v0, pl.slabs, i == 0, r.scale, slabs, dw, dw_dtype, sms, stream);
+    if (rc != JB200_OK) return rc;
+  }
+  if (dx && !direct) {
+    const size_t n = N * h->C;
+    launch_dep(dx_dtype == 1 ? head_dx_kernel<true> : head_dx_kernel<false>, unsigned((n / 8 + 255) / 256), 256, 0, stream, slabs, pl.slabs, n, dx);
+    JB_LAUNCH_CHECK("head_dx_kernel");
+  }
+  return JB200_OK;
+}
+
+int head_plan_host(int N, int V, int C, int sms, int32_t* out3) {
+  if (N < 1 || V < 1 || C < 1 || sms < 2 || !out3) return JB200_ERR_ARG;
+  const HeadPlan pl = head_plan(N, V, C, sms / 2);
+  out3[0] = pl.cols; out3[1] = pl.pieces; out3[2] = pl.slabs;
+  return JB200_OK;
+}
+
+}  // namespace jb

@@ -160,6 +160,18 @@ int launch_step_cluster(const jb200_layer* layers, int n_layers, const jb200_for
                         cudaStream_t stream, bool* taken);
 int launch_cross_entropy(const void* logits, int ld, int n_rows, int V, const int64_t* targets, float* row_loss,
                          const float* aux_a, int stride_a, const float* aux_b, int n_aux, float* loss, cudaStream_t stream);
+// The head's losses (head_loss.cu) and the norm's gradient (norm_grad.cu).
+int launch_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, int* ids_out,
+                        float* q_out, float* neg_entropy, cudaStream_t stream);
+size_t head_loss_scratch_bytes(int N, int V, int ce, int kd);
+int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* means, void* scratch, cudaStream_t stream);
+size_t head_loss_backward_scratch_bytes(int N, int V, int C);
+int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_stride, const float* n_ce, const float* g_kd, int g_kd_stride,
+                              const float* n_kd, void* dx, int dx_dtype, void* dw, int dw_dtype, void* scratch, cudaStream_t stream);
+int head_plan_host(int N, int V, int C, int sms, int32_t* out3);
+size_t rmsnorm_backward_scratch_bytes(int n_rows, int C);
+int launch_rmsnorm_backward(const void* x, int x_dtype, const float* w, float eps, const void* dy, int dy_dtype, int n_rows, int C, void* dx,
+                            float* dw, void* scratch, cudaStream_t stream);
 int mid_ring_host(int bn, int K, int coarse, int32_t* out);
 int dispatch_plan_host(int tokens, int C, int hidden, int sms, int32_t* out);
 int expert_tiles_host(int tokens, int second, int C, int E, int hidden, int sms, int32_t* out);

@@ -18,6 +18,7 @@
 #include "common.cuh"
 #include "gemm_shared.cuh"
 #include "launchers.h"
+#include "pair_mma.cuh"
 
 namespace jb {
 
@@ -46,74 +47,6 @@ constexpr size_t smem_bytes(bool resid) {
 }
 static_assert(smem_bytes(false) <= 227 * 1024 && smem_bytes(true) <= 227 * 1024, "shared memory of one CTA");
 
-// ---- cta_group::2 forms of the wrappers in common.cuh ----
-__device__ __forceinline__ void pair_tmem_alloc(uint32_t dst_smem, uint32_t ncols) {
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void pair_tmem_relinquish() {
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void pair_umma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
-      "}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// Arrive on the barrier at this offset in both CTAs once all previously issued MMAs of this thread retire.
-__device__ __forceinline__ void pair_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-               ::"r"(bar), "h"(uint16_t(3)) : "memory");
-}
-// Tile load into this CTA whose bytes are counted by a barrier of the pair's leader.
-__device__ __forceinline__ void pair_tma_load_2d(uint32_t dst_smem, const void* tmap, int c0, int c1, uint32_t leader_bar) {
-  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-               ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(leader_bar) : "memory");
-}
-// (with .release.cluster every arrival waits for the warp's outstanding memory operations: 1400 cycles per K-block)
-__device__ __forceinline__ void cluster_mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// Bounded wait that also orders what the other CTA did before its arrival.
-__device__ __forceinline__ bool cluster_mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "}"
-      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-  return done != 0;
-}
-__device__ __forceinline__ bool cluster_mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, unsigned int* status,
-                                                  unsigned int code) {
-  if (cluster_mbar_try(bar, parity)) return true;
-  const unsigned long long t0 = globaltimer_ns();
-  for (;;) {
-#pragma unroll 1
-    for (int i = 0; i < 32; ++i)
-      if (cluster_mbar_try(bar, parity)) return true;
-    if (*abort_flag) return false;
-    if (globaltimer_ns() - t0 > JB_WAIT_LIMIT_NS) {
-      *abort_flag = 1u;
-      atomicCAS(status, 0u, code);
-      return false;
-    }
-  }
-}
-
-__device__ __forceinline__ void st_global_256(void* p, const uint32_t* w) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-               ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-               : "memory");
-}
 // 32 consecutive out-features of one token: alpha, epilogue, 32-byte accesses.  `o`: element offset of the first.
 __device__ __forceinline__ void store_row_chunk(const GemmParams& p, uint32_t (&v)[32], float alpha, size_t o) {
   if (p.epilogue == JB200_EPI_BF16 || p.epilogue == JB200_EPI_GELU_BF16) {

@@ -47,6 +47,7 @@ def parse_args(argv=None):
     p.add_argument("--skip-train-eval", action="store_true")
     p.add_argument("--skip-gen", action="store_true")
     p.add_argument("--stateful", action="store_true", help="decode with the carried recurrent state (not the 256-token re-run)")
+    p.add_argument("--no-logits", action="store_true", help="corpus loss straight from the hidden rows: no logits in memory, long windows")
     p.add_argument("--layers", type=int, default=24)
     p.add_argument("--d-model", type=int, default=1024)
     p.add_argument("--heads", type=int, default=16)
@@ -146,15 +147,16 @@ def window_starts(n_tokens: int, num_windows: int, seq_len: int, seed: int):
 
 
 @torch.no_grad()
-def evaluate_corpus(model, tokens: torch.Tensor, num_windows=200, seq_len=256, seed=42, label="HOLDOUT"):
-    """Mean / stdev of the per-window loss `model(x, targets=y)` and exp(mean) (evaluate_jarvis.py:323-377)."""
+def evaluate_corpus(model, tokens: torch.Tensor, num_windows=200, seq_len=256, seed=42, label="HOLDOUT", no_logits=False):
+    """Mean / stdev of the per-window loss `model(x, targets=y)` and exp(mean) (evaluate_jarvis.py:323-377).  no_logits: the
+    loss by `model.loss`, which stores none (long windows)."""
     dev = model.tok_emb.weight.device
     tokens = tokens.to(dev)
     losses, bad = [], False
     for s in window_starts(int(tokens.numel()), num_windows, seq_len, seed):
         x = tokens[s:s + seq_len].unsqueeze(0)
         y = tokens[s + 1:s + seq_len + 1].unsqueeze(0)
-        _, loss = model(x, targets=y, persist_state=False)
+        loss = model.loss(x, y) if no_logits else model(x, targets=y, persist_state=False)[1]
         v = float(loss)
         bad = bad or math.isnan(v) or math.isinf(v)
         losses.append(v)
@@ -258,10 +260,11 @@ def main(argv=None):
     if args.prompt:
         generate_streaming(model, enc, args.prompt, args)
         return
-    reports = [evaluate_corpus(model, load_token_file(args.eval_file, enc), args.num_windows, args.seq_len, args.seed, "HOLDOUT")]
+    reports = [evaluate_corpus(model, load_token_file(args.eval_file, enc), args.num_windows, args.seq_len, args.seed, "HOLDOUT",
+                               args.no_logits)]
     if not args.skip_train_eval:
         reports.append(evaluate_corpus(model, load_token_file(args.train_file, enc), args.num_windows, args.seq_len,
-                                       args.seed, "TRAIN"))
+                                       args.seed, "TRAIN", args.no_logits))
     for r in reports:
         print(f"{r['label']:8s} windows {r['windows_evaluated']}  loss {r['mean_loss']:.4f} +- {r['std_loss']:.4f}  "
               f"ppl {r['perplexity']:.2f}{'  NaN/Inf seen' if r['has_nan_inf'] else ''}")

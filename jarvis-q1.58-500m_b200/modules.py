@@ -3,7 +3,8 @@
 Constructors, parameter / buffer names (so state dicts interchange: 23 tensors per block, 555 for
 the 24-layer model), forward signatures and return tuples follow jarvis_engine/jarvis_model.py and
 the CUDA drop-ins in associative_attention_cuda/associative_attention.py and
-sparse_model_cuda/sparse_model.py.  Inference only (no autograd through the kernels), CUDA only:
+sparse_model_cuda/sparse_model.py.  Inference only (no autograd through the blocks; `Jarvis.head_loss` has gradients of final norm
+and lm_head), CUDA only:
 a CPU tensor or a missing library raises, nothing falls back.
 
 Numerics: the residual stream is carried in fp32, GEMM inputs and scan inputs are bf16, every
@@ -15,7 +16,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import chain, ops
+from . import chain, losses, ops
 
 # ----------------------------------------------------------------------------------------------
 # small pieces
@@ -635,6 +636,13 @@ class Jarvis(nn.Module):
 
     def hidden_rows(self, idx, persist_state=False):
         """Embedding + all blocks + final norm -> bf16 (B*T, C) hidden rows."""
+        return self._rows(idx, persist_state, True)
+
+    def _residual_rows(self, idx):
+        """Embedding + all blocks -> the f32 (B*T, C) residual stream that final_norm takes; no state is carried."""
+        return self._rows(idx, False, False)
+
+    def _rows(self, idx, persist_state, normed):
         if self.training:
             raise RuntimeError("Jarvis (sm_100a): inference only; call .eval() first")
         B, T = idx.shape
@@ -649,11 +657,16 @@ class Jarvis(nn.Module):
                 h_in = [h if h is not None and h.shape[0] == B else None for h in self._h_states]
                 if self.carry_attention_state:
                     s_in = [s if s is not None and s.shape[0] == B else None for s in self._attn_states]
-            r = self._chain_rows(tab, idx, start_pos, h_in, s_in, self.carry_attention_state)
+            if normed:
+                r = self._chain_rows(tab, idx, start_pos, h_in, s_in, self.carry_attention_state)
+                out = r.hidden
+            else:
+                out = torch.empty((B * T, self.d_model), dtype=torch.float32, device=idx.device)
+                r = chain.run(tab, out, B, T, ids=idx, table=_f32(self.tok_emb.weight), start_pos=start_pos)
             self._h_states = r.h
             self._attn_states = r.S if r.S is not None else [None] * tab.n
             self._aux, self._reflect = r.scalars, r.reflect
-            return r.hidden
+            return out
         self._reflect = None
         x = ops.embedding(idx, _f32(self.tok_emb.weight)).view(B * T, self.d_model)
         h_prevs = self._h_states if persist_state else [None] * len(self.blocks)
@@ -679,6 +692,8 @@ class Jarvis(nn.Module):
         self._h_states = new_h
         self._attn_states = new_s
         self._aux = aux
+        if not normed:
+            return x
         return ops.rmsnorm(x, _f32(self.final_norm.weight), self.final_norm.eps)
 
     @torch.no_grad()
@@ -724,10 +739,24 @@ class Jarvis(nn.Module):
             hidden = ops.rmsnorm(x, _f32(self.final_norm.weight), self.final_norm.eps)
         return self._logits(hidden, B, T), {"h": new_h, "S": new_s}
 
+    def _lm_head_rows(self):
+        """lm_head's weight in bf16 without the padding rows."""
+        return self._lm_head_weight()[:self.lm_head.weight.shape[0]]
+
     def _logits(self, hidden, B, T):
         """Dense bf16 lm_head on the same tcgen05 pipeline as the ternary layers (weight tiles by TMA); the padded
         vocabulary columns are sliced off as a view."""
         return ops.dense_linear(hidden, self._lm_head_weight()).view(B, T, -1)[..., :self.lm_head.weight.shape[0]]
+
+    def _aux_terms(self, device):
+        """What the last forward adds to a loss: f32 (layers, 3) with l_balance first, and the layers' reflective penalties."""
+        aux = self._aux if torch.is_tensor(self._aux) else torch.stack(self._aux)
+        reflect = self._reflect
+        if reflect is None:
+            # whatever a penalty of the caller's own returns: a tensor or a number
+            reflect = torch.stack([torch.as_tensor(b.reflect(sc[1], sc[2]), dtype=torch.float32, device=device).reshape(())
+                                   for b, sc in zip(self.blocks, self._aux)])
+        return aux, reflect
 
     @torch.no_grad()
     def forward(self, idx, targets=None, persist_state=False):
@@ -735,16 +764,42 @@ class Jarvis(nn.Module):
         logits = self._logits(self.hidden_rows(idx, persist_state), B, T)
         loss = None
         if targets is not None:
-            aux = self._aux if torch.is_tensor(self._aux) else torch.stack(self._aux)
-            reflect = self._reflect
-            if reflect is None:
-                # whatever a penalty of the caller's own returns: a tensor or a number
-                reflect = torch.stack([torch.as_tensor(b.reflect(sc[1], sc[2]), dtype=torch.float32, device=logits.device).reshape(())
-                                       for b, sc in zip(self.blocks, self._aux)])
-            loss = ops.cross_entropy(logits, targets, aux, reflect)
+            loss = ops.cross_entropy(logits, targets, *self._aux_terms(logits.device))
         if self.logits_dtype != torch.bfloat16:
             logits = logits.to(self.logits_dtype)
         return logits, loss
+
+    @torch.no_grad()
+    def loss(self, idx, targets, persist_state=False):
+        """The loss of forward(idx, targets) without its logits, which are never stored (2 bytes a token and vocabulary entry
+        there): cross entropy over the targets other than -100 plus the layers' auxiliary terms, f32 scalar.  The logits enter the
+        softmax as f32, forward's as bf16: the two agree as far as that rounding goes."""
+        r = ops.head_loss(self.hidden_rows(idx, persist_state), self._lm_head_rows(),
+                          ops._need(targets.reshape(-1).contiguous(), torch.int64, "loss.targets"))
+        aux, reflect = self._aux_terms(r.ce.device)
+        return r.means[0] + aux[:, 0].sum() + reflect.sum()
+
+    def head_loss(self, idx, targets=None, teacher_ids=None, teacher_logits=None, *, temperature: float = 1.0):
+        """Losses to train the head by: the blocks run as they are (inference, no gradient), then final norm and lm_head with
+        gradients of `final_norm.weight` and `lm_head.weight`, through `losses`.  With targets (B, T): the mean cross entropy; with
+        a teacher's top logits, teacher_ids and teacher_logits (B, T, K): the mean distillation loss; with both: the pair."""
+        if targets is None and teacher_ids is None:
+            raise RuntimeError("head_loss: neither targets nor a teacher")
+        if (teacher_ids is None) != (teacher_logits is None):
+            raise RuntimeError("head_loss: a teacher has ids and logits")
+        with torch.no_grad():
+            x = self._residual_rows(idx)
+        hidden = losses.rms_norm(x, self.final_norm.weight, self.final_norm.eps)
+        w = self.lm_head.weight
+        if targets is not None:
+            targets = targets.reshape(-1)
+        if teacher_ids is None:
+            return losses.linear_cross_entropy(hidden, w, targets)
+        k = teacher_ids.shape[-1]
+        teacher_ids, teacher_logits = teacher_ids.reshape(-1, k), teacher_logits.reshape(-1, k)
+        if targets is None:
+            return losses.linear_distillation(hidden, w, teacher_ids, teacher_logits, temperature=temperature)
+        return losses.linear_losses(hidden, w, targets, teacher_ids, teacher_logits, temperature=temperature)
 
     def set_batch_split(self, group, global_tokens=None):
         """Treat the ranks of `group` as holding slices of ONE batch: every layer all-reduces its MoE

@@ -6,6 +6,8 @@ Output tensors are allocated here with torch (device memory plumbing only).
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -558,6 +560,172 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, aux: torch.Tensor
     _lib.check(lib.jb200_cross_entropy(_ptr(logits), ld, B * T, V, _ptr(y), _ptr(buf), _ptr(aux), aux.stride(0), _ptr(reflect),
                                        reflect.numel(), _ptr(loss), _stream()), "jb200_cross_entropy")
     return loss
+
+
+# --------------------------------------------------------------------------- losses of the head, gradients
+def _together(what: str, first: torch.Tensor, *others):
+    """Every tensor on the first one's device, which is what the launch goes to."""
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"{what}: tensors on {first.device} and {t.device}")
+
+
+def _launch(on: torch.Tensor, fn, *args) -> int:
+    """fn(*args, stream) on the device of `on`, on that device's current stream."""
+    if _raw_device is not None and on.get_device() == _raw_device():
+        return fn(*args, _stream())
+    with torch.cuda.device(on.device):
+        return fn(*args, _stream())
+
+
+class TeacherRows:
+    """A teacher's rows as the head's loss reads them: what teacher_rows leaves."""
+    __slots__ = ("ids", "q", "neg_entropy", "K", "vocab", "temperature")
+
+
+def teacher_rows(ids: torch.Tensor, logits: torch.Tensor, vocab: int, temperature: float = 1.0) -> TeacherRows:
+    """Top logits of a teacher, ids int64 (N, K) with logits f32 or bf16 (N, K), K <= 256, as probabilities at `temperature`
+    over each row's entries.  A negative id is no entry, whatever its logit; a row may have none; an id beyond the vocabulary makes the
+    row's loss NaN; an id that comes twice has both probabilities."""
+    lib = _lib.load()
+    _need(ids, torch.int64, "teacher_rows.ids")
+    _dt(logits)
+    _need(logits, logits.dtype, "teacher_rows.logits")
+    if ids.dim() != 2 or logits.shape != ids.shape:
+        raise RuntimeError(f"teacher_rows: ids {tuple(ids.shape)} and logits {tuple(logits.shape)} must be (N, K) alike")
+    _together("teacher_rows", ids, logits)
+    N, K = ids.shape
+    t = TeacherRows()
+    buf = torch.empty(2 * K * N + N, dtype=torch.float32, device=ids.device)
+    t.q, t.neg_entropy = buf[:K * N], buf[2 * K * N:]
+    t.ids = buf[K * N:2 * K * N].view(torch.int32)
+    t.K, t.vocab, t.temperature = K, int(vocab), float(temperature)
+    _lib.check(_launch(ids, lib.jb200_teacher_rows, _ptr(ids), _ptr(logits), _dt(logits), N, K, t.vocab, t.temperature, _ptr(t.ids),
+                       _ptr(t.q), _ptr(t.neg_entropy)), "jb200_teacher_rows")
+    return t
+
+
+class HeadLoss:
+    """What head_loss leaves: ce / kd f32 (N,) (None where not asked for), means f32 (4,) [mean ce, rows with a target, mean kd, rows with a
+    teacher] or None, and lse / lse_t (2 N,), the softmaxes' sums for the backward call."""
+    __slots__ = ("ce", "kd", "means", "lse", "lse_t")
+
+
+def _head(x, w, targets, teacher, what):
+    _need(x, torch.bfloat16, what + ".x")
+    _need(w, torch.bfloat16, what + ".w")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise RuntimeError(f"{what}: rows {tuple(x.shape)} and weight {tuple(w.shape)} must be (N, C) and (V, C)")
+    if targets is None and teacher is None:
+        raise RuntimeError(f"{what}: neither targets nor a teacher")
+    h = _lib.Head()
+    h.N, h.V, h.C = x.shape[0], w.shape[0], x.shape[1]
+    h.x, h.w = x.data_ptr(), w.data_ptr()
+    h.temperature = 1.0
+    if targets is not None:
+        _need(targets, torch.int64, what + ".targets")
+        if targets.numel() != h.N:
+            raise RuntimeError(f"{what}: one target per row is needed, got {targets.numel()} for {h.N}")
+        h.targets = targets.data_ptr()
+    if teacher is not None:
+        if teacher.neg_entropy.numel() != h.N or teacher.vocab != h.V:
+            raise RuntimeError(f"{what}: the teacher's rows are {teacher.neg_entropy.numel()} over a vocabulary of {teacher.vocab}, "
+                               f"the loss has {h.N} over {h.V}")
+        h.K, h.ids, h.q, h.neg_entropy = teacher.K, teacher.ids.data_ptr(), teacher.q.data_ptr(), teacher.neg_entropy.data_ptr()
+        h.temperature = teacher.temperature
+    _together(what, x, w, targets, None if teacher is None else teacher.q)
+    return h
+
+
+def head_loss(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor | None = None, teacher: TeacherRows | None = None, *,
+              want_means: bool = True) -> HeadLoss:
+    """Losses of lm_head (jarvis_engine/jarvis_model.py:535-540) straight from its rows, the logits x w^T never stored: cross entropy
+    against int64 `targets` (N,) (-100: none, loss 0; otherwise outside the vocabulary: NaN), the divergence t^2 KL(teacher || student)
+    from `teacher`, or both.  x: bf16 (N, C); w: bf16 (V, C), any V (no padding needed), C a multiple of 8 and at least 64."""
+    lib = _lib.load()
+    h = _head(x, w, targets, teacher, "head_loss")
+    N = h.N
+    r = HeadLoss()
+    has_ce, has_kd = targets is not None, teacher is not None
+    buf = torch.empty(6 * N + 4, dtype=torch.float32, device=x.device)
+    at = buf.data_ptr()
+    r.ce, r.lse = (buf[:N], buf[N:3 * N]) if has_ce else (None, None)
+    r.kd, r.lse_t = (buf[3 * N:4 * N], buf[4 * N:6 * N]) if has_kd else (None, None)
+    r.means = buf[6 * N:] if want_means else None
+    if has_ce:
+        h.lse = at + 4 * N
+    if has_kd:
+        h.lse_t = at + 16 * N
+    scratch = torch.empty(lib.jb200_head_loss_scratch_bytes(N, h.V, has_ce, has_kd), dtype=torch.uint8, device=x.device)
+    _lib.check(_launch(x, lib.jb200_head_loss, ctypes.byref(h), at if has_ce else None, at + 12 * N if has_kd else None,
+                       at + 24 * N if want_means else None, _ptr(scratch)), "jb200_head_loss")
+    return r
+
+
+def head_loss_backward(x: torch.Tensor, w: torch.Tensor, fwd: HeadLoss, targets: torch.Tensor | None = None,
+                       teacher: TeacherRows | None = None, *, g_ce: torch.Tensor | None = None, g_kd: torch.Tensor | None = None,
+                       mean: bool = True, dx_dtype=torch.bfloat16, dw_dtype=torch.bfloat16, want_dx: bool = True, want_dw: bool = True):
+    """Gradients (dx (N, C), dw (V, C)) of g_ce . ce + g_kd . kd, the same arguments as in the forward call.  mean: g_ce and g_kd are
+    f32 scalars for the means of `fwd`; else f32 (N,) for the rows' losses.  One that is not wanted is not computed and None."""
+    lib = _lib.load()
+    h = _head(x, w, targets, teacher, "head_loss_backward")
+    n = [None, None]
+    for i, (g, rows, name) in enumerate(((g_ce, fwd.lse, "g_ce"), (g_kd, fwd.lse_t, "g_kd"))):
+        if (targets, teacher)[i] is None:
+            continue
+        if rows is None or rows.numel() != 2 * h.N:
+            raise RuntimeError("head_loss_backward: `fwd` is not the forward call's result for these rows")
+        if g is None:
+            raise RuntimeError(f"head_loss_backward: {name} is needed")
+        _need(g, torch.float32, "head_loss_backward." + name)
+        if g.numel() != (1 if mean else h.N):
+            raise RuntimeError(f"head_loss_backward: {name} must have {'one value' if mean else 'one value per row'}, got {g.numel()}")
+        if mean:
+            if fwd.means is None:
+                raise RuntimeError("head_loss_backward: the forward call left no means")
+            n[i] = fwd.means.data_ptr() + (4 if i == 0 else 12)
+    _together("head_loss_backward", x, g_ce, g_kd, fwd.lse, fwd.lse_t)
+    if targets is not None:
+        h.lse = fwd.lse.data_ptr()
+    if teacher is not None:
+        h.lse_t = fwd.lse_t.data_ptr()
+    codes = {torch.float32: 0, torch.bfloat16: 1}
+    if dx_dtype not in codes or dw_dtype not in codes:
+        raise RuntimeError("head_loss_backward: gradients are float32 or bfloat16")
+    dx = torch.empty(x.shape, dtype=dx_dtype, device=x.device) if want_dx else None
+    dw = torch.empty(w.shape, dtype=dw_dtype, device=x.device) if want_dw else None
+    stride = 0 if mean else 1
+
+    def run(stream):
+        scratch = torch.empty(lib.jb200_head_loss_backward_scratch_bytes(h.N, h.V, h.C), dtype=torch.uint8, device=x.device)
+        return lib.jb200_head_loss_backward(ctypes.byref(h), _ptr(g_ce) if targets is not None else None, stride, n[0],
+                                            _ptr(g_kd) if teacher is not None else None, stride, n[1], _ptr(dx), codes[dx_dtype],
+                                            _ptr(dw), codes[dw_dtype], _ptr(scratch), stream)
+    _lib.check(_launch(x, run), "jb200_head_loss_backward")
+    return dx, dw
+
+
+def rmsnorm_backward(x: torch.Tensor, weight: torch.Tensor, dy: torch.Tensor, eps: float = 1e-6):
+    """Gradients (dx of x's dtype, dweight f32) of rmsnorm for the output's gradient dy (f32 or bf16, x's shape)."""
+    lib = _lib.load()
+    _dt(x), _dt(dy)
+    _need(x, x.dtype, "rmsnorm_backward.x")
+    _need(dy, dy.dtype, "rmsnorm_backward.dy")
+    _need(weight, torch.float32, "rmsnorm_backward.weight")
+    width = x.shape[-1]
+    if dy.shape != x.shape or weight.numel() != width:
+        raise RuntimeError(f"rmsnorm_backward: x {tuple(x.shape)}, dy {tuple(dy.shape)}, weight {tuple(weight.shape)} do not belong together")
+    _together("rmsnorm_backward", x, weight, dy)
+    rows = x.numel() // width if width else 0
+    dx = torch.empty_like(x)
+    dw = torch.empty(width, dtype=torch.float32, device=x.device)
+
+    def run(stream):
+        scratch = torch.empty(lib.jb200_rmsnorm_backward_scratch_bytes(rows, width), dtype=torch.uint8, device=x.device)
+        return lib.jb200_rmsnorm_backward(_ptr(x), _dt(x), _ptr(weight), eps, _ptr(dy), _dt(dy), rows, width, _ptr(dx), _ptr(dw),
+                                          _ptr(scratch), stream)
+    _lib.check(_launch(x, run), "jb200_rmsnorm_backward")
+    return dx, dw
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor | None = None, *, temperature: float = 0.7, top_k: int = 50,

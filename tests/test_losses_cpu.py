@@ -1,0 +1,85 @@
+"""The head's losses and the norm's gradient without a GPU: refusals that need no launch, and how a backward pass is cut."""
+import ctypes as C
+
+import pytest
+import torch
+
+from jarvis_b200 import _lib, losses, ops
+
+
+def _head(**kw):
+    h = _lib.Head()
+    h.N, h.V, h.C, h.temperature = 4, 100, 64, 1.0
+    h.x = h.w = h.targets = h.lse = 4096         # never read: every call here is refused first
+    for k, v in kw.items():
+        setattr(h, k, v)
+    return h
+
+
+@pytest.mark.parametrize("kw,text", [(dict(C=60), "multiple of 8"), (dict(C=56), "at least 64"), (dict(V=0), "bad shape"), (dict(N=-1), "bad shape"),
+                                     (dict(x=None), "null pointer"), (dict(x=4104), "16-byte"), (dict(targets=None), "neither targets nor a teacher"),
+                                     (dict(lse=None), "lse is needed"), (dict(ids=4096, K=0), "1 to 256 entries"),
+                                     (dict(ids=4096, K=257), "1 to 256 entries"), (dict(ids=4096, K=3), "null pointer"),
+                                     (dict(ids=4096, K=3, q=4096, neg_entropy=4096, lse_t=4096, temperature=0.0), "temperature"),
+                                     (dict(ids=4096, K=3, q=4096, neg_entropy=4096, lse_t=4096, temperature=float("nan")), "temperature"),
+                                     (dict(ids=4096, K=3, q=4096, neg_entropy=4096, lse_t=4096, temperature=1e-39), "temperature"),
+                                     (dict(N=2**30, V=2**30), "too many logits")])
+def test_head_calls_refuse_bad_arguments(kw, text):
+    lib = _lib.load()
+    h = _head(**kw)
+    assert lib.jb200_head_loss(C.byref(h), 4096, 4096, None, 4096, None) == _lib.ERR_ARG
+    assert text in _lib.last_error()
+    assert lib.jb200_head_loss_backward(C.byref(h), 4096, 0, None, 4096, 0, None, 4096, 1, 4096, 1, 4096, None) == _lib.ERR_ARG
+    assert text in _lib.last_error()
+
+
+def test_head_calls_refuse_missing_outputs():
+    lib = _lib.load()
+    h = _head()
+    assert lib.jb200_head_loss(C.byref(h), None, None, None, 4096, None) == _lib.ERR_ARG
+    assert lib.jb200_head_loss(C.byref(h), 4096, None, None, None, None) == _lib.ERR_ARG
+    for dx, dxt, dw, scratch, stride, text in ((4096, 2, 4096, 4096, 0, "dtype"), (4096, 1, 4112, 4096, 0, "32-byte"),
+                                               (4100, 1, 4096, 4096, 0, "16-byte"), (4096, 1, 4096, 4100, 0, "256-byte"),
+                                               (4096, 1, 4096, 4096, 2, "strides")):
+        assert lib.jb200_head_loss_backward(C.byref(h), 4096, stride, None, None, 0, None, dx, dxt, dw, 1, scratch, None) == _lib.ERR_ARG
+        assert text in _lib.last_error()
+    assert lib.jb200_head_loss_backward(C.byref(h), None, 0, None, None, 0, None, 4096, 1, 4096, 1, 4096, None) == _lib.ERR_ARG
+    assert lib.jb200_teacher_rows(4096, 4096, 0, 4, 257, 100, 1.0, 4096, 4096, 4096, None) == _lib.ERR_ARG
+    assert lib.jb200_teacher_rows(4096, 4096, 3, 4, 2, 100, 1.0, 4096, 4096, 4096, None) == _lib.ERR_ARG
+    assert lib.jb200_teacher_rows(4096, 4096, 0, 4, 2, 100, -1.0, 4096, 4096, 4096, None) == _lib.ERR_ARG
+    assert lib.jb200_teacher_rows(None, 4096, 0, 4, 2, 100, 1.0, 4096, 4096, 4096, None) == _lib.ERR_ARG
+    for width, text in ((60, "multiple of 8"), (4104, "at most 4096"), (0, "bad shape")):
+        assert lib.jb200_rmsnorm_backward(4096, 0, 4096, 1e-6, 4096, 0, 4, width, 4096, 4096, 4096, None) == _lib.ERR_ARG
+        assert text in _lib.last_error()
+    assert lib.jb200_rmsnorm_backward(4096, 2, 4096, 1e-6, 4096, 0, 4, 64, 4096, 4096, 4096, None) == _lib.ERR_ARG
+    assert lib.jb200_rmsnorm_backward(4100, 0, 4096, 1e-6, 4096, 0, 4, 64, 4096, 4096, 4096, None) == _lib.ERR_ARG
+    assert lib.jb200_rmsnorm_backward(4096, 0, 4096, 1e-6, 4096, 0, 4, 64, 4096, None, 4096, None) == _lib.ERR_ARG
+
+
+def test_cpu_tensors_and_bad_reductions_raise():
+    h, w, t = torch.zeros(4, 64), torch.zeros(100, 64), torch.zeros(4, dtype=torch.int64)
+    ids, lg = torch.zeros(4, 3, dtype=torch.int64), torch.zeros(4, 3)
+    for call in (lambda: losses.linear_cross_entropy(h, w, t), lambda: losses.linear_distillation(h, w, ids, lg),
+                 lambda: losses.linear_losses(h, w, t, ids, lg), lambda: losses.rms_norm(h, torch.ones(64)),
+                 lambda: ops.rmsnorm_backward(h, torch.ones(64), h), lambda: ops.teacher_rows(ids, lg, 100),
+                 lambda: ops.head_loss(h.bfloat16(), w.bfloat16(), t)):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            call()
+    with pytest.raises(RuntimeError, match="reduction"):
+        losses.linear_cross_entropy(h, w, t, reduction="median")
+
+
+@pytest.mark.parametrize("sms", [148, 132, 2])
+def test_backward_passes_are_cut_into_pieces_that_cover_the_vocabulary(sms):
+    lib = _lib.load()
+    out = (C.c_int32 * 3)()
+    for N in (1, 37, 255, 2048, 5000, 16384, 300000, 2000000):
+        for V in (1, 256, 257, 1000, 32003, 50257, 200000):
+            for width in (64, 200, 1024, 2048):
+                assert lib.jb200_host_head_plan(N, V, width, sms, out) == 0
+                cols, pieces, slabs = out
+                assert cols % 256 == 0 and (pieces - 1) * cols < V <= pieces * cols
+                assert cols == 256 or N * cols * 2 <= 256 << 20        # the workspace is bounded, down to one tile of columns
+                # every slab of the first piece has K-blocks of 64 columns to sum
+                assert 1 <= slabs <= 64 and slabs <= (min(V, cols) + 63) // 64
+    assert lib.jb200_host_head_plan(0, 5, 64, 148, out) == _lib.ERR_ARG
