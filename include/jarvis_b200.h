@@ -397,7 +397,7 @@ int jb200_cross_entropy(const void* logits, int ld, int n_rows, int V, const int
 /* ---- losses of the head from hidden rows, without the logits, and their gradients ------------------------ */
 
 /* lm_head and the loss on its logits (jarvis_engine/jarvis_model.py:535-540) as one operator: the N x V logits z = x w^T are never
- * stored.  Cross entropy when `targets` is given, distillation from a teacher's top logits when `ids` is, or both of the same rows:
+ * stored.  Cross entropy when `targets` is given, distillation from a teacher's top logits when `teacher` is, or both of the same rows:
  *   ce[n] = log sum_v exp(z[n][v]) - z[n][targets[n]]
  *   kd[n] = t^2 * sum_k q[n][k] (log q[n][k] - log softmax(z[n] / t)[id[n][k]]),   t the temperature
  * The losses and their statistics are f32; products accumulate in f32 from bf16 operands. */
@@ -408,18 +408,17 @@ typedef struct jb200_head {
   const int64_t* targets;     /* [N] or NULL; -100: the row has none, its loss is 0; otherwise outside [0, V): its loss is NaN */
   float* lse;                 /* [2][N], with targets: r and s with sum exp(z) = 2^r s, left by the forward call, read by the backward one */
   int K;                      /* entries of a teacher's row, 1 to 256 */
-  const int32_t* ids;         /* [K][N] or NULL: what jb200_teacher_rows leaves */
-  const float* q;             /* [K][N] */
-  const float* neg_entropy;   /* [N] */
+  const void* teacher;        /* NULL or what jb200_teacher_rows leaves for these N, K, V and temperature */
   float temperature;
   float* lse_t;               /* [2][N], with a teacher: the same of sum exp(z / temperature) */
 } jb200_head;
 
-/* Teacher rows (ids i64 [N][K], logits f32 or bf16 [N][K]) -> entries in ascending order of id with q = softmax(logits / temperature)
- * over the row's entries, transposed, and sum q log q (+inf for a row without any, whose loss is 0; NaN where an id is >= V).  A
- * negative id is no entry, whatever its logit.  An id may come twice: its probabilities add. */
-int jb200_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, int32_t* ids_sorted,
-                       float* q, float* neg_entropy, void* stream);
+/* Teacher rows (ids i64 [N][K], logits f32 or bf16 [N][K]) -> `rows`, jb200_teacher_rows_bytes, 16-byte aligned: first, f32 [N], sum q log q
+ * with q = softmax(logits / temperature) over the row's entries (+inf for a row without any, whose loss is 0; NaN where an id is >= V),
+ * then the entries in the order in which the loss meets them.  A negative id is no entry, whatever its logit.  An id may come
+ * twice: its probabilities add. */
+size_t jb200_teacher_rows_bytes(int N, int K, int V);
+int jb200_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, void* rows, void* stream);
 
 /* ce, kd: f32 [N], where asked for.  means: NULL or f32 [4]: mean of ce over the rows with a target (NaN without any), their number, then
  * the same of kd.  Without rows both means are NaN of 0.

@@ -42,8 +42,8 @@ class Forward(C.Structure):
 
 class Head(C.Structure):
     """jb200_head"""
-    _fields_ = [("N", _I), ("V", _I), ("C", _I), ("x", _P), ("w", _P), ("targets", _P), ("lse", _P), ("K", _I), ("ids", _P), ("q", _P),
-                ("neg_entropy", _P), ("temperature", _F), ("lse_t", _P)]
+    _fields_ = [("N", _I), ("V", _I), ("C", _I), ("x", _P), ("w", _P), ("targets", _P), ("lse", _P), ("K", _I), ("teacher", _P),
+                ("temperature", _F), ("lse_t", _P)]
 
 
 # name -> (restype, argtypes); must list every function declared in include/jarvis_b200.h
@@ -84,7 +84,8 @@ PROTOTYPES = {
     "jb200_lsf_step_norm": (_I, [_P, _P, _P, _P, _I, C.c_longlong, C.c_longlong, _F, _P, _P, _F, _F, _P, _P, _P, _P, _F, _P,
                                  _I, _I, _P]),
     "jb200_cross_entropy": (_I, [_P, _I, _I, _I, _P, _P, _P, _I, _P, _I, _P, _P]),
-    "jb200_teacher_rows": (_I, [_P, _P, _I, _I, _I, _I, _F, _P, _P, _P, _P]),
+    "jb200_teacher_rows_bytes": (_Z, [_I] * 3),
+    "jb200_teacher_rows": (_I, [_P, _P, _I, _I, _I, _I, _F, _P, _P]),
     "jb200_head_loss_scratch_bytes": (_Z, [_I] * 4),
     "jb200_head_loss": (_I, [C.POINTER(Head), _P, _P, _P, _P, _P]),
     "jb200_head_loss_backward_scratch_bytes": (_Z, [_I] * 3),

@@ -468,9 +468,9 @@ int jb200_cross_entropy(const void* logits, int ld, int n_rows, int V, const int
                               static_cast<cudaStream_t>(stream));
 }
 
-int jb200_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, int32_t* ids_sorted,
-                       float* q, float* neg_entropy, void* stream) {
-  return launch_teacher_rows(ids, logits, logits_dtype, N, K, V, temperature, ids_sorted, q, neg_entropy, static_cast<cudaStream_t>(stream));
+size_t jb200_teacher_rows_bytes(int N, int K, int V) { return teacher_rows_bytes(N, K, V); }
+int jb200_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, void* rows, void* stream) {
+  return launch_teacher_rows(ids, logits, logits_dtype, N, K, V, temperature, rows, static_cast<cudaStream_t>(stream));
 }
 size_t jb200_head_loss_scratch_bytes(int N, int V, int ce, int kd) { return N < 1 || V < 1 ? 0 : head_loss_scratch_bytes(N, V, ce, kd); }
 int jb200_head_loss(const jb200_head* h, float* ce, float* kd, float* means, void* scratch, void* stream) {

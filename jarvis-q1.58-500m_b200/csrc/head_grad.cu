@@ -103,7 +103,7 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
     tma_prefetch_desc(&tmap_w);
     tma_prefetch_desc(&tmap_x);
   }
-  pair_ring_init(ctl, warp);
+  pair_ring_init(ctl, warp, 16);
   pdl_wait();
   pdl_trigger();
   const uint32_t tmem = ctl->tmem_base;

@@ -30,6 +30,8 @@ constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int TEACHER_MAX = 256;
 constexpr size_t PIECE_BYTES = size_t(256) << 20;      // bf16 gradients of the logits kept at a time
 
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -37,98 +39,116 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // ---------------------------------------------------------------------------
-// The teacher's rows: entries sorted by id (a tile's epilogue walks them in step with its columns) with their probabilities.
+// The teacher's rows: entries (id, q) by ascending id, [N][K], and where each 256 columns' entries begin, [N][tiles], so that a tile's
+// epilogue finds its own with one load.
 // ---------------------------------------------------------------------------
-constexpr int TEACHER_ROWS = 32, TEACHER_WARPS = 8;
+constexpr int TEACHER_WARPS = 8;
 
-template <typename T> __device__ __forceinline__ float teacher_value(const T* p);
-template <> __device__ __forceinline__ float teacher_value<float>(const float* p) { return *p; }
-template <> __device__ __forceinline__ float teacher_value<__nv_bfloat16>(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+struct TeacherLayout {
+  size_t entries, starts, total;         // neg_entropy, f32 [N], comes first
+};
+TeacherLayout teacher_layout(int N, int K, int V) {
+  TeacherLayout l;
+  l.entries = up256(size_t(N) * 4);
+  l.starts = l.entries + up256(size_t(N) * K * 8);
+  l.total = l.starts + up256(size_t(N) * ((size_t(V) + HEAD_TILE - 1) / HEAD_TILE) * 2);
+  return l;
+}
 
-// One warp takes a row at a time; [K][32 rows] tiles leave through shared memory, since the consumers' lanes are rows.
-// neg_entropy: sum q log q; +inf for a row without entries, NaN for one with an id beyond the vocabulary.
+__device__ __forceinline__ float teacher_value(const float* p) { return *p; }
+__device__ __forceinline__ float teacher_value(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+
+// A warp a row; an entry's place is the number of entries before it.  neg_entropy: sum q log q; +inf for a row without entries,
+// NaN for one with an id beyond the vocabulary.
 template <typename T>
 __global__ void __launch_bounds__(32 * TEACHER_WARPS)
 teacher_rows_kernel(const int64_t* __restrict__ ids, const T* __restrict__ logits, int N, int K, int V, float inv_tau,
-                    int* __restrict__ ids_out, float* __restrict__ q_out, float* __restrict__ neg_entropy) {
+                    float* __restrict__ neg_entropy, int2* __restrict__ entries, uint16_t* __restrict__ starts) {
   pdl_wait();
   pdl_trigger();
-  extern __shared__ int s_teacher[];
-  int* t_id = s_teacher;                                       // [K][33]
-  float* t_q = reinterpret_cast<float*>(t_id + K * 33);        // [K][33]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int* w_id = t_id + 2 * K * 33 + warp * K;                    // [warps][K]: the row as it came
-  const int row0 = blockIdx.x * TEACHER_ROWS;
-  for (int r = warp; r < TEACHER_ROWS; r += TEACHER_WARPS) {
-    const int row = row0 + r;
-    if (row >= N) break;
-    constexpr int PER = TEACHER_MAX / 32;
-    float v[PER];
-    int id[PER];
-    bool bad = false;
-    float top = -INFINITY;
+  constexpr int PER = TEACHER_MAX / 32;
+  __shared__ __align__(16) int s_id[TEACHER_WARPS][TEACHER_MAX];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * TEACHER_WARPS + warp;
+  if (row >= N) return;
+  int* mine = s_id[warp];
+  const int per = (K + 31) >> 5;         // entries of a lane
+  float v[PER];
+  int id[PER];
+  bool bad = false;
+  float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int k = i * 32 + lane;
-      v[i] = -INFINITY;
-      id[i] = INT_MAX;
-      if (k < K) {
-        const long long y = ids[size_t(row) * K + k];
-        if (y >= 0) {
-          v[i] = teacher_value(logits + size_t(row) * K + k) * inv_tau;
-          if (y >= V) bad = true; else id[i] = int(y);
-        }
-        w_id[k] = id[i];
-        top = fmaxf(top, v[i]);
+  for (int i = 0; i < PER; ++i) {
+    v[i] = -INFINITY;
+    id[i] = INT_MAX;
+    const int k = i * 32 + lane;
+    if (k < K) {
+      const long long y = ids[size_t(row) * K + k];
+      if (y >= 0) {
+        v[i] = teacher_value(logits + size_t(row) * K + k) * inv_tau;
+        if (y >= V) bad = true; else id[i] = int(y);
       }
+      top = fmaxf(top, v[i]);
     }
-    bad = __any_sync(0xffffffffu, bad);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    // a row whose kept values are all -inf has no probabilities either (a NaN among them: NaN)
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const float e = top == -INFINITY && v[i] == -INFINITY ? 0.f : expf(v[i] - (top == -INFINITY ? 0.f : top));
-      v[i] -= top;
-      sum += id[i] == INT_MAX ? 0.f : e;
-    }
-    sum = warp_sum(sum);
-    const float inv = 1.0f / sum, log_sum = logf(sum);
-    const bool none = sum == 0.f && !bad;
-    float ent = 0.f;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int k = i * 32 + lane;
-      if (k >= K) break;
-      float q = 0.f;
-      if (id[i] != INT_MAX && !none) {
-        if (v[i] != -INFINITY) {
-          q = expf(v[i]) * inv;
-          ent += q * (v[i] - log_sum);
-        }
-      }
-      int at = 0;                                              // its place: how many come before it
-      for (int j = 0; j < K; ++j) {
-        const int other = w_id[j];
-        at += other < id[i] || (other == id[i] && j < k);
-      }
-      t_id[at * 33 + r] = none ? INT_MAX : id[i];
-      t_q[at * 33 + r] = q;
-    }
-    ent = warp_sum(ent);
-    if (lane == 0) neg_entropy[row] = bad ? __int_as_float(0x7fc00000) : none ? INFINITY : ent;
-    __syncwarp();
+    if (i < per) mine[k] = id[i];        // the places beyond K: behind everything
   }
-  __syncthreads();
-  const int rows = min(TEACHER_ROWS, N - row0);
-  for (int i = threadIdx.x; i < K * TEACHER_ROWS; i += 32 * TEACHER_WARPS) {
-    const int k = i >> 5, r = i & 31;
-    if (r < rows) {
-      ids_out[size_t(k) * N + row0 + r] = t_id[k * 33 + r];
-      q_out[size_t(k) * N + row0 + r] = t_q[k * 33 + r];
+  bad = __any_sync(0xffffffffu, bad);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  // a row whose kept values are all -inf has no probabilities either (a NaN among them: NaN)
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    v[i] -= base;
+    if (id[i] != INT_MAX) sum += expf(v[i]);
+  }
+  sum = warp_sum(sum);
+  const float inv = 1.0f / sum, log_sum = logf(sum);
+  const bool none = sum == 0.f && !bad;
+  float ent = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const float q = expf(v[i]) * inv;
+    if (none) id[i] = INT_MAX;
+    if (id[i] != INT_MAX && v[i] != -INFINITY) ent += q * (v[i] - log_sum);
+    v[i] = q;
+  }
+  ent = warp_sum(ent);
+  if (lane == 0) neg_entropy[row] = bad ? __int_as_float(0x7fc00000) : none ? INFINITY : ent;
+  __syncwarp();
+  int at[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) at[i] = 0;
+  for (int j = 0; j < 32 * per; j += 4) {
+    const int4 o = *reinterpret_cast<const int4*>(mine + j);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (i >= per) break;
+      const int k = i * 32 + lane;       // of equal ids the earlier one comes first
+      at[i] += (o.x < id[i] || (o.x == id[i] && j < k)) + (o.y < id[i] || (o.y == id[i] && j + 1 < k)) +
+               (o.z < id[i] || (o.z == id[i] && j + 2 < k)) + (o.w < id[i] || (o.w == id[i] && j + 3 < k));
     }
+  }
+  __syncwarp();
+  int2* out = entries + size_t(row) * K;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (i >= per) break;
+    if (none) at[i] = i * 32 + lane;     // (its ids in shared memory are not INT_MAX)
+    if (at[i] < K) {
+      out[at[i]] = make_int2(id[i], __float_as_int(id[i] == INT_MAX ? 0.f : v[i]));
+      mine[at[i]] = id[i];
+    }
+  }
+  __syncwarp();
+  const int tiles = (V + HEAD_TILE - 1) / HEAD_TILE;
+  for (int t = lane; t < tiles; t += 32) {
+    int lo = 0, hi = K;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (mine[mid] < t * HEAD_TILE) lo = mid + 1; else hi = mid;
+    }
+    starts[size_t(row) * tiles + t] = uint16_t(lo);
   }
 }
 
@@ -139,12 +159,14 @@ struct HeadLogits {
   int N, V, C;
   int v0, cols;              // vocabulary columns [v0, v0 + cols) of this launch
   const int64_t* targets;    // CE
-  const int* ids;            // KD: [K][N], ascending in every row
-  const float* q;
-  int K;
+  const int2* entries;       // KD: what teacher_rows_kernel leaves
+  const uint16_t* starts;
+  int K, v_tiles;            // tiles of the whole vocabulary
   float inv_tau;
-  float* part;               // statistics: [2 tiles + half][values][N]
+  float* part;               // statistics: [parts][values][N]
+  int carry;                 // a pair's tiles are all of the same rows: it leaves one part a group of epilogue warps, else every tile does
   float* z_target;           // [N]
+  unsigned int* ticket;      // set to 0 for the join
   // gradient, [3][N] each: the sum's reference point, the row's factor, and the factor over the sum
   const float *r_ce, *r_kd;
   __nv_bfloat16* g;          // gradient: [N][ldg]
@@ -192,10 +214,41 @@ struct RunningSum {
   }
 };
 
+// A row's teacher entries from one on; the next is on its way while the current is used.
+struct Entries {
+  const int2* row;
+  int at, K, id = INT_MAX;
+  float q = 0.f;
+  int2 next = {INT_MAX, 0};
+  __device__ __forceinline__ void fetch() {
+    next = at < K ? __ldg(row + at) : make_int2(INT_MAX, 0);
+    ++at;
+  }
+  __device__ __forceinline__ void step() {
+    id = next.x;
+    q = __int_as_float(next.y);
+    fetch();
+  }
+  __device__ __forceinline__ void begin(const int2* entries, int n_entries, int start) {
+    row = entries; K = n_entries; at = start;
+    fetch();
+    step();
+  }
+};
+
 constexpr int head_values(bool ce, bool kd) { return (ce ? 2 : 0) + (kd ? 3 : 0); }
 
-// A lane of an epilogue warp is a row, its registers are 32 consecutive columns.  Bound by the tensor pipe: a tile is 8 C / 64 x 512
-// cycles of MMA against about 1200 issue cycles of epilogue.
+template <bool CE, bool KD>
+__device__ __forceinline__ void head_part(const HeadLogits& p, int part, int row, const RunningSum& s1, const RunningSum& s2, float dot) {
+  float* o = p.part + size_t(part) * head_values(CE, KD) * p.N + row;
+  if (CE) { o[0] = s1.ref; o[p.N] = s1.sum; o += 2 * size_t(p.N); }
+  if (KD) { o[0] = s2.ref; o[p.N] = s2.sum; o[2 * size_t(p.N)] = dot; }
+}
+
+// A lane of an epilogue warp is a row, its registers are 32 consecutive columns.  Two groups of four epilogue warps drain alternate
+// tiles, each the accumulator of its own (eight warps on every tile leave twice the parts to join).  A column of a row that the
+// teacher asks for is not known to the compiler: where a warp has one, 16 columns go through shared memory, lanes side by side (32
+// compared registers an entry cost 6 to 30 % of a launch at 32 to 64 entries a row).
 template <bool CE, bool KD, bool GRAD>
 __global__ void __launch_bounds__(HEAD_THREADS, 1)
 head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
@@ -204,14 +257,15 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
   const uint32_t a_base = base, b_base = base + HEAD_STAGES * HEAD_OPERAND;
-  HeadRing* ctl = reinterpret_cast<HeadRing*>(smem_raw + (base - raw_addr) + 2 * HEAD_STAGES * HEAD_OPERAND);
+  uint8_t* behind = smem_raw + (base - raw_addr) + 2 * HEAD_STAGES * HEAD_OPERAND;
+  HeadRing* ctl = reinterpret_cast<HeadRing*>(behind);
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int rank = int(cluster_rank());
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmap_x);
     tma_prefetch_desc(&tmap_w);
   }
-  pair_ring_init(ctl, warp);
+  pair_ring_init(ctl, warp, 8);
   pdl_wait();
   pdl_trigger();
   const uint32_t tmem = ctl->tmem_base;
@@ -219,6 +273,8 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
   const int pair = int(blockIdx.x >> 1), n_pairs = int(gridDim.x >> 1);
   const int tm = (p.N + HEAD_TILE - 1) / HEAD_TILE, tv = (p.cols + HEAD_TILE - 1) / HEAD_TILE, total = tm * tv;
   const int n_kb = (p.C + HEAD_BK - 1) / HEAD_BK;
+
+  if (!GRAD && blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0u;
 
   if (warp == 0) {
     // ---------------- TMA: this CTA's rows and its half of the columns ----------------
@@ -275,47 +331,37 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
   } else {
     // ---------------- epilogue ----------------
     const int quarter = warp & 3;                              // TMEM lanes this warp may read
-    const int half = (warp - HEAD_EPI_WARP0) >> 2;             // which of the alternating 32-column chunks
+    const uint32_t group = uint32_t(warp - HEAD_EPI_WARP0) >> 2;
+    // [16 columns][32 lanes] of this warp
+    float* stage = reinterpret_cast<float*>(behind + HEAD_CTL) + (warp - HEAD_EPI_WARP0) * 512 + lane;
     const float k1 = LOG2E, k2 = LOG2E * p.inv_tau;
-    uint32_t tile = 0u;
-    for (int t = pair; t < total; t += n_pairs, ++tile) {
-      const uint32_t acc = tile & 1u;
+    RunningSum s1, s2;
+    float dot = 0.f;
+    uint32_t ph = 0u;
+    for (int t = pair + int(group) * n_pairs; t < total; t += 2 * n_pairs, ph ^= 1u) {
       int m, v;
       head_tile(t, tm, tv, &m, &v);
       const int f0 = p.v0 + v * HEAD_TILE;                     // first vocabulary column, and the first beyond the launch's
       const int f_end = min(f0 + HEAD_TILE, p.v0 + p.cols);
       const int row = m * HEAD_TILE + rank * (HEAD_TILE / 2) + quarter * 32 + lane;
       const bool on = row < p.N;
+      Entries e;
+      if (KD && on) e.begin(p.entries + size_t(row) * p.K, p.K, __ldg(p.starts + size_t(row) * p.v_tiles + f0 / HEAD_TILE));
       int target = -1;
       if (CE && on) {
         const long long y = p.targets[row];
         if (y >= f0 && y < f_end) target = int(y) - f0;
-      }
-      // the row's first entry in this tile
-      int at = p.K, next = INT_MAX;
-      const int* ids = p.ids + row;
-      const float* q = p.q + row;
-      if (KD && on) {
-        int lo = 0, hi = p.K;
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (__ldg(ids + size_t(mid) * p.N) < f0) lo = mid + 1; else hi = mid;
-        }
-        at = lo;
-        if (at < p.K) next = __ldg(ids + size_t(at) * p.N);
       }
       float l1 = 0.f, l2 = 0.f, g1 = 0.f, g2 = 0.f, p1 = 0.f, p2 = 0.f;
       if (GRAD && on) {
         if (CE) { l1 = p.r_ce[row]; g1 = p.r_ce[size_t(p.N) + row]; p1 = p.r_ce[2 * size_t(p.N) + row]; }
         if (KD) { l2 = p.r_kd[row]; g2 = p.r_kd[size_t(p.N) + row]; p2 = p.r_kd[2 * size_t(p.N) + row]; }
       }
-      RunningSum s1, s2;
-      float dot = 0.f;
-      if (!mbar_wait(smem_u32(&ctl->acc_full[acc]), (tile >> 1) & 1u, abort_flag, p.status, JB200_STATUS_HEAD_EPILOGUE)) break;
+      if (!mbar_wait(smem_u32(&ctl->acc_full[group]), ph, abort_flag, p.status, JB200_STATUS_HEAD_EPILOGUE)) break;
       tc_fence_after_sync();
       __syncwarp();
-      const uint32_t t_lane = tmem + (uint32_t(quarter * 32) << 16) + acc * HEAD_TILE;
-      for (int c0 = half * 32; c0 < HEAD_TILE; c0 += 64) {
+      const uint32_t t_lane = tmem + (uint32_t(quarter * 32) << 16) + group * HEAD_TILE;
+      for (int c0 = 0; c0 < HEAD_TILE; c0 += 32) {
         const int col = f0 + c0;
         if (!GRAD && col >= f_end) break;
         uint32_t z[32];
@@ -337,16 +383,17 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
               if (target - c0 == j) g[j] -= g1;
           }
           if (KD) {
-            while (__any_sync(0xffffffffu, next < col + 32)) {
-              if (next < col + 32) {
-                const int j0 = next - col;                     // below 0: the other half's
-                const float d = j0 < 0 ? 0.f : g2 * __ldg(q + size_t(at) * p.N);
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (j0 == j) g[j] -= d;
-                ++at;
-                next = at < p.K ? __ldg(ids + size_t(at) * p.N) : INT_MAX;
+            for (int h = 0; h < 32; h += 16) {
+              if (!__any_sync(0xffffffffu, e.id < col + h + 16)) continue;
+#pragma unroll
+              for (int j = 0; j < 16; ++j) stage[j * 32] = g[h + j];
+              while (e.id < col + h + 16) {                    // an id may come twice
+                stage[(e.id - col - h) * 32] -= g2 * e.q;
+                e.step();
               }
+#pragma unroll
+              for (int j = 0; j < 16; ++j) g[h + j] = stage[j * 32];
               __syncwarp();
             }
           }
@@ -369,15 +416,14 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
             if (unsigned(target - c0) < 32u) p.z_target[row] = x;
           }
           if (KD) {
-            while (__any_sync(0xffffffffu, next < col + 32)) {
-              if (next < col + 32) {
-                const int j0 = next - col;
-                if (j0 >= 0) {
-                  const float w = __ldg(q + size_t(at) * p.N);
-                  if (w != 0.f) dot = fmaf(w, pick32(z, j0), dot);
-                }
-                ++at;
-                next = at < p.K ? __ldg(ids + size_t(at) * p.N) : INT_MAX;
+#pragma unroll
+            for (int h = 0; h < 32; h += 16) {
+              if (!__any_sync(0xffffffffu, e.id < col + h + 16)) continue;
+#pragma unroll
+              for (int j = 0; j < 16; ++j) stage[j * 32] = __uint_as_float(z[h + j]);
+              while (e.id < col + h + 16) {
+                if (e.q != 0.f) dot = fmaf(e.q, stage[(e.id - col - h) * 32], dot);
+                e.step();
               }
               __syncwarp();
             }
@@ -396,13 +442,16 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
       }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) cluster_mbar_arrive(cluster_map(smem_u32(&ctl->acc_empty[acc]), 0u));
-      if (!GRAD && on) {
-        constexpr int F = head_values(CE, KD);
-        float* o = p.part + size_t(2 * v + half) * F * p.N + row;
-        if (CE) { o[0] = s1.ref; o[p.N] = s1.sum; o += 2 * size_t(p.N); }
-        if (KD) { o[0] = s2.ref; o[p.N] = s2.sum; o[2 * size_t(p.N)] = dot; }
+      if (lane == 0) cluster_mbar_arrive(cluster_map(smem_u32(&ctl->acc_empty[group]), 0u));
+      if (!GRAD && !p.carry) {
+        if (on) head_part<CE, KD>(p, v, row, s1, s2, dot);
+        s1 = s2 = RunningSum();
+        dot = 0.f;
       }
+    }
+    if (!GRAD && p.carry) {
+      const int row = pair % tm * HEAD_TILE + rank * (HEAD_TILE / 2) + quarter * 32 + lane;
+      if (row < p.N) head_part<CE, KD>(p, 2 * (pair / tm) + int(group), row, s1, s2, dot);
     }
   }
   pair_ring_close(tmem, warp);
@@ -418,71 +467,104 @@ struct HeadRowsOut {
   const float* z_target;
   float *lse, *ce, *lse_t, *kd;
   float* means;              // mean and number of the rows with a target, then of those with a teacher; null: not wanted
+  unsigned int* ticket;
   int N, V, parts;
   float inv_tau, tau;
 };
 
-__device__ __forceinline__ void join(float& ref, float& sum, float r, float s) {
-  const float to = fmaxf(ref, r);
-  sum = to == -INFINITY ? sum + s : (ref == -INFINITY ? sum : sum * ex2(ref - to)) + (r == -INFINITY ? s : s * ex2(r - to));
+// 2^ref sum += sum over i of 2^r[i] s[i].  Parts without a finite logit have ref = -inf and a sum of 0 or NaN.
+template <int N>
+__device__ __forceinline__ void join(float& ref, float& sum, const float (&r)[N], const float (&s)[N]) {
+  float to = ref;
+#pragma unroll
+  for (int i = 0; i < N; ++i) to = fmaxf(to, r[i]);
+  const float at = to == -INFINITY ? 0.f : to;
+  sum *= ex2(ref - at);
+#pragma unroll
+  for (int i = 0; i < N; ++i) sum = fmaf(s[i], ex2(r[i] - at), sum);
   ref = to;
 }
+__device__ __forceinline__ void join_lanes(float& ref, float& sum, int o) {
+  const float r[1] = {__shfl_xor_sync(0xffffffffu, ref, o)}, s[1] = {__shfl_xor_sync(0xffffffffu, sum, o)};
+  join(ref, sum, r, s);
+}
 
-constexpr int JOIN_GROUPS = 32;      // warps of a CTA: each takes every 32nd part of the CTA's 32 rows
+// A CTA takes 32 rows: lanes are rows while the parts are read (each warp every 32nd of them), then every warp joins one row's 32 sums.
+// The CTA that ends last forms the means over all rows in a fixed order: thread, warp, warps.
+constexpr int JOIN_WARPS = 32;
 
 template <bool CE, bool KD>
-__global__ void __launch_bounds__(32 * JOIN_GROUPS) head_join_kernel(const __grid_constant__ HeadRowsOut p) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS) head_join_kernel(const __grid_constant__ HeadRowsOut p) {
   pdl_wait();
   pdl_trigger();
   constexpr int F = head_values(CE, KD);
-  __shared__ float s_v[JOIN_GROUPS][F][33];
-  const int g = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * 32 + lane;
+  __shared__ float s_v[JOIN_WARPS][F][33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float r1 = -INFINITY, s1 = 0.f, r2 = -INFINITY, s2 = 0.f, dot = 0.f;
-  if (row < p.N) {
-#pragma unroll 4
-    for (int i = g; i < p.parts; i += JOIN_GROUPS) {
-      const float* v = p.part + size_t(i) * F * p.N + row;
-      if (CE) { join(r1, s1, v[0], v[p.N]); v += 2 * size_t(p.N); }
-      if (KD) { join(r2, s2, v[0], v[p.N]); dot += v[2 * size_t(p.N)]; }
+  if (const int row = blockIdx.x * 32 + lane; row < p.N) {
+    constexpr int U = 4;                 // parts asked for at a time
+    for (int i0 = warp; i0 < p.parts; i0 += U * JOIN_WARPS) {
+      float ar[U], as[U], br[U], bs[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * JOIN_WARPS;
+        ar[u] = br[u] = -INFINITY;
+        as[u] = bs[u] = 0.f;
+        if (i < p.parts) {
+          const float* v = p.part + size_t(i) * F * p.N + row;
+          if (CE) { ar[u] = __ldcs(v); as[u] = __ldcs(v + p.N); v += 2 * size_t(p.N); }
+          if (KD) { br[u] = __ldcs(v); bs[u] = __ldcs(v + p.N); dot += __ldcs(v + 2 * size_t(p.N)); }
+        }
+      }
+      if (CE) join(r1, s1, ar, as);
+      if (KD) join(r2, s2, br, bs);
     }
   }
-  if (CE) { s_v[g][0][lane] = r1; s_v[g][1][lane] = s1; }
-  if (KD) { s_v[g][F - 3][lane] = r2; s_v[g][F - 2][lane] = s2; s_v[g][F - 1][lane] = dot; }
+  if (CE) { s_v[warp][0][lane] = r1; s_v[warp][1][lane] = s1; }
+  if (KD) { s_v[warp][F - 3][lane] = r2; s_v[warp][F - 2][lane] = s2; s_v[warp][F - 1][lane] = dot; }
   __syncthreads();
-  if (g != 0 || row >= p.N) return;
-  for (int i = 1; i < JOIN_GROUPS; ++i) {
-    if (CE) join(r1, s1, s_v[i][0][lane], s_v[i][1][lane]);
-    if (KD) { join(r2, s2, s_v[i][F - 3][lane], s_v[i][F - 2][lane]); dot += s_v[i][F - 1][lane]; }
+  if (CE) { r1 = s_v[lane][0][warp]; s1 = s_v[lane][1][warp]; }
+  if (KD) { r2 = s_v[lane][F - 3][warp]; s2 = s_v[lane][F - 2][warp]; dot = s_v[lane][F - 1][warp]; }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (CE) join_lanes(r1, s1, o);
+    if (KD) {
+      join_lanes(r2, s2, o);
+      dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    }
   }
-  const float nan = __int_as_float(0x7fc00000);
-  if (CE) {
-    const double l = (double(r1) + log2(double(s1))) / double(LOG2E);
-    const long long y = p.targets[row];
-    p.lse[row] = r1;
-    p.lse[size_t(p.N) + row] = s1;
-    p.ce[row] = y == -100 ? 0.f : y >= 0 && y < p.V ? float(l - double(p.z_target[row])) : nan;
+  if (const int row = blockIdx.x * 32 + warp; lane == 0 && row < p.N) {
+    if (CE) {
+      const double l = (double(r1) + log2(double(s1))) / double(LOG2E);
+      const long long y = p.targets[row];
+      p.lse[row] = r1;
+      p.lse[size_t(p.N) + row] = s1;
+      p.ce[row] = y == -100 ? 0.f : y >= 0 && y < p.V ? float(l - double(p.z_target[row])) : __int_as_float(0x7fc00000);
+    }
+    if (KD) {
+      const double l = (double(r2) + log2(double(s2))) / double(LOG2E * p.inv_tau);      // tau times the logarithm of sum exp(z / tau)
+      const float e = p.neg_entropy[row];
+      p.lse_t[row] = r2;
+      p.lse_t[size_t(p.N) + row] = s2;
+      p.kd[row] = e == INFINITY ? 0.f : float(double(p.tau) * (double(p.tau) * double(e) + (l - double(dot))));
+    }
   }
-  if (KD) {
-    const double l = (double(r2) + log2(double(s2))) / double(LOG2E * p.inv_tau);      // tau times the logarithm of sum exp(z / tau)
-    const float e = p.neg_entropy[row];
-    p.lse_t[row] = r2;
-    p.lse_t[size_t(p.N) + row] = s2;
-    p.kd[row] = e == INFINITY ? 0.f : float(double(p.tau) * (double(p.tau) * double(e) + (l - double(dot))));
-  }
-}
+  if (!p.means) return;
 
-// Means over the rows that count, in a fixed order: thread, warp, warps.
-template <bool CE, bool KD>
-__global__ void __launch_bounds__(1024) head_mean_kernel(const __grid_constant__ HeadRowsOut p) {
-  pdl_wait();
-  pdl_trigger();
+  __shared__ bool s_last;
   __shared__ double s_sum[2][32];
   __shared__ int s_cnt[2][32];
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = gridDim.x == 1 || atomicAdd(p.ticket, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
   double sum[2] = {0.0, 0.0};
   int cnt[2] = {0, 0};
-  for (int r = threadIdx.x; r < p.N; r += 1024) {
-    if (CE) { sum[0] += double(p.ce[r]); cnt[0] += p.targets[r] != -100; }
-    if (KD) { sum[1] += double(p.kd[r]); cnt[1] += p.neg_entropy[r] != INFINITY; }
+  for (int r = threadIdx.x; r < p.N; r += 32 * JOIN_WARPS) {
+    if (CE) { sum[0] += double(__ldcg(p.ce + r)); cnt[0] += p.targets[r] != -100; }
+    if (KD) { sum[1] += double(__ldcg(p.kd + r)); cnt[1] += p.neg_entropy[r] != INFINITY; }
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -491,7 +573,7 @@ __global__ void __launch_bounds__(1024) head_mean_kernel(const __grid_constant__
       sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
       cnt[i] += __shfl_xor_sync(0xffffffffu, cnt[i], o);
     }
-    if ((threadIdx.x & 31) == 0) { s_sum[i][threadIdx.x >> 5] = sum[i]; s_cnt[i][threadIdx.x >> 5] = cnt[i]; }
+    if (lane == 0) { s_sum[i][warp] = sum[i]; s_cnt[i][warp] = cnt[i]; }
   }
   __syncthreads();
   if (threadIdx.x < 2 && (threadIdx.x == 0 ? CE : KD)) {
@@ -623,13 +705,21 @@ __global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ 
   }
 }
 
+// Pairs of a launch.  Where as many waves do with a multiple of the row tiles, that: a pair then keeps to its rows.
+int head_pairs(int N, int cols, int sms) {
+  const long long tm = (N + HEAD_TILE - 1) / HEAD_TILE, tiles = tm * ((cols + HEAD_TILE - 1) / HEAD_TILE);
+  const long long pairs = tiles < sms / 2 ? tiles : sms / 2;
+  if (tm > pairs) return int(pairs);
+  const long long even = pairs / tm * tm;
+  return int((tiles + even - 1) / even == (tiles + pairs - 1) / pairs ? even : pairs);
+}
 template <bool CE, bool KD, bool GRAD>
 int launch_logits(const CUtensorMap& tx, const CUtensorMap& tw, const HeadLogits& p, int sms, cudaStream_t stream) {
-  const long long tiles = (long long)((p.N + HEAD_TILE - 1) / HEAD_TILE) * ((p.cols + HEAD_TILE - 1) / HEAD_TILE);
-  const int pairs = sms / 2;
   auto kernel = head_logits_kernel<CE, KD, GRAD>;
-  JB_MAX_SMEM(kernel, HEAD_SMEM);
-  launch_dep_cluster(kernel, dim3(2 * unsigned(tiles < pairs ? tiles : pairs)), dim3(HEAD_THREADS), HEAD_SMEM, 2, stream, tx, tw, p);
+  constexpr size_t smem = HEAD_SMEM + (KD ? 8 * 512 * 4 : 0);
+  static_assert(smem <= 227 * 1024, "shared memory of one CTA");
+  JB_MAX_SMEM(kernel, smem);
+  launch_dep_cluster(kernel, dim3(2 * unsigned(head_pairs(p.N, p.cols, sms))), dim3(HEAD_THREADS), smem, 2, stream, tx, tw, p);
   JB_LAUNCH_CHECK("head_logits_kernel");
   return JB200_OK;
 }
@@ -638,8 +728,6 @@ int launch_logits(bool ce, bool kd, const CUtensorMap& tx, const CUtensorMap& tw
   if (ce && kd) return launch_logits<true, true, GRAD>(tx, tw, p, sms, stream);
   return ce ? launch_logits<true, false, GRAD>(tx, tw, p, sms, stream) : launch_logits<false, true, GRAD>(tx, tw, p, sms, stream);
 }
-
-size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Everything about the arguments that both directions share.
 int check_head(const jb200_head* h, const char* what) {
@@ -650,11 +738,12 @@ int check_head(const jb200_head* h, const char* what) {
   JB_REQUIRE(tiles < INT_MAX / 4 && h->V <= INT_MAX - HEAD_TILE && h->N <= INT_MAX - HEAD_TILE, "%s: too many logits (%d x %d)", what, h->N, h->V);
   JB_REQUIRE(h->N == 0 || (h->x && h->w), "%s: null pointer", what);
   JB_REQUIRE(aligned16(h->x) && aligned16(h->w), "%s: rows and weight must be 16-byte aligned", what);
-  JB_REQUIRE(h->N == 0 || h->targets || h->ids, "%s: neither targets nor a teacher", what);
+  JB_REQUIRE(h->N == 0 || h->targets || h->teacher, "%s: neither targets nor a teacher", what);
   JB_REQUIRE(h->N == 0 || !h->targets || h->lse, "%s: lse is needed with targets", what);
-  if (h->ids) {
+  if (h->teacher) {
     JB_REQUIRE(h->K >= 1 && h->K <= TEACHER_MAX, "%s: a teacher has 1 to %d entries a row, got %d", what, TEACHER_MAX, h->K);
-    JB_REQUIRE(h->q && h->neg_entropy && h->lse_t, "%s: null pointer (teacher)", what);
+    JB_REQUIRE(h->lse_t, "%s: null pointer (teacher)", what);
+    JB_REQUIRE((reinterpret_cast<uintptr_t>(h->teacher) & 15u) == 0, "%s: teacher rows must be 16-byte aligned", what);
     JB_REQUIRE(h->temperature > 0.f && h->temperature <= FLT_MAX && 1.0f / h->temperature <= FLT_MAX, "%s: temperature must be positive and finite", what);
   }
   return JB200_OK;
@@ -689,57 +778,78 @@ HeadPlan head_plan(int N, int V, int C, int pairs) {
   return pl;
 }
 
-int launch_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, int* ids_out,
-                        float* q_out, float* neg_entropy, cudaStream_t stream) {
+size_t teacher_rows_bytes(int N, int K, int V) { return N < 1 || K < 1 || V < 1 ? 0 : teacher_layout(N, K, V).total; }
+
+int launch_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, void* rows,
+                        cudaStream_t stream) {
   JB_REQUIRE(N >= 0 && V >= 1, "teacher_rows: bad shape");
   JB_REQUIRE(K >= 1 && K <= TEACHER_MAX, "teacher_rows: a teacher has 1 to %d entries a row, got %d", TEACHER_MAX, K);
   JB_REQUIRE(logits_dtype == 0 || logits_dtype == 1, "teacher_rows: dtype must be 0 (f32) or 1 (bf16)");
   JB_REQUIRE(temperature > 0.f && temperature <= FLT_MAX && 1.0f / temperature <= FLT_MAX, "teacher_rows: temperature must be positive and finite");
   if (N == 0) return JB200_OK;
-  JB_REQUIRE(ids && logits && ids_out && q_out && neg_entropy, "teacher_rows: null pointer");
-  const size_t smem = size_t(K) * (2 * 33 + TEACHER_WARPS) * 4;
-  const dim3 grid((N + TEACHER_ROWS - 1) / TEACHER_ROWS), block(32 * TEACHER_WARPS);
-  const size_t most = size_t(TEACHER_MAX) * (2 * 33 + TEACHER_WARPS) * 4;
+  JB_REQUIRE(ids && logits && rows, "teacher_rows: null pointer");
+  JB_REQUIRE(aligned16(rows), "teacher_rows: rows must be 16-byte aligned");
+  const TeacherLayout at = teacher_layout(N, K, V);
+  uint8_t* base = static_cast<uint8_t*>(rows);
+  float* neg_entropy = static_cast<float*>(rows);
+  int2* entries = reinterpret_cast<int2*>(base + at.entries);
+  uint16_t* starts = reinterpret_cast<uint16_t*>(base + at.starts);
+  const dim3 grid((N + TEACHER_WARPS - 1) / TEACHER_WARPS), block(32 * TEACHER_WARPS);
   if (logits_dtype == 0) {
-    JB_MAX_SMEM(teacher_rows_kernel<float>, most);
-    launch_dep(teacher_rows_kernel<float>, grid, block, smem, stream, ids, static_cast<const float*>(logits), N, K, V, 1.0f / temperature,
-               ids_out, q_out, neg_entropy);
+    launch_dep(teacher_rows_kernel<float>, grid, block, 0, stream, ids, static_cast<const float*>(logits), N, K, V, 1.0f / temperature,
+               neg_entropy, entries, starts);
   } else {
-    JB_MAX_SMEM(teacher_rows_kernel<__nv_bfloat16>, most);
-    launch_dep(teacher_rows_kernel<__nv_bfloat16>, grid, block, smem, stream, ids, static_cast<const __nv_bfloat16*>(logits), N, K, V,
-               1.0f / temperature, ids_out, q_out, neg_entropy);
+    launch_dep(teacher_rows_kernel<__nv_bfloat16>, grid, block, 0, stream, ids, static_cast<const __nv_bfloat16*>(logits), N, K, V,
+               1.0f / temperature, neg_entropy, entries, starts);
   }
   JB_LAUNCH_CHECK("teacher_rows_kernel");
   return JB200_OK;
 }
 
+namespace {
+void set_teacher(HeadLogits& p, const jb200_head* h) {
+  if (!h->teacher) return;
+  const TeacherLayout at = teacher_layout(h->N, h->K, h->V);
+  const uint8_t* base = static_cast<const uint8_t*>(h->teacher);
+  p.entries = reinterpret_cast<const int2*>(base + at.entries);
+  p.starts = reinterpret_cast<const uint16_t*>(base + at.starts);
+  p.K = h->K;
+  p.v_tiles = (h->V + HEAD_TILE - 1) / HEAD_TILE;
+}
+}  // namespace
+
 size_t head_loss_scratch_bytes(int N, int V, int ce, int kd) {
-  const size_t parts = 2 * ((size_t(V) + HEAD_TILE - 1) / HEAD_TILE);
-  return (parts * head_values(ce != 0, kd != 0) + 1) * size_t(N) * 4;
+  const size_t parts = (size_t(V) + HEAD_TILE - 1) / HEAD_TILE;
+  return (parts * head_values(ce != 0, kd != 0) + 1) * size_t(N) * 4 + 4;
 }
 
 int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* means, void* scratch, cudaStream_t stream) {
   int rc = check_head(h, "head_loss");
   if (rc != JB200_OK) return rc;
   JB_REQUIRE(h->N == 0 || scratch, "head_loss: null pointer (scratch)");
-  JB_REQUIRE(h->N == 0 || ((!h->targets || ce) && (!h->ids || kd)), "head_loss: null pointer (losses)");
-  const bool has_ce = h->targets != nullptr, has_kd = h->ids != nullptr;
+  JB_REQUIRE(h->N == 0 || ((!h->targets || ce) && (!h->teacher || kd)), "head_loss: null pointer (losses)");
+  const bool has_ce = h->targets != nullptr, has_kd = h->teacher != nullptr;
   if (h->N == 0 && !means) return JB200_OK;
   HeadRowsOut o{};
-  o.targets = h->targets; o.neg_entropy = h->neg_entropy;
+  o.targets = h->targets; o.neg_entropy = static_cast<const float*>(h->teacher);
   o.lse = h->lse; o.ce = ce; o.lse_t = h->lse_t; o.kd = kd; o.means = means;
   o.N = h->N; o.V = h->V;
   o.tau = has_kd ? h->temperature : 1.f;
   o.inv_tau = 1.0f / o.tau;
-  o.parts = 2 * ((h->V + HEAD_TILE - 1) / HEAD_TILE);
+  o.parts = (h->V + HEAD_TILE - 1) / HEAD_TILE;
   if (h->N > 0) {
     const int sms = sm_count();
     if (sms < 2) return JB200_ERR_CUDA;
     HeadLogits p{};
     p.N = h->N; p.V = h->V; p.C = h->C; p.v0 = 0; p.cols = h->V;
-    p.targets = h->targets; p.ids = h->ids; p.q = h->q; p.K = h->K; p.inv_tau = o.inv_tau;
+    p.targets = h->targets; p.inv_tau = o.inv_tau;
+    set_teacher(p, h);
+    const int tm = (h->N + HEAD_TILE - 1) / HEAD_TILE, pairs = head_pairs(h->N, h->V, sms);
+    p.carry = pairs % tm == 0 && tm <= HEAD_GROUP && 2 * (pairs / tm) <= o.parts;
+    if (p.carry) o.parts = 2 * (pairs / tm);
     p.part = static_cast<float*>(scratch);
     p.z_target = p.part + size_t(o.parts) * head_values(has_ce, has_kd) * h->N;
+    p.ticket = o.ticket = reinterpret_cast<unsigned int*>(p.z_target + h->N);
     p.status = device_status_ptr();
     if (!p.status) return JB200_ERR_CUDA;
     o.part = p.part; o.z_target = p.z_target;
@@ -747,16 +857,11 @@ int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* means, vo
     if ((rc = encode_head_map(&tx, h->x, h->C, h->N, HEAD_TILE / 2, "head_loss (rows)")) != JB200_OK) return rc;
     if ((rc = encode_head_map(&tw, h->w, h->C, h->V, HEAD_TILE / 2, "head_loss (weight)")) != JB200_OK) return rc;
     if ((rc = launch_logits<false>(has_ce, has_kd, tx, tw, p, sms, stream)) != JB200_OK) return rc;
-    auto join = has_ce && has_kd ? head_join_kernel<true, true> : has_ce ? head_join_kernel<true, false> : head_join_kernel<false, true>;
-    launch_dep(join, (h->N + 31) / 32, 32 * JOIN_GROUPS, 0, stream, o);
-    JB_LAUNCH_CHECK("head_join_kernel");
   }
-  if (means) {
-    // (without rows both means are written: nothing says which was asked for)
-    auto mean = (has_ce && has_kd) || h->N == 0 ? head_mean_kernel<true, true> : has_ce ? head_mean_kernel<true, false> : head_mean_kernel<false, true>;
-    launch_dep(mean, 1, 1024, 0, stream, o);
-    JB_LAUNCH_CHECK("head_mean_kernel");
-  }
+  // (without rows both means are written: nothing says which was asked for)
+  auto join = (has_ce && has_kd) || h->N == 0 ? head_join_kernel<true, true> : has_ce ? head_join_kernel<true, false> : head_join_kernel<false, true>;
+  launch_dep(join, h->N > 0 ? (h->N + 31) / 32 : 1, 32 * JOIN_WARPS, 0, stream, o);
+  JB_LAUNCH_CHECK("head_join_kernel");
   return JB200_OK;
 }
 
@@ -794,7 +899,7 @@ int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_s
   }
   JB_REQUIRE(aligned16(dx) && scratch && (reinterpret_cast<uintptr_t>(scratch) & 255u) == 0,
              "head_loss_backward: dx must be 16-byte, scratch 256-byte aligned");
-  JB_REQUIRE((!h->targets || g_ce) && (!h->ids || g_kd), "head_loss_backward: null pointer (gradients of the losses)");
+  JB_REQUIRE((!h->targets || g_ce) && (!h->teacher || g_kd), "head_loss_backward: null pointer (gradients of the losses)");
   JB_REQUIRE((g_ce_stride == 0 || g_ce_stride == 1) && (g_kd_stride == 0 || g_kd_stride == 1), "head_loss_backward: strides must be 0 or 1");
   const int sms = sm_count();
   if (sms < 2) return JB200_ERR_CUDA;
@@ -806,13 +911,13 @@ int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_s
 
   HeadRowsIn r{};
   r.x = static_cast<const __nv_bfloat16*>(h->x);
-  r.targets = h->targets; r.neg_entropy = h->ids ? h->neg_entropy : nullptr;
+  r.targets = h->targets; r.neg_entropy = static_cast<const float*>(h->teacher);
   r.lse_in = h->lse; r.lse_t_in = h->lse_t;
   r.g_ce = g_ce; r.g_kd = g_kd; r.g_ce_stride = g_ce_stride; r.g_kd_stride = g_kd_stride; r.n_ce = n_ce; r.n_kd = n_kd;
   r.xs = reinterpret_cast<__nv_bfloat16*>(base + at.xs);
   r.r_ce = rows; r.r_kd = rows + 3 * N;
   r.N = h->N; r.V = h->V; r.C = h->C;
-  r.tau = h->ids ? h->temperature : 1.f;
+  r.tau = h->teacher ? h->temperature : 1.f;
   r.scale = rows + 6 * N;
   if (g_ce_stride != 0 || g_kd_stride != 0) {
     launch_dep(head_scale_kernel, 1, 1024, 0, stream, r);
@@ -823,7 +928,8 @@ int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_s
 
   HeadLogits p{};
   p.N = h->N; p.V = h->V; p.C = h->C;
-  p.targets = h->targets; p.ids = h->ids; p.q = h->q; p.K = h->K; p.inv_tau = 1.0f / r.tau;
+  p.targets = h->targets; p.inv_tau = 1.0f / r.tau;
+  set_teacher(p, h);
   p.r_ce = r.r_ce; p.r_kd = r.r_kd;
   p.g = reinterpret_cast<__nv_bfloat16*>(base + at.g);
   p.ldg = pl.cols;
@@ -838,7 +944,7 @@ int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_s
   for (int i = 0; i < pl.pieces; ++i) {
     p.v0 = i * pl.cols;
     p.cols = h->V - p.v0 < pl.cols ? h->V - p.v0 : pl.cols;
-    if ((rc = launch_logits<true>(h->targets != nullptr, h->ids != nullptr, tx, tw, p, sms, stream)) != JB200_OK) return rc;
+    if ((rc = launch_logits<true>(h->targets != nullptr, h->teacher != nullptr, tx, tw, p, sms, stream)) != JB200_OK) return rc;
     rc = launch_head_products(p.g, pl.cols, p.cols, r.xs, h->w, h->N, h->V, h->C, p.v0, pl.slabs, i == 0, r.scale, slabs, dw, dw_dtype, sms, stream);
     if (rc != JB200_OK) return rc;
   }

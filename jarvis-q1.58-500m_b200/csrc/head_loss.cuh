@@ -8,7 +8,8 @@ constexpr int HEAD_TILE = 256, HEAD_BK = 64, HEAD_STAGES = 6;      // rows and c
 constexpr int HEAD_OPERAND = HEAD_TILE / 2 * HEAD_BK * 2;          // 16 KiB: one CTA's half of an operand's stage
 constexpr int HEAD_EPI_WARP0 = 2, HEAD_THREADS = 32 * (HEAD_EPI_WARP0 + 8);
 typedef PairRing<HEAD_STAGES> HeadRing;
-constexpr size_t HEAD_SMEM = 1024 + size_t(HEAD_STAGES) * 2 * HEAD_OPERAND + (sizeof(HeadRing) + 127) / 128 * 128;
+constexpr size_t HEAD_CTL = (sizeof(HeadRing) + 127) / 128 * 128;
+constexpr size_t HEAD_SMEM = 1024 + size_t(HEAD_STAGES) * 2 * HEAD_OPERAND + HEAD_CTL;
 static_assert(HEAD_SMEM <= 227 * 1024, "shared memory of one CTA");
 
 // How a backward pass is cut: `pieces` pieces of `cols` vocabulary columns (the last one shorter) whose gradients of the logits are

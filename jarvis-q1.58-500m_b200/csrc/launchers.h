@@ -161,8 +161,9 @@ int launch_step_cluster(const jb200_layer* layers, int n_layers, const jb200_for
 int launch_cross_entropy(const void* logits, int ld, int n_rows, int V, const int64_t* targets, float* row_loss,
                          const float* aux_a, int stride_a, const float* aux_b, int n_aux, float* loss, cudaStream_t stream);
 // The head's losses (head_loss.cu) and the norm's gradient (norm_grad.cu).
-int launch_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, int* ids_out,
-                        float* q_out, float* neg_entropy, cudaStream_t stream);
+size_t teacher_rows_bytes(int N, int K, int V);
+int launch_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, void* rows,
+                        cudaStream_t stream);
 size_t head_loss_scratch_bytes(int N, int V, int ce, int kd);
 int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* means, void* scratch, cudaStream_t stream);
 size_t head_loss_backward_scratch_bytes(int N, int V, int C);

@@ -75,7 +75,7 @@ __device__ __forceinline__ void st_global_256(void* p, const uint32_t* w) {
 
 // Control block of a persistent CTA pair whose operands both come by TMA: a ring of `STAGES` K-blocks and two accumulators.  The pair's
 // leader (cluster rank 0) issues every MMA; its `full` barriers count its own expectation and the bytes of both CTAs' loads, `empty`
-// and `acc_full` are committed to both CTAs, `acc_empty` counts the eight epilogue warps of each.
+// and `acc_full` are committed to both CTAs, `acc_empty` counts the epilogue warps of both that drain a tile.
 template <int STAGES>
 struct PairRing {
   uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
@@ -85,7 +85,7 @@ constexpr uint32_t PAIR_TMEM_COLS = 512;
 
 // Barriers and tensor memory (its address in ctl->tmem_base); all threads of both CTAs.
 template <int STAGES>
-__device__ __forceinline__ void pair_ring_init(PairRing<STAGES>* ctl, int warp) {
+__device__ __forceinline__ void pair_ring_init(PairRing<STAGES>* ctl, int warp, int drain_warps) {
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&ctl->full[s]), 1);
@@ -93,7 +93,7 @@ __device__ __forceinline__ void pair_ring_init(PairRing<STAGES>* ctl, int warp) 
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(smem_u32(&ctl->acc_full[a]), 1);
-      mbar_init(smem_u32(&ctl->acc_empty[a]), 16);
+      mbar_init(smem_u32(&ctl->acc_empty[a]), drain_warps);
     }
     ctl->abort_flag = 0;
     fence_mbar_init();

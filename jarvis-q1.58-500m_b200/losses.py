@@ -29,7 +29,7 @@ def _bf16(t: torch.Tensor, what: str) -> torch.Tensor:
         raise RuntimeError(f"{what}: expected a CUDA tensor (this path has no CPU fallback)")
     if t.dtype not in (torch.bfloat16, torch.float32):
         raise RuntimeError(f"{what}: expected float32 or bfloat16, got {t.dtype}")
-    return t.to(torch.bfloat16).contiguous()
+    return (t if t.dtype is torch.bfloat16 else t.to(torch.bfloat16)).contiguous()
 
 
 def _rows(t: torch.Tensor, lead, dtypes, what: str, columns: int | None = None) -> torch.Tensor:
@@ -42,60 +42,81 @@ def _rows(t: torch.Tensor, lead, dtypes, what: str, columns: int | None = None) 
     return t.reshape(-1) if columns is None else t.reshape(-1, columns).contiguous()
 
 
+def _forward(hidden, weight, targets, ids, logits, temperature, mean):
+    """The operators' common forward pass -> (bf16 rows, bf16 weight, targets, teacher, result, leading shape)."""
+    x, w = _bf16(hidden, "hidden"), _bf16(weight, "weight")
+    if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise RuntimeError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} must be (..., C) and (V, C)")
+    lead = x.shape[:-1]
+    if x.dim() != 2:
+        x = x.view(-1, w.shape[1])
+    teacher = None
+    if targets is not None:
+        targets = _rows(targets, lead, (torch.int64,), "targets").contiguous()
+    if ids is not None:
+        if ids.dim() < 1 or ids.shape[-1] < 1:
+            raise RuntimeError(f"teacher_ids: expected (..., K) with at least one entry a row, got {tuple(ids.shape)}")
+        ids = _rows(ids, lead, (torch.int64,), "teacher_ids", ids.shape[-1])
+        logits = _rows(logits, lead, (torch.float32, torch.bfloat16), "teacher_logits", ids.shape[1])
+        teacher = ops.teacher_rows(ids, logits, w.shape[0], temperature)
+    return x, w, targets, teacher, ops.head_loss(x, w, targets, teacher, want_means=mean), lead
+
+
+def _results(r, lead):
+    """(cross entropy, distillation), None where not asked for."""
+    if r.has_means:
+        return (r.buf[6 * r.N] if r.has_ce else None), (r.buf[6 * r.N + 2] if r.has_kd else None)
+    return (r.ce.view(lead) if r.has_ce else None), (r.kd.view(lead) if r.has_kd else None)
+
+
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, targets, ids, logits, temperature, reduction):
-        x, w = _bf16(hidden, "hidden"), _bf16(weight, "weight")
-        if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
-            raise RuntimeError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} must be (..., C) and (V, C)")
-        lead = x.shape[:-1]
-        x = x.view(-1, w.shape[1])
-        teacher = None
-        if targets is not None:
-            targets = _rows(targets, lead, (torch.int64,), "targets").contiguous()
-        if ids is not None:
-            if ids.dim() < 1 or ids.shape[-1] < 1:
-                raise RuntimeError(f"teacher_ids: expected (..., K) with at least one entry a row, got {tuple(ids.shape)}")
-            ids = _rows(ids, lead, (torch.int64,), "teacher_ids", ids.shape[-1])
-            logits = _rows(logits, lead, (torch.float32, torch.bfloat16), "teacher_logits", ids.shape[1])
-            teacher = ops.teacher_rows(ids, logits, w.shape[0], temperature)
-        r = ops.head_loss(x, w, targets, teacher, want_means=reduction == "mean")
-        ctx.save_for_backward(x, w, targets, r.ce, r.kd, r.means, r.lse, r.lse_t,
-                              *((teacher.ids, teacher.q, teacher.neg_entropy) if teacher is not None else (None, None, None)))
-        ctx.info = (hidden.shape, hidden.dtype, weight.dtype, None if teacher is None else (teacher.K, teacher.vocab, teacher.temperature))
-        ctx.mean = reduction == "mean"
-        if ctx.mean:
-            return (r.means[0] if targets is not None else None), (r.means[2] if teacher is not None else None)
-        return (r.ce.view(lead) if targets is not None else None), (r.kd.view(lead) if teacher is not None else None)
+    def forward(ctx, hidden, weight, targets, ids, logits, temperature, mean):
+        x, w, targets, teacher, r, lead = _forward(hidden, weight, targets, ids, logits, temperature, mean)
+        ctx.save_for_backward(x, w, targets, r.buf, None if teacher is None else teacher.buf)
+        ctx.info = (hidden.shape, hidden.dtype, weight.dtype, mean, None if teacher is None else (teacher.K, teacher.vocab, teacher.temperature))
+        return _results(r, lead)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_ce, g_kd):
-        x, w, targets, ce, kd, means, lse, lse_t, ids, q, neg_entropy = ctx.saved_tensors
-        shape, hidden_dtype, weight_dtype, info = ctx.info
-        teacher, fwd = None, ops.HeadLoss()
-        if info is not None:
-            teacher = ops.TeacherRows()
-            teacher.ids, teacher.q, teacher.neg_entropy = ids, q, neg_entropy
-            teacher.K, teacher.vocab, teacher.temperature = info
-        fwd.ce, fwd.kd, fwd.means, fwd.lse, fwd.lse_t = ce, kd, means, lse, lse_t
+        return _head_backward_once(ctx, g_ce, g_kd) if torch.is_grad_enabled() else _head_backward(ctx, g_ce, g_kd)
+
+
+def _head_backward(ctx, g_ce, g_kd):
+    x, w, targets, buf, teacher = ctx.saved_tensors
+    shape, dx_dtype, dw_dtype, mean, info = ctx.info
+    N = x.shape[0]
+    if teacher is not None:
+        teacher = ops.TeacherRows(teacher, N, *info)
+    if not mean:
         g_ce, g_kd = (None if g is None else g.reshape(-1).contiguous() for g in (g_ce, g_kd))
-        dx, dw = ops.head_loss_backward(x, w, fwd, targets, teacher, g_ce=g_ce, g_kd=g_kd, mean=ctx.mean, dx_dtype=hidden_dtype,
-                                        dw_dtype=weight_dtype, want_dx=ctx.needs_input_grad[0], want_dw=ctx.needs_input_grad[1])
-        return (None if dx is None else dx.view(shape)), dw, None, None, None, None, None
+    want_dx, want_dw = ctx.needs_input_grad[:2]
+    dx, dw = ops.head_loss_backward(x, w, ops.HeadLoss(buf, N, targets is not None, teacher is not None, mean), targets, teacher, g_ce=g_ce,
+                                    g_kd=g_kd, mean=mean, dx_dtype=dx_dtype, dw_dtype=dw_dtype, want_dx=want_dx, want_dw=want_dw)
+    if want_dx and len(shape) != 2:
+        dx = dx.view(shape)
+    return dx, dw, None, None, None, None, None
 
 
-def _reduction(reduction: str) -> str:
+# under create_graph: gradients that refuse to be differentiated (the wrapper's own cost is 10 us of a call)
+_head_backward_once = once_differentiable(_head_backward)
+
+
+def _head_loss(hidden, weight, targets, ids, logits, temperature, reduction):
     if reduction not in ("mean", "none"):
         raise RuntimeError(f"reduction must be 'mean' or 'none', got {reduction!r}")
-    return reduction
+    mean = reduction == "mean"
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _HeadLoss.apply(hidden, weight, targets, ids, logits, temperature, mean)
+    r, lead = _forward(hidden, weight, targets, ids, logits, temperature, mean)[4:]
+    return _results(r, lead)
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, reduction: str = "mean") -> torch.Tensor:
     """-log softmax(hidden @ weight.T)[targets], differentiable in hidden (..., C) and weight (V, C).  targets: int64 (...); -100 marks a row
     without one (loss 0, no part in any gradient), another value outside [0, V) makes its row NaN.  reduction: "mean" over the rows
     with a target (NaN when there is none) -> f32 scalar; "none" -> f32 (...).  C: a multiple of 8, at least 64."""
-    return _HeadLoss.apply(hidden, weight, targets, None, None, 1.0, _reduction(reduction))[0]
+    return _head_loss(hidden, weight, targets, None, None, 1.0, reduction)[0]
 
 
 def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
@@ -104,34 +125,41 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids:
     hidden and weight.  teacher_ids: int64 (..., K), teacher_logits: f32 or bf16 (..., K), K <= 256, in any order; a negative id is no
     entry, a row without entries has no part (loss 0), an id beyond the vocabulary makes its row NaN.  "mean": over the
     rows with entries."""
-    return _HeadLoss.apply(hidden, weight, None, teacher_ids, teacher_logits, temperature, _reduction(reduction))[1]
+    return _head_loss(hidden, weight, None, teacher_ids, teacher_logits, temperature, reduction)[1]
 
 
 def linear_losses(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, teacher_ids: torch.Tensor,
                   teacher_logits: torch.Tensor, *, temperature: float = 1.0, reduction: str = "mean"):
     """(linear_cross_entropy, linear_distillation) of the same rows: one pass forward, one pass backward whatever their weights are."""
-    return _HeadLoss.apply(hidden, weight, targets, teacher_ids, teacher_logits, temperature, _reduction(reduction))
+    return _head_loss(hidden, weight, targets, teacher_ids, teacher_logits, temperature, reduction)
 
 
 class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps, out_dtype):
-        x = x.contiguous()
-        w = weight.float().contiguous()
-        if w.shape != x.shape[-1:]:
-            raise RuntimeError(f"rms_norm: weight {tuple(weight.shape)} does not fit rows of {x.shape[-1]}")
+        x, w = x.contiguous(), weight.float().contiguous()
         ctx.save_for_backward(x, w)
         ctx.eps, ctx.weight_dtype = eps, weight.dtype
         return ops.rmsnorm(x, w, eps, out_dtype)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, w = ctx.saved_tensors
-        dx, dw = ops.rmsnorm_backward(x, w, dy.contiguous(), ctx.eps)
-        return dx, dw.to(ctx.weight_dtype), None, None
+        return _norm_backward_once(ctx, dy) if torch.is_grad_enabled() else _norm_backward(ctx, dy)
+
+
+def _norm_backward(ctx, dy):
+    x, w = ctx.saved_tensors
+    dx, dw = ops.rmsnorm_backward(x, w, dy.contiguous(), ctx.eps)
+    return dx, dw if ctx.weight_dtype is torch.float32 else dw.to(ctx.weight_dtype), None, None
+
+
+_norm_backward_once = once_differentiable(_norm_backward)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, out_dtype=torch.bfloat16) -> torch.Tensor:
     """RMSNorm.forward (jarvis_engine/jarvis_model.py:25-26) over the last axis, differentiable in x (f32 or bf16) and weight."""
-    return _RMSNorm.apply(x, weight, eps, out_dtype)
+    if weight.dim() != 1 or x.dim() < 1 or weight.shape[0] != x.shape[-1]:
+        raise RuntimeError(f"rms_norm: weight {tuple(weight.shape)} does not fit rows of {tuple(x.shape)}")
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _RMSNorm.apply(x, weight, eps, out_dtype)
+    return ops.rmsnorm(x.contiguous(), weight.float().contiguous(), eps, out_dtype)

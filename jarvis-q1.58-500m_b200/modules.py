@@ -776,7 +776,7 @@ class Jarvis(nn.Module):
         softmax as f32, forward's as bf16: the two agree as far as that rounding goes."""
         r = ops.head_loss(self.hidden_rows(idx, persist_state), self._lm_head_rows(),
                           ops._need(targets.reshape(-1).contiguous(), torch.int64, "loss.targets"))
-        aux, reflect = self._aux_terms(r.ce.device)
+        aux, reflect = self._aux_terms(r.buf.device)
         return r.means[0] + aux[:, 0].sum() + reflect.sum()
 
     def head_loss(self, idx, targets=None, teacher_ids=None, teacher_logits=None, *, temperature: float = 1.0):

@@ -579,8 +579,15 @@ def _launch(on: torch.Tensor, fn, *args) -> int:
 
 
 class TeacherRows:
-    """A teacher's rows as the head's loss reads them: what teacher_rows leaves."""
-    __slots__ = ("ids", "q", "neg_entropy", "K", "vocab", "temperature")
+    """A teacher's rows as the head's loss reads them, what teacher_rows leaves: the rows' `neg_entropy` f32 (N,), then their entries."""
+    __slots__ = ("buf", "N", "K", "vocab", "temperature")
+
+    def __init__(self, buf, N, K, vocab, temperature):
+        self.buf, self.N, self.K, self.vocab, self.temperature = buf, N, K, vocab, temperature
+
+    @property
+    def neg_entropy(self):
+        return self.buf[:4 * self.N].view(torch.float32)
 
 
 def teacher_rows(ids: torch.Tensor, logits: torch.Tensor, vocab: int, temperature: float = 1.0) -> TeacherRows:
@@ -589,51 +596,65 @@ def teacher_rows(ids: torch.Tensor, logits: torch.Tensor, vocab: int, temperatur
     row's loss NaN; an id that comes twice has both probabilities."""
     lib = _lib.load()
     _need(ids, torch.int64, "teacher_rows.ids")
-    _dt(logits)
+    dt = _dt(logits)
     _need(logits, logits.dtype, "teacher_rows.logits")
     if ids.dim() != 2 or logits.shape != ids.shape:
         raise RuntimeError(f"teacher_rows: ids {tuple(ids.shape)} and logits {tuple(logits.shape)} must be (N, K) alike")
     _together("teacher_rows", ids, logits)
     N, K = ids.shape
-    t = TeacherRows()
-    buf = torch.empty(2 * K * N + N, dtype=torch.float32, device=ids.device)
-    t.q, t.neg_entropy = buf[:K * N], buf[2 * K * N:]
-    t.ids = buf[K * N:2 * K * N].view(torch.int32)
-    t.K, t.vocab, t.temperature = K, int(vocab), float(temperature)
-    _lib.check(_launch(ids, lib.jb200_teacher_rows, _ptr(ids), _ptr(logits), _dt(logits), N, K, t.vocab, t.temperature, _ptr(t.ids),
-                       _ptr(t.q), _ptr(t.neg_entropy)), "jb200_teacher_rows")
+    t = TeacherRows(torch.empty(lib.jb200_teacher_rows_bytes(N, K, vocab), dtype=torch.uint8, device=ids.device), N, K, int(vocab),
+                    float(temperature))
+    _lib.check(_launch(ids, lib.jb200_teacher_rows, ids.data_ptr(), logits.data_ptr(), dt, N, K, t.vocab, t.temperature, t.buf.data_ptr()),
+               "jb200_teacher_rows")
     return t
 
 
 class HeadLoss:
-    """What head_loss leaves: ce / kd f32 (N,) (None where not asked for), means f32 (4,) [mean ce, rows with a target, mean kd, rows with a
-    teacher] or None, and lse / lse_t (2 N,), the softmaxes' sums for the backward call."""
-    __slots__ = ("ce", "kd", "means", "lse", "lse_t")
+    """What head_loss leaves: the rows' losses `ce` and `kd` (N,), `means` (4,) [mean ce, rows with a target, mean kd, rows with a teacher],
+    all f32 and None where not asked for, and the softmaxes' sums for the backward call."""
+    __slots__ = ("buf", "N", "has_ce", "has_kd", "has_means")       # buf: f32, ce, its sums (2 N), kd, its sums (2 N), means
+
+    def __init__(self, buf, N, has_ce, has_kd, has_means):
+        self.buf, self.N, self.has_ce, self.has_kd, self.has_means = buf, N, has_ce, has_kd, has_means
+
+    @property
+    def ce(self):
+        return self.buf[:self.N] if self.has_ce else None
+
+    @property
+    def kd(self):
+        return self.buf[3 * self.N:4 * self.N] if self.has_kd else None
+
+    @property
+    def means(self):
+        return self.buf[6 * self.N:] if self.has_means else None
 
 
 def _head(x, w, targets, teacher, what):
-    _need(x, torch.bfloat16, what + ".x")
-    _need(w, torch.bfloat16, what + ".w")
-    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+    _need(x, torch.bfloat16, what)
+    _need(w, torch.bfloat16, what)
+    (N, width), (V, columns) = x.shape, w.shape
+    if width != columns:
         raise RuntimeError(f"{what}: rows {tuple(x.shape)} and weight {tuple(w.shape)} must be (N, C) and (V, C)")
-    if targets is None and teacher is None:
-        raise RuntimeError(f"{what}: neither targets nor a teacher")
-    h = _lib.Head()
-    h.N, h.V, h.C = x.shape[0], w.shape[0], x.shape[1]
-    h.x, h.w = x.data_ptr(), w.data_ptr()
-    h.temperature = 1.0
+    dev = x.device
+    h = _lib.Head(N, V, width, x.data_ptr(), w.data_ptr())
     if targets is not None:
-        _need(targets, torch.int64, what + ".targets")
-        if targets.numel() != h.N:
-            raise RuntimeError(f"{what}: one target per row is needed, got {targets.numel()} for {h.N}")
+        _need(targets, torch.int64, what)
+        if targets.numel() != N:
+            raise RuntimeError(f"{what}: one target per row is needed, got {targets.numel()} for {N}")
         h.targets = targets.data_ptr()
+        if targets.device != dev:
+            raise RuntimeError(f"{what}: tensors on {dev} and {targets.device}")
+    elif teacher is None:
+        raise RuntimeError(f"{what}: neither targets nor a teacher")
     if teacher is not None:
-        if teacher.neg_entropy.numel() != h.N or teacher.vocab != h.V:
-            raise RuntimeError(f"{what}: the teacher's rows are {teacher.neg_entropy.numel()} over a vocabulary of {teacher.vocab}, "
-                               f"the loss has {h.N} over {h.V}")
-        h.K, h.ids, h.q, h.neg_entropy = teacher.K, teacher.ids.data_ptr(), teacher.q.data_ptr(), teacher.neg_entropy.data_ptr()
-        h.temperature = teacher.temperature
-    _together(what, x, w, targets, None if teacher is None else teacher.q)
+        if teacher.N != N or teacher.vocab != V:
+            raise RuntimeError(f"{what}: the teacher's rows are {teacher.N} over a vocabulary of {teacher.vocab}, the loss has {N} over {V}")
+        h.K, h.teacher, h.temperature = teacher.K, teacher.buf.data_ptr(), teacher.temperature
+        if teacher.buf.device != dev:
+            raise RuntimeError(f"{what}: tensors on {dev} and {teacher.buf.device}")
+    if w.device != dev:
+        raise RuntimeError(f"{what}: tensors on {dev} and {w.device}")
     return h
 
 
@@ -644,22 +665,23 @@ def head_loss(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor | None = N
     from `teacher`, or both.  x: bf16 (N, C); w: bf16 (V, C), any V (no padding needed), C a multiple of 8 and at least 64."""
     lib = _lib.load()
     h = _head(x, w, targets, teacher, "head_loss")
-    N = h.N
-    r = HeadLoss()
-    has_ce, has_kd = targets is not None, teacher is not None
-    buf = torch.empty(6 * N + 4, dtype=torch.float32, device=x.device)
-    at = buf.data_ptr()
-    r.ce, r.lse = (buf[:N], buf[N:3 * N]) if has_ce else (None, None)
-    r.kd, r.lse_t = (buf[3 * N:4 * N], buf[4 * N:6 * N]) if has_kd else (None, None)
-    r.means = buf[6 * N:] if want_means else None
-    if has_ce:
-        h.lse = at + 4 * N
-    if has_kd:
-        h.lse_t = at + 16 * N
-    scratch = torch.empty(lib.jb200_head_loss_scratch_bytes(N, h.V, has_ce, has_kd), dtype=torch.uint8, device=x.device)
-    _lib.check(_launch(x, lib.jb200_head_loss, ctypes.byref(h), at if has_ce else None, at + 12 * N if has_kd else None,
-                       at + 24 * N if want_means else None, _ptr(scratch)), "jb200_head_loss")
+    N, dev = h.N, x.device
+    r = HeadLoss(torch.empty(6 * N + 4, dtype=torch.float32, device=dev), N, targets is not None, teacher is not None, want_means)
+    at = r.buf.data_ptr()
+    h.lse, h.lse_t = at + 4 * N, at + 16 * N
+    scratch = torch.empty(lib.jb200_head_loss_scratch_bytes(N, h.V, r.has_ce, r.has_kd), dtype=torch.uint8, device=dev)
+    _lib.check(_launch(x, lib.jb200_head_loss, ctypes.byref(h), at, at + 12 * N, at + 24 * N if want_means else None, scratch.data_ptr()),
+               "jb200_head_loss")
     return r
+
+
+def _loss_gradient(g, count, what):
+    if g is None:
+        raise RuntimeError(f"head_loss_backward: {what} is needed")
+    _need(g, torch.float32, "head_loss_backward." + what)
+    if g.numel() != count:
+        raise RuntimeError(f"head_loss_backward: {what} must have {count} value{'s' * (count != 1)}, got {g.numel()}")
+    return g.data_ptr()
 
 
 def head_loss_backward(x: torch.Tensor, w: torch.Tensor, fwd: HeadLoss, targets: torch.Tensor | None = None,
@@ -669,38 +691,28 @@ def head_loss_backward(x: torch.Tensor, w: torch.Tensor, fwd: HeadLoss, targets:
     f32 scalars for the means of `fwd`; else f32 (N,) for the rows' losses.  One that is not wanted is not computed and None."""
     lib = _lib.load()
     h = _head(x, w, targets, teacher, "head_loss_backward")
-    n = [None, None]
-    for i, (g, rows, name) in enumerate(((g_ce, fwd.lse, "g_ce"), (g_kd, fwd.lse_t, "g_kd"))):
-        if (targets, teacher)[i] is None:
-            continue
-        if rows is None or rows.numel() != 2 * h.N:
-            raise RuntimeError("head_loss_backward: `fwd` is not the forward call's result for these rows")
-        if g is None:
-            raise RuntimeError(f"head_loss_backward: {name} is needed")
-        _need(g, torch.float32, "head_loss_backward." + name)
-        if g.numel() != (1 if mean else h.N):
-            raise RuntimeError(f"head_loss_backward: {name} must have {'one value' if mean else 'one value per row'}, got {g.numel()}")
-        if mean:
-            if fwd.means is None:
-                raise RuntimeError("head_loss_backward: the forward call left no means")
-            n[i] = fwd.means.data_ptr() + (4 if i == 0 else 12)
-    _together("head_loss_backward", x, g_ce, g_kd, fwd.lse, fwd.lse_t)
-    if targets is not None:
-        h.lse = fwd.lse.data_ptr()
-    if teacher is not None:
-        h.lse_t = fwd.lse_t.data_ptr()
-    codes = {torch.float32: 0, torch.bfloat16: 1}
-    if dx_dtype not in codes or dw_dtype not in codes:
-        raise RuntimeError("head_loss_backward: gradients are float32 or bfloat16")
-    dx = torch.empty(x.shape, dtype=dx_dtype, device=x.device) if want_dx else None
-    dw = torch.empty(w.shape, dtype=dw_dtype, device=x.device) if want_dw else None
+    N, dev = h.N, x.device
+    if fwd.N != N or fwd.has_ce != (targets is not None) or fwd.has_kd != (teacher is not None) or (mean and not fwd.has_means):
+        raise RuntimeError("head_loss_backward: `fwd` is not the forward call's result for these arguments")
+    at = fwd.buf.data_ptr()
+    h.lse, h.lse_t = at + 4 * N, at + 16 * N
+    pc = pk = nc = nk = None
+    if fwd.has_ce:
+        pc = _loss_gradient(g_ce, 1 if mean else N, "g_ce")
+        nc = at + 24 * N + 4 if mean else None
+    if fwd.has_kd:
+        pk = _loss_gradient(g_kd, 1 if mean else N, "g_kd")
+        nk = at + 24 * N + 12 if mean else None
+    _together("head_loss_backward", x, fwd.buf, g_ce, g_kd)
+    dx = torch.empty((N, h.C), dtype=dx_dtype, device=dev) if want_dx else None
+    dw = torch.empty((h.V, h.C), dtype=dw_dtype, device=dev) if want_dw else None
+    tx, tw = (1 if dx is None else _dt(dx)), (1 if dw is None else _dt(dw))
     stride = 0 if mean else 1
 
     def run(stream):
-        scratch = torch.empty(lib.jb200_head_loss_backward_scratch_bytes(h.N, h.V, h.C), dtype=torch.uint8, device=x.device)
-        return lib.jb200_head_loss_backward(ctypes.byref(h), _ptr(g_ce) if targets is not None else None, stride, n[0],
-                                            _ptr(g_kd) if teacher is not None else None, stride, n[1], _ptr(dx), codes[dx_dtype],
-                                            _ptr(dw), codes[dw_dtype], _ptr(scratch), stream)
+        scratch = torch.empty(lib.jb200_head_loss_backward_scratch_bytes(N, h.V, h.C), dtype=torch.uint8, device=dev)
+        return lib.jb200_head_loss_backward(ctypes.byref(h), pc, stride, nc, pk, stride, nk, _ptr(dx), tx, _ptr(dw), tw, scratch.data_ptr(),
+                                            stream)
     _lib.check(_launch(x, run), "jb200_head_loss_backward")
     return dx, dw
 
@@ -708,7 +720,7 @@ def head_loss_backward(x: torch.Tensor, w: torch.Tensor, fwd: HeadLoss, targets:
 def rmsnorm_backward(x: torch.Tensor, weight: torch.Tensor, dy: torch.Tensor, eps: float = 1e-6):
     """Gradients (dx of x's dtype, dweight f32) of rmsnorm for the output's gradient dy (f32 or bf16, x's shape)."""
     lib = _lib.load()
-    _dt(x), _dt(dy)
+    tx, ty = _dt(x), _dt(dy)
     _need(x, x.dtype, "rmsnorm_backward.x")
     _need(dy, dy.dtype, "rmsnorm_backward.dy")
     _need(weight, torch.float32, "rmsnorm_backward.weight")
@@ -722,8 +734,8 @@ def rmsnorm_backward(x: torch.Tensor, weight: torch.Tensor, dy: torch.Tensor, ep
 
     def run(stream):
         scratch = torch.empty(lib.jb200_rmsnorm_backward_scratch_bytes(rows, width), dtype=torch.uint8, device=x.device)
-        return lib.jb200_rmsnorm_backward(_ptr(x), _dt(x), _ptr(weight), eps, _ptr(dy), _dt(dy), rows, width, _ptr(dx), _ptr(dw),
-                                          _ptr(scratch), stream)
+        return lib.jb200_rmsnorm_backward(x.data_ptr(), tx, weight.data_ptr(), eps, dy.data_ptr(), ty, rows, width, dx.data_ptr(), dw.data_ptr(),
+                                          scratch.data_ptr(), stream)
     _lib.check(_launch(x, run), "jb200_rmsnorm_backward")
     return dx, dw
 

@@ -18,11 +18,11 @@ def _head(**kw):
 
 @pytest.mark.parametrize("kw,text", [(dict(C=60), "multiple of 8"), (dict(C=56), "at least 64"), (dict(V=0), "bad shape"), (dict(N=-1), "bad shape"),
                                      (dict(x=None), "null pointer"), (dict(x=4104), "16-byte"), (dict(targets=None), "neither targets nor a teacher"),
-                                     (dict(lse=None), "lse is needed"), (dict(ids=4096, K=0), "1 to 256 entries"),
-                                     (dict(ids=4096, K=257), "1 to 256 entries"), (dict(ids=4096, K=3), "null pointer"),
-                                     (dict(ids=4096, K=3, q=4096, neg_entropy=4096, lse_t=4096, temperature=0.0), "temperature"),
-                                     (dict(ids=4096, K=3, q=4096, neg_entropy=4096, lse_t=4096, temperature=float("nan")), "temperature"),
-                                     (dict(ids=4096, K=3, q=4096, neg_entropy=4096, lse_t=4096, temperature=1e-39), "temperature"),
+                                     (dict(lse=None), "lse is needed"), (dict(teacher=4096, K=0), "1 to 256 entries"),
+                                     (dict(teacher=4096, K=257), "1 to 256 entries"), (dict(teacher=4096, K=3), "null pointer"), (dict(teacher=4104, K=3, lse_t=4096), "16-byte"),
+                                     (dict(teacher=4096, K=3, lse_t=4096, temperature=0.0), "temperature"),
+                                     (dict(teacher=4096, K=3, lse_t=4096, temperature=float("nan")), "temperature"),
+                                     (dict(teacher=4096, K=3, lse_t=4096, temperature=1e-39), "temperature"),
                                      (dict(N=2**30, V=2**30), "too many logits")])
 def test_head_calls_refuse_bad_arguments(kw, text):
     lib = _lib.load()
@@ -44,10 +44,11 @@ def test_head_calls_refuse_missing_outputs():
         assert lib.jb200_head_loss_backward(C.byref(h), 4096, stride, None, None, 0, None, dx, dxt, dw, 1, scratch, None) == _lib.ERR_ARG
         assert text in _lib.last_error()
     assert lib.jb200_head_loss_backward(C.byref(h), None, 0, None, None, 0, None, 4096, 1, 4096, 1, 4096, None) == _lib.ERR_ARG
-    assert lib.jb200_teacher_rows(4096, 4096, 0, 4, 257, 100, 1.0, 4096, 4096, 4096, None) == _lib.ERR_ARG
-    assert lib.jb200_teacher_rows(4096, 4096, 3, 4, 2, 100, 1.0, 4096, 4096, 4096, None) == _lib.ERR_ARG
-    assert lib.jb200_teacher_rows(4096, 4096, 0, 4, 2, 100, -1.0, 4096, 4096, 4096, None) == _lib.ERR_ARG
-    assert lib.jb200_teacher_rows(None, 4096, 0, 4, 2, 100, 1.0, 4096, 4096, 4096, None) == _lib.ERR_ARG
+    assert lib.jb200_teacher_rows(4096, 4096, 0, 4, 257, 100, 1.0, 4096, None) == _lib.ERR_ARG
+    assert lib.jb200_teacher_rows(4096, 4096, 3, 4, 2, 100, 1.0, 4096, None) == _lib.ERR_ARG
+    assert lib.jb200_teacher_rows(4096, 4096, 0, 4, 2, 100, -1.0, 4096, None) == _lib.ERR_ARG
+    assert lib.jb200_teacher_rows(4096, 4096, 0, 4, 2, 100, 1.0, 4100, None) == _lib.ERR_ARG
+    assert lib.jb200_teacher_rows(None, 4096, 0, 4, 2, 100, 1.0, 4096, None) == _lib.ERR_ARG
     for width, text in ((60, "multiple of 8"), (4104, "at most 4096"), (0, "bad shape")):
         assert lib.jb200_rmsnorm_backward(4096, 0, 4096, 1e-6, 4096, 0, 4, width, 4096, 4096, 4096, None) == _lib.ERR_ARG
         assert text in _lib.last_error()
