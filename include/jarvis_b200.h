@@ -435,6 +435,9 @@ int jb200_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_st
                              const float* n_kd, void* dx, int dx_dtype, void* dw, int dw_dtype, void* scratch, void* stream);
 /* How such a pass is cut on a device with `sms` SMs: columns of a piece, pieces, slabs of dx. */
 int jb200_host_head_plan(int N, int V, int C, int sms, int32_t* out3);
+/* The i-th item of a pair of its products' launch, which has long items (k_long K-blocks) and short ones: a long one's index, n_long +
+ * a short one's, -1 behind the last. */
+int jb200_host_head_walk(int n_long, int k_long, int n_short, int k_short, int pairs, int pair, int i);
 
 /* Gradient of jb200_rmsnorm: dx (x's dtype) and dw f32 [C], both overwritten; statistics are formed anew from x.  C a multiple of 8, at
  * most 4096.  dw is summed in f32 in a fixed order. */

@@ -90,6 +90,7 @@ PROTOTYPES = {
     "jb200_head_loss": (_I, [C.POINTER(Head), _P, _P, _P, _P, _P]),
     "jb200_head_loss_backward_scratch_bytes": (_Z, [_I] * 3),
     "jb200_head_loss_backward": (_I, [C.POINTER(Head), _P, _I, _P, _P, _I, _P, _P, _I, _P, _I, _P, _P]),
+    "jb200_host_head_walk": (_I, [_I] * 7),
     "jb200_host_head_plan": (_I, [_I] * 4 + [C.POINTER(C.c_int32)]),
     "jb200_rmsnorm_backward_scratch_bytes": (_Z, [_I] * 2),
     "jb200_rmsnorm_backward": (_I, [_P, _I, _P, _F, _P, _I, _I, _I, _P, _P, _P, _P]),

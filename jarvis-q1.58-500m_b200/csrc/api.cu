@@ -483,6 +483,9 @@ int jb200_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_st
                                    static_cast<cudaStream_t>(stream));
 }
 int jb200_host_head_plan(int N, int V, int C, int sms, int32_t* out3) { return head_plan_host(N, V, C, sms, out3); }
+int jb200_host_head_walk(int n_long, int k_long, int n_short, int k_short, int pairs, int pair, int i) {
+  return head_walk_host(n_long, k_long, n_short, k_short, pairs, pair, i);
+}
 size_t jb200_rmsnorm_backward_scratch_bytes(int n_rows, int C) { return rmsnorm_backward_scratch_bytes(n_rows, C); }
 int jb200_rmsnorm_backward(const void* x, int x_dtype, const float* w, float eps, const void* dy, int dy_dtype, int n_rows, int C, void* dx,
                            float* dw, void* scratch, void* stream) {

@@ -19,7 +19,8 @@ struct HeadProducts {
   int first;                 // dx slabs are stored; else added to
   int width;                 // columns of a tile: 256, or 128 where there are no more
   int dx_items, dw_items;
-  int dw_first;
+  int dw_first;              // dW's items are the long ones
+  HeadShares shares;
   const float* scale;        // [1]
   float* dx;                 // [slabs][N][C]
   void* dw;                  // [V][C]
@@ -34,27 +35,29 @@ struct Item {
   int slab;
 };
 
-__device__ __forceinline__ Item head_item(const HeadProducts& p, int t) {
-  Item it;
-  const int tc = (p.C + p.width - 1) / p.width;
-  it.is_dw = p.dw_first ? t < p.dw_items : t >= p.dx_items;
-  int i = it.is_dw ? (p.dw_first ? t : t - p.dx_items) : (p.dw_first ? t - p.dw_items : t);
-  const int n = i % tc;
-  i /= tc;
-  it.n0 = n * p.width;
-  if (it.is_dw) {
-    it.m0 = i * HEAD_TILE;
-    it.kb0 = 0;
-    it.kb1 = (p.N + HEAD_BK - 1) / HEAD_BK;
-    it.slab = 0;
+// The i-th item of a pair; false behind its last.
+__device__ __forceinline__ bool head_item(const HeadProducts& p, int pair, int n_pairs, int i, Item* it) {
+  const int n_long = p.dw_first ? p.dw_items : p.dx_items, n_short = p.dw_first ? p.dx_items : p.dw_items;
+  int t = head_walk(p.shares, n_long, n_short, pair, n_pairs, i);
+  if (t < 0) return false;
+  it->is_dw = (t < n_long) == (p.dw_first != 0);
+  if (t >= n_long) t -= n_long;
+  const int tc = (p.C + p.width - 1) / p.width, n = t % tc;
+  t /= tc;
+  it->n0 = n * p.width;
+  if (it->is_dw) {
+    it->m0 = t * HEAD_TILE;
+    it->kb0 = 0;
+    it->kb1 = (p.N + HEAD_BK - 1) / HEAD_BK;
+    it->slab = 0;
   } else {
     const int tm = (p.N + HEAD_TILE - 1) / HEAD_TILE, kb = (p.n_cols + HEAD_BK - 1) / HEAD_BK;
-    it.slab = i / tm;
-    it.m0 = (i - it.slab * tm) * HEAD_TILE;
-    it.kb0 = int((long long)(kb) * it.slab / p.slabs);
-    it.kb1 = int((long long)(kb) * (it.slab + 1) / p.slabs);
+    it->slab = t / tm;
+    it->m0 = (t - it->slab * tm) * HEAD_TILE;
+    it->kb0 = int((long long)(kb) * it->slab / p.slabs);
+    it->kb1 = int((long long)(kb) * (it->slab + 1) / p.slabs);
   }
-  return it;
+  return true;
 }
 
 // 32 (or, at the edge, a multiple of 8) consecutive channels of a row.
@@ -108,7 +111,8 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
   pdl_trigger();
   const uint32_t tmem = ctl->tmem_base;
   volatile uint32_t* abort_flag = &ctl->abort_flag;
-  const int pair = int(blockIdx.x >> 1), n_pairs = int(gridDim.x >> 1), total = p.dx_items + p.dw_items;
+  const int pair = int(blockIdx.x >> 1), n_pairs = int(gridDim.x >> 1);
+  Item it;
   constexpr uint32_t BOX = HEAD_BK * HEAD_BK * 2;              // 8 KiB: [64 rows][64 columns]
   const int half_width = p.width / 2;                          // columns that this CTA loads for the pair
 
@@ -117,8 +121,7 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
     int s = 0;
     uint32_t ph = 1u;
     bool ok = true;
-    for (int t = pair; ok && t < total; t += n_pairs) {
-      const Item it = head_item(p, t);
+    for (int i = 0; ok && head_item(p, pair, n_pairs, i, &it); ++i) {
       const int row = it.m0 + rank * (HEAD_TILE / 2), col = it.n0 + rank * half_width;
       const uint32_t bytes = 2u * (uint32_t(HEAD_OPERAND) + uint32_t(half_width) * HEAD_BK * 2);     // of both CTAs
 #pragma unroll 1
@@ -153,8 +156,7 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
       int s = 0;
       uint32_t ph = 0u, tile = 0u;
       bool ok = true;
-      for (int t = pair; ok && t < total; t += n_pairs, ++tile) {
-        const Item it = head_item(p, t);
+      for (; ok && head_item(p, pair, n_pairs, int(tile), &it); ++tile) {
         const uint64_t ad0 = it.is_dw ? a_mn : a_k;
         const uint32_t a_step = it.is_dw ? 128u : 2u, id = it.is_dw ? idesc + IDESC_A_MN : idesc;
         const uint32_t acc = tile & 1u;
@@ -183,8 +185,7 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
     const int quarter = warp & 3, half = (warp - HEAD_EPI_WARP0) >> 2;
     const float scale = *p.scale;
     uint32_t tile = 0u;
-    for (int t = pair; t < total; t += n_pairs, ++tile) {
-      const Item it = head_item(p, t);
+    for (; head_item(p, pair, n_pairs, int(tile), &it); ++tile) {
       const uint32_t acc = tile & 1u;
       const int row = it.m0 + rank * (HEAD_TILE / 2) + quarter * 32 + lane;
       const bool on = row < (it.is_dw ? p.n_cols : p.N);
@@ -231,7 +232,8 @@ int launch_head_products(const void* g, int cols, int n_cols, const void* xs, co
   const int tc = (C + p.width - 1) / p.width, tm = (N + HEAD_TILE - 1) / HEAD_TILE;
   p.dx_items = dx_slabs ? p.slabs * tm * tc : 0;
   p.dw_items = dw ? (n_cols + HEAD_TILE - 1) / HEAD_TILE * tc : 0;
-  p.dw_first = kn > kb / p.slabs ? 1 : 0;
+  const int k_dx = (kb + p.slabs - 1) / p.slabs;
+  p.dw_first = kn > k_dx ? 1 : 0;
   p.scale = scale; p.dx = dx_slabs; p.dw = dw; p.dw_bf16 = dw_dtype;
   p.status = device_status_ptr();
   if (!p.status) return JB200_ERR_CUDA;
@@ -240,9 +242,10 @@ int launch_head_products(const void* g, int cols, int n_cols, const void* xs, co
   if ((rc = encode_head_map(&tg, g, cols, N, HEAD_BK, "head_loss_backward (gradient of the logits)")) != JB200_OK) return rc;
   if ((rc = encode_head_map(&tw, w, C, V, HEAD_BK, "head_loss_backward (weight)")) != JB200_OK) return rc;
   if ((rc = encode_head_map(&tx, xs, C, N, HEAD_BK, "head_loss_backward (rows)")) != JB200_OK) return rc;
-  const int pairs = sms / 2, items = p.dx_items + p.dw_items;
+  const int items = p.dx_items + p.dw_items, pairs = items < sms / 2 ? items : sms / 2;
+  p.shares = p.dw_first ? head_shares(p.dw_items, kn, p.dx_items, k_dx, pairs) : head_shares(p.dx_items, k_dx, p.dw_items, kn, pairs);
   JB_MAX_SMEM(head_products_kernel, HEAD_SMEM);
-  launch_dep_cluster(head_products_kernel, dim3(2 * unsigned(items < pairs ? items : pairs)), dim3(HEAD_THREADS), HEAD_SMEM, 2, stream, tg, tw,
+  launch_dep_cluster(head_products_kernel, dim3(2 * unsigned(pairs)), dim3(HEAD_THREADS), HEAD_SMEM, 2, stream, tg, tw,
                      tx, p);
   JB_LAUNCH_CHECK("head_products_kernel");
   return JB200_OK;

@@ -28,7 +28,7 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int TEACHER_MAX = 256;
-constexpr size_t PIECE_BYTES = size_t(256) << 20;      // bf16 gradients of the logits kept at a time
+constexpr size_t PIECE_BYTES = size_t(320) << 20;      // bf16 gradients of the logits kept at a time, at most
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -759,23 +759,74 @@ int encode_head_map(CUtensorMap* tm, const void* ptr, long long cols, long long 
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, what);
 }
 
+HeadShares head_shares(int n_long, int k_long, int n_short, int k_short, int pairs) {
+  HeadShares best{};
+  best.span = LLONG_MAX;
+  const int turns = n_long / pairs, uneven = n_long % pairs, rest = pairs - uneven;
+  for (int up = 0; up < 2; ++up) {
+    const int more = uneven == 0 ? 0 : k_long / k_short + up;
+    const long long left = n_short - (long long)rest * more;
+    const int rounds = left > 0 ? int((left + pairs - 1) / pairs) : 0;
+    const long long a = uneven ? (long long)(turns + 1) * k_long + (long long)rounds * k_short : 0;
+    // (where the others alone have more than there are, they share those)
+    const long long take = left > 0 ? rounds + more : (n_short + rest - 1) / rest;
+    const long long b = (long long)turns * k_long + take * k_short;
+    const long long span = a > b ? a : b;
+    if (span < best.span) best = {uneven, rounds, more, span};
+  }
+  return best;
+}
+
+namespace {
+// K-blocks' time of an item of k of them: its epilogue hides behind the next item's products, but not below some eight.
+int item_time(int k) { return k > 8 ? k : 8; }
+
+// Time of a piece of n tiles in K-blocks of a pair (512 cycles), and of what follows from its slabs.
+long long piece_time(long long n, int N, int C, int slabs, int pairs) {
+  const int tm = (N + HEAD_TILE - 1) / HEAD_TILE, tc = (C + HEAD_TILE - 1) / HEAD_TILE, kc = (C + HEAD_BK - 1) / HEAD_BK;
+  const int k_dw = item_time((N + HEAD_BK - 1) / HEAD_BK), k_dx = item_time(int((n * (HEAD_TILE / HEAD_BK) + slabs - 1) / slabs));
+  const int n_dw = int(n) * tc, n_dx = slabs * tm * tc;
+  const HeadShares s = k_dw > k_dx ? head_shares(n_dw, k_dw, n_dx, k_dx, pairs) : head_shares(n_dx, k_dx, n_dw, k_dw, pairs);
+  return (tm * n + pairs - 1) / pairs * item_time(kc) + s.span + 24;      // 24: two launches
+}
+}  // namespace
+
+// The fastest of some cuts by that count.  Candidates: the fewest pieces that the workspace allows and a few more, even ones, and those
+// whose tiles fill the pairs without a rest.  (16384 x 50257 x 1024: seven even pieces of 29 tiles, 512 K-blocks of one kind and 464 of
+// the other on the busiest pair where the mean is 802, took 5.4 ms; pieces of 37, all pairs busy to 1 %, see below.)
 HeadPlan head_plan(int N, int V, int C, int pairs) {
-  HeadPlan pl;
-  const long long tv = (V + HEAD_TILE - 1) / HEAD_TILE, tm = (N + HEAD_TILE - 1) / HEAD_TILE, tc = (C + HEAD_TILE - 1) / HEAD_TILE;
+  struct Kept { int N, V, C, pairs; HeadPlan plan; };
+  thread_local Kept kept{};
+  if (kept.N == N && kept.V == V && kept.C == C && kept.pairs == pairs) return kept.plan;
+  const long long tv = (V + HEAD_TILE - 1) / HEAD_TILE, tm = (N + HEAD_TILE - 1) / HEAD_TILE;
   long long most = (long long)(PIECE_BYTES / (size_t(N > 0 ? N : 1) * HEAD_TILE * 2));
-  if (most < 1) most = 1;
-  pl.pieces = int((tv + most - 1) / most);
-  const long long per = (tv + pl.pieces - 1) / pl.pieces;      // tiles of a piece
-  pl.pieces = int((tv + per - 1) / per);
-  pl.cols = int(per) * HEAD_TILE;
-  // dx: tm * tc items of per * 4 K-blocks, beside per * tc items of dW.  Few of them would outlast the others: cut.
-  const long long kb = per * (HEAD_TILE / HEAD_BK), work = tm * tc * kb + per * tc * ((N + HEAD_BK - 1) / HEAD_BK);
-  const long long share = (work + pairs - 1) / pairs;          // K-blocks of a pair, were all alike
-  long long s = (kb + share - 1) / (share > 0 ? share : 1);
-  if (s > kb / 8) s = kb / 8;                                  // at least eight K-blocks each
-  if (s > 64) s = 64;
-  pl.slabs = int(s < 1 ? 1 : s);
-  return pl;
+  most = most < 1 ? 1 : most > tv ? tv : most;
+  long long cand[12];
+  int n_cand = 0;
+  const long long fewest = (tv + most - 1) / most;
+  for (int i = 0; i < 6 && fewest + i <= tv; ++i) cand[n_cand++] = (tv + fewest + i - 1) / (fewest + i);
+  long long step = pairs;                                      // smallest number of tiles whose row tiles fill the pairs
+  for (long long a = pairs, b = tm; b; ) { const long long r = a % b; a = b; b = r; step = pairs / a; }
+  for (int i = 0; i < 4; ++i) {
+    const long long n = (most / step - i) * step;
+    if (n > 0) cand[n_cand++] = n;
+  }
+  HeadPlan best{};
+  long long best_time = LLONG_MAX;
+  for (int i = 0; i < n_cand; ++i) {
+    const long long per = cand[i], pieces = (tv + per - 1) / per, last = tv - (pieces - 1) * per;
+    for (int slabs = 1; slabs <= 64; slabs += slabs < 4 ? 1 : slabs / 4) {
+      if (slabs > 1 && per * (HEAD_TILE / HEAD_BK) / slabs < 8) break;      // at least eight K-blocks each
+      const long long reduce = (long long)slabs * N * C / 400000;           // 4 bytes read at 6 TB/s
+      const long long time = (pieces - 1) * piece_time(per, N, C, slabs, pairs) + piece_time(last, N, C, slabs, pairs) + reduce;
+      if (time < best_time) {
+        best_time = time;
+        best = {int(per) * HEAD_TILE, int(pieces), slabs};
+      }
+    }
+  }
+  kept = {N, V, C, pairs, best};
+  return best;
 }
 
 size_t teacher_rows_bytes(int N, int K, int V) { return N < 1 || K < 1 || V < 1 ? 0 : teacher_layout(N, K, V).total; }
@@ -961,6 +1012,11 @@ int head_plan_host(int N, int V, int C, int sms, int32_t* out3) {
   const HeadPlan pl = head_plan(N, V, C, sms / 2);
   out3[0] = pl.cols; out3[1] = pl.pieces; out3[2] = pl.slabs;
   return JB200_OK;
+}
+
+int head_walk_host(int n_long, int k_long, int n_short, int k_short, int pairs, int pair, int i) {
+  if (n_long < 0 || n_short < 0 || k_long < 1 || k_short < 1 || pairs < 1 || pair < 0 || pair >= pairs || i < 0) return JB200_ERR_ARG;
+  return head_walk(head_shares(n_long, k_long, n_short, k_short, pairs), n_long, n_short, pair, pairs, i);
 }
 
 }  // namespace jb

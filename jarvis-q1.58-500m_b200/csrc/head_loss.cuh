@@ -19,6 +19,28 @@ struct HeadPlan {
 };
 HeadPlan head_plan(int N, int V, int C, int pairs);
 
+// The items of a products launch on its pairs: the long ones first, one a pair in turn, then the short ones, of which the pairs that
+// got fewer long ones take `more` more each.
+struct HeadShares {
+  int uneven;                // pairs [0, uneven) have one long item more than the others
+  int rounds, more;          // short items of those pairs; the others have rounds + more
+  long long span;            // K-blocks of the busiest pair
+};
+HeadShares head_shares(int n_long, int k_long, int n_short, int k_short, int pairs);
+
+// The i-th item of a pair: a long one below n_long, n_long + a short one from there on, -1 behind the pair's last.
+__host__ __device__ __forceinline__ int head_walk(const HeadShares& s, int n_long, int n_short, int pair, int pairs, int i) {
+  const bool uneven = pair < s.uneven;
+  const int turns = n_long / pairs + (uneven ? 1 : 0), r = i - turns;
+  if (r < 0) return pair + i * pairs;
+  int t = pair + r * pairs;
+  if (r >= s.rounds) {
+    if (uneven || r >= s.rounds + s.more) return -1;
+    t = s.rounds * pairs + (r - s.rounds) * (pairs - s.uneven) + pair - s.uneven;
+  }
+  return t < n_short ? n_long + t : -1;
+}
+
 int encode_head_map(CUtensorMap* tm, const void* ptr, long long cols, long long rows, int box_rows, const char* what);
 
 // dx slabs += G W and dW = G^T xs of one piece (head_grad.cu); a null one is not wanted.  g: bf16 [N][cols]; piece columns [0, n_cols) are vocabulary rows

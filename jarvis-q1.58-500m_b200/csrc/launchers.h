@@ -170,6 +170,7 @@ size_t head_loss_backward_scratch_bytes(int N, int V, int C);
 int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_stride, const float* n_ce, const float* g_kd, int g_kd_stride,
                               const float* n_kd, void* dx, int dx_dtype, void* dw, int dw_dtype, void* scratch, cudaStream_t stream);
 int head_plan_host(int N, int V, int C, int sms, int32_t* out3);
+int head_walk_host(int n_long, int k_long, int n_short, int k_short, int pairs, int pair, int i);
 size_t rmsnorm_backward_scratch_bytes(int n_rows, int C);
 int launch_rmsnorm_backward(const void* x, int x_dtype, const float* w, float eps, const void* dy, int dy_dtype, int n_rows, int C, void* dx,
                             float* dw, void* scratch, cudaStream_t stream);

@@ -80,7 +80,26 @@ def test_backward_passes_are_cut_into_pieces_that_cover_the_vocabulary(sms):
                 assert lib.jb200_host_head_plan(N, V, width, sms, out) == 0
                 cols, pieces, slabs = out
                 assert cols % 256 == 0 and (pieces - 1) * cols < V <= pieces * cols
-                assert cols == 256 or N * cols * 2 <= 256 << 20        # the workspace is bounded, down to one tile of columns
+                assert cols == 256 or N * cols * 2 <= 320 << 20        # the workspace is bounded, down to one tile of columns
                 # every slab of the first piece has K-blocks of 64 columns to sum
                 assert 1 <= slabs <= 64 and slabs <= (min(V, cols) + 63) // 64
     assert lib.jb200_host_head_plan(0, 5, 64, 148, out) == _lib.ERR_ARG
+
+
+@pytest.mark.parametrize("n_long,k_long,n_short,k_short,pairs", [(148, 256, 512, 74, 74), (116, 256, 256, 116, 74), (788, 32, 64, 394, 74), (4, 786, 788, 1, 74),
+                                                                 (0, 5, 10, 3, 10), (7, 9, 0, 2, 7), (3, 100, 2, 1, 5), (75, 10, 1, 9, 74),
+                                                                 (10, 1000, 500, 1, 7), (1, 1, 1, 1, 2), (13, 8, 100, 8, 13)])
+def test_every_item_of_the_gradients_products_is_done_once(n_long, k_long, n_short, k_short, pairs):
+    lib = _lib.load()
+    seen, busiest = [], 0
+    for pair in range(pairs):
+        i = load = 0
+        while (t := lib.jb200_host_head_walk(n_long, k_long, n_short, k_short, pairs, pair, i)) >= 0:
+            seen.append(t)
+            load += k_long if t < n_long else k_short
+            i += 1
+        assert t == -1 and lib.jb200_host_head_walk(n_long, k_long, n_short, k_short, pairs, pair, i + 1) == -1
+        busiest = max(busiest, load)
+    assert sorted(seen) == list(range(n_long + n_short))
+    # no pair has more than its even share, rounded up by an item of each kind
+    assert busiest <= (n_long * k_long + n_short * k_short) / pairs + k_long + k_short
