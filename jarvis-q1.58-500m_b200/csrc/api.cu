@@ -105,8 +105,14 @@ int encode_tiled(CUtensorMap* tm, CUtensorMapDataType dt, int rank, const void* 
       return JB200_ERR_CUDA;
     }
     const cuuint32_t estr[3] = {1, 1, 1};
-    const CUresult cr = fn(&e.map, dt, cuuint32_t(rank), const_cast<void*>(ptr), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CUresult cr = CUDA_ERROR_INVALID_CONTEXT;
+    for (int tries = 0; cr == CUDA_ERROR_INVALID_CONTEXT && tries < 2; ++tries) {
+      // a thread that has made no runtime call yet (autograd's) has no context: cudaSetDevice binds the device's own
+      int dev = 0;
+      if (tries == 1 && (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess)) break;
+      cr = fn(&e.map, dt, cuuint32_t(rank), const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    }
     if (cr != CUDA_SUCCESS) {
       memset(&e.key, 0, sizeof(e.key));
       set_error("%s: cuTensorMapEncodeTiled failed (%d)", what, int(cr));

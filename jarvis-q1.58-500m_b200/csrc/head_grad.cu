@@ -4,29 +4,14 @@
 // CTA pairs as in the logits' kernel: 256 x 256 tiles, K-blocks of 64.  No operand is transposed in memory: G is the M operand K-major
 // for dx (rows x vocabulary) and MN-major for dW (read as vocabulary x rows), W and xs are the N operands MN-major, all from the
 // same kind of [64 rows][64 columns] boxes.  Both products are items of one list, the longer kind first, so that their last waves
-// fill each other's gaps.
+// fill each other's gaps.  Where there are few rows dx is summed over parts of the piece side by side, in slabs of their own, which a
+// launch of its own adds up in their order (done by the warps that store a tile last it took 30 us of 37 rows instead of 5).
 #include "head_loss.cuh"
 #include "launchers.h"
 
 namespace jb {
 
 namespace {
-
-struct HeadProducts {
-  int N, V, C;
-  int v0, n_cols;            // the piece's vocabulary rows
-  int slabs;
-  int first;                 // dx slabs are stored; else added to
-  int width;                 // columns of a tile: 256, or 128 where there are no more
-  int dx_items, dw_items;
-  int dw_first;              // dW's items are the long ones
-  HeadShares shares;
-  const float* scale;        // [1]
-  float* dx;                 // [slabs][N][C]
-  void* dw;                  // [V][C]
-  int dw_bf16;
-  unsigned int* status;
-};
 
 struct Item {
   bool is_dw;
@@ -77,6 +62,17 @@ __device__ __forceinline__ void store_f32(float* d, const uint32_t (&v)[32], int
     }
   }
 }
+__device__ __forceinline__ void add_f32(uint32_t (&v)[32], const float* d, int n) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (4 * j < n) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(d) + j);
+      v[4 * j] = __float_as_uint(x.x + __uint_as_float(v[4 * j]));
+      v[4 * j + 1] = __float_as_uint(x.y + __uint_as_float(v[4 * j + 1]));
+      v[4 * j + 2] = __float_as_uint(x.z + __uint_as_float(v[4 * j + 2]));
+      v[4 * j + 3] = __float_as_uint(x.w + __uint_as_float(v[4 * j + 3]));
+    }
+}
 __device__ __forceinline__ void store_bf16(__nv_bfloat16* d, const uint32_t (&v)[32], int n, bool wide) {
   uint32_t w[16];
 #pragma unroll
@@ -114,7 +110,7 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
   const int pair = int(blockIdx.x >> 1), n_pairs = int(gridDim.x >> 1);
   Item it;
   constexpr uint32_t BOX = HEAD_BK * HEAD_BK * 2;              // 8 KiB: [64 rows][64 columns]
-  const int half_width = p.width / 2;                          // columns that this CTA loads for the pair
+  const int half_width = p.width / 2, boxes = (half_width + HEAD_BK - 1) / HEAD_BK;      // columns of the pair's tile from this CTA
 
   if (warp == 0) {
     // ---------------- TMA ----------------
@@ -123,7 +119,7 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
     bool ok = true;
     for (int i = 0; ok && head_item(p, pair, n_pairs, i, &it); ++i) {
       const int row = it.m0 + rank * (HEAD_TILE / 2), col = it.n0 + rank * half_width;
-      const uint32_t bytes = 2u * (uint32_t(HEAD_OPERAND) + uint32_t(half_width) * HEAD_BK * 2);     // of both CTAs
+      const uint32_t bytes = 2u * (uint32_t(HEAD_OPERAND) + uint32_t(boxes) * BOX);     // of both CTAs
 #pragma unroll 1
       for (int kb = it.kb0; kb < it.kb1; ++kb) {
         if (!mbar_wait(smem_u32(&ctl->empty[s]), ph, abort_flag, p.status, JB200_STATUS_HEAD_LOAD)) { ok = false; break; }
@@ -135,12 +131,11 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
           if (it.is_dw) {
             pair_tma_load_2d(a, &tmap_g, row, k, full);
             pair_tma_load_2d(a + BOX, &tmap_g, row + HEAD_BK, k, full);
-            for (int c = 0; c < half_width; c += HEAD_BK) pair_tma_load_2d(b + uint32_t(c / HEAD_BK) * BOX, &tmap_x, col + c, k, full);
+            for (int c = 0; c < boxes; ++c) pair_tma_load_2d(b + uint32_t(c) * BOX, &tmap_x, col + c * HEAD_BK, k, full);
           } else {
             pair_tma_load_2d(a, &tmap_g, k, row, full);
             pair_tma_load_2d(a + BOX, &tmap_g, k, row + HEAD_BK, full);
-            for (int c = 0; c < half_width; c += HEAD_BK)
-              pair_tma_load_2d(b + uint32_t(c / HEAD_BK) * BOX, &tmap_w, col + c, p.v0 + k, full);
+            for (int c = 0; c < boxes; ++c) pair_tma_load_2d(b + uint32_t(c) * BOX, &tmap_w, col + c * HEAD_BK, p.v0 + k, full);
           }
         }
         __syncwarp();
@@ -183,7 +178,7 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
   } else {
     // ---------------- epilogue: a lane is a row, its registers are channels ----------------
     const int quarter = warp & 3, half = (warp - HEAD_EPI_WARP0) >> 2;
-    const float scale = *p.scale;
+    const float scale = head_scale(p.grads);
     uint32_t tile = 0u;
     for (; head_item(p, pair, n_pairs, int(tile), &it); ++tile) {
       const uint32_t acc = tile & 1u;
@@ -204,7 +199,14 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
           for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(scale * __uint_as_float(v[j]));
           const int n = min(32, p.C - col);
           if (!it.is_dw) {
-            store_f32(p.dx + (size_t(it.slab) * p.N + row) * p.C + col, v, n, p.first == 0);
+            const size_t o = size_t(row) * p.C + col;
+            if (p.last && p.all_slabs == 1 && p.dx_bf16) {
+              // the only slab: its sum so far and this piece's, rounded from here
+              if (!p.first) add_f32(v, p.dx_slabs + o, n);
+              store_bf16(static_cast<__nv_bfloat16*>(p.dx) + o, v, n, p.C % 16 == 0);
+            } else {
+              store_f32(p.dx_slabs + size_t(it.slab) * p.N * p.C + o, v, n, p.first == 0);
+            }
           } else if (p.dw_bf16) {
             store_bf16(static_cast<__nv_bfloat16*>(p.dw) + (size_t(p.v0) + row) * p.C + col, v, n, p.C % 16 == 0);
           } else {
@@ -222,32 +224,63 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
 
 }  // namespace
 
-int launch_head_products(const void* g, int cols, int n_cols, const void* xs, const void* w, int N, int V, int C, int v0, int slabs,
-                         bool first, const float* scale, float* dx_slabs, void* dw, int dw_dtype, int sms, cudaStream_t stream) {
-  HeadProducts p{};
-  p.N = N; p.V = V; p.C = C; p.v0 = v0; p.n_cols = n_cols; p.first = first ? 1 : 0;
-  p.width = C > 128 ? 256 : 128;
-  const int kb = (n_cols + HEAD_BK - 1) / HEAD_BK, kn = (N + HEAD_BK - 1) / HEAD_BK;
-  p.slabs = slabs < kb ? slabs : kb;      // a last piece may be shorter than the slabs are many
-  const int tc = (C + p.width - 1) / p.width, tm = (N + HEAD_TILE - 1) / HEAD_TILE;
-  p.dx_items = dx_slabs ? p.slabs * tm * tc : 0;
-  p.dw_items = dw ? (n_cols + HEAD_TILE - 1) / HEAD_TILE * tc : 0;
+namespace {
+// Sum of the slabs in their order -> dx.
+template <bool BF16_OUT>
+__global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ slabs, int n_slabs, size_t n, void* __restrict__ dx) {
+  pdl_wait();
+  pdl_trigger();
+  const size_t i = (size_t(blockIdx.x) * 256 + threadIdx.x) * 8;
+  if (i >= n) return;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+#pragma unroll 8
+  for (int s = 0; s < n_slabs; ++s) {
+    const float4* v = reinterpret_cast<const float4*>(slabs + size_t(s) * n + i);
+    const float4 x = __ldcs(v), y = __ldcs(v + 1);
+    a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+    b.x += y.x; b.y += y.y; b.z += y.z; b.w += y.w;
+  }
+  if constexpr (BF16_OUT) {
+    reinterpret_cast<uint4*>(dx)[i / 8] = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
+  } else {
+    reinterpret_cast<float4*>(dx)[i / 4] = a;
+    reinterpret_cast<float4*>(dx)[i / 4 + 1] = b;
+  }
+}
+}  // namespace
+
+// Channels of a tile: as few tiles of at most 256 as there can be, of the same width (a multiple of 32, what an MMA of 256 rows takes).
+int head_width(int C) {
+  const int tc = (C + HEAD_TILE - 1) / HEAD_TILE;
+  return ((C + tc - 1) / tc + 31) / 32 * 32;
+}
+
+int launch_head_products(HeadProducts p, const void* g, const void* xs, const void* w, int sms, cudaStream_t stream) {
+  p.width = head_width(p.C);
+  const int kb = (p.n_cols + HEAD_BK - 1) / HEAD_BK, kn = (p.N + HEAD_BK - 1) / HEAD_BK;
+  p.all_slabs = p.slabs;
+  p.slabs = p.slabs < kb ? p.slabs : kb;      // a last piece may be shorter than the slabs are many
+  const int tc = (p.C + p.width - 1) / p.width, tm = (p.N + HEAD_TILE - 1) / HEAD_TILE;
+  p.dx_items = p.dx ? p.slabs * tm * tc : 0;
+  p.dw_items = p.dw ? (p.n_cols + HEAD_TILE - 1) / HEAD_TILE * tc : 0;
   const int k_dx = (kb + p.slabs - 1) / p.slabs;
   p.dw_first = kn > k_dx ? 1 : 0;
-  p.scale = scale; p.dx = dx_slabs; p.dw = dw; p.dw_bf16 = dw_dtype;
-  p.status = device_status_ptr();
-  if (!p.status) return JB200_ERR_CUDA;
-  CUtensorMap tg, tw, tx;
-  int rc;
-  if ((rc = encode_head_map(&tg, g, cols, N, HEAD_BK, "head_loss_backward (gradient of the logits)")) != JB200_OK) return rc;
-  if ((rc = encode_head_map(&tw, w, C, V, HEAD_BK, "head_loss_backward (weight)")) != JB200_OK) return rc;
-  if ((rc = encode_head_map(&tx, xs, C, N, HEAD_BK, "head_loss_backward (rows)")) != JB200_OK) return rc;
   const int items = p.dx_items + p.dw_items, pairs = items < sms / 2 ? items : sms / 2;
   p.shares = p.dw_first ? head_shares(p.dw_items, kn, p.dx_items, k_dx, pairs) : head_shares(p.dx_items, k_dx, p.dw_items, kn, pairs);
+  CUtensorMap tg, tw, tx;
+  int rc;
+  if ((rc = encode_head_map(&tg, g, p.ldg, p.ldg, p.N, HEAD_BK, "head_loss_backward (gradient of the logits)")) != JB200_OK) return rc;
+  if ((rc = encode_head_map(&tw, w, p.C, p.C, p.V, HEAD_BK, "head_loss_backward (weight)")) != JB200_OK) return rc;
+  if ((rc = encode_head_map(&tx, xs, p.C, head_pitch(p.C), p.N, HEAD_BK, "head_loss_backward (rows)")) != JB200_OK) return rc;
   JB_MAX_SMEM(head_products_kernel, HEAD_SMEM);
-  launch_dep_cluster(head_products_kernel, dim3(2 * unsigned(pairs)), dim3(HEAD_THREADS), HEAD_SMEM, 2, stream, tg, tw,
-                     tx, p);
+  launch_dep_cluster(head_products_kernel, dim3(2 * unsigned(pairs)), dim3(HEAD_THREADS), HEAD_SMEM, 2, stream, tg, tw, tx, p);
   JB_LAUNCH_CHECK("head_products_kernel");
+  if (p.dx && p.last && p.all_slabs > 1) {
+    const size_t n = size_t(p.N) * p.C;
+    launch_dep(p.dx_bf16 ? head_dx_kernel<true> : head_dx_kernel<false>, unsigned((n / 8 + 255) / 256), 256, 0, stream, p.dx_slabs, p.all_slabs, n,
+               p.dx);
+    JB_LAUNCH_CHECK("head_dx_kernel");
+  }
   return JB200_OK;
 }
 

@@ -167,10 +167,12 @@ struct HeadLogits {
   int carry;                 // a pair's tiles are all of the same rows: it leaves one part a group of epilogue warps, else every tile does
   float* z_target;           // [N]
   unsigned int* ticket;      // set to 0 for the join
-  // gradient, [3][N] each: the sum's reference point, the row's factor, and the factor over the sum
-  const float *r_ce, *r_kd;
+  HeadGrads grads;           // gradient
   __nv_bfloat16* g;          // gradient: [N][ldg]
   int ldg;
+  const uint4* x;            // gradient: rows to copy, those without a loss as zeros
+  uint4* xs;                 // null: not to be copied
+  int box_rows;              // rows of x that a CTA asks for at a time
   unsigned int* status;
 };
 
@@ -238,6 +240,64 @@ struct Entries {
 
 constexpr int head_values(bool ce, bool kd) { return (ce ? 2 : 0) + (kd ? 3 : 0); }
 
+// A row's part in the gradient: the sum's reference point, the row's factor, the factor over the sum.  A row without target and teacher
+// takes part in nothing, whatever it holds.
+template <bool CE, bool KD>
+struct RowGrad {
+  float l1 = 0.f, g1 = 0.f, p1 = 0.f, l2 = 0.f, g2 = 0.f, p2 = 0.f;
+  bool live = false;
+  __device__ __forceinline__ void load(const HeadGrads& p, int row, float scale) {
+    const float nan = __int_as_float(0x7fc00000);
+    if (CE) {
+      const long long y = p.targets[row];
+      if (y != -100) {
+        live = true;
+        l1 = p.lse[row];
+        g1 = y < 0 || y >= p.V ? nan : row_factor(p.g_ce, p.g_ce_stride, p.n_ce, row) / scale;
+        p1 = g1 / p.lse[size_t(p.N) + row];
+      }
+    }
+    if (KD) {
+      const float e = p.neg_entropy[row];
+      if (e != INFINITY) {
+        live = true;
+        l2 = p.lse_t[row];
+        g2 = e != e ? nan : row_factor(p.g_kd, p.g_kd_stride, p.n_kd, row) * p.tau / scale;
+        p2 = g2 / p.lse_t[size_t(p.N) + row];
+      }
+    }
+  }
+};
+template <bool CE, bool KD>
+__device__ __forceinline__ bool row_is_live(const HeadGrads& p, int row) {
+  return (CE && p.targets[row] != -100) || (KD && p.neg_entropy[row] != INFINITY);
+}
+
+// Rows for dW's product, by two warps of every CTA beside the products: those that take no part become zeros, so that a NaN or an
+// infinity in one does not reach the others' sums.  Four rows a warp at a time.
+template <bool CE, bool KD>
+__device__ __forceinline__ void copy_rows(const HeadLogits& p, int warp, int lane) {
+  const int per_row = p.C / 8, pitch = head_pitch(p.C) / 8, step = int(gridDim.x) * 2 * 4;
+  for (int r0 = (int(blockIdx.x) * 2 + warp) * 4; r0 < p.N; r0 += step) {
+    bool live[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) live[i] = r0 + i < p.N && row_is_live<CE, KD>(p.grads, r0 + i);
+    for (int c = lane; c < per_row; c += 64) {
+      uint4 v[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          v[i][u] = live[i] && c + 32 * u < per_row ? __ldg(p.x + size_t(r0 + i) * per_row + c + 32 * u) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (r0 + i < p.N && c + 32 * u < per_row) p.xs[size_t(r0 + i) * pitch + c + 32 * u] = v[i][u];
+    }
+  }
+}
+
 template <bool CE, bool KD>
 __device__ __forceinline__ void head_part(const HeadLogits& p, int part, int row, const RunningSum& s1, const RunningSum& s2, float dot) {
   float* o = p.part + size_t(part) * head_values(CE, KD) * p.N + row;
@@ -249,8 +309,10 @@ __device__ __forceinline__ void head_part(const HeadLogits& p, int part, int row
 // tiles, each the accumulator of its own (eight warps on every tile leave twice the parts to join).  A column of a row that the
 // teacher asks for is not known to the compiler: where a warp has one, 16 columns go through shared memory, lanes side by side (32
 // compared registers an entry cost 6 to 30 % of a launch at 32 to 64 entries a row).
+constexpr int logits_threads(bool grad) { return HEAD_THREADS + (grad ? 64 : 0); }
+
 template <bool CE, bool KD, bool GRAD>
-__global__ void __launch_bounds__(HEAD_THREADS, 1)
+__global__ void __launch_bounds__(logits_threads(GRAD), 1)
 head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                    const __grid_constant__ HeadLogits p) {
   extern __shared__ uint8_t smem_raw[];
@@ -278,6 +340,10 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
 
   if (warp == 0) {
     // ---------------- TMA: this CTA's rows and its half of the columns ----------------
+    // Where 128 rows are more than there are, the rest of the operand's memory holds anything: it makes rows of the accumulator that
+    // nobody reads.
+    const bool has_rows = rank == 0 || p.N > HEAD_TILE / 2;
+    const uint32_t bytes = 2 * HEAD_OPERAND + uint32_t(p.box_rows) * (HEAD_BK * 2) * (p.N > HEAD_TILE / 2 ? 2 : 1);       // of both CTAs
     int s = 0;
     uint32_t ph = 1u;
     bool ok = true;
@@ -290,8 +356,8 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
         if (!mbar_wait(smem_u32(&ctl->empty[s]), ph, abort_flag, p.status, JB200_STATUS_HEAD_LOAD)) { ok = false; break; }
         const uint32_t full = cluster_map(smem_u32(&ctl->full[s]), 0u);
         if (elect_one()) {
-          if (rank == 0) mbar_arrive_expect_tx(smem_u32(&ctl->full[s]), 4 * HEAD_OPERAND);       // of both CTAs
-          pair_tma_load_2d(a_base + uint32_t(s) * HEAD_OPERAND, &tmap_x, kb * HEAD_BK, row, full);
+          if (rank == 0) mbar_arrive_expect_tx(smem_u32(&ctl->full[s]), bytes);
+          if (has_rows) pair_tma_load_2d(a_base + uint32_t(s) * HEAD_OPERAND, &tmap_x, kb * HEAD_BK, row, full);
           pair_tma_load_2d(b_base + uint32_t(s) * HEAD_OPERAND, &tmap_w, kb * HEAD_BK, col, full);
         }
         __syncwarp();
@@ -328,9 +394,12 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
         }
       }
     }
+  } else if (GRAD && warp >= HEAD_EPI_WARP0 + 8) {
+    if (p.xs) copy_rows<CE, KD>(p, warp - HEAD_EPI_WARP0 - 8, lane);
   } else {
     // ---------------- epilogue ----------------
     const int quarter = warp & 3;                              // TMEM lanes this warp may read
+    const float scale = GRAD ? head_scale(p.grads) : 1.f;
     const uint32_t group = uint32_t(warp - HEAD_EPI_WARP0) >> 2;
     // [16 columns][32 lanes] of this warp
     float* stage = reinterpret_cast<float*>(behind + HEAD_CTL) + (warp - HEAD_EPI_WARP0) * 512 + lane;
@@ -352,11 +421,8 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
         const long long y = p.targets[row];
         if (y >= f0 && y < f_end) target = int(y) - f0;
       }
-      float l1 = 0.f, l2 = 0.f, g1 = 0.f, g2 = 0.f, p1 = 0.f, p2 = 0.f;
-      if (GRAD && on) {
-        if (CE) { l1 = p.r_ce[row]; g1 = p.r_ce[size_t(p.N) + row]; p1 = p.r_ce[2 * size_t(p.N) + row]; }
-        if (KD) { l2 = p.r_kd[row]; g2 = p.r_kd[size_t(p.N) + row]; p2 = p.r_kd[2 * size_t(p.N) + row]; }
-      }
+      RowGrad<CE, KD> rg;
+      if (GRAD && on) rg.load(p.grads, row, scale);
       if (!mbar_wait(smem_u32(&ctl->acc_full[group]), ph, abort_flag, p.status, JB200_STATUS_HEAD_EPILOGUE)) break;
       tc_fence_after_sync();
       __syncwarp();
@@ -373,14 +439,14 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
           for (int j = 0; j < 32; ++j) {
             const float x = __uint_as_float(z[j]);
             float y = 0.f;
-            if (CE) y = p1 * ex2(fmaf(x, k1, -l1));
-            if (KD) y = fmaf(p2, ex2(fmaf(x, k2, -l2)), y);
+            if (CE) y = rg.p1 * ex2(fmaf(x, k1, -rg.l1));
+            if (KD) y = fmaf(rg.p2, ex2(fmaf(x, k2, -rg.l2)), y);
             g[j] = y;
           }
           if (CE && __any_sync(0xffffffffu, unsigned(target - c0) < 32u)) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (target - c0 == j) g[j] -= g1;
+              if (target - c0 == j) g[j] -= rg.g1;
           }
           if (KD) {
 #pragma unroll
@@ -389,7 +455,7 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
 #pragma unroll
               for (int j = 0; j < 16; ++j) stage[j * 32] = g[h + j];
               while (e.id < col + h + 16) {                    // an id may come twice
-                stage[(e.id - col - h) * 32] -= g2 * e.q;
+                stage[(e.id - col - h) * 32] -= rg.g2 * e.q;
                 e.step();
               }
 #pragma unroll
@@ -405,7 +471,7 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
           if (on) {
             uint32_t w[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(g[2 * j], g[2 * j + 1]);
+            for (int j = 0; j < 16; ++j) w[j] = rg.live ? pack_bf16x2(g[2 * j], g[2 * j + 1]) : 0u;
             __nv_bfloat16* d = p.g + size_t(row) * p.ldg + (col - p.v0);
             st_global_256(d, w);
             st_global_256(d + 16, w + 8);
@@ -586,39 +652,8 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) head_join_kernel(const __grid
   }
 }
 
-// ---------------------------------------------------------------------------
-// Backward: the rows' factors, and the rows that have a gradient at all.
-// ---------------------------------------------------------------------------
-struct HeadRowsIn {
-  const __nv_bfloat16* x;
-  const int64_t* targets;
-  const float* neg_entropy;
-  const float *lse_in, *lse_t_in;
-  const float *g_ce, *g_kd;               // gradients of the rows' losses (stride 0: the same for all)
-  int g_ce_stride, g_kd_stride;
-  const float *n_ce, *n_kd;               // divisors (the means' row counts) or null
-  __nv_bfloat16* xs;
-  float *r_ce, *r_kd;                     // [3][N], as HeadLogits has them
-  float* scale;                           // [1]
-  int N, V, C;
-  float tau;
-};
-
-// The gradients of the logits are kept relative to one factor of the whole call, which the products apply to their f32 sums: rows of a
-// mean then have the factor 1, and a target of small probability -1, which bf16 holds.  (With 1 / rows in them that entry, half of a
-// row's gradient, had the same rounding in every row: an error of up to 2^-8 of dx and dW, and no noise that averages out.)
-__device__ __forceinline__ float common_factor(float ce, float kd) {
-  const bool by_ce = ce > 0.f && ce <= FLT_MAX && !(kd > ce * 1e18f);
-  const float s = by_ce ? ce : kd;
-  return s > 0.f && s <= FLT_MAX ? s : 1.f;
-}
-__device__ __forceinline__ float row_factor(const float* g, int stride, const float* n, int row) {
-  const float c = g[size_t(row) * stride];
-  return n ? c / *n : c;
-}
-
-// Losses of the rows: the largest finite factor of each kind.
-__global__ void __launch_bounds__(1024) head_scale_kernel(const __grid_constant__ HeadRowsIn p) {
+// Gradients row by row: their common factor, the largest finite one of its kind.
+__global__ void __launch_bounds__(1024) head_scale_kernel(const __grid_constant__ HeadGrads p) {
   pdl_wait();
   pdl_trigger();
   __shared__ float s_top[2][32];
@@ -646,65 +681,6 @@ __global__ void __launch_bounds__(1024) head_scale_kernel(const __grid_constant_
   }
 }
 
-// A row without target and teacher takes part in nothing: it becomes a row of zeros with factors of 0, so that a NaN or
-// an infinity in it reaches neither its own gradient nor the weight's.
-__global__ void __launch_bounds__(256) head_rows_kernel(const __grid_constant__ HeadRowsIn p) {
-  pdl_wait();
-  pdl_trigger();
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= p.N) return;
-  const float nan = __int_as_float(0x7fc00000);
-  const bool same = p.g_ce_stride == 0 && p.g_kd_stride == 0;      // else the scale is there already
-  float c1 = p.targets ? row_factor(p.g_ce, p.g_ce_stride, p.n_ce, row) : 0.f;
-  float c2 = p.neg_entropy ? row_factor(p.g_kd, p.g_kd_stride, p.n_kd, row) * p.tau : 0.f;
-  const float scale = same ? common_factor(fabsf(c1), fabsf(c2)) : *p.scale;
-  if (same && row == 0 && lane == 0) *p.scale = scale;
-  bool live = false;
-  if (p.targets) {
-    const long long y = p.targets[row];
-    const bool on = y != -100;
-    live |= on;
-    c1 = !on ? 0.f : y < 0 || y >= p.V ? nan : c1 / scale;
-  }
-  if (p.neg_entropy) {
-    const float e = p.neg_entropy[row];
-    const bool on = e != INFINITY;
-    live |= on;
-    c2 = !on ? 0.f : e != e ? nan : c2 / scale;
-  }
-  if (lane == 0) {
-    const size_t N = size_t(p.N);
-    if (p.targets) { p.r_ce[row] = live ? p.lse_in[row] : 0.f; p.r_ce[N + row] = c1; p.r_ce[2 * N + row] = live ? c1 / p.lse_in[N + row] : 0.f; }
-    if (p.neg_entropy) { p.r_kd[row] = live ? p.lse_t_in[row] : 0.f; p.r_kd[N + row] = c2; p.r_kd[2 * N + row] = live ? c2 / p.lse_t_in[N + row] : 0.f; }
-  }
-  const uint4* src = reinterpret_cast<const uint4*>(p.x + size_t(row) * p.C);
-  uint4* dst = reinterpret_cast<uint4*>(p.xs + size_t(row) * p.C);
-  for (int c = lane; c < p.C / 8; c += 32) dst[c] = live ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
-}
-
-// Sum of the slabs in their order -> dx.
-template <bool BF16_OUT>
-__global__ void __launch_bounds__(256) head_dx_kernel(const float* __restrict__ slabs, int n_slabs, size_t n, void* __restrict__ dx) {
-  pdl_wait();
-  pdl_trigger();
-  const size_t i = (size_t(blockIdx.x) * 256 + threadIdx.x) * 8;
-  if (i >= n) return;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-#pragma unroll 4
-  for (int s = 0; s < n_slabs; ++s) {
-    const float4* v = reinterpret_cast<const float4*>(slabs + size_t(s) * n + i);
-    const float4 x = __ldcs(v), y = __ldcs(v + 1);
-    a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
-    b.x += y.x; b.y += y.y; b.z += y.z; b.w += y.w;
-  }
-  if constexpr (BF16_OUT) {
-    reinterpret_cast<uint4*>(dx)[i / 8] = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
-  } else {
-    reinterpret_cast<float4*>(dx)[i / 4] = a;
-    reinterpret_cast<float4*>(dx)[i / 4 + 1] = b;
-  }
-}
-
 // Pairs of a launch.  Where as many waves do with a multiple of the row tiles, that: a pair then keeps to its rows.
 int head_pairs(int N, int cols, int sms) {
   const long long tm = (N + HEAD_TILE - 1) / HEAD_TILE, tiles = tm * ((cols + HEAD_TILE - 1) / HEAD_TILE);
@@ -719,7 +695,7 @@ int launch_logits(const CUtensorMap& tx, const CUtensorMap& tw, const HeadLogits
   constexpr size_t smem = HEAD_SMEM + (KD ? 8 * 512 * 4 : 0);
   static_assert(smem <= 227 * 1024, "shared memory of one CTA");
   JB_MAX_SMEM(kernel, smem);
-  launch_dep_cluster(kernel, dim3(2 * unsigned(head_pairs(p.N, p.cols, sms))), dim3(HEAD_THREADS), smem, 2, stream, tx, tw, p);
+  launch_dep_cluster(kernel, dim3(2 * unsigned(head_pairs(p.N, p.cols, sms))), dim3(logits_threads(GRAD)), smem, 2, stream, tx, tw, p);
   JB_LAUNCH_CHECK("head_logits_kernel");
   return JB200_OK;
 }
@@ -751,9 +727,9 @@ int check_head(const jb200_head* h, const char* what) {
 
 }  // namespace
 
-int encode_head_map(CUtensorMap* tm, const void* ptr, long long cols, long long rows, int box_rows, const char* what) {
+int encode_head_map(CUtensorMap* tm, const void* ptr, long long cols, long long pitch, long long rows, int box_rows, const char* what) {
   const cuuint64_t dim[2] = {cuuint64_t(cols), cuuint64_t(rows)};
-  const cuuint64_t stride[1] = {cuuint64_t(cols) * 2};
+  const cuuint64_t stride[1] = {cuuint64_t(pitch) * 2};
   const cuuint32_t box[2] = {HEAD_BK, cuuint32_t(box_rows)};
   return encode_tiled(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dim, stride, box, CU_TENSOR_MAP_SWIZZLE_128B,
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, what);
@@ -783,11 +759,11 @@ int item_time(int k) { return k > 8 ? k : 8; }
 
 // Time of a piece of n tiles in K-blocks of a pair (512 cycles), and of what follows from its slabs.
 long long piece_time(long long n, int N, int C, int slabs, int pairs) {
-  const int tm = (N + HEAD_TILE - 1) / HEAD_TILE, tc = (C + HEAD_TILE - 1) / HEAD_TILE, kc = (C + HEAD_BK - 1) / HEAD_BK;
+  const int width = head_width(C), tm = (N + HEAD_TILE - 1) / HEAD_TILE, tc = (C + width - 1) / width, kc = (C + HEAD_BK - 1) / HEAD_BK;
   const int k_dw = item_time((N + HEAD_BK - 1) / HEAD_BK), k_dx = item_time(int((n * (HEAD_TILE / HEAD_BK) + slabs - 1) / slabs));
   const int n_dw = int(n) * tc, n_dx = slabs * tm * tc;
   const HeadShares s = k_dw > k_dx ? head_shares(n_dw, k_dw, n_dx, k_dx, pairs) : head_shares(n_dx, k_dx, n_dw, k_dw, pairs);
-  return (tm * n + pairs - 1) / pairs * item_time(kc) + s.span + 24;      // 24: two launches
+  return (tm * n + pairs - 1) / pairs * item_time(kc) + s.span * width / HEAD_TILE + 24;      // 24: two launches
 }
 }  // namespace
 
@@ -817,7 +793,7 @@ HeadPlan head_plan(int N, int V, int C, int pairs) {
     const long long per = cand[i], pieces = (tv + per - 1) / per, last = tv - (pieces - 1) * per;
     for (int slabs = 1; slabs <= 64; slabs += slabs < 4 ? 1 : slabs / 4) {
       if (slabs > 1 && per * (HEAD_TILE / HEAD_BK) / slabs < 8) break;      // at least eight K-blocks each
-      const long long reduce = (long long)slabs * N * C / 400000;           // 4 bytes read at 6 TB/s
+      const long long reduce = slabs == 1 ? 0 : 12 + (long long)slabs * N * C / 400000;      // a launch; 4 bytes read at 6 TB/s
       const long long time = (pieces - 1) * piece_time(per, N, C, slabs, pairs) + piece_time(last, N, C, slabs, pairs) + reduce;
       if (time < best_time) {
         best_time = time;
@@ -858,6 +834,9 @@ int launch_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype
 }
 
 namespace {
+// (one row: 35 us against 26 us with boxes of 128, nearly all of them beyond the matrix)
+int box_rows(int N) { return N >= HEAD_TILE / 2 ? HEAD_TILE / 2 : (N + 7) / 8 * 8; }
+
 void set_teacher(HeadLogits& p, const jb200_head* h) {
   if (!h->teacher) return;
   const TeacherLayout at = teacher_layout(h->N, h->K, h->V);
@@ -905,8 +884,9 @@ int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* means, vo
     if (!p.status) return JB200_ERR_CUDA;
     o.part = p.part; o.z_target = p.z_target;
     CUtensorMap tx, tw;
-    if ((rc = encode_head_map(&tx, h->x, h->C, h->N, HEAD_TILE / 2, "head_loss (rows)")) != JB200_OK) return rc;
-    if ((rc = encode_head_map(&tw, h->w, h->C, h->V, HEAD_TILE / 2, "head_loss (weight)")) != JB200_OK) return rc;
+    p.box_rows = box_rows(h->N);
+    if ((rc = encode_head_map(&tx, h->x, h->C, h->C, h->N, p.box_rows, "head_loss (rows)")) != JB200_OK) return rc;
+    if ((rc = encode_head_map(&tw, h->w, h->C, h->C, h->V, HEAD_TILE / 2, "head_loss (weight)")) != JB200_OK) return rc;
     if ((rc = launch_logits<false>(has_ce, has_kd, tx, tw, p, sms, stream)) != JB200_OK) return rc;
   }
   // (without rows both means are written: nothing says which was asked for)
@@ -918,13 +898,13 @@ int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* means, vo
 
 namespace {
 struct BackwardScratch {
-  size_t xs, rows, g, slabs, total;
+  size_t xs, scale, g, slabs, total;
 };
 BackwardScratch backward_scratch(int N, int C, const HeadPlan& pl) {
   BackwardScratch s;
   s.xs = 0;
-  s.rows = up256(size_t(N) * C * 2);
-  s.g = s.rows + up256((size_t(N) * 6 + 1) * 4);
+  s.scale = up256(size_t(N) * head_pitch(C) * 2);
+  s.g = s.scale + 256;
   s.slabs = s.g + up256(size_t(N) * pl.cols * 2);
   s.total = s.slabs + up256(size_t(pl.slabs) * N * C * 4);
   return s;
@@ -942,14 +922,13 @@ int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_s
   int rc = check_head(h, "head_loss_backward");
   if (rc != JB200_OK) return rc;
   JB_REQUIRE((dx_dtype == 0 || dx_dtype == 1) && (dw_dtype == 0 || dw_dtype == 1), "head_loss_backward: dtype must be 0 (f32) or 1 (bf16)");
-  JB_REQUIRE((reinterpret_cast<uintptr_t>(dw) & 31u) == 0, "head_loss_backward: dw must be 32-byte aligned");
+  JB_REQUIRE(((reinterpret_cast<uintptr_t>(dw) | reinterpret_cast<uintptr_t>(dx)) & 31u) == 0, "head_loss_backward: dx and dw must be 32-byte aligned");
   if (!dx && !dw) return JB200_OK;
   if (h->N == 0) {
     if (dw) JB_CUDA(cudaMemsetAsync(dw, 0, size_t(h->V) * h->C * (dw_dtype ? 2 : 4), stream));
     return JB200_OK;
   }
-  JB_REQUIRE(aligned16(dx) && scratch && (reinterpret_cast<uintptr_t>(scratch) & 255u) == 0,
-             "head_loss_backward: dx must be 16-byte, scratch 256-byte aligned");
+  JB_REQUIRE(scratch && (reinterpret_cast<uintptr_t>(scratch) & 255u) == 0, "head_loss_backward: scratch must be 256-byte aligned");
   JB_REQUIRE((!h->targets || g_ce) && (!h->teacher || g_kd), "head_loss_backward: null pointer (gradients of the losses)");
   JB_REQUIRE((g_ce_stride == 0 || g_ce_stride == 1) && (g_kd_stride == 0 || g_kd_stride == 1), "head_loss_backward: strides must be 0 or 1");
   const int sms = sm_count();
@@ -957,52 +936,51 @@ int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_s
   const HeadPlan pl = head_plan(h->N, h->V, h->C, sms / 2);
   const BackwardScratch at = backward_scratch(h->N, h->C, pl);
   uint8_t* base = static_cast<uint8_t*>(scratch);
-  float* rows = reinterpret_cast<float*>(base + at.rows);
-  const size_t N = size_t(h->N);
 
-  HeadRowsIn r{};
-  r.x = static_cast<const __nv_bfloat16*>(h->x);
+  HeadGrads r{};
   r.targets = h->targets; r.neg_entropy = static_cast<const float*>(h->teacher);
-  r.lse_in = h->lse; r.lse_t_in = h->lse_t;
+  r.lse = h->lse; r.lse_t = h->lse_t;
   r.g_ce = g_ce; r.g_kd = g_kd; r.g_ce_stride = g_ce_stride; r.g_kd_stride = g_kd_stride; r.n_ce = n_ce; r.n_kd = n_kd;
-  r.xs = reinterpret_cast<__nv_bfloat16*>(base + at.xs);
-  r.r_ce = rows; r.r_kd = rows + 3 * N;
-  r.N = h->N; r.V = h->V; r.C = h->C;
+  r.N = h->N; r.V = h->V;
   r.tau = h->teacher ? h->temperature : 1.f;
-  r.scale = rows + 6 * N;
-  if (g_ce_stride != 0 || g_kd_stride != 0) {
+  if ((h->targets && g_ce_stride) || (h->teacher && g_kd_stride)) {
+    r.scale = reinterpret_cast<float*>(base + at.scale);
     launch_dep(head_scale_kernel, 1, 1024, 0, stream, r);
     JB_LAUNCH_CHECK("head_scale_kernel");
   }
-  launch_dep(head_rows_kernel, (h->N + 7) / 8, 256, 0, stream, r);
-  JB_LAUNCH_CHECK("head_rows_kernel");
 
   HeadLogits p{};
   p.N = h->N; p.V = h->V; p.C = h->C;
   p.targets = h->targets; p.inv_tau = 1.0f / r.tau;
   set_teacher(p, h);
-  p.r_ce = r.r_ce; p.r_kd = r.r_kd;
+  p.grads = r;
   p.g = reinterpret_cast<__nv_bfloat16*>(base + at.g);
   p.ldg = pl.cols;
+  if (dw) { p.x = static_cast<const uint4*>(h->x); p.xs = reinterpret_cast<uint4*>(base + at.xs); }
+  HeadProducts q{};
   p.status = device_status_ptr();
   if (!p.status) return JB200_ERR_CUDA;
+  p.box_rows = box_rows(h->N);
   CUtensorMap tx, tw;
-  if ((rc = encode_head_map(&tx, r.xs, h->C, h->N, HEAD_TILE / 2, "head_loss_backward (rows)")) != JB200_OK) return rc;
-  if ((rc = encode_head_map(&tw, h->w, h->C, h->V, HEAD_TILE / 2, "head_loss_backward (weight)")) != JB200_OK) return rc;
+  if ((rc = encode_head_map(&tx, h->x, h->C, h->C, h->N, p.box_rows, "head_loss_backward (rows)")) != JB200_OK) return rc;
+  if ((rc = encode_head_map(&tw, h->w, h->C, h->C, h->V, HEAD_TILE / 2, "head_loss_backward (weight)")) != JB200_OK) return rc;
+  q.N = h->N; q.V = h->V; q.C = h->C;
+  q.ldg = pl.cols;
+  q.grads = r;
+  q.dx = dx; q.dx_bf16 = dx_dtype;
   // one slab in f32 is the result itself
-  const bool direct = dx_dtype == 0 && pl.slabs == 1 && (reinterpret_cast<uintptr_t>(dx) & 31u) == 0;
-  float* slabs = !dx ? nullptr : direct ? static_cast<float*>(dx) : reinterpret_cast<float*>(base + at.slabs);
+  q.dx_slabs = !dx ? nullptr : dx_dtype == 0 && pl.slabs == 1 ? static_cast<float*>(dx) : reinterpret_cast<float*>(base + at.slabs);
+  q.dw = dw; q.dw_bf16 = dw_dtype;
+  q.status = p.status;
   for (int i = 0; i < pl.pieces; ++i) {
-    p.v0 = i * pl.cols;
-    p.cols = h->V - p.v0 < pl.cols ? h->V - p.v0 : pl.cols;
+    p.v0 = q.v0 = i * pl.cols;
+    p.cols = q.n_cols = h->V - p.v0 < pl.cols ? h->V - p.v0 : pl.cols;
+    q.slabs = pl.slabs;
+    q.first = i == 0;
+    q.last = i + 1 == pl.pieces;
     if ((rc = launch_logits<true>(h->targets != nullptr, h->teacher != nullptr, tx, tw, p, sms, stream)) != JB200_OK) return rc;
-    rc = launch_head_products(p.g, pl.cols, p.cols, r.xs, h->w, h->N, h->V, h->C, p.v0, pl.slabs, i == 0, r.scale, slabs, dw, dw_dtype, sms, stream);
-    if (rc != JB200_OK) return rc;
-  }
-  if (dx && !direct) {
-    const size_t n = N * h->C;
-    launch_dep(dx_dtype == 1 ? head_dx_kernel<true> : head_dx_kernel<false>, unsigned((n / 8 + 255) / 256), 256, 0, stream, slabs, pl.slabs, n, dx);
-    JB_LAUNCH_CHECK("head_dx_kernel");
+    if ((rc = launch_head_products(q, p.g, base + at.xs, h->w, sms, stream)) != JB200_OK) return rc;
+    p.xs = nullptr;
   }
   return JB200_OK;
 }

@@ -12,6 +12,38 @@ constexpr size_t HEAD_CTL = (sizeof(HeadRing) + 127) / 128 * 128;
 constexpr size_t HEAD_SMEM = 1024 + size_t(HEAD_STAGES) * 2 * HEAD_OPERAND + HEAD_CTL;
 static_assert(HEAD_SMEM <= 227 * 1024, "shared memory of one CTA");
 
+// Gradients of the losses and what the forward call left, as the backward kernels read them.
+struct HeadGrads {
+  const int64_t* targets;                 // null: no cross entropy
+  const float* neg_entropy;               // null: no teacher
+  const float *lse, *lse_t;               // [2][N]: reference point and sum
+  const float *g_ce, *g_kd;               // gradients of the rows' losses (stride 0: the same for all)
+  int g_ce_stride, g_kd_stride;
+  const float *n_ce, *n_kd;               // divisors (the means' row counts) or null
+  float* scale;                           // [1], with gradients row by row: their common factor, made by a launch of its own
+  int N, V;
+  float tau;
+};
+
+#if defined(__CUDACC__)
+// The gradients of the logits are kept relative to one factor of the whole call, which the products apply to their f32 sums: rows of a
+// mean then have the factor 1, and a target of small probability -1, which bf16 holds.  (With 1 / rows in them that entry, half of a
+// row's gradient, had the same rounding in every row: an error of up to 2^-8 of dx and dW, and no noise that averages out.)
+__device__ __forceinline__ float common_factor(float ce, float kd) {
+  const bool by_ce = ce > 0.f && ce <= 3.4e38f && !(kd > ce * 1e18f);
+  const float s = by_ce ? ce : kd;
+  return s > 0.f && s <= 3.4e38f ? s : 1.f;
+}
+__device__ __forceinline__ float row_factor(const float* g, int stride, const float* n, int row) {
+  const float c = g[size_t(row) * stride];
+  return n ? c / *n : c;
+}
+__device__ __forceinline__ float head_scale(const HeadGrads& p) {
+  if (p.scale) return *p.scale;
+  return common_factor(p.targets ? fabsf(row_factor(p.g_ce, 0, p.n_ce, 0)) : 0.f, p.neg_entropy ? fabsf(row_factor(p.g_kd, 0, p.n_kd, 0)) * p.tau : 0.f);
+}
+#endif
+
 // How a backward pass is cut: `pieces` pieces of `cols` vocabulary columns (the last one shorter) whose gradients of the logits are
 // kept as bf16, and `slabs` parts of a piece over which the hidden rows' gradient is summed side by side.
 struct HeadPlan {
@@ -41,11 +73,33 @@ __host__ __device__ __forceinline__ int head_walk(const HeadShares& s, int n_lon
   return t < n_short ? n_long + t : -1;
 }
 
-int encode_head_map(CUtensorMap* tm, const void* ptr, long long cols, long long rows, int box_rows, const char* what);
+// Boxes of 64 columns of a bf16 matrix whose rows are `pitch` elements apart.
+int encode_head_map(CUtensorMap* tm, const void* ptr, long long cols, long long pitch, long long rows, int box_rows, const char* what);
+// Pitch of the copied rows: whole 128-byte lines, where a box's rows are one line each.
+__host__ __device__ inline int head_pitch(int C) { return (C + HEAD_BK - 1) / HEAD_BK * HEAD_BK; }
 
-// dx slabs += G W and dW = G^T xs of one piece (head_grad.cu); a null one is not wanted.  g: bf16 [N][cols]; piece columns [0, n_cols) are vocabulary rows
-// [v0, v0 + n_cols) of w and dw.
-int launch_head_products(const void* g, int cols, int n_cols, const void* xs, const void* w, int N, int V, int C, int v0, int slabs,
-                         bool first, const float* scale, float* dx_slabs, void* dw, int dw_dtype, int sms, cudaStream_t stream);
+// dx += scale G W and dw = scale G^T xs of one piece (head_grad.cu); a null one is not wanted.
+struct HeadProducts {
+  int N, V, C;
+  int v0, n_cols;            // the piece's vocabulary rows
+  int ldg;                   // columns of G
+  int slabs;
+  int first, last;           // of the pieces
+  HeadGrads grads;
+  float* dx_slabs;           // [slabs][N][C] f32: sums so far; may be dx itself
+  void* dx;                  // [N][C], written by the last piece
+  int dx_bf16;
+  void* dw;                  // [V][C]
+  int dw_bf16;
+  // made by the launch
+  int all_slabs;             // of dx_slabs; a short last piece adds to `slabs` of them
+  int width;                 // columns of a tile
+  int dx_items, dw_items;
+  int dw_first;              // dW's items are the long ones
+  HeadShares shares;
+  unsigned int* status;
+};
+int head_width(int C);
+int launch_head_products(HeadProducts p, const void* g, const void* xs, const void* w, int sms, cudaStream_t stream);
 
 }  // namespace jb

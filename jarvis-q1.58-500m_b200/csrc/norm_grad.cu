@@ -125,23 +125,21 @@ rmsnorm_backward_kernel(const TX* __restrict__ x, const float* __restrict__ w, f
   }
 }
 
-// dw[c] = sum of the CTAs' parts in a fixed order.
-__global__ void __launch_bounds__(256) rmsnorm_dw_kernel(const float* __restrict__ part, int n_parts, int C, float* __restrict__ dw) {
+// dw[c] = sum of the CTAs' parts in a fixed order: a warp every 32nd of them, then the warps.
+__global__ void __launch_bounds__(1024) rmsnorm_dw_kernel(const float* __restrict__ part, int n_parts, int C, float* __restrict__ dw) {
   pdl_wait();
   pdl_trigger();
-  __shared__ float s[8][33];
+  __shared__ float s[32][33];
   const int g = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane;
   float sum = 0.f;
   if (c < C) {
-#pragma unroll 8
-    for (int i = g; i < n_parts; i += 8) sum += part[size_t(i) * C + c];
+#pragma unroll 10
+    for (int i = g; i < n_parts; i += 32) sum += part[size_t(i) * C + c];
   }
   s[g][lane] = sum;
   __syncthreads();
-  if (g == 0 && c < C) {
-    for (int i = 1; i < 8; ++i) sum += s[i][lane];
-    dw[c] = sum;
-  }
+  sum = warp_sum(s[lane][g]);
+  if (lane == 0 && blockIdx.x * 32 + g < C) dw[blockIdx.x * 32 + g] = sum;
 }
 
 int norm_warps(int C) { return C <= NG_SPAN ? 1 : C <= 2 * NG_SPAN ? 2 : 4; }
@@ -192,7 +190,7 @@ int launch_rmsnorm_backward(const void* x, int x_dtype, const float* w, float ep
   else if (dy_dtype == 0) rc = launch_rmsnorm_backward_t<b16, float>(x, w, eps, dy, n_rows, C, dx, part, ctas, stream);
   else rc = launch_rmsnorm_backward_t<b16, b16>(x, w, eps, dy, n_rows, C, dx, part, ctas, stream);
   if (rc != JB200_OK) return rc;
-  launch_dep(rmsnorm_dw_kernel, (C + 31) / 32, 256, 0, stream, part, ctas, C, dw);
+  launch_dep(rmsnorm_dw_kernel, (C + 31) / 32, 1024, 0, stream, part, ctas, C, dw);
   JB_LAUNCH_CHECK("rmsnorm_dw_kernel");
   return JB200_OK;
 }

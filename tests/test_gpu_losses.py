@@ -487,3 +487,26 @@ def test_corpus_evaluation_without_logits():
     b = evaluate.evaluate_corpus(model, toks, num_windows=3, seq_len=64, seed=1, no_logits=True)
     assert abs(a["mean_loss"] - b["mean_loss"]) <= 2.0 ** -7 * 4 and not b["has_nan_inf"]
     assert evaluate.parse_args(["--no-logits"]).no_logits and not evaluate.parse_args([]).no_logits
+
+
+def test_first_call_of_a_thread():
+    """A thread that has made no CUDA call of its own yet, as autograd's, may begin with any of these calls."""
+    import threading
+    h, w, t, ids, logits = _problem(40, 500, 64, 6)
+    r = ops.head_loss(h, w, t)
+    g = torch.ones((), device="cuda")
+    want = ops.head_loss_backward(h, w, r, t, g_ce=g)
+    torch.cuda.synchronize()
+    got = []
+
+    def run(f):
+        try:
+            got.append(f())
+        except Exception as exc:       # reported by the assertion below
+            got.append(exc)
+    for f in (lambda: ops.head_loss_backward(h, w, r, t, g_ce=g), lambda: ops.head_loss(h, w, t).ce):
+        th = threading.Thread(target=run, args=(f,))
+        th.start()
+        th.join()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0][0], want[0]) and torch.equal(got[0][1], want[1]) and torch.equal(got[1], r.ce)

@@ -39,7 +39,7 @@ def test_head_calls_refuse_missing_outputs():
     assert lib.jb200_head_loss(C.byref(h), None, None, None, 4096, None) == _lib.ERR_ARG
     assert lib.jb200_head_loss(C.byref(h), 4096, None, None, None, None) == _lib.ERR_ARG
     for dx, dxt, dw, scratch, stride, text in ((4096, 2, 4096, 4096, 0, "dtype"), (4096, 1, 4112, 4096, 0, "32-byte"),
-                                               (4100, 1, 4096, 4096, 0, "16-byte"), (4096, 1, 4096, 4100, 0, "256-byte"),
+                                               (4112, 1, 4096, 4096, 0, "32-byte"), (4096, 1, 4096, 4100, 0, "256-byte"),
                                                (4096, 1, 4096, 4096, 2, "strides")):
         assert lib.jb200_head_loss_backward(C.byref(h), 4096, stride, None, None, 0, None, dx, dxt, dw, 1, scratch, None) == _lib.ERR_ARG
         assert text in _lib.last_error()
