@@ -87,7 +87,7 @@ PROTOTYPES = {
     "jb200_teacher_rows_bytes": (_Z, [_I] * 3),
     "jb200_teacher_rows": (_I, [_P, _P, _I, _I, _I, _I, _F, _P, _P]),
     "jb200_head_loss_scratch_bytes": (_Z, [_I] * 4),
-    "jb200_head_loss": (_I, [C.POINTER(Head), _P, _P, _P, _P, _P]),
+    "jb200_head_loss": (_I, [C.POINTER(Head), _P, _P, _P, _P, _P, _P, _P]),
     "jb200_head_loss_backward_scratch_bytes": (_Z, [_I] * 3),
     "jb200_head_loss_backward": (_I, [C.POINTER(Head), _P, _I, _P, _P, _I, _P, _P, _I, _P, _I, _P, _P]),
     "jb200_host_head_walk": (_I, [_I] * 7),

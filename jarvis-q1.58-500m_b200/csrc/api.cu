@@ -479,8 +479,8 @@ int jb200_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype,
   return launch_teacher_rows(ids, logits, logits_dtype, N, K, V, temperature, rows, static_cast<cudaStream_t>(stream));
 }
 size_t jb200_head_loss_scratch_bytes(int N, int V, int ce, int kd) { return N < 1 || V < 1 ? 0 : head_loss_scratch_bytes(N, V, ce, kd); }
-int jb200_head_loss(const jb200_head* h, float* ce, float* kd, float* means, void* scratch, void* stream) {
-  return launch_head_loss(h, ce, kd, means, scratch, static_cast<cudaStream_t>(stream));
+int jb200_head_loss(const jb200_head* h, float* ce, float* kd, float* mean_ce, float* mean_kd, float* counts, void* scratch, void* stream) {
+  return launch_head_loss(h, ce, kd, mean_ce, mean_kd, counts, scratch, static_cast<cudaStream_t>(stream));
 }
 size_t jb200_head_loss_backward_scratch_bytes(int N, int V, int C) { return head_loss_backward_scratch_bytes(N, V, C); }
 int jb200_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_stride, const float* n_ce, const float* g_kd, int g_kd_stride,

@@ -532,7 +532,8 @@ struct HeadRowsOut {
   const float* part;
   const float* z_target;
   float *lse, *ce, *lse_t, *kd;
-  float* means;              // mean and number of the rows with a target, then of those with a teacher; null: not wanted
+  float *mean_ce, *mean_kd;  // null: not wanted
+  float* counts;             // with means: rows with a target, rows with a teacher
   unsigned int* ticket;
   int N, V, parts;
   float inv_tau, tau;
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) head_join_kernel(const __grid
       p.kd[row] = e == INFINITY ? 0.f : float(double(p.tau) * (double(p.tau) * double(e) + (l - double(dot))));
     }
   }
-  if (!p.means) return;
+  if (!p.counts) return;
 
   __shared__ bool s_last;
   __shared__ double s_sum[2][32];
@@ -647,8 +648,9 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) head_join_kernel(const __grid
     double a = 0.0;
     int n = 0;
     for (int w = 0; w < 32; ++w) { a += s_sum[i][w]; n += s_cnt[i][w]; }
-    p.means[2 * i] = float(a / double(n));             // no row that counts: 0 / 0 = NaN, as the mean of the logits' loss has it
-    p.means[2 * i + 1] = float(n);
+    float* mean = i == 0 ? p.mean_ce : p.mean_kd;
+    if (mean) *mean = float(a / double(n));            // no row that counts: 0 / 0 = NaN, as the mean of the logits' loss has it
+    p.counts[i] = float(n);
   }
 }
 
@@ -850,19 +852,20 @@ void set_teacher(HeadLogits& p, const jb200_head* h) {
 
 size_t head_loss_scratch_bytes(int N, int V, int ce, int kd) {
   const size_t parts = (size_t(V) + HEAD_TILE - 1) / HEAD_TILE;
-  return (parts * head_values(ce != 0, kd != 0) + 1) * size_t(N) * 4 + 4;
+  return (parts * head_values(ce != 0, kd != 0) + 3) * size_t(N) * 4 + 4;
 }
 
-int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* means, void* scratch, cudaStream_t stream) {
+int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* mean_ce, float* mean_kd, float* counts, void* scratch, cudaStream_t stream) {
   int rc = check_head(h, "head_loss");
   if (rc != JB200_OK) return rc;
   JB_REQUIRE(h->N == 0 || scratch, "head_loss: null pointer (scratch)");
-  JB_REQUIRE(h->N == 0 || ((!h->targets || ce) && (!h->teacher || kd)), "head_loss: null pointer (losses)");
+  JB_REQUIRE(counts || (!mean_ce && !mean_kd), "head_loss: null pointer (counts)");
   const bool has_ce = h->targets != nullptr, has_kd = h->teacher != nullptr;
-  if (h->N == 0 && !means) return JB200_OK;
+  if (h->N == 0 && !counts) return JB200_OK;
   HeadRowsOut o{};
   o.targets = h->targets; o.neg_entropy = static_cast<const float*>(h->teacher);
-  o.lse = h->lse; o.ce = ce; o.lse_t = h->lse_t; o.kd = kd; o.means = means;
+  o.lse = h->lse; o.lse_t = h->lse_t;
+  o.mean_ce = mean_ce; o.mean_kd = mean_kd; o.counts = counts;
   o.N = h->N; o.V = h->V;
   o.tau = has_kd ? h->temperature : 1.f;
   o.inv_tau = 1.0f / o.tau;
@@ -879,7 +882,10 @@ int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* means, vo
     if (p.carry) o.parts = 2 * (pairs / tm);
     p.part = static_cast<float*>(scratch);
     p.z_target = p.part + size_t(o.parts) * head_values(has_ce, has_kd) * h->N;
-    p.ticket = o.ticket = reinterpret_cast<unsigned int*>(p.z_target + h->N);
+    // rows' losses that the caller does not ask for live here
+    o.ce = ce ? ce : p.z_target + size_t(h->N);
+    o.kd = kd ? kd : p.z_target + 2 * size_t(h->N);
+    p.ticket = o.ticket = reinterpret_cast<unsigned int*>(p.z_target + 3 * size_t(h->N));
     p.status = device_status_ptr();
     if (!p.status) return JB200_ERR_CUDA;
     o.part = p.part; o.z_target = p.z_target;

@@ -59,14 +59,16 @@ def _forward(hidden, weight, targets, ids, logits, temperature, mean):
         ids = _rows(ids, lead, (torch.int64,), "teacher_ids", ids.shape[-1])
         logits = _rows(logits, lead, (torch.float32, torch.bfloat16), "teacher_logits", ids.shape[1])
         teacher = ops.teacher_rows(ids, logits, w.shape[0], temperature)
-    return x, w, targets, teacher, ops.head_loss(x, w, targets, teacher, want_means=mean), lead
+    return x, w, targets, teacher, ops.head_loss(x, w, targets, teacher, want_rows=not mean, want_means=mean), lead
 
 
 def _results(r, lead):
     """(cross entropy, distillation), None where not asked for."""
-    if r.has_means:
-        return (r.buf[6 * r.N] if r.has_ce else None), (r.buf[6 * r.N + 2] if r.has_kd else None)
-    return (r.ce.view(lead) if r.has_ce else None), (r.kd.view(lead) if r.has_kd else None)
+    if r.info[2]:
+        return r.mean_ce, r.mean_kd
+    if len(lead) == 1:
+        return r.ce, r.kd
+    return (None if r.ce is None else r.ce.view(lead)), (None if r.kd is None else r.kd.view(lead))
 
 
 class _HeadLoss(torch.autograd.Function):
@@ -91,7 +93,7 @@ def _head_backward(ctx, g_ce, g_kd):
     if not mean:
         g_ce, g_kd = (None if g is None else g.reshape(-1).contiguous() for g in (g_ce, g_kd))
     want_dx, want_dw = ctx.needs_input_grad[:2]
-    dx, dw = ops.head_loss_backward(x, w, ops.HeadLoss(buf, N, targets is not None, teacher is not None, mean), targets, teacher, g_ce=g_ce,
+    dx, dw = ops.head_loss_backward(x, w, ops.HeadLoss(N, buf, (targets is not None, teacher is not None, mean)), targets, teacher, g_ce=g_ce,
                                     g_kd=g_kd, mean=mean, dx_dtype=dx_dtype, dw_dtype=dw_dtype, want_dx=want_dx, want_dw=want_dw)
     if want_dx and len(shape) != 2:
         dx = dx.view(shape)

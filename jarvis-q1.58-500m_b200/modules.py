@@ -775,9 +775,9 @@ class Jarvis(nn.Module):
         there): cross entropy over the targets other than -100 plus the layers' auxiliary terms, f32 scalar.  The logits enter the
         softmax as f32, forward's as bf16: the two agree as far as that rounding goes."""
         r = ops.head_loss(self.hidden_rows(idx, persist_state), self._lm_head_rows(),
-                          ops._need(targets.reshape(-1).contiguous(), torch.int64, "loss.targets"))
+                          ops._need(targets.reshape(-1).contiguous(), torch.int64, "loss.targets"), want_rows=False)
         aux, reflect = self._aux_terms(r.buf.device)
-        return r.means[0] + aux[:, 0].sum() + reflect.sum()
+        return r.mean_ce + aux[:, 0].sum() + reflect.sum()
 
     def head_loss(self, idx, targets=None, teacher_ids=None, teacher_logits=None, *, temperature: float = 1.0):
         """Losses to train the head by: the blocks run as they are (inference, no gradient), then final norm and lm_head with

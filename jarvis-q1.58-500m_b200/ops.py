@@ -610,34 +610,22 @@ def teacher_rows(ids: torch.Tensor, logits: torch.Tensor, vocab: int, temperatur
 
 
 class HeadLoss:
-    """What head_loss leaves: the rows' losses `ce` and `kd` (N,), `means` (4,) [mean ce, rows with a target, mean kd, rows with a teacher],
-    all f32 and None where not asked for, and the softmaxes' sums for the backward call."""
-    __slots__ = ("buf", "N", "has_ce", "has_kd", "has_means")       # buf: f32, ce, its sums (2 N), kd, its sums (2 N), means
+    """What head_loss leaves, f32, None where not asked for: the rows' losses `ce` and `kd` (N,), their means `mean_ce` and `mean_kd` ();
+    and, for the backward call, the softmaxes' sums and the rows that the means are over."""
+    __slots__ = ("N", "buf", "ce", "kd", "mean_ce", "mean_kd", "info")      # buf: sums (2 N), sums of the distillation (2 N), counts (2)
 
-    def __init__(self, buf, N, has_ce, has_kd, has_means):
-        self.buf, self.N, self.has_ce, self.has_kd, self.has_means = buf, N, has_ce, has_kd, has_means
-
-    @property
-    def ce(self):
-        return self.buf[:self.N] if self.has_ce else None
-
-    @property
-    def kd(self):
-        return self.buf[3 * self.N:4 * self.N] if self.has_kd else None
-
-    @property
-    def means(self):
-        return self.buf[6 * self.N:] if self.has_means else None
+    def __init__(self, N, buf, info):
+        self.N, self.buf, self.info = N, buf, info          # info: (with targets, with a teacher, with means)
+        self.ce = self.kd = self.mean_ce = self.mean_kd = None
 
 
 def _head(x, w, targets, teacher, what):
     _need(x, torch.bfloat16, what)
     _need(w, torch.bfloat16, what)
-    (N, width), (V, columns) = x.shape, w.shape
-    if width != columns:
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise RuntimeError(f"{what}: rows {tuple(x.shape)} and weight {tuple(w.shape)} must be (N, C) and (V, C)")
-    dev = x.device
-    h = _lib.Head(N, V, width, x.data_ptr(), w.data_ptr())
+    N, V, dev = x.shape[0], w.shape[0], x.device
+    h = _lib.Head(N, V, x.shape[1], x.data_ptr(), w.data_ptr())
     if targets is not None:
         _need(targets, torch.int64, what)
         if targets.numel() != N:
@@ -659,19 +647,34 @@ def _head(x, w, targets, teacher, what):
 
 
 def head_loss(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor | None = None, teacher: TeacherRows | None = None, *,
-              want_means: bool = True) -> HeadLoss:
+              want_rows: bool = True, want_means: bool = True) -> HeadLoss:
     """Losses of lm_head (jarvis_engine/jarvis_model.py:535-540) straight from its rows, the logits x w^T never stored: cross entropy
     against int64 `targets` (N,) (-100: none, loss 0; otherwise outside the vocabulary: NaN), the divergence t^2 KL(teacher || student)
     from `teacher`, or both.  x: bf16 (N, C); w: bf16 (V, C), any V (no padding needed), C a multiple of 8 and at least 64."""
     lib = _lib.load()
     h = _head(x, w, targets, teacher, "head_loss")
-    N, dev = h.N, x.device
-    r = HeadLoss(torch.empty(6 * N + 4, dtype=torch.float32, device=dev), N, targets is not None, teacher is not None, want_means)
+    N, dev, f32 = h.N, x.device, torch.float32
+    has_ce, has_kd = targets is not None, teacher is not None
+    r = HeadLoss(N, torch.empty(4 * N + 2, dtype=f32, device=dev), (has_ce, has_kd, want_means))
     at = r.buf.data_ptr()
-    h.lse, h.lse_t = at + 4 * N, at + 16 * N
-    scratch = torch.empty(lib.jb200_head_loss_scratch_bytes(N, h.V, r.has_ce, r.has_kd), dtype=torch.uint8, device=dev)
-    _lib.check(_launch(x, lib.jb200_head_loss, ctypes.byref(h), at, at + 12 * N, at + 24 * N if want_means else None, scratch.data_ptr()),
-               "jb200_head_loss")
+    h.lse, h.lse_t = at, at + 8 * N
+    p = [None] * 4
+    if want_rows:
+        if has_ce:
+            r.ce = torch.empty(N, dtype=f32, device=dev)
+            p[0] = r.ce.data_ptr()
+        if has_kd:
+            r.kd = torch.empty(N, dtype=f32, device=dev)
+            p[1] = r.kd.data_ptr()
+    if want_means:
+        if has_ce:
+            r.mean_ce = torch.empty((), dtype=f32, device=dev)
+            p[2] = r.mean_ce.data_ptr()
+        if has_kd:
+            r.mean_kd = torch.empty((), dtype=f32, device=dev)
+            p[3] = r.mean_kd.data_ptr()
+    scratch = torch.empty(lib.jb200_head_loss_scratch_bytes(N, h.V, has_ce, has_kd), dtype=torch.uint8, device=dev)
+    _lib.check(_launch(x, lib.jb200_head_loss, ctypes.byref(h), *p, at + 16 * N if want_means else None, scratch.data_ptr()), "jb200_head_loss")
     return r
 
 
@@ -692,17 +695,18 @@ def head_loss_backward(x: torch.Tensor, w: torch.Tensor, fwd: HeadLoss, targets:
     lib = _lib.load()
     h = _head(x, w, targets, teacher, "head_loss_backward")
     N, dev = h.N, x.device
-    if fwd.N != N or fwd.has_ce != (targets is not None) or fwd.has_kd != (teacher is not None) or (mean and not fwd.has_means):
+    has_ce, has_kd = targets is not None, teacher is not None
+    if fwd.N != N or fwd.info[:2] != (has_ce, has_kd) or (mean and not fwd.info[2]):
         raise RuntimeError("head_loss_backward: `fwd` is not the forward call's result for these arguments")
     at = fwd.buf.data_ptr()
-    h.lse, h.lse_t = at + 4 * N, at + 16 * N
+    h.lse, h.lse_t = at, at + 8 * N
     pc = pk = nc = nk = None
-    if fwd.has_ce:
+    if has_ce:
         pc = _loss_gradient(g_ce, 1 if mean else N, "g_ce")
-        nc = at + 24 * N + 4 if mean else None
-    if fwd.has_kd:
+        nc = at + 16 * N if mean else None
+    if has_kd:
         pk = _loss_gradient(g_kd, 1 if mean else N, "g_kd")
-        nk = at + 24 * N + 12 if mean else None
+        nk = at + 16 * N + 4 if mean else None
     _together("head_loss_backward", x, fwd.buf, g_ce, g_kd)
     dx = torch.empty((N, h.C), dtype=dx_dtype, device=dev) if want_dx else None
     dw = torch.empty((h.V, h.C), dtype=dw_dtype, device=dev) if want_dw else None

@@ -303,6 +303,24 @@ def test_one_gradient_alone():
     _check_grad(got[1], want["dw"], want["dw_bound"])
 
 
+def test_losses_may_be_changed_in_place():
+    """`loss /= steps`, `rows *= mask`: the results are nobody else's memory."""
+    h, w, t, ids, logits = _problem(30, 300, 64, 5)
+    x, wt = h.clone().requires_grad_(), w.clone().requires_grad_()
+    want = torch.autograd.grad(losses.linear_cross_entropy(x, wt, t) / 4, (x, wt))
+    loss = losses.linear_cross_entropy(x, wt, t)
+    loss /= 4
+    for a, b in zip(torch.autograd.grad(loss, (x, wt)), want):
+        assert torch.equal(a, b)
+    mask = (torch.arange(30, device="cuda") % 3 != 0).float()
+    ce, kd = losses.linear_losses(x, wt, t, ids, logits, reduction="none")
+    want = torch.autograd.grad((ce * mask + kd).sum(), (x, wt), retain_graph=True)
+    ce, kd = losses.linear_losses(x, wt, t, ids, logits, reduction="none")
+    ce *= mask
+    for a, b in zip(torch.autograd.grad((ce + kd).sum(), (x, wt)), want):
+        assert torch.equal(a, b)
+
+
 def test_shapes_strides_and_types():
     h, w, t, ids, logits = _problem(24, 300, 128, 5)
     want = losses.linear_losses(h, w, t, ids, logits.bfloat16().float(), reduction="none")
@@ -314,11 +332,22 @@ def test_shapes_strides_and_types():
     got = losses.linear_losses(h.float(), w.float(), t, ids, logits.bfloat16(), reduction="none")
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     for bad in (dict(h=h.half()), dict(w=w[:, :64]), dict(t=t[:5]), dict(t=t.int()), dict(ids=ids[:, :3]), dict(logits=logits.double()),
-                dict(w=w.t()), dict(h=h[:, :60], w=w[:, :60])):
+                dict(w=w.t()), dict(h=h[:, :60], w=w[:, :60]), dict(w=w[0])):
         a = dict(h=h, w=w, t=t, ids=ids, logits=logits)
         a.update(bad)
         with pytest.raises(RuntimeError):
             losses.linear_losses(a["h"], a["w"], a["t"], a["ids"], a["logits"])
+    for x2, w2 in ((h[0], w), (h, w[None]), (h.float(), w), (h, w.float()), (h.t().contiguous().t(), w)):
+        with pytest.raises(RuntimeError):
+            ops.head_loss(x2, w2, t)
+    r = ops.head_loss(h, w, t, want_means=False)
+    one = torch.ones((), device="cuda")
+    for args in (dict(targets=t, g_ce=one), dict(teacher=ops.teacher_rows(ids, logits, 300), g_kd=one, mean=False),
+                 dict(targets=t, g_ce=one, mean=False), dict(targets=t, mean=False)):
+        with pytest.raises(RuntimeError):
+            ops.head_loss_backward(h, w, r, **args)
+    with pytest.raises(RuntimeError, match="vocabulary"):
+        ops.head_loss(h, w, teacher=ops.teacher_rows(ids, logits, 301))
     for tau in (0.0, -1.0, math.nan, math.inf):
         with pytest.raises(RuntimeError, match="temperature"):
             losses.linear_distillation(h, w, ids, logits, temperature=tau)
@@ -455,8 +484,9 @@ def test_model_losses():
     assert abs(float(got) - float(want)) <= 2 * 2.0 ** -8 * top + 1e-5
     ce = model.head_loss(idx, y)
     aux, reflect = model._aux_terms(ce.device)
-    assert abs(float(ce) - float(got - aux[:, 0].sum() - reflect.sum())) <= 1e-5 * abs(float(got))
     ce.backward()
+    ce = ce.detach()
+    assert abs(float(ce) - float(got - aux[:, 0].sum() - reflect.sum())) <= 1e-5 * abs(float(got))
     named = {n: p.grad for n, p in model.named_parameters() if p.grad is not None}
     assert set(named) == {"final_norm.weight", "lm_head.weight"}
     assert all(torch.isfinite(v).all() and v.abs().max() > 0 and v.dtype == torch.float32 for v in named.values())
@@ -468,7 +498,7 @@ def test_model_losses():
     assert (named["lm_head.weight"].double() - dref).norm() <= 2.0 ** -8 * dref.norm()      # dz's rounding alone
     # the kernel-by-kernel path has the same
     model.use_chain = False
-    assert abs(float(model.head_loss(idx, y)) - float(ce)) <= 1e-3 * float(ce)
+    assert abs(float(model.head_loss(idx, y).detach()) - float(ce)) <= 1e-3 * float(ce)
     model.use_chain = True
     top_l, top_i = logits.float().topk(9, dim=-1)
     kd = model.head_loss(idx, teacher_ids=top_i, teacher_logits=top_l, temperature=2.0)

@@ -27,7 +27,7 @@ def _head(**kw):
 def test_head_calls_refuse_bad_arguments(kw, text):
     lib = _lib.load()
     h = _head(**kw)
-    assert lib.jb200_head_loss(C.byref(h), 4096, 4096, None, 4096, None) == _lib.ERR_ARG
+    assert lib.jb200_head_loss(C.byref(h), 4096, 4096, None, None, None, 4096, None) == _lib.ERR_ARG
     assert text in _lib.last_error()
     assert lib.jb200_head_loss_backward(C.byref(h), 4096, 0, None, 4096, 0, None, 4096, 1, 4096, 1, 4096, None) == _lib.ERR_ARG
     assert text in _lib.last_error()
@@ -36,8 +36,8 @@ def test_head_calls_refuse_bad_arguments(kw, text):
 def test_head_calls_refuse_missing_outputs():
     lib = _lib.load()
     h = _head()
-    assert lib.jb200_head_loss(C.byref(h), None, None, None, 4096, None) == _lib.ERR_ARG
-    assert lib.jb200_head_loss(C.byref(h), 4096, None, None, None, None) == _lib.ERR_ARG
+    assert lib.jb200_head_loss(C.byref(h), 4096, None, 4096, None, None, 4096, None) == _lib.ERR_ARG and "counts" in _lib.last_error()
+    assert lib.jb200_head_loss(C.byref(h), 4096, None, None, None, None, None, None) == _lib.ERR_ARG and "scratch" in _lib.last_error()
     for dx, dxt, dw, scratch, stride, text in ((4096, 2, 4096, 4096, 0, "dtype"), (4096, 1, 4112, 4096, 0, "32-byte"),
                                                (4112, 1, 4096, 4096, 0, "32-byte"), (4096, 1, 4096, 4100, 0, "256-byte"),
                                                (4096, 1, 4096, 4096, 2, "strides")):
