@@ -540,3 +540,40 @@ def test_first_call_of_a_thread():
         th.join()
     torch.cuda.synchronize()
     assert torch.equal(got[0][0], want[0]) and torch.equal(got[0][1], want[1]) and torch.equal(got[1], r.ce)
+
+
+def test_weights_beyond_two_to_the_31_elements():
+    """Offsets of weight, its gradient and the logits' gradients pass 32 bits: a weight of zeros but for rows near its end.  Logits of the
+    zero rows are 0, so their probabilities are one value a row and the definition needs the other rows alone."""
+    V, width, N = 1_060_003, 2048, 5
+    g = _gen(2)
+    w = torch.zeros(V, width, dtype=BF16, device="cuda")
+    far = torch.tensor([V - 1, V - 2, V - 300, V - 5000], device="cuda")
+    w[far] = (torch.randn(4, width, generator=g, device="cuda") / 30).bfloat16()
+    h = torch.randn(N, width, generator=g, device="cuda").bfloat16()
+    t = torch.tensor([V - 1, 3, -100, V - 300, V // 2], device="cuda")
+    z = h.double() @ w[far].double().t()
+    lse = torch.log(z.exp().sum(1) + (V - 4))
+    zt = torch.stack([z[0, 0], z[1, 0] * 0, z[2, 0] * 0, z[3, 2], z[4, 0] * 0])
+    x, wt = h.clone().requires_grad_(), w.requires_grad_()
+    rows = losses.linear_cross_entropy(x, wt, t, reduction="none")
+    Z = (width / 16 + 8) * 2.0 ** -23 * float((h.double().abs() @ w.detach()[far].double().abs().t()).max())
+    want = torch.where(t >= 0, lse - zt, 0.0)
+    assert ((rows.double() - want).abs() <= 2 * Z + 2.0 ** -20 * want.abs()).all()
+    dx, dw = torch.autograd.grad(rows.sum(), (x, wt))
+    p = (z - lse[:, None]).exp() * (t >= 0)[:, None]
+    flat = (-lse).exp() * (t >= 0)
+    dz = p.clone()
+    dz[0, 0] -= 1
+    dz[3, 2] -= 1
+    size = p.clone()
+    size[0, 0] += 1
+    size[3, 2] += 1
+    _check_grad(dx, dz @ w.detach()[far].double(), (2.0 ** -8 + 3 * Z + 2.0 ** -19 + (V / 16 + 72) * 2.0 ** -23) * (size @ w.detach()[far].double().abs()))
+    _check_grad(dw[far], dz.t() @ h.double(), (2.0 ** -8 + 3 * Z + 2.0 ** -18) * (size.t() @ h.double().abs()))
+    for row, n in ((3, 1), (V // 2, 4), (12345, None), (V - 10, None)):
+        col = flat.clone()
+        if n is not None:
+            col[n] -= 1
+        big = flat + (0 if n is None else (torch.arange(N, device="cuda") == n))
+        _check_grad(dw[row], col @ h.double(), (2.0 ** -8 + 3 * Z + 2.0 ** -18) * (big @ h.double().abs()))
