@@ -1,8 +1,8 @@
-// The products of the head's gradient, one launch per piece of the vocabulary:  dx += s G W  and  dW = s G^T xs,  where G (bf16, rows x piece)
-// is the gradient of the logits, relative to the factor s, that head_loss.cu's epilogue left.
+// The products of the head's gradient, one launch per piece of the vocabulary:  dx += s G W  and  dW = s G^T xs,  where G (f16, rows x piece)
+// is the gradient of the logits, relative to the factor s, that head_loss.cu's epilogue left, beside f16 copies of W and of the rows.
 //
 // CTA pairs as in the logits' kernel: 256 x 256 tiles, K-blocks of 64.  No operand is transposed in memory: G is the M operand K-major
-// for dx (rows x vocabulary) and MN-major for dW (read as vocabulary x rows), W and xs are the N operands MN-major, all from the
+// for dx (rows x vocabulary) and MN-major for dW (read as vocabulary x rows), the copies are the N operands MN-major, all from the
 // same kind of [64 rows][64 columns] boxes.  Both products are items of one list, the longer kind first, so that their last waves
 // fill each other's gaps.  Where there are few rows dx is summed over parts of the piece side by side, in slabs of their own, which a
 // launch of its own adds up in their order (done by the warps that store a tile last it took 30 us of 37 rows instead of 5).
@@ -135,7 +135,7 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
           } else {
             pair_tma_load_2d(a, &tmap_g, k, row, full);
             pair_tma_load_2d(a + BOX, &tmap_g, k, row + HEAD_BK, full);
-            for (int c = 0; c < boxes; ++c) pair_tma_load_2d(b + uint32_t(c) * BOX, &tmap_w, col + c * HEAD_BK, p.v0 + k, full);
+            for (int c = 0; c < boxes; ++c) pair_tma_load_2d(b + uint32_t(c) * BOX, &tmap_w, col + c * HEAD_BK, k, full);
           }
         }
         __syncwarp();
@@ -147,7 +147,7 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
     if (rank == 0) {
       // a K-step of 16: 32 bytes inside K-major rows, two groups of eight 128-byte rows of an MN-major block
       const uint64_t a_k = umma_desc_k_sw128(a_base), a_mn = umma_desc_mn_sw128(a_base, BOX), b_mn = umma_desc_mn_sw128(b_base, BOX);
-      const uint32_t idesc = umma_idesc_bf16(HEAD_TILE, p.width) + IDESC_B_MN;
+      const uint32_t idesc = umma_idesc_bf16(HEAD_TILE, p.width) + IDESC_F16 + IDESC_B_MN;
       int s = 0;
       uint32_t ph = 0u, tile = 0u;
       bool ok = true;
@@ -178,7 +178,8 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
   } else {
     // ---------------- epilogue: a lane is a row, its registers are channels ----------------
     const int quarter = warp & 3, half = (warp - HEAD_EPI_WARP0) >> 2;
-    const float scale = head_scale(p.grads);
+    const float common = head_scale(p.grads);
+    const float dx_scale = ldexpf(common, -HEAD_G_EXP - p.exps[0]), dw_scale = ldexpf(common, -HEAD_G_EXP - p.exps[1]);
     uint32_t tile = 0u;
     for (; head_item(p, pair, n_pairs, int(tile), &it); ++tile) {
       const uint32_t acc = tile & 1u;
@@ -195,6 +196,7 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
         tmem_ld_32x32(t_lane + c0, v);
         tmem_ld_wait();
         if (on) {
+          const float scale = it.is_dw ? dw_scale : dx_scale;
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(scale * __uint_as_float(v[j]));
           const int n = min(32, p.C - col);
@@ -255,7 +257,7 @@ int head_width(int C) {
   return ((C + tc - 1) / tc + 31) / 32 * 32;
 }
 
-int launch_head_products(HeadProducts p, const void* g, const void* xs, const void* w, int sms, cudaStream_t stream) {
+int launch_head_products(HeadProducts p, const void* g, const void* xs, const void* ws, int sms, cudaStream_t stream) {
   p.width = head_width(p.C);
   const int kb = (p.n_cols + HEAD_BK - 1) / HEAD_BK, kn = (p.N + HEAD_BK - 1) / HEAD_BK;
   p.all_slabs = p.slabs;
@@ -270,7 +272,7 @@ int launch_head_products(HeadProducts p, const void* g, const void* xs, const vo
   CUtensorMap tg, tw, tx;
   int rc;
   if ((rc = encode_head_map(&tg, g, p.ldg, p.ldg, p.N, HEAD_BK, "head_loss_backward (gradient of the logits)")) != JB200_OK) return rc;
-  if ((rc = encode_head_map(&tw, w, p.C, p.C, p.V, HEAD_BK, "head_loss_backward (weight)")) != JB200_OK) return rc;
+  if ((rc = encode_head_map(&tw, ws, p.C, head_pitch(p.C), p.n_cols, HEAD_BK, "head_loss_backward (weight)")) != JB200_OK) return rc;
   if ((rc = encode_head_map(&tx, xs, p.C, head_pitch(p.C), p.N, HEAD_BK, "head_loss_backward (rows)")) != JB200_OK) return rc;
   JB_MAX_SMEM(head_products_kernel, HEAD_SMEM);
   launch_dep_cluster(head_products_kernel, dim3(2 * unsigned(pairs)), dim3(HEAD_THREADS), HEAD_SMEM, 2, stream, tg, tw, tx, p);

@@ -9,13 +9,14 @@
 //
 // Forward: a product kernel whose epilogue keeps, per row of a 256 x 256 tile, the maximum, the sum of exponentials and the logits that
 // the target and the teacher ask for; a second kernel joins the tiles.  Backward: the same product again, whose epilogue writes dz
-// of a piece of the vocabulary as bf16 (the operand type of the products dx += dz W and dW = dz^T x that follow, head_grad.cu), so
+// of a piece of the vocabulary as f16 (an operand of the products dx += dz W and dW = dz^T x that follow, head_grad.cu), so
 // that the workspace stays bounded whatever the vocabulary: 8 N V C operations for a training step, where 6 N V C would need the
 // logits kept.
 //
 // Exponentials are base 2 with a whole number as the reference point: 2^(z k - r), k the f32 value next to log2(e), has one rounding in its
 // argument and rescaling by 2^(r - r') has none.  A row's sum travels as the pair (r, sum 2^(z k - r)), and logarithms are divided by
 // that very k, so that logits of any size keep their differences.
+#include <cuda_fp16.h>
 #include <float.h>
 #include <limits.h>
 
@@ -28,7 +29,7 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int TEACHER_MAX = 256;
-constexpr size_t PIECE_BYTES = size_t(320) << 20;      // bf16 gradients of the logits kept at a time, at most
+constexpr size_t PIECE_BYTES = size_t(320) << 20;      // gradients of the logits kept at a time, at most
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -168,10 +169,11 @@ struct HeadLogits {
   float* z_target;           // [N]
   unsigned int* ticket;      // set to 0 for the join
   HeadGrads grads;           // gradient
-  __nv_bfloat16* g;          // gradient: [N][ldg]
+  __half* g;                 // gradient: [N][ldg]
   int ldg;
-  const uint4* x;            // gradient: rows to copy, those without a loss as zeros
-  uint4* xs;                 // null: not to be copied
+  const uint4 *x, *w;        // gradient: rows and weight
+  uint4 *xs, *ws;            // their copies, the weight's of these columns; null: not wanted
+  int* exps;                 // exponents of the copies' factors, weight and rows: made by the first piece, read by the others
   int box_rows;              // rows of x that a CTA asks for at a time
   unsigned int* status;
 };
@@ -184,6 +186,11 @@ __device__ __forceinline__ void head_tile(int t, int tm, int tv, int* m, int* v)
   const int r = t - base * tv;
   *v = r / size;
   *m = base + r - *v * size;
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 __device__ __forceinline__ float pick32(const uint32_t (&v)[32], int j) {
@@ -273,29 +280,87 @@ __device__ __forceinline__ bool row_is_live(const HeadGrads& p, int row) {
   return (CE && p.targets[row] != -100) || (KD && p.neg_entropy[row] != INFINITY);
 }
 
-// Rows for dW's product, by two warps of every CTA beside the products: those that take no part become zeros, so that a NaN or an
-// infinity in one does not reach the others' sums.  Four rows a warp at a time.
-template <bool CE, bool KD>
-__device__ __forceinline__ void copy_rows(const HeadLogits& p, int warp, int lane) {
-  const int per_row = p.C / 8, pitch = head_pitch(p.C) / 8, step = int(gridDim.x) * 2 * 4;
-  for (int r0 = (int(blockIdx.x) * 2 + warp) * 4; r0 < p.N; r0 += step) {
-    bool live[4];
+// ---- f16 copies of the products' other operands, by eight warps of every CTA beside the products ----
+constexpr int COPY_WARPS = 8;
+
+// Largest finite magnitude, as bf16 bits, that this warp's share of the sample holds; rows that take no part are left out.
+template <typename Live>
+__device__ __forceinline__ unsigned sample_rows(const uint4* m, int n_rows, int per_row, int warp, int lane, Live live_row) {
+  unsigned top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) live[i] = r0 + i < p.N && row_is_live<CE, KD>(p.grads, r0 + i);
-    for (int c = lane; c < per_row; c += 64) {
-      uint4 v[4][2];
+  for (int i = 0; i < HEAD_SAMPLES / COPY_WARPS; ++i) {
+    const long long row = (long long)(i * COPY_WARPS + warp) * (n_rows - 1) / (HEAD_SAMPLES - 1);
+    if (!live_row(int(row))) continue;
+#pragma unroll 4
+    for (int c = lane; c < per_row; c += 32) {
+      const uint4 v = __ldg(m + row * per_row + c);
+      const unsigned a[4] = {v.x & 0x7fff7fffu, v.y & 0x7fff7fffu, v.z & 0x7fff7fffu, v.w & 0x7fff7fffu};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          v[i][u] = live[i] && c + 32 * u < per_row ? __ldg(p.x + size_t(r0 + i) * per_row + c + 32 * u) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (r0 + i < p.N && c + 32 * u < per_row) p.xs[size_t(r0 + i) * pitch + c + 32 * u] = v[i][u];
+      for (int j = 0; j < 4; ++j) top = __vmaxu2(top, a[j] & __vcmpltu2(a[j], 0x7f807f80u));
     }
   }
+  top = max(top & 0xffffu, top >> 16);
+  return __reduce_max_sync(0xffffffffu, top);
+}
+// Exponent of the factor that brings it to [1, 2); nothing but zeros (or subnormal numbers): 0.
+__device__ __forceinline__ int copy_exponent(unsigned top) {
+  const int e = int(top >> 7);
+  return e == 0 ? 0 : max(-100, min(100, 127 - e));
+}
+
+__device__ __forceinline__ uint32_t f16x2_of_bf16x2(uint32_t w, float factor) {
+  const __half2 h = __floats2half2_rn(bf16_lo(w) * factor, bf16_hi(w) * factor);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// With few rows of x the weight's copy is what the launch waits for (37 rows of 50257 x 1024: 47 us, with four warps 65).  Rows that take no
+// part become zeros, so that a NaN or an infinity in one does not reach the others' sums.
+template <typename Live>
+__device__ __forceinline__ void copy_f16(const uint4* src, uint4* dst, int n_rows, int C, float factor, int warp, int lane, Live live_row) {
+  constexpr int R = 4;
+  const int per_row = C / 8, pitch = head_pitch(C) / 8, step = int(gridDim.x) * COPY_WARPS * R;
+  for (int r0 = (int(blockIdx.x) * COPY_WARPS + warp) * R; r0 < n_rows; r0 += step) {
+    const bool live = lane < R && r0 + lane < n_rows && live_row(r0 + lane);
+    const unsigned rows = __ballot_sync(0xffffffffu, live);
+    for (int c = lane; c < per_row; c += 64) {
+      uint4 v[R][2];
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          v[i][u] = (rows >> i & 1u) && c + 32 * u < per_row ? __ldg(src + size_t(r0 + i) * per_row + c + 32 * u) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (r0 + i < n_rows && c + 32 * u < per_row)
+            dst[size_t(r0 + i) * pitch + c + 32 * u] = make_uint4(f16x2_of_bf16x2(v[i][u].x, factor), f16x2_of_bf16x2(v[i][u].y, factor),
+                                                                 f16x2_of_bf16x2(v[i][u].z, factor), f16x2_of_bf16x2(v[i][u].w, factor));
+    }
+  }
+}
+
+template <bool CE, bool KD>
+__device__ __forceinline__ void make_copies(const HeadLogits& p, unsigned* s_top, int warp, int lane) {
+  int ew, ex;
+  const auto live = [&](int row) { return row_is_live<CE, KD>(p.grads, row); };
+  const auto all = [](int) { return true; };
+  if (p.v0 == 0) {
+    const unsigned tw = p.ws ? sample_rows(p.w, p.V, p.C / 8, warp, lane, all) : 0u;
+    const unsigned tx = p.xs ? sample_rows(p.x, p.N, p.C / 8, warp, lane, live) : 0u;
+    if (lane == 0) { s_top[warp] = tw; s_top[COPY_WARPS + warp] = tx; }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * COPY_WARPS) : "memory");        // the copying warps alone, which wait for nothing else
+    unsigned mw = 0, mx = 0;
+#pragma unroll
+    for (int i = 0; i < COPY_WARPS; ++i) { mw = max(mw, s_top[i]); mx = max(mx, s_top[COPY_WARPS + i]); }
+    ew = copy_exponent(mw);
+    ex = copy_exponent(mx);
+    if (blockIdx.x == 0 && warp == 0 && lane == 0) { p.exps[0] = ew; p.exps[1] = ex; }
+  } else {
+    ew = p.exps[0];
+    ex = p.exps[1];
+  }
+  if (p.xs) copy_f16(p.x, p.xs, p.N, p.C, ldexpf(1.f, ex), warp, lane, live);
+  if (p.ws) copy_f16(p.w + size_t(p.v0) * (p.C / 8), p.ws, p.cols, p.C, ldexpf(1.f, ew), warp, lane, all);
 }
 
 template <bool CE, bool KD>
@@ -309,7 +374,7 @@ __device__ __forceinline__ void head_part(const HeadLogits& p, int part, int row
 // tiles, each the accumulator of its own (eight warps on every tile leave twice the parts to join).  A column of a row that the
 // teacher asks for is not known to the compiler: where a warp has one, 16 columns go through shared memory, lanes side by side (32
 // compared registers an entry cost 6 to 30 % of a launch at 32 to 64 entries a row).
-constexpr int logits_threads(bool grad) { return HEAD_THREADS + (grad ? 64 : 0); }
+constexpr int logits_threads(bool grad) { return HEAD_THREADS + (grad ? 32 * COPY_WARPS : 0); }
 
 template <bool CE, bool KD, bool GRAD>
 __global__ void __launch_bounds__(logits_threads(GRAD), 1)
@@ -395,11 +460,12 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
       }
     }
   } else if (GRAD && warp >= HEAD_EPI_WARP0 + 8) {
-    if (p.xs) copy_rows<CE, KD>(p, warp - HEAD_EPI_WARP0 - 8, lane);
+    __shared__ unsigned s_top[2 * COPY_WARPS];
+    make_copies<CE, KD>(p, s_top, warp - HEAD_EPI_WARP0 - 8, lane);
   } else {
     // ---------------- epilogue ----------------
     const int quarter = warp & 3;                              // TMEM lanes this warp may read
-    const float scale = GRAD ? head_scale(p.grads) : 1.f;
+    const float scale = GRAD ? head_scale(p.grads) * (1.f / (1 << HEAD_G_EXP)) : 1.f;
     const uint32_t group = uint32_t(warp - HEAD_EPI_WARP0) >> 2;
     // [16 columns][32 lanes] of this warp
     float* stage = reinterpret_cast<float*>(behind + HEAD_CTL) + (warp - HEAD_EPI_WARP0) * 512 + lane;
@@ -471,8 +537,8 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
           if (on) {
             uint32_t w[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = rg.live ? pack_bf16x2(g[2 * j], g[2 * j + 1]) : 0u;
-            __nv_bfloat16* d = p.g + size_t(row) * p.ldg + (col - p.v0);
+            for (int j = 0; j < 16; ++j) w[j] = rg.live ? pack_f16x2(g[2 * j], g[2 * j + 1]) : 0u;
+            __half* d = p.g + size_t(row) * p.ldg + (col - p.v0);
             st_global_256(d, w);
             st_global_256(d + 16, w + 8);
           }
@@ -904,12 +970,14 @@ int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* mean_ce, 
 
 namespace {
 struct BackwardScratch {
-  size_t xs, scale, g, slabs, total;
+  size_t xs, ws, scale, exps, g, slabs, total;
 };
 BackwardScratch backward_scratch(int N, int C, const HeadPlan& pl) {
   BackwardScratch s;
   s.xs = 0;
-  s.scale = up256(size_t(N) * head_pitch(C) * 2);
+  s.ws = up256(size_t(N) * head_pitch(C) * 2);
+  s.scale = s.ws + up256(size_t(pl.cols) * head_pitch(C) * 2);
+  s.exps = s.scale + 16;
   s.g = s.scale + 256;
   s.slabs = s.g + up256(size_t(N) * pl.cols * 2);
   s.total = s.slabs + up256(size_t(pl.slabs) * N * C * 4);
@@ -960,9 +1028,13 @@ int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_s
   p.targets = h->targets; p.inv_tau = 1.0f / r.tau;
   set_teacher(p, h);
   p.grads = r;
-  p.g = reinterpret_cast<__nv_bfloat16*>(base + at.g);
+  p.g = reinterpret_cast<__half*>(base + at.g);
   p.ldg = pl.cols;
-  if (dw) { p.x = static_cast<const uint4*>(h->x); p.xs = reinterpret_cast<uint4*>(base + at.xs); }
+  p.x = static_cast<const uint4*>(h->x);
+  p.w = static_cast<const uint4*>(h->w);
+  if (dw) p.xs = reinterpret_cast<uint4*>(base + at.xs);
+  if (dx) p.ws = reinterpret_cast<uint4*>(base + at.ws);
+  p.exps = reinterpret_cast<int*>(base + at.exps);
   HeadProducts q{};
   p.status = device_status_ptr();
   if (!p.status) return JB200_ERR_CUDA;
@@ -973,6 +1045,7 @@ int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_s
   q.N = h->N; q.V = h->V; q.C = h->C;
   q.ldg = pl.cols;
   q.grads = r;
+  q.exps = p.exps;
   q.dx = dx; q.dx_bf16 = dx_dtype;
   // one slab in f32 is the result itself
   q.dx_slabs = !dx ? nullptr : dx_dtype == 0 && pl.slabs == 1 ? static_cast<float*>(dx) : reinterpret_cast<float*>(base + at.slabs);
@@ -985,7 +1058,7 @@ int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_s
     q.first = i == 0;
     q.last = i + 1 == pl.pieces;
     if ((rc = launch_logits<true>(h->targets != nullptr, h->teacher != nullptr, tx, tw, p, sms, stream)) != JB200_OK) return rc;
-    if ((rc = launch_head_products(q, p.g, base + at.xs, h->w, sms, stream)) != JB200_OK) return rc;
+    if ((rc = launch_head_products(q, p.g, base + at.xs, base + at.ws, sms, stream)) != JB200_OK) return rc;
     p.xs = nullptr;
   }
   return JB200_OK;

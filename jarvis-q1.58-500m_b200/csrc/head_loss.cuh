@@ -26,12 +26,10 @@ struct HeadGrads {
 };
 
 #if defined(__CUDACC__)
-// The gradients of the logits are kept relative to one factor of the whole call, which the products apply to their f32 sums: rows of a
-// mean then have the factor 1, and a target of small probability -1, which bf16 holds.  (With 1 / rows in them that entry, half of a
-// row's gradient, had the same rounding in every row: an error of up to 2^-8 of dx and dW, and no noise that averages out.)
+// The gradients of the logits are kept relative to one factor of the whole call, the largest there is, which the products apply to their
+// f32 sums.  (With 1 / rows in them a target's entry, -1 / rows and half of a row's gradient, had the same rounding in every row.)
 __device__ __forceinline__ float common_factor(float ce, float kd) {
-  const bool by_ce = ce > 0.f && ce <= 3.4e38f && !(kd > ce * 1e18f);
-  const float s = by_ce ? ce : kd;
+  const float s = ce <= 3.4e38f && !(kd <= 3.4e38f && kd > ce) ? ce : kd;
   return s > 0.f && s <= 3.4e38f ? s : 1.f;
 }
 __device__ __forceinline__ float row_factor(const float* g, int stride, const float* n, int row) {
@@ -44,8 +42,15 @@ __device__ __forceinline__ float head_scale(const HeadGrads& p) {
 }
 #endif
 
+// Operands of the gradient's products are f16, whose rounding is an eighth of bf16's: the logits' gradients times 2^13 (at most 2 of them
+// add up to 2^14; they keep all their bits down to 2^-27 and vanish below 2^-38), and copies of weight and rows times powers of two by
+// which 16 rows of each, taken evenly, have their largest value in [1, 2).  A bf16 value within 2^17 of that is exact there, a smaller one
+// off by at most 2^-25 of the largest, one 2^15 times larger overflows.  (As bf16 the logits' gradients gave dx and dW an error
+// of sqrt(2) times their own rounding.)
+constexpr int HEAD_G_EXP = 13, HEAD_SAMPLES = 16;
+
 // How a backward pass is cut: `pieces` pieces of `cols` vocabulary columns (the last one shorter) whose gradients of the logits are
-// kept as bf16, and `slabs` parts of a piece over which the hidden rows' gradient is summed side by side.
+// kept at a time, and `slabs` parts of a piece over which the hidden rows' gradient is summed side by side.
 struct HeadPlan {
   int cols, pieces, slabs;
 };
@@ -73,9 +78,9 @@ __host__ __device__ __forceinline__ int head_walk(const HeadShares& s, int n_lon
   return t < n_short ? n_long + t : -1;
 }
 
-// Boxes of 64 columns of a bf16 matrix whose rows are `pitch` elements apart.
+// Boxes of 64 columns of a bf16 or f16 matrix whose rows are `pitch` elements apart.
 int encode_head_map(CUtensorMap* tm, const void* ptr, long long cols, long long pitch, long long rows, int box_rows, const char* what);
-// Pitch of the copied rows: whole 128-byte lines, where a box's rows are one line each.
+// Pitch of the copies: whole 128-byte lines, where a box's rows are one line each.
 __host__ __device__ inline int head_pitch(int C) { return (C + HEAD_BK - 1) / HEAD_BK * HEAD_BK; }
 
 // dx += scale G W and dw = scale G^T xs of one piece (head_grad.cu); a null one is not wanted.
@@ -86,6 +91,7 @@ struct HeadProducts {
   int slabs;
   int first, last;           // of the pieces
   HeadGrads grads;
+  const int* exps;           // [2]: exponents of the factors of the weight's copy and of the rows'
   float* dx_slabs;           // [slabs][N][C] f32: sums so far; may be dx itself
   void* dx;                  // [N][C], written by the last piece
   int dx_bf16;
@@ -100,6 +106,7 @@ struct HeadProducts {
   unsigned int* status;
 };
 int head_width(int C);
-int launch_head_products(HeadProducts p, const void* g, const void* xs, const void* w, int sms, cudaStream_t stream);
+// g: f16 [N][ldg]; xs, ws: the f16 copies of rows and of the piece's weight, head_pitch(C) apart.
+int launch_head_products(HeadProducts p, const void* g, const void* xs, const void* ws, int sms, cudaStream_t stream);
 
 }  // namespace jb

@@ -126,6 +126,7 @@ __device__ __forceinline__ void pair_ring_close(uint32_t tmem, int warp) {
 __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t block) {
   return (umma_desc_k_sw128(smem_addr) & ~(uint64_t(0x3FFF) << 16)) | uint64_t(block >> 4) << 16;
 }
+constexpr uint32_t IDESC_F16 = 0u - (1u << 7) - (1u << 10);         // added to umma_idesc_bf16: both operands f16
 constexpr uint32_t IDESC_A_MN = 1u << 15, IDESC_B_MN = 1u << 16;      // operand read MN-major (with umma_idesc_bf16)
 
 }  // namespace jb

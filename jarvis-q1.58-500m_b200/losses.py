@@ -13,8 +13,8 @@ autograd).  A captured training step takes its gradients with torch.autograd.gra
 holds the same parameters' accumulators; the operators themselves launch on the current stream and synchronise with nothing.
 
 Numerics: hidden rows and weight enter the products as bf16 (an f32 argument is rounded to it, as under autocast), sums and softmax are
-f32, the gradient of the logits is rounded to bf16 for the products it enters, gradients are returned in their argument's
-dtype from f32 sums.
+f32, the gradient of the logits is rounded to f16 for the products it enters (2^-11 of a value, relative to the call's largest factor
+down to 2^-38), gradients are returned in their argument's dtype from f32 sums.
 """
 from __future__ import annotations
 

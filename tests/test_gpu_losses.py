@@ -5,9 +5,11 @@ How far results may lie from those is bounded element by element from the roundi
            sum inside a group: Z = (C / 16 + 8) 2^-23 max sum |x w|
   losses   a log of a sum whose terms move by a factor exp(+-Z), and the target's logit: 2 Z, plus 2^-22 of the value (f32 logarithm,
            storage); a temperature divides Z and its square multiplies the loss
-  dz       e^2Z - 1 < 3 Z of the probability (plus 2^-20 for the exponential and its argument), then bf16: 2^-8
-  dx, dW   the products of those: |error| <= (2^-8 + 3 Z + 2^-19) sum |dz| |operand|, plus the f32 sum (terms / 16 + 72) 2^-23 of the same
-           sum, plus the result's own rounding, 2^-8 for bf16
+  dz       e^2Z - 1 < 3 Z of the probability (plus 2^-20 for the exponential and its argument), then f16 relative to 2^-13 of the largest
+           factor: 2^-11, and 2^-38 of that factor where f16 is subnormal
+  dx, dW   the products of those: |error| <= (2^-11 + 3 Z + 2^-19) sum |dz| |operand|, plus the f32 sum (terms / 16 + 72) 2^-23 of the same
+           sum, plus what f16 takes from the other operand, at most 2^-25 of its largest value each, plus the result's own
+           rounding, 2^-8 for bf16
 where sum |dz| |operand| takes the positive and the negative parts of dz apart (a probability and a target of the same entry cancel only
 after the first has been rounded).
 """
@@ -73,9 +75,12 @@ def _definition(h, w, t, ids, logits, tau, g_ce, g_kd):
         dz = dz + f * (lp.exp() - full)
     out["dx"], out["dw"] = dz @ wd, dz.t() @ x
     size = pos + neg
-    rel = 2.0 ** -8 + 3 * Z + 2.0 ** -19
-    out["dx_bound"] = (rel + (w.shape[0] / 16 + 72) * 2.0 ** -23) * (size @ wd.abs())
-    out["dw_bound"] = (rel + (N / 16 + 72) * 2.0 ** -23) * (size.t() @ x.abs())
+    rel = 2.0 ** -11 + 3 * Z + 2.0 ** -19
+    factor = max(0.0 if t is None else float((g_ce.abs() * (t != -100)).max()), 0.0 if ids is None else float(g_kd.abs().max()) * tau)
+    out["dx_bound"] = (rel + (w.shape[0] / 16 + 72) * 2.0 ** -23) * (size @ wd.abs()) + 2.0 ** -25 * wd.abs().max() * size.sum(1, keepdim=True) + \
+        2.0 ** -38 * factor * wd.abs().sum(0)
+    out["dw_bound"] = (rel + (N / 16 + 72) * 2.0 ** -23) * (size.t() @ x.abs()) + 2.0 ** -25 * x.abs().max() * size.sum(0)[:, None] + \
+        2.0 ** -38 * factor * x.abs().sum(0)
     return out
 
 
@@ -201,6 +206,24 @@ def test_rows_that_have_no_part():
     ce, kd = losses.linear_losses(xc, wc, t, ids, logits)
     want = torch.autograd.grad(ce + kd, (xc, wc))
     assert torch.equal(dw, want[1]) and torch.equal(dx, want[0])
+
+
+def test_operands_of_any_scale():
+    """The f16 copies of the products' operands follow the operands' size: the gradients of scaled rows and weights are the scaled gradients,
+    to the bit where the scales are powers of two and the logits the same; large values in rows that take no part change nothing."""
+    h, w, t, ids, logits = _problem(60, 700, 128, 6)
+    t[1::3], ids[1::3] = -100, -1
+    ref = None
+    for k in (0, -20, 20, -60, 60):
+        x, wt = (h * 2.0 ** k).requires_grad_(), (w * 2.0 ** -k).requires_grad_()
+        with torch.no_grad():
+            x[1::3] = 3e38
+        ce, kd = losses.linear_losses(x, wt, t, ids, logits)
+        dx, dw = torch.autograd.grad(ce + kd, (x, wt))
+        got = (ce, kd, dx * 2.0 ** k, dw * 2.0 ** -k)
+        ref = ref or got
+        for a, b in zip(got, ref):
+            assert torch.equal(a, b)
 
 
 def test_nothing_to_learn_from():
@@ -494,7 +517,7 @@ def test_model_losses():
     hd, wd = hidden.double(), model.lm_head.weight.detach().bfloat16().double().requires_grad_()
     ref = torch.nn.functional.cross_entropy(hd @ wd.t(), y.view(-1))
     dref, = torch.autograd.grad(ref, wd)
-    assert abs(float(ce) - float(ref)) <= 1e-5 * float(ref)
+    assert abs(float(ce) - ref.item()) <= 1e-5 * ref.item()
     assert (named["lm_head.weight"].double() - dref).norm() <= 2.0 ** -8 * dref.norm()      # dz's rounding alone
     # the kernel-by-kernel path has the same
     model.use_chain = False
@@ -569,11 +592,13 @@ def test_weights_beyond_two_to_the_31_elements():
     size = p.clone()
     size[0, 0] += 1
     size[3, 2] += 1
-    _check_grad(dx, dz @ w.detach()[far].double(), (2.0 ** -8 + 3 * Z + 2.0 ** -19 + (V / 16 + 72) * 2.0 ** -23) * (size @ w.detach()[far].double().abs()))
-    _check_grad(dw[far], dz.t() @ h.double(), (2.0 ** -8 + 3 * Z + 2.0 ** -18) * (size.t() @ h.double().abs()))
+    wf, hd = w.detach()[far].double(), h.double()
+    _check_grad(dx, dz @ wf, (2.0 ** -11 + 3 * Z + 2.0 ** -18) * (size @ wf.abs()) + 2.0 ** -25 * wf.abs().max() * size.sum(1, keepdim=True))
+    rel, floor = 2.0 ** -11 + 3 * Z + 2.0 ** -18, 2.0 ** -25 * hd.abs().max()
+    _check_grad(dw[far], dz.t() @ hd, rel * (size.t() @ hd.abs()) + floor * size.sum(0)[:, None])
     for row, n in ((3, 1), (V // 2, 4), (12345, None), (V - 10, None)):
         col = flat.clone()
         if n is not None:
             col[n] -= 1
         big = flat + (0 if n is None else (torch.arange(N, device="cuda") == n))
-        _check_grad(dw[row], col @ h.double(), (2.0 ** -8 + 3 * Z + 2.0 ** -18) * (big @ h.double().abs()))
+        _check_grad(dw[row], col @ hd, rel * (big @ hd.abs()) + floor * big.sum())
