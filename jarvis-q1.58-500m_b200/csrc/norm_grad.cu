@@ -4,7 +4,8 @@
 //
 // Nothing of the forward is needed but x: both sums of a row come from the values that its dx needs anyway.  Bound by HBM: x and dy
 // are read once, dx written once.  A row belongs to as many warps as it has thousands of channels; a lane keeps its channels' sums
-// of dw in registers over all rows it sees, the CTAs' sums are added in a fixed order by a second launch.
+// of dw in registers over all rows it sees, the CTAs' sums are added in a fixed order: by a second launch, or, of few rows, by a
+// cluster that has them all.
 #include "common.cuh"
 #include "launchers.h"
 
@@ -32,8 +33,14 @@ __device__ __forceinline__ void ng_store8(__nv_bfloat16* p, const float (&v)[8])
   *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
-// WPR: warps of a row (1, 2 or 4).
-template <typename TX, typename TY, int WPR>
+__device__ __forceinline__ float cluster_ld(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// WPR: warps of a row (1, 2 or 4).  ONE: the grid is one cluster and leaves dw itself in dw_part.
+template <typename TX, typename TY, int WPR, bool ONE>
 __global__ void __launch_bounds__(32 * NG_WARPS, 2)
 rmsnorm_backward_kernel(const TX* __restrict__ x, const float* __restrict__ w, float eps, const TY* __restrict__ dy, int n_rows, int C,
                         TX* __restrict__ dx, float* __restrict__ dw_part) {
@@ -121,7 +128,23 @@ rmsnorm_backward_kernel(const TX* __restrict__ x, const float* __restrict__ w, f
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) sum += s_dw[i * WPR + pt][at];
-    dw_part[size_t(blockIdx.x) * C + c] = sum;
+    if constexpr (ONE) s_dw[pt][at] = sum;
+    else dw_part[size_t(blockIdx.x) * C + c] = sum;
+  }
+  if constexpr (ONE) {
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    for (int c = int(blockIdx.x) * 32 * NG_WARPS + threadIdx.x; c < C; c += int(gridDim.x) * 32 * NG_WARPS) {
+      const int pt = c / NG_SPAN, in = c % NG_SPAN, at = (in & ~255) + (in & 7) * 32 + (in >> 3 & 31);
+      const uint32_t addr = smem_u32(&s_dw[pt][at]);
+      float sum = 0.f;
+      for (int r = 0; r < int(gridDim.x); ++r) sum += cluster_ld(cluster_map(addr, uint32_t(r)));
+      dw_part[c] = sum;
+    }
+    __syncwarp();
+    cluster_arrive();               // none leaves while another reads its sums
+    cluster_wait();
   }
 }
 
@@ -147,15 +170,37 @@ int norm_ctas(int n_rows, int C, int sms) {
   const long long rows = NG_WARPS / norm_warps(C), n = (n_rows + rows - 1) / rows;
   return int(n < 2 * sms ? n : 2 * sms);
 }
+// CTAs of the one cluster that takes all rows, 0 where there are too many.  A turn of its warps takes 3 us: 128 rows of 1024 channels 11.7 us,
+// 256 rows 15 us, where two launches take 11 us of the device but 5 us more of the host, which few rows wait for.
+constexpr int NG_ONE_TURNS = 4;                       // rows that a warp of it takes one after the other
+int norm_cluster(int n_rows, int C) {
+  const int rows = NG_WARPS / norm_warps(C);
+  if (n_rows > 8 * rows * NG_ONE_TURNS) return 0;
+  int n = 1;
+  while (n < 8 && n * rows < n_rows) n *= 2;
+  return n;
+}
 
+template <typename TX, typename TY, bool ONE>
+auto norm_kernel(int wpr) {
+  return wpr == 1 ? rmsnorm_backward_kernel<TX, TY, 1, ONE> : wpr == 2 ? rmsnorm_backward_kernel<TX, TY, 2, ONE> : rmsnorm_backward_kernel<TX, TY, 4, ONE>;
+}
 template <typename TX, typename TY>
-int launch_rmsnorm_backward_t(const void* x, const float* w, float eps, const void* dy, int n_rows, int C, void* dx, float* part, int ctas,
+int launch_rmsnorm_backward_t(const void* x, const float* w, float eps, const void* dy, int n_rows, int C, void* dx, float* dw, float* part, int sms,
                               cudaStream_t stream) {
-  const int wpr = norm_warps(C);
-  auto kernel = wpr == 1 ? rmsnorm_backward_kernel<TX, TY, 1> : wpr == 2 ? rmsnorm_backward_kernel<TX, TY, 2> : rmsnorm_backward_kernel<TX, TY, 4>;
-  launch_dep(kernel, ctas, 32 * NG_WARPS, 0, stream, static_cast<const TX*>(x), w, eps, static_cast<const TY*>(dy), n_rows, C,
+  const int wpr = norm_warps(C), cluster = norm_cluster(n_rows, C);
+  if (cluster) {
+    launch_dep_cluster(norm_kernel<TX, TY, true>(wpr), cluster, 32 * NG_WARPS, 0, cluster, stream, static_cast<const TX*>(x), w, eps,
+                       static_cast<const TY*>(dy), n_rows, C, static_cast<TX*>(dx), dw);
+    JB_LAUNCH_CHECK("rmsnorm_backward_kernel");
+    return JB200_OK;
+  }
+  const int ctas = norm_ctas(n_rows, C, sms);
+  launch_dep(norm_kernel<TX, TY, false>(wpr), ctas, 32 * NG_WARPS, 0, stream, static_cast<const TX*>(x), w, eps, static_cast<const TY*>(dy), n_rows, C,
              static_cast<TX*>(dx), part);
   JB_LAUNCH_CHECK("rmsnorm_backward_kernel");
+  launch_dep(rmsnorm_dw_kernel, (C + 31) / 32, 1024, 0, stream, part, ctas, C, dw);
+  JB_LAUNCH_CHECK("rmsnorm_dw_kernel");
   return JB200_OK;
 }
 
@@ -163,7 +208,7 @@ int launch_rmsnorm_backward_t(const void* x, const float* w, float eps, const vo
 
 size_t rmsnorm_backward_scratch_bytes(int n_rows, int C) {
   const int sms = sm_count();
-  if (n_rows < 1 || C < 1 || C > 4 * NG_SPAN || sms < 1) return 0;
+  if (n_rows < 1 || C < 1 || C > 4 * NG_SPAN || sms < 1 || norm_cluster(n_rows, C)) return 0;
   return size_t(norm_ctas(n_rows, C, sms)) * C * 4;
 }
 
@@ -177,22 +222,16 @@ int launch_rmsnorm_backward(const void* x, int x_dtype, const float* w, float ep
     JB_CUDA(cudaMemsetAsync(dw, 0, size_t(C) * 4, stream));
     return JB200_OK;
   }
-  JB_REQUIRE(x && w && dy && dx && scratch, "rmsnorm_backward: null pointer");
+  JB_REQUIRE(x && w && dy && dx && (scratch || norm_cluster(n_rows, C)), "rmsnorm_backward: null pointer");
   JB_REQUIRE(aligned16(x) && aligned16(w) && aligned16(dy) && aligned16(dx), "rmsnorm_backward: pointers must be 16-byte aligned");
   const int sms = sm_count();
   if (sms < 1) return JB200_ERR_CUDA;
-  const int ctas = norm_ctas(n_rows, C, sms);
   float* part = static_cast<float*>(scratch);
   typedef __nv_bfloat16 b16;
-  int rc;
-  if (x_dtype == 0 && dy_dtype == 0) rc = launch_rmsnorm_backward_t<float, float>(x, w, eps, dy, n_rows, C, dx, part, ctas, stream);
-  else if (x_dtype == 0) rc = launch_rmsnorm_backward_t<float, b16>(x, w, eps, dy, n_rows, C, dx, part, ctas, stream);
-  else if (dy_dtype == 0) rc = launch_rmsnorm_backward_t<b16, float>(x, w, eps, dy, n_rows, C, dx, part, ctas, stream);
-  else rc = launch_rmsnorm_backward_t<b16, b16>(x, w, eps, dy, n_rows, C, dx, part, ctas, stream);
-  if (rc != JB200_OK) return rc;
-  launch_dep(rmsnorm_dw_kernel, (C + 31) / 32, 1024, 0, stream, part, ctas, C, dw);
-  JB_LAUNCH_CHECK("rmsnorm_dw_kernel");
-  return JB200_OK;
+  if (x_dtype == 0 && dy_dtype == 0) return launch_rmsnorm_backward_t<float, float>(x, w, eps, dy, n_rows, C, dx, dw, part, sms, stream);
+  if (x_dtype == 0) return launch_rmsnorm_backward_t<float, b16>(x, w, eps, dy, n_rows, C, dx, dw, part, sms, stream);
+  if (dy_dtype == 0) return launch_rmsnorm_backward_t<b16, float>(x, w, eps, dy, n_rows, C, dx, dw, part, sms, stream);
+  return launch_rmsnorm_backward_t<b16, b16>(x, w, eps, dy, n_rows, C, dx, dw, part, sms, stream);
 }
 
 }  // namespace jb

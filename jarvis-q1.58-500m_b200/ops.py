@@ -266,7 +266,7 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, out_dtype=
         raise RuntimeError("rmsnorm: expected a contiguous CUDA tensor")
     _need(weight, torch.float32, "rmsnorm.weight")
     C = x.shape[-1]
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    y = torch.empty_like(x, dtype=out_dtype)
     _lib.check(lib.jb200_rmsnorm(_ptr(x), _dt(x), _ptr(weight), eps, _ptr(y), _dt(y), x.numel() // C, C, _stream()),
                "jb200_rmsnorm")
     return y
@@ -570,12 +570,9 @@ def _together(what: str, first: torch.Tensor, *others):
             raise RuntimeError(f"{what}: tensors on {first.device} and {t.device}")
 
 
-def _launch(on: torch.Tensor, fn, *args) -> int:
-    """fn(*args, stream) on the device of `on`, on that device's current stream."""
-    if _raw_device is not None and on.get_device() == _raw_device():
-        return fn(*args, _stream())
-    with torch.cuda.device(on.device):
-        return fn(*args, _stream())
+def _elsewhere(t: torch.Tensor) -> bool:
+    """True where `t` is not on the current device: the call is then made again with the tensor's device current."""
+    return t.get_device() != (_raw_device() if _raw_device is not None else torch.cuda.current_device())
 
 
 class TeacherRows:
@@ -601,10 +598,13 @@ def teacher_rows(ids: torch.Tensor, logits: torch.Tensor, vocab: int, temperatur
     if ids.dim() != 2 or logits.shape != ids.shape:
         raise RuntimeError(f"teacher_rows: ids {tuple(ids.shape)} and logits {tuple(logits.shape)} must be (N, K) alike")
     _together("teacher_rows", ids, logits)
+    if _elsewhere(ids):
+        with torch.cuda.device(ids.device):
+            return teacher_rows(ids, logits, vocab, temperature)
     N, K = ids.shape
     t = TeacherRows(torch.empty(lib.jb200_teacher_rows_bytes(N, K, vocab), dtype=torch.uint8, device=ids.device), N, K, int(vocab),
                     float(temperature))
-    _lib.check(_launch(ids, lib.jb200_teacher_rows, ids.data_ptr(), logits.data_ptr(), dt, N, K, t.vocab, t.temperature, t.buf.data_ptr()),
+    _lib.check(lib.jb200_teacher_rows(ids.data_ptr(), logits.data_ptr(), dt, N, K, t.vocab, t.temperature, t.buf.data_ptr(), _stream()),
                "jb200_teacher_rows")
     return t
 
@@ -653,6 +653,9 @@ def head_loss(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor | None = N
     from `teacher`, or both.  x: bf16 (N, C); w: bf16 (V, C), any V (no padding needed), C a multiple of 8 and at least 64."""
     lib = _lib.load()
     h = _head(x, w, targets, teacher, "head_loss")
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return head_loss(x, w, targets, teacher, want_rows=want_rows, want_means=want_means)
     N, dev, f32 = h.N, x.device, torch.float32
     has_ce, has_kd = targets is not None, teacher is not None
     r = HeadLoss(N, torch.empty(4 * N + 2, dtype=f32, device=dev), (has_ce, has_kd, want_means))
@@ -674,7 +677,7 @@ def head_loss(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor | None = N
             r.mean_kd = torch.empty((), dtype=f32, device=dev)
             p[3] = r.mean_kd.data_ptr()
     scratch = torch.empty(lib.jb200_head_loss_scratch_bytes(N, h.V, has_ce, has_kd), dtype=torch.uint8, device=dev)
-    _lib.check(_launch(x, lib.jb200_head_loss, ctypes.byref(h), *p, at + 16 * N if want_means else None, scratch.data_ptr()), "jb200_head_loss")
+    _lib.check(lib.jb200_head_loss(ctypes.byref(h), *p, at + 16 * N if want_means else None, scratch.data_ptr(), _stream()), "jb200_head_loss")
     return r
 
 
@@ -694,7 +697,11 @@ def head_loss_backward(x: torch.Tensor, w: torch.Tensor, fwd: HeadLoss, targets:
     f32 scalars for the means of `fwd`; else f32 (N,) for the rows' losses.  One that is not wanted is not computed and None."""
     lib = _lib.load()
     h = _head(x, w, targets, teacher, "head_loss_backward")
-    N, dev = h.N, x.device
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return head_loss_backward(x, w, fwd, targets, teacher, g_ce=g_ce, g_kd=g_kd, mean=mean, dx_dtype=dx_dtype, dw_dtype=dw_dtype,
+                                      want_dx=want_dx, want_dw=want_dw)
+    N = h.N
     has_ce, has_kd = targets is not None, teacher is not None
     if fwd.N != N or fwd.info[:2] != (has_ce, has_kd) or (mean and not fwd.info[2]):
         raise RuntimeError("head_loss_backward: `fwd` is not the forward call's result for these arguments")
@@ -708,16 +715,12 @@ def head_loss_backward(x: torch.Tensor, w: torch.Tensor, fwd: HeadLoss, targets:
         pk = _loss_gradient(g_kd, 1 if mean else N, "g_kd")
         nk = at + 16 * N + 4 if mean else None
     _together("head_loss_backward", x, fwd.buf, g_ce, g_kd)
-    dx = torch.empty((N, h.C), dtype=dx_dtype, device=dev) if want_dx else None
-    dw = torch.empty((h.V, h.C), dtype=dw_dtype, device=dev) if want_dw else None
-    tx, tw = (1 if dx is None else _dt(dx)), (1 if dw is None else _dt(dw))
+    dx = torch.empty_like(x, dtype=dx_dtype) if want_dx else None
+    dw = torch.empty_like(w, dtype=dw_dtype) if want_dw else None
     stride = 0 if mean else 1
-
-    def run(stream):
-        scratch = torch.empty(lib.jb200_head_loss_backward_scratch_bytes(N, h.V, h.C), dtype=torch.uint8, device=dev)
-        return lib.jb200_head_loss_backward(ctypes.byref(h), pc, stride, nc, pk, stride, nk, _ptr(dx), tx, _ptr(dw), tw, scratch.data_ptr(),
-                                            stream)
-    _lib.check(_launch(x, run), "jb200_head_loss_backward")
+    scratch = torch.empty(lib.jb200_head_loss_backward_scratch_bytes(N, h.V, h.C), dtype=torch.uint8, device=x.device)
+    _lib.check(lib.jb200_head_loss_backward(ctypes.byref(h), pc, stride, nc, pk, stride, nk, _ptr(dx), 1 if dx is None else _dt(dx), _ptr(dw),
+                                            1 if dw is None else _dt(dw), scratch.data_ptr(), _stream()), "jb200_head_loss_backward")
     return dx, dw
 
 
@@ -732,15 +735,15 @@ def rmsnorm_backward(x: torch.Tensor, weight: torch.Tensor, dy: torch.Tensor, ep
     if dy.shape != x.shape or weight.numel() != width:
         raise RuntimeError(f"rmsnorm_backward: x {tuple(x.shape)}, dy {tuple(dy.shape)}, weight {tuple(weight.shape)} do not belong together")
     _together("rmsnorm_backward", x, weight, dy)
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return rmsnorm_backward(x, weight, dy, eps)
     rows = x.numel() // width if width else 0
-    dx = torch.empty_like(x)
-    dw = torch.empty(width, dtype=torch.float32, device=x.device)
-
-    def run(stream):
-        scratch = torch.empty(lib.jb200_rmsnorm_backward_scratch_bytes(rows, width), dtype=torch.uint8, device=x.device)
-        return lib.jb200_rmsnorm_backward(x.data_ptr(), tx, weight.data_ptr(), eps, dy.data_ptr(), ty, rows, width, dx.data_ptr(), dw.data_ptr(),
-                                          scratch.data_ptr(), stream)
-    _lib.check(_launch(x, run), "jb200_rmsnorm_backward")
+    dx, dw = torch.empty_like(x), torch.empty_like(weight)
+    nbytes = lib.jb200_rmsnorm_backward_scratch_bytes(rows, width)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    _lib.check(lib.jb200_rmsnorm_backward(x.data_ptr(), tx, weight.data_ptr(), eps, dy.data_ptr(), ty, rows, width, dx.data_ptr(), dw.data_ptr(),
+                                          _ptr(scratch), _stream()), "jb200_rmsnorm_backward")
     return dx, dw
 
 
