@@ -312,7 +312,8 @@ __device__ __forceinline__ uint32_t f16x2_of_bf16x2(uint32_t w, float factor) {
   const __half2 h = __floats2half2_rn(bf16_lo(w) * factor, bf16_hi(w) * factor);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// With few rows of x the weight's copy is what the launch waits for (37 rows of 50257 x 1024: 47 us, with four warps 65).  Rows that take no
+// With few rows of x the weight's copy is what the launch waits for (37 rows of 50257 x 1024: 47 us where the logits alone take 26, and
+// HBM 32 for the weight and its copy; four warps: 65; loads ahead of the conversion, or each CTA the rows that its products read: no change).  Rows that take no
 // part become zeros, so that a NaN or an infinity in one does not reach the others' sums.
 template <typename Live>
 __device__ __forceinline__ void copy_f16(const uint4* src, uint4* dst, int n_rows, int C, float factor, int warp, int lane, Live live_row) {
@@ -622,25 +623,24 @@ __device__ __forceinline__ void join_lanes(float& ref, float& sum, int o) {
   join(ref, sum, r, s);
 }
 
-// A CTA takes 32 rows: lanes are rows while the parts are read (each warp every 32nd of them), then every warp joins one row's 32 sums.
-// The CTA that ends last forms the means over all rows in a fixed order: thread, warp, warps.
-constexpr int JOIN_WARPS = 32;
-
-template <bool CE, bool KD>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) head_join_kernel(const __grid_constant__ HeadRowsOut p) {
+// A CTA takes 32 rows: lanes are rows while the parts are read (WARPS of them at a time), then a warp joins the WARPS sums of 32 / WARPS rows.
+// The CTA that ends last forms the means over all rows in a fixed order: thread, warp, warps.  Bound by latency; many warps where a
+// wave of such CTAs holds all rows, else few, so that it does (16384 rows: 28 us with 32 warps).
+template <bool CE, bool KD, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) head_join_kernel(const __grid_constant__ HeadRowsOut p) {
   pdl_wait();
   pdl_trigger();
   constexpr int F = head_values(CE, KD);
-  __shared__ float s_v[JOIN_WARPS][F][33];
+  __shared__ float s_v[WARPS][F][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float r1 = -INFINITY, s1 = 0.f, r2 = -INFINITY, s2 = 0.f, dot = 0.f;
   if (const int row = blockIdx.x * 32 + lane; row < p.N) {
-    constexpr int U = 4;                 // parts asked for at a time
-    for (int i0 = warp; i0 < p.parts; i0 += U * JOIN_WARPS) {
+    constexpr int U = 8;                 // parts asked for at a time
+    for (int i0 = warp; i0 < p.parts; i0 += U * WARPS) {
       float ar[U], as[U], br[U], bs[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * JOIN_WARPS;
+        const int i = i0 + u * WARPS;
         ar[u] = br[u] = -INFINITY;
         as[u] = bs[u] = 0.f;
         if (i < p.parts) {
@@ -656,17 +656,19 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) head_join_kernel(const __grid
   if (CE) { s_v[warp][0][lane] = r1; s_v[warp][1][lane] = s1; }
   if (KD) { s_v[warp][F - 3][lane] = r2; s_v[warp][F - 2][lane] = s2; s_v[warp][F - 1][lane] = dot; }
   __syncthreads();
-  if (CE) { r1 = s_v[lane][0][warp]; s1 = s_v[lane][1][warp]; }
-  if (KD) { r2 = s_v[lane][F - 3][warp]; s2 = s_v[lane][F - 2][warp]; dot = s_v[lane][F - 1][warp]; }
+  // lanes are now (row of the warp's, part)
+  const int mine = warp * (32 / WARPS) + lane / WARPS, from = lane % WARPS;
+  if (CE) { r1 = s_v[from][0][mine]; s1 = s_v[from][1][mine]; }
+  if (KD) { r2 = s_v[from][F - 3][mine]; s2 = s_v[from][F - 2][mine]; dot = s_v[from][F - 1][mine]; }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = WARPS / 2; o > 0; o >>= 1) {
     if (CE) join_lanes(r1, s1, o);
     if (KD) {
       join_lanes(r2, s2, o);
       dot += __shfl_xor_sync(0xffffffffu, dot, o);
     }
   }
-  if (const int row = blockIdx.x * 32 + warp; lane == 0 && row < p.N) {
+  if (const int row = blockIdx.x * 32 + mine; from == 0 && row < p.N) {
     if (CE) {
       const double l = (double(r1) + log2(double(s1))) / double(LOG2E);
       const long long y = p.targets[row];
@@ -685,8 +687,8 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) head_join_kernel(const __grid
   if (!p.counts) return;
 
   __shared__ bool s_last;
-  __shared__ double s_sum[2][32];
-  __shared__ int s_cnt[2][32];
+  __shared__ double s_sum[2][WARPS];
+  __shared__ int s_cnt[2][WARPS];
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) s_last = gridDim.x == 1 || atomicAdd(p.ticket, 1u) == gridDim.x - 1;
@@ -695,7 +697,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) head_join_kernel(const __grid
   __threadfence();
   double sum[2] = {0.0, 0.0};
   int cnt[2] = {0, 0};
-  for (int r = threadIdx.x; r < p.N; r += 32 * JOIN_WARPS) {
+  for (int r = threadIdx.x; r < p.N; r += 32 * WARPS) {
     if (CE) { sum[0] += double(__ldcg(p.ce + r)); cnt[0] += p.targets[r] != -100; }
     if (KD) { sum[1] += double(__ldcg(p.kd + r)); cnt[1] += p.neg_entropy[r] != INFINITY; }
   }
@@ -713,7 +715,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) head_join_kernel(const __grid
     const int i = threadIdx.x;
     double a = 0.0;
     int n = 0;
-    for (int w = 0; w < 32; ++w) { a += s_sum[i][w]; n += s_cnt[i][w]; }
+    for (int w = 0; w < WARPS; ++w) { a += s_sum[i][w]; n += s_cnt[i][w]; }
     float* mean = i == 0 ? p.mean_ce : p.mean_kd;
     if (mean) *mean = float(a / double(n));            // no row that counts: 0 / 0 = NaN, as the mean of the logits' loss has it
     p.counts[i] = float(n);
@@ -771,6 +773,15 @@ template <bool GRAD>
 int launch_logits(bool ce, bool kd, const CUtensorMap& tx, const CUtensorMap& tw, const HeadLogits& p, int sms, cudaStream_t stream) {
   if (ce && kd) return launch_logits<true, true, GRAD>(tx, tw, p, sms, stream);
   return ce ? launch_logits<true, false, GRAD>(tx, tw, p, sms, stream) : launch_logits<false, true, GRAD>(tx, tw, p, sms, stream);
+}
+
+template <bool CE, bool KD>
+int launch_join(const HeadRowsOut& o, cudaStream_t stream) {
+  const int ctas = o.N > 0 ? (o.N + 31) / 32 : 1;
+  const bool many = ctas <= sm_count();
+  launch_dep(many ? head_join_kernel<CE, KD, 32> : head_join_kernel<CE, KD, 8>, ctas, many ? 1024 : 256, 0, stream, o);
+  JB_LAUNCH_CHECK("head_join_kernel");
+  return JB200_OK;
 }
 
 // Everything about the arguments that both directions share.
@@ -962,9 +973,9 @@ int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* mean_ce, 
     if ((rc = launch_logits<false>(has_ce, has_kd, tx, tw, p, sms, stream)) != JB200_OK) return rc;
   }
   // (without rows both means are written: nothing says which was asked for)
-  auto join = (has_ce && has_kd) || h->N == 0 ? head_join_kernel<true, true> : has_ce ? head_join_kernel<true, false> : head_join_kernel<false, true>;
-  launch_dep(join, h->N > 0 ? (h->N + 31) / 32 : 1, 32 * JOIN_WARPS, 0, stream, o);
-  JB_LAUNCH_CHECK("head_join_kernel");
+  const int rc2 = (has_ce && has_kd) || h->N == 0 ? launch_join<true, true>(o, stream) : has_ce ? launch_join<true, false>(o, stream)
+                                                                                                : launch_join<false, true>(o, stream);
+  if (rc2 != JB200_OK) return rc2;
   return JB200_OK;
 }
 
