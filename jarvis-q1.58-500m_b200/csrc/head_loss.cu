@@ -247,29 +247,30 @@ struct Entries {
 
 constexpr int head_values(bool ce, bool kd) { return (ce ? 2 : 0) + (kd ? 3 : 0); }
 
-// A row's part in the gradient: the sum's reference point, the row's factor, the factor over the sum.  A row without target and teacher
-// takes part in nothing, whatever it holds.
+// A row's part in the gradient: the sums' reference points, the row's factors times 2^13, the factors over the sums.  A row without target
+// and teacher takes part in nothing, whatever it holds; one with either has both reference points, with which no exponential is large.
 template <bool CE, bool KD>
 struct RowGrad {
   float l1 = 0.f, g1 = 0.f, p1 = 0.f, l2 = 0.f, g2 = 0.f, p2 = 0.f;
   bool live = false;
   __device__ __forceinline__ void load(const HeadGrads& p, int row, float scale) {
     const float nan = __int_as_float(0x7fc00000);
+    constexpr float unit = float(1 << HEAD_G_EXP);
     if (CE) {
+      l1 = p.lse[row];
       const long long y = p.targets[row];
       if (y != -100) {
         live = true;
-        l1 = p.lse[row];
-        g1 = y < 0 || y >= p.V ? nan : row_factor(p.g_ce, p.g_ce_stride, p.n_ce, row) / scale;
+        g1 = y < 0 || y >= p.V ? nan : row_factor(p.g_ce, p.g_ce_stride, p.n_ce, row) / scale * unit;
         p1 = g1 / p.lse[size_t(p.N) + row];
       }
     }
     if (KD) {
+      l2 = p.lse_t[row];
       const float e = p.neg_entropy[row];
       if (e != INFINITY) {
         live = true;
-        l2 = p.lse_t[row];
-        g2 = e != e ? nan : row_factor(p.g_kd, p.g_kd_stride, p.n_kd, row) * p.tau / scale;
+        g2 = e != e ? nan : row_factor(p.g_kd, p.g_kd_stride, p.n_kd, row) * p.tau / scale * unit;
         p2 = g2 / p.lse_t[size_t(p.N) + row];
       }
     }
@@ -313,8 +314,8 @@ __device__ __forceinline__ uint32_t f16x2_of_bf16x2(uint32_t w, float factor) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 // With few rows of x the weight's copy is what the launch waits for (37 rows of 50257 x 1024: 47 us where the logits alone take 26, and
-// HBM 32 for the weight and its copy; four warps: 65; loads ahead of the conversion, or each CTA the rows that its products read: no change).  Rows that take no
-// part become zeros, so that a NaN or an infinity in one does not reach the others' sums.
+// HBM 32 for the weight and its copy; four warps: 65; loads ahead of the conversion, or each CTA the rows that its products read:
+// no change).  Rows that take no part become zeros, so that a NaN or an infinity in one does not reach the others' sums.
 template <typename Live>
 __device__ __forceinline__ void copy_f16(const uint4* src, uint4* dst, int n_rows, int C, float factor, int warp, int lane, Live live_row) {
   constexpr int R = 4;
@@ -466,7 +467,7 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
   } else {
     // ---------------- epilogue ----------------
     const int quarter = warp & 3;                              // TMEM lanes this warp may read
-    const float scale = GRAD ? head_scale(p.grads) * (1.f / (1 << HEAD_G_EXP)) : 1.f;
+    const float scale = GRAD ? head_scale(p.grads) : 1.f;
     const uint32_t group = uint32_t(warp - HEAD_EPI_WARP0) >> 2;
     // [16 columns][32 lanes] of this warp
     float* stage = reinterpret_cast<float*>(behind + HEAD_CTL) + (warp - HEAD_EPI_WARP0) * 512 + lane;

@@ -208,6 +208,34 @@ def test_rows_that_have_no_part():
     assert torch.equal(dw, want[1]) and torch.equal(dx, want[0])
 
 
+def test_rows_with_one_of_the_two_losses():
+    """Logits of a thousand in rows that have a target but no teacher, and the other way round: the loss that a row lacks has no part."""
+    h, w, t, ids, logits = _problem(64, 600, 64, 6)
+    h = (h * 300).bfloat16()
+    t[10:20], ids[30:40] = -100, -1
+    ids[10:20, 0], logits[10:20, 0], t[30:40] = 5, 1.0, 7
+    x, wt = h.clone().requires_grad_(), w.clone().requires_grad_()
+    ce, kd = losses.linear_losses(x, wt, t, ids, logits)
+    dx, dw = torch.autograd.grad(ce + kd, (x, wt))
+    n_ce, n_kd = int((t != -100).sum()), int((ids >= 0).any(1).sum())
+    one = torch.ones(64, device="cuda", dtype=F64)
+    want = _definition(h, w, t, ids, logits, 1.0, one / n_ce, one / n_kd)
+    _check_rows(losses.linear_cross_entropy(h, w, t, reduction="none"), want["ce"], want["Z"])
+    _check_grad(dx, want["dx"], want["dx_bound"])
+    _check_grad(dw, want["dw"], want["dw_bound"])
+
+
+def test_gradients_of_tiny_losses():
+    """A loss scaled down to the smallest normal numbers: its gradients are the scaled ones."""
+    h, w, t, ids, logits = _problem(40, 500, 64, 6)
+    x, wt = h.float().requires_grad_(), w.float().requires_grad_()
+    ce, kd = losses.linear_losses(x, wt, t, ids, logits)
+    want = torch.autograd.grad(ce + kd, (x, wt), retain_graph=True)
+    got = torch.autograd.grad(ce + kd, (x, wt), grad_outputs=torch.tensor(2.0 ** -100, device="cuda"))
+    for a, b in zip(got, want):
+        assert torch.equal(a * 2.0 ** 60, b * 2.0 ** -40)
+
+
 def test_operands_of_any_scale():
     """The f16 copies of the products' operands follow the operands' size: the gradients of scaled rows and weights are the scaled gradients,
     to the bit where the scales are powers of two and the logits the same; large values in rows that take no part change nothing."""
