@@ -29,7 +29,9 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int TEACHER_MAX = 256;
-constexpr size_t PIECE_BYTES = size_t(320) << 20;      // gradients of the logits kept at a time, at most
+// Gradients of the logits kept at a time, at most.  Each piece adds to dx once more: 16384 x 50257 x 1024 in pieces of 64 MiB 5.8 ms, 320 MiB 5.4,
+// 640 MiB 5.25, 1280 MiB 5.27.
+constexpr size_t PIECE_BYTES = size_t(640) << 20;
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -848,8 +850,8 @@ long long piece_time(long long n, int N, int C, int slabs, int pairs) {
 }  // namespace
 
 // The fastest of some cuts by that count.  Candidates: the fewest pieces that the workspace allows and a few more, even ones, and those
-// whose tiles fill the pairs without a rest.  (16384 x 50257 x 1024: seven even pieces of 29 tiles, 512 K-blocks of one kind and 464 of
-// the other on the busiest pair where the mean is 802, took 5.4 ms; pieces of 37, all pairs busy to 1 %, see below.)
+// whose tiles fill the pairs without a rest.  (16384 x 50257 x 1024, backward products: seven even pieces of 29 tiles, the busiest pair
+// with 976 K-blocks where the mean is 802, 2390 us; pieces of 37, 1030 for 1024, 2151 us.)
 HeadPlan head_plan(int N, int V, int C, int pairs) {
   struct Kept { int N, V, C, pairs; HeadPlan plan; };
   thread_local Kept kept{};

@@ -80,7 +80,7 @@ def test_backward_passes_are_cut_into_pieces_that_cover_the_vocabulary(sms):
                 assert lib.jb200_host_head_plan(N, V, width, sms, out) == 0
                 cols, pieces, slabs = out
                 assert cols % 256 == 0 and (pieces - 1) * cols < V <= pieces * cols
-                assert cols == 256 or N * cols * 2 <= 320 << 20        # the workspace is bounded, down to one tile of columns
+                assert cols == 256 or N * cols * 2 <= 640 << 20        # the workspace is bounded, down to one tile of columns
                 # every slab of the first piece has K-blocks of 64 columns to sum
                 assert 1 <= slabs <= 64 and slabs <= (min(V, cols) + 63) // 64
     assert lib.jb200_host_head_plan(0, 5, 64, 148, out) == _lib.ERR_ARG
