@@ -832,7 +832,7 @@ int check_head(const jb200_head* h, const char* what) {
     JB_REQUIRE(h->K >= 1 && h->K <= TEACHER_MAX, "%s: a teacher has 1 to %d entries a row, got %d", what, TEACHER_MAX, h->K);
     JB_REQUIRE(h->lse_t, "%s: null pointer (teacher)", what);
     JB_REQUIRE((reinterpret_cast<uintptr_t>(h->teacher) & 15u) == 0, "%s: teacher rows must be 16-byte aligned", what);
-    JB_REQUIRE(h->temperature > 0.f && h->temperature <= FLT_MAX && 1.0f / h->temperature <= FLT_MAX, "%s: temperature must be positive and finite", what);
+    JB_REQUIRE(h->temperature > 0.f && h->temperature <= FLT_MAX && 1.5f / h->temperature <= FLT_MAX, "%s: temperature must be positive and finite", what);
   }
   return JB200_OK;
 }
@@ -924,7 +924,7 @@ int launch_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype
   JB_REQUIRE(N >= 0 && V >= 1, "teacher_rows: bad shape");
   JB_REQUIRE(K >= 1 && K <= TEACHER_MAX, "teacher_rows: a teacher has 1 to %d entries a row, got %d", TEACHER_MAX, K);
   JB_REQUIRE(logits_dtype == 0 || logits_dtype == 1, "teacher_rows: dtype must be 0 (f32) or 1 (bf16)");
-  JB_REQUIRE(temperature > 0.f && temperature <= FLT_MAX && 1.0f / temperature <= FLT_MAX, "teacher_rows: temperature must be positive and finite");
+  JB_REQUIRE(temperature > 0.f && temperature <= FLT_MAX && 1.5f / temperature <= FLT_MAX, "teacher_rows: temperature must be positive and finite");
   if (N == 0) return JB200_OK;
   JB_REQUIRE(ids && logits && rows, "teacher_rows: null pointer");
   JB_REQUIRE(aligned16(rows), "teacher_rows: rows must be 16-byte aligned");

@@ -630,3 +630,54 @@ def test_weights_beyond_two_to_the_31_elements():
             col[n] -= 1
         big = flat + (0 if n is None else (torch.arange(N, device="cuda") == n))
         _check_grad(dw[row], col @ hd, rel * (big @ hd.abs()) + floor * big.sum())
+
+
+def test_two_threads_at_once():
+    """Calls from two threads on two streams, each over its own rows: the results of calls one after the other."""
+    import threading
+    sets = [_problem(300 + 100 * i, 4001, 128, 9, seed=i) for i in range(2)]
+    want = [_step(s[0].clone().requires_grad_(), s[1].clone().requires_grad_(), *s[2:]) for s in sets]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            x, w = sets[i][0].clone().requires_grad_(), sets[i][1].clone().requires_grad_()
+            for _ in range(20):
+                got[i] = _step(x, w, *sets[i][2:])
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for g, w in zip(got, want):
+        assert g is not None and all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+def test_gradients_are_not_differentiable_and_say_so():
+    h, w, t, _, _ = _problem(20, 300, 64, 3)
+    x = h.float().requires_grad_()
+    g, = torch.autograd.grad(losses.linear_cross_entropy(x, w, t), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    nw = torch.ones(64, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(losses.rms_norm(x, nw).float().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_a_weight_used_twice_and_rows_that_are_one_row():
+    """Gradients of the same tensor from two uses add up; an expanded row's are the sum over its rows."""
+    h, w, t, _, _ = _problem(24, 300, 64, 3)
+    wt = w.float().requires_grad_()
+    both, = torch.autograd.grad(losses.linear_cross_entropy(h[:10], wt, t[:10], reduction="none").sum() +
+                                losses.linear_cross_entropy(h[10:], wt, t[10:], reduction="none").sum(), wt)
+    one, = torch.autograd.grad(losses.linear_cross_entropy(h, wt, t, reduction="none").sum(), wt)
+    want = _definition(h, w, t, None, None, 1.0, torch.ones(24, device="cuda"), None)
+    _check_grad(both, want["dw"], 2 * want["dw_bound"])
+    _check_grad(one, want["dw"], want["dw_bound"])
+    row = h[:1].float().requires_grad_()
+    dx, = torch.autograd.grad(losses.linear_cross_entropy(row.expand(24, 64), w, t, reduction="none").sum(), row)
+    want = _definition(h[:1].expand(24, 64), w, t, None, None, 1.0, torch.ones(24, device="cuda"), None)
+    _check_grad(dx, want["dx"].sum(0, keepdim=True), want["dx_bound"].sum(0, keepdim=True) * 1.01)

@@ -22,7 +22,7 @@ def _head(**kw):
                                      (dict(teacher=4096, K=257), "1 to 256 entries"), (dict(teacher=4096, K=3), "null pointer"), (dict(teacher=4104, K=3, lse_t=4096), "16-byte"),
                                      (dict(teacher=4096, K=3, lse_t=4096, temperature=0.0), "temperature"),
                                      (dict(teacher=4096, K=3, lse_t=4096, temperature=float("nan")), "temperature"),
-                                     (dict(teacher=4096, K=3, lse_t=4096, temperature=1e-39), "temperature"),
+                                     (dict(teacher=4096, K=3, lse_t=4096, temperature=4e-39), "temperature"),
                                      (dict(N=2**30, V=2**30), "too many logits")])
 def test_head_calls_refuse_bad_arguments(kw, text):
     lib = _lib.load()
