@@ -179,7 +179,8 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
     // ---------------- epilogue: a lane is a row, its registers are channels ----------------
     const int quarter = warp & 3, half = (warp - HEAD_EPI_WARP0) >> 2;
     const float common = head_scale(p.grads);
-    const float dx_scale = ldexpf(common, -HEAD_G_EXP - p.exps[0]), dw_scale = ldexpf(common, -HEAD_G_EXP - p.exps[1]);
+    // two factors: their product may be below f32's range where the result is not
+    const float dx_unit = ldexpf(1.f, -HEAD_G_EXP - p.exps[0]), dw_unit = ldexpf(1.f, -HEAD_G_EXP - p.exps[1]);
     uint32_t tile = 0u;
     for (; head_item(p, pair, n_pairs, int(tile), &it); ++tile) {
       const uint32_t acc = tile & 1u;
@@ -196,9 +197,9 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
         tmem_ld_32x32(t_lane + c0, v);
         tmem_ld_wait();
         if (on) {
-          const float scale = it.is_dw ? dw_scale : dx_scale;
+          const float unit = it.is_dw ? dw_unit : dx_unit;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(scale * __uint_as_float(v[j]));
+          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(common * (unit * __uint_as_float(v[j])));
           const int n = min(32, p.C - col);
           if (!it.is_dw) {
             const size_t o = size_t(row) * p.C + col;

@@ -175,6 +175,8 @@ struct HeadLogits {
   int ldg;
   const uint4 *x, *w;        // gradient: rows and weight
   uint4 *xs, *ws;            // their copies, the weight's of these columns; null: not wanted
+  const unsigned* tops;      // [2][HEAD_RANGE_CTAS], n_tops of each: largest magnitudes of the weight and of the rows, part by part
+  int n_tops;
   int* exps;                 // exponents of the copies' factors, weight and rows: made by the first piece, read by the others
   int box_rows;              // rows of x that a CTA asks for at a time
   unsigned int* status;
@@ -278,37 +280,22 @@ struct RowGrad {
     }
   }
 };
-template <bool CE, bool KD>
+template <bool CE = true, bool KD = true>
 __device__ __forceinline__ bool row_is_live(const HeadGrads& p, int row) {
-  return (CE && p.targets[row] != -100) || (KD && p.neg_entropy[row] != INFINITY);
+  return (CE && p.targets && p.targets[row] != -100) || (KD && p.neg_entropy && p.neg_entropy[row] != INFINITY);
 }
 
 // ---- f16 copies of the products' other operands, by eight warps of every CTA beside the products ----
 constexpr int COPY_WARPS = 8;
 
-// Largest finite magnitude, as bf16 bits, that this warp's share of the sample holds; rows that take no part are left out.
-template <typename Live>
-__device__ __forceinline__ unsigned sample_rows(const uint4* m, int n_rows, int per_row, int warp, int lane, Live live_row) {
+// Exponent of the factor that brings the largest magnitude (as bf16 bits) to [2^15, 2^16), where f16 ends at 65504 and bf16 has no value
+// beyond 65280; nothing but zeros (or subnormal numbers): as far up as there is.
+__device__ __forceinline__ int copy_exponent(unsigned top) { return min(126, 127 + 15 - int(top >> 7)); }
+// Largest of what head_range_kernel's CTAs found, by a warp.
+__device__ __forceinline__ unsigned range_top(const unsigned* tops, int n, int lane) {
   unsigned top = 0;
-#pragma unroll
-  for (int i = 0; i < HEAD_SAMPLES / COPY_WARPS; ++i) {
-    const long long row = (long long)(i * COPY_WARPS + warp) * (n_rows - 1) / (HEAD_SAMPLES - 1);
-    if (!live_row(int(row))) continue;
-#pragma unroll 4
-    for (int c = lane; c < per_row; c += 32) {
-      const uint4 v = __ldg(m + row * per_row + c);
-      const unsigned a[4] = {v.x & 0x7fff7fffu, v.y & 0x7fff7fffu, v.z & 0x7fff7fffu, v.w & 0x7fff7fffu};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) top = __vmaxu2(top, a[j] & __vcmpltu2(a[j], 0x7f807f80u));
-    }
-  }
-  top = max(top & 0xffffu, top >> 16);
+  for (int i = lane; i < n; i += 32) top = max(top, tops[i]);
   return __reduce_max_sync(0xffffffffu, top);
-}
-// Exponent of the factor that brings it to [1, 2); nothing but zeros (or subnormal numbers): 0.
-__device__ __forceinline__ int copy_exponent(unsigned top) {
-  const int e = int(top >> 7);
-  return e == 0 ? 0 : max(-100, min(100, 127 - e));
 }
 
 __device__ __forceinline__ uint32_t f16x2_of_bf16x2(uint32_t w, float factor) {
@@ -344,20 +331,13 @@ __device__ __forceinline__ void copy_f16(const uint4* src, uint4* dst, int n_row
 }
 
 template <bool CE, bool KD>
-__device__ __forceinline__ void make_copies(const HeadLogits& p, unsigned* s_top, int warp, int lane) {
+__device__ __forceinline__ void make_copies(const HeadLogits& p, int warp, int lane) {
   int ew, ex;
   const auto live = [&](int row) { return row_is_live<CE, KD>(p.grads, row); };
   const auto all = [](int) { return true; };
   if (p.v0 == 0) {
-    const unsigned tw = p.ws ? sample_rows(p.w, p.V, p.C / 8, warp, lane, all) : 0u;
-    const unsigned tx = p.xs ? sample_rows(p.x, p.N, p.C / 8, warp, lane, live) : 0u;
-    if (lane == 0) { s_top[warp] = tw; s_top[COPY_WARPS + warp] = tx; }
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * COPY_WARPS) : "memory");        // the copying warps alone, which wait for nothing else
-    unsigned mw = 0, mx = 0;
-#pragma unroll
-    for (int i = 0; i < COPY_WARPS; ++i) { mw = max(mw, s_top[i]); mx = max(mx, s_top[COPY_WARPS + i]); }
-    ew = copy_exponent(mw);
-    ex = copy_exponent(mx);
+    ew = copy_exponent(range_top(p.tops, p.n_tops, lane));
+    ex = copy_exponent(range_top(p.tops + HEAD_RANGE_CTAS, p.n_tops, lane));
     if (blockIdx.x == 0 && warp == 0 && lane == 0) { p.exps[0] = ew; p.exps[1] = ex; }
   } else {
     ew = p.exps[0];
@@ -464,8 +444,7 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
       }
     }
   } else if (GRAD && warp >= HEAD_EPI_WARP0 + 8) {
-    __shared__ unsigned s_top[2 * COPY_WARPS];
-    make_copies<CE, KD>(p, s_top, warp - HEAD_EPI_WARP0 - 8, lane);
+    make_copies<CE, KD>(p, warp - HEAD_EPI_WARP0 - 8, lane);
   } else {
     // ---------------- epilogue ----------------
     const int quarter = warp & 3;                              // TMEM lanes this warp may read
@@ -755,13 +734,30 @@ __global__ void __launch_bounds__(32 * WARPS) head_join_kernel(const __grid_cons
   }
 }
 
-// Gradients row by row: their common factor, the largest finite one of its kind.
-__global__ void __launch_bounds__(1024) head_scale_kernel(const __grid_constant__ HeadGrads p) {
-  pdl_wait();
-  pdl_trigger();
+// Ahead of a backward pass: the largest finite magnitudes of the weight and of the rows that take part, which the f16 copies are scaled
+// by; a CTA leaves what it found (bf16 bits) of both.  Bound by HBM: 50257 x 1024 take 19 us alone; of a step of 37 rows 11, since it goes backwards
+// and what the logits' kernel begins with has come last and is in L2.  With gradients row by row one more CTA finds their common factor, the largest finite one of its kind.
+constexpr int RANGE_THREADS = 1024;
+struct HeadRange {
+  HeadGrads grads;
+  const uint4 *w, *x;        // null: not wanted
+  int V, N, per_row;         // rows of both, and their length in uint4
+  unsigned* tops;            // [2][HEAD_RANGE_CTAS]
+  int ctas;
+};
+
+// Larger one by 16-bit halves of `top` and v's finite magnitudes.
+__device__ __forceinline__ unsigned finite_top(unsigned top, uint4 v) {
+  const unsigned a[4] = {v.x & 0x7fff7fffu, v.y & 0x7fff7fffu, v.z & 0x7fff7fffu, v.w & 0x7fff7fffu};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) top = __vmaxu2(top, a[j] & __vcmpltu2(a[j], 0x7f807f80u));
+  return top;
+}
+
+__device__ void head_scale_job(const HeadGrads& p) {
   __shared__ float s_top[2][32];
   float ce = 0.f, kd = 0.f;
-  for (int r = threadIdx.x; r < p.N; r += 1024) {
+  for (int r = threadIdx.x; r < p.N; r += RANGE_THREADS) {
     if (p.targets && p.targets[r] != -100) {
       const float c = fabsf(row_factor(p.g_ce, p.g_ce_stride, p.n_ce, r));
       if (c <= FLT_MAX) ce = fmaxf(ce, c);
@@ -779,8 +775,48 @@ __global__ void __launch_bounds__(1024) head_scale_kernel(const __grid_constant_
   if ((threadIdx.x & 31) == 0) { s_top[0][threadIdx.x >> 5] = ce; s_top[1][threadIdx.x >> 5] = kd; }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < 32; ++w) { ce = fmaxf(ce, s_top[0][w]); kd = fmaxf(kd, s_top[1][w]); }
+    for (int w = 1; w < RANGE_THREADS / 32; ++w) { ce = fmaxf(ce, s_top[0][w]); kd = fmaxf(kd, s_top[1][w]); }
     *p.scale = common_factor(ce, kd);
+  }
+}
+
+__global__ void __launch_bounds__(RANGE_THREADS) head_range_kernel(const __grid_constant__ HeadRange p) {
+  pdl_wait();
+  pdl_trigger();
+  if (int(blockIdx.x) == p.ctas) {
+    head_scale_job(p.grads);
+    return;
+  }
+  __shared__ unsigned s_top[2][RANGE_THREADS / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned tw = 0, tx = 0;
+  if (p.x) {
+    for (int row = int(blockIdx.x) * (RANGE_THREADS / 32) + warp; row < p.N; row += p.ctas * (RANGE_THREADS / 32)) {
+      if (!row_is_live(p.grads, row)) continue;
+#pragma unroll 4
+      for (int c = lane; c < p.per_row; c += 32) tx = finite_top(tx, __ldg(p.x + size_t(row) * p.per_row + c));
+    }
+  }
+  if (p.w) {
+    constexpr int U = 8;
+    const long long step = (long long)(p.ctas) * RANGE_THREADS;
+    long long i = (long long)(p.V) * p.per_row - 1 - ((long long)(blockIdx.x) * RANGE_THREADS + threadIdx.x);
+    for (; i >= (U - 1) * step; i -= U * step) {
+      uint4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = __ldg(p.w + (i - u * step));
+#pragma unroll
+      for (int u = 0; u < U; ++u) tw = finite_top(tw, v[u]);
+    }
+    for (; i >= 0; i -= step) tw = finite_top(tw, __ldg(p.w + i));
+  }
+  tw = __reduce_max_sync(0xffffffffu, max(tw & 0xffffu, tw >> 16));
+  tx = __reduce_max_sync(0xffffffffu, max(tx & 0xffffu, tx >> 16));
+  if (lane == 0) { s_top[0][warp] = tw; s_top[1][warp] = tx; }
+  __syncthreads();
+  if (warp < 2) {
+    const unsigned top = __reduce_max_sync(0xffffffffu, s_top[warp][lane]);
+    if (lane == 0) p.tops[warp * HEAD_RANGE_CTAS + blockIdx.x] = top;
   }
 }
 
@@ -1014,7 +1050,7 @@ int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* mean_ce, 
 
 namespace {
 struct BackwardScratch {
-  size_t xs, ws, scale, exps, g, slabs, total;
+  size_t xs, ws, scale, exps, tops, g, slabs, total;
 };
 BackwardScratch backward_scratch(int N, int C, const HeadPlan& pl) {
   BackwardScratch s;
@@ -1022,7 +1058,8 @@ BackwardScratch backward_scratch(int N, int C, const HeadPlan& pl) {
   s.ws = up256(size_t(N) * head_pitch(C) * 2);
   s.scale = s.ws + up256(size_t(pl.cols) * head_pitch(C) * 2);
   s.exps = s.scale + 16;
-  s.g = s.scale + 256;
+  s.tops = s.scale + 256;
+  s.g = s.tops + up256(2 * HEAD_RANGE_CTAS * 4);
   s.slabs = s.g + up256(size_t(N) * pl.cols * 2);
   s.total = s.slabs + up256(size_t(pl.slabs) * N * C * 4);
   return s;
@@ -1061,11 +1098,8 @@ int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_s
   r.g_ce = g_ce; r.g_kd = g_kd; r.g_ce_stride = g_ce_stride; r.g_kd_stride = g_kd_stride; r.n_ce = n_ce; r.n_kd = n_kd;
   r.N = h->N; r.V = h->V;
   r.tau = h->teacher ? h->temperature : 1.f;
-  if ((h->targets && g_ce_stride) || (h->teacher && g_kd_stride)) {
-    r.scale = reinterpret_cast<float*>(base + at.scale);
-    launch_dep(head_scale_kernel, 1, 1024, 0, stream, r);
-    JB_LAUNCH_CHECK("head_scale_kernel");
-  }
+  const bool by_row = (h->targets && g_ce_stride) || (h->teacher && g_kd_stride);
+  if (by_row) r.scale = reinterpret_cast<float*>(base + at.scale);
 
   HeadLogits p{};
   p.N = h->N; p.V = h->V; p.C = h->C;
@@ -1079,6 +1113,17 @@ int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_s
   if (dw) p.xs = reinterpret_cast<uint4*>(base + at.xs);
   if (dx) p.ws = reinterpret_cast<uint4*>(base + at.ws);
   p.exps = reinterpret_cast<int*>(base + at.exps);
+  HeadRange o{};
+  o.grads = r;
+  o.w = dx ? p.w : nullptr;
+  o.x = dw ? p.x : nullptr;
+  o.V = h->V; o.N = h->N; o.per_row = h->C / 8;
+  o.tops = reinterpret_cast<unsigned*>(base + at.tops);
+  o.ctas = 2 * sms < HEAD_RANGE_CTAS ? 2 * sms : HEAD_RANGE_CTAS;
+  p.tops = o.tops;
+  p.n_tops = o.ctas;
+  launch_dep(head_range_kernel, o.ctas + (by_row ? 1 : 0), RANGE_THREADS, 0, stream, o);
+  JB_LAUNCH_CHECK("head_range_kernel");
   HeadProducts q{};
   p.status = device_status_ptr();
   if (!p.status) return JB200_ERR_CUDA;

@@ -254,6 +254,27 @@ def test_operands_of_any_scale():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("which", ["weight", "rows", "both"])
+@pytest.mark.parametrize("N,V", [(600, 900), (9000, 40001)])
+def test_one_row_a_million_times_larger_than_the_others(N, V, which):
+    h, w, t, ids, logits = _problem(N, V, 128, 8)
+    small = 2.0 ** -20                   # exact in bf16; logits of at most some tens
+    if which != "rows":
+        w *= small
+        w[V - 99] /= small
+    if which != "weight":
+        h *= small
+        h[37] /= small
+    one = torch.ones(N, device="cuda", dtype=F64)
+    n_ce, n_kd = int((t != -100).sum()), int((ids >= 0).any(1).sum())
+    want = _definition(h, w, t, ids, logits, 2.0, one / n_ce, one / n_kd)
+    x, wt = h.clone().requires_grad_(), w.clone().requires_grad_()
+    ce, kd = losses.linear_losses(x, wt, t, ids, logits, temperature=2.0)
+    dx, dw = torch.autograd.grad(ce + kd, (x, wt))
+    _check_grad(dx, want["dx"], want["dx_bound"])
+    _check_grad(dw, want["dw"], want["dw_bound"])
+
+
 def test_nothing_to_learn_from():
     h, w, t, ids, logits = _problem(300, 500, 64, 6)
     t[:], ids[:] = -100, -1
