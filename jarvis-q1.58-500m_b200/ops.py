@@ -266,6 +266,12 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, out_dtype=
         raise RuntimeError("rmsnorm: expected a contiguous CUDA tensor")
     _need(weight, torch.float32, "rmsnorm.weight")
     C = x.shape[-1]
+    if weight.numel() != C:
+        raise RuntimeError(f"rmsnorm: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not belong together")
+    _together("rmsnorm", x, weight)
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return rmsnorm(x, weight, eps, out_dtype)
     y = torch.empty_like(x, dtype=out_dtype)
     _lib.check(lib.jb200_rmsnorm(_ptr(x), _dt(x), _ptr(weight), eps, _ptr(y), _dt(y), x.numel() // C, C, _stream()),
                "jb200_rmsnorm")

@@ -103,3 +103,59 @@ def test_every_item_of_the_gradients_products_is_done_once(n_long, k_long, n_sho
     assert sorted(seen) == list(range(n_long + n_short))
     # no pair has more than its even share, rounded up by an item of each kind
     assert busiest <= (n_long * k_long + n_short * k_short) / pairs + k_long + k_short
+
+
+class _OnCard(torch.Tensor):
+    """A host tensor that says it is on the card `card`."""
+    card = 0
+    is_cuda = property(lambda self: True)
+    device = property(lambda self: torch.device("cuda", self.card))
+
+    def get_device(self):
+        return self.card
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        with torch._C.DisableTorchFunctionSubclass():
+            return func(*args, **(kwargs or {}))
+
+
+def _on(card, *shape, dtype=torch.float32):
+    t = torch.zeros(*shape, dtype=dtype).as_subclass(_OnCard)
+    t.card = card
+    return t
+
+
+def test_norm_launches_on_its_tensors_card(monkeypatch):
+    current, seen = [0], []
+
+    class Card:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Lib:
+        def __getattr__(self, name):
+            if name.endswith("_scratch_bytes"):
+                return lambda *a: 0
+            return lambda *a: seen.append((name, current[0])) or 0
+
+    monkeypatch.setattr(ops._lib, "load", lambda: Lib())
+    monkeypatch.setattr(ops, "_raw_device", lambda: current[0])
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops.torch.cuda, "device", Card)
+    for card in (1, 0):
+        ops.rmsnorm(_on(card, 4, 64), _on(card, 64))
+        ops.rmsnorm_backward(_on(card, 4, 64), _on(card, 64), _on(card, 4, 64))
+        assert seen == [("jb200_rmsnorm", card), ("jb200_rmsnorm_backward", card)] and current == [0]
+        seen.clear()
+    with pytest.raises(RuntimeError, match="cuda:1 and cuda:0"):
+        ops.rmsnorm(_on(1, 4, 64), _on(0, 64))
+    with pytest.raises(RuntimeError, match="do not belong together"):
+        ops.rmsnorm(_on(0, 4, 64), _on(0, 32))
+    assert not seen
