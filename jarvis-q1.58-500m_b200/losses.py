@@ -14,7 +14,8 @@ holds the same parameters' accumulators; the operators themselves launch on the 
 
 Numerics: hidden rows and weight enter the products as bf16 (an f32 argument is rounded to it, as under autocast), sums and softmax are
 f32, the gradient of the logits is rounded to f16 for the products it enters (2^-11 of a value, relative to the call's largest factor
-down to 2^-38), gradients are returned in their argument's dtype from f32 sums.
+down to 2^-38; rows and weight enter those exactly within 2^32 of their largest value), gradients are returned in their argument's
+dtype from f32 sums.
 """
 from __future__ import annotations
 
