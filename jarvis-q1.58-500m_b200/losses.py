@@ -33,6 +33,12 @@ def _bf16(t: torch.Tensor, what: str) -> torch.Tensor:
     return (t if t.dtype is torch.bfloat16 else t.to(torch.bfloat16)).contiguous()
 
 
+def _trains(weight: torch.Tensor):
+    """Marks a weight that is about to get a gradient: updates may leave no trace on it, so nobody keeps a copy (modules._in_training)."""
+    if weight.requires_grad:
+        weight._jb_trained = True
+
+
 def _rows(t: torch.Tensor, lead, dtypes, what: str, columns: int | None = None) -> torch.Tensor:
     """`t` of shape (*lead) or (*lead, columns) as contiguous rows."""
     if t.dtype not in dtypes:
@@ -110,6 +116,7 @@ def _head_loss(hidden, weight, targets, ids, logits, temperature, reduction):
         raise RuntimeError(f"reduction must be 'mean' or 'none', got {reduction!r}")
     mean = reduction == "mean"
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        _trains(weight)
         return _HeadLoss.apply(hidden, weight, targets, ids, logits, temperature, mean)
     r, lead = _forward(hidden, weight, targets, ids, logits, temperature, mean)[4:]
     return _results(r, lead)
@@ -164,5 +171,6 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, out_dtype
     if weight.dim() != 1 or x.dim() < 1 or weight.shape[0] != x.shape[-1]:
         raise RuntimeError(f"rms_norm: weight {tuple(weight.shape)} does not fit rows of {tuple(x.shape)}")
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        _trains(weight)
         return _RMSNorm.apply(x, weight, eps, out_dtype)
     return ops.rmsnorm(x.contiguous(), weight.float().contiguous(), eps, out_dtype)

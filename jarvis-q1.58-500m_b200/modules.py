@@ -23,14 +23,20 @@ from . import chain, losses, ops
 # ----------------------------------------------------------------------------------------------
 
 
+def _in_training(p: torch.Tensor) -> bool:
+    """True where updates of `p` may leave no trace on it, as those of fused optimizers and of captured steps do (its version is not
+    counted up): it has been through a loss or a norm with gradients (`losses`), or has a gradient.  No copy of it is kept then."""
+    return getattr(p, "_jb_trained", False) or (p.is_leaf and p.grad is not None)
+
+
 def _f32(p: torch.Tensor, scalar: bool = False) -> torch.Tensor:
     """`p.detach().float().contiguous()` (reshaped to (1,) for scalars), cached on the parameter until it changes
     (in-place update or new storage): the views cost a few microseconds each, several times per layer."""
     key = (p.data_ptr(), p._version, scalar)
     c = getattr(p, "_jb_f32", None)
-    if c is None or c[0] != key:
+    if c is None or c[0] != key or (c[2] and _in_training(p)):
         t = p.detach().float().contiguous()
-        c = (key, t.reshape(1) if scalar else t)
+        c = (key, t.reshape(1) if scalar else t, t.data_ptr() != p.data_ptr())       # the last: it is a copy, not a view
         p._jb_f32 = c
     return c[1]
 
@@ -609,10 +615,20 @@ class Jarvis(nn.Module):
         scal = torch.zeros((n, 3), dtype=torch.float32, device=device)
         return [(acc[i], hist[i], scal[i]) for i in range(n)]
 
+    def refresh_head(self):
+        """Drops what is kept of lm_head's and final_norm's weights, and keeps copies of them again.  Training by `head_loss` or by `losses`
+        needs no call for its updates to be seen: from the first loss with gradients on each forward converts the weights anew
+        (50257 x 1024: 47 us at the copy rate).  Call it when training is over, or after an update that neither a loss here, a gradient on
+        the weight nor its version shows (another library's, through `.data`)."""
+        self._lm_head_bf16 = None
+        for p in (self.lm_head.weight, self.final_norm.weight):
+            p._jb_trained, p._jb_f32 = False, None
+
     def _lm_head_weight(self):
         w = self.lm_head.weight
         key = (w.data_ptr(), w._version)
-        if self._lm_head_bf16 is None or self._lm_head_bf16[0] != key:
+        if self._lm_head_bf16 is None or self._lm_head_bf16[0] != key or _in_training(w):
+            self._lm_head_bf16 = None
             # rows padded with zeros to a multiple of 128, the out-feature tile of the GEMM kernel
             v = w.shape[0]
             wp = torch.zeros(((v + 127) // 128 * 128, w.shape[1]), dtype=torch.bfloat16, device=w.device)
@@ -740,8 +756,8 @@ class Jarvis(nn.Module):
         return self._logits(hidden, B, T), {"h": new_h, "S": new_s}
 
     def _lm_head_rows(self):
-        """lm_head's weight in bf16 without the padding rows."""
-        return self._lm_head_weight()[:self.lm_head.weight.shape[0]]
+        """lm_head's weight as it is, in bf16 without padding rows."""
+        return self.lm_head.weight.detach().to(torch.bfloat16).contiguous()
 
     def _logits(self, hidden, B, T):
         """Dense bf16 lm_head on the same tcgen05 pipeline as the ternary layers (weight tiles by TMA); the padded
@@ -782,7 +798,9 @@ class Jarvis(nn.Module):
     def head_loss(self, idx, targets=None, teacher_ids=None, teacher_logits=None, *, temperature: float = 1.0):
         """Losses to train the head by: the blocks run as they are (inference, no gradient), then final norm and lm_head with
         gradients of `final_norm.weight` and `lm_head.weight`, through `losses`.  With targets (B, T): the mean cross entropy; with
-        a teacher's top logits, teacher_ids and teacher_logits (B, T, K): the mean distillation loss; with both: the pair."""
+        a teacher's top logits, teacher_ids and teacher_logits (B, T, K): the mean distillation loss; with both: the pair.  Whatever
+        updates the weights, forward, step and loss see it (`refresh_head` when training is over); a session captured earlier is
+        captured again."""
         if targets is None and teacher_ids is None:
             raise RuntimeError("head_loss: neither targets nor a teacher")
         if (teacher_ids is None) != (teacher_logits is None):

@@ -702,3 +702,75 @@ def test_a_weight_used_twice_and_rows_that_are_one_row():
     dx, = torch.autograd.grad(losses.linear_cross_entropy(row.expand(24, 64), w, t, reduction="none").sum(), row)
     want = _definition(h[:1].expand(24, 64), w, t, None, None, 1.0, torch.ones(24, device="cuda"), None)
     _check_grad(dx, want["dx"].sum(0, keepdim=True), want["dx_bound"].sum(0, keepdim=True) * 1.01)
+
+
+# ------------------------------------------------------------------------------------------------ a head that is being trained
+def _fresh(model):
+    """A model of the same weights that has kept nothing."""
+    from jarvis_b200 import modules as jm
+    twin = jm.Jarvis(vocab_size=301, d_model=128, n_layers=2, n_heads=2, max_seq_len=64).cuda().eval()
+    twin.load_state_dict(model.state_dict())
+    twin.final_norm.to(model.final_norm.weight.dtype)
+    with torch.no_grad():
+        twin.final_norm.weight.copy_(model.final_norm.weight)
+    return twin
+
+
+def _same_as_fresh(model, idx, y):
+    twin = _fresh(model)
+    for a, b in zip(model(idx, targets=y), twin(idx, targets=y)):
+        assert torch.equal(a, b)
+    assert torch.equal(model.loss(idx, y), twin.loss(idx, y))
+    assert torch.equal(model.step(idx)[0], twin.step(idx)[0])
+
+
+@pytest.mark.parametrize("norm_dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("fused", [True, False])
+def test_every_path_reads_the_head_as_it_is_trained(fused, norm_dtype):
+    """An update may leave no trace on a tensor (fused optimizers do not count its version up): logits, losses and steps follow it."""
+    model = _model()
+    model.final_norm.to(norm_dtype)
+    g = _gen(6)
+    idx, y = (torch.randint(0, 301, (2, 33), generator=g, device="cuda") for _ in range(2))
+    params = [model.final_norm.weight, model.lm_head.weight]
+    opt = torch.optim.AdamW(params, lr=0.1, fused=fused)
+    model(idx, targets=y)                                            # whatever is kept of the weights is there before the first update
+    for i in range(3):
+        before = model.lm_head.weight.detach().clone()
+        model.head_loss(idx, y).backward()
+        model(idx)                                                   # ... and made again between backward pass and update
+        opt.step()
+        opt.zero_grad()
+        assert (model.lm_head.weight - before).abs().max() > 0.01
+        _same_as_fresh(model, idx, y)
+    model.refresh_head()                                             # training is over: copies are kept again
+    kept = model._lm_head_weight()
+    assert model._lm_head_weight() is kept
+    _same_as_fresh(model, idx, y)
+
+
+def test_every_path_reads_a_head_that_a_captured_step_trains():
+    model = _model()
+    g = _gen(7)
+    idx, y = (torch.randint(0, 301, (2, 33), generator=g, device="cuda") for _ in range(2))
+    params = [model.final_norm.weight, model.lm_head.weight]
+
+    def step():
+        grads = torch.autograd.grad(model.head_loss(idx, y), params)
+        with torch.no_grad():
+            for p, d in zip(params, grads):
+                p.sub_(0.5 * d)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    model(idx, targets=y)
+    before = model.lm_head.weight.detach().clone()
+    for _ in range(3):
+        graph.replay()
+        _same_as_fresh(model, idx, y)
+    assert (model.lm_head.weight - before).abs().max() > 2.0 ** -8 * before.abs().max()

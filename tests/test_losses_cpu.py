@@ -159,3 +159,31 @@ def test_norm_launches_on_its_tensors_card(monkeypatch):
     with pytest.raises(RuntimeError, match="do not belong together"):
         ops.rmsnorm(_on(0, 4, 64), _on(0, 32))
     assert not seen
+
+
+def test_the_heads_copies_follow_updates_that_leave_no_trace():
+    from jarvis_b200 import modules as jm
+    torch.manual_seed(1)
+    model = jm.Jarvis(vocab_size=301, d_model=128, n_layers=1, n_heads=2, max_seq_len=64).eval()
+    w = model.lm_head.weight
+    model._lm_head_rows(), model._lm_head_weight()
+    opt = torch.optim.AdamW([w], lr=0.1, fused=True)
+    for _ in range(2):
+        version, w.grad = w._version, torch.randn(301, 128)
+        opt.step()
+        assert w._version == version                                 # what the test is about
+        want = w.detach().bfloat16()
+        assert torch.equal(model._lm_head_rows(), want)
+        assert torch.equal(model._lm_head_weight()[:301], want) and not model._lm_head_weight()[301:].any()
+    opt.zero_grad()
+    # an update that neither a loss of this package nor a gradient on the weight announces
+    with torch.no_grad():
+        w.data.add_(1)
+    assert torch.equal(model._lm_head_rows(), w.detach().bfloat16())
+    model.refresh_head()
+    assert torch.equal(model._lm_head_weight()[:301], w.detach().bfloat16())
+    kept = model._lm_head_weight()
+    assert model._lm_head_weight() is kept
+    # a head in bf16 is its own copy
+    model.lm_head.to(torch.bfloat16)
+    assert model._lm_head_rows().data_ptr() == model.lm_head.weight.data_ptr()
