@@ -9,8 +9,9 @@ The reference forms lm_head's logits and takes F.cross_entropy of them (jarvis_e
 vocabulary those are 1.6 GB in bf16.  Here they are not stored, in neither direction.
 
 These are torch.autograd functions over the calls in `ops` (which have a forward and a backward call each, for programs without
-autograd).  A captured training step takes its gradients with torch.autograd.grad, or backward() when no graph from outside the capture
-holds the same parameters' accumulators; the operators themselves launch on the current stream and synchronise with nothing.
+autograd).  Gradients formed under create_graph raise when they are differentiated.  A captured training step takes its gradients with
+torch.autograd.grad, or backward() when no graph from outside the capture holds the same parameters' accumulators; the operators
+themselves launch on the current stream and synchronise with nothing.
 
 Numerics: hidden rows and weight enter the products as bf16 (an f32 argument is rounded to it, as under autocast), sums and softmax are
 f32, the gradient of the logits is rounded to f16 for the products it enters (2^-11 of a value, relative to the call's largest factor
@@ -20,7 +21,6 @@ dtype from f32 sums.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -78,21 +78,57 @@ def _results(r, lead):
     return (None if r.ce is None else r.ce.view(lead)), (None if r.kd is None else r.kd.view(lead))
 
 
+class _FirstOnly(torch.autograd.Function):
+    """A gradient formed under create_graph: part of the graph of all it was formed from, so that whoever differentiates it meets the error
+    (without the node it would be a constant, and a penalty on gradients lose this operator's term without a word)."""
+
+    @staticmethod
+    def forward(ctx, gradient, what, *formed_from):
+        ctx.what = what
+        return gradient.view_as(gradient)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError(f"the gradients of {ctx.what} cannot be differentiated: there is no second derivative")
+
+
+def _first_only(gradients, what, formed_from):
+    formed_from = [t for t in formed_from if t is not None]
+    return tuple(g if g is None else _FirstOnly.apply(g, what, *formed_from) for g in gradients)
+
+
+def _origin(t: torch.Tensor, saved: torch.Tensor):
+    """What leads to `t`'s graph where `saved`, the form of it that is kept for the backward pass, does not: `t` itself when it is a leaf,
+    which the graph holds anyway, else an empty tensor made from it, which keeps none of its memory."""
+    if saved is t or not t.requires_grad:
+        return None
+    if t.is_leaf:
+        return t
+    with torch.enable_grad():
+        return t[..., :0].clone()
+
+
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, ids, logits, temperature, mean):
         x, w, targets, teacher, r, lead = _forward(hidden, weight, targets, ids, logits, temperature, mean)
+        ctx.origins = (_origin(hidden, x), _origin(weight, w))
         ctx.save_for_backward(x, w, targets, r.buf, None if teacher is None else teacher.buf)
         ctx.info = (hidden.shape, hidden.dtype, weight.dtype, mean, None if teacher is None else (teacher.K, teacher.vocab, teacher.temperature))
         return _results(r, lead)
 
     @staticmethod
     def backward(ctx, g_ce, g_kd):
-        return _head_backward_once(ctx, g_ce, g_kd) if torch.is_grad_enabled() else _head_backward(ctx, g_ce, g_kd)
+        saved = ctx.saved_tensors
+        if not torch.is_grad_enabled():
+            return _head_backward(ctx, saved, g_ce, g_kd)
+        with torch.no_grad():
+            got = _head_backward(ctx, saved, g_ce, g_kd)
+        return _first_only(got, "the head's losses", (*saved[:2], *ctx.origins, g_ce, g_kd))
 
 
-def _head_backward(ctx, g_ce, g_kd):
-    x, w, targets, buf, teacher = ctx.saved_tensors
+def _head_backward(ctx, saved, g_ce, g_kd):
+    x, w, targets, buf, teacher = saved
     shape, dx_dtype, dw_dtype, mean, info = ctx.info
     N = x.shape[0]
     if teacher is not None:
@@ -105,10 +141,6 @@ def _head_backward(ctx, g_ce, g_kd):
     if want_dx and len(shape) != 2:
         dx = dx.view(shape)
     return dx, dw, None, None, None, None, None
-
-
-# under create_graph: gradients that refuse to be differentiated (the wrapper's own cost is 10 us of a call)
-_head_backward_once = once_differentiable(_head_backward)
 
 
 def _head_loss(hidden, weight, targets, ids, logits, temperature, reduction):
@@ -147,23 +179,25 @@ def linear_losses(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Ten
 class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps, out_dtype):
-        x, w = x.contiguous(), weight.float().contiguous()
-        ctx.save_for_backward(x, w)
-        ctx.eps, ctx.weight_dtype = eps, weight.dtype
-        return ops.rmsnorm(x, w, eps, out_dtype)
+        rows, w = x.contiguous(), weight.float().contiguous()
+        ctx.save_for_backward(rows, w)
+        ctx.eps, ctx.weight_dtype, ctx.origins = eps, weight.dtype, (_origin(x, rows), _origin(weight, w))
+        return ops.rmsnorm(rows, w, eps, out_dtype)
 
     @staticmethod
     def backward(ctx, dy):
-        return _norm_backward_once(ctx, dy) if torch.is_grad_enabled() else _norm_backward(ctx, dy)
+        saved = ctx.saved_tensors
+        if not torch.is_grad_enabled():
+            return _norm_backward(ctx, saved, dy)
+        with torch.no_grad():
+            got = _norm_backward(ctx, saved, dy)
+        return _first_only(got, "rms_norm", (*saved, *ctx.origins, dy))
 
 
-def _norm_backward(ctx, dy):
-    x, w = ctx.saved_tensors
+def _norm_backward(ctx, saved, dy):
+    x, w = saved
     dx, dw = ops.rmsnorm_backward(x, w, dy.contiguous(), ctx.eps)
     return dx, dw if ctx.weight_dtype is torch.float32 else dw.to(ctx.weight_dtype), None, None
-
-
-_norm_backward_once = once_differentiable(_norm_backward)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, out_dtype=torch.bfloat16) -> torch.Tensor:

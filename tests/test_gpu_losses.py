@@ -774,3 +774,40 @@ def test_every_path_reads_a_head_that_a_captured_step_trains():
         graph.replay()
         _same_as_fresh(model, idx, y)
     assert (model.lm_head.weight - before).abs().max() > 2.0 ** -8 * before.abs().max()
+
+
+@pytest.mark.parametrize("how", ["bf16", "f32", "strided", "three axes"])
+@pytest.mark.parametrize("op", ["ce", "kd", "norm"])
+def test_a_penalty_on_the_gradients_is_refused(op, how):
+    """Under create_graph the first gradients are those of any pass; what is formed of them cannot be differentiated with respect to anything
+    ahead of the operator, the weight or a factor behind it."""
+    _, _, t, ids, logits = _problem(24, 300, 64, 3)
+    g = _gen(11)
+    theta = torch.randn(24, 128, generator=g, device="cuda", requires_grad=True)
+    phi = torch.randn(300 if op != "norm" else 1, 64, generator=g, device="cuda", requires_grad=True)
+    s = torch.ones((), device="cuda", requires_grad=True)
+
+    def loss():
+        h = theta.tanh()
+        if how != "f32":
+            h = h.bfloat16()
+        h = h[:, ::2] if how == "strided" else h[:, :64].contiguous()
+        if how == "three axes":
+            h = h.view(2, 12, 64)
+        w = phi.sin()
+        if op == "norm":
+            return s * losses.rms_norm(h, w[0]).float().square().sum()
+        if op == "ce":
+            return s * losses.linear_cross_entropy(h, w, t.view(h.shape[:-1]))
+        return s * losses.linear_distillation(h, w, ids.view(*h.shape[:-1], 3), logits.view(*h.shape[:-1], 3))
+    want = torch.autograd.grad(loss(), (theta, phi))
+    got = torch.autograd.grad(loss(), (theta, phi), create_graph=True)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    for first in got:
+        for by in (theta, phi, s):
+            with pytest.raises(RuntimeError, match="cannot be differentiated"):
+                torch.autograd.grad(first.square().sum(), by, retain_graph=True)
+        with pytest.raises(RuntimeError, match="cannot be differentiated"):
+            first.square().sum().backward(retain_graph=True)
+    assert theta.grad is None
