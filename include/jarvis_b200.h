@@ -421,9 +421,10 @@ size_t jb200_teacher_rows_bytes(int N, int K, int V);
 int jb200_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, void* rows, void* stream);
 
 /* ce, kd: f32 [N] or NULL, the rows' losses.  mean_ce, mean_kd: f32 [1] or NULL, their means over the rows with a target and over those
- * with a teacher (NaN without any; without rows at all both are); with either, counts: f32 [2], how many those are.  scratch:
- * jb200_head_loss_scratch_bytes (ce, kd: whether the losses are asked for). */
-size_t jb200_head_loss_scratch_bytes(int N, int V, int ce, int kd);
+ * with a teacher (NaN without any; without rows at all both are); with either, counts: f32 [2], how many those are.  scratch, 4-byte
+ * aligned: jb200_head_loss_scratch_bytes, has_targets and has_teacher being whether h->targets and h->teacher are given, whichever of
+ * the outputs are NULL (the statistics of both are formed where both are given). */
+size_t jb200_head_loss_scratch_bytes(int N, int V, int has_targets, int has_teacher);
 int jb200_head_loss(const jb200_head* h, float* ce, float* kd, float* mean_ce, float* mean_kd, float* counts, void* scratch, void* stream);
 
 /* Gradients of sum_n g_ce[n] ce[n] / *n_ce + g_kd[n] kd[n] / *n_kd: dx [N][C] and dw [V][C] (dtype 0: f32, 1: bf16), overwritten, NULL

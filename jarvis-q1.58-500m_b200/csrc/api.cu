@@ -478,7 +478,9 @@ size_t jb200_teacher_rows_bytes(int N, int K, int V) { return teacher_rows_bytes
 int jb200_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, void* rows, void* stream) {
   return launch_teacher_rows(ids, logits, logits_dtype, N, K, V, temperature, rows, static_cast<cudaStream_t>(stream));
 }
-size_t jb200_head_loss_scratch_bytes(int N, int V, int ce, int kd) { return N < 1 || V < 1 ? 0 : head_loss_scratch_bytes(N, V, ce, kd); }
+size_t jb200_head_loss_scratch_bytes(int N, int V, int has_targets, int has_teacher) {
+  return N < 1 || V < 1 ? 0 : head_loss_scratch_bytes(N, V, has_targets, has_teacher);
+}
 int jb200_head_loss(const jb200_head* h, float* ce, float* kd, float* mean_ce, float* mean_kd, float* counts, void* scratch, void* stream) {
   return launch_head_loss(h, ce, kd, mean_ce, mean_kd, counts, scratch, static_cast<cudaStream_t>(stream));
 }

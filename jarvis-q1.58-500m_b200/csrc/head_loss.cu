@@ -996,9 +996,10 @@ void set_teacher(HeadLogits& p, const jb200_head* h) {
 }
 }  // namespace
 
-size_t head_loss_scratch_bytes(int N, int V, int ce, int kd) {
+// What launch_head_loss lays out in it: the parts, z_target and the rows' losses that the caller does not ask for, the ticket.
+size_t head_loss_scratch_bytes(int N, int V, int has_targets, int has_teacher) {
   const size_t parts = (size_t(V) + HEAD_TILE - 1) / HEAD_TILE;
-  return (parts * head_values(ce != 0, kd != 0) + 3) * size_t(N) * 4 + 4;
+  return (parts * head_values(has_targets != 0, has_teacher != 0) + 3) * size_t(N) * 4 + 4;
 }
 
 int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* mean_ce, float* mean_kd, float* counts, void* scratch, cudaStream_t stream) {

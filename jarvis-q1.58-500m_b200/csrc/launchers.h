@@ -164,7 +164,7 @@ int launch_cross_entropy(const void* logits, int ld, int n_rows, int V, const in
 size_t teacher_rows_bytes(int N, int K, int V);
 int launch_teacher_rows(const int64_t* ids, const void* logits, int logits_dtype, int N, int K, int V, float temperature, void* rows,
                         cudaStream_t stream);
-size_t head_loss_scratch_bytes(int N, int V, int ce, int kd);
+size_t head_loss_scratch_bytes(int N, int V, int has_targets, int has_teacher);
 int launch_head_loss(const jb200_head* h, float* ce, float* kd, float* mean_ce, float* mean_kd, float* counts, void* scratch, cudaStream_t stream);
 size_t head_loss_backward_scratch_bytes(int N, int V, int C);
 int launch_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_stride, const float* n_ce, const float* g_kd, int g_kd_stride,

@@ -187,3 +187,18 @@ def test_the_heads_copies_follow_updates_that_leave_no_trace():
     # a head in bf16 is its own copy
     model.lm_head.to(torch.bfloat16)
     assert model._lm_head_rows().data_ptr() == model.lm_head.weight.data_ptr()
+
+
+def test_scratch_is_sized_by_what_is_given():
+    """The size goes by the inputs (targets, a teacher), which decide what the statistics hold; the names of the declaration are not those of the
+    outputs that may be NULL."""
+    import os
+    import re
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "jarvis_b200.h")).read()
+    names = re.search(r"jb200_head_loss_scratch_bytes\(([^)]*)\)", text).group(1).replace("int ", "").split(", ")
+    assert names == ["N", "V", "has_targets", "has_teacher"]
+    lib = _lib.load()
+    for N, V in ((1, 1), (37, 1000), (16384, 50257)):
+        ce, kd, both = (lib.jb200_head_loss_scratch_bytes(N, V, *f) for f in ((1, 0), (0, 1), (1, 1)))
+        tiles = (V + 255) // 256
+        assert (ce, kd, both) == tuple((tiles * k + 3) * N * 4 + 4 for k in (2, 3, 5))
