@@ -87,7 +87,7 @@ teacher_rows_kernel(const int64_t* __restrict__ ids, const T* __restrict__ logit
     if (k < K) {
       const long long y = ids[size_t(row) * K + k];
       if (y >= 0) {
-        v[i] = teacher_value(logits + size_t(row) * K + k) * inv_tau;
+        v[i] = teacher_value(logits + size_t(row) * K + k);
         if (y >= V) bad = true; else id[i] = int(y);
       }
       top = fmaxf(top, v[i]);
@@ -97,12 +97,13 @@ teacher_rows_kernel(const int64_t* __restrict__ ids, const T* __restrict__ logit
   bad = __any_sync(0xffffffffu, bad);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  // a row whose kept values are all -inf has no probabilities either (a NaN among them: NaN)
+  // a row whose kept values are all -inf has no probabilities either (a NaN among them: NaN).  The temperature divides the differences: the
+  // values themselves may be the type's lowest, which a temperature below 1 would make -inf, or its largest.
   const float base = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    v[i] -= base;
+    v[i] = (v[i] - base) * inv_tau;
     if (id[i] != INT_MAX) sum += expf(v[i]);
   }
   sum = warp_sum(sum);

@@ -811,3 +811,28 @@ def test_a_penalty_on_the_gradients_is_refused(op, how):
         with pytest.raises(RuntimeError, match="cannot be differentiated"):
             first.square().sum().backward(retain_graph=True)
     assert theta.grad is None
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("tau", [0.25, 0.5, 0.9, 1.0, 2.0])
+def test_teachers_of_the_types_largest_and_lowest_values(tau, dtype):
+    """Probabilities are those of the differences: a row whose entries all hold the type's lowest value has even ones, at any temperature, and an
+    entry far above the rest has all."""
+    h, w, _, _, _ = _problem(8, 300, 64, 4)
+    lo, hi = torch.finfo(dtype).min, torch.finfo(dtype).max
+    ids = torch.arange(8 * 4, device="cuda").view(8, 4)
+    logits = torch.tensor([[lo, lo, lo, lo], [lo, lo, 0, lo], [hi, hi, 0, lo], [hi, lo, lo, hi], [0, 0, 0, lo], [hi, hi, hi, hi],
+                           [-math.inf, lo, lo, -math.inf], [-math.inf] * 4], device="cuda").to(dtype)
+    q = torch.tensor([[1, 1, 1, 1], [0, 0, 1, 0], [1, 1, 0, 0], [1, 0, 0, 1], [1, 1, 1, 0], [1, 1, 1, 1], [0, 1, 1, 0], [0, 0, 0, 0]],
+                     device="cuda", dtype=F64)
+    # the same probabilities from ordinary values
+    plain = torch.where(q > 0, 1.0, -math.inf).float()
+    got = losses.linear_distillation(h, w, ids, logits, temperature=tau, reduction="none")
+    want = losses.linear_distillation(h, w, ids, plain, temperature=tau, reduction="none")
+    assert torch.equal(got, want) and got[7] == 0 and (got[:7] > 0).all()
+    q = q / q.sum(1, keepdim=True).clamp(min=1)
+    z = h.double() @ w.double().t()
+    lp = torch.log_softmax(z / tau, 1).gather(1, ids)
+    ref = tau * tau * (torch.special.xlogy(q, q) - q * lp).sum(1)
+    Z = (64 / 16 + 8) * 2.0 ** -23 * float((h.double().abs() @ w.double().abs().t()).max())
+    _check_rows(got, ref, Z, tau)
