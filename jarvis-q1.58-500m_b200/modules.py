@@ -655,7 +655,8 @@ class Jarvis(nn.Module):
         return self._rows(idx, persist_state, True)
 
     def _residual_rows(self, idx):
-        """Embedding + all blocks -> the f32 (B*T, C) residual stream that final_norm takes; no state is carried."""
+        """Embedding + all blocks -> the f32 (B*T, C) residual stream that final_norm takes; no state is carried, and one that a sequence in
+        progress has left stays."""
         return self._rows(idx, False, False)
 
     def _rows(self, idx, persist_state, normed):
@@ -679,8 +680,9 @@ class Jarvis(nn.Module):
             else:
                 out = torch.empty((B * T, self.d_model), dtype=torch.float32, device=idx.device)
                 r = chain.run(tab, out, B, T, ids=idx, table=_f32(self.tok_emb.weight), start_pos=start_pos)
-            self._h_states = r.h
-            self._attn_states = r.S if r.S is not None else [None] * tab.n
+            if normed:
+                self._h_states = r.h
+                self._attn_states = r.S if r.S is not None else [None] * tab.n
             self._aux, self._reflect = r.scalars, r.reflect
             return out
         self._reflect = None
@@ -700,16 +702,16 @@ class Jarvis(nn.Module):
             if s_prev is not None and s_prev.shape[0] != B:
                 s_prev = None
             h_last, sc, state = block.forward_rows(x, B, T, h_prev, start_pos, s_prev,
-                                                   want_attn_state=self.carry_attention_state, scratch=scratch[i],
+                                                   want_attn_state=self.carry_attention_state and normed, scratch=scratch[i],
                                                    cp=self._cp)
             new_h.append(h_last)
             new_s.append(state)
             aux.append(sc)
-        self._h_states = new_h
-        self._attn_states = new_s
         self._aux = aux
         if not normed:
             return x
+        self._h_states = new_h
+        self._attn_states = new_s
         return ops.rmsnorm(x, _f32(self.final_norm.weight), self.final_norm.eps)
 
     @torch.no_grad()

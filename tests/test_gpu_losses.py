@@ -836,3 +836,19 @@ def test_teachers_of_the_types_largest_and_lowest_values(tau, dtype):
     ref = tau * tau * (torch.special.xlogy(q, q) - q * lp).sum(1)
     Z = (64 / 16 + 8) * 2.0 ** -23 * float((h.double().abs() @ w.double().abs().t()).max())
     _check_rows(got, ref, Z, tau)
+
+
+@pytest.mark.parametrize("use_chain", [True, False])
+def test_training_the_head_leaves_a_carried_state_alone(use_chain):
+    """A sequence in progress goes on as if no head_loss had come between."""
+    g = _gen(12)
+    idx, y = (torch.randint(0, 301, (2, 20), generator=g, device="cuda") for _ in range(2))
+    out = []
+    for between in (False, True):
+        model = _model()
+        model.use_chain, model.carry_attention_state = use_chain, True
+        model(idx, persist_state=True)
+        if between:
+            model.head_loss(y, idx)
+        out.append(model(y, persist_state=True)[0])
+    assert torch.equal(*out)
