@@ -9,9 +9,9 @@ The reference forms lm_head's logits and takes F.cross_entropy of them (jarvis_e
 vocabulary those are 1.6 GB in bf16.  Here they are not stored, in neither direction.
 
 These are torch.autograd functions over the calls in `ops` (which have a forward and a backward call each, for programs without
-autograd).  Gradients formed under create_graph raise when they are differentiated.  A captured training step takes its gradients with
-torch.autograd.grad, or backward() when no graph from outside the capture holds the same parameters' accumulators; the operators
-themselves launch on the current stream and synchronise with nothing.
+autograd).  Gradients formed under create_graph raise when they are differentiated, and tensors with a forward-mode tangent are refused.
+A captured training step takes its gradients with torch.autograd.grad, or backward() when no graph from outside the capture holds the
+same parameters' accumulators; the operators themselves launch on the current stream and synchronise with nothing.
 
 Numerics: hidden rows and weight enter the products as bf16 (an f32 argument is rounded to it, as under autocast), sums and softmax are
 f32, the gradient of the logits is rounded to f16 for the products it enters (2^-11 of a value, relative to the call's largest factor
@@ -21,6 +21,7 @@ dtype from f32 sums.
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import ops
 
@@ -37,6 +38,13 @@ def _trains(weight: torch.Tensor):
     """Marks a weight that is about to get a gradient: updates may leave no trace on it, so nobody keeps a copy (modules._in_training)."""
     if weight.requires_grad:
         weight._jb_trained = True
+
+
+def _no_tangents(what: str, *tensors):
+    """Dual tensors do not require gradients: their tangents would go missing where nothing else does."""
+    for t in tensors:
+        if t is not None and unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what}: a tensor carries a tangent, and there is no forward-mode derivative")
 
 
 def _rows(t: torch.Tensor, lead, dtypes, what: str, columns: int | None = None) -> torch.Tensor:
@@ -146,6 +154,9 @@ def _head_backward(ctx, saved, g_ce, g_kd):
 def _head_loss(hidden, weight, targets, ids, logits, temperature, reduction):
     if reduction not in ("mean", "none"):
         raise RuntimeError(f"reduction must be 'mean' or 'none', got {reduction!r}")
+    _no_tangents("the head's losses", hidden, weight, logits)
+    if logits is not None and logits.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("teacher_logits: no gradient is formed for them; pass them detached")
     mean = reduction == "mean"
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         _trains(weight)
@@ -165,8 +176,8 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids:
                         temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
     """t^2 KL(softmax(teacher_logits / t) over the row's entries || softmax(hidden @ weight.T / t)), t the temperature, differentiable in
     hidden and weight.  teacher_ids: int64 (..., K), teacher_logits: f32 or bf16 (..., K), K <= 256, in any order; a negative id is no
-    entry, a row without entries has no part (loss 0), an id beyond the vocabulary makes its row NaN.  "mean": over the
-    rows with entries."""
+    entry, a row without entries has no part (loss 0), an id beyond the vocabulary makes its row NaN.  No gradient is formed for
+    teacher_logits: ones that require one are refused.  "mean": over the rows with entries."""
     return _head_loss(hidden, weight, None, teacher_ids, teacher_logits, temperature, reduction)[1]
 
 
@@ -204,6 +215,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, out_dtype
     """RMSNorm.forward (jarvis_engine/jarvis_model.py:25-26) over the last axis, differentiable in x (f32 or bf16) and weight."""
     if weight.dim() != 1 or x.dim() < 1 or weight.shape[0] != x.shape[-1]:
         raise RuntimeError(f"rms_norm: weight {tuple(weight.shape)} does not fit rows of {tuple(x.shape)}")
+    _no_tangents("rms_norm", x, weight)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         _trains(weight)
         return _RMSNorm.apply(x, weight, eps, out_dtype)

@@ -202,3 +202,24 @@ def test_scratch_is_sized_by_what_is_given():
         ce, kd, both = (lib.jb200_head_loss_scratch_bytes(N, V, *f) for f in ((1, 0), (0, 1), (1, 1)))
         tiles = (V + 255) // 256
         assert (ce, kd, both) == tuple((tiles * k + 3) * N * 4 + 4 for k in (2, 3, 5))
+
+
+def test_tangents_and_a_teachers_gradient_are_refused():
+    """Neither is formed, so neither is dropped without a word."""
+    import torch.autograd.forward_ad as fw
+    h, w, t = torch.zeros(4, 64), torch.zeros(100, 64), torch.zeros(4, dtype=torch.int64)
+    ids, lg = torch.zeros(4, 3, dtype=torch.int64), torch.zeros(4, 3)
+    with fw.dual_level():
+        dual = lambda x: fw.make_dual(x, torch.ones_like(x))         # noqa: E731
+        for call in (lambda: losses.linear_cross_entropy(dual(h), w, t), lambda: losses.linear_cross_entropy(h, dual(w), t),
+                     lambda: losses.linear_distillation(h, w, ids, dual(lg)), lambda: losses.linear_losses(dual(h), w, t, ids, lg),
+                     lambda: losses.rms_norm(dual(h), torch.ones(64)), lambda: losses.rms_norm(h, dual(torch.ones(64)))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="tangent"):
+                    call()
+    lg.requires_grad_()
+    for call in (lambda: losses.linear_distillation(h, w, ids, lg), lambda: losses.linear_losses(h, w, t, ids, lg)):
+        with pytest.raises(RuntimeError, match="teacher_logits: no gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensor"):      # nothing to lose here
+            call()
