@@ -441,8 +441,8 @@ int jb200_host_head_plan(int N, int V, int C, int sms, int32_t* out3);
  * a short one's, -1 behind the last. */
 int jb200_host_head_walk(int n_long, int k_long, int n_short, int k_short, int pairs, int pair, int i);
 
-/* Gradient of jb200_rmsnorm: dx (x's dtype) and dw f32 [C], both overwritten; statistics are formed anew from x.  C a multiple of 8, at
- * most 4096.  dw is summed in f32 in a fixed order.  scratch: jb200_rmsnorm_backward_scratch_bytes (few rows need none). */
+/* Gradient of jb200_rmsnorm: dx (x's dtype; NULL where not wanted) and dw f32 [C], both overwritten; statistics are formed anew from x.  C
+ * a multiple of 8, at most 4096.  dw is summed in f32 in a fixed order.  scratch: jb200_rmsnorm_backward_scratch_bytes (few rows need none). */
 size_t jb200_rmsnorm_backward_scratch_bytes(int n_rows, int C);
 int jb200_rmsnorm_backward(const void* x, int x_dtype, const float* w, float eps, const void* dy, int dy_dtype, int n_rows, int C, void* dx,
                            float* dw, void* scratch, void* stream);

@@ -39,7 +39,7 @@ __device__ __forceinline__ float cluster_ld(uint32_t addr) {
   return v;
 }
 
-// WPR: warps of a row (1, 2 or 4).  ONE: the grid is one cluster and leaves dw itself in dw_part.
+// WPR: warps of a row (1, 2 or 4).  ONE: the grid is one cluster and leaves dw itself in dw_part.  dx: null where not wanted.
 template <typename TX, typename TY, int WPR, bool ONE>
 __global__ void __launch_bounds__(32 * NG_WARPS, 2)
 rmsnorm_backward_kernel(const TX* __restrict__ x, const float* __restrict__ w, float eps, const TY* __restrict__ dy, int n_rows, int C,
@@ -101,7 +101,7 @@ rmsnorm_backward_kernel(const TX* __restrict__ x, const float* __restrict__ w, f
     }
     if (on) {
       const float r = rsqrtf(ss * inv_c + eps), k = along * inv_c * r * r;      // dx = r (w dy - x k)
-      TX* dr = dx + size_t(row) * C;
+      TX* dr = dx ? dx + size_t(row) * C : nullptr;
 #pragma unroll
       for (int i = 0; i < NG_VEC; ++i)
         if (c0 + i * 256 < C) {
@@ -113,7 +113,7 @@ rmsnorm_backward_kernel(const TX* __restrict__ x, const float* __restrict__ w, f
             acc[i][j] = fmaf(g[i][j], xv[i][j] * r, acc[i][j]);
             o[j] = r * fmaf(-xv[i][j], k, wv[j] * g[i][j]);
           }
-          ng_store8(dr + c0 + i * 256, o);
+          if (dr) ng_store8(dr + c0 + i * 256, o);
         }
     }
   }
@@ -222,7 +222,7 @@ int launch_rmsnorm_backward(const void* x, int x_dtype, const float* w, float ep
     JB_CUDA(cudaMemsetAsync(dw, 0, size_t(C) * 4, stream));
     return JB200_OK;
   }
-  JB_REQUIRE(x && w && dy && dx && (scratch || norm_cluster(n_rows, C)), "rmsnorm_backward: null pointer");
+  JB_REQUIRE(x && w && dy && (scratch || norm_cluster(n_rows, C)), "rmsnorm_backward: null pointer");
   JB_REQUIRE(aligned16(x) && aligned16(w) && aligned16(dy) && aligned16(dx), "rmsnorm_backward: pointers must be 16-byte aligned");
   const int sms = sm_count();
   if (sms < 1) return JB200_ERR_CUDA;

@@ -207,8 +207,9 @@ class _RMSNorm(torch.autograd.Function):
 
 def _norm_backward(ctx, saved, dy):
     x, w = saved
-    dx, dw = ops.rmsnorm_backward(x, w, dy.contiguous(), ctx.eps)
-    return dx, dw if ctx.weight_dtype is torch.float32 else dw.to(ctx.weight_dtype), None, None
+    want_dx, want_dw = ctx.needs_input_grad[:2]
+    dx, dw = ops.rmsnorm_backward(x, w, dy.contiguous(), ctx.eps, want_dx=want_dx)
+    return dx, dw.to(ctx.weight_dtype) if want_dw else None, None, None
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, out_dtype=torch.bfloat16) -> torch.Tensor:

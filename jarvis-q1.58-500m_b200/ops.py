@@ -730,8 +730,9 @@ def head_loss_backward(x: torch.Tensor, w: torch.Tensor, fwd: HeadLoss, targets:
     return dx, dw
 
 
-def rmsnorm_backward(x: torch.Tensor, weight: torch.Tensor, dy: torch.Tensor, eps: float = 1e-6):
-    """Gradients (dx of x's dtype, dweight f32) of rmsnorm for the output's gradient dy (f32 or bf16, x's shape)."""
+def rmsnorm_backward(x: torch.Tensor, weight: torch.Tensor, dy: torch.Tensor, eps: float = 1e-6, *, want_dx: bool = True):
+    """Gradients (dx of x's dtype, dweight f32) of rmsnorm for the output's gradient dy (f32 or bf16, x's shape).  dx is None, and
+    not stored, where it is not wanted."""
     lib = _lib.load()
     tx, ty = _dt(x), _dt(dy)
     _need(x, x.dtype, "rmsnorm_backward.x")
@@ -743,12 +744,12 @@ def rmsnorm_backward(x: torch.Tensor, weight: torch.Tensor, dy: torch.Tensor, ep
     _together("rmsnorm_backward", x, weight, dy)
     if _elsewhere(x):
         with torch.cuda.device(x.device):
-            return rmsnorm_backward(x, weight, dy, eps)
+            return rmsnorm_backward(x, weight, dy, eps, want_dx=want_dx)
     rows = x.numel() // width if width else 0
-    dx, dw = torch.empty_like(x), torch.empty_like(weight)
+    dx, dw = torch.empty_like(x) if want_dx else None, torch.empty_like(weight)
     nbytes = lib.jb200_rmsnorm_backward_scratch_bytes(rows, width)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    _lib.check(lib.jb200_rmsnorm_backward(x.data_ptr(), tx, weight.data_ptr(), eps, dy.data_ptr(), ty, rows, width, dx.data_ptr(), dw.data_ptr(),
+    _lib.check(lib.jb200_rmsnorm_backward(x.data_ptr(), tx, weight.data_ptr(), eps, dy.data_ptr(), ty, rows, width, _ptr(dx), dw.data_ptr(),
                                           _ptr(scratch), _stream()), "jb200_rmsnorm_backward")
     return dx, dw
 

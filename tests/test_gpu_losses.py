@@ -852,3 +852,25 @@ def test_training_the_head_leaves_a_carried_state_alone(use_chain):
             model.head_loss(y, idx)
         out.append(model(y, persist_state=True)[0])
     assert torch.equal(*out)
+
+
+@pytest.mark.parametrize("N,width", [(37, 1024), (300, 1024), (3, 4096)])
+def test_norm_gradients_that_are_not_wanted_are_not_formed(N, width, monkeypatch):
+    g = _gen(13)
+    x = torch.randn(N, width, generator=g, device="cuda")
+    w = torch.randn(width, generator=g, device="cuda")
+    dy = torch.randn(N, width, generator=g, device="cuda").bfloat16()
+    dx, dw = ops.rmsnorm_backward(x, w, dy)
+    none, alone = ops.rmsnorm_backward(x, w, dy, want_dx=False)
+    assert none is None and torch.equal(alone, dw)
+    seen, inner = [], ops.rmsnorm_backward
+    monkeypatch.setattr(ops, "rmsnorm_backward", lambda *a, **k: seen.append(k) or inner(*a, **k))
+    for want in (False, True):
+        xx = x.clone().requires_grad_(want)
+        ww = w.clone().requires_grad_()
+        losses.rms_norm(xx, ww).backward(dy)
+        assert torch.equal(ww.grad, dw) and (torch.equal(xx.grad, dx) if want else xx.grad is None)
+    assert [k["want_dx"] for k in seen] == [False, True]
+    xx, ww = x.clone().requires_grad_(), w.clone()
+    losses.rms_norm(xx, ww).backward(dy)
+    assert torch.equal(xx.grad, dx)
