@@ -346,6 +346,7 @@ def test_infinite_and_extreme_logits():
     assert (dx == 0).all() and (dw == 0).all()
 
 
+# (What is rounded is f16 by now: the bound below is f16's, 2^-12 of a target's entry, where the docstring names bf16's 2^-9.)
 def test_gradients_of_equal_rows_have_no_common_rounding():
     """1 / rows is no factor of what is rounded to bf16: with flat probabilities a target's entry is -1 + 1 / V, and the gradients of
     2047 rows are as good as those of 2048.  (-1 + 1 / V rounds to -1: 2^-9 of 1 / V for the rest of the row.)"""
@@ -874,3 +875,10 @@ def test_norm_gradients_that_are_not_wanted_are_not_formed(N, width, monkeypatch
     xx, ww = x.clone().requires_grad_(), w.clone()
     losses.rms_norm(xx, ww).backward(dy)
     assert torch.equal(xx.grad, dx)
+
+
+@pytest.mark.parametrize("dtype,dy_dtype", [(torch.float32, BF16), (BF16, torch.float32)])
+@pytest.mark.parametrize("N,width", [(1, 4096), (2, 2056), (33, 2056), (64, 4096), (65, 4096), (128, 2048), (129, 2048), (256, 1024), (257, 1024)])
+def test_norm_gradients_at_the_limits_of_one_cluster(N, width, dtype, dy_dtype):
+    """Rows on one, two and four warps, in one cluster up to 256, 128 and 64 rows and beyond."""
+    test_norm_gradients(N, width, dtype, dy_dtype)

@@ -223,3 +223,49 @@ def test_tangents_and_a_teachers_gradient_are_refused():
             call()
         with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensor"):      # nothing to lose here
             call()
+
+
+def test_the_heads_calls_launch_on_their_tensors_card(monkeypatch):
+    current, seen = [0], []
+
+    class Card:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Lib:
+        def __getattr__(self, name):
+            if name.endswith("_bytes"):
+                return lambda *a: 64
+            return lambda *a: seen.append((name, current[0])) or 0
+
+    real = {n: getattr(torch, n) for n in ("empty", "empty_like")}
+    monkeypatch.setattr(ops._lib, "load", lambda: Lib())
+    monkeypatch.setattr(ops, "_raw_device", lambda: current[0])
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops.torch.cuda, "device", Card)
+    monkeypatch.setattr(ops.torch, "empty", lambda s, dtype=None, device=None: _on(device.index, s if isinstance(s, tuple) else (s,), dtype=dtype))
+    monkeypatch.setattr(ops.torch, "empty_like", lambda t, dtype=None: real["empty_like"](t, dtype=dtype).as_subclass(_OnCard))
+
+    def rows(card):
+        bf, i64 = torch.bfloat16, torch.int64
+        return _on(card, 4, 64, dtype=bf), _on(card, 100, 64, dtype=bf), _on(card, 4, dtype=i64), _on(card, 4, 3, dtype=i64), _on(card, 4, 3), _on(card, 1)
+    for card in (1, 0):
+        x, w, t, ids, lg, g = rows(card)
+        teacher = ops.teacher_rows(ids, lg, 100)
+        r = ops.head_loss(x, w, t, teacher)
+        ops.head_loss_backward(x, w, r, t, teacher, g_ce=g, g_kd=g)
+        assert seen == [(n, card) for n in ("jb200_teacher_rows", "jb200_head_loss", "jb200_head_loss_backward")] and current == [0]
+        seen.clear()
+    x, w, t, ids, lg, g = rows(0)
+    _, w1, t1, _, lg1, g1 = rows(1)
+    for call in (lambda: ops.teacher_rows(ids, lg1, 100), lambda: ops.head_loss(x, w1, t), lambda: ops.head_loss(x, w, t1),
+                 lambda: ops.head_loss_backward(x, w, r, t, teacher, g_ce=g1, g_kd=g)):
+        with pytest.raises(RuntimeError, match="cuda:0 and cuda:1"):
+            call()
+    assert not seen
