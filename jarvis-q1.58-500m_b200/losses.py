@@ -21,7 +21,7 @@ dtype from f32 sums.
 from __future__ import annotations
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 
 from . import ops
 
@@ -42,8 +42,10 @@ def _trains(weight: torch.Tensor):
 
 def _no_tangents(what: str, *tensors):
     """Dual tensors do not require gradients: their tangents would go missing where nothing else does."""
+    if getattr(forward_ad, "_current_level", 0) < 0:       # outside every dual_level there are none
+        return
     for t in tensors:
-        if t is not None and unpack_dual(t).tangent is not None:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise RuntimeError(f"{what}: a tensor carries a tangent, and there is no forward-mode derivative")
 
 
@@ -209,7 +211,9 @@ def _norm_backward(ctx, saved, dy):
     x, w = saved
     want_dx, want_dw = ctx.needs_input_grad[:2]
     dx, dw = ops.rmsnorm_backward(x, w, dy.contiguous(), ctx.eps, want_dx=want_dx)
-    return dx, dw.to(ctx.weight_dtype) if want_dw else None, None, None
+    if not want_dw:
+        return dx, None, None, None
+    return dx, dw if ctx.weight_dtype is torch.float32 else dw.to(ctx.weight_dtype), None, None
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, out_dtype=torch.bfloat16) -> torch.Tensor:
