@@ -186,6 +186,7 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
       const uint32_t acc = tile & 1u;
       const int row = it.m0 + rank * (HEAD_TILE / 2) + quarter * 32 + lane;
       const bool on = row < (it.is_dw ? p.n_cols : p.N);
+      const float by = !it.is_dw && on ? row_scale(p.grads, row, common) : common;
       if (!mbar_wait(smem_u32(&ctl->acc_full[acc]), (tile >> 1) & 1u, abort_flag, p.status, JB200_STATUS_HEAD_EPILOGUE)) break;
       tc_fence_after_sync();
       __syncwarp();
@@ -199,7 +200,7 @@ head_products_kernel(const __grid_constant__ CUtensorMap tmap_g, const __grid_co
         if (on) {
           const float unit = it.is_dw ? dw_unit : dx_unit;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(common * (unit * __uint_as_float(v[j])));
+          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(by * (unit * __uint_as_float(v[j])));
           const int n = min(32, p.C - col);
           if (!it.is_dw) {
             const size_t o = size_t(row) * p.C + col;

@@ -305,14 +305,17 @@ __device__ __forceinline__ uint32_t f16x2_of_bf16x2(uint32_t w, float factor) {
 }
 // With few rows of x the weight's copy is what the launch waits for (37 rows of 50257 x 1024: 47 us where the logits alone take 26, and
 // HBM 32 for the weight and its copy; four warps: 65; loads ahead of the conversion, or each CTA the rows that its products read:
-// no change).  Rows that take no part become zeros, so that a NaN or an infinity in one does not reach the others' sums.
-template <typename Live>
-__device__ __forceinline__ void copy_f16(const uint4* src, uint4* dst, int n_rows, int C, float factor, int warp, int lane, Live live_row) {
+// no change).  Rows that take no part (a factor of 0) become zeros, so that a NaN or an infinity in one does not reach the others' sums.
+template <typename Factor>
+__device__ __forceinline__ void copy_f16(const uint4* src, uint4* dst, int n_rows, int C, int warp, int lane, Factor row_factor_of) {
   constexpr int R = 4;
   const int per_row = C / 8, pitch = head_pitch(C) / 8, step = int(gridDim.x) * COPY_WARPS * R;
   for (int r0 = (int(blockIdx.x) * COPY_WARPS + warp) * R; r0 < n_rows; r0 += step) {
-    const bool live = lane < R && r0 + lane < n_rows && live_row(r0 + lane);
-    const unsigned rows = __ballot_sync(0xffffffffu, live);
+    const float mine = lane < R && r0 + lane < n_rows ? row_factor_of(r0 + lane) : 0.f;
+    const unsigned rows = __ballot_sync(0xffffffffu, mine != 0.f);
+    float factor[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) factor[i] = __shfl_sync(0xffffffffu, mine, i);
     for (int c = lane; c < per_row; c += 64) {
       uint4 v[R][2];
 #pragma unroll
@@ -325,8 +328,8 @@ __device__ __forceinline__ void copy_f16(const uint4* src, uint4* dst, int n_row
 #pragma unroll
         for (int u = 0; u < 2; ++u)
           if (r0 + i < n_rows && c + 32 * u < per_row)
-            dst[size_t(r0 + i) * pitch + c + 32 * u] = make_uint4(f16x2_of_bf16x2(v[i][u].x, factor), f16x2_of_bf16x2(v[i][u].y, factor),
-                                                                 f16x2_of_bf16x2(v[i][u].z, factor), f16x2_of_bf16x2(v[i][u].w, factor));
+            dst[size_t(r0 + i) * pitch + c + 32 * u] = make_uint4(f16x2_of_bf16x2(v[i][u].x, factor[i]), f16x2_of_bf16x2(v[i][u].y, factor[i]),
+                                                                 f16x2_of_bf16x2(v[i][u].z, factor[i]), f16x2_of_bf16x2(v[i][u].w, factor[i]));
     }
   }
 }
@@ -334,8 +337,6 @@ __device__ __forceinline__ void copy_f16(const uint4* src, uint4* dst, int n_row
 template <bool CE, bool KD>
 __device__ __forceinline__ void make_copies(const HeadLogits& p, int warp, int lane) {
   int ew, ex;
-  const auto live = [&](int row) { return row_is_live<CE, KD>(p.grads, row); };
-  const auto all = [](int) { return true; };
   if (p.v0 == 0) {
     ew = copy_exponent(range_top(p.tops, p.n_tops, lane));
     ex = copy_exponent(range_top(p.tops + HEAD_RANGE_CTAS, p.n_tops, lane));
@@ -344,8 +345,13 @@ __device__ __forceinline__ void make_copies(const HeadLogits& p, int warp, int l
     ew = p.exps[0];
     ex = p.exps[1];
   }
-  if (p.xs) copy_f16(p.x, p.xs, p.N, p.C, ldexpf(1.f, ex), warp, lane, live);
-  if (p.ws) copy_f16(p.w + size_t(p.v0) * (p.C / 8), p.ws, p.cols, p.C, ldexpf(1.f, ew), warp, lane, all);
+  if (p.xs) {
+    const float scale = head_scale(p.grads);
+    copy_f16(p.x, p.xs, p.N, p.C, warp, lane, [&](int row) {
+      return row_is_live<CE, KD>(p.grads, row) ? ldexpf(1.f, ex - row_halvings(p.grads, row, scale)) : 0.f;
+    });
+  }
+  if (p.ws) copy_f16(p.w + size_t(p.v0) * (p.C / 8), p.ws, p.cols, p.C, warp, lane, [f = ldexpf(1.f, ew)](int) { return f; });
 }
 
 template <bool CE, bool KD>
@@ -472,7 +478,7 @@ head_logits_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
         if (y >= f0 && y < f_end) target = int(y) - f0;
       }
       RowGrad<CE, KD> rg;
-      if (GRAD && on) rg.load(p.grads, row, scale);
+      if (GRAD && on) rg.load(p.grads, row, row_scale(p.grads, row, scale));
       if (!mbar_wait(smem_u32(&ctl->acc_full[group]), ph, abort_flag, p.status, JB200_STATUS_HEAD_EPILOGUE)) break;
       tc_fence_after_sync();
       __syncwarp();
@@ -759,14 +765,9 @@ __device__ void head_scale_job(const HeadGrads& p) {
   __shared__ float s_top[2][32];
   float ce = 0.f, kd = 0.f;
   for (int r = threadIdx.x; r < p.N; r += RANGE_THREADS) {
-    if (p.targets && p.targets[r] != -100) {
-      const float c = fabsf(row_factor(p.g_ce, p.g_ce_stride, p.n_ce, r));
-      if (c <= FLT_MAX) ce = fmaxf(ce, c);
-    }
-    if (p.neg_entropy && p.neg_entropy[r] != INFINITY) {
-      const float c = fabsf(row_factor(p.g_kd, p.g_kd_stride, p.n_kd, r)) * p.tau;
-      if (c <= FLT_MAX) kd = fmaxf(kd, c);
-    }
+    const float2 f = row_factors(p, r);
+    ce = fmaxf(ce, f.x);
+    kd = fmaxf(kd, f.y);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {

@@ -26,8 +26,10 @@ struct HeadGrads {
 };
 
 #if defined(__CUDACC__)
-// The gradients of the logits are kept relative to one factor of the whole call, the largest there is, which the products apply to their
-// f32 sums.  (With 1 / rows in them a target's entry, -1 / rows and half of a row's gradient, had the same rounding in every row.)
+// The gradients of the logits are kept relative to a factor, which the products apply to their f32 sums.  (With 1 / rows in them a
+// target's entry, -1 / rows and half of a row's gradient, had the same rounding in every row.)  It is the largest of the whole call,
+// and with gradients row by row that times the power of two by which the row's own is smaller: a light row keeps its bits, dx has its
+// factor back as a row of the product, and for dw, which sums over rows, the copy of its hidden row is smaller by that power of two.
 __device__ __forceinline__ float common_factor(float ce, float kd) {
   const float s = ce <= 3.4e38f && !(kd <= 3.4e38f && kd > ce) ? ce : kd;
   return s > 0.f && s <= 3.4e38f ? s : 1.f;
@@ -40,12 +42,37 @@ __device__ __forceinline__ float head_scale(const HeadGrads& p) {
   if (p.scale) return *p.scale;
   return common_factor(p.targets ? fabsf(row_factor(p.g_ce, 0, p.n_ce, 0)) : 0.f, p.neg_entropy ? fabsf(row_factor(p.g_kd, 0, p.n_kd, 0)) * p.tau : 0.f);
 }
+// Largest finite factors of a row, 0 for a loss that it has no part in.
+__device__ __forceinline__ float2 row_factors(const HeadGrads& p, int row) {
+  float2 f = make_float2(0.f, 0.f);
+  if (p.targets && p.targets[row] != -100) {
+    const float c = fabsf(row_factor(p.g_ce, p.g_ce_stride, p.n_ce, row));
+    if (c <= 3.4e38f) f.x = c;
+  }
+  if (p.neg_entropy && p.neg_entropy[row] != INFINITY) {
+    const float c = fabsf(row_factor(p.g_kd, p.g_kd_stride, p.n_kd, row)) * p.tau;
+    if (c <= 3.4e38f) f.y = c;
+  }
+  return f;
+}
+// How many times the call's factor is halved for a row: until its own is more than half of what is left.
+__device__ __forceinline__ int row_halvings(const HeadGrads& p, int row, float scale) {
+  if (!p.scale) return 0;
+  const float2 v = row_factors(p, row);
+  const float f = fmaxf(v.x, v.y);
+  if (!(f > 0.f && f <= scale)) return 0;
+  const int k = ilogbf(scale) - ilogbf(f);
+  return f > ldexpf(scale, -k) ? k - 1 : k;
+}
+__device__ __forceinline__ float row_scale(const HeadGrads& p, int row, float scale) {
+  return p.scale ? ldexpf(scale, -row_halvings(p, row, scale)) : scale;
+}
 #endif
 
 // Operands of the gradient's products are f16, whose rounding is an eighth of bf16's: the logits' gradients times 2^13 (at most 2 of them
 // add up to 2^14; they keep all their bits down to 2^-27 and vanish below 2^-38), and copies of weight and rows times the powers of two by
 // which the largest finite value of each comes to lie in [2^15, 2^16).  A bf16 value within 2^32 of that is exact there, a smaller one off
-// by at most 2^-40 of the largest.  (As bf16 the logits' gradients gave dx and dW an error of sqrt(2) times their own rounding.)
+// by at most 2^-40 of the largest; the rows' values count as halved with their factors there.  (As bf16 the logits' gradients gave dx and dW an error of sqrt(2) times their own rounding.)
 constexpr int HEAD_G_EXP = 13, HEAD_RANGE_CTAS = 512;
 
 // How a backward pass is cut: `pieces` pieces of `cols` vocabulary columns (the last one shorter) whose gradients of the logits are

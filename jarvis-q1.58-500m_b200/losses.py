@@ -14,9 +14,10 @@ A captured training step takes its gradients with torch.autograd.grad, or backwa
 same parameters' accumulators; the operators themselves launch on the current stream and synchronise with nothing.
 
 Numerics: hidden rows and weight enter the products as bf16 (an f32 argument is rounded to it, as under autocast), sums and softmax are
-f32, the gradient of the logits is rounded to f16 for the products it enters (2^-11 of a value, relative to the call's largest factor
-down to 2^-38; rows and weight enter those exactly within 2^32 of their largest value), gradients are returned in their argument's
-dtype from f32 sums.
+f32, the gradient of the logits is rounded to f16 for the products it enters (2^-12 of a value down to 2^-27 of the row's factor in the
+loss, whatever the other rows' are; values below 2^-38 of it are lost), rows and weight enter those exactly within 2^32 of their
+largest value (in the weight's gradient: of a row's value times its factor), gradients are returned in their argument's dtype from f32
+sums.
 """
 from __future__ import annotations
 

@@ -882,3 +882,31 @@ def test_norm_gradients_that_are_not_wanted_are_not_formed(N, width, monkeypatch
 def test_norm_gradients_at_the_limits_of_one_cluster(N, width, dtype, dy_dtype):
     """Rows on one, two and four warps, in one cluster up to 256, 128 and 64 rows and beyond."""
     test_norm_gradients(N, width, dtype, dy_dtype)
+
+
+@pytest.mark.parametrize("mode", ["ce", "kd", "both"])
+def test_rows_of_very_uneven_weights(mode):
+    """Rows weighted down to 2^-30 of the heaviest, some not at all: a row's own gradient is as good as if it were alone, and the weight's is off by
+    no more than the heaviest rows' share allows."""
+    N, V, width = 64, 5000, 128
+    h, w, t, ids, logits = _problem(N, V, width, 5)
+    t, ids = (t if mode != "kd" else None), (ids if mode != "ce" else None)
+    a = 2.0 ** -(torch.arange(N, device="cuda").float() % 31)
+    a[5] = 0
+    b = a.flip(0) if mode == "both" else a
+    x, wt = h.float().requires_grad_(), w.float().requires_grad_()
+    if mode == "ce":
+        loss = (losses.linear_cross_entropy(x, wt, t, reduction="none") * a).sum()
+    elif mode == "kd":
+        loss = (losses.linear_distillation(x, wt, ids, logits, temperature=2.0, reduction="none") * b).sum()
+    else:
+        ce, kd = losses.linear_losses(x, wt, t, ids, logits, temperature=2.0, reduction="none")
+        loss = (ce * a).sum() + (kd * b).sum()
+    dx, dw = torch.autograd.grad(loss, (x, wt))
+    want = _definition(h, w, t, ids, logits, 2.0, a, b)
+    # dx: the last term of its bound goes by the row's own factor instead of the call's
+    own = torch.maximum(a if t is not None else 0 * a, 2 * b if ids is not None else 0 * b).double()[:, None]
+    call = float(own.max())
+    column = w.double().abs().sum(0)
+    _check_grad(dx, want["dx"], want["dx_bound"] - 2.0 ** -38 * call * column + 2.0 ** -37 * own * column)
+    _check_grad(dw, want["dw"], want["dw_bound"] + 2.0 ** -38 * call * N * h.double().abs().max())
