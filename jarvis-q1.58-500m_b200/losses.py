@@ -123,7 +123,7 @@ class _HeadLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, ids, logits, temperature, mean):
         x, w, targets, teacher, r, lead = _forward(hidden, weight, targets, ids, logits, temperature, mean)
-        ctx.origins = (_origin(hidden, x), _origin(weight, w))
+        ctx.origins = None if x is hidden and w is weight else (_origin(hidden, x), _origin(weight, w))
         ctx.save_for_backward(x, w, targets, r.buf, None if teacher is None else teacher.buf)
         ctx.info = (hidden.shape, hidden.dtype, weight.dtype, mean, None if teacher is None else (teacher.K, teacher.vocab, teacher.temperature))
         return _results(r, lead)
@@ -135,7 +135,7 @@ class _HeadLoss(torch.autograd.Function):
             return _head_backward(ctx, saved, g_ce, g_kd)
         with torch.no_grad():
             got = _head_backward(ctx, saved, g_ce, g_kd)
-        return _first_only(got, "the head's losses", (*saved[:2], *ctx.origins, g_ce, g_kd))
+        return _first_only(got, "the head's losses", (*saved[:2], *(ctx.origins or ()), g_ce, g_kd))
 
 
 def _head_backward(ctx, saved, g_ce, g_kd):
@@ -195,7 +195,7 @@ class _RMSNorm(torch.autograd.Function):
     def forward(ctx, x, weight, eps, out_dtype):
         rows, w = x.contiguous(), weight.float().contiguous()
         ctx.save_for_backward(rows, w)
-        ctx.eps, ctx.weight_dtype, ctx.origins = eps, weight.dtype, (_origin(x, rows), _origin(weight, w))
+        ctx.eps, ctx.weight_dtype, ctx.origins = eps, weight.dtype, None if rows is x and w is weight else (_origin(x, rows), _origin(weight, w))
         return ops.rmsnorm(rows, w, eps, out_dtype)
 
     @staticmethod
@@ -205,7 +205,7 @@ class _RMSNorm(torch.autograd.Function):
             return _norm_backward(ctx, saved, dy)
         with torch.no_grad():
             got = _norm_backward(ctx, saved, dy)
-        return _first_only(got, "rms_norm", (*saved, *ctx.origins, dy))
+        return _first_only(got, "rms_norm", (*saved, *(ctx.origins or ()), dy))
 
 
 def _norm_backward(ctx, saved, dy):
