@@ -618,7 +618,7 @@ class Jarvis(nn.Module):
     def refresh_head(self):
         """Drops what is kept of lm_head's and final_norm's weights, and keeps copies of them again.  Training by `head_loss` or by `losses`
         needs no call for its updates to be seen: from the first loss with gradients on each forward converts the weights anew
-        (50257 x 1024: 47 us at the copy rate).  Call it when training is over, or after an update that neither a loss here, a gradient on
+        (50257 x 1024: 47 us of the device).  Call it when training is over, or after an update that neither a loss here, a gradient on
         the weight nor its version shows (another library's, through `.data`)."""
         self._lm_head_bf16 = None
         for p in (self.lm_head.weight, self.final_norm.weight):
@@ -631,8 +631,9 @@ class Jarvis(nn.Module):
             self._lm_head_bf16 = None
             # rows padded with zeros to a multiple of 128, the out-feature tile of the GEMM kernel
             v = w.shape[0]
-            wp = torch.zeros(((v + 127) // 128 * 128, w.shape[1]), dtype=torch.bfloat16, device=w.device)
-            wp[:v] = w.detach().to(torch.bfloat16)
+            wp = torch.empty(((v + 127) // 128 * 128, w.shape[1]), dtype=torch.bfloat16, device=w.device)
+            wp[:v].copy_(w.detach())
+            wp[v:].zero_()
             self._lm_head_bf16 = (key, wp)
         return self._lm_head_bf16[1]
 
