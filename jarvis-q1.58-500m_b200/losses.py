@@ -6,7 +6,8 @@
     y = rms_norm(x, weight)
 
 The reference forms lm_head's logits and takes F.cross_entropy of them (jarvis_engine/jarvis_model.py:535-540); at 16,384 rows and its
-vocabulary those are 1.6 GB in bf16.  Here they are not stored, in neither direction.
+vocabulary those are 1.6 GB in bf16.  Here they are not stored, in neither direction; a backward pass holds their gradients, in f16 and at
+most 640 MiB at a time (beyond some 6,600 rows of that vocabulary less than all of them).
 
 These are torch.autograd functions over the calls in `ops` (which have a forward and a backward call each, for programs without
 autograd).  Gradients formed under create_graph raise when they are differentiated, and tensors with a forward-mode tangent are refused.
@@ -169,18 +170,21 @@ def _head_loss(hidden, weight, targets, ids, logits, temperature, reduction):
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, reduction: str = "mean") -> torch.Tensor:
-    """-log softmax(hidden @ weight.T)[targets], differentiable in hidden (..., C) and weight (V, C).  targets: int64 (...); -100 marks a row
-    without one (loss 0, no part in any gradient), another value outside [0, V) makes its row NaN.  reduction: "mean" over the rows
-    with a target (NaN when there is none) -> f32 scalar; "none" -> f32 (...).  C: a multiple of 8, at least 64."""
+    """-log softmax(hidden @ weight.T)[targets], differentiable in hidden (..., C) and weight (V, C), bf16, or f32 and rounded to bf16
+    for the products.  targets: int64 (...); -100 marks a row without one (loss 0, no part in any gradient), another value outside
+    [0, V) makes its row NaN.  reduction: "mean" over the rows with a target (NaN when there is none) -> f32 scalar; "none" -> f32
+    (...).  C: a multiple of 8, at least 64.  The gradient of a logit is rounded to f16 relative to its row's factor in the whole
+    loss: 2^-12 of itself, nothing of what is below 2^-38 of that factor."""
     return _head_loss(hidden, weight, targets, None, None, 1.0, reduction)[0]
 
 
 def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
                         temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
     """t^2 KL(softmax(teacher_logits / t) over the row's entries || softmax(hidden @ weight.T / t)), t the temperature, differentiable in
-    hidden and weight.  teacher_ids: int64 (..., K), teacher_logits: f32 or bf16 (..., K), K <= 256, in any order; a negative id is no
+    hidden and weight (their types and roundings: linear_cross_entropy).  teacher_ids: int64 (..., K), teacher_logits: f32 or bf16 (..., K), K <= 256, in any order; a negative id is no
     entry, a row without entries has no part (loss 0), an id beyond the vocabulary makes its row NaN.  No gradient is formed for
-    teacher_logits: ones that require one are refused.  "mean": over the rows with entries."""
+    teacher_logits: ones that require one are refused.  "mean": over the rows with entries.  A difference of f32 logarithms: off by up to
+    t^2 2^-19."""
     return _head_loss(hidden, weight, None, teacher_ids, teacher_logits, temperature, reduction)[1]
 
 
