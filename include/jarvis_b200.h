@@ -429,8 +429,8 @@ int jb200_head_loss(const jb200_head* h, float* ce, float* kd, float* mean_ce, f
 
 /* Gradients of sum_n g_ce[n] ce[n] / *n_ce + g_kd[n] kd[n] / *n_kd: dx [N][C] and dw [V][C] (dtype 0: f32, 1: bf16), overwritten, NULL
  * where not wanted.  g_ce, g_kd: device f32, stride 0 (one value for all rows) or 1; n_ce, n_kd: device f32 or NULL (1).
- * The gradients of the logits are rounded to f16, a piece of the vocabulary at a time: relative to the call's largest factor g / n or, with
- * a stride of 1, to the row's own within two, all bits down to 2^-27 of it, nothing below 2^-38.  dx and dw are f32 sums of their products with w
+ * The gradients of the logits are rounded to f16, a piece of the vocabulary at a time: relative to the row's own largest factor, g_ce / n_ce
+ * or g_kd t / n_kd, within two, all bits down to 2^-27 of it, nothing below 2^-38.  dx and dw are f32 sums of their products with w
  * and x, which enter exactly within 2^32 of their largest finite value (for dw a row's values count as times its own factor over the
  * largest).  A row without target and teacher has a gradient of 0 and no part in dw, whatever it holds.  dx and dw 32-byte, scratch 256-byte aligned; sums are formed in a fixed order. */
 size_t jb200_head_loss_backward_scratch_bytes(int N, int V, int C);

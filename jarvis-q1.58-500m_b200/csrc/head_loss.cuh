@@ -28,8 +28,9 @@ struct HeadGrads {
 #if defined(__CUDACC__)
 // The gradients of the logits are kept relative to a factor, which the products apply to their f32 sums.  (With 1 / rows in them a
 // target's entry, -1 / rows and half of a row's gradient, had the same rounding in every row.)  It is the largest of the whole call,
-// and with gradients row by row that times the power of two by which the row's own is smaller: a light row keeps its bits, dx has its
-// factor back as a row of the product, and for dw, which sums over rows, the copy of its hidden row is smaller by that power of two.
+// and where rows differ (gradients row by row, or rows with one of two losses) that times the power of two by which the row's own is
+// smaller: a light row keeps its bits, dx has its factor back as a row of the product, and for dw, which sums over rows, the copy of its
+// hidden row is smaller by that power of two.
 __device__ __forceinline__ float common_factor(float ce, float kd) {
   const float s = ce <= 3.4e38f && !(kd <= 3.4e38f && kd > ce) ? ce : kd;
   return s > 0.f && s <= 3.4e38f ? s : 1.f;
@@ -57,7 +58,7 @@ __device__ __forceinline__ float2 row_factors(const HeadGrads& p, int row) {
 }
 // How many times the call's factor is halved for a row: until its own is more than half of what is left.
 __device__ __forceinline__ int row_halvings(const HeadGrads& p, int row, float scale) {
-  if (!p.scale) return 0;
+  if (!p.scale && !(p.targets && p.neg_entropy)) return 0;      // one loss's mean: all rows have the same
   const float2 v = row_factors(p, row);
   const float f = fmaxf(v.x, v.y);
   if (!(f > 0.f && f <= scale)) return 0;
@@ -65,7 +66,8 @@ __device__ __forceinline__ int row_halvings(const HeadGrads& p, int row, float s
   return f > ldexpf(scale, -k) ? k - 1 : k;
 }
 __device__ __forceinline__ float row_scale(const HeadGrads& p, int row, float scale) {
-  return p.scale ? ldexpf(scale, -row_halvings(p, row, scale)) : scale;
+  const int k = row_halvings(p, row, scale);
+  return k ? ldexpf(scale, -k) : scale;
 }
 #endif
 

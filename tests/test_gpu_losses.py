@@ -910,3 +910,23 @@ def test_rows_of_very_uneven_weights(mode):
     column = w.double().abs().sum(0)
     _check_grad(dx, want["dx"], want["dx_bound"] - 2.0 ** -38 * call * column + 2.0 ** -37 * own * column)
     _check_grad(dw, want["dw"], want["dw_bound"] + 2.0 ** -38 * call * N * h.double().abs().max())
+
+
+def test_losses_of_very_uneven_weights():
+    """Means of both losses, one weighted 2^-30 of the other: the rows that have the light one alone keep their gradient's bits."""
+    N, V, width = 64, 5000, 128
+    h, w, t, ids, logits = _problem(N, V, width, 5)
+    t[:20], ids[20:40] = -100, -1
+    t[20:40] = torch.arange(20, device="cuda") * 7
+    n_ce, n_kd = int((t != -100).sum()), int((ids >= 0).any(1).sum())
+    one = torch.ones(N, device="cuda", dtype=F64)
+    column = w.double().abs().sum(0)
+    for a, b in ((2.0 ** -30, 1.0), (1.0, 2.0 ** -30)):
+        x, wt = h.float().requires_grad_(), w.float().requires_grad_()
+        ce, kd = losses.linear_losses(x, wt, t, ids, logits, temperature=2.0)
+        dx, dw = torch.autograd.grad(a * ce + b * kd, (x, wt))
+        want = _definition(h, w, t, ids, logits, 2.0, one * a / n_ce, one * b / n_kd)
+        own = torch.maximum(a / n_ce * (t != -100), 2 * b / n_kd * (ids >= 0).any(1)).double()[:, None]
+        call = max(a / n_ce, 2 * b / n_kd)
+        _check_grad(dx, want["dx"], want["dx_bound"] - 2.0 ** -38 * call * column + 2.0 ** -37 * own * column)
+        _check_grad(dw, want["dw"], want["dw_bound"] + 2.0 ** -38 * call * N * h.double().abs().max())
