@@ -432,7 +432,8 @@ int jb200_head_loss(const jb200_head* h, float* ce, float* kd, float* mean_ce, f
  * The gradients of the logits are rounded to f16, a piece of the vocabulary at a time: relative to the row's own largest factor, g_ce / n_ce
  * or g_kd t / n_kd, within two, all bits down to 2^-27 of it, nothing below 2^-38.  dx and dw are f32 sums of their products with w
  * and x, which enter exactly within 2^32 of their largest finite value (for dw a row's values count as times its own factor over the
- * largest).  A row without target and teacher has a gradient of 0 and no part in dw, whatever it holds.  dx and dw 32-byte, scratch 256-byte aligned; sums are formed in a fixed order. */
+ * largest).  A row without target and teacher has a gradient of 0 and no part in dw, whatever it holds.  dx and dw 32-byte, scratch
+ * 256-byte aligned; sums are formed in a fixed order. */
 size_t jb200_head_loss_backward_scratch_bytes(int N, int V, int C);
 int jb200_head_loss_backward(const jb200_head* h, const float* g_ce, int g_ce_stride, const float* n_ce, const float* g_kd, int g_kd_stride,
                              const float* n_kd, void* dx, int dx_dtype, void* dw, int dw_dtype, void* scratch, void* stream);

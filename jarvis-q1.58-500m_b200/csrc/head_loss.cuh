@@ -74,7 +74,8 @@ __device__ __forceinline__ float row_scale(const HeadGrads& p, int row, float sc
 // Operands of the gradient's products are f16, whose rounding is an eighth of bf16's: the logits' gradients times 2^13 (at most 2 of them
 // add up to 2^14; they keep all their bits down to 2^-27 and vanish below 2^-38), and copies of weight and rows times the powers of two by
 // which the largest finite value of each comes to lie in [2^15, 2^16).  A bf16 value within 2^32 of that is exact there, a smaller one off
-// by at most 2^-40 of the largest; the rows' values count as halved with their factors there.  (As bf16 the logits' gradients gave dx and dW an error of sqrt(2) times their own rounding.)
+// by at most 2^-40 of the largest; the rows' values count as halved with their factors there.  (As bf16 the logits' gradients gave dx
+// and dW an error of sqrt(2) times their own rounding.)
 constexpr int HEAD_G_EXP = 13, HEAD_RANGE_CTAS = 512;
 
 // How a backward pass is cut: `pieces` pieces of `cols` vocabulary columns (the last one shorter) whose gradients of the logits are

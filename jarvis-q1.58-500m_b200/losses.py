@@ -181,9 +181,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
 def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
                         temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
     """t^2 KL(softmax(teacher_logits / t) over the row's entries || softmax(hidden @ weight.T / t)), t the temperature, differentiable in
-    hidden and weight (their types and roundings: linear_cross_entropy).  teacher_ids: int64 (..., K), teacher_logits: f32 or bf16 (..., K), K <= 256, in any order; a negative id is no
-    entry, a row without entries has no part (loss 0), an id beyond the vocabulary makes its row NaN.  No gradient is formed for
-    teacher_logits: ones that require one are refused.  "mean": over the rows with entries.  A difference of f32 logarithms: off by up to
+    hidden and weight (their types and roundings: linear_cross_entropy).  teacher_ids: int64 (..., K), teacher_logits: f32 or bf16 (..., K),
+    K <= 256, in any order; a negative id is no entry, a row without entries has no part (loss 0), an id beyond the vocabulary makes its
+    row NaN.  No gradient is formed for teacher_logits: ones that require one are refused.  "mean": over the rows with entries.  A difference of f32 logarithms: off by up to
     t^2 2^-19."""
     return _head_loss(hidden, weight, None, teacher_ids, teacher_logits, temperature, reduction)[1]
 
