@@ -162,6 +162,35 @@ int jb200_ternary_linear_grouped(const void* x, int M, int K, const uint8_t* pac
                                  int G, const int32_t* seg_offsets, int epilogue, void* out, int token_tile,
                                  int w_layout, void* stream);
 
+/* ---- gated delta rule ----------------------------------------------------------------- */
+
+/* The scan of jb200_attn_scan's family whose write first takes out what the key holds:
+ *   S_t = a_t S_{t-1} (I - beta_t k_t k_t^T) + beta_t v_t k_t^T,   a_t = exp(log_decay_t),   o_t = scale S_t q_t
+ * per (sequence, head), S f32 [64 values][64 keys] as in jb200_attn_scan.  q, k: bf16 rows [B T] of key_heads heads of 64; value head h takes
+ * key head h / (H / key_heads).  v, o: bf16 rows of H heads.  log_decay (0 or below; -inf forgets all that was), beta: f32 rows of H.  ld*: row
+ * strides in elements, multiples of 8 (ldg: any).  JB200_DELTA_NORMALIZE: k and q are divided by sqrt(|.|^2 + 1e-6); without it the caller
+ * sees to beta |k|^2 <= 2, beyond which the rule itself diverges.  lengths: int32 [B] or NULL; rows t >= lengths[b] (clamped to 0..T) of a
+ * sequence are not read, their output is 0, and the state is the one after the last row before them.  s_in NULL: zeros.  s_out NULL: not wanted;
+ * may be s_in itself, else the two must not overlap; o must overlap no input.  o NULL: the state alone.  scratch:
+ * jb200_gated_delta_scratch_bytes (0: may be NULL), 16-byte aligned; NULL where bytes are wanted: sequences are not cut into pieces.
+ * An infinity or NaN in a row reaches the rows of its chunk of 64 tokens, in that value row (from k, q and the gates: in that head), and what follows. */
+#define JB200_DELTA_NORMALIZE 1
+typedef struct jb200_delta {
+  int B, T, H, key_heads, head_dim, flags;
+  const void *q, *k, *v;
+  long long ldq, ldk, ldv;
+  const float *log_decay, *beta;
+  long long ldg;
+  const int32_t* lengths;
+  float scale;
+  const float* s_in;
+  void* o;
+  long long ldo;
+  float* s_out;
+} jb200_delta;
+size_t jb200_gated_delta_scratch_bytes(int B, int T, int H);
+int jb200_gated_delta(const jb200_delta* d, void* scratch, void* stream);
+
 /* ---- block glue --------------------------------------------------------------------- */
 
 /* RMSNorm.forward (jarvis_engine/jarvis_model.py:25-26): y = x * rsqrt(mean(x^2) + eps) * w.
@@ -449,6 +478,19 @@ size_t jb200_rmsnorm_backward_scratch_bytes(int n_rows, int C);
 int jb200_rmsnorm_backward(const void* x, int x_dtype, const float* w, float eps, const void* dy, int dy_dtype, int n_rows, int C, void* dx,
                            float* dw, void* scratch, void* stream);
 
+/* n = y * rsqrt(mean(y^2) + eps) * w [* silu(gate)], the mean over groups of `group` columns: the whole row (w: f32 [C]), or a power of two
+ * from 8 to 256 that divides C (w: f32 [group], every group's).  Behind a scan: group 64, one a head.  y, gate: f32 (dtype 0) or bf16 (1)
+ * [n_rows], row strides ldy, ldg (multiples of 8); gate may be NULL.  out: f32 or bf16 [n_rows][C].  C: a multiple of 8, at most 8192.  After
+ * RMSNorm.forward (jarvis_engine/jarvis_model.py:25-26). */
+int jb200_gated_norm(const void* y, int y_dtype, long long ldy, const float* w, const void* gate, long long ldg, int group, float eps, void* out,
+                     int out_dtype, int n_rows, int C, void* stream);
+
+/* The end of a block and the beginning of the next (jarvis_engine/jarvis_model.py:428-436) with a norm behind the block:
+ *   x' = x + scale * (y * rsqrt(mean(y^2) + eps) * w_after [* silu(gate)]),   xn = x' * rsqrt(mean(x'^2) + eps) * w_before
+ * x, x_out: f32 [n_rows][C], x_out may be x; scale: f32 [C] or NULL (1); xn: f32 (dtype 0) or bf16 (1) [n_rows][C]; the others as above. */
+int jb200_residual_norm(const float* x, const void* y, int y_dtype, long long ldy, const float* w_after, const void* gate, long long ldg,
+                        const float* scale, const float* w_before, float eps, float* x_out, void* xn, int xn_dtype, int n_rows, int C, void* stream);
+
 /* ---- expert parallelism over peer memory (no counterpart: the reference is single-GPU) ------------------- */
 
 /* Device buffers that other processes on the node can map (CUDA IPC).  alloc: cudaMalloc on the current device and
@@ -512,6 +554,29 @@ int jb200_ep_pull_combine(const void* const* peer_y, const void* const* peer_met
  * out_prob (optional, f32 [n_rows]): probability of the drawn token under the filtered distribution. */
 int jb200_sample(const void* logits, int logits_dtype, int ld, int n_rows, int V, float temperature, int top_k,
                  float top_p, const float* u, int64_t* out_token, float* out_prob, void* stream);
+
+/* One draw per row over the whole vocabulary, every row with settings of its own (jb200_sample, without its bound on top_k and with min-p).
+ * Order: logits descending, equal ones by the lower id; w = exp((x - x_max) / max(temperature, 1e-5)).  Three cuts of that order:
+ *   top_k > 0:          x >= the top_k-th largest (ties stay)
+ *   0 < top_p < 1:      the sum of w before a token <= top_p times the sum over what top_k left; the first token always stays
+ *   min_p > 0:          w >= min_p (the largest logit always stays)
+ * and the token is the first whose running sum over what is left exceeds u times the whole, u in [0, 1).  temperature <= 0 (or NaN): the
+ * largest logit, the lowest id among equals.  Logits: f32 (logits_dtype 0) or bf16 (1), row stride ld >= V elements; NaN is -inf.  A row without any
+ * logit above -inf gives token 0 with probability 0.  temperature, top_k, top_p, min_p: [n_rows], or NULL and one value for all rows.
+ * prob (optional, f32 [n_rows]): the token's probability among what is left.  Weights are f64, rounded to 2^-45 of the largest (of
+ * 2^-(63 - log2 V) beyond 2^18 tokens); the same inputs give the same token in every call. */
+typedef struct jb200_sampling {
+  const void* logits;
+  long long ld;
+  int logits_dtype, V;
+  const float *u, *temperature;
+  const int32_t* top_k;
+  const float *top_p, *min_p;
+  float temperature_all;
+  int top_k_all;
+  float top_p_all, min_p_all;
+} jb200_sampling;
+int jb200_sample_rows(const jb200_sampling* s, int n_rows, int64_t* token, float* prob, void* stream);
 
 /* Host-side copy of the bit manipulation the GEMM's decoder warps run: 16 two-bit codes
  * (one little-endian u32 of the packed layout) -> 16 bf16 values in out8[8] (two per u32,

@@ -17,6 +17,7 @@ _HEADER = os.path.join(os.path.dirname(_build.PKG_DIR), "include", "jarvis_b200.
 OK, ERR_ARG, ERR_CUDA = 0, -1, 1
 EPI_BF16, EPI_GELU_BF16, EPI_RESID_F32, EPI_F32 = 0, 1, 2, 3
 ATTN_QK_PREPARED = 1   # JB200_ATTN_QK_PREPARED
+DELTA_NORMALIZE = 1    # JB200_DELTA_NORMALIZE
 
 _P = C.c_void_p
 _I = C.c_int
@@ -44,6 +45,20 @@ class Head(C.Structure):
     """jb200_head"""
     _fields_ = [("N", _I), ("V", _I), ("C", _I), ("x", _P), ("w", _P), ("targets", _P), ("lse", _P), ("K", _I), ("teacher", _P),
                 ("temperature", _F), ("lse_t", _P)]
+
+
+class Delta(C.Structure):
+    """jb200_delta"""
+    _fields_ = [(n, _I) for n in ("B", "T", "H", "key_heads", "head_dim", "flags")] + [("q", _P), ("k", _P), ("v", _P)] + \
+               [(n, C.c_longlong) for n in ("ldq", "ldk", "ldv")] + \
+               [("log_decay", _P), ("beta", _P), ("ldg", C.c_longlong), ("lengths", _P), ("scale", _F), ("s_in", _P), ("o", _P),
+                ("ldo", C.c_longlong), ("s_out", _P)]
+
+
+class Sampling(C.Structure):
+    """jb200_sampling"""
+    _fields_ = [("logits", _P), ("ld", C.c_longlong), ("logits_dtype", _I), ("V", _I), ("u", _P), ("temperature", _P), ("top_k", _P),
+                ("top_p", _P), ("min_p", _P), ("temperature_all", _F), ("top_k_all", _I), ("top_p_all", _F), ("min_p_all", _F)]
 
 
 # name -> (restype, argtypes); must list every function declared in include/jarvis_b200.h
@@ -94,6 +109,10 @@ PROTOTYPES = {
     "jb200_host_head_plan": (_I, [_I] * 4 + [C.POINTER(C.c_int32)]),
     "jb200_rmsnorm_backward_scratch_bytes": (_Z, [_I] * 2),
     "jb200_rmsnorm_backward": (_I, [_P, _I, _P, _F, _P, _I, _I, _I, _P, _P, _P, _P]),
+    "jb200_gated_delta_scratch_bytes": (_Z, [_I] * 3),
+    "jb200_gated_delta": (_I, [C.POINTER(Delta), _P, _P]),
+    "jb200_gated_norm": (_I, [_P, _I, C.c_longlong, _P, _P, C.c_longlong, _I, _F, _P, _I, _I, _I, _P]),
+    "jb200_residual_norm": (_I, [_P, _P, _I, C.c_longlong, _P, _P, C.c_longlong, _P, _P, _F, _P, _P, _I, _I, _I, _P]),
     "jb200_accumulator_bytes": (_Z, [_I]),
     "jb200_routing_layout": (_Z, [_I, _I, C.POINTER(_Z)]),
     "jb200_forward_workspace_bytes": (_Z, [_I] * 6),
@@ -111,6 +130,7 @@ PROTOTYPES = {
     "jb200_ep_pull_gather": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P]),
     "jb200_ep_pull_combine": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _I, _P, _P]),
     "jb200_sample": (_I, [_P, _I, _I, _I, _I, _F, _I, _F, _P, _P, _P, _P]),
+    "jb200_sample_rows": (_I, [C.POINTER(Sampling), _I, _P, _P, _P]),
     "jb200_host_decode16": (None, [C.c_uint32, C.POINTER(C.c_uint32)]),
     "jb200_host_expert_tiles": (_I, [_I] * 6 + [C.POINTER(C.c_int32)]),
     "jb200_host_mid_ring": (_I, [_I] * 3 + [C.POINTER(C.c_int32)]),

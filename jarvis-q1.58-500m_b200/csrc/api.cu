@@ -500,6 +500,23 @@ int jb200_rmsnorm_backward(const void* x, int x_dtype, const float* w, float eps
   return launch_rmsnorm_backward(x, x_dtype, w, eps, dy, dy_dtype, n_rows, C, dx, dw, scratch, static_cast<cudaStream_t>(stream));
 }
 
+size_t jb200_gated_delta_scratch_bytes(int B, int T, int H) { return gated_delta_scratch_bytes(B, T, H); }
+int jb200_gated_delta(const jb200_delta* d, void* scratch, void* stream) {
+  return launch_gated_delta(d, scratch, static_cast<cudaStream_t>(stream));
+}
+int jb200_gated_norm(const void* y, int y_dtype, long long ldy, const float* w, const void* gate, long long ldg, int group, float eps, void* out,
+                     int out_dtype, int n_rows, int C, void* stream) {
+  return launch_gated_norm(y, y_dtype, ldy, w, gate, ldg, group, eps, out, out_dtype, n_rows, C, static_cast<cudaStream_t>(stream));
+}
+int jb200_residual_norm(const float* x, const void* y, int y_dtype, long long ldy, const float* w_after, const void* gate, long long ldg,
+                        const float* scale, const float* w_before, float eps, float* x_out, void* xn, int xn_dtype, int n_rows, int C, void* stream) {
+  return launch_residual_norm(x, y, y_dtype, ldy, w_after, gate, ldg, scale, w_before, eps, x_out, xn, xn_dtype, n_rows, C,
+                              static_cast<cudaStream_t>(stream));
+}
+int jb200_sample_rows(const jb200_sampling* s, int n_rows, int64_t* token, float* prob, void* stream) {
+  return launch_sample_rows(s, n_rows, token, prob, static_cast<cudaStream_t>(stream));
+}
+
 int jb200_prepare_weights(const uint8_t* packed, size_t n_bytes, uint8_t* prepared, void* stream) {
   return launch_prepare_weights(packed, n_bytes, prepared, static_cast<cudaStream_t>(stream));
 }

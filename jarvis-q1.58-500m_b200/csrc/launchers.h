@@ -193,4 +193,13 @@ int launch_ep_pull_combine(const void* const* peer_y, const void* const* peer_me
 int launch_sample(const void* logits, int logits_dtype, int ld, int n_rows, int V, float temperature, int top_k,
                   float top_p, const float* u, int64_t* out_token, float* out_prob, cudaStream_t stream);
 
+size_t gated_delta_scratch_bytes(int B, int T, int H);
+int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream);
+int launch_gated_norm(const void* y, int y_dtype, long long ldy, const float* w, const void* gate, long long ldg, int group, float eps, void* out,
+                      int out_dtype, int n_rows, int C, cudaStream_t stream);
+int launch_residual_norm(const float* x, const void* y, int y_dtype, long long ldy, const float* w_after, const void* gate, long long ldg,
+                         const float* scale, const float* w_before, float eps, float* x_out, void* xn, int xn_dtype, int n_rows, int C,
+                         cudaStream_t stream);
+int launch_sample_rows(const jb200_sampling* s, int n_rows, int64_t* token, float* prob, cudaStream_t stream);
+
 }  // namespace jb

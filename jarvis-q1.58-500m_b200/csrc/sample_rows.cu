@@ -1,0 +1,401 @@
+// Next token of every row with settings of its own, over the whole vocabulary: temperature, then top-k, top-p and min-p, each a cut of the
+// descending order of the logits, then one draw from what is left.  Where sampling.cu (sample_next_token,
+// jarvis_engine/evaluate_jarvis.py:158-185) sorts up to 2048 survivors of a top-k, nothing is sorted here and there need not be a top-k.
+//
+//   order:  logits descending, equal ones by the lower id;  w_i = exp((x_i - x_max) / T)
+//   top-k:  x_i >= the k-th largest (ties stay)
+//   top-p:  the sum of w before i <= top_p times the sum over what top-k left; the first token always stays
+//   min-p:  w_i >= min_p
+//   draw:   the first i whose running sum over what is left exceeds u times the whole
+//
+// All of them ask "which token covers position z of the running sum", once with every weight 1 (top-k).  Weights are taken in f64 and held as
+// integers of 2^-45 of the largest one's, so that sums do not depend on the order of the atomics that form them, and a token that the exact
+// sums choose is missed only where u lies within some 1e-12 of a border.  A CTA has a row.  A histogram of counts and sums over 2048 bins of
+// 1/32 of an e-fold finds the bin that covers z; its tokens (some hundred) are ranked by comparison with one another.  A bin of more than
+// 256 tokens is first cut by the bits of their keys, 512 parts a time.
+#include "common.cuh"
+#include "launchers.h"
+
+namespace jb {
+
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int THREADS = 1024;
+constexpr int BINS = 2048;              // 1/32 of an e-fold each; the last: everything 64 e-folds or more below the largest, whose weight is 0
+constexpr float BINS_A_FOLD = 32.f;
+constexpr int FINE = 512;
+constexpr int LIST = 256;
+
+struct Sampling {
+  const void* logits;
+  size_t ld;
+  int V, shift;                         // weights are multiples of 2^-shift
+  const float *u, *temperature, *top_p, *min_p;
+  const int32_t* top_k;
+  float temperature_all, top_p_all, min_p_all;
+  int top_k_all;
+  int64_t* token;
+  float* prob;
+};
+
+struct Item {
+  uint32_t key;
+  int id;
+  u64 w;
+};
+
+struct Smem {
+  uint32_t count[BINS], lo[BINS], hi[BINS];       // then, as running sums before every bin: count, (lo, hi)
+  uint32_t fcount[FINE], flo[FINE], fhi[FINE];
+  Item list[LIST];
+  u64 warp_sum[THREADS / 32];
+  uint32_t warp_count[THREADS / 32];
+  u64 best;                                       // (key, ~id) of the largest
+  uint32_t n, key_min, key_max;
+  // what a search leaves
+  uint32_t key, ties;
+  u64 above, weight;                              // the sum over keys above, the weight of one of the ties
+  int bin, id;
+  u64 sum;
+};
+
+// order-preserving map float -> uint32; NaN is treated as -inf, -0 as 0
+__device__ __forceinline__ uint32_t key_of(float x) {
+  if (x != x) x = -INFINITY;
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key); }
+
+template <typename T>
+__device__ __forceinline__ float widen(T x) { return x; }
+template <>
+__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// f(id, value) for every element of the row, 16 bytes a load where they are aligned
+template <typename T, typename F>
+__device__ __forceinline__ void every(const T* row, int V, F&& f) {
+  constexpr int PER = 16 / sizeof(T);
+  const int head = min(V, int((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / int(sizeof(T)));
+  const int vectors = (V - head) / PER, tail = head + vectors * PER;
+  const uint4* body = reinterpret_cast<const uint4*>(row + head);
+  if (int(threadIdx.x) < head) f(int(threadIdx.x), widen(row[threadIdx.x]));
+#pragma unroll 2
+  for (int i = threadIdx.x; i < vectors; i += THREADS) {
+    const uint4 x = __ldg(body + i);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    const int id = head + i * PER;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 2) {
+        f(id + 2 * j, bf16_lo(w[j]));
+        f(id + 2 * j + 1, bf16_hi(w[j]));
+      } else {
+        f(id + j, __uint_as_float(w[j]));
+      }
+    }
+  }
+  if (tail + int(threadIdx.x) < V) f(tail + int(threadIdx.x), widen(row[tail + threadIdx.x]));
+}
+
+struct Row {
+  float top, fold;                      // the largest logit; bins an e-fold of the row's temperature
+  double rate;                          // 1 / temperature
+  double unit;                          // 2^shift
+
+  __device__ __forceinline__ int bin(float x) const {
+    const float d = x == top ? 0.f : (top - x) * fold;
+    return d < float(BINS - 1) ? int(d) : BINS - 1;            // NaN and infinities are the last bin's
+  }
+  __device__ __forceinline__ double ratio(float x) const { return x == top ? 1.0 : exp((double(x) - double(top)) * rate); }
+  __device__ __forceinline__ u64 weight(float x) const { return __double2ull_rn(ratio(x) * unit); }
+};
+
+__device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, u64 w) {
+  const uint32_t a = uint32_t(w), before = atomicAdd(lo, a);
+  const uint32_t up = uint32_t(w >> 32) + (before + a < before ? 1u : 0u);
+  if (up) atomicAdd(hi, up);
+}
+
+// Running sums before each of PER N-thread bins in place; the first N threads hold PER neighbouring ones.
+template <int N_BINS>
+__device__ void running_sums(uint32_t* count, uint32_t* lo, uint32_t* hi, Smem& sm, u64 sum0, uint32_t count0) {
+  constexpr int PER = N_BINS >= THREADS ? N_BINS / THREADS : 1;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool on = tid * PER < N_BINS;
+  u64 s[PER], mine = 0;
+  uint32_t c[PER], cnt = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    s[i] = on ? (u64(hi[tid * PER + i]) << 32) + lo[tid * PER + i] : 0;
+    c[i] = on ? count[tid * PER + i] : 0;
+    mine += s[i];
+    cnt += c[i];
+  }
+  u64 incl = mine;
+  uint32_t cincl = cnt;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 a = __shfl_up_sync(0xffffffffu, incl, o);
+    const uint32_t b = __shfl_up_sync(0xffffffffu, cincl, o);
+    if (lane >= o) { incl += a; cincl += b; }
+  }
+  if (lane == 31) { sm.warp_sum[warp] = incl; sm.warp_count[warp] = cincl; }
+  __syncthreads();
+  u64 before = sum0 + incl - mine;
+  uint32_t cbefore = count0 + cincl - cnt;
+  for (int i = 0; i < warp; ++i) { before += sm.warp_sum[i]; cbefore += sm.warp_count[i]; }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (on) {
+      lo[tid * PER + i] = uint32_t(before);
+      hi[tid * PER + i] = uint32_t(before >> 32);
+      count[tid * PER + i] = cbefore;
+    }
+    before += s[i];
+    cbefore += c[i];
+  }
+  __syncthreads();
+}
+
+// The bin that covers position z: the last whose sum before it is not beyond z among those that hold anything of it.
+template <int N_BINS, bool BY_COUNT>
+__device__ int covering(const uint32_t* count, const uint32_t* lo, const uint32_t* hi, Smem& sm, u64 z) {
+  if (threadIdx.x == 0) sm.bin = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < N_BINS; i += THREADS) {
+    const u64 a = BY_COUNT ? count[i] : (u64(hi[i]) << 32) + lo[i];
+    const u64 b = i + 1 == N_BINS ? ~0ull : BY_COUNT ? count[i + 1] : (u64(hi[i + 1]) << 32) + lo[i + 1];
+    if (a <= z && z < b) sm.bin = i;
+  }
+  __syncthreads();
+  const int bin = sm.bin;
+  __syncthreads();
+  return bin;
+}
+
+// The key that covers position z of the running sum (of the running count): sm.key, .above, .weight, .ties; draw: also sm.id, the token.
+template <typename T, bool BY_COUNT>
+__device__ void search(const T* row, int V, const Row& r, Smem& sm, u64 z, bool draw) {
+  const int tid = threadIdx.x;
+  const int bin = covering<BINS, BY_COUNT>(sm.count, sm.lo, sm.hi, sm, z);
+  u64 above = (u64(sm.hi[bin]) << 32) + sm.lo[bin];
+  uint32_t cabove = sm.count[bin];
+  uint32_t from = 0, to = 0xffffffffu;              // keys in question, beside the bin
+  for (;;) {
+    if (tid == 0) { sm.n = 0; sm.key_min = 0xffffffffu; sm.key_max = 0; }
+    __syncthreads();
+    every(row, V, [&](int id, float x) {
+      if (r.bin(x) != bin) return;
+      const uint32_t key = key_of(x);
+      if (key < from || key > to) return;
+      const uint32_t slot = atomicAdd(&sm.n, 1u);
+      if (slot < LIST) { sm.list[slot].key = key; sm.list[slot].id = id; }
+      atomicMin(&sm.key_min, key);
+      atomicMax(&sm.key_max, key);
+    });
+    __syncthreads();
+    const uint32_t n = sm.n;
+    from = sm.key_min;
+    to = sm.key_max;
+    if (n <= LIST) break;
+    if (from == to) {                               // one key of many tokens
+      const u64 w = r.weight(value_of(to));
+      __syncthreads();
+      if (tid == 0) { sm.key = to; sm.ties = n; sm.above = above; sm.weight = w; }
+      if (draw) {                                   // its tokens in order of ids: every thread counts those of a piece of the row
+        const int piece = (V + THREADS - 1) / THREADS, a = min(V, tid * piece), b = min(V, a + piece);
+        uint32_t mine = 0;
+        for (int i = a; i < b; ++i) mine += key_of(widen(row[i])) == to;
+        uint32_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
+          if ((tid & 31) >= o) incl += x;
+        }
+        if ((tid & 31) == 31) sm.warp_count[tid >> 5] = incl;
+        __syncthreads();
+        uint32_t before = incl - mine;
+        for (int i = 0; i < (tid >> 5); ++i) before += sm.warp_count[i];
+        const uint32_t want = uint32_t((z - above) / w);
+        if (want >= before && want < before + mine) {
+          uint32_t left = want - before;
+          for (int i = a; i < b; ++i)
+            if (key_of(widen(row[i])) == to && left-- == 0) { sm.id = i; break; }
+        }
+      }
+      __syncthreads();
+      return;
+    }
+    int cut = 0;
+    while (((to - from) >> cut) >= FINE) ++cut;
+    for (int i = tid; i < FINE; i += THREADS) sm.fcount[i] = sm.flo[i] = sm.fhi[i] = 0;
+    __syncthreads();
+    every(row, V, [&](int id, float x) {
+      if (r.bin(x) != bin) return;
+      const uint32_t key = key_of(x);
+      if (key < from || key > to) return;
+      const uint32_t at = (to - key) >> cut;
+      atomicAdd(&sm.fcount[at], 1u);
+      add64(&sm.flo[at], &sm.fhi[at], r.weight(x));
+    });
+    __syncthreads();
+    running_sums<FINE>(sm.fcount, sm.flo, sm.fhi, sm, above, cabove);
+    const int at = covering<FINE, BY_COUNT>(sm.fcount, sm.flo, sm.fhi, sm, z);
+    above = (u64(sm.fhi[at]) << 32) + sm.flo[at];
+    cabove = sm.fcount[at];
+    const uint32_t high = to - (uint32_t(at) << cut), size = (1u << cut) - 1u;
+    from = high - from > size ? high - size : from;
+    to = high;
+    __syncthreads();
+  }
+  const int n = int(sm.n);
+  Item mine;
+  if (tid < n) {
+    mine = sm.list[tid];
+    mine.w = r.weight(value_of(mine.key));
+    sm.list[tid].w = mine.w;
+  }
+  __syncthreads();
+  if (tid < n) {
+    u64 over = 0;
+    uint32_t higher = 0, ties = 0, rank = 0;
+    for (int j = 0; j < n; ++j) {
+      const Item it = sm.list[j];
+      if (it.key > mine.key) { over += it.w; ++higher; }
+      else if (it.key == mine.key) { ++ties; rank += it.id < mine.id; }
+    }
+    const u64 first = BY_COUNT ? cabove + higher : above + over;
+    const u64 size = BY_COUNT ? ties : mine.w * ties;
+    if (first <= z && z - first < size) {
+      if (rank == 0) { sm.key = mine.key; sm.ties = ties; sm.above = above + over; sm.weight = mine.w; }
+      if (draw && uint32_t((z - first) / mine.w) == rank) sm.id = mine.id;
+    }
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ u64 share(double part, u64 whole) {
+  const double z = part * double(whole);
+  if (!(z > 0.0)) return 0;
+  return min(z < 1.8e19 ? __double2ull_rd(z) : ~0ull, whole - 1);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) sample_rows_kernel(Sampling p) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  const int tid = threadIdx.x, V = p.V;
+  const size_t at = blockIdx.x;
+  if (tid == 0) sm.best = 0;
+  for (int i = tid; i < BINS; i += THREADS) sm.count[i] = sm.lo[i] = sm.hi[i] = 0;
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+  const T* row = static_cast<const T*>(p.logits) + at * p.ld;
+  const float temperature = p.temperature != nullptr ? p.temperature[at] : p.temperature_all;
+  const float top_p = p.top_p != nullptr ? p.top_p[at] : p.top_p_all, min_p = p.min_p != nullptr ? p.min_p[at] : p.min_p_all;
+  const int top_k = p.top_k != nullptr ? p.top_k[at] : p.top_k_all;
+
+  u64 best = 0;
+  every(row, V, [&](int id, float x) { best = max(best, (u64(key_of(x)) << 32) | uint32_t(~id)); });
+  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if ((tid & 31) == 0) atomicMax(&sm.best, best);
+  __syncthreads();
+  best = sm.best;
+  Row r;
+  r.top = value_of(uint32_t(best >> 32));
+  const bool nothing = r.top == -INFINITY;
+  if (!(temperature > 0.f) || nothing) {              // the largest, lowest id among equals; no logit above -inf: token 0 with probability 0
+    if (tid == 0) {
+      p.token[at] = nothing ? 0 : int64_t(~uint32_t(best));
+      if (p.prob != nullptr) p.prob[at] = nothing ? 0.f : 1.f;
+    }
+    return;
+  }
+  r.rate = 1.0 / fmax(double(temperature), 1e-5);
+  r.fold = float(r.rate) * BINS_A_FOLD;
+  r.unit = double(1ull << p.shift);
+
+  every(row, V, [&](int id, float x) {
+    const int b = r.bin(x);
+    atomicAdd(&sm.count[b], 1u);
+    if (b < BINS - 1) {
+      const u64 w = r.weight(x);
+      if (w) add64(&sm.lo[b], &sm.hi[b], w);
+    }
+  });
+  __syncthreads();
+  // the last bin's weights are 0, so that the sum before it is the whole
+  running_sums<BINS>(sm.count, sm.lo, sm.hi, sm, 0, 0);
+  u64 whole = (u64(sm.hi[BINS - 1]) << 32) + sm.lo[BINS - 1];
+  if (top_k > 0 && top_k < V) {
+    search<T, true>(row, V, r, sm, u64(top_k - 1), false);
+    whole = sm.above + sm.weight * sm.ties;
+    __syncthreads();
+  }
+  u64 left = whole;
+  if (top_p > 0.f && top_p < 1.f) {
+    const u64 z = share(double(top_p), whole);
+    search<T, false>(row, V, r, sm, z, false);
+    left = sm.above + ((z - sm.above) / sm.weight + 1) * sm.weight;
+    __syncthreads();
+  }
+  if (min_p > 0.f) {
+    // bins well above the border are in, those well below out; weights decide in the three around it (the bins' borders are rounded)
+    const double d = -log(double(min_p)) * double(BINS_A_FOLD);
+    const int mid = d < double(BINS - 3) ? max(int(d), 0) : BINS - 3, first = max(mid - 1, 0), last = mid + 1;
+    if (tid == 0) sm.sum = (u64(sm.hi[first]) << 32) + sm.lo[first];
+    __syncthreads();
+    u64 mine = 0;
+    every(row, V, [&](int id, float x) {
+      const int b = r.bin(x);
+      if (b >= first && b <= last) {
+        const double w = r.ratio(x);
+        if (w >= double(min_p)) mine += __double2ull_rn(w * r.unit);
+      }
+    });
+    if (mine) atomicAdd(&sm.sum, mine);
+    __syncthreads();
+    left = max(min(left, sm.sum), u64(1) << p.shift);           // min_p beyond 1 leaves the largest
+    __syncthreads();
+  }
+  const double u = double(p.u[at]);
+  search<T, false>(row, V, r, sm, share(u, left), true);
+  if (tid == 0) {
+    p.token[at] = sm.id;
+    if (p.prob != nullptr) p.prob[at] = float(r.ratio(value_of(sm.key)) * r.unit / double(left));
+  }
+}
+
+}  // namespace
+
+int launch_sample_rows(const jb200_sampling* s, int n_rows, int64_t* token, float* prob, cudaStream_t stream) {
+  JB_REQUIRE(s != nullptr, "sample_rows: null pointer");
+  JB_REQUIRE(n_rows >= 0 && s->V > 0 && s->ld >= s->V, "sample_rows: bad shape (rows=%d, V=%d, ld=%lld)", n_rows, s->V, s->ld);
+  JB_REQUIRE(s->V <= 1 << 24, "sample_rows: at most 2^24 tokens (V=%d)", s->V);
+  JB_REQUIRE(s->logits_dtype == 0 || s->logits_dtype == 1, "sample_rows: logits dtype must be 0 (f32) or 1 (bf16)");
+  if (n_rows == 0) return JB200_OK;
+  JB_REQUIRE(s->logits && s->u && token, "sample_rows: null pointer");
+  Sampling p;
+  p.logits = s->logits; p.ld = size_t(s->ld); p.V = s->V;
+  int bits = 0;
+  while ((1 << bits) < s->V) ++bits;
+  p.shift = 63 - bits < 45 ? 63 - bits : 45;        // V weights of at most 2^shift fit 63 bits
+  p.u = s->u; p.temperature = s->temperature; p.top_k = s->top_k; p.top_p = s->top_p; p.min_p = s->min_p;
+  p.temperature_all = s->temperature_all; p.top_k_all = s->top_k_all; p.top_p_all = s->top_p_all; p.min_p_all = s->min_p_all;
+  p.token = token; p.prob = prob;
+  if (s->logits_dtype == 0) {
+    JB_MAX_SMEM(sample_rows_kernel<float>, sizeof(Smem));
+    launch_dep(sample_rows_kernel<float>, n_rows, THREADS, sizeof(Smem), stream, p);
+  } else {
+    JB_MAX_SMEM(sample_rows_kernel<__nv_bfloat16>, sizeof(Smem));
+    launch_dep(sample_rows_kernel<__nv_bfloat16>, n_rows, THREADS, sizeof(Smem), stream, p);
+  }
+  JB_LAUNCH_CHECK("sample_rows_kernel");
+  return JB200_OK;
+}
+
+}  // namespace jb

@@ -782,3 +782,229 @@ def sample(logits: torch.Tensor, u: torch.Tensor | None = None, *, temperature: 
         "jb200_sample",
     )
     return (out, prob) if want_prob else out
+
+
+# --------------------------------------------------------------------------- gated delta rule, norms around a block, draws
+def _forward_only(what: str, *tensors):
+    """These operators have no gradients: a graph that runs through one would lose its part without a word."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what}: a tensor requires a gradient, and none is formed here (call it under torch.no_grad() or detach)")
+
+
+def _row_view(t: torch.Tensor, rows: int, columns: int, dtype, what: str) -> torch.Tensor:
+    """A 2-D CUDA view (rows, columns) with unit inner stride, e.g. columns of a fused projection."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{what}: expected a CUDA tensor (this path has no CPU fallback)")
+    if t.dtype != dtype:
+        raise RuntimeError(f"{what}: expected dtype {dtype}, got {t.dtype}")
+    if t.dim() != 2 or tuple(t.shape) != (rows, columns) or (columns > 1 and t.stride(1) != 1):
+        raise RuntimeError(f"{what}: expected ({rows}, {columns}) rows with unit inner stride, got {tuple(t.shape)} with strides {tuple(t.stride())}")
+    return t
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements from row to row; of a tensor of at most one row, whose stride says nothing, its width."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _touch(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """True when the spans of two tensors in memory intersect (views of one buffer that interleave count)."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    span = [(t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) * t.element_size()) for t in (a, b)]
+    return span[0][0] < span[1][1] and span[1][0] < span[0][1]
+
+
+def gated_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, beta: torch.Tensor, B: int, T: int, H: int, *,
+                     key_heads: int | None = None, scale: float | None = None, normalize: bool = True, lengths: torch.Tensor | None = None,
+                     state_in: torch.Tensor | None = None, want_state: bool = False, state_out: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None, want_out: bool = True):
+    """The gated delta rule over sequences of T tokens, T = 1 being a decode step:
+    S_t = a_t S_{t-1} (I - b_t k k^T) + b_t v k^T with a = exp(log_decay), o_t = scale S_t q_t.
+    q, k: bf16 2-D views (B*T, key_heads*64), v: bf16 (B*T, H*64), each with a row stride of its own (e.g. column slices of a fused
+    projection; 16-byte aligned, strides multiples of 8); value head h takes key head h // (H // key_heads).  log_decay (<= 0), beta: f32 (B*T, H), column
+    slices allowed.  normalize: k and q are divided by their norms, sqrt(|.|^2 + 1e-6).  scale: 1/8 unless given.  lengths: int32 (B,), for padded
+    batches: rows behind a sequence's length are not read, their output is 0, the state is that after its last row.
+    Returns (o bf16 (B*T, H*64) or None, state f32 (B, H, 64 values, 64 keys) or None).  state_out may be state_in itself."""
+    lib = _lib.load()
+    what = "gated_delta_scan"
+    KH = H if key_heads is None else key_heads
+    if B < 0 or T < 0 or H < 1 or KH < 1 or H % KH:
+        raise RuntimeError(f"{what}: bad shape (B={B}, T={T}, H={H}, key_heads={KH})")
+    N, bf16, f32 = B * T, torch.bfloat16, torch.float32
+    _row_view(q, N, KH * 64, bf16, what + ".q")
+    _row_view(k, N, KH * 64, bf16, what + ".k")
+    _row_view(v, N, H * 64, bf16, what + ".v")
+    _row_view(log_decay, N, H, f32, what + ".log_decay")
+    _row_view(beta, N, H, f32, what + ".beta")
+    if _row_stride(log_decay) != _row_stride(beta):
+        raise RuntimeError(f"{what}: log_decay and beta must share their row stride")
+    if lengths is not None and _need(lengths, torch.int32, what + ".lengths").numel() != B:
+        raise RuntimeError(f"{what}: one length per sequence is needed")
+    _forward_only(what, q, k, v, log_decay, beta, state_in)
+    _together(what, q, k, v, log_decay, beta, lengths, state_in, state_out, out)
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return gated_delta_scan(q, k, v, log_decay, beta, B, T, H, key_heads=key_heads, scale=scale, normalize=normalize, lengths=lengths,
+                                    state_in=state_in, want_state=want_state, state_out=state_out, out=out, want_out=want_out)
+    dev = q.device
+    for name, t in (("state_in", state_in), ("state_out", state_out)):
+        if t is not None and tuple(_need(t, f32, f"{what}.{name}").shape) != (B, H, 64, 64):
+            raise RuntimeError(f"{what}: {name} must be (B, H, 64, 64)")
+    if state_out is None and want_state:
+        state_out = torch.empty((B, H, 64, 64), dtype=f32, device=dev)
+    elif state_out is not None and state_in is not None and state_out.data_ptr() != state_in.data_ptr() and _overlap(state_out, state_in):
+        raise RuntimeError(f"{what}: state_out overlaps state_in without being it")
+    if not want_out:
+        if out is not None:
+            raise RuntimeError(f"{what}: out is given and want_out is False")
+        if state_out is None:
+            raise RuntimeError(f"{what}: neither an output nor a state is asked for")
+    elif out is None:
+        out = torch.empty((N, H * 64), dtype=bf16, device=dev)
+    else:
+        _row_view(out, N, H * 64, bf16, what + ".out")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what}: out requires a gradient")
+        if any(t is not None and _touch(out, t) for t in (q, k, v, log_decay, beta, lengths, state_in, state_out)):
+            raise RuntimeError(f"{what}: out overlaps another argument")
+    if state_out is not None and any(t is not None and _touch(state_out, t) for t in (q, k, v, log_decay, beta, lengths)):
+        raise RuntimeError(f"{what}: state_out overlaps another argument")
+    if B == 0:
+        return out, state_out
+    d = _lib.Delta(B, T, H, KH, 64, _lib.DELTA_NORMALIZE if normalize else 0, _ptr(q), _ptr(k), _ptr(v), _row_stride(q), _row_stride(k), _row_stride(v),
+                   _ptr(log_decay), _ptr(beta), _row_stride(beta), _ptr(lengths), 0.125 if scale is None else float(scale), _ptr(state_in), _ptr(out),
+                   0 if out is None else _row_stride(out), _ptr(state_out))
+    nbytes = lib.jb200_gated_delta_scratch_bytes(B, T, H)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _lib.check(lib.jb200_gated_delta(ctypes.byref(d), _ptr(scratch), _stream()), "jb200_gated_delta")
+    return out, state_out
+
+
+def _norm_arguments(what, y, gate):
+    """Rows of y and gate as 2-D views: leading dimensions must fold into one row stride."""
+    if y.dim() < 1 or (gate is not None and gate.shape != y.shape):
+        raise RuntimeError(f"{what}: y {tuple(y.shape)} and gate {tuple(gate.shape) if gate is not None else None} do not belong together")
+    width = y.shape[-1]
+    if width < 1:
+        raise RuntimeError(f"{what}: rows without columns")
+    views = []
+    for name, t in (("y", y), ("gate", gate)):
+        if t is None:
+            views.append(None)
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{what}.{name}: expected a CUDA tensor (this path has no CPU fallback)")
+        _dt(t)
+        if t.dtype != y.dtype:
+            raise RuntimeError(f"{what}: gate must have y's dtype ({y.dtype}), got {t.dtype}")
+        try:
+            t = t.view(-1, width) if t.numel() else t.reshape(0, width)
+        except RuntimeError:
+            raise RuntimeError(f"{what}.{name}: rows of one stride are needed, got {tuple(t.shape)} with strides {tuple(t.stride())}") from None
+        if width > 1 and t.stride(1) != 1:
+            raise RuntimeError(f"{what}.{name}: rows must have unit inner stride, got {tuple(t.stride())}")
+        views.append(t)
+    return views
+
+
+def gated_norm(y: torch.Tensor, weight: torch.Tensor, gate: torch.Tensor | None = None, *, group: int | None = None, eps: float = 1e-6,
+               out_dtype=torch.bfloat16) -> torch.Tensor:
+    """y * rsqrt(mean(y^2) + eps) * weight [* silu(gate)], the mean over groups of `group` columns: all of them unless given (weight (C,)),
+    else a power of two from 8 to 256 that divides C (weight (group,)), e.g. 64 for the heads behind a scan.  y, gate: f32 or bf16 (..., C),
+    rows of one stride; weight f32.  After RMSNorm.forward (jarvis_engine/jarvis_model.py:25-26)."""
+    lib = _lib.load()
+    what = "gated_norm"
+    rows, g = _norm_arguments(what, y, gate)
+    _need(weight, torch.float32, what + ".weight")
+    N, width = rows.shape
+    group = width if group is None else int(group)
+    if weight.numel() != group:
+        raise RuntimeError(f"{what}: groups of {group} columns and weight {tuple(weight.shape)} do not belong together")
+    _forward_only(what, y, weight, gate)
+    _together(what, y, weight, gate)
+    if _elsewhere(y):
+        with torch.cuda.device(y.device):
+            return gated_norm(y, weight, gate, group=group, eps=eps, out_dtype=out_dtype)
+    out = torch.empty(y.shape, dtype=out_dtype, device=y.device)
+    _lib.check(lib.jb200_gated_norm(_ptr(rows), _dt(rows), _row_stride(rows), _ptr(weight), _ptr(g), 0 if g is None else _row_stride(g), group, eps,
+                                    _ptr(out), _dt(out), N, width, _stream()), "jb200_gated_norm")
+    return out
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor, w_after: torch.Tensor, w_before: torch.Tensor, *, gate: torch.Tensor | None = None,
+                  scale: torch.Tensor | None = None, eps: float = 1e-6, out: torch.Tensor | None = None, out_dtype=torch.bfloat16):
+    """The end of a block and the beginning of the next: x' = x + scale * (norm(y) * w_after [* silu(gate)]), xn = norm(x') * w_before,
+    norm(z) = z * rsqrt(mean(z^2) + eps) over rows.  x: f32 (..., C), contiguous; y, gate: f32 or bf16 of x's shape, rows of one stride; w_after,
+    w_before, scale: f32 (C,).  out: where x' goes, x itself for an update in place; a new tensor unless given.  Returns (x', xn)."""
+    lib = _lib.load()
+    what = "residual_norm"
+    rows, g = _norm_arguments(what, y, gate)
+    _need(x, torch.float32, what + ".x")
+    N, width = rows.shape
+    if x.shape != y.shape:
+        raise RuntimeError(f"{what}: x {tuple(x.shape)} and y {tuple(y.shape)} must have one shape")
+    for name, t in (("w_after", w_after), ("w_before", w_before), ("scale", scale)):
+        if t is not None and _need(t, torch.float32, f"{what}.{name}").numel() != width:
+            raise RuntimeError(f"{what}: {name} {tuple(t.shape)} does not fit rows of {width}")
+    _forward_only(what, x, y, w_after, w_before, gate, scale, out)
+    _together(what, x, y, w_after, w_before, gate, scale, out)
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return residual_norm(x, y, w_after, w_before, gate=gate, scale=scale, eps=eps, out=out, out_dtype=out_dtype)
+    if out is None:
+        out = torch.empty_like(x)
+    else:
+        _need(out, torch.float32, what + ".out")
+        if out.shape != x.shape:
+            raise RuntimeError(f"{what}: out {tuple(out.shape)} must have x's shape {tuple(x.shape)}")
+        if out.data_ptr() != x.data_ptr() and _touch(out, x):
+            raise RuntimeError(f"{what}: out overlaps x without being it")
+        if any(t is not None and _touch(out, t) for t in (rows, g, w_after, w_before, scale)):
+            raise RuntimeError(f"{what}: out overlaps another argument")
+    xn = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    _lib.check(lib.jb200_residual_norm(_ptr(x), _ptr(rows), _dt(rows), _row_stride(rows), _ptr(w_after), _ptr(g), 0 if g is None else _row_stride(g),
+                                       _ptr(scale), _ptr(w_before), eps, _ptr(out), _ptr(xn), _dt(xn), N, width, _stream()), "jb200_residual_norm")
+    return out, xn
+
+
+def sample_rows(logits: torch.Tensor, u: torch.Tensor, *, temperature=0.7, top_k=None, top_p=None, min_p=None, want_prob: bool = False):
+    """One token per row of `logits` ((B, V) f32 or bf16, rows may be strided), every filter over the whole vocabulary and each either one value
+    or a tensor (B,) with every row's own: temperature f32 (<= 0: argmax), top_k int32 (None or 0: off), top_p f32 (None or outside (0, 1): off),
+    min_p f32 (None or 0: off).  In descending order of the logits (ties: lower id) with w = exp((x - x_max) / temperature): top_k keeps x >= the
+    k-th largest, top_p drops a token when the sum of w before it exceeds top_p of what top_k left (never the first), min_p keeps w >= min_p, and the
+    token is the first whose running sum over the rest exceeds u (f32 (B,), uniform in [0, 1)) times its whole.  Cf. sample_next_token
+    (jarvis_engine/evaluate_jarvis.py:158-185).  NaN logits are -inf; a row without any logit above -inf gives token 0, probability 0.
+    -> int64 (B, 1) [, f32 (B,) probability of the token among what is left]."""
+    lib = _lib.load()
+    what = "sample_rows"
+    if not logits.is_cuda:
+        raise RuntimeError(f"{what}.logits: expected a CUDA tensor (this path has no CPU fallback)")
+    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise RuntimeError(f"{what}: logits must be (B, V) with contiguous rows")
+    B, V = logits.shape
+    s = _lib.Sampling(_ptr(logits), _row_stride(logits), _dt(logits), V)
+    if _need(u, torch.float32, what + ".u").numel() != B:
+        raise RuntimeError(f"{what}: u must hold one number per row")
+    s.u = _ptr(u)
+    given = [logits, u]
+    for name, value, dtype, off in (("temperature", temperature, torch.float32, 0.0), ("top_k", top_k, torch.int32, 0),
+                                    ("top_p", top_p, torch.float32, 0.0), ("min_p", min_p, torch.float32, 0.0)):
+        if torch.is_tensor(value):
+            if _need(value, dtype, f"{what}.{name}").numel() != B:
+                raise RuntimeError(f"{what}: {name} must be one value or hold one per row")
+            setattr(s, name, _ptr(value))
+            given.append(value)
+        else:
+            value = off if value is None else value
+            setattr(s, name + "_all", min(max(int(value), 0), 2 ** 31 - 1) if dtype is torch.int32 else float(value))
+    _together(what, *given)
+    if B > 1 and logits.stride(0) < V:
+        raise RuntimeError(f"{what}: rows of logits overlap (stride {logits.stride(0)}, {V} columns)")
+    if _elsewhere(logits):
+        with torch.cuda.device(logits.device):
+            return sample_rows(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, want_prob=want_prob)
+    out = torch.empty((B, 1), dtype=torch.int64, device=logits.device)
+    prob = torch.empty((B,), dtype=torch.float32, device=logits.device) if want_prob else None
+    _lib.check(lib.jb200_sample_rows(ctypes.byref(s), B, _ptr(out), _ptr(prob), _stream()), "jb200_sample_rows")
+    return (out, prob) if want_prob else out
