@@ -141,11 +141,12 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 // u of a chunk solve a triangular system, and everything else is products of 64 x 64 matrices:
 //   X = b (V - e^G K S^T),   U = T X with T = (I + A)^-1,  A_ij = b_i e^(G_i - G_j) k_i.k_j  (j < i)
 //   O = e^G Q S^T + P U with P_ij = e^(G_i - G_j) q_i.k_j  (j <= i),   S' = e^Gc S + (e^(Gc - G) U)^T K
-// A CTA follows one head of one sequence.  Four warps prepare a chunk (K, Q, T, P: nothing of the state) while the other four take the chunk
-// before it through the state; each of those holds 16 value rows of S in its accumulators and everything transposed (X^T, U^T, O^T: 16 values x
-// 64 tokens), so that a product's accumulators are the next one's first operand where they are, and the four never wait for one another.
+// A CTA follows one head of one sequence, in four groups of four warps.  Two take turns in preparing chunks (K, T: nothing of the state); one
+// takes a chunk through the state, each warp 16 value rows of S in its accumulators, everything transposed (X^T, U^T: 16 values x 64 tokens), so that a
+// product's accumulators are the next one's first operand where they are, and the four never wait for one another; one forms P and, from
+// S and U as the state's warps leave them, the outputs.
 //
-// mma.sync, not tcgen05: a chunk is a chain of five dependent products of 16 x 64 x 64 a warp with a rescaling between them; through tensor
+// mma.sync, not tcgen05: a chunk is a chain of three dependent products of 16 x 64 x 64 a warp with a rescaling between them; through tensor
 // memory each link would cost a commit, a wait and two copies, several times the product itself.
 //
 // Precision: the state is f32 and stays it.  What is multiplied is f16 in two terms, x = hi + lo (22 bits), with an exact power of two per row that
@@ -155,24 +156,32 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int CHUNK = 64;
 constexpr int TILE = CHUNK * D * 2;        // bytes of 64 rows of 128, the 16-byte units of row r at unit ^ (r & 7)
+constexpr int STAGES = 3;
+constexpr int GROUP = 128;                 // threads of a group of warps
 constexpr float LEAST_LOG2 = -300.f;       // 2^-300 is 0 in f32: a decay of less, -inf among them, is this one
 
 struct alignas(128) Stage {
-  uint8_t k[TILE], q[TILE], v[TILE];
+  uint8_t k[TILE], v[TILE];
   uint8_t t_hi[TILE], t_lo[TILE];          // T^T [j][i] on and above the diagonal's 16 x 16 blocks; -A [i][j] below them while T is formed
-  uint8_t p[TILE];                         // P [i][j]; before that, the diagonal blocks of -A in f32
-  float of_v[CHUNK], of_y[CHUNK], of_u[CHUNK], grow[CHUNK], of_o[CHUNK];
+  float diagonal[4][16 * 20];              // the diagonal blocks of -A in f32
+  float g_hi[CHUNK], g_lo[CHUNK], rk[CHUNK], nk[CHUNK], beta[CHUNK];
+  float of_v[CHUNK], of_y[CHUNK], of_u[CHUNK], grow[CHUNK];
   float whole;
 };
 struct alignas(128) ChunkSmem {
-  Stage stage[2];
-  float g_hi[CHUNK], g_lo[CHUNK], beta[CHUNK], rk[CHUNK], nk[CHUNK], rq[CHUNK];
+  Stage stage[STAGES];
+  uint8_t q[2][TILE], p[TILE], o[TILE];
+  float of_o[2][CHUNK];
+  uint4 s16[4][4][32], u16[4][4][32];      // of every warp of the state: S and U as first operands, lane by lane
+  float4 scales[4][32];
 };
-static_assert(sizeof(Stage) % 128 == 0 && TILE % 128 == 0, "tiles are read 16 bytes at a time in both stages");
+static_assert(sizeof(Stage) % 128 == 0 && TILE % 128 == 0, "tiles are read 16 bytes at a time in every stage");
 
+// The CTA's barriers.  Ready and free of a stage: the preparing group arrives and waits, the others wait and arrive.
+enum { BAR_GROUP = 0 /* + group */, BAR_READY = 2 /* + stage: for the state */, BAR_READY_O = 5 /* + stage: for the outputs */, BAR_FREE = 8 /* + stage */,
+       BAR_GIVEN = 11, BAR_TAKEN = 12, BAR_OUT = 13 };
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
-// barriers of the CTA: 1 the four preparing warps, 2 the two that form T, 3 + s stage s is ready, 5 + s stage s is free
 __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -221,157 +230,121 @@ __device__ __forceinline__ uint32_t unit_at(int row, int unit) { return uint32_t
 __device__ __forceinline__ uint32_t across(int row, int unit, int lane) { return unit_at(row + ((lane >> 4) << 3) + (lane & 7), unit + ((lane >> 3) & 1)); }
 __device__ __forceinline__ uint32_t down(int row, int unit, int lane) { return unit_at(row + (((lane >> 3) & 1) << 3) + (lane & 7), unit + (lane >> 4)); }
 
-// ---- the preparing warps ---------------------------------------------------------------------------------------------
-struct Loads {
-  uint4 k[4], q[4];
-  float g[2], beta[2];
+// The tokens that a CTA takes: of sequence b from row `begin` (of the sequence) on, `chunks` chunks, none from `len` on.
+struct Part {
+  int b, h, begin, len, chunks;
 };
 
-template <bool OUT>
+// Sixteen rows of a bf16 matrix a warp, eight lanes a row, four rows a lane: from memory ...
+__device__ __forceinline__ void fetch_rows(uint4 (&x)[4], const __nv_bfloat16* rows, size_t ld, int row0, int n, int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = row0 + 4 * i + (lane >> 3);
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (row < n) x[i] = __ldg(reinterpret_cast<const uint4*>(rows + size_t(row) * ld) + (lane & 7));
+  }
+}
+// ... and to f16 in a tile, times the power of two s that brings their norm into [1, 2); ss: the sum of squares after that.  A sum of squares
+// beyond f32's range makes the row NaN, one below it makes it 0.
+__device__ __forceinline__ void convert_rows(const uint4 (&x)[4], uint8_t* tile, int row0, int lane, float (&ss)[4], float (&s)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    float a = 0.f, c = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { a = fmaf(bf16_lo(in[j]), bf16_lo(in[j]), a); c = fmaf(bf16_hi(in[j]), bf16_hi(in[j]), c); }
+    ss[i] = a + c;
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss[i] += __shfl_xor_sync(0xffffffffu, ss[i], o);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int half = (int(__float_as_uint(ss[i]) >> 23) - 127) >> 1;             // ss in [4^half, 4^(half + 1))
+    s[i] = __uint_as_float(uint32_t(127 - half) << 23);
+    ss[i] = ss[i] * s[i] * s[i];
+    const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    uint32_t out[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = pack_f16x2(bf16_lo(in[j]) * s[i], bf16_hi(in[j]) * s[i]);
+    *reinterpret_cast<uint4*>(tile + unit_at(row0 + 4 * i + (lane >> 3), lane & 7)) = make_uint4(out[0], out[1], out[2], out[3]);
+  }
+}
+
+// Blocks on and below the diagonal of a 4 x 4 grid, three or two a warp, the diagonal's first
+__device__ __forceinline__ int blocks_of(int w) { return w < 2 ? 3 : 2; }
+__device__ __forceinline__ int block_row(int w, int i) { return i == 0 ? w : w < 2 ? 1 + i : w == 2 ? 1 : 3; }
+__device__ __forceinline__ int block_col(int w, int i) { return i == 0 ? w : w < 2 ? w : w == 2 ? 0 : 2; }
+
+// A block of rows ib of tile `a` times rows jb of tile `b`, 64 long
+__device__ __forceinline__ void block_products(float (&c)[2][4], const uint8_t* a, int ib, const uint8_t* b, int jb, int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[0][i] = c[1][i] = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    uint32_t f[4], r[4];
+    ldm4(r, smem_u32(a) + down(16 * ib, 2 * ks, lane));
+    ldm4(f, smem_u32(b) + across(16 * jb, 2 * ks, lane));
+    mma(c[0], r, f[0], f[1]);
+    mma(c[1], r, f[2], f[3]);
+  }
+}
+// ... times f_i r_j e^(G_i - G_j)
+__device__ __forceinline__ void decayed(float (&c)[2][4], const Stage& st, int i0, int jb, float f0, float f1, int lane) {
+  const float gh0 = st.g_hi[i0], gl0 = st.g_lo[i0], gh1 = st.g_hi[i0 + 8], gl1 = st.g_lo[i0 + 8];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int j = 16 * jb + 8 * n + 2 * (lane & 3);
+    const float2 gh = *reinterpret_cast<const float2*>(st.g_hi + j), gl = *reinterpret_cast<const float2*>(st.g_lo + j);
+    const float2 r = *reinterpret_cast<const float2*>(st.rk + j);
+    c[n][0] *= f0 * r.x * exp2_fast((gh0 - gh.x) + (gl0 - gl.x));
+    c[n][1] *= f0 * r.y * exp2_fast((gh0 - gh.y) + (gl0 - gl.y));
+    c[n][2] *= f1 * r.x * exp2_fast((gh1 - gh.x) + (gl1 - gl.x));
+    c[n][3] *= f1 * r.y * exp2_fast((gh1 - gh.y) + (gl1 - gl.y));
+  }
+}
+
+// ---- the preparing groups --------------------------------------------------------------------------------------------
 struct Prepare {
   const DeltaParams& p;
   ChunkSmem& sm;
-  int b, h, w, lane, len;
+  Part part;
+  int group, w, lane;
+  int takers;                                // threads that wait for a stage and free it
 
-  __device__ __forceinline__ void fetch(Loads& x, int t0) const {
-    const size_t first = size_t(b) * p.T + t0;
-    const int sub = lane >> 3, unit = lane & 7;
+  // running sums of log2 a, in f64 for differences of late tokens
+  __device__ __forceinline__ void gates(Stage& st, float ga, float gb, float beta_a, float beta_b) const {
+    double g0 = double(ga) * 1.4426950408889634, g1 = double(gb) * 1.4426950408889634;
+    if (g0 < double(LEAST_LOG2)) g0 = double(LEAST_LOG2);
+    if (g1 < double(LEAST_LOG2)) g1 = double(LEAST_LOG2);
+    double sum = g0 + g1;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 16 * w + 4 * i + sub;
-      const bool on = t0 + row < len;
-      x.k[i] = x.q[i] = make_uint4(0, 0, 0, 0);
-      if (on) x.k[i] = __ldg(reinterpret_cast<const uint4*>(p.k + (first + row) * p.ldk + size_t(h / p.per_key) * D) + unit);
-      if (OUT && on) x.q[i] = __ldg(reinterpret_cast<const uint4*>(p.q + (first + row) * p.ldq + size_t(h / p.per_key) * D) + unit);
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
     }
-    if (w == 0) {
+    const double end = __shfl_sync(0xffffffffu, sum, 31);
+    const double at[2] = {sum - g1, sum};
+    float hi[2], lo[2], grow[2], of_u[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = 2 * lane + i;
-        const bool on = t0 + row < len;
-        x.g[i] = on ? __ldg(p.log_decay + (first + row) * p.ldg + h) : 0.f;
-        x.beta[i] = on ? __ldg(p.beta + (first + row) * p.ldg + h) : 0.f;
-      }
+    for (int i = 0; i < 2; ++i) {
+      hi[i] = float(at[i]);
+      lo[i] = float(at[i] - double(hi[i]));
+      grow[i] = exp2f(hi[i]);
+      of_u[i] = exp2f(float(end - at[i]));
     }
+    *reinterpret_cast<float2*>(st.g_hi + 2 * lane) = make_float2(hi[0], hi[1]);
+    *reinterpret_cast<float2*>(st.g_lo + 2 * lane) = make_float2(lo[0], lo[1]);
+    *reinterpret_cast<float2*>(st.beta + 2 * lane) = make_float2(beta_a, beta_b);
+    *reinterpret_cast<float2*>(st.grow + 2 * lane) = make_float2(grow[0], grow[1]);
+    *reinterpret_cast<float2*>(st.of_u + 2 * lane) = make_float2(of_u[0], of_u[1]);
+    if (lane == 0) st.whole = exp2f(float(end));
   }
 
-  // one row of bf16 by eight lanes -> f16 times a power of two (the largest value in [1, 2)), the sum of squares of that, the power
-  __device__ __forceinline__ uint4 to_f16(uint4 x, float& ss, float& s) const {
-    const uint32_t m4 = 0x7fff7fffu;
-    const uint32_t m2 = __vmaxu2(__vmaxu2(x.x & m4, x.y & m4), __vmaxu2(x.z & m4, x.w & m4));
-    uint32_t m = max(m2 >> 16, m2 & 0xffffu);
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
-    s = __uint_as_float(uint32_t(max(254 - int(m >> 7), 1)) << 23);
-    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-    uint32_t out[4];
-    ss = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float a = bf16_lo(in[j]) * s, c = bf16_hi(in[j]) * s;
-      ss = fmaf(a, a, fmaf(c, c, ss));
-      out[j] = pack_f16x2(a, c);
-    }
-    ss = sum8(ss);
-    return make_uint4(out[0], out[1], out[2], out[3]);
-  }
-
-  __device__ __forceinline__ void convert(const Loads& x, Stage& st) const {
-    const int sub = lane >> 3, unit = lane & 7;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 16 * w + 4 * i + sub;
-      float ss, s;
-      *reinterpret_cast<uint4*>(st.k + unit_at(row, unit)) = to_f16(x.k[i], ss, s);
-      if (unit == 0) {
-        // k = n (k16 r) with |k16 r| = 1, or of the normalised key n = 1 and k16 r its value
-        const float r = p.normalize ? rsqrtf(fmaf(NORM_EPS * s, s, ss)) : ss > 0.f ? rsqrtf(ss) : 0.f;
-        sm.rk[row] = r;
-        sm.nk[row] = p.normalize ? 1.f : ss * r / s;
-      }
-      if (OUT) {
-        *reinterpret_cast<uint4*>(st.q + unit_at(row, unit)) = to_f16(x.q[i], ss, s);
-        if (unit == 0) sm.rq[row] = p.scale * (p.normalize ? rsqrtf(fmaf(NORM_EPS * s, s, ss)) : 1.f / s);
-      }
-    }
-    if (w == 0) {                              // running sums of log2 a, in f64 for differences of late tokens
-      double g0 = double(x.g[0]) * 1.4426950408889634, g1 = double(x.g[1]) * 1.4426950408889634;
-      if (g0 < double(LEAST_LOG2)) g0 = double(LEAST_LOG2);
-      if (g1 < double(LEAST_LOG2)) g1 = double(LEAST_LOG2);
-      double sum = g0 + g1;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double up = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += up;
-      }
-      const double at0 = sum - g1, end = __shfl_sync(0xffffffffu, sum, 31);
-      const double at[2] = {at0, sum};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = 2 * lane + i;
-        const float hi = float(at[i]);
-        sm.g_hi[row] = hi;
-        sm.g_lo[row] = float(at[i] - double(hi));
-        sm.beta[row] = x.beta[i];
-        st.grow[row] = exp2f(hi);
-        st.of_u[row] = exp2f(float(end - at[i]));
-      }
-      if (lane == 0) st.whole = exp2f(float(end));
-    }
-  }
-
-  // 16 rows ib of `a` times 16 rows jb of K, 64 long
-  __device__ __forceinline__ void products(float (&c)[2][4], const uint32_t (&a)[4][4], const Stage& st, int jb) const {
-    const uint32_t kb = smem_u32(st.k);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[0][i] = c[1][i] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      uint32_t f[4];
-      ldm4(f, kb + across(16 * jb, 2 * ks, lane));
-      mma(c[0], a[ks], f[0], f[1]);
-      mma(c[1], a[ks], f[2], f[3]);
-    }
-  }
-
-  __device__ __forceinline__ void row_of_a(Stage& st) const {
-    uint32_t a[4][4];
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) ldm4(a[ks], smem_u32(st.k) + down(16 * w, 2 * ks, lane));
-    const int i0 = 16 * w + (lane >> 2), i1 = i0 + 8;
-    const float gh0 = sm.g_hi[i0], gl0 = sm.g_lo[i0], gh1 = sm.g_hi[i1], gl1 = sm.g_lo[i1];
-    const float n0 = sm.nk[i0], n1 = sm.nk[i1];
-    const float f0 = -sm.beta[i0] * n0 * n0 * sm.rk[i0], f1 = -sm.beta[i1] * n1 * n1 * sm.rk[i1];
-    float* dg = reinterpret_cast<float*>(st.p) + w * 16 * 20;
-    for (int jb = 0; jb <= w; ++jb) {
-      float c[2][4];
-      products(c, a, st, jb);
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int j = 16 * jb + 8 * n + 2 * (lane & 3);
-        const float2 gh = *reinterpret_cast<const float2*>(sm.g_hi + j), gl = *reinterpret_cast<const float2*>(sm.g_lo + j);
-        const float2 r = *reinterpret_cast<const float2*>(sm.rk + j);
-        const float x0 = f0 * r.x * c[n][0] * exp2_fast((gh0 - gh.x) + (gl0 - gl.x)), x1 = f0 * r.y * c[n][1] * exp2_fast((gh0 - gh.y) + (gl0 - gl.y));
-        const float x2 = f1 * r.x * c[n][2] * exp2_fast((gh1 - gh.x) + (gl1 - gl.x)), x3 = f1 * r.y * c[n][3] * exp2_fast((gh1 - gh.y) + (gl1 - gl.y));
-        if (jb < w) {
-          const uint32_t at0 = unit_at(i0, j >> 3) + (j & 7) * 2, at1 = unit_at(i1, j >> 3) + (j & 7) * 2;
-          uint32_t hi, lo;
-          split(x0, x1, hi, lo);
-          *reinterpret_cast<uint32_t*>(st.t_hi + at0) = hi;
-          *reinterpret_cast<uint32_t*>(st.t_lo + at0) = lo;
-          split(x2, x3, hi, lo);
-          *reinterpret_cast<uint32_t*>(st.t_hi + at1) = hi;
-          *reinterpret_cast<uint32_t*>(st.t_lo + at1) = lo;
-        } else {
-          const int jl = 8 * n + 2 * (lane & 3);
-          *reinterpret_cast<float2*>(dg + (lane >> 2) * 20 + jl) = make_float2(x0, x1);
-          *reinterpret_cast<float2*>(dg + ((lane >> 2) + 8) * 20 + jl) = make_float2(x2, x3);
-        }
-      }
-    }
-    __syncwarp();
-    // the diagonal block's inverse, a column of T (a row of T^T) a lane: t_i = -sum_(j < i) A_ij t_j below t_c = 1
+  // the diagonal block's inverse, a column of T (a row of T^T) a lane: t_i = -sum_(j < i) A_ij t_j below t_c = 1
+  __device__ __forceinline__ void diagonal(Stage& st) const {
+    const float* dg = st.diagonal[w];
     float t[16];
     const int c = lane & 15;
 #pragma unroll
@@ -399,6 +372,38 @@ struct Prepare {
         const uint32_t at = unit_at(16 * w + c, 2 * w + u);
         *reinterpret_cast<uint4*>(st.t_hi + at) = make_uint4(hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
         *reinterpret_cast<uint4*>(st.t_lo + at) = make_uint4(lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
+      }
+    }
+  }
+
+  // this warp's blocks of -A, the diagonal's inverted
+  __device__ __forceinline__ void blocks_of_a(Stage& st) const {
+    for (int n = 0; n < blocks_of(w); ++n) {
+      const int ib = block_row(w, n), jb = block_col(w, n);
+      float c[2][4];
+      block_products(c, st.k, ib, st.k, jb, lane);
+      const int i0 = 16 * ib + (lane >> 2), i1 = i0 + 8;
+      const float n0 = st.nk[i0], n1 = st.nk[i1];
+      decayed(c, st, i0, jb, -st.beta[i0] * n0 * n0 * st.rk[i0], -st.beta[i1] * n1 * n1 * st.rk[i1], lane);
+      if (n == 0) {
+        float* dg = st.diagonal[w] + (lane >> 2) * 20 + 2 * (lane & 3);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          *reinterpret_cast<float2*>(dg + 8 * i) = make_float2(c[i][0], c[i][1]);
+          *reinterpret_cast<float2*>(dg + 8 * 20 + 8 * i) = make_float2(c[i][2], c[i][3]);
+        }
+        __syncwarp();
+        diagonal(st);
+      } else {
+        const Pair x = as_operand(c);
+        const int col = (lane & 3) * 4;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          *reinterpret_cast<uint32_t*>(st.t_hi + unit_at(i0, 2 * jb + i) + col) = x.hi[2 * i];
+          *reinterpret_cast<uint32_t*>(st.t_lo + unit_at(i0, 2 * jb + i) + col) = x.lo[2 * i];
+          *reinterpret_cast<uint32_t*>(st.t_hi + unit_at(i1, 2 * jb + i) + col) = x.hi[2 * i + 1];
+          *reinterpret_cast<uint32_t*>(st.t_lo + unit_at(i1, 2 * jb + i) + col) = x.lo[2 * i + 1];
+        }
       }
     }
   }
@@ -456,113 +461,111 @@ struct Prepare {
     for (int i = 0; i < 4; ++i) c[0][i] = c[1][i] = 0.f;
   }
 
-  // T's blocks off the diagonal from those on it, by halves: T_10 and T_32 first (warp 0, warp 1), then column 0, column 1 of the lower left quarter:
+  // T's blocks off the diagonal from those on it, by halves: T_10 and T_32 first (warps 0, 1), then columns 0 and 1 of the lower left quarter:
   //   [T_20 T_21; T_30 T_31] = -[T_22 0; T_32 T_33] [A_20 A_21; A_30 A_31] [T_00 0; T_10 T_11]
   __device__ __forceinline__ void off_diagonal(Stage& st) const {
-    float c[2][4], m2[2][4], m3[2][4];
-    zero(c);
-    times_a(c, first_operand(st, 2 * w, 2 * w), st, 2 * w + 1, 2 * w);
-    const Pair x = as_operand(c);
-    zero(c);
-    times_t(c, x, st, 2 * w + 1, 2 * w + 1);
-    store_t(c, st, 2 * w + 1, 2 * w);
-    bar_sync(2, 64);
-    zero(m2);
-    zero(m3);
-    for (int l = w; l < 2; ++l) {
-      const Pair t = first_operand(st, w, l);
-      times_a(m2, t, st, 2, l);
-      times_a(m3, t, st, 3, l);
-    }
-    const Pair a2 = as_operand(m2), a3 = as_operand(m3);
-    zero(m2);
-    zero(m3);
-    times_t(m2, a2, st, 2, 2);
-    times_t(m3, a2, st, 3, 2);
-    times_t(m3, a3, st, 3, 3);
-    store_t(m2, st, 2, w);
-    store_t(m3, st, 3, w);
-  }
-
-  __device__ __forceinline__ void row_of_p(Stage& st, int ib) const {
-    uint32_t a[4][4];
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) ldm4(a[ks], smem_u32(st.q) + down(16 * ib, 2 * ks, lane));
-    const int i0 = 16 * ib + (lane >> 2), i1 = i0 + 8;
-    const float gh0 = sm.g_hi[i0], gl0 = sm.g_lo[i0], gh1 = sm.g_hi[i1], gl1 = sm.g_lo[i1];
-    for (int jb = 0; jb <= ib; ++jb) {
+    if (w < 2) {
       float c[2][4];
-      products(c, a, st, jb);
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int j = 16 * jb + 8 * n + 2 * (lane & 3);
-        const float2 gh = *reinterpret_cast<const float2*>(sm.g_hi + j), gl = *reinterpret_cast<const float2*>(sm.g_lo + j);
-        const float2 r = *reinterpret_cast<const float2*>(sm.rk + j);
-        float x0 = r.x * c[n][0] * exp2_fast((gh0 - gh.x) + (gl0 - gl.x)), x1 = r.y * c[n][1] * exp2_fast((gh0 - gh.y) + (gl0 - gl.y));
-        float x2 = r.x * c[n][2] * exp2_fast((gh1 - gh.x) + (gl1 - gl.x)), x3 = r.y * c[n][3] * exp2_fast((gh1 - gh.y) + (gl1 - gl.y));
-        if (jb == ib) {                          // above the diagonal nothing
-          if (j > i0) x0 = 0.f;
-          if (j + 1 > i0) x1 = 0.f;
-          if (j > i1) x2 = 0.f;
-          if (j + 1 > i1) x3 = 0.f;
-        }
-        *reinterpret_cast<uint32_t*>(st.p + unit_at(i0, j >> 3) + (j & 7) * 2) = pack_f16x2(x0, x1);
-        *reinterpret_cast<uint32_t*>(st.p + unit_at(i1, j >> 3) + (j & 7) * 2) = pack_f16x2(x2, x3);
+      zero(c);
+      times_a(c, first_operand(st, 2 * w, 2 * w), st, 2 * w + 1, 2 * w);
+      const Pair x = as_operand(c);
+      zero(c);
+      times_t(c, x, st, 2 * w + 1, 2 * w + 1);
+      store_t(c, st, 2 * w + 1, 2 * w);
+    }
+    bar_sync(BAR_GROUP + group, GROUP);
+    if (w < 2) {
+      float m2[2][4], m3[2][4];
+      zero(m2);
+      zero(m3);
+      for (int l = w; l < 2; ++l) {
+        const Pair t = first_operand(st, w, l);
+        times_a(m2, t, st, 2, l);
+        times_a(m3, t, st, 3, l);
       }
+      const Pair a2 = as_operand(m2), a3 = as_operand(m3);
+      zero(m2);
+      zero(m3);
+      times_t(m2, a2, st, 2, 2);
+      times_t(m3, a2, st, 3, 2);
+      times_t(m3, a3, st, 3, 3);
+      store_t(m2, st, 2, w);
+      store_t(m3, st, 3, w);
     }
   }
 
-  __device__ __forceinline__ void run(int t_begin, int chunks) const {
-    Loads x;
-    fetch(x, t_begin);
-    for (int n = 0; n < chunks; ++n) {
-      const int s = n & 1, t0 = t_begin + n * CHUNK;
+  __device__ __forceinline__ void run() const {
+    const size_t first = size_t(part.b) * p.T;
+    const __nv_bfloat16* kp = p.k + first * p.ldk + size_t(part.h / p.per_key) * D;
+    const __nv_bfloat16* vp = p.v + first * p.ldv + size_t(part.h) * D;
+    uint4 k[4];
+    float g0 = 0.f, g1 = 0.f, b0 = 0.f, b1 = 0.f;
+    auto fetch = [&](int t0) {
+      fetch_rows(k, kp, p.ldk, t0 + 16 * w, part.len, lane);
+      if (w == 3) {
+        const int t = t0 + 2 * lane;
+        g0 = t < part.len ? __ldg(p.log_decay + (first + t) * p.ldg + part.h) : 0.f;
+        b0 = t < part.len ? __ldg(p.beta + (first + t) * p.ldg + part.h) : 0.f;
+        g1 = t + 1 < part.len ? __ldg(p.log_decay + (first + t + 1) * p.ldg + part.h) : 0.f;
+        b1 = t + 1 < part.len ? __ldg(p.beta + (first + t + 1) * p.ldg + part.h) : 0.f;
+      }
+    };
+    if (group < part.chunks) fetch(part.begin + group * CHUNK);
+    for (int n = group; n < part.chunks; n += 2) {
+      const int s = n % STAGES, t0 = part.begin + n * CHUNK;
       Stage& st = sm.stage[s];
-      if (n >= 2) bar_sync(5 + s, 256);
+      if (n >= STAGES) bar_sync(BAR_FREE + s, GROUP + takers);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {              // V as it is
         const int row = 16 * w + 4 * i + (lane >> 3), unit = lane & 7;
         uint8_t* to = st.v + unit_at(row, unit);
-        if (t0 + row < len) copy_async_16(smem_u32(to), p.v + (size_t(b) * p.T + t0 + row) * p.ldv + size_t(h) * D + unit * 8);
+        if (t0 + row < part.len) copy_async_16(smem_u32(to), vp + size_t(t0 + row) * p.ldv + unit * 8);
         else *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
       }
-      convert(x, st);
-      if (n + 1 < chunks) fetch(x, t0 + CHUNK);
-      bar_sync(1, 128);
-      row_of_a(st);
-      if (w == 0) {
+      float ss[4], sc[4];
+      convert_rows(k, st.k, 16 * w, lane, ss, sc);
+      if ((lane & 7) == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // k = n (k16 r) with |k16 r| = 1, or of the normalised key n = 1 and k16 r its value
+          const int row = 16 * w + 4 * i + (lane >> 3);
+          const float r = p.normalize ? rsqrtf(fmaf(NORM_EPS * sc[i], sc[i], ss[i])) : ss[i] > 0.f ? rsqrtf(ss[i]) : 0.f;
+          st.rk[row] = r;
+          st.nk[row] = p.normalize ? 1.f : ss[i] * r / sc[i];
+        }
+      }
+      if (w == 3) gates(st, g0, g1, b0, b1);
+      if (n + 2 < part.chunks) fetch(t0 + 2 * CHUNK);
+      bar_sync(BAR_GROUP + group, GROUP);
+      blocks_of_a(st);
+      if (w == 2) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int row = lane + 32 * i;
-          const float r = sm.rk[row], n1 = sm.nk[row], beta = sm.beta[row];
+          const float r = st.rk[row], n1 = st.nk[row], beta = st.beta[row];
           st.of_v[row] = beta * n1;
           st.of_y[row] = beta * n1 * n1 * st.grow[row] * r;
           st.of_u[row] *= r;
-          if (OUT) st.of_o[row] = sm.rq[row];
         }
       }
-      bar_sync(1, 128);
-      if (w < 2) {
-        off_diagonal(st);
-      } else if (OUT) {
-        row_of_p(st, w == 2 ? 1 : 3);
-        row_of_p(st, w == 2 ? 2 : 0);
-      }
+      bar_sync(BAR_GROUP + group, GROUP);
+      off_diagonal(st);
       copy_async_wait();
-      bar_arrive(3 + s, 256);
-      bar_sync(1, 128);                          // rk, g and the others are overwritten next
+      bar_arrive(BAR_READY + s, 2 * GROUP);
+      if (takers == 2 * GROUP) bar_arrive(BAR_READY_O + s, 2 * GROUP);
     }
   }
 };
 
-// ---- the warps of the state -------------------------------------------------------------------------------------------
-template <bool OUT>
+// ---- the group of the state ------------------------------------------------------------------------------------------
+// OUT: gives S and U to the group of the outputs.  VALUES: false where v counts as 0.
+template <bool OUT, bool VALUES>
 struct Follow {
-  const DeltaParams& p;
   ChunkSmem& sm;
-  int b, h, w, lane, len;
+  int w, lane;
 
-  __device__ __forceinline__ void chunk(float (&S)[8][4], Stage& st, int t0) const {
+  // S: accumulators of 16 x 64, times inv0 (rows lane / 4) and inv1 (those and eight) the state
+  __device__ __forceinline__ void chunk(float (&S)[8][4], float& inv0, float& inv1, Stage& st, bool wait) const {
     const int c2 = 2 * (lane & 3);
     // S in two terms
     float m0 = 0.f, m1 = 0.f;
@@ -571,11 +574,13 @@ struct Follow {
       m0 = fmaxf(m0, fmaxf(fabsf(S[n][0]), fabsf(S[n][1])));
       m1 = fmaxf(m1, fmaxf(fabsf(S[n][2]), fabsf(S[n][3])));
     }
-    m0 = quad_max(m0);
-    m1 = quad_max(m1);
+    m0 = quad_max(m0) * inv0;
+    m1 = quad_max(m1) * inv1;
     float s0, s1, is0, is1;
     power_scale<14>(m0, s0, is0);
     power_scale<14>(m1, s1, is1);
+    s0 *= inv0;
+    s1 *= inv1;
     uint32_t sh[4][4], sl[4][4];
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
@@ -584,6 +589,10 @@ struct Follow {
       split(S[2 * ks + 1][0] * s0, S[2 * ks + 1][1] * s0, sh[ks][2], sl[ks][2]);
       split(S[2 * ks + 1][2] * s1, S[2 * ks + 1][3] * s1, sh[ks][3], sl[ks][3]);
     }
+    if (OUT && wait) bar_sync(BAR_TAKEN, 2 * GROUP);
+    if constexpr (OUT)
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) sm.s16[w][ks][lane] = make_uint4(sh[ks][0], sh[ks][1], sh[ks][2], sh[ks][3]);
     // Y^T = S K^T
     float y[8][4];
     const uint32_t kb = smem_u32(st.k), lane4 = unit_at(lane & 7, lane >> 3);   // four neighbouring units of eight rows
@@ -605,8 +614,8 @@ struct Follow {
     float x0 = m0 * 8.6736174e-19f, x1 = m1 * 8.6736174e-19f;      // 2^-60: X's power must leave S in range, too
 #pragma unroll
     for (int n2 = 0; n2 < 4; ++n2) {
-      uint32_t f[4];
-      ldm4t(f, smem_u32(st.v) + unit_at(16 * n2 + ((lane >> 4) << 3) + (lane & 7), 2 * w + ((lane >> 3) & 1)));
+      uint32_t f[4] = {};
+      if constexpr (VALUES) ldm4t(f, smem_u32(st.v) + unit_at(16 * n2 + ((lane >> 4) << 3) + (lane & 7), 2 * w + ((lane >> 3) & 1)));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float(&t)[4] = y[2 * n2 + i];
@@ -653,68 +662,16 @@ struct Follow {
       }
     }
     if constexpr (OUT) {
-      // O^T = e^G S Q^T + U^T P^T
-      float o[8][4];
-      const uint32_t qb = smem_u32(st.q), across0 = across(0, 0, lane);
-      const float q0 = is0 * e0, q1 = is1 * e1;
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t f[4];
-          ldm4(f, qb + n * 1024 + (lane4 ^ (half << 6)));
-          mma(o[n], sh[2 * half], f[0], f[1]);
-          mma(o[n], sh[2 * half + 1], f[2], f[3]);
-        }
-        const float2 grow = *reinterpret_cast<const float2*>(st.grow + 8 * n + c2);
-        o[n][0] *= grow.x * q0;
-        o[n][1] *= grow.y * q0;
-        o[n][2] *= grow.x * q1;
-        o[n][3] *= grow.y * q1;
-      }
-      uint32_t uf[4][4];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        uf[ks][0] = pack_f16x2(u[2 * ks][0], u[2 * ks][1]);
-        uf[ks][1] = pack_f16x2(u[2 * ks][2], u[2 * ks][3]);
-        uf[ks][2] = pack_f16x2(u[2 * ks + 1][0], u[2 * ks + 1][1]);
-        uf[ks][3] = pack_f16x2(u[2 * ks + 1][2], u[2 * ks + 1][3]);
-      }
-#pragma unroll
-      for (int ib = 0; ib < 4; ++ib)
-#pragma unroll
-        for (int jb = 0; jb <= ib; ++jb) {
-          uint32_t f[4];
-          ldm4(f, smem_u32(st.p) + ib * 2048 + (across0 ^ (jb << 5)));
-          mma(o[2 * ib], uf[jb], f[0], f[1]);
-          mma(o[2 * ib + 1], uf[jb], f[2], f[3]);
-        }
-      // into the columns of V that this warp alone has read, then out by rows
-#pragma unroll
-      for (int n2 = 0; n2 < 4; ++n2) {
-        uint32_t f[4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float2 fo = *reinterpret_cast<const float2*>(st.of_o + 16 * n2 + 8 * i + c2);
-          const float(&t)[4] = o[2 * n2 + i];
-          f[2 * i] = pack_bf16x2(t[0] * (fo.x * ie0), t[1] * (fo.y * ie0));
-          f[2 * i + 1] = pack_bf16x2(t[2] * (fo.x * ie1), t[3] * (fo.y * ie1));
-        }
-        stm4t(smem_u32(st.v) + unit_at(16 * n2 + ((lane >> 4) << 3) + (lane & 7), 2 * w + ((lane >> 3) & 1)), f[0], f[1], f[2], f[3]);
-      }
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * i + (lane >> 1), unit = 2 * w + (lane & 1);
-        if (t0 + row < len)
-          *(reinterpret_cast<uint4*>(p.o + (size_t(b) * p.T + t0 + row) * p.ldo + size_t(h) * D) + unit) = *reinterpret_cast<const uint4*>(st.v + unit_at(row, unit));
-      }
+      for (int ks = 0; ks < 4; ++ks)
+        sm.u16[w][ks][lane] = make_uint4(pack_f16x2(u[2 * ks][0], u[2 * ks][1]), pack_f16x2(u[2 * ks][2], u[2 * ks][3]),
+                                         pack_f16x2(u[2 * ks + 1][0], u[2 * ks + 1][1]), pack_f16x2(u[2 * ks + 1][2], u[2 * ks + 1][3]));
+      sm.scales[w][lane] = make_float4(is0 * e0, is1 * e1, ie0, ie1);
+      bar_arrive(BAR_GIVEN, 2 * GROUP);
     }
     // S' = e^Gc S + (e^(Gc - G) U)^T K, at X's power
     const float whole = st.whole;
-    const float k0 = whole * e0, k1 = whole * e1;
+    const float k0 = whole * (e0 * inv0), k1 = whole * (e1 * inv1);
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       S[n][0] *= k0; S[n][1] *= k0; S[n][2] *= k1; S[n][3] *= k1;
@@ -739,54 +696,194 @@ struct Follow {
         mma(S[2 * n2 + 1], ul, f[2], f[3]);
       }
     }
+    inv0 = ie0;
+    inv1 = ie1;
+  }
+
+  // from `from` (null: 0; `one`: the identity) through the part's chunks to `to` (or nowhere)
+  __device__ __forceinline__ void run(const Part& part, const float* from, bool one, float* to, int ready, int takers) const {
+    float S[8][4];
+    const int row = 16 * w + (lane >> 2), at = row * D + 2 * (lane & 3);
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      S[n][0] *= ie0; S[n][1] *= ie0; S[n][2] *= ie1; S[n][3] *= ie1;
+      float2 x = make_float2(0.f, 0.f), y = x;
+      if (from != nullptr) {
+        x = *reinterpret_cast<const float2*>(from + at + 8 * n);
+        y = *reinterpret_cast<const float2*>(from + at + 8 * D + 8 * n);
+      } else if (one) {
+        const int d = row - 8 * n - 2 * (lane & 3);
+        x = make_float2(d == 0, d == 1);
+        y = make_float2(d == -8, d == -7);
+      }
+      S[n][0] = x.x; S[n][1] = x.y; S[n][2] = y.x; S[n][3] = y.y;
+    }
+    float inv0 = 1.f, inv1 = 1.f;
+    for (int n = 0; n < part.chunks; ++n) {
+      const int s = n % STAGES;
+      bar_sync(ready + s, 2 * GROUP);
+      chunk(S, inv0, inv1, sm.stage[s], n > 0);
+      if (n + STAGES < part.chunks) bar_arrive(BAR_FREE + s, GROUP + takers);
+    }
+    if (to != nullptr) {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        *reinterpret_cast<float2*>(to + at + 8 * n) = make_float2(S[n][0] * inv0, S[n][1] * inv0);
+        *reinterpret_cast<float2*>(to + at + 8 * D + 8 * n) = make_float2(S[n][2] * inv1, S[n][3] * inv1);
+      }
+    }
+  }
+};
+
+// ---- the group of the outputs ----------------------------------------------------------------------------------------
+struct Outputs {
+  const DeltaParams& p;
+  ChunkSmem& sm;
+  Part part;
+  int w, lane;
+
+  __device__ __forceinline__ void blocks_of_p(const uint8_t* q, const Stage& st) const {
+    for (int n = 0; n < blocks_of(w); ++n) {
+      const int ib = block_row(w, n), jb = block_col(w, n), i0 = 16 * ib + (lane >> 2), col = (lane & 3) * 4;
+      float c[2][4];
+      block_products(c, q, ib, st.k, jb, lane);
+      decayed(c, st, i0, jb, 1.f, 1.f, lane);
+      if (n == 0) {                            // above the diagonal nothing
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int d = (lane >> 2) - 8 * i - 2 * (lane & 3);
+          if (d < 0) c[i][0] = 0.f;
+          if (d < 1) c[i][1] = 0.f;
+          if (d < -8) c[i][2] = 0.f;
+          if (d < -7) c[i][3] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        *reinterpret_cast<uint32_t*>(sm.p + unit_at(i0, 2 * jb + i) + col) = pack_f16x2(c[i][0], c[i][1]);
+        *reinterpret_cast<uint32_t*>(sm.p + unit_at(i0 + 8, 2 * jb + i) + col) = pack_f16x2(c[i][2], c[i][3]);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void run() const {
+    const size_t first = size_t(part.b) * p.T;
+    const __nv_bfloat16* qp = p.q + first * p.ldq + size_t(part.h / p.per_key) * D;
+    __nv_bfloat16* op = p.o + first * p.ldo + size_t(part.h) * D;
+    const int c2 = 2 * (lane & 3);
+    const uint32_t lane4 = unit_at(lane & 7, lane >> 3), across0 = across(0, 0, lane);
+    uint4 x[4];
+    if (part.chunks > 0) fetch_rows(x, qp, p.ldq, part.begin + 16 * w, part.len, lane);
+    for (int n = 0; n < part.chunks; ++n) {
+      const int s = n % STAGES, t0 = part.begin + n * CHUNK;
+      const Stage& st = sm.stage[s];
+      uint8_t* q = sm.q[n & 1];                // the other one may still be read
+      float* of_o = sm.of_o[n & 1];
+      float ss[4], sc[4];
+      convert_rows(x, q, 16 * w, lane, ss, sc);
+      if ((lane & 7) == 0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          of_o[16 * w + 4 * i + (lane >> 3)] = p.scale * (p.normalize ? rsqrtf(fmaf(NORM_EPS * sc[i], sc[i], ss[i])) : 1.f / sc[i]);
+      if (n + 1 < part.chunks) fetch_rows(x, qp, p.ldq, t0 + CHUNK + 16 * w, part.len, lane);
+      bar_sync(BAR_READY_O + s, 2 * GROUP);
+      blocks_of_p(q, st);
+      float2 grow[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) grow[i] = *reinterpret_cast<const float2*>(st.grow + 8 * i + c2);
+      bar_sync(BAR_OUT, GROUP);
+      if (n + STAGES < part.chunks) bar_arrive(BAR_FREE + s, 3 * GROUP);
+      bar_sync(BAR_GIVEN, 2 * GROUP);
+      uint32_t sh[4][4], uf[4][4];
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const uint4 a = sm.s16[w][ks][lane], c = sm.u16[w][ks][lane];
+        sh[ks][0] = a.x; sh[ks][1] = a.y; sh[ks][2] = a.z; sh[ks][3] = a.w;
+        uf[ks][0] = c.x; uf[ks][1] = c.y; uf[ks][2] = c.z; uf[ks][3] = c.w;
+      }
+      const float4 scales = sm.scales[w][lane];
+      if (n + 1 < part.chunks) bar_arrive(BAR_TAKEN, 2 * GROUP);
+      // O^T = e^G S Q^T + U^T P^T
+      float o[8][4];
+#pragma unroll
+      for (int m = 0; m < 8; ++m) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[m][i] = 0.f;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t f[4];
+          ldm4(f, smem_u32(q) + m * 1024 + (lane4 ^ (half << 6)));
+          mma(o[m], sh[2 * half], f[0], f[1]);
+          mma(o[m], sh[2 * half + 1], f[2], f[3]);
+        }
+        o[m][0] *= grow[m].x * scales.x;
+        o[m][1] *= grow[m].y * scales.x;
+        o[m][2] *= grow[m].x * scales.y;
+        o[m][3] *= grow[m].y * scales.y;
+      }
+#pragma unroll
+      for (int ib = 0; ib < 4; ++ib)
+#pragma unroll
+        for (int jb = 0; jb <= ib; ++jb) {
+          uint32_t f[4];
+          ldm4(f, smem_u32(sm.p) + ib * 2048 + (across0 ^ (jb << 5)));
+          mma(o[2 * ib], uf[jb], f[0], f[1]);
+          mma(o[2 * ib + 1], uf[jb], f[2], f[3]);
+        }
+      // by way of this warp's columns of a tile, out by rows
+#pragma unroll
+      for (int n2 = 0; n2 < 4; ++n2) {
+        uint32_t f[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 fo = *reinterpret_cast<const float2*>(of_o + 16 * n2 + 8 * i + c2);
+          const float(&t)[4] = o[2 * n2 + i];
+          f[2 * i] = pack_bf16x2(t[0] * (fo.x * scales.z), t[1] * (fo.y * scales.z));
+          f[2 * i + 1] = pack_bf16x2(t[2] * (fo.x * scales.w), t[3] * (fo.y * scales.w));
+        }
+        stm4t(smem_u32(sm.o) + unit_at(16 * n2 + ((lane >> 4) << 3) + (lane & 7), 2 * w + ((lane >> 3) & 1)), f[0], f[1], f[2], f[3]);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * i + (lane >> 1), unit = 2 * w + (lane & 1);
+        if (t0 + row < part.len)
+          *(reinterpret_cast<uint4*>(op + size_t(t0 + row) * p.ldo) + unit) = *reinterpret_cast<const uint4*>(sm.o + unit_at(row, unit));
+      }
+      __syncwarp();
     }
   }
 };
 
 template <bool OUT>
-__global__ void __launch_bounds__(256, 2) delta_chunk_kernel(DeltaParams p) {
+__global__ void __launch_bounds__(4 * GROUP, 1) delta_chunk_kernel(DeltaParams p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   ChunkSmem& sm = *reinterpret_cast<ChunkSmem*>(smem_raw);
-  const int warp = warp_index(), lane = threadIdx.x & 31;
-  const int b = blockIdx.x / p.H, h = blockIdx.x % p.H;
+  const int warp = warp_index(), lane = threadIdx.x & 31, w = warp & 3;
+  Part part;
+  part.b = blockIdx.x / p.H;
+  part.h = blockIdx.x % p.H;
+  part.begin = 0;
   pdl_wait();
   pdl_trigger();
-  const int len = sequence_length(p, b), chunks = (len + CHUNK - 1) / CHUNK;
-  if (warp >= 4) {
-    if (chunks > 0) Prepare<OUT>{p, sm, b, h, warp - 4, lane, len}.run(0, chunks);
-    return;
+  part.len = sequence_length(p, part.b);
+  part.chunks = (part.len + CHUNK - 1) / CHUNK;
+  constexpr int TAKERS = OUT ? 2 * GROUP : GROUP;
+  const size_t state = size_t(blockIdx.x) * D * D;
+  switch (warp >> 2) {
+    case 0:
+      Follow<OUT, true>{sm, w, lane}.run(part, p.s_in == nullptr ? nullptr : p.s_in + state, false, p.s_out == nullptr ? nullptr : p.s_out + state,
+                                         BAR_READY, TAKERS);
+      break;
+    case 1:
+      if (OUT) {
+        Outputs{p, sm, part, w, lane}.run();
+        for (int t = part.len + (threadIdx.x - GROUP) / 8; t < p.T; t += GROUP / 8)
+          *(reinterpret_cast<uint4*>(p.o + (size_t(part.b) * p.T + t) * p.ldo + size_t(part.h) * D) + (threadIdx.x & 7)) = make_uint4(0, 0, 0, 0);
+      }
+      break;
+    default:
+      Prepare{p, sm, part, (warp >> 2) - 2, w, lane, TAKERS}.run();
   }
-  const Follow<OUT> f{p, sm, b, h, warp, lane, len};
-  float S[8][4];
-  const size_t at = size_t(blockIdx.x) * D * D + size_t(16 * warp + (lane >> 2)) * D + 2 * (lane & 3);
-#pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    float2 x = make_float2(0.f, 0.f), y = x;
-    if (p.s_in != nullptr) {
-      x = *reinterpret_cast<const float2*>(p.s_in + at + 8 * n);
-      y = *reinterpret_cast<const float2*>(p.s_in + at + 8 * D + 8 * n);
-    }
-    S[n][0] = x.x; S[n][1] = x.y; S[n][2] = y.x; S[n][3] = y.y;
-  }
-  for (int n = 0; n < chunks; ++n) {
-    const int s = n & 1;
-    bar_sync(3 + s, 256);
-    f.chunk(S, sm.stage[s], n * CHUNK);
-    if (n + 2 < chunks) bar_arrive(5 + s, 256);
-  }
-  if (p.s_out != nullptr) {
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      *reinterpret_cast<float2*>(p.s_out + at + 8 * n) = make_float2(S[n][0], S[n][1]);
-      *reinterpret_cast<float2*>(p.s_out + at + 8 * D + 8 * n) = make_float2(S[n][2], S[n][3]);
-    }
-  }
-  if (OUT)
-    for (int t = len + (threadIdx.x >> 3); t < p.T; t += 16)
-      *(reinterpret_cast<uint4*>(p.o + (size_t(b) * p.T + t) * p.ldo + size_t(h) * D) + (threadIdx.x & 7)) = make_uint4(0, 0, 0, 0);
 }
 
 }  // namespace
@@ -819,10 +916,10 @@ int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream)
   if (T >= 24) {
     if (p.o != nullptr) {
       JB_MAX_SMEM(delta_chunk_kernel<true>, sizeof(ChunkSmem));
-      launch_dep(delta_chunk_kernel<true>, B * H, 256, sizeof(ChunkSmem), stream, p);
+      launch_dep(delta_chunk_kernel<true>, B * H, 4 * GROUP, sizeof(ChunkSmem), stream, p);
     } else {
       JB_MAX_SMEM(delta_chunk_kernel<false>, sizeof(ChunkSmem));
-      launch_dep(delta_chunk_kernel<false>, B * H, 256, sizeof(ChunkSmem), stream, p);
+      launch_dep(delta_chunk_kernel<false>, B * H, 4 * GROUP, sizeof(ChunkSmem), stream, p);
     }
     JB_LAUNCH_CHECK("delta_chunk_kernel");
     return JB200_OK;
