@@ -141,45 +141,77 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 // u of a chunk solve a triangular system, and everything else is products of 64 x 64 matrices:
 //   X = b (V - e^G K S^T),   U = T X with T = (I + A)^-1,  A_ij = b_i e^(G_i - G_j) k_i.k_j  (j < i)
 //   O = e^G Q S^T + P U with P_ij = e^(G_i - G_j) q_i.k_j  (j <= i),   S' = e^Gc S + (e^(Gc - G) U)^T K
-// A CTA follows one head of one sequence, in four groups of four warps.  Two take turns in preparing chunks (K, T: nothing of the state); one
-// takes a chunk through the state, each warp 16 value rows of S in its accumulators, everything transposed (X^T, U^T: 16 values x 64 tokens), so that a
-// product's accumulators are the next one's first operand where they are, and the four never wait for one another; one forms P and, from
-// S and U as the state's warps leave them, the outputs.
+// A CTA follows one head of one sequence:
+//   warps 0-3          the state: S in tensor memory (f32, a value row and 32 keys a thread); per chunk three products, K S^T, T X and U^T K, with
+//                      X, U and S back in shared memory as their operands between them: the chain that everything waits for
+//   warps 4-7, 8-11    by turns prepare a chunk, nothing of the state: K and Q as f16, A and T, P
+//   warps 12, 13       output rows from Q S^T and P U, which the state's warps issue beside their own
+// The products are tcgen05.mma, 128 rows at a time: a chunk has 64, so that the operand is there twice (K twice in memory; a second reading
+// of T^T and U, MN-major) and all four of a group's warps find 64 rows x 32 columns in their lanes; for P it is [K; Q], of Q and P as operands
+// the upper half is what happens to follow, in lanes that nobody reads.  T's blocks come from mma.sync: products of 16 x 16.
 //
-// mma.sync, not tcgen05: a chunk is a chain of three dependent products of 16 x 64 x 64 a warp with a rescaling between them; through tensor
-// memory each link would cost a commit, a wait and two copies, several times the product itself.
-//
-// Precision: the state is f32 and stays it.  What is multiplied is f16 in two terms, x = hi + lo (22 bits), with an exact power of two per row that
-// puts the row's largest value near the top of f16's range: 2^-24 of the row's maximum each.  K and Q come as bf16 and fit one term, scaled by
-// a power of two per row; their norms are factors on rows and columns.  X T^T takes hi hi + hi lo + lo hi.  What only the output sees
-// (Q S^T, P U) is one term, 2^-12 of a value where the output's own rounding is 2^-9.
+// Precision: the state is f32 and stays it.  What it is multiplied by and into is f16 in two terms, x = hi + lo (22 bits), at a power of two
+// that brings a bound of its size to 2^15, so that f16's subnormals lie 2^-39 below: |X|, |U| <= 16 max|S| + 130 max|b v| and
+// max|S'| <= 8 e^Gc max|S| + 64 max|b v|, since a (I - b k k^T) with b |k|^2 <= 2 enlarges nothing (rows have 64 entries, a chunk 64 tokens).
+// The bounds need no exchange between warps where the chain would wait for it; typical values lie 2^4 to 2^8 below them.  K and Q come as bf16 and fit one
+// term, with a power of two per row; their norms are factors of rows and columns.  T X is hi hi + hi lo + lo hi.  What only the output sees (Q S^T, P U)
+// is one term, 2^-12 of a value where the output's own rounding is 2^-9.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int CHUNK = 64;
-constexpr int TILE = CHUNK * D * 2;        // bytes of 64 rows of 128, the 16-byte units of row r at unit ^ (r & 7)
+constexpr int TILE = CHUNK * D * 2;        // bytes of 64 rows of 128, the 16-byte units of row r at unit ^ (r & 7): the 128-byte swizzle
 constexpr int STAGES = 3;
-constexpr int GROUP = 128;                 // threads of a group of warps
+constexpr int GROUP = 128;                 // threads of the state's group, of a preparing one
+constexpr int OUT_THREADS = 64;
 constexpr float LEAST_LOG2 = -300.f;       // 2^-300 is 0 in f32: a decay of less, -inf among them, is this one
 
-struct alignas(128) Stage {
-  uint8_t k[TILE], v[TILE];
-  uint8_t t_hi[TILE], t_lo[TILE];          // T^T [j][i] on and above the diagonal's 16 x 16 blocks; -A [i][j] below them while T is formed
-  float diagonal[4][16 * 20];              // the diagonal blocks of -A in f32
-  float g_hi[CHUNK], g_lo[CHUNK], rk[CHUNK], nk[CHUNK], beta[CHUNK];
-  float of_v[CHUNK], of_y[CHUNK], of_u[CHUNK], grow[CHUNK];
+struct alignas(1024) Stage {
+  uint8_t k_again[TILE], k[TILE], q[TILE], p[TILE];    // rows of K twice: K; K and K; Q are 128 rows each
+  uint8_t t_hi[TILE], t_lo[TILE];                      // T^T [j][i], 0 below the diagonal's 16 x 16 blocks
+  float2 column[CHUNK];                                // -G in two terms, the lower one with log2 r: r = k / k16
+  float2 g[CHUNK];                                     // G in two terms
+  float rk[CHUNK], nk[CHUNK], beta[CHUNK];
+  float of_v[CHUNK], of_y[CHUNK], of_u[CHUNK], of_s[CHUNK], of_o[CHUNK];
   float whole;
 };
-struct alignas(128) ChunkSmem {
-  Stage stage[STAGES];
-  uint8_t q[2][TILE], p[TILE], o[TILE];
-  float of_o[2][CHUNK];
-  uint4 s16[4][4][32], u16[4][4][32];      // of every warp of the state: S and U as first operands, lane by lane
-  float4 scales[4][32];
+struct Solve {                                         // of a preparing group
+  uint8_t a_hi[6][512], a_lo[6][512];                  // -A below the diagonal, blocks (1,0) (2,0) (2,1) (3,0) .. of 16 rows of 32 bytes
+  float diagonal[4][16 * 20];                          // its diagonal blocks
 };
-static_assert(sizeof(Stage) % 128 == 0 && TILE % 128 == 0, "tiles are read 16 bytes at a time in every stage");
+struct alignas(1024) ChunkSmem {
+  Stage stage[STAGES];
+  uint8_t s_hi[TILE], s_lo[TILE];                      // S [value][key]
+  uint8_t x_hi[TILE], x_lo[TILE];                      // X, then e^(Gc - G) U, [token][value]
+  uint8_t u[TILE];                                     // U, one term
+  Solve solve[2];
+  float most_s[2][4], most_v[2][4];                    // of every warp of the state
+  float2 inverse[2];                                   // of the powers of S and of X and U
+  unsigned long long bar_y, bar_u, bar_s, bar_o, bar_a[2];
+  uint32_t tmem, abort_flag;
+};
+static_assert(sizeof(Stage) % 1024 == 0, "tiles lie on 1024-byte boundaries");
+constexpr size_t CHUNK_SMEM = sizeof(ChunkSmem) + 1024;
 
+// tensor memory: accumulators of 64 columns
+enum { TM_A = 0 /* + 64 group */, TM_Y = 128, TM_U = 192, TM_S = 256, TM_QS = 320, TM_PU = 384, TM_STATE = 448, TM_COLUMNS = 512 };
+// 8 columns of the thread's lane
+__device__ __forceinline__ void tmem_ld8(uint32_t at, float (&x)[8]) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(at)
+               : "memory");
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st8(uint32_t at, const float (&x)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(__float_as_uint(x[0])), "r"(__float_as_uint(x[1])),
+               "r"(__float_as_uint(x[2])), "r"(__float_as_uint(x[3])), "r"(__float_as_uint(x[4])), "r"(__float_as_uint(x[5])),
+               "r"(__float_as_uint(x[6])), "r"(__float_as_uint(x[7]))
+               : "memory");
+}
 // The CTA's barriers.  Ready and free of a stage: the preparing group arrives and waits, the others wait and arrive.
-enum { BAR_GROUP = 0 /* + group */, BAR_READY = 2 /* + stage: for the state */, BAR_READY_O = 5 /* + stage: for the outputs */, BAR_FREE = 8 /* + stage */,
-       BAR_GIVEN = 11, BAR_TAKEN = 12, BAR_OUT = 13 };
+enum { BAR_GROUP = 1 /* + group */, BAR_STATE = 3, BAR_READY = 4 /* + stage */, BAR_FREE = 7 /* + stage */, BAR_TAKEN = 10, BAR_GIVEN = 11, BAR_PAIR = 12 /* + group */ };
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
@@ -187,9 +219,6 @@ __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
 }
 __device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void stm4t(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -201,120 +230,148 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// (x, y) as two f16 terms each
-__device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
-  hi = pack_f16x2(x, y);
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  lo = pack_f16x2(x - f.x, y - f.y);
+// Two f32 at a time
+__device__ __forceinline__ unsigned long long bits2(float2 x) { return (unsigned long long)(__float_as_uint(x.y)) << 32 | __float_as_uint(x.x); }
+__device__ __forceinline__ float2 float2_of(unsigned long long x) { return make_float2(__uint_as_float(uint32_t(x)), __uint_as_float(uint32_t(x >> 32))); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return float2_of(r);
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+  return float2_of(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+  return float2_of(r);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+// (x, y) as two f16 terms each
+__device__ __forceinline__ void split(float2 x, uint32_t& hi, uint32_t& lo) {
+  hi = pack_f16x2(x.x, x.y);
+  const float2 rest = fma2(__half22float2(*reinterpret_cast<const __half2*>(&hi)), both(-1.f), x);
+  lo = pack_f16x2(rest.x, rest.y);
+}
+__device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) { split(make_float2(x, y), hi, lo); }
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// A power of two s with s m in [2^TO, 2^(TO + 1)) and its inverse; of m = 0, infinities and what is too small any that are finite
-template <int TO>
+// A power of two s with s m in [2^14, 2^15) and its inverse; of m = 0, infinities and what is too small any that are finite
 __device__ __forceinline__ void power_scale(float m, float& s, float& inv) {
-  const int e = max(int(__float_as_uint(m) >> 23), TO + 3);
-  s = __uint_as_float(uint32_t(254 + TO - e) << 23);
-  inv = __uint_as_float(uint32_t(e - TO) << 23);
-}
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+  const int e = max(int(__float_as_uint(m) >> 23), 17);
+  s = __uint_as_float(uint32_t(254 + 14 - e) << 23);
+  inv = __uint_as_float(uint32_t(e - 14) << 23);
 }
 __device__ __forceinline__ uint32_t unit_at(int row, int unit) { return uint32_t(row * 128 + ((unit ^ (row & 7)) << 4)); }
 
-// Lane's address part for four 8 x 8 matrices of a tile.  ACROSS: matrices 0, 1 are neighbouring units (columns), 2, 3 those of the next eight
-// rows; DOWN: 0, 1 are rows r, r + 8 of one unit, 2, 3 those of the next unit.
-__device__ __forceinline__ uint32_t across(int row, int unit, int lane) { return unit_at(row + ((lane >> 4) << 3) + (lane & 7), unit + ((lane >> 3) & 1)); }
-__device__ __forceinline__ uint32_t down(int row, int unit, int lane) { return unit_at(row + (((lane >> 3) & 1) << 3) + (lane & 7), unit + (lane >> 4)); }
+// Operands of tcgen05.mma in the 128-byte swizzle.  K-major (rows of the operand are rows of the tile): 16 elements on are +2 in the address field.
+// MN-major (its rows are the tile's columns): 16 on are 16 rows, +128; `twice`: 64 columns read as rows 0-63 and again as 64-127.
+__device__ __forceinline__ uint64_t operand(const uint8_t* tile, bool twice = false) {
+  return uint64_t((smem_u32(tile) & 0x3FFFFu) >> 4) | uint64_t(twice ? 0 : 64) << 16 | uint64_t(64) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+constexpr uint32_t idesc(int a_mn, int b_mn) {         // f16 operands, f32 sums, 128 x 64
+  return (1u << 4) | uint32_t(a_mn) << 15 | uint32_t(b_mn) << 16 | uint32_t(64 >> 3) << 17 | uint32_t(128 >> 4) << 24;
+}
+// By a whole warp, one lane of it issuing
+template <int A_MN, int B_MN>
+__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, bool add) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (elect_one()) umma_bf16_ss(d, a + uint64_t(i * (A_MN ? 128 : 2)), b + uint64_t(i * (B_MN ? 128 : 2)), idesc(A_MN, B_MN), add || i != 0);
+}
+__device__ __forceinline__ void commit(unsigned long long& bar) {
+  if (elect_one()) umma_commit(smem_u32(&bar));
+  __syncwarp();
+}
 
 // The tokens that a CTA takes: of sequence b from row `begin` (of the sequence) on, `chunks` chunks, none from `len` on.
 struct Part {
   int b, h, begin, len, chunks;
 };
 
-// Sixteen rows of a bf16 matrix a warp, eight lanes a row, four rows a lane: from memory ...
-__device__ __forceinline__ void fetch_rows(uint4 (&x)[4], const __nv_bfloat16* rows, size_t ld, int row0, int n, int lane) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = row0 + 4 * i + (lane >> 3);
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (row < n) x[i] = __ldg(reinterpret_cast<const uint4*>(rows + size_t(row) * ld) + (lane & 7));
-  }
+// 16 bytes that are asked for here and not where they are used (an ordinary read-only load may be moved there, behind barriers and all)
+__device__ __forceinline__ uint4 load_now(const void* p) {
+  uint4 x;
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p) : "memory");
+  return x;
 }
-// ... and to f16 in a tile, times the power of two s that brings their norm into [1, 2); ss: the sum of squares after that.  A sum of squares
-// beyond f32's range makes the row NaN, one below it makes it 0.
-__device__ __forceinline__ void convert_rows(const uint4 (&x)[4], uint8_t* tile, int row0, int lane, float (&ss)[4], float (&s)[4]) {
+__device__ __forceinline__ float load_now(const float* p) {
+  float x;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(x) : "l"(p) : "memory");
+  return x;
+}
+
+// Half a row of a bf16 matrix a thread: from memory ...
+__device__ __forceinline__ void fetch_half(uint4 (&x)[4], const __nv_bfloat16* at, bool on) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = on ? load_now(static_cast<const void*>(at + 8 * i)) : make_uint4(0, 0, 0, 0);
+}
+// ... and to f16 in a tile (`twice`: and in the next one), times the power of two s that brings the row's norm into [1, 2); returns the sum of squares after that.  A sum of
+// squares beyond f32's range makes the row NaN, one below it makes it 0.
+__device__ __forceinline__ float convert_half(const uint4 (&x)[4], uint8_t* tile, bool twice, int row, int half, float& s) {
+  float ss = 0.f, other = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-    float a = 0.f, c = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { a = fmaf(bf16_lo(in[j]), bf16_lo(in[j]), a); c = fmaf(bf16_hi(in[j]), bf16_hi(in[j]), c); }
-    ss[i] = a + c;
+    for (int j = 0; j < 4; ++j) { ss = fmaf(bf16_lo(in[j]), bf16_lo(in[j]), ss); other = fmaf(bf16_hi(in[j]), bf16_hi(in[j]), other); }
   }
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ss[i] += __shfl_xor_sync(0xffffffffu, ss[i], o);
+  ss += other;
+  ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+  const int e = (int(__float_as_uint(ss) >> 23) - 127) >> 1;                     // ss in [4^e, 4^(e + 1))
+  s = __uint_as_float(uint32_t(127 - e) << 23);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int half = (int(__float_as_uint(ss[i]) >> 23) - 127) >> 1;             // ss in [4^half, 4^(half + 1))
-    s[i] = __uint_as_float(uint32_t(127 - half) << 23);
-    ss[i] = ss[i] * s[i] * s[i];
     const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
     uint32_t out[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = pack_f16x2(bf16_lo(in[j]) * s[i], bf16_hi(in[j]) * s[i]);
-    *reinterpret_cast<uint4*>(tile + unit_at(row0 + 4 * i + (lane >> 3), lane & 7)) = make_uint4(out[0], out[1], out[2], out[3]);
+    for (int j = 0; j < 4; ++j) out[j] = pack_f16x2(bf16_lo(in[j]) * s, bf16_hi(in[j]) * s);
+    uint8_t* to = tile + unit_at(row, 4 * half + i);
+    *reinterpret_cast<uint4*>(to) = make_uint4(out[0], out[1], out[2], out[3]);
+    if (twice) *reinterpret_cast<uint4*>(to + TILE) = make_uint4(out[0], out[1], out[2], out[3]);
   }
+  return ss * s * s;
 }
 
-// Blocks on and below the diagonal of a 4 x 4 grid, three or two a warp, the diagonal's first
-__device__ __forceinline__ int blocks_of(int w) { return w < 2 ? 3 : 2; }
-__device__ __forceinline__ int block_row(int w, int i) { return i == 0 ? w : w < 2 ? 1 + i : w == 2 ? 1 : 3; }
-__device__ __forceinline__ int block_col(int w, int i) { return i == 0 ? w : w < 2 ? w : w == 2 ? 0 : 2; }
-
-// A block of rows ib of tile `a` times rows jb of tile `b`, 64 long
-__device__ __forceinline__ void block_products(float (&c)[2][4], const uint8_t* a, int ib, const uint8_t* b, int jb, int lane) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) c[0][i] = c[1][i] = 0.f;
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks) {
-    uint32_t f[4], r[4];
-    ldm4(r, smem_u32(a) + down(16 * ib, 2 * ks, lane));
-    ldm4(f, smem_u32(b) + across(16 * jb, 2 * ks, lane));
-    mma(c[0], r, f[0], f[1]);
-    mma(c[1], r, f[2], f[3]);
-  }
-}
-// ... times f_i r_j e^(G_i - G_j)
-__device__ __forceinline__ void decayed(float (&c)[2][4], const Stage& st, int i0, int jb, float f0, float f1, int lane) {
-  const float gh0 = st.g_hi[i0], gl0 = st.g_lo[i0], gh1 = st.g_hi[i0 + 8], gl1 = st.g_lo[i0 + 8];
-#pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const int j = 16 * jb + 8 * n + 2 * (lane & 3);
-    const float2 gh = *reinterpret_cast<const float2*>(st.g_hi + j), gl = *reinterpret_cast<const float2*>(st.g_lo + j);
-    const float2 r = *reinterpret_cast<const float2*>(st.rk + j);
-    c[n][0] *= f0 * r.x * exp2_fast((gh0 - gh.x) + (gl0 - gl.x));
-    c[n][1] *= f0 * r.y * exp2_fast((gh0 - gh.y) + (gl0 - gl.y));
-    c[n][2] *= f1 * r.x * exp2_fast((gh1 - gh.x) + (gl1 - gl.x));
-    c[n][3] *= f1 * r.y * exp2_fast((gh1 - gh.y) + (gl1 - gl.y));
-  }
-}
-
-// ---- the preparing groups --------------------------------------------------------------------------------------------
-struct Prepare {
+struct Common {
   const DeltaParams& p;
   ChunkSmem& sm;
   Part part;
-  int group, w, lane;
-  int takers;                                // threads that wait for a stage and free it
+  int w, lane;
+  uint32_t tm;                               // tensor memory, this warp's lanes
+  unsigned int* status;
 
-  // running sums of log2 a, in f64 for differences of late tokens
-  __device__ __forceinline__ void gates(Stage& st, float ga, float gb, float beta_a, float beta_b) const {
+  // The waits are bounded; one that runs out leaves its code in the status word, and everybody carries on with what there is.
+  __device__ __forceinline__ void wait(unsigned long long& bar, int n) const {
+    if (!mbar_try_wait(smem_u32(&bar), uint32_t(n) & 1u)) wait_on(smem_u32(&bar), uint32_t(n) & 1u, &sm.abort_flag, status);
+    tc_fence_after_sync();
+  }
+  static __device__ __noinline__ void wait_on(uint32_t bar, uint32_t parity, uint32_t* abort_flag, unsigned int* status) {
+    (void)mbar_wait(bar, parity, abort_flag, status, JB200_STATUS_ATTN_MMA);
+  }
+  // before a group's barrier: what was written is there for the tensor cores, what was read of tensor memory may be overwritten
+  __device__ __forceinline__ static void settle() {
+    fence_proxy_async_smem();
+    tc_fence_before_sync();
+  }
+};
+
+// ---- the preparing groups --------------------------------------------------------------------------------------------
+template <bool OUT>
+struct Prepare : Common {
+  int group;
+
+  // Running sums of log2 a, in f64 for differences of late tokens: of two tokens a lane
+  struct Gates {
+    float2 hi, lo, grow, of_u;
+    float whole;
+  };
+  __device__ __forceinline__ Gates gates(float ga, float gb) const {
     double g0 = double(ga) * 1.4426950408889634, g1 = double(gb) * 1.4426950408889634;
     if (g0 < double(LEAST_LOG2)) g0 = double(LEAST_LOG2);
     if (g1 < double(LEAST_LOG2)) g1 = double(LEAST_LOG2);
@@ -324,27 +381,75 @@ struct Prepare {
       const double up = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += up;
     }
-    const double end = __shfl_sync(0xffffffffu, sum, 31);
-    const double at[2] = {sum - g1, sum};
-    float hi[2], lo[2], grow[2], of_u[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      hi[i] = float(at[i]);
-      lo[i] = float(at[i] - double(hi[i]));
-      grow[i] = exp2f(hi[i]);
-      of_u[i] = exp2f(float(end - at[i]));
-    }
-    *reinterpret_cast<float2*>(st.g_hi + 2 * lane) = make_float2(hi[0], hi[1]);
-    *reinterpret_cast<float2*>(st.g_lo + 2 * lane) = make_float2(lo[0], lo[1]);
-    *reinterpret_cast<float2*>(st.beta + 2 * lane) = make_float2(beta_a, beta_b);
-    *reinterpret_cast<float2*>(st.grow + 2 * lane) = make_float2(grow[0], grow[1]);
-    *reinterpret_cast<float2*>(st.of_u + 2 * lane) = make_float2(of_u[0], of_u[1]);
-    if (lane == 0) st.whole = exp2f(float(end));
+    const double end = __shfl_sync(0xffffffffu, sum, 31), before = sum - g1;
+    Gates x;
+    x.hi = make_float2(float(before), float(sum));
+    x.lo = make_float2(float(before - double(x.hi.x)), float(sum - double(x.hi.y)));
+    x.grow = make_float2(exp2f(x.hi.x), exp2f(x.hi.y));
+    x.of_u = make_float2(exp2f(float(end - before)), exp2f(float(end - sum)));
+    x.whole = exp2f(float(end));
+    return x;
   }
 
-  // the diagonal block's inverse, a column of T (a row of T^T) a lane: t_i = -sum_(j < i) A_ij t_j below t_c = 1
-  __device__ __forceinline__ void diagonal(Stage& st) const {
-    const float* dg = st.diagonal[w];
+  // Eight columns from c on of this thread's row of a product with K^T, times f r_j e^(G_i - G_j); g: G_i in two terms
+  __device__ __forceinline__ void decayed(const Stage& st, int c, float2 g, float f, float (&x)[8]) const {
+    tmem_ld8(tm + TM_A + 64 * group + c, x);
+    const float4* col = reinterpret_cast<const float4*>(st.column + c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float4 at = col[e];
+      const float2 d = add2(add2(both(g.x), make_float2(at.x, at.z)), add2(both(g.y), make_float2(at.y, at.w)));
+      const float2 v = mul2(mul2(make_float2(x[2 * e], x[2 * e + 1]), both(f)), make_float2(exp2_fast(d.x), exp2_fast(d.y)));
+      x[2 * e] = v.x;
+      x[2 * e + 1] = v.y;
+    }
+  }
+
+  // Rows of -A: K K^T is there for two warps a row, which take half of its columns below the diagonal each
+  __device__ __forceinline__ void rows_of_a(const Stage& st, Solve& so) const {
+    const int i = 32 * (w & 1) + lane, ib = i >> 4, row = i & 15, units = 2 + 2 * (w & 1);
+    const float n = st.nk[i], f = -st.beta[i] * n * n * st.rk[i];
+    const float2 g = st.g[i];
+#pragma unroll 1
+    for (int c = (w >> 1) * units * 8, end = c + units * 8; c < end; c += 8) {
+      float x[8];
+      decayed(st, c, g, f, x);
+      const int jb = c >> 4, unit = (c >> 3) & 1;
+      if (jb < ib) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split(x[2 * e], x[2 * e + 1], hi[e], lo[e]);
+        const int at = (ib * (ib - 1) / 2 + jb) * 512 + row * 32 + ((unit ^ ((row >> 2) & 1)) << 4);
+        *reinterpret_cast<uint4*>(so.a_hi[0] + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(so.a_lo[0] + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      } else if (jb == ib) {
+        float* to = so.diagonal[ib] + row * 20 + 8 * unit;
+        *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
+      }
+    }
+  }
+
+  // Rows of P: a row a thread of warps 2, 3
+  __device__ __forceinline__ void rows_of_p(Stage& st) const {
+    const int i = 32 * (w - 2) + lane, reach = 32 * (w - 1);
+    const float2 g = st.g[i];
+#pragma unroll 1
+    for (int c = 0; c < 64; c += 8) {
+      uint32_t v[4] = {};
+      if (c < reach) {
+        float x[8];
+        decayed(st, c, g, 1.f, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = pack_f16x2(c + 2 * e <= i ? x[2 * e] : 0.f, c + 2 * e + 1 <= i ? x[2 * e + 1] : 0.f);
+      }
+      *reinterpret_cast<uint4*>(st.p + unit_at(i, c >> 3)) = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+  }
+
+  // A diagonal block's inverse, a column of T (a row of T^T) a lane: t_i = -sum_(j < i) A_ij t_j below t_c = 1
+  __device__ __forceinline__ void diagonal(Stage& st, const Solve& so) const {
+    const float* dg = so.diagonal[w];
     float t[16];
     const int c = lane & 15;
 #pragma unroll
@@ -361,58 +466,28 @@ struct Prepare {
         if (j & 1) other = fmaf(row[j], t[j], other);
         else sum = fmaf(row[j], t[j], sum);
       }
-      t[i] = i < c ? 0.f : sum + other;
+      t[i] = sum + other;                        // 0 for i < c: so is every t_j of the sum
     }
     if (lane < 16) {
-      uint32_t hi[8], lo[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) split(t[2 * i], t[2 * i + 1], hi[i], lo[i]);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split(t[8 * u + 2 * e], t[8 * u + 2 * e + 1], hi[e], lo[e]);
         const uint32_t at = unit_at(16 * w + c, 2 * w + u);
-        *reinterpret_cast<uint4*>(st.t_hi + at) = make_uint4(hi[4 * u], hi[4 * u + 1], hi[4 * u + 2], hi[4 * u + 3]);
-        *reinterpret_cast<uint4*>(st.t_lo + at) = make_uint4(lo[4 * u], lo[4 * u + 1], lo[4 * u + 2], lo[4 * u + 3]);
+        *reinterpret_cast<uint4*>(st.t_hi + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(st.t_lo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
   }
 
-  // this warp's blocks of -A, the diagonal's inverted
-  __device__ __forceinline__ void blocks_of_a(Stage& st) const {
-    for (int n = 0; n < blocks_of(w); ++n) {
-      const int ib = block_row(w, n), jb = block_col(w, n);
-      float c[2][4];
-      block_products(c, st.k, ib, st.k, jb, lane);
-      const int i0 = 16 * ib + (lane >> 2), i1 = i0 + 8;
-      const float n0 = st.nk[i0], n1 = st.nk[i1];
-      decayed(c, st, i0, jb, -st.beta[i0] * n0 * n0 * st.rk[i0], -st.beta[i1] * n1 * n1 * st.rk[i1], lane);
-      if (n == 0) {
-        float* dg = st.diagonal[w] + (lane >> 2) * 20 + 2 * (lane & 3);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          *reinterpret_cast<float2*>(dg + 8 * i) = make_float2(c[i][0], c[i][1]);
-          *reinterpret_cast<float2*>(dg + 8 * 20 + 8 * i) = make_float2(c[i][2], c[i][3]);
-        }
-        __syncwarp();
-        diagonal(st);
-      } else {
-        const Pair x = as_operand(c);
-        const int col = (lane & 3) * 4;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          *reinterpret_cast<uint32_t*>(st.t_hi + unit_at(i0, 2 * jb + i) + col) = x.hi[2 * i];
-          *reinterpret_cast<uint32_t*>(st.t_lo + unit_at(i0, 2 * jb + i) + col) = x.lo[2 * i];
-          *reinterpret_cast<uint32_t*>(st.t_hi + unit_at(i1, 2 * jb + i) + col) = x.hi[2 * i + 1];
-          *reinterpret_cast<uint32_t*>(st.t_lo + unit_at(i1, 2 * jb + i) + col) = x.lo[2 * i + 1];
-        }
-      }
-    }
-  }
-
-  struct Pair { uint32_t hi[4], lo[4]; };     // a 16 x 16 block as first operand, in two terms
-  __device__ __forceinline__ Pair first_operand(const Stage& st, int rb, int cb) const {
+  // Blocks of 16 x 16 by mma.sync.  Everything is transposed, so that a product's accumulators are the next one's first operand.
+  struct Pair { uint32_t hi[4], lo[4]; };     // a first operand in two terms
+  __device__ __forceinline__ Pair t_block(const Stage& st, int i, int j) const {      // T_ij^T
     Pair x;
-    ldm4(x.hi, smem_u32(st.t_hi) + down(16 * rb, 2 * cb, lane));
-    ldm4(x.lo, smem_u32(st.t_lo) + down(16 * rb, 2 * cb, lane));
+    const uint32_t at = unit_at(16 * j + (((lane >> 3) & 1) << 3) + (lane & 7), 2 * i + (lane >> 4));
+    ldm4(x.hi, smem_u32(st.t_hi) + at);
+    ldm4(x.lo, smem_u32(st.t_lo) + at);
     return x;
   }
   __device__ __forceinline__ static Pair as_operand(const float (&c)[2][4]) {
@@ -431,18 +506,21 @@ struct Prepare {
     mma(c[0], a.lo, hi[0], hi[1]);
     mma(c[1], a.lo, hi[2], hi[3]);
   }
-  // c += x (-A_il)^T, -A stored by rows i
-  __device__ __forceinline__ void times_a(float (&c)[2][4], const Pair& x, const Stage& st, int i, int l) const {
+  // c += x (-A_il)^T, by rows i
+  __device__ __forceinline__ void times_a(float (&c)[2][4], const Pair& x, const Solve& so, int i, int l) const {
     uint32_t hi[4], lo[4];
-    ldm4(hi, smem_u32(st.t_hi) + across(16 * i, 2 * l, lane));
-    ldm4(lo, smem_u32(st.t_lo) + across(16 * i, 2 * l, lane));
+    const int row = ((lane >> 4) << 3) + (lane & 7), unit = (lane >> 3) & 1, block = i * (i - 1) / 2 + l;
+    const uint32_t at = block * 512 + row * 32 + ((unit ^ ((row >> 2) & 1)) << 4);
+    ldm4(hi, smem_u32(so.a_hi) + at);
+    ldm4(lo, smem_u32(so.a_lo) + at);
     mma3(c, x, hi, lo);
   }
-  // c += x T_il^T, T^T stored by rows l
+  // c += x T_il^T, T^T by rows l
   __device__ __forceinline__ void times_t(float (&c)[2][4], const Pair& x, const Stage& st, int i, int l) const {
     uint32_t hi[4], lo[4];
-    ldm4t(hi, smem_u32(st.t_hi) + down(16 * l, 2 * i, lane));
-    ldm4t(lo, smem_u32(st.t_lo) + down(16 * l, 2 * i, lane));
+    const uint32_t at = unit_at(16 * l + (((lane >> 3) & 1) << 3) + (lane & 7), 2 * i + (lane >> 4));
+    ldm4t(hi, smem_u32(st.t_hi) + at);
+    ldm4t(lo, smem_u32(st.t_lo) + at);
     mma3(c, x, hi, lo);
   }
   __device__ __forceinline__ void store_t(const float (&c)[2][4], Stage& st, int i, int j) const {
@@ -460,28 +538,27 @@ struct Prepare {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[0][i] = c[1][i] = 0.f;
   }
-
   // T's blocks off the diagonal from those on it, by halves: T_10 and T_32 first (warps 0, 1), then columns 0 and 1 of the lower left quarter:
   //   [T_20 T_21; T_30 T_31] = -[T_22 0; T_32 T_33] [A_20 A_21; A_30 A_31] [T_00 0; T_10 T_11]
-  __device__ __forceinline__ void off_diagonal(Stage& st) const {
-    if (w < 2) {
+  __device__ __forceinline__ void off_diagonal(Stage& st, const Solve& so) const {
+    {
       float c[2][4];
       zero(c);
-      times_a(c, first_operand(st, 2 * w, 2 * w), st, 2 * w + 1, 2 * w);
+      times_a(c, t_block(st, 2 * w, 2 * w), so, 2 * w + 1, 2 * w);
       const Pair x = as_operand(c);
       zero(c);
       times_t(c, x, st, 2 * w + 1, 2 * w + 1);
       store_t(c, st, 2 * w + 1, 2 * w);
     }
-    bar_sync(BAR_GROUP + group, GROUP);
-    if (w < 2) {
+    bar_sync(BAR_PAIR + group, GROUP / 2);
+    {
       float m2[2][4], m3[2][4];
       zero(m2);
       zero(m3);
       for (int l = w; l < 2; ++l) {
-        const Pair t = first_operand(st, w, l);
-        times_a(m2, t, st, 2, l);
-        times_a(m3, t, st, 3, l);
+        const Pair t = t_block(st, l, w);
+        times_a(m2, t, so, 2, l);
+        times_a(m3, t, so, 3, l);
       }
       const Pair a2 = as_operand(m2), a3 = as_operand(m3);
       zero(m2);
@@ -497,368 +574,340 @@ struct Prepare {
   __device__ __forceinline__ void run() const {
     const size_t first = size_t(part.b) * p.T;
     const __nv_bfloat16* kp = p.k + first * p.ldk + size_t(part.h / p.per_key) * D;
-    const __nv_bfloat16* vp = p.v + first * p.ldv + size_t(part.h) * D;
-    uint4 k[4];
+    const __nv_bfloat16* qp = p.q + first * p.ldq + size_t(part.h / p.per_key) * D;
+    Solve& so = sm.solve[group];
+    const int row = 16 * w + (lane >> 1), half = lane & 1;
+    uint4 k[4], q[4];
     float g0 = 0.f, g1 = 0.f, b0 = 0.f, b1 = 0.f;
     auto fetch = [&](int t0) {
-      fetch_rows(k, kp, p.ldk, t0 + 16 * w, part.len, lane);
+      const int at = t0 + row;
+      fetch_half(k, kp + size_t(at) * p.ldk + 32 * half, at < part.len);
+      if (OUT) fetch_half(q, qp + size_t(at) * p.ldq + 32 * half, at < part.len);
       if (w == 3) {
         const int t = t0 + 2 * lane;
-        g0 = t < part.len ? __ldg(p.log_decay + (first + t) * p.ldg + part.h) : 0.f;
-        b0 = t < part.len ? __ldg(p.beta + (first + t) * p.ldg + part.h) : 0.f;
-        g1 = t + 1 < part.len ? __ldg(p.log_decay + (first + t + 1) * p.ldg + part.h) : 0.f;
-        b1 = t + 1 < part.len ? __ldg(p.beta + (first + t + 1) * p.ldg + part.h) : 0.f;
+        g0 = t < part.len ? load_now(p.log_decay + (first + t) * p.ldg + part.h) : 0.f;
+        b0 = t < part.len ? load_now(p.beta + (first + t) * p.ldg + part.h) : 0.f;
+        g1 = t + 1 < part.len ? load_now(p.log_decay + (first + t + 1) * p.ldg + part.h) : 0.f;
+        b1 = t + 1 < part.len ? load_now(p.beta + (first + t + 1) * p.ldg + part.h) : 0.f;
       }
     };
+    Gates x = {};
     if (group < part.chunks) fetch(part.begin + group * CHUNK);
-    for (int n = group; n < part.chunks; n += 2) {
+    if (w == 3) x = gates(g0, g1);
+    for (int n = group, uses = 0; n < part.chunks; n += 2) {
       const int s = n % STAGES, t0 = part.begin + n * CHUNK;
       Stage& st = sm.stage[s];
-      if (n >= STAGES) bar_sync(BAR_FREE + s, GROUP + takers);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {              // V as it is
-        const int row = 16 * w + 4 * i + (lane >> 3), unit = lane & 7;
-        uint8_t* to = st.v + unit_at(row, unit);
-        if (t0 + row < part.len) copy_async_16(smem_u32(to), vp + size_t(t0 + row) * p.ldv + unit * 8);
-        else *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
+      if (n >= STAGES) bar_sync(BAR_FREE + s, 2 * GROUP + (OUT ? OUT_THREADS : 0));
+      if (w == 3) {
+        *reinterpret_cast<float2*>(st.beta + 2 * lane) = make_float2(b0, b1);
+        *reinterpret_cast<float2*>(st.of_s + 2 * lane) = x.grow;
+        *reinterpret_cast<float2*>(st.of_u + 2 * lane) = x.of_u;
+        *reinterpret_cast<float4*>(&st.g[2 * lane]) = make_float4(x.hi.x, x.lo.x, x.hi.y, x.lo.y);
+        if (lane == 0) st.whole = x.whole;
       }
-      float ss[4], sc[4];
-      convert_rows(k, st.k, 16 * w, lane, ss, sc);
-      if ((lane & 7) == 0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
+#pragma unroll 1
+      for (int m = 0; m < (OUT ? 2 : 1); ++m) {  // K twice, Q
+        float sc;
+        const float ss = convert_half(k, m == 0 ? st.k_again : st.q, m == 0, row, half, sc);
+        if (half == 0) {
           // k = n (k16 r) with |k16 r| = 1, or of the normalised key n = 1 and k16 r its value
-          const int row = 16 * w + 4 * i + (lane >> 3);
-          const float r = p.normalize ? rsqrtf(fmaf(NORM_EPS * sc[i], sc[i], ss[i])) : ss[i] > 0.f ? rsqrtf(ss[i]) : 0.f;
-          st.rk[row] = r;
-          st.nk[row] = p.normalize ? 1.f : ss[i] * r / sc[i];
+          const float r = p.normalize ? rsqrtf(fmaf(NORM_EPS * sc, sc, ss)) : ss > 0.f ? rsqrtf(ss) : 0.f;
+          if (m == 0) {
+            st.rk[row] = r;
+            st.nk[row] = p.normalize ? 1.f : ss * r / sc;
+          } else {
+            st.of_o[row] = p.scale * (p.normalize ? r : 1.f / sc);
+          }
         }
-      }
-      if (w == 3) gates(st, g0, g1, b0, b1);
-      if (n + 2 < part.chunks) fetch(t0 + 2 * CHUNK);
-      bar_sync(BAR_GROUP + group, GROUP);
-      blocks_of_a(st);
-      if (w == 2) {
+        if (OUT && m == 0) {
+          settle();
+          bar_sync(BAR_GROUP + group, GROUP);
+          if (w == 0) {
+            tc_fence_after_sync();
+            product<0, 0>(sm.tmem + TM_A + 64 * group, operand(st.k_again), operand(st.k), false);
+            commit(sm.bar_a[group]);
+          }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = lane + 32 * i;
-          const float r = st.rk[row], n1 = st.nk[row], beta = st.beta[row];
-          st.of_v[row] = beta * n1;
-          st.of_y[row] = beta * n1 * n1 * st.grow[row] * r;
-          st.of_u[row] *= r;
+          for (int i = 0; i < 4; ++i) k[i] = q[i];
         }
       }
+      if (!OUT) {
+        settle();
+        bar_sync(BAR_GROUP + group, GROUP);
+        if (w == 0) {
+          tc_fence_after_sync();
+          product<0, 0>(sm.tmem + TM_A + 64 * group, operand(st.k_again), operand(st.k), false);
+          commit(sm.bar_a[group]);
+        }
+      }
+      if (n + 2 < part.chunks) fetch(t0 + 2 * CHUNK);
+      if (w >= 2) {                              // b v - b e^G r K S^T, its share of U^T K
+        const int i = 32 * (w - 2) + lane;
+        const float r = st.rk[i], n1 = st.nk[i], beta = st.beta[i];
+        const float2 g = st.g[i];
+        st.column[i] = make_float2(-g.x, __log2f(r) - g.y);
+        st.of_v[i] = beta * n1;
+        st.of_y[i] = beta * n1 * n1 * st.of_s[i] * r;
+        st.of_u[i] *= r;
+      }
+      settle();
       bar_sync(BAR_GROUP + group, GROUP);
-      off_diagonal(st);
-      copy_async_wait();
+      wait(sm.bar_a[group], uses++);
+      rows_of_a(st, so);
+      settle();
+      bar_sync(BAR_GROUP + group, GROUP);
+      if (OUT && w == 2) {
+        tc_fence_after_sync();
+        product<0, 0>(sm.tmem + TM_A + 64 * group, operand(st.k), operand(st.k), false);
+        commit(sm.bar_a[group]);
+      }
+      diagonal(st, so);
+      bar_sync(BAR_GROUP + group, GROUP);
+      if (w < 2) {
+        off_diagonal(st, so);
+        if (OUT) ++uses;
+      } else {
+        if (OUT) {
+          st.of_s[32 * (w - 2) + lane] *= st.of_o[32 * (w - 2) + lane];
+          wait(sm.bar_a[group], uses++);
+          rows_of_p(st);
+        }
+        if (w == 3) x = gates(g0, g1);
+      }
+      settle();
       bar_arrive(BAR_READY + s, 2 * GROUP);
-      if (takers == 2 * GROUP) bar_arrive(BAR_READY_O + s, 2 * GROUP);
     }
   }
 };
 
 // ---- the group of the state ------------------------------------------------------------------------------------------
-// OUT: gives S and U to the group of the outputs.  VALUES: false where v counts as 0.
-template <bool OUT, bool VALUES>
-struct Follow {
-  ChunkSmem& sm;
-  int w, lane;
-
-  // S: accumulators of 16 x 64, times inv0 (rows lane / 4) and inv1 (those and eight) the state
-  __device__ __forceinline__ void chunk(float (&S)[8][4], float& inv0, float& inv1, Stage& st, bool wait) const {
-    const int c2 = 2 * (lane & 3);
-    // S in two terms
-    float m0 = 0.f, m1 = 0.f;
+template <bool OUT>
+struct Follow : Common {
+  // Eight values of a row in two terms
+  __device__ __forceinline__ static void put(const float2 (&x)[4], float f, uint8_t* hi_tile, uint8_t* lo_tile, uint32_t at) {
+    uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      m0 = fmaxf(m0, fmaxf(fabsf(S[n][0]), fabsf(S[n][1])));
-      m1 = fmaxf(m1, fmaxf(fabsf(S[n][2]), fabsf(S[n][3])));
-    }
-    m0 = quad_max(m0) * inv0;
-    m1 = quad_max(m1) * inv1;
-    float s0, s1, is0, is1;
-    power_scale<14>(m0, s0, is0);
-    power_scale<14>(m1, s1, is1);
-    s0 *= inv0;
-    s1 *= inv1;
-    uint32_t sh[4][4], sl[4][4];
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      split(S[2 * ks][0] * s0, S[2 * ks][1] * s0, sh[ks][0], sl[ks][0]);
-      split(S[2 * ks][2] * s1, S[2 * ks][3] * s1, sh[ks][1], sl[ks][1]);
-      split(S[2 * ks + 1][0] * s0, S[2 * ks + 1][1] * s0, sh[ks][2], sl[ks][2]);
-      split(S[2 * ks + 1][2] * s1, S[2 * ks + 1][3] * s1, sh[ks][3], sl[ks][3]);
-    }
-    if (OUT && wait) bar_sync(BAR_TAKEN, 2 * GROUP);
-    if constexpr (OUT)
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) sm.s16[w][ks][lane] = make_uint4(sh[ks][0], sh[ks][1], sh[ks][2], sh[ks][3]);
-    // Y^T = S K^T
-    float y[8][4];
-    const uint32_t kb = smem_u32(st.k), lane4 = unit_at(lane & 7, lane >> 3);   // four neighbouring units of eight rows
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[n][i] = 0.f;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t f[4];
-        ldm4(f, kb + n * 1024 + (lane4 ^ (half << 6)));
-        mma(y[n], sh[2 * half], f[0], f[1]);
-        mma(y[n], sh[2 * half + 1], f[2], f[3]);
-        mma(y[n], sl[2 * half], f[0], f[1]);
-        mma(y[n], sl[2 * half + 1], f[2], f[3]);
-      }
-    }
-    // X^T = b (V - e^G Y)
-    float x0 = m0 * 8.6736174e-19f, x1 = m1 * 8.6736174e-19f;      // 2^-60: X's power must leave S in range, too
-#pragma unroll
-    for (int n2 = 0; n2 < 4; ++n2) {
-      uint32_t f[4] = {};
-      if constexpr (VALUES) ldm4t(f, smem_u32(st.v) + unit_at(16 * n2 + ((lane >> 4) << 3) + (lane & 7), 2 * w + ((lane >> 3) & 1)));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float(&t)[4] = y[2 * n2 + i];
-        const int j = 16 * n2 + 8 * i + c2;
-        const float2 fv = *reinterpret_cast<const float2*>(st.of_v + j), fy = *reinterpret_cast<const float2*>(st.of_y + j);
-        t[0] = fmaf(fv.x, bf16_lo(f[2 * i]), -(fy.x * is0) * t[0]);
-        t[1] = fmaf(fv.y, bf16_hi(f[2 * i]), -(fy.y * is0) * t[1]);
-        t[2] = fmaf(fv.x, bf16_lo(f[2 * i + 1]), -(fy.x * is1) * t[2]);
-        t[3] = fmaf(fv.y, bf16_hi(f[2 * i + 1]), -(fy.y * is1) * t[3]);
-        x0 = fmaxf(x0, fmaxf(fabsf(t[0]), fabsf(t[1])));
-        x1 = fmaxf(x1, fmaxf(fabsf(t[2]), fabsf(t[3])));
-      }
-    }
-    // |T_ij| <= 2 where b |k|^2 <= 2, so that U <= 128 X stays in range
-    float e0, e1, ie0, ie1;
-    power_scale<7>(quad_max(x0), e0, ie0);
-    power_scale<7>(quad_max(x1), e1, ie1);
-    uint32_t xh[4][4], xl[4][4];
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      split(y[2 * ks][0] * e0, y[2 * ks][1] * e0, xh[ks][0], xl[ks][0]);
-      split(y[2 * ks][2] * e1, y[2 * ks][3] * e1, xh[ks][1], xl[ks][1]);
-      split(y[2 * ks + 1][0] * e0, y[2 * ks + 1][1] * e0, xh[ks][2], xl[ks][2]);
-      split(y[2 * ks + 1][2] * e1, y[2 * ks + 1][3] * e1, xh[ks][3], xl[ks][3]);
-    }
-    // U^T = X^T T^T, times the row's power
-    float u[8][4];
-    const uint32_t down0 = down(0, 0, lane);
-#pragma unroll
-    for (int ib = 0; ib < 4; ++ib) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) u[2 * ib][i] = u[2 * ib + 1][i] = 0.f;
-#pragma unroll
-      for (int jb = 0; jb <= ib; ++jb) {
-        uint32_t f[4];
-        ldm4t(f, smem_u32(st.t_hi) + jb * 2048 + (down0 ^ (ib << 5)));
-        mma(u[2 * ib], xh[jb], f[0], f[1]);
-        mma(u[2 * ib + 1], xh[jb], f[2], f[3]);
-        mma(u[2 * ib], xl[jb], f[0], f[1]);
-        mma(u[2 * ib + 1], xl[jb], f[2], f[3]);
-        ldm4t(f, smem_u32(st.t_lo) + jb * 2048 + (down0 ^ (ib << 5)));
-        mma(u[2 * ib], xh[jb], f[0], f[1]);
-        mma(u[2 * ib + 1], xh[jb], f[2], f[3]);
-      }
-    }
-    if constexpr (OUT) {
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-        sm.u16[w][ks][lane] = make_uint4(pack_f16x2(u[2 * ks][0], u[2 * ks][1]), pack_f16x2(u[2 * ks][2], u[2 * ks][3]),
-                                         pack_f16x2(u[2 * ks + 1][0], u[2 * ks + 1][1]), pack_f16x2(u[2 * ks + 1][2], u[2 * ks + 1][3]));
-      sm.scales[w][lane] = make_float4(is0 * e0, is1 * e1, ie0, ie1);
-      bar_arrive(BAR_GIVEN, 2 * GROUP);
-    }
-    // S' = e^Gc S + (e^(Gc - G) U)^T K, at X's power
-    const float whole = st.whole;
-    const float k0 = whole * (e0 * inv0), k1 = whole * (e1 * inv1);
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      S[n][0] *= k0; S[n][1] *= k0; S[n][2] *= k1; S[n][3] *= k1;
-    }
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      uint32_t uh[4], ul[4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float2 fu = *reinterpret_cast<const float2*>(st.of_u + 16 * ks + 8 * i + c2);
-        const float(&t)[4] = u[2 * ks + i];
-        split(t[0] * fu.x, t[1] * fu.y, uh[2 * i], ul[2 * i]);
-        split(t[2] * fu.x, t[3] * fu.y, uh[2 * i + 1], ul[2 * i + 1]);
-      }
-#pragma unroll
-      for (int n2 = 0; n2 < 4; ++n2) {
-        uint32_t f[4];
-        ldm4t(f, kb + ks * 2048 + (down0 ^ (n2 << 5)));
-        mma(S[2 * n2], uh, f[0], f[1]);
-        mma(S[2 * n2 + 1], uh, f[2], f[3]);
-        mma(S[2 * n2], ul, f[0], f[1]);
-        mma(S[2 * n2 + 1], ul, f[2], f[3]);
-      }
-    }
-    inv0 = ie0;
-    inv1 = ie1;
+    for (int e = 0; e < 4; ++e) split(mul2(x[e], both(f)), hi[e], lo[e]);
+    *reinterpret_cast<uint4*>(hi_tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(lo_tile + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
+  __device__ __forceinline__ static float most(const float (&m)[4]) { return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])); }
+  __device__ __forceinline__ static float warp_most(float m) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))); }
 
-  // from `from` (null: 0; `one`: the identity) through the part's chunks to `to` (or nowhere)
-  __device__ __forceinline__ void run(const Part& part, const float* from, bool one, float* to, int ready, int takers) const {
-    float S[8][4];
-    const int row = 16 * w + (lane >> 2), at = row * D + 2 * (lane & 3);
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      float2 x = make_float2(0.f, 0.f), y = x;
+  // The loops over a thread's 32 columns stay loops: the roles of this kernel share the instruction caches, and unrolled (77 KB in all) every one of
+  // them waited for its instructions (a chunk took 9600 cycles on 128 SMs).
+  __device__ __forceinline__ void run(const float* from, float* to) const {
+    const int row = 32 * (w & 1) + lane, half = w >> 1;          // a value (S) or a token (X, U), and which 32 keys or values of it
+    const uint32_t cols = tm + 32 * half;
+    const __nv_bfloat16* vp = p.v + size_t(part.b) * p.T * p.ldv + size_t(part.h) * D + 32 * half;
+    uint4 v[4];
+    if (part.chunks > 0) fetch_half(v, vp + size_t(part.begin + row) * p.ldv, part.begin + row < part.len);
+    // the state before the first chunk is the product of none: TM_S
+    float m = 0.f;
+#pragma unroll 1
+    for (int c = 0; c < 32; c += 8) {
+      float x[8] = {};
+      tmem_st8(cols + TM_STATE + c, x);
       if (from != nullptr) {
-        x = *reinterpret_cast<const float2*>(from + at + 8 * n);
-        y = *reinterpret_cast<const float2*>(from + at + 8 * D + 8 * n);
-      } else if (one) {
-        const int d = row - 8 * n - 2 * (lane & 3);
-        x = make_float2(d == 0, d == 1);
-        y = make_float2(d == -8, d == -7);
+        const float4* at = reinterpret_cast<const float4*>(from + row * D + 32 * half + c);
+        const float4 a = at[0], b = at[1];
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
       }
-      S[n][0] = x.x; S[n][1] = x.y; S[n][2] = y.x; S[n][3] = y.y;
+      tmem_st8(cols + TM_S + c, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
     }
-    float inv0 = 1.f, inv1 = 1.f;
-    for (int n = 0; n < part.chunks; ++n) {
+    tmem_st_wait();
+    m = warp_most(m);
+    if (lane == 0) sm.most_s[1][w] = m;
+    bar_sync(BAR_STATE, GROUP);
+    float bound = most(sm.most_s[1]), ix = 1.f, whole = 0.f;
+    for (int n = 0;; ++n) {
+      float ps, is, px;
+      power_scale(bound, ps, is);
+      m = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < 32; c += 8) {
+        float x[8], y[8];
+        tmem_ld8(cols + TM_STATE + c, x);
+        tmem_ld8(cols + TM_S + c, y);
+        float2 z[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          z[e] = fma2(make_float2(y[2 * e], y[2 * e + 1]), both(ix), mul2(make_float2(x[2 * e], x[2 * e + 1]), both(whole)));
+          m = fmaxf(m, fmaxf(fabsf(z[e].x), fabsf(z[e].y)));
+          x[2 * e] = z[e].x;
+          x[2 * e + 1] = z[e].y;
+        }
+        tmem_st8(cols + TM_STATE + c, x);
+        put(z, ps, sm.s_hi, sm.s_lo, unit_at(row, 4 * half + (c >> 3)));
+      }
+      tmem_st_wait();
+      if (n == part.chunks) break;
       const int s = n % STAGES;
-      bar_sync(ready + s, 2 * GROUP);
-      chunk(S, inv0, inv1, sm.stage[s], n > 0);
-      if (n + STAGES < part.chunks) bar_arrive(BAR_FREE + s, GROUP + takers);
+      Stage& st = sm.stage[s];
+      bar_sync(BAR_READY + s, 2 * GROUP);
+      m = warp_most(m);
+      uint32_t m2 = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t m4 = 0x7fff7fffu;
+        m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(v[i].x & m4, v[i].y & m4), __vmaxu2(v[i].z & m4, v[i].w & m4)));
+      }
+      const float fv = st.of_v[row], mv = warp_most(fabsf(fv) * fmaxf(bf16_lo(m2), bf16_hi(m2)));
+      if (lane == 0) {
+        sm.most_s[n & 1][w] = m;
+        sm.most_v[n & 1][w] = mv;
+      }
+      settle();
+      if (OUT && n > 0) bar_sync(BAR_TAKEN, GROUP + OUT_THREADS);
+      else bar_sync(BAR_STATE, GROUP);
+      if (w == 0) {
+        tc_fence_after_sync();
+        product<0, 0>(sm.tmem + TM_Y, operand(st.k_again), operand(sm.s_hi), false);
+        product<0, 0>(sm.tmem + TM_Y, operand(st.k_again), operand(sm.s_lo), true);
+        commit(sm.bar_y);
+        if (OUT) product<0, 0>(sm.tmem + TM_QS, operand(st.q), operand(sm.s_hi), false);
+      }
+      const float ms = most(sm.most_s[n & 1]), mb = most(sm.most_v[n & 1]);
+      power_scale(fmaxf(fmaf(16.f, ms, 130.f * mb), bound * 7.8886091e-31f), px, ix);      // 2^-100: the powers' quotient stays in range
+      whole = st.whole;
+      bound = fmaf(8.f * whole, ms, 64.f * mb);
+      const float fx = fv * px, fy = st.of_y[row] * (is * px), fu = st.of_u[row];
+      if (OUT && threadIdx.x == 0) sm.inverse[n & 1] = make_float2(is, ix);
+      wait(sm.bar_y, n);
+      if (n > 0 && n - 1 + STAGES < part.chunks) bar_arrive(BAR_FREE + (n - 1) % STAGES, 2 * GROUP + (OUT ? OUT_THREADS : 0));
+#pragma unroll 1
+      for (int c = 0; c < 32; c += 8) {
+        float x[8];
+        tmem_ld8(cols + TM_Y + c, x);
+        const uint32_t in[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+        v[0] = v[1];
+        v[1] = v[2];
+        v[2] = v[3];
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          split(fma2(make_float2(x[2 * e], x[2 * e + 1]), both(-fy), mul2(make_float2(bf16_lo(in[e]), bf16_hi(in[e])), both(fx))), hi[e], lo[e]);
+        const uint32_t at = unit_at(row, 4 * half + (c >> 3));
+        *reinterpret_cast<uint4*>(sm.x_hi + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(sm.x_lo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      settle();
+      bar_sync(BAR_STATE, GROUP);
+      if (w == 0) {
+        tc_fence_after_sync();
+        product<1, 1>(sm.tmem + TM_U, operand(st.t_hi, true), operand(sm.x_hi), false);
+        product<1, 1>(sm.tmem + TM_U, operand(st.t_hi, true), operand(sm.x_lo), true);
+        product<1, 1>(sm.tmem + TM_U, operand(st.t_lo, true), operand(sm.x_hi), true);
+        commit(sm.bar_u);
+      }
+      if (n + 1 < part.chunks) {
+        const int t = part.begin + (n + 1) * CHUNK + row;
+        fetch_half(v, vp + size_t(t) * p.ldv, t < part.len);
+      }
+      wait(sm.bar_u, n);
+#pragma unroll 1
+      for (int c = 0; c < 32; c += 8) {
+        float x[8];
+        tmem_ld8(cols + TM_U + c, x);
+        const uint32_t at = unit_at(row, 4 * half + (c >> 3));
+        if (OUT)
+          *reinterpret_cast<uint4*>(sm.u + at) =
+              make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
+        const float2 z[4] = {make_float2(x[0], x[1]), make_float2(x[2], x[3]), make_float2(x[4], x[5]), make_float2(x[6], x[7])};
+        put(z, fu, sm.x_hi, sm.x_lo, at);
+      }
+      settle();
+      bar_sync(BAR_STATE, GROUP);
+      if (OUT) bar_arrive(BAR_GIVEN, GROUP + OUT_THREADS);
+      if (w == 0) {
+        tc_fence_after_sync();
+        product<1, 1>(sm.tmem + TM_S, operand(sm.x_hi, true), operand(st.k), false);
+        product<1, 1>(sm.tmem + TM_S, operand(sm.x_lo, true), operand(st.k), true);
+        commit(sm.bar_s);
+        if (OUT) {
+          product<0, 1>(sm.tmem + TM_PU, operand(st.p), operand(sm.u), false);
+          commit(sm.bar_o);
+        }
+      }
+      wait(sm.bar_s, n);
     }
     if (to != nullptr) {
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        *reinterpret_cast<float2*>(to + at + 8 * n) = make_float2(S[n][0] * inv0, S[n][1] * inv0);
-        *reinterpret_cast<float2*>(to + at + 8 * D + 8 * n) = make_float2(S[n][2] * inv1, S[n][3] * inv1);
+#pragma unroll 1
+      for (int c = 0; c < 32; c += 8) {
+        float x[8];
+        tmem_ld8(cols + TM_STATE + c, x);
+        float4* at = reinterpret_cast<float4*>(to + row * D + 32 * half + c);
+        at[0] = make_float4(x[0], x[1], x[2], x[3]);
+        at[1] = make_float4(x[4], x[5], x[6], x[7]);
       }
     }
   }
 };
 
-// ---- the group of the outputs ----------------------------------------------------------------------------------------
-struct Outputs {
-  const DeltaParams& p;
-  ChunkSmem& sm;
-  Part part;
-  int w, lane;
-
-  __device__ __forceinline__ void blocks_of_p(const uint8_t* q, const Stage& st) const {
-    for (int n = 0; n < blocks_of(w); ++n) {
-      const int ib = block_row(w, n), jb = block_col(w, n), i0 = 16 * ib + (lane >> 2), col = (lane & 3) * 4;
-      float c[2][4];
-      block_products(c, q, ib, st.k, jb, lane);
-      decayed(c, st, i0, jb, 1.f, 1.f, lane);
-      if (n == 0) {                            // above the diagonal nothing
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int d = (lane >> 2) - 8 * i - 2 * (lane & 3);
-          if (d < 0) c[i][0] = 0.f;
-          if (d < 1) c[i][1] = 0.f;
-          if (d < -8) c[i][2] = 0.f;
-          if (d < -7) c[i][3] = 0.f;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        *reinterpret_cast<uint32_t*>(sm.p + unit_at(i0, 2 * jb + i) + col) = pack_f16x2(c[i][0], c[i][1]);
-        *reinterpret_cast<uint32_t*>(sm.p + unit_at(i0 + 8, 2 * jb + i) + col) = pack_f16x2(c[i][2], c[i][3]);
-      }
-    }
-  }
-
+// ---- the outputs: a token a thread --------------------------------------------------------------------------------------
+struct Outputs : Common {
   __device__ __forceinline__ void run() const {
-    const size_t first = size_t(part.b) * p.T;
-    const __nv_bfloat16* qp = p.q + first * p.ldq + size_t(part.h / p.per_key) * D;
-    __nv_bfloat16* op = p.o + first * p.ldo + size_t(part.h) * D;
-    const int c2 = 2 * (lane & 3);
-    const uint32_t lane4 = unit_at(lane & 7, lane >> 3), across0 = across(0, 0, lane);
-    uint4 x[4];
-    if (part.chunks > 0) fetch_rows(x, qp, p.ldq, part.begin + 16 * w, part.len, lane);
+    __nv_bfloat16* op = p.o + size_t(part.b) * p.T * p.ldo + size_t(part.h) * D;
+    const int row = 32 * w + lane;
     for (int n = 0; n < part.chunks; ++n) {
-      const int s = n % STAGES, t0 = part.begin + n * CHUNK;
+      const int s = n % STAGES, t = part.begin + n * CHUNK + row;
       const Stage& st = sm.stage[s];
-      uint8_t* q = sm.q[n & 1];                // the other one may still be read
-      float* of_o = sm.of_o[n & 1];
-      float ss[4], sc[4];
-      convert_rows(x, q, 16 * w, lane, ss, sc);
-      if ((lane & 7) == 0)
+      bar_sync(BAR_GIVEN, GROUP + OUT_THREADS);
+      const float2 inverse = sm.inverse[n & 1];
+      const float fs = st.of_s[row] * inverse.x, fu = st.of_o[row] * inverse.y;
+      if (n + STAGES < part.chunks) bar_arrive(BAR_FREE + s, 2 * GROUP + OUT_THREADS);
+      wait(sm.bar_o, n);
+#pragma unroll 1
+      for (int c = 0; c < D; c += 8) {
+        float a[8], b[8];
+        tmem_ld8(tm + TM_QS + c, a);
+        tmem_ld8(tm + TM_PU + c, b);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          of_o[16 * w + 4 * i + (lane >> 3)] = p.scale * (p.normalize ? rsqrtf(fmaf(NORM_EPS * sc[i], sc[i], ss[i])) : 1.f / sc[i]);
-      if (n + 1 < part.chunks) fetch_rows(x, qp, p.ldq, t0 + CHUNK + 16 * w, part.len, lane);
-      bar_sync(BAR_READY_O + s, 2 * GROUP);
-      blocks_of_p(q, st);
-      float2 grow[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) grow[i] = *reinterpret_cast<const float2*>(st.grow + 8 * i + c2);
-      bar_sync(BAR_OUT, GROUP);
-      if (n + STAGES < part.chunks) bar_arrive(BAR_FREE + s, 3 * GROUP);
-      bar_sync(BAR_GIVEN, 2 * GROUP);
-      uint32_t sh[4][4], uf[4][4];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const uint4 a = sm.s16[w][ks][lane], c = sm.u16[w][ks][lane];
-        sh[ks][0] = a.x; sh[ks][1] = a.y; sh[ks][2] = a.z; sh[ks][3] = a.w;
-        uf[ks][0] = c.x; uf[ks][1] = c.y; uf[ks][2] = c.z; uf[ks][3] = c.w;
+        for (int e = 0; e < 8; ++e) a[e] = fmaf(fu, b[e], fs * a[e]);
+        if (t < part.len)
+          *reinterpret_cast<uint4*>(op + size_t(t) * p.ldo + c) =
+              make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
       }
-      const float4 scales = sm.scales[w][lane];
-      if (n + 1 < part.chunks) bar_arrive(BAR_TAKEN, 2 * GROUP);
-      // O^T = e^G S Q^T + U^T P^T
-      float o[8][4];
-#pragma unroll
-      for (int m = 0; m < 8; ++m) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[m][i] = 0.f;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t f[4];
-          ldm4(f, smem_u32(q) + m * 1024 + (lane4 ^ (half << 6)));
-          mma(o[m], sh[2 * half], f[0], f[1]);
-          mma(o[m], sh[2 * half + 1], f[2], f[3]);
-        }
-        o[m][0] *= grow[m].x * scales.x;
-        o[m][1] *= grow[m].y * scales.x;
-        o[m][2] *= grow[m].x * scales.y;
-        o[m][3] *= grow[m].y * scales.y;
-      }
-#pragma unroll
-      for (int ib = 0; ib < 4; ++ib)
-#pragma unroll
-        for (int jb = 0; jb <= ib; ++jb) {
-          uint32_t f[4];
-          ldm4(f, smem_u32(sm.p) + ib * 2048 + (across0 ^ (jb << 5)));
-          mma(o[2 * ib], uf[jb], f[0], f[1]);
-          mma(o[2 * ib + 1], uf[jb], f[2], f[3]);
-        }
-      // by way of this warp's columns of a tile, out by rows
-#pragma unroll
-      for (int n2 = 0; n2 < 4; ++n2) {
-        uint32_t f[4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float2 fo = *reinterpret_cast<const float2*>(of_o + 16 * n2 + 8 * i + c2);
-          const float(&t)[4] = o[2 * n2 + i];
-          f[2 * i] = pack_bf16x2(t[0] * (fo.x * scales.z), t[1] * (fo.y * scales.z));
-          f[2 * i + 1] = pack_bf16x2(t[2] * (fo.x * scales.w), t[3] * (fo.y * scales.w));
-        }
-        stm4t(smem_u32(sm.o) + unit_at(16 * n2 + ((lane >> 4) << 3) + (lane & 7), 2 * w + ((lane >> 3) & 1)), f[0], f[1], f[2], f[3]);
-      }
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * i + (lane >> 1), unit = 2 * w + (lane & 1);
-        if (t0 + row < part.len)
-          *(reinterpret_cast<uint4*>(op + size_t(t0 + row) * p.ldo) + unit) = *reinterpret_cast<const uint4*>(sm.o + unit_at(row, unit));
-      }
-      __syncwarp();
+      tc_fence_before_sync();
+      if (n + 1 < part.chunks) bar_arrive(BAR_TAKEN, GROUP + OUT_THREADS);
     }
+    for (int t = part.begin + part.chunks * CHUNK + row; t < p.T; t += OUT_THREADS) zero_row(op, t);
+    if (part.chunks > 0 && part.begin + (part.chunks - 1) * CHUNK + row >= part.len && part.begin + (part.chunks - 1) * CHUNK + row < p.T)
+      zero_row(op, part.begin + (part.chunks - 1) * CHUNK + row);
+  }
+  __device__ __forceinline__ void zero_row(__nv_bfloat16* op, int t) const {
+#pragma unroll 1
+    for (int u = 0; u < 8; ++u) *(reinterpret_cast<uint4*>(op + size_t(t) * p.ldo) + u) = make_uint4(0, 0, 0, 0);
   }
 };
 
 template <bool OUT>
-__global__ void __launch_bounds__(4 * GROUP, 1) delta_chunk_kernel(DeltaParams p) {
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  ChunkSmem& sm = *reinterpret_cast<ChunkSmem*>(smem_raw);
+__global__ void __launch_bounds__(3 * GROUP + (OUT ? OUT_THREADS : 0), 1) delta_chunk_kernel(DeltaParams p, unsigned int* status) {
+  extern __shared__ uint8_t smem_raw[];
+  ChunkSmem& sm = *reinterpret_cast<ChunkSmem*>(smem_raw + (1024u - (smem_u32(smem_raw) & 1023u)) % 1024u);
   const int warp = warp_index(), lane = threadIdx.x & 31, w = warp & 3;
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&sm.tmem), TM_COLUMNS);
+    tmem_relinquish();
+    if (lane == 0) {
+      mbar_init(smem_u32(&sm.bar_y), 1);
+      mbar_init(smem_u32(&sm.bar_u), 1);
+      mbar_init(smem_u32(&sm.bar_s), 1);
+      mbar_init(smem_u32(&sm.bar_o), 1);
+      mbar_init(smem_u32(&sm.bar_a[0]), 1);
+      mbar_init(smem_u32(&sm.bar_a[1]), 1);
+      sm.abort_flag = 0;
+      fence_mbar_init();
+    }
+  }
+  for (int s = 0; s < STAGES; ++s)             // T^T: what lies below the blocks of the diagonal stays 0
+    for (int i = threadIdx.x; i < 2 * TILE / 16; i += blockDim.x) reinterpret_cast<uint4*>(sm.stage[s].t_hi)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
   Part part;
   part.b = blockIdx.x / p.H;
   part.h = blockIdx.x % p.H;
@@ -867,22 +916,20 @@ __global__ void __launch_bounds__(4 * GROUP, 1) delta_chunk_kernel(DeltaParams p
   pdl_trigger();
   part.len = sequence_length(p, part.b);
   part.chunks = (part.len + CHUNK - 1) / CHUNK;
-  constexpr int TAKERS = OUT ? 2 * GROUP : GROUP;
   const size_t state = size_t(blockIdx.x) * D * D;
-  switch (warp >> 2) {
-    case 0:
-      Follow<OUT, true>{sm, w, lane}.run(part, p.s_in == nullptr ? nullptr : p.s_in + state, false, p.s_out == nullptr ? nullptr : p.s_out + state,
-                                         BAR_READY, TAKERS);
-      break;
-    case 1:
-      if (OUT) {
-        Outputs{p, sm, part, w, lane}.run();
-        for (int t = part.len + (threadIdx.x - GROUP) / 8; t < p.T; t += GROUP / 8)
-          *(reinterpret_cast<uint4*>(p.o + (size_t(part.b) * p.T + t) * p.ldo + size_t(part.h) * D) + (threadIdx.x & 7)) = make_uint4(0, 0, 0, 0);
-      }
-      break;
-    default:
-      Prepare{p, sm, part, (warp >> 2) - 2, w, lane, TAKERS}.run();
+  const Common common{p, sm, part, w, lane, sm.tmem + (uint32_t(w) << 21), status};
+  if (warp < 4) {
+    Follow<OUT>{common}.run(p.s_in == nullptr ? nullptr : p.s_in + state, p.s_out == nullptr ? nullptr : p.s_out + state);
+  } else if (warp < 12) {
+    Prepare<OUT>{common, (warp >> 2) - 1}.run();
+  } else if (OUT) {
+    Outputs{common}.run();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after_sync();
+    tmem_dealloc(sm.tmem, TM_COLUMNS);
   }
 }
 
@@ -915,11 +962,11 @@ int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream)
   p.scale = d->scale; p.normalize = d->flags & JB200_DELTA_NORMALIZE;
   if (T >= 24) {
     if (p.o != nullptr) {
-      JB_MAX_SMEM(delta_chunk_kernel<true>, sizeof(ChunkSmem));
-      launch_dep(delta_chunk_kernel<true>, B * H, 4 * GROUP, sizeof(ChunkSmem), stream, p);
+      JB_MAX_SMEM(delta_chunk_kernel<true>, CHUNK_SMEM);
+      launch_dep(delta_chunk_kernel<true>, B * H, 3 * GROUP + OUT_THREADS, CHUNK_SMEM, stream, p, device_status_ptr());
     } else {
-      JB_MAX_SMEM(delta_chunk_kernel<false>, sizeof(ChunkSmem));
-      launch_dep(delta_chunk_kernel<false>, B * H, 4 * GROUP, sizeof(ChunkSmem), stream, p);
+      JB_MAX_SMEM(delta_chunk_kernel<false>, CHUNK_SMEM);
+      launch_dep(delta_chunk_kernel<false>, B * H, 3 * GROUP, CHUNK_SMEM, stream, p, device_status_ptr());
     }
     JB_LAUNCH_CHECK("delta_chunk_kernel");
     return JB200_OK;
