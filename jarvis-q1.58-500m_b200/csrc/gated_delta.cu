@@ -142,13 +142,16 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 //   X = b (V - e^G K S^T),   U = T X with T = (I + A)^-1,  A_ij = b_i e^(G_i - G_j) k_i.k_j  (j < i)
 //   O = e^G Q S^T + P U with P_ij = e^(G_i - G_j) q_i.k_j  (j <= i),   S' = e^Gc S + (e^(Gc - G) U)^T K
 // A CTA follows one head of one sequence:
-//   warps 0-3          the state: S in tensor memory (f32, a value row and 32 keys a thread); per chunk three products, K S^T, T X and U^T K, with
+//   warps 0-3          the state: S in tensor memory (f32, a key and 32 values a thread); per chunk three products, K S^T, T X and K^T U, with
 //                      X, U and S back in shared memory as their operands between them: the chain that everything waits for
-//   warps 4-7, 8-11    by turns prepare a chunk, nothing of the state: K and Q as f16, A and T, P
+//   warps 4-7, 8-11    by turns prepare a chunk, nothing of the state: K as f16, A and T
 //   warps 12, 13       output rows from Q S^T and P U, which the state's warps issue beside their own
+//   warps 14, 15       Q as f16, P
 // The products are tcgen05.mma, 128 rows at a time: a chunk has 64, so that the operand is there twice (K twice in memory; a second reading
-// of T^T and U, MN-major) and all four of a group's warps find 64 rows x 32 columns in their lanes; for P it is [K; Q], of Q and P as operands
-// the upper half is what happens to follow, in lanes that nobody reads.  T's blocks come from mma.sync: products of 16 x 16.
+// of T^T and K, MN-major) and all four of a group's warps find 64 rows in their lanes; for P it is [K; Q], of Q and P as operands the
+// upper half is what happens to follow, in lanes that nobody reads.  Both terms of S, X and U (below) are one operand of 128 columns: the product reads its other operand
+// once for both, and what bounds these small products is reading (6 KB in 48 cycles, 8 KB in 64, for 32 and 64 of mathematics).  T's blocks come from
+// mma.sync: products of 16 x 16.
 //
 // Precision: the state is f32 and stays it.  What it is multiplied by and into is f16 in two terms, x = hi + lo (22 bits), at a power of two
 // that brings a bound of its size to 2^15, so that f16's subnormals lie 2^-39 below: |X|, |U| <= 16 max|S| + 130 max|b v| and
@@ -161,7 +164,7 @@ constexpr int CHUNK = 64;
 constexpr int TILE = CHUNK * D * 2;        // bytes of 64 rows of 128, the 16-byte units of row r at unit ^ (r & 7): the 128-byte swizzle
 constexpr int STAGES = 3;
 constexpr int GROUP = 128;                 // threads of the state's group, of a preparing one
-constexpr int OUT_THREADS = 64;
+constexpr int OUT_THREADS = 64;            // those of the output rows, of P
 constexpr float LEAST_LOG2 = -300.f;       // 2^-300 is 0 in f32: a decay of less, -inf among them, is this one
 
 struct alignas(1024) Stage {
@@ -179,39 +182,64 @@ struct Solve {                                         // of a preparing group
 };
 struct alignas(1024) ChunkSmem {
   Stage stage[STAGES];
-  uint8_t s_hi[TILE], s_lo[TILE];                      // S [value][key]
+  uint8_t s_hi[TILE], s_lo[TILE];                      // S [key][value]
   uint8_t x_hi[TILE], x_lo[TILE];                      // X, then e^(Gc - G) U, [token][value]
   uint8_t u[TILE];                                     // U, one term
   Solve solve[2];
   float most_s[2][4], most_v[2][4];                    // of every warp of the state
   float2 inverse[2];                                   // of the powers of S and of X and U
-  unsigned long long bar_y, bar_u, bar_s, bar_o, bar_a[2];
+  unsigned long long bar_y, bar_u, bar_s, bar_o, bar_a[2], bar_p, bar_k[STAGES];
   uint32_t tmem, abort_flag;
 };
 static_assert(sizeof(Stage) % 1024 == 0, "tiles lie on 1024-byte boundaries");
 constexpr size_t CHUNK_SMEM = sizeof(ChunkSmem) + 1024;
 
-// tensor memory: accumulators of 64 columns
-enum { TM_A = 0 /* + 64 group */, TM_Y = 128, TM_U = 192, TM_S = 256, TM_QS = 320, TM_PU = 384, TM_STATE = 448, TM_COLUMNS = 512 };
-// 8 columns of the thread's lane
+// tensor memory: accumulators of 64 columns; TM_CHAIN, the state's three products one after the other, has two
+enum { TM_A = 0 /* + 64 group */, TM_CHAIN = 128, TM_QS = 256, TM_PU = 320, TM_STATE = 384, TM_P = 448, TM_COLUMNS = 512 };
+// Columns of the thread's lane
+#define JB_R8(x, i) "=&r"(x[i]), "=&r"(x[i + 1]), "=&r"(x[i + 2]), "=&r"(x[i + 3]), "=&r"(x[i + 4]), "=&r"(x[i + 5]), "=&r"(x[i + 6]), "=&r"(x[i + 7])
 __device__ __forceinline__ void tmem_ld8(uint32_t at, float (&x)[8]) {
   uint32_t r[8];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+               : JB_R8(r, 0)
                : "r"(at)
                : "memory");
-  tmem_ld_wait();
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_st8(uint32_t at, const float (&x)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(__float_as_uint(x[0])), "r"(__float_as_uint(x[1])),
-               "r"(__float_as_uint(x[2])), "r"(__float_as_uint(x[3])), "r"(__float_as_uint(x[4])), "r"(__float_as_uint(x[5])),
-               "r"(__float_as_uint(x[6])), "r"(__float_as_uint(x[7]))
+// 16 from a on and 16 from b on
+__device__ __forceinline__ void tmem_ld16x2(uint32_t a, uint32_t b, float2 (&x)[8], float2 (&y)[8]) {
+  uint32_t r[16], s[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : JB_R8(r, 0), JB_R8(r, 8), JB_R8(s, 0), JB_R8(s, 8)
+      : "r"(a), "r"(b)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+    y[i] = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+  }
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t a, float2 (&x)[8]) {
+  uint32_t r[16];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+               : JB_R8(r, 0), JB_R8(r, 8)
+               : "r"(a)
+               : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const float2 (&x)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "f"(x[0].x), "f"(x[0].y),
+               "f"(x[1].x), "f"(x[1].y), "f"(x[2].x), "f"(x[2].y), "f"(x[3].x), "f"(x[3].y), "f"(x[4].x), "f"(x[4].y), "f"(x[5].x), "f"(x[5].y),
+               "f"(x[6].x), "f"(x[6].y), "f"(x[7].x), "f"(x[7].y)
                : "memory");
 }
 // The CTA's barriers.  Ready and free of a stage: the preparing group arrives and waits, the others wait and arrive.
-enum { BAR_GROUP = 1 /* + group */, BAR_STATE = 3, BAR_READY = 4 /* + stage */, BAR_FREE = 7 /* + stage */, BAR_TAKEN = 10, BAR_GIVEN = 11, BAR_PAIR = 12 /* + group */ };
+enum { BAR_GROUP = 1 /* + group */, BAR_STATE = 3, BAR_READY = 4 /* + stage */, BAR_FREE = 7 /* + stage */, BAR_TAKEN = 10, BAR_GIVEN = 11, BAR_PAIR = 12 /* + group */, BAR_SCORES = 14 };
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
@@ -267,22 +295,24 @@ __device__ __forceinline__ void power_scale(float m, float& s, float& inv) {
   s = __uint_as_float(uint32_t(254 + 14 - e) << 23);
   inv = __uint_as_float(uint32_t(e - 14) << 23);
 }
+__device__ __forceinline__ float inverse_power(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }      // of a power of two
 __device__ __forceinline__ uint32_t unit_at(int row, int unit) { return uint32_t(row * 128 + ((unit ^ (row & 7)) << 4)); }
 
 // Operands of tcgen05.mma in the 128-byte swizzle.  K-major (rows of the operand are rows of the tile): 16 elements on are +2 in the address field.
-// MN-major (its rows are the tile's columns): 16 on are 16 rows, +128; `twice`: 64 columns read as rows 0-63 and again as 64-127.
-__device__ __forceinline__ uint64_t operand(const uint8_t* tile, bool twice = false) {
-  return uint64_t((smem_u32(tile) & 0x3FFFFu) >> 4) | uint64_t(twice ? 0 : 64) << 16 | uint64_t(64) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+// MN-major (its rows are the tile's columns): 16 on are 16 rows, +128, and behind 64 columns those of the tile TWO_TILES away, or the same again.
+enum { ONE_TILE = 64, SAME_TWICE = 0, TWO_TILES = TILE >> 4 };
+__device__ __forceinline__ uint64_t operand(const uint8_t* tile, int next = ONE_TILE) {
+  return uint64_t((smem_u32(tile) & 0x3FFFFu) >> 4) | uint64_t(next) << 16 | uint64_t(64) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
 }
-constexpr uint32_t idesc(int a_mn, int b_mn) {         // f16 operands, f32 sums, 128 x 64
-  return (1u << 4) | uint32_t(a_mn) << 15 | uint32_t(b_mn) << 16 | uint32_t(64 >> 3) << 17 | uint32_t(128 >> 4) << 24;
+constexpr uint32_t idesc(int n, int a_mn, int b_mn) {  // f16 operands, f32 sums, 128 x n
+  return (1u << 4) | uint32_t(a_mn) << 15 | uint32_t(b_mn) << 16 | uint32_t(n >> 3) << 17 | uint32_t(128 >> 4) << 24;
 }
 // By a whole warp, one lane of it issuing
-template <int A_MN, int B_MN>
+template <int N, int A_MN, int B_MN>
 __device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, bool add) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (elect_one()) umma_bf16_ss(d, a + uint64_t(i * (A_MN ? 128 : 2)), b + uint64_t(i * (B_MN ? 128 : 2)), idesc(A_MN, B_MN), add || i != 0);
+    if (elect_one()) umma_bf16_ss(d, a + uint64_t(i * (A_MN ? 128 : 2)), b + uint64_t(i * (B_MN ? 128 : 2)), idesc(N, A_MN, B_MN), add || i != 0);
 }
 __device__ __forceinline__ void commit(unsigned long long& bar) {
   if (elect_one()) umma_commit(smem_u32(&bar));
@@ -351,6 +381,19 @@ struct Common {
     if (!mbar_try_wait(smem_u32(&bar), uint32_t(n) & 1u)) wait_on(smem_u32(&bar), uint32_t(n) & 1u, &sm.abort_flag, status);
     tc_fence_after_sync();
   }
+  // Eight columns of this thread's row of a product with K^T, c and the row's place in the chunk apart, times f r_j e^(G_i - G_j); g: G_i in two terms
+  __device__ __forceinline__ void decayed(uint32_t columns, const Stage& st, int c, float2 g, float f, float (&x)[8]) const {
+    tmem_ld8(tm + columns + c, x);
+    const float4* col = reinterpret_cast<const float4*>(st.column + c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float4 at = col[e];
+      const float2 d = add2(add2(both(g.x), make_float2(at.x, at.z)), add2(both(g.y), make_float2(at.y, at.w)));
+      const float2 v = mul2(mul2(make_float2(x[2 * e], x[2 * e + 1]), both(f)), make_float2(exp2_fast(d.x), exp2_fast(d.y)));
+      x[2 * e] = v.x;
+      x[2 * e + 1] = v.y;
+    }
+  }
   static __device__ __noinline__ void wait_on(uint32_t bar, uint32_t parity, uint32_t* abort_flag, unsigned int* status) {
     (void)mbar_wait(bar, parity, abort_flag, status, JB200_STATUS_ATTN_MMA);
   }
@@ -391,20 +434,6 @@ struct Prepare : Common {
     return x;
   }
 
-  // Eight columns from c on of this thread's row of a product with K^T, times f r_j e^(G_i - G_j); g: G_i in two terms
-  __device__ __forceinline__ void decayed(const Stage& st, int c, float2 g, float f, float (&x)[8]) const {
-    tmem_ld8(tm + TM_A + 64 * group + c, x);
-    const float4* col = reinterpret_cast<const float4*>(st.column + c);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float4 at = col[e];
-      const float2 d = add2(add2(both(g.x), make_float2(at.x, at.z)), add2(both(g.y), make_float2(at.y, at.w)));
-      const float2 v = mul2(mul2(make_float2(x[2 * e], x[2 * e + 1]), both(f)), make_float2(exp2_fast(d.x), exp2_fast(d.y)));
-      x[2 * e] = v.x;
-      x[2 * e + 1] = v.y;
-    }
-  }
-
   // Rows of -A: K K^T is there for two warps a row, which take half of its columns below the diagonal each
   __device__ __forceinline__ void rows_of_a(const Stage& st, Solve& so) const {
     const int i = 32 * (w & 1) + lane, ib = i >> 4, row = i & 15, units = 2 + 2 * (w & 1);
@@ -413,7 +442,7 @@ struct Prepare : Common {
 #pragma unroll 1
     for (int c = (w >> 1) * units * 8, end = c + units * 8; c < end; c += 8) {
       float x[8];
-      decayed(st, c, g, f, x);
+      decayed(TM_A + 64 * group, st, c, g, f, x);
       const int jb = c >> 4, unit = (c >> 3) & 1;
       if (jb < ib) {
         uint32_t hi[4], lo[4];
@@ -427,23 +456,6 @@ struct Prepare : Common {
         *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
         *reinterpret_cast<float4*>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
       }
-    }
-  }
-
-  // Rows of P: a row a thread of warps 2, 3
-  __device__ __forceinline__ void rows_of_p(Stage& st) const {
-    const int i = 32 * (w - 2) + lane, reach = 32 * (w - 1);
-    const float2 g = st.g[i];
-#pragma unroll 1
-    for (int c = 0; c < 64; c += 8) {
-      uint32_t v[4] = {};
-      if (c < reach) {
-        float x[8];
-        decayed(st, c, g, 1.f, x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = pack_f16x2(c + 2 * e <= i ? x[2 * e] : 0.f, c + 2 * e + 1 <= i ? x[2 * e + 1] : 0.f);
-      }
-      *reinterpret_cast<uint4*>(st.p + unit_at(i, c >> 3)) = make_uint4(v[0], v[1], v[2], v[3]);
     }
   }
 
@@ -574,15 +586,13 @@ struct Prepare : Common {
   __device__ __forceinline__ void run() const {
     const size_t first = size_t(part.b) * p.T;
     const __nv_bfloat16* kp = p.k + first * p.ldk + size_t(part.h / p.per_key) * D;
-    const __nv_bfloat16* qp = p.q + first * p.ldq + size_t(part.h / p.per_key) * D;
     Solve& so = sm.solve[group];
     const int row = 16 * w + (lane >> 1), half = lane & 1;
-    uint4 k[4], q[4];
+    uint4 k[4];
     float g0 = 0.f, g1 = 0.f, b0 = 0.f, b1 = 0.f;
     auto fetch = [&](int t0) {
       const int at = t0 + row;
       fetch_half(k, kp + size_t(at) * p.ldk + 32 * half, at < part.len);
-      if (OUT) fetch_half(q, qp + size_t(at) * p.ldq + 32 * half, at < part.len);
       if (w == 3) {
         const int t = t0 + 2 * lane;
         g0 = t < part.len ? load_now(p.log_decay + (first + t) * p.ldg + part.h) : 0.f;
@@ -594,7 +604,7 @@ struct Prepare : Common {
     Gates x = {};
     if (group < part.chunks) fetch(part.begin + group * CHUNK);
     if (w == 3) x = gates(g0, g1);
-    for (int n = group, uses = 0; n < part.chunks; n += 2) {
+    for (int n = group; n < part.chunks; n += 2) {
       const int s = n % STAGES, t0 = part.begin + n * CHUNK;
       Stage& st = sm.stage[s];
       if (n >= STAGES) bar_sync(BAR_FREE + s, 2 * GROUP + (OUT ? OUT_THREADS : 0));
@@ -605,43 +615,22 @@ struct Prepare : Common {
         *reinterpret_cast<float4*>(&st.g[2 * lane]) = make_float4(x.hi.x, x.lo.x, x.hi.y, x.lo.y);
         if (lane == 0) st.whole = x.whole;
       }
-#pragma unroll 1
-      for (int m = 0; m < (OUT ? 2 : 1); ++m) {  // K twice, Q
-        float sc;
-        const float ss = convert_half(k, m == 0 ? st.k_again : st.q, m == 0, row, half, sc);
-        if (half == 0) {
-          // k = n (k16 r) with |k16 r| = 1, or of the normalised key n = 1 and k16 r its value
-          const float r = p.normalize ? rsqrtf(fmaf(NORM_EPS * sc, sc, ss)) : ss > 0.f ? rsqrtf(ss) : 0.f;
-          if (m == 0) {
-            st.rk[row] = r;
-            st.nk[row] = p.normalize ? 1.f : ss * r / sc;
-          } else {
-            st.of_o[row] = p.scale * (p.normalize ? r : 1.f / sc);
-          }
-        }
-        if (OUT && m == 0) {
-          settle();
-          bar_sync(BAR_GROUP + group, GROUP);
-          if (w == 0) {
-            tc_fence_after_sync();
-            product<0, 0>(sm.tmem + TM_A + 64 * group, operand(st.k_again), operand(st.k), false);
-            commit(sm.bar_a[group]);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) k[i] = q[i];
-        }
-      }
-      if (!OUT) {
-        settle();
-        bar_sync(BAR_GROUP + group, GROUP);
-        if (w == 0) {
-          tc_fence_after_sync();
-          product<0, 0>(sm.tmem + TM_A + 64 * group, operand(st.k_again), operand(st.k), false);
-          commit(sm.bar_a[group]);
-        }
+      float sc;
+      const float ss = convert_half(k, st.k_again, true, row, half, sc);
+      if (half == 0) {
+        // k = n (k16 r) with |k16 r| = 1, or of the normalised key n = 1 and k16 r its value
+        const float r = p.normalize ? rsqrtf(fmaf(NORM_EPS * sc, sc, ss)) : ss > 0.f ? rsqrtf(ss) : 0.f;
+        st.rk[row] = r;
+        st.nk[row] = p.normalize ? 1.f : ss * r * inverse_power(sc);
       }
       if (n + 2 < part.chunks) fetch(t0 + 2 * CHUNK);
-      if (w >= 2) {                              // b v - b e^G r K S^T, its share of U^T K
+      settle();
+      bar_sync(BAR_GROUP + group, GROUP);
+      if (w == 0) {
+        tc_fence_after_sync();
+        product<64, 0, 0>(sm.tmem + TM_A + 64 * group, operand(st.k_again), operand(st.k), false);
+        commit(sm.bar_a[group]);
+      } else if (w >= 2) {                       // b v - b e^G r K S^T, its share of K^T U
         const int i = 32 * (w - 2) + lane;
         const float r = st.rk[i], n1 = st.nk[i], beta = st.beta[i];
         const float2 g = st.g[i];
@@ -650,32 +639,68 @@ struct Prepare : Common {
         st.of_y[i] = beta * n1 * n1 * st.of_s[i] * r;
         st.of_u[i] *= r;
       }
-      settle();
       bar_sync(BAR_GROUP + group, GROUP);
-      wait(sm.bar_a[group], uses++);
+      if (OUT && lane == 0) mbar_arrive(smem_u32(&sm.bar_k[s]));
+      wait(sm.bar_a[group], n >> 1);
       rows_of_a(st, so);
-      settle();
       bar_sync(BAR_GROUP + group, GROUP);
-      if (OUT && w == 2) {
-        tc_fence_after_sync();
-        product<0, 0>(sm.tmem + TM_A + 64 * group, operand(st.k), operand(st.k), false);
-        commit(sm.bar_a[group]);
-      }
       diagonal(st, so);
       bar_sync(BAR_GROUP + group, GROUP);
-      if (w < 2) {
-        off_diagonal(st, so);
-        if (OUT) ++uses;
-      } else {
-        if (OUT) {
-          st.of_s[32 * (w - 2) + lane] *= st.of_o[32 * (w - 2) + lane];
-          wait(sm.bar_a[group], uses++);
-          rows_of_p(st);
+      if (w < 2) off_diagonal(st, so);
+      if (w == 3) x = gates(g0, g1);
+      settle();
+      bar_arrive(BAR_READY + s, 2 * GROUP + (OUT ? OUT_THREADS : 0));
+    }
+  }
+};
+
+// ---- Q and P: two warps --------------------------------------------------------------------------------------------------
+struct Scores : Common {
+  __device__ __forceinline__ void run() const {
+    const __nv_bfloat16* qp = p.q + size_t(part.b) * p.T * p.ldq + size_t(part.h / p.per_key) * D;
+    const int i = 32 * (w - 2) + lane, row = i >> 1, half = i & 1, reach = 32 * (w - 1);
+    uint4 q[2][4];
+    auto fetch = [&](int t0) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m) fetch_half(q[m], qp + size_t(t0 + 32 * m + row) * p.ldq + 32 * half, t0 + 32 * m + row < part.len);
+    };
+    if (part.chunks > 0) fetch(part.begin);
+    for (int n = 0; n < part.chunks; ++n) {
+      const int s = n % STAGES;
+      Stage& st = sm.stage[s];
+      wait(sm.bar_k[s], n / STAGES);             // the stage is free, K is there
+#pragma unroll 1
+      for (int m = 0; m < 2; ++m) {
+        float sc;
+        const float ss = convert_half(q[0], st.q, false, 32 * m + row, half, sc);
+        if (half == 0) st.of_o[32 * m + row] = p.scale * (p.normalize ? rsqrtf(fmaf(NORM_EPS * sc, sc, ss)) : inverse_power(sc));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[0][e] = q[1][e];
+      }
+      if (n + 1 < part.chunks) fetch(part.begin + (n + 1) * CHUNK);
+      settle();
+      bar_sync(BAR_SCORES, OUT_THREADS);
+      if (w == 2) {
+        tc_fence_after_sync();
+        product<64, 0, 0>(sm.tmem + TM_P, operand(st.k), operand(st.k), false);
+        commit(sm.bar_p);
+      }
+      st.of_s[i] *= st.of_o[i];
+      const float2 g = st.g[i];
+      wait(sm.bar_p, n);
+#pragma unroll 1
+      for (int c = 0; c < 64; c += 8) {
+        uint32_t v[4] = {};
+        if (c < reach) {
+          float x[8];
+          decayed(TM_P, st, c, g, 1.f, x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = pack_f16x2(c + 2 * e <= i ? x[2 * e] : 0.f, c + 2 * e + 1 <= i ? x[2 * e + 1] : 0.f);
         }
-        if (w == 3) x = gates(g0, g1);
+        *reinterpret_cast<uint4*>(st.p + unit_at(i, c >> 3)) = make_uint4(v[0], v[1], v[2], v[3]);
       }
       settle();
-      bar_arrive(BAR_READY + s, 2 * GROUP);
+      bar_arrive(BAR_READY + s, 2 * GROUP + OUT_THREADS);
     }
   }
 };
@@ -683,13 +708,17 @@ struct Prepare : Common {
 // ---- the group of the state ------------------------------------------------------------------------------------------
 template <bool OUT>
 struct Follow : Common {
-  // Eight values of a row in two terms
-  __device__ __forceinline__ static void put(const float2 (&x)[4], float f, uint8_t* hi_tile, uint8_t* lo_tile, uint32_t at) {
-    uint32_t hi[4], lo[4];
+  // 16 values of a row in two terms, from unit `unit` on
+  __device__ __forceinline__ static void put(const float2 (&x)[8], uint8_t* hi_tile, uint8_t* lo_tile, int row, int unit) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) split(mul2(x[e], both(f)), hi[e], lo[e]);
-    *reinterpret_cast<uint4*>(hi_tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4*>(lo_tile + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    for (int u = 0; u < 2; ++u) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split(x[4 * u + e], hi[e], lo[e]);
+      const uint32_t at = unit_at(row, unit + u);
+      *reinterpret_cast<uint4*>(hi_tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(lo_tile + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
   }
   __device__ __forceinline__ static float most(const float (&m)[4]) { return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])); }
   __device__ __forceinline__ static float warp_most(float m) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))); }
@@ -697,25 +726,24 @@ struct Follow : Common {
   // The loops over a thread's 32 columns stay loops: the roles of this kernel share the instruction caches, and unrolled (77 KB in all) every one of
   // them waited for its instructions (a chunk took 9600 cycles on 128 SMs).
   __device__ __forceinline__ void run(const float* from, float* to) const {
-    const int row = 32 * (w & 1) + lane, half = w >> 1;          // a value (S) or a token (X, U), and which 32 keys or values of it
-    const uint32_t cols = tm + 32 * half;
+    const int row = 32 * (w & 1) + lane, half = w >> 1;          // a key (S) or a token (X, U), and which 32 values of it
+    const uint32_t cols = tm + TM_CHAIN + 32 * half, state = tm + TM_STATE + 32 * half;
     const __nv_bfloat16* vp = p.v + size_t(part.b) * p.T * p.ldv + size_t(part.h) * D + 32 * half;
     uint4 v[4];
     if (part.chunks > 0) fetch_half(v, vp + size_t(part.begin + row) * p.ldv, part.begin + row < part.len);
-    // the state before the first chunk is the product of none: TM_S
+    // the state before the first chunk is added to none as if it were a product
     float m = 0.f;
 #pragma unroll 1
-    for (int c = 0; c < 32; c += 8) {
-      float x[8] = {};
-      tmem_st8(cols + TM_STATE + c, x);
-      if (from != nullptr) {
-        const float4* at = reinterpret_cast<const float4*>(from + row * D + 32 * half + c);
-        const float4 a = at[0], b = at[1];
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-      }
-      tmem_st8(cols + TM_S + c, x);
+    for (int c = 0; c < 32; c += 16) {
+      float2 x[8] = {};
+      tmem_st16(state + c, x);
+      tmem_st16(cols + 64 + c, x);
+      if (from != nullptr)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
+        for (int e = 0; e < 8; ++e) x[e] = make_float2(from[(32 * half + c + 2 * e) * D + row], from[(32 * half + c + 2 * e + 1) * D + row]);
+      tmem_st16(cols + c, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, fmaxf(fabsf(x[e].x), fabsf(x[e].y)));
     }
     tmem_st_wait();
     m = warp_most(m);
@@ -727,26 +755,24 @@ struct Follow : Common {
       power_scale(bound, ps, is);
       m = 0.f;
 #pragma unroll 1
-      for (int c = 0; c < 32; c += 8) {
-        float x[8], y[8];
-        tmem_ld8(cols + TM_STATE + c, x);
-        tmem_ld8(cols + TM_S + c, y);
-        float2 z[4];
+      for (int c = 0; c < 32; c += 16) {
+        float2 x[8], y[8], z[8];
+        tmem_ld16x2(cols + c, cols + 64 + c, x, y);
+        tmem_ld16(state + c, z);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          z[e] = fma2(make_float2(y[2 * e], y[2 * e + 1]), both(ix), mul2(make_float2(x[2 * e], x[2 * e + 1]), both(whole)));
+        for (int e = 0; e < 8; ++e) {
+          z[e] = fma2(add2(x[e], y[e]), both(ix), mul2(z[e], both(whole)));
           m = fmaxf(m, fmaxf(fabsf(z[e].x), fabsf(z[e].y)));
-          x[2 * e] = z[e].x;
-          x[2 * e + 1] = z[e].y;
+          x[e] = mul2(z[e], both(ps));
         }
-        tmem_st8(cols + TM_STATE + c, x);
-        put(z, ps, sm.s_hi, sm.s_lo, unit_at(row, 4 * half + (c >> 3)));
+        tmem_st16(state + c, z);
+        put(x, sm.s_hi, sm.s_lo, row, 4 * half + (c >> 3));
       }
       tmem_st_wait();
       if (n == part.chunks) break;
       const int s = n % STAGES;
       Stage& st = sm.stage[s];
-      bar_sync(BAR_READY + s, 2 * GROUP);
+      bar_sync(BAR_READY + s, 2 * GROUP + (OUT ? OUT_THREADS : 0));
       m = warp_most(m);
       uint32_t m2 = 0;
 #pragma unroll
@@ -764,10 +790,10 @@ struct Follow : Common {
       else bar_sync(BAR_STATE, GROUP);
       if (w == 0) {
         tc_fence_after_sync();
-        product<0, 0>(sm.tmem + TM_Y, operand(st.k_again), operand(sm.s_hi), false);
-        product<0, 0>(sm.tmem + TM_Y, operand(st.k_again), operand(sm.s_lo), true);
+        product<128, 0, 1>(sm.tmem + TM_CHAIN, operand(st.k_again), operand(sm.s_hi, TWO_TILES), false);
         commit(sm.bar_y);
-        if (OUT) product<0, 0>(sm.tmem + TM_QS, operand(st.q), operand(sm.s_hi), false);
+        if (OUT) product<64, 0, 1>(sm.tmem + TM_QS, operand(st.q), operand(sm.s_hi), false);
+        __syncwarp();
       }
       const float ms = most(sm.most_s[n & 1]), mb = most(sm.most_v[n & 1]);
       power_scale(fmaxf(fmaf(16.f, ms, 130.f * mb), bound * 7.8886091e-31f), px, ix);      // 2^-100: the powers' quotient stays in range
@@ -778,28 +804,23 @@ struct Follow : Common {
       wait(sm.bar_y, n);
       if (n > 0 && n - 1 + STAGES < part.chunks) bar_arrive(BAR_FREE + (n - 1) % STAGES, 2 * GROUP + (OUT ? OUT_THREADS : 0));
 #pragma unroll 1
-      for (int c = 0; c < 32; c += 8) {
-        float x[8];
-        tmem_ld8(cols + TM_Y + c, x);
-        const uint32_t in[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
-        v[0] = v[1];
-        v[1] = v[2];
-        v[2] = v[3];
-        uint32_t hi[4], lo[4];
+      for (int c = 0; c < 32; c += 16) {
+        float2 x[8], y[8];
+        tmem_ld16x2(cols + c, cols + 64 + c, x, y);
+        const uint32_t in[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+        v[0] = v[2];
+        v[1] = v[3];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          split(fma2(make_float2(x[2 * e], x[2 * e + 1]), both(-fy), mul2(make_float2(bf16_lo(in[e]), bf16_hi(in[e])), both(fx))), hi[e], lo[e]);
-        const uint32_t at = unit_at(row, 4 * half + (c >> 3));
-        *reinterpret_cast<uint4*>(sm.x_hi + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(sm.x_lo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        for (int e = 0; e < 8; ++e)
+          x[e] = fma2(add2(x[e], y[e]), both(-fy), mul2(make_float2(bf16_lo(in[e]), bf16_hi(in[e])), both(fx)));
+        put(x, sm.x_hi, sm.x_lo, row, 4 * half + (c >> 3));
       }
       settle();
       bar_sync(BAR_STATE, GROUP);
       if (w == 0) {
         tc_fence_after_sync();
-        product<1, 1>(sm.tmem + TM_U, operand(st.t_hi, true), operand(sm.x_hi), false);
-        product<1, 1>(sm.tmem + TM_U, operand(st.t_hi, true), operand(sm.x_lo), true);
-        product<1, 1>(sm.tmem + TM_U, operand(st.t_lo, true), operand(sm.x_hi), true);
+        product<128, 1, 1>(sm.tmem + TM_CHAIN, operand(st.t_hi, SAME_TWICE), operand(sm.x_hi, TWO_TILES), false);
+        product<64, 1, 1>(sm.tmem + TM_CHAIN, operand(st.t_lo, SAME_TWICE), operand(sm.x_hi), true);
         commit(sm.bar_u);
       }
       if (n + 1 < part.chunks) {
@@ -808,26 +829,31 @@ struct Follow : Common {
       }
       wait(sm.bar_u, n);
 #pragma unroll 1
-      for (int c = 0; c < 32; c += 8) {
-        float x[8];
-        tmem_ld8(cols + TM_U + c, x);
-        const uint32_t at = unit_at(row, 4 * half + (c >> 3));
-        if (OUT)
-          *reinterpret_cast<uint4*>(sm.u + at) =
-              make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
-        const float2 z[4] = {make_float2(x[0], x[1]), make_float2(x[2], x[3]), make_float2(x[4], x[5]), make_float2(x[6], x[7])};
-        put(z, fu, sm.x_hi, sm.x_lo, at);
+      for (int c = 0; c < 32; c += 16) {
+        float2 x[8], y[8];
+        tmem_ld16x2(cols + c, cols + 64 + c, x, y);
+        uint32_t one[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = add2(x[e], y[e]);
+          one[e] = pack_f16x2(x[e].x, x[e].y);
+          x[e] = mul2(x[e], both(fu));
+        }
+        if (OUT) {
+          *reinterpret_cast<uint4*>(sm.u + unit_at(row, 4 * half + (c >> 3))) = make_uint4(one[0], one[1], one[2], one[3]);
+          *reinterpret_cast<uint4*>(sm.u + unit_at(row, 4 * half + (c >> 3) + 1)) = make_uint4(one[4], one[5], one[6], one[7]);
+        }
+        put(x, sm.x_hi, sm.x_lo, row, 4 * half + (c >> 3));
       }
       settle();
       bar_sync(BAR_STATE, GROUP);
       if (OUT) bar_arrive(BAR_GIVEN, GROUP + OUT_THREADS);
       if (w == 0) {
         tc_fence_after_sync();
-        product<1, 1>(sm.tmem + TM_S, operand(sm.x_hi, true), operand(st.k), false);
-        product<1, 1>(sm.tmem + TM_S, operand(sm.x_lo, true), operand(st.k), true);
+        product<128, 1, 1>(sm.tmem + TM_CHAIN, operand(st.k, SAME_TWICE), operand(sm.x_hi, TWO_TILES), false);
         commit(sm.bar_s);
         if (OUT) {
-          product<0, 1>(sm.tmem + TM_PU, operand(st.p), operand(sm.u), false);
+          product<64, 0, 1>(sm.tmem + TM_PU, operand(st.p), operand(sm.u), false);
           commit(sm.bar_o);
         }
       }
@@ -835,12 +861,14 @@ struct Follow : Common {
     }
     if (to != nullptr) {
 #pragma unroll 1
-      for (int c = 0; c < 32; c += 8) {
-        float x[8];
-        tmem_ld8(cols + TM_STATE + c, x);
-        float4* at = reinterpret_cast<float4*>(to + row * D + 32 * half + c);
-        at[0] = make_float4(x[0], x[1], x[2], x[3]);
-        at[1] = make_float4(x[4], x[5], x[6], x[7]);
+      for (int c = 0; c < 32; c += 16) {
+        float2 x[8];
+        tmem_ld16(state + c, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          to[(32 * half + c + 2 * e) * D + row] = x[e].x;
+          to[(32 * half + c + 2 * e + 1) * D + row] = x[e].y;
+        }
       }
     }
   }
@@ -860,15 +888,20 @@ struct Outputs : Common {
       if (n + STAGES < part.chunks) bar_arrive(BAR_FREE + s, 2 * GROUP + OUT_THREADS);
       wait(sm.bar_o, n);
 #pragma unroll 1
-      for (int c = 0; c < D; c += 8) {
-        float a[8], b[8];
-        tmem_ld8(tm + TM_QS + c, a);
-        tmem_ld8(tm + TM_PU + c, b);
+      for (int c = 0; c < D; c += 16) {
+        float2 a[8], b[8];
+        tmem_ld16x2(tm + TM_QS + c, tm + TM_PU + c, a, b);
+        uint32_t x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[e] = fmaf(fu, b[e], fs * a[e]);
-        if (t < part.len)
-          *reinterpret_cast<uint4*>(op + size_t(t) * p.ldo + c) =
-              make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
+        for (int e = 0; e < 8; ++e) {
+          a[e] = fma2(b[e], both(fu), mul2(a[e], both(fs)));
+          x[e] = pack_bf16x2(a[e].x, a[e].y);
+        }
+        if (t < part.len) {
+          uint4* to = reinterpret_cast<uint4*>(op + size_t(t) * p.ldo + c);
+          to[0] = make_uint4(x[0], x[1], x[2], x[3]);
+          to[1] = make_uint4(x[4], x[5], x[6], x[7]);
+        }
       }
       tc_fence_before_sync();
       if (n + 1 < part.chunks) bar_arrive(BAR_TAKEN, GROUP + OUT_THREADS);
@@ -884,7 +917,7 @@ struct Outputs : Common {
 };
 
 template <bool OUT>
-__global__ void __launch_bounds__(3 * GROUP + (OUT ? OUT_THREADS : 0), 1) delta_chunk_kernel(DeltaParams p, unsigned int* status) {
+__global__ void __launch_bounds__(3 * GROUP + (OUT ? 2 * OUT_THREADS : 0), 1) delta_chunk_kernel(DeltaParams p, unsigned int* status) {
   extern __shared__ uint8_t smem_raw[];
   ChunkSmem& sm = *reinterpret_cast<ChunkSmem*>(smem_raw + (1024u - (smem_u32(smem_raw) & 1023u)) % 1024u);
   const int warp = warp_index(), lane = threadIdx.x & 31, w = warp & 3;
@@ -898,6 +931,8 @@ __global__ void __launch_bounds__(3 * GROUP + (OUT ? OUT_THREADS : 0), 1) delta_
       mbar_init(smem_u32(&sm.bar_o), 1);
       mbar_init(smem_u32(&sm.bar_a[0]), 1);
       mbar_init(smem_u32(&sm.bar_a[1]), 1);
+      mbar_init(smem_u32(&sm.bar_p), 1);
+      for (int s = 0; s < STAGES; ++s) mbar_init(smem_u32(&sm.bar_k[s]), GROUP / 32);
       sm.abort_flag = 0;
       fence_mbar_init();
     }
@@ -923,7 +958,8 @@ __global__ void __launch_bounds__(3 * GROUP + (OUT ? OUT_THREADS : 0), 1) delta_
   } else if (warp < 12) {
     Prepare<OUT>{common, (warp >> 2) - 1}.run();
   } else if (OUT) {
-    Outputs{common}.run();
+    if (warp < 14) Outputs{common}.run();
+    else Scores{common}.run();
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -963,7 +999,7 @@ int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream)
   if (T >= 24) {
     if (p.o != nullptr) {
       JB_MAX_SMEM(delta_chunk_kernel<true>, CHUNK_SMEM);
-      launch_dep(delta_chunk_kernel<true>, B * H, 3 * GROUP + OUT_THREADS, CHUNK_SMEM, stream, p, device_status_ptr());
+      launch_dep(delta_chunk_kernel<true>, B * H, 3 * GROUP + 2 * OUT_THREADS, CHUNK_SMEM, stream, p, device_status_ptr());
     } else {
       JB_MAX_SMEM(delta_chunk_kernel<false>, CHUNK_SMEM);
       launch_dep(delta_chunk_kernel<false>, B * H, 3 * GROUP, CHUNK_SMEM, stream, p, device_status_ptr());
