@@ -145,8 +145,8 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 //   warps 0-3          the state: S in tensor memory (f32, a key and 32 values a thread); per chunk three products, K S^T, T X and K^T U, with
 //                      X, U and S back in shared memory as their operands between them: the chain that everything waits for
 //   warps 4-7, 8-11    by turns prepare a chunk, nothing of the state: K as f16, A and T
-//   warps 12, 13       output rows from Q S^T and P U, which the state's warps issue beside their own
-//   warps 14, 15       Q as f16, P
+//   warps 12, 13       Q as f16; output rows from Q S^T and P U, which the state's warps issue beside their own
+//   warps 14, 15       P
 // The products are tcgen05.mma, 128 rows at a time: a chunk has 64, so that the operand is there twice (K twice in memory; a second reading
 // of T^T and K, MN-major) and all four of a group's warps find 64 rows in their lanes; for P it is [K; Q], of Q and P as operands the
 // upper half is what happens to follow, in lanes that nobody reads.  Both terms of S, X and U (below) are one operand of 128 columns: the product reads its other operand
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 constexpr int CHUNK = 64;
 constexpr int TILE = CHUNK * D * 2;        // bytes of 64 rows of 128, the 16-byte units of row r at unit ^ (r & 7): the 128-byte swizzle
 constexpr int STAGES = 3;
-constexpr int GROUP = 128;                 // threads of the state's group, of a preparing one
+constexpr int STATE = 128, GROUP = 128;    // threads of the state's group, of a preparing one
 constexpr int OUT_THREADS = 64;            // those of the output rows, of P
 constexpr float LEAST_LOG2 = -300.f;       // 2^-300 is 0 in f32: a decay of less, -inf among them, is this one
 
@@ -307,12 +307,29 @@ __device__ __forceinline__ uint64_t operand(const uint8_t* tile, int next = ONE_
 constexpr uint32_t idesc(int n, int a_mn, int b_mn) {  // f16 operands, f32 sums, 128 x n
   return (1u << 4) | uint32_t(a_mn) << 15 | uint32_t(b_mn) << 16 | uint32_t(n >> 3) << 17 | uint32_t(128 >> 4) << 24;
 }
-// By a whole warp, one lane of it issuing
+// By a whole warp, one lane of it issuing: 64 long
 template <int N, int A_MN, int B_MN>
 __device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, bool add) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (elect_one()) umma_bf16_ss(d, a + uint64_t(i * (A_MN ? 128 : 2)), b + uint64_t(i * (B_MN ? 128 : 2)), idesc(N, A_MN, B_MN), add || i != 0);
+  asm volatile(
+      "{\n\t"
+      ".reg .pred one, more, all;\n\t"
+      ".reg .b64 a, b;\n\t"
+      "elect.sync _|one, 0xffffffff;\n\t"
+      "setp.ne.b32 more, %4, 0;\n\t"
+      "setp.eq.b32 all, 0, 0;\n\t"
+      "@one tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, more;\n\t"
+      "add.u64 a, %1, %5;\n\t"
+      "add.u64 b, %2, %6;\n\t"
+      "@one tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, all;\n\t"
+      "add.u64 a, a, %5;\n\t"
+      "add.u64 b, b, %6;\n\t"
+      "@one tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, all;\n\t"
+      "add.u64 a, a, %5;\n\t"
+      "add.u64 b, b, %6;\n\t"
+      "@one tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, all;\n\t"
+      "}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc(N, A_MN, B_MN)), "r"(add ? 1 : 0), "n"(A_MN ? 128 : 2), "n"(B_MN ? 128 : 2)
+      : "memory");
 }
 __device__ __forceinline__ void commit(unsigned long long& bar) {
   if (elect_one()) umma_commit(smem_u32(&bar));
@@ -601,13 +618,13 @@ struct Prepare : Common {
         b1 = t + 1 < part.len ? load_now(p.beta + (first + t + 1) * p.ldg + part.h) : 0.f;
       }
     };
-    Gates x = {};
     if (group < part.chunks) fetch(part.begin + group * CHUNK);
-    if (w == 3) x = gates(g0, g1);
     for (int n = group; n < part.chunks; n += 2) {
       const int s = n % STAGES, t0 = part.begin + n * CHUNK;
       Stage& st = sm.stage[s];
-      if (n >= STAGES) bar_sync(BAR_FREE + s, 2 * GROUP + (OUT ? OUT_THREADS : 0));
+      Gates x;
+      if (w == 3) x = gates(g0, g1);
+      if (n >= STAGES) bar_sync(BAR_FREE + s, GROUP + STATE + (OUT ? OUT_THREADS : 0));
       if (w == 3) {
         *reinterpret_cast<float2*>(st.beta + 2 * lane) = make_float2(b0, b1);
         *reinterpret_cast<float2*>(st.of_s + 2 * lane) = x.grow;
@@ -647,39 +664,21 @@ struct Prepare : Common {
       diagonal(st, so);
       bar_sync(BAR_GROUP + group, GROUP);
       if (w < 2) off_diagonal(st, so);
-      if (w == 3) x = gates(g0, g1);
       settle();
-      bar_arrive(BAR_READY + s, 2 * GROUP + (OUT ? OUT_THREADS : 0));
+      bar_arrive(BAR_READY + s, GROUP + STATE + (OUT ? OUT_THREADS : 0));
     }
   }
 };
 
-// ---- Q and P: two warps --------------------------------------------------------------------------------------------------
+// ---- P: a row a thread of two warps ----------------------------------------------------------------------------------------
 struct Scores : Common {
   __device__ __forceinline__ void run() const {
-    const __nv_bfloat16* qp = p.q + size_t(part.b) * p.T * p.ldq + size_t(part.h / p.per_key) * D;
-    const int i = 32 * (w - 2) + lane, row = i >> 1, half = i & 1, reach = 32 * (w - 1);
-    uint4 q[2][4];
-    auto fetch = [&](int t0) {
-#pragma unroll
-      for (int m = 0; m < 2; ++m) fetch_half(q[m], qp + size_t(t0 + 32 * m + row) * p.ldq + 32 * half, t0 + 32 * m + row < part.len);
-    };
-    if (part.chunks > 0) fetch(part.begin);
+    const int i = 32 * (w - 2) + lane, reach = 32 * (w - 1);
+#pragma unroll 1
     for (int n = 0; n < part.chunks; ++n) {
       const int s = n % STAGES;
       Stage& st = sm.stage[s];
-      wait(sm.bar_k[s], n / STAGES);             // the stage is free, K is there
-#pragma unroll 1
-      for (int m = 0; m < 2; ++m) {
-        float sc;
-        const float ss = convert_half(q[0], st.q, false, 32 * m + row, half, sc);
-        if (half == 0) st.of_o[32 * m + row] = p.scale * (p.normalize ? rsqrtf(fmaf(NORM_EPS * sc, sc, ss)) : inverse_power(sc));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[0][e] = q[1][e];
-      }
-      if (n + 1 < part.chunks) fetch(part.begin + (n + 1) * CHUNK);
-      settle();
-      bar_sync(BAR_SCORES, OUT_THREADS);
+      bar_sync(BAR_SCORES, 2 * OUT_THREADS);     // Q is there, K before it
       if (w == 2) {
         tc_fence_after_sync();
         product<64, 0, 0>(sm.tmem + TM_P, operand(st.k), operand(st.k), false);
@@ -700,7 +699,7 @@ struct Scores : Common {
         *reinterpret_cast<uint4*>(st.p + unit_at(i, c >> 3)) = make_uint4(v[0], v[1], v[2], v[3]);
       }
       settle();
-      bar_arrive(BAR_READY + s, 2 * GROUP + OUT_THREADS);
+      bar_arrive(BAR_READY + s, GROUP + STATE + OUT_THREADS);
     }
   }
 };
@@ -748,7 +747,7 @@ struct Follow : Common {
     tmem_st_wait();
     m = warp_most(m);
     if (lane == 0) sm.most_s[1][w] = m;
-    bar_sync(BAR_STATE, GROUP);
+    bar_sync(BAR_STATE, STATE);
     float bound = most(sm.most_s[1]), ix = 1.f, whole = 0.f;
     for (int n = 0;; ++n) {
       float ps, is, px;
@@ -772,7 +771,7 @@ struct Follow : Common {
       if (n == part.chunks) break;
       const int s = n % STAGES;
       Stage& st = sm.stage[s];
-      bar_sync(BAR_READY + s, 2 * GROUP + (OUT ? OUT_THREADS : 0));
+      bar_sync(BAR_READY + s, GROUP + STATE + (OUT ? OUT_THREADS : 0));
       m = warp_most(m);
       uint32_t m2 = 0;
 #pragma unroll
@@ -786,8 +785,8 @@ struct Follow : Common {
         sm.most_v[n & 1][w] = mv;
       }
       settle();
-      if (OUT && n > 0) bar_sync(BAR_TAKEN, GROUP + OUT_THREADS);
-      else bar_sync(BAR_STATE, GROUP);
+      if (OUT && n > 0) bar_sync(BAR_TAKEN, STATE + OUT_THREADS);
+      else bar_sync(BAR_STATE, STATE);
       if (w == 0) {
         tc_fence_after_sync();
         product<128, 0, 1>(sm.tmem + TM_CHAIN, operand(st.k_again), operand(sm.s_hi, TWO_TILES), false);
@@ -802,7 +801,6 @@ struct Follow : Common {
       const float fx = fv * px, fy = st.of_y[row] * (is * px), fu = st.of_u[row];
       if (OUT && threadIdx.x == 0) sm.inverse[n & 1] = make_float2(is, ix);
       wait(sm.bar_y, n);
-      if (n > 0 && n - 1 + STAGES < part.chunks) bar_arrive(BAR_FREE + (n - 1) % STAGES, 2 * GROUP + (OUT ? OUT_THREADS : 0));
 #pragma unroll 1
       for (int c = 0; c < 32; c += 16) {
         float2 x[8], y[8];
@@ -816,7 +814,7 @@ struct Follow : Common {
         put(x, sm.x_hi, sm.x_lo, row, 4 * half + (c >> 3));
       }
       settle();
-      bar_sync(BAR_STATE, GROUP);
+      bar_sync(BAR_STATE, STATE);
       if (w == 0) {
         tc_fence_after_sync();
         product<128, 1, 1>(sm.tmem + TM_CHAIN, operand(st.t_hi, SAME_TWICE), operand(sm.x_hi, TWO_TILES), false);
@@ -846,8 +844,8 @@ struct Follow : Common {
         put(x, sm.x_hi, sm.x_lo, row, 4 * half + (c >> 3));
       }
       settle();
-      bar_sync(BAR_STATE, GROUP);
-      if (OUT) bar_arrive(BAR_GIVEN, GROUP + OUT_THREADS);
+      bar_sync(BAR_STATE, STATE);
+      if (OUT) bar_arrive(BAR_GIVEN, STATE + OUT_THREADS);
       if (w == 0) {
         tc_fence_after_sync();
         product<128, 1, 1>(sm.tmem + TM_CHAIN, operand(st.k, SAME_TWICE), operand(sm.x_hi, TWO_TILES), false);
@@ -857,7 +855,8 @@ struct Follow : Common {
           commit(sm.bar_o);
         }
       }
-      wait(sm.bar_s, n);
+      wait(sm.bar_s, n);                         // the outputs' group waits for P U before it frees the stage as well
+      if (n + STAGES < part.chunks) bar_arrive(BAR_FREE + s, GROUP + STATE + (OUT ? OUT_THREADS : 0));
     }
     if (to != nullptr) {
 #pragma unroll 1
@@ -874,41 +873,70 @@ struct Follow : Common {
   }
 };
 
-// ---- the outputs: a token a thread --------------------------------------------------------------------------------------
+// ---- Q, and the outputs: a token a thread of two warps ----------------------------------------------------------------------
 struct Outputs : Common {
+  __device__ __forceinline__ void rows(__nv_bfloat16* op, int n) const {
+    const int s = n % STAGES, row = 32 * w + lane, t = part.begin + n * CHUNK + row;
+    const Stage& st = sm.stage[s];
+    bar_sync(BAR_GIVEN, STATE + OUT_THREADS);
+    const float2 inverse = sm.inverse[n & 1];
+    const float fs = st.of_s[row] * inverse.x, fu = st.of_o[row] * inverse.y;
+    wait(sm.bar_o, n);
+    if (n + STAGES < part.chunks) bar_arrive(BAR_FREE + s, GROUP + STATE + OUT_THREADS);
+#pragma unroll 1
+    for (int c = 0; c < D; c += 16) {
+      float2 a[8], b[8];
+      tmem_ld16x2(tm + TM_QS + c, tm + TM_PU + c, a, b);
+      uint32_t x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        a[e] = fma2(b[e], both(fu), mul2(a[e], both(fs)));
+        x[e] = pack_bf16x2(a[e].x, a[e].y);
+      }
+      if (t < part.len) {
+        uint4* to = reinterpret_cast<uint4*>(op + size_t(t) * p.ldo + c);
+        to[0] = make_uint4(x[0], x[1], x[2], x[3]);
+        to[1] = make_uint4(x[4], x[5], x[6], x[7]);
+      }
+    }
+    tc_fence_before_sync();
+    if (n + 1 < part.chunks) bar_arrive(BAR_TAKEN, STATE + OUT_THREADS);
+  }
+
   __device__ __forceinline__ void run() const {
     __nv_bfloat16* op = p.o + size_t(part.b) * p.T * p.ldo + size_t(part.h) * D;
-    const int row = 32 * w + lane;
-    for (int n = 0; n < part.chunks; ++n) {
-      const int s = n % STAGES, t = part.begin + n * CHUNK + row;
-      const Stage& st = sm.stage[s];
-      bar_sync(BAR_GIVEN, GROUP + OUT_THREADS);
-      const float2 inverse = sm.inverse[n & 1];
-      const float fs = st.of_s[row] * inverse.x, fu = st.of_o[row] * inverse.y;
-      if (n + STAGES < part.chunks) bar_arrive(BAR_FREE + s, 2 * GROUP + OUT_THREADS);
-      wait(sm.bar_o, n);
-#pragma unroll 1
-      for (int c = 0; c < D; c += 16) {
-        float2 a[8], b[8];
-        tmem_ld16x2(tm + TM_QS + c, tm + TM_PU + c, a, b);
-        uint32_t x[8];
+    const __nv_bfloat16* qp = p.q + size_t(part.b) * p.T * p.ldq + size_t(part.h / p.per_key) * D;
+    const int row = (32 * w + lane) >> 1, half = lane & 1;
+    uint4 q[2][4];
+    auto fetch = [&](int t0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          a[e] = fma2(b[e], both(fu), mul2(a[e], both(fs)));
-          x[e] = pack_bf16x2(a[e].x, a[e].y);
+      for (int m = 0; m < 2; ++m) fetch_half(q[m], qp + size_t(t0 + 32 * m + row) * p.ldq + 32 * half, t0 + 32 * m + row < part.len);
+    };
+    if (part.chunks > 0) fetch(part.begin);
+    // Q of a chunk before the outputs of the one before it
+#pragma unroll 1
+    for (int n = 0; n <= part.chunks; ++n) {
+      if (n < part.chunks) {
+        const int s = n % STAGES;
+        Stage& st = sm.stage[s];
+        wait(sm.bar_k[s], n / STAGES);           // the stage is free, K is there
+#pragma unroll 1
+        for (int m = 0; m < 2; ++m) {
+          float sc;
+          const float ss = convert_half(q[0], st.q, false, 32 * m + row, half, sc);
+          if (half == 0) st.of_o[32 * m + row] = p.scale * (p.normalize ? rsqrtf(fmaf(NORM_EPS * sc, sc, ss)) : inverse_power(sc));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[0][e] = q[1][e];
         }
-        if (t < part.len) {
-          uint4* to = reinterpret_cast<uint4*>(op + size_t(t) * p.ldo + c);
-          to[0] = make_uint4(x[0], x[1], x[2], x[3]);
-          to[1] = make_uint4(x[4], x[5], x[6], x[7]);
-        }
+        if (n + 1 < part.chunks) fetch(part.begin + (n + 1) * CHUNK);
+        settle();
+        bar_arrive(BAR_SCORES, 2 * OUT_THREADS);
       }
-      tc_fence_before_sync();
-      if (n + 1 < part.chunks) bar_arrive(BAR_TAKEN, GROUP + OUT_THREADS);
+      if (n > 0) rows(op, n - 1);
     }
-    for (int t = part.begin + part.chunks * CHUNK + row; t < p.T; t += OUT_THREADS) zero_row(op, t);
-    if (part.chunks > 0 && part.begin + (part.chunks - 1) * CHUNK + row >= part.len && part.begin + (part.chunks - 1) * CHUNK + row < p.T)
-      zero_row(op, part.begin + (part.chunks - 1) * CHUNK + row);
+    const int first = part.begin + part.chunks * CHUNK, t = first - CHUNK + 32 * w + lane;
+    if (part.chunks > 0 && t >= part.len && t < p.T) zero_row(op, t);
+    for (int i = first + 32 * w + lane; i < p.T; i += OUT_THREADS) zero_row(op, i);
   }
   __device__ __forceinline__ void zero_row(__nv_bfloat16* op, int t) const {
 #pragma unroll 1
