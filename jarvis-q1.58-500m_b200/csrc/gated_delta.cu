@@ -142,10 +142,10 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 //   X = b (V - e^G K S^T),   U = T X with T = (I + A)^-1,  A_ij = b_i e^(G_i - G_j) k_i.k_j  (j < i)
 //   O = e^G Q S^T + P U with P_ij = e^(G_i - G_j) q_i.k_j  (j <= i),   S' = e^Gc S + (e^(Gc - G) U)^T K
 // A CTA follows one head of one sequence:
-//   warps 0-3          the state: S in tensor memory (f32, a key and 32 values a thread); per chunk three products, K S^T, T X and K^T U, with
+//   warps 0-3          the state: S in registers (f32, a key and 32 values a thread); per chunk three products, K S^T, T X and K^T U, with
 //                      X, U and S back in shared memory as their operands between them: the chain that everything waits for
-//   warps 4-7, 8-11    by turns prepare a chunk, nothing of the state: K as f16, A and T
-//   warps 12, 13       Q as f16; output rows from Q S^T and P U, which the state's warps issue beside their own
+//   warps 4-7, 8-11    by turns prepare a chunk, nothing of the state: K and Q as f16, A and T
+//   warps 12, 13       output rows from Q S^T and P U, which the state's warps issue beside their own
 //   warps 14, 15       P
 // The products are tcgen05.mma, 128 rows at a time: a chunk has 64, so that the operand is there twice (K twice in memory; a second reading
 // of T^T and K, MN-major) and all four of a group's warps find 64 rows in their lanes; for P it is [K; Q], of Q and P as operands the
@@ -195,7 +195,7 @@ static_assert(sizeof(Stage) % 1024 == 0, "tiles lie on 1024-byte boundaries");
 constexpr size_t CHUNK_SMEM = sizeof(ChunkSmem) + 1024;
 
 // tensor memory: accumulators of 64 columns; TM_CHAIN, the state's three products one after the other, has two
-enum { TM_A = 0 /* + 64 group */, TM_CHAIN = 128, TM_QS = 256, TM_PU = 320, TM_STATE = 384, TM_P = 448, TM_COLUMNS = 512 };
+enum { TM_A = 0 /* + 64 group */, TM_CHAIN = 128, TM_QS = 256, TM_PU = 320, TM_P = 384, TM_COLUMNS = 512 };
 // Columns of the thread's lane
 #define JB_R8(x, i) "=&r"(x[i]), "=&r"(x[i + 1]), "=&r"(x[i + 2]), "=&r"(x[i + 3]), "=&r"(x[i + 4]), "=&r"(x[i + 5]), "=&r"(x[i + 6]), "=&r"(x[i + 7])
 __device__ __forceinline__ void tmem_ld8(uint32_t at, float (&x)[8]) {
@@ -222,15 +222,6 @@ __device__ __forceinline__ void tmem_ld16x2(uint32_t a, uint32_t b, float2 (&x)[
     x[i] = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
     y[i] = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
   }
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t a, float2 (&x)[8]) {
-  uint32_t r[16];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
-               : JB_R8(r, 0), JB_R8(r, 8)
-               : "r"(a)
-               : "memory");
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t at, const float2 (&x)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "f"(x[0].x), "f"(x[0].y),
@@ -295,6 +286,13 @@ __device__ __forceinline__ void power_scale(float m, float& s, float& inv) {
   s = __uint_as_float(uint32_t(254 + 14 - e) << 23);
   inv = __uint_as_float(uint32_t(e - 14) << 23);
 }
+// The larger sizes of two pairs of f16
+__device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {
+  const __half2 m = __hmax2(__habs2(*reinterpret_cast<const __half2*>(&a)), __habs2(*reinterpret_cast<const __half2*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ float f16_lo(uint32_t x) { return __low2float(*reinterpret_cast<const __half2*>(&x)); }
+__device__ __forceinline__ float f16_hi(uint32_t x) { return __high2float(*reinterpret_cast<const __half2*>(&x)); }
 __device__ __forceinline__ float inverse_power(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }      // of a power of two
 __device__ __forceinline__ uint32_t unit_at(int row, int unit) { return uint32_t(row * 128 + ((unit ^ (row & 7)) << 4)); }
 
@@ -603,13 +601,15 @@ struct Prepare : Common {
   __device__ __forceinline__ void run() const {
     const size_t first = size_t(part.b) * p.T;
     const __nv_bfloat16* kp = p.k + first * p.ldk + size_t(part.h / p.per_key) * D;
+    const __nv_bfloat16* qp = p.q + first * p.ldq + size_t(part.h / p.per_key) * D;
     Solve& so = sm.solve[group];
     const int row = 16 * w + (lane >> 1), half = lane & 1;
-    uint4 k[4];
+    uint4 k[4], q[4];
     float g0 = 0.f, g1 = 0.f, b0 = 0.f, b1 = 0.f;
     auto fetch = [&](int t0) {
       const int at = t0 + row;
       fetch_half(k, kp + size_t(at) * p.ldk + 32 * half, at < part.len);
+      if (OUT) fetch_half(q, qp + size_t(at) * p.ldq + 32 * half, at < part.len);
       if (w == 3) {
         const int t = t0 + 2 * lane;
         g0 = t < part.len ? load_now(p.log_decay + (first + t) * p.ldg + part.h) : 0.f;
@@ -632,13 +632,24 @@ struct Prepare : Common {
         *reinterpret_cast<float4*>(&st.g[2 * lane]) = make_float4(x.hi.x, x.lo.x, x.hi.y, x.lo.y);
         if (lane == 0) st.whole = x.whole;
       }
-      float sc;
-      const float ss = convert_half(k, st.k_again, true, row, half, sc);
-      if (half == 0) {
-        // k = n (k16 r) with |k16 r| = 1, or of the normalised key n = 1 and k16 r its value
-        const float r = p.normalize ? rsqrtf(fmaf(NORM_EPS * sc, sc, ss)) : ss > 0.f ? rsqrtf(ss) : 0.f;
-        st.rk[row] = r;
-        st.nk[row] = p.normalize ? 1.f : ss * r * inverse_power(sc);
+#pragma unroll 1
+      for (int m = 0; m < (OUT ? 2 : 1); ++m) {  // K twice, Q
+        float sc;
+        const float ss = convert_half(k, m == 0 ? st.k_again : st.q, m == 0, row, half, sc);
+        if (half == 0) {
+          // k = n (k16 r) with |k16 r| = 1, or of the normalised key n = 1 and k16 r its value
+          const float r = p.normalize ? rsqrtf(fmaf(NORM_EPS * sc, sc, ss)) : ss > 0.f ? rsqrtf(ss) : 0.f;
+          if (m == 0) {
+            st.rk[row] = r;
+            st.nk[row] = p.normalize ? 1.f : ss * r * inverse_power(sc);
+          } else {
+            st.of_o[row] = p.scale * (p.normalize ? r : inverse_power(sc));
+          }
+        }
+        if (OUT) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) k[i] = q[i];
+        }
       }
       if (n + 2 < part.chunks) fetch(t0 + 2 * CHUNK);
       settle();
@@ -678,7 +689,8 @@ struct Scores : Common {
     for (int n = 0; n < part.chunks; ++n) {
       const int s = n % STAGES;
       Stage& st = sm.stage[s];
-      bar_sync(BAR_SCORES, 2 * OUT_THREADS);     // Q is there, K before it
+      wait(sm.bar_k[s], n / STAGES);             // the stage is free, K and Q are there
+      bar_sync(BAR_SCORES, OUT_THREADS);         // both warps have read the chunk before
       if (w == 2) {
         tc_fence_after_sync();
         product<64, 0, 0>(sm.tmem + TM_P, operand(st.k), operand(st.k), false);
@@ -707,13 +719,16 @@ struct Scores : Common {
 // ---- the group of the state ------------------------------------------------------------------------------------------
 template <bool OUT>
 struct Follow : Common {
-  // 16 values of a row in two terms, from unit `unit` on
-  __device__ __forceinline__ static void put(const float2 (&x)[8], uint8_t* hi_tile, uint8_t* lo_tile, int row, int unit) {
+  // 16 values of a row in two terms, from unit `unit` on; most: the largest sizes among the hi terms
+  __device__ __forceinline__ static void put(const float2 (&x)[8], uint8_t* hi_tile, uint8_t* lo_tile, int row, int unit, uint32_t& most) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) split(x[4 * u + e], hi[e], lo[e]);
+      for (int e = 0; e < 4; ++e) {
+        split(x[4 * u + e], hi[e], lo[e]);
+        most = max_f16x2(most, hi[e]);
+      }
       const uint32_t at = unit_at(row, unit + u);
       *reinterpret_cast<uint4*>(hi_tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       *reinterpret_cast<uint4*>(lo_tile + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -726,21 +741,21 @@ struct Follow : Common {
   // them waited for its instructions (a chunk took 9600 cycles on 128 SMs).
   __device__ __forceinline__ void run(const float* from, float* to) const {
     const int row = 32 * (w & 1) + lane, half = w >> 1;          // a key (S) or a token (X, U), and which 32 values of it
-    const uint32_t cols = tm + TM_CHAIN + 32 * half, state = tm + TM_STATE + 32 * half;
+    const uint32_t cols = tm + TM_CHAIN + 32 * half;
     const __nv_bfloat16* vp = p.v + size_t(part.b) * p.T * p.ldv + size_t(part.h) * D + 32 * half;
     uint4 v[4];
     if (part.chunks > 0) fetch_half(v, vp + size_t(part.begin + row) * p.ldv, part.begin + row < part.len);
     // the state before the first chunk is added to none as if it were a product
     float m = 0.f;
-#pragma unroll 1
-    for (int c = 0; c < 32; c += 16) {
+    float2 S[16] = {};
+#pragma unroll
+    for (int c = 0; c < 16; c += 8) {
       float2 x[8] = {};
-      tmem_st16(state + c, x);
-      tmem_st16(cols + 64 + c, x);
+      tmem_st16(cols + 64 + 2 * c, x);
       if (from != nullptr)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = make_float2(from[(32 * half + c + 2 * e) * D + row], from[(32 * half + c + 2 * e + 1) * D + row]);
-      tmem_st16(cols + c, x);
+        for (int e = 0; e < 8; ++e) x[e] = make_float2(from[(32 * half + 2 * (c + e)) * D + row], from[(32 * half + 2 * (c + e) + 1) * D + row]);
+      tmem_st16(cols + 2 * c, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = fmaxf(m, fmaxf(fabsf(x[e].x), fabsf(x[e].y)));
     }
@@ -752,28 +767,24 @@ struct Follow : Common {
     for (int n = 0;; ++n) {
       float ps, is, px;
       power_scale(bound, ps, is);
-      m = 0.f;
-#pragma unroll 1
-      for (int c = 0; c < 32; c += 16) {
-        float2 x[8], y[8], z[8];
-        tmem_ld16x2(cols + c, cols + 64 + c, x, y);
-        tmem_ld16(state + c, z);
+      uint32_t m2 = 0;                           // of the hi terms, f16
+#pragma unroll
+      for (int c = 0; c < 16; c += 8) {
+        float2 x[8], y[8];
+        tmem_ld16x2(cols + 2 * c, cols + 64 + 2 * c, x, y);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          z[e] = fma2(add2(x[e], y[e]), both(ix), mul2(z[e], both(whole)));
-          m = fmaxf(m, fmaxf(fabsf(z[e].x), fabsf(z[e].y)));
-          x[e] = mul2(z[e], both(ps));
+          S[c + e] = fma2(add2(x[e], y[e]), both(ix), mul2(S[c + e], both(whole)));
+          x[e] = mul2(S[c + e], both(ps));
         }
-        tmem_st16(state + c, z);
-        put(x, sm.s_hi, sm.s_lo, row, 4 * half + (c >> 3));
+        put(x, sm.s_hi, sm.s_lo, row, 4 * half + (c >> 2), m2);
       }
-      tmem_st_wait();
       if (n == part.chunks) break;
       const int s = n % STAGES;
       Stage& st = sm.stage[s];
       bar_sync(BAR_READY + s, GROUP + STATE + (OUT ? OUT_THREADS : 0));
-      m = warp_most(m);
-      uint32_t m2 = 0;
+      const float m = warp_most(fmaxf(f16_lo(m2), f16_hi(m2))) * is;
+      m2 = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t m4 = 0x7fff7fffu;
@@ -800,6 +811,7 @@ struct Follow : Common {
       bound = fmaf(8.f * whole, ms, 64.f * mb);
       const float fx = fv * px, fy = st.of_y[row] * (is * px), fu = st.of_u[row];
       if (OUT && threadIdx.x == 0) sm.inverse[n & 1] = make_float2(is, ix);
+      uint32_t unused = 0;
       wait(sm.bar_y, n);
 #pragma unroll 1
       for (int c = 0; c < 32; c += 16) {
@@ -811,7 +823,7 @@ struct Follow : Common {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           x[e] = fma2(add2(x[e], y[e]), both(-fy), mul2(make_float2(bf16_lo(in[e]), bf16_hi(in[e])), both(fx)));
-        put(x, sm.x_hi, sm.x_lo, row, 4 * half + (c >> 3));
+        put(x, sm.x_hi, sm.x_lo, row, 4 * half + (c >> 3), unused);
       }
       settle();
       bar_sync(BAR_STATE, STATE);
@@ -841,7 +853,7 @@ struct Follow : Common {
           *reinterpret_cast<uint4*>(sm.u + unit_at(row, 4 * half + (c >> 3))) = make_uint4(one[0], one[1], one[2], one[3]);
           *reinterpret_cast<uint4*>(sm.u + unit_at(row, 4 * half + (c >> 3) + 1)) = make_uint4(one[4], one[5], one[6], one[7]);
         }
-        put(x, sm.x_hi, sm.x_lo, row, 4 * half + (c >> 3));
+        put(x, sm.x_hi, sm.x_lo, row, 4 * half + (c >> 3), unused);
       }
       settle();
       bar_sync(BAR_STATE, STATE);
@@ -859,84 +871,51 @@ struct Follow : Common {
       if (n + STAGES < part.chunks) bar_arrive(BAR_FREE + s, GROUP + STATE + (OUT ? OUT_THREADS : 0));
     }
     if (to != nullptr) {
-#pragma unroll 1
-      for (int c = 0; c < 32; c += 16) {
-        float2 x[8];
-        tmem_ld16(state + c, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          to[(32 * half + c + 2 * e) * D + row] = x[e].x;
-          to[(32 * half + c + 2 * e + 1) * D + row] = x[e].y;
-        }
+      for (int e = 0; e < 16; ++e) {
+        to[(32 * half + 2 * e) * D + row] = S[e].x;
+        to[(32 * half + 2 * e + 1) * D + row] = S[e].y;
       }
     }
   }
 };
 
-// ---- Q, and the outputs: a token a thread of two warps ----------------------------------------------------------------------
+// ---- the outputs: a token a thread of two warps --------------------------------------------------------------------------
 struct Outputs : Common {
-  __device__ __forceinline__ void rows(__nv_bfloat16* op, int n) const {
-    const int s = n % STAGES, row = 32 * w + lane, t = part.begin + n * CHUNK + row;
-    const Stage& st = sm.stage[s];
-    bar_sync(BAR_GIVEN, STATE + OUT_THREADS);
-    const float2 inverse = sm.inverse[n & 1];
-    const float fs = st.of_s[row] * inverse.x, fu = st.of_o[row] * inverse.y;
-    wait(sm.bar_o, n);
-    if (n + STAGES < part.chunks) bar_arrive(BAR_FREE + s, GROUP + STATE + OUT_THREADS);
-#pragma unroll 1
-    for (int c = 0; c < D; c += 16) {
-      float2 a[8], b[8];
-      tmem_ld16x2(tm + TM_QS + c, tm + TM_PU + c, a, b);
-      uint32_t x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        a[e] = fma2(b[e], both(fu), mul2(a[e], both(fs)));
-        x[e] = pack_bf16x2(a[e].x, a[e].y);
-      }
-      if (t < part.len) {
-        uint4* to = reinterpret_cast<uint4*>(op + size_t(t) * p.ldo + c);
-        to[0] = make_uint4(x[0], x[1], x[2], x[3]);
-        to[1] = make_uint4(x[4], x[5], x[6], x[7]);
-      }
-    }
-    tc_fence_before_sync();
-    if (n + 1 < part.chunks) bar_arrive(BAR_TAKEN, STATE + OUT_THREADS);
-  }
-
   __device__ __forceinline__ void run() const {
     __nv_bfloat16* op = p.o + size_t(part.b) * p.T * p.ldo + size_t(part.h) * D;
-    const __nv_bfloat16* qp = p.q + size_t(part.b) * p.T * p.ldq + size_t(part.h / p.per_key) * D;
-    const int row = (32 * w + lane) >> 1, half = lane & 1;
-    uint4 q[2][4];
-    auto fetch = [&](int t0) {
-#pragma unroll
-      for (int m = 0; m < 2; ++m) fetch_half(q[m], qp + size_t(t0 + 32 * m + row) * p.ldq + 32 * half, t0 + 32 * m + row < part.len);
-    };
-    if (part.chunks > 0) fetch(part.begin);
-    // Q of a chunk before the outputs of the one before it
+    const int row = 32 * w + lane;
 #pragma unroll 1
-    for (int n = 0; n <= part.chunks; ++n) {
-      if (n < part.chunks) {
-        const int s = n % STAGES;
-        Stage& st = sm.stage[s];
-        wait(sm.bar_k[s], n / STAGES);           // the stage is free, K is there
+    for (int n = 0; n < part.chunks; ++n) {
+      const int s = n % STAGES, t = part.begin + n * CHUNK + row;
+      const Stage& st = sm.stage[s];
+      bar_sync(BAR_GIVEN, STATE + OUT_THREADS);
+      const float2 inverse = sm.inverse[n & 1];
+      const float fs = st.of_s[row] * inverse.x, fu = st.of_o[row] * inverse.y;
+      wait(sm.bar_o, n);
+      if (n + STAGES < part.chunks) bar_arrive(BAR_FREE + s, GROUP + STATE + OUT_THREADS);
 #pragma unroll 1
-        for (int m = 0; m < 2; ++m) {
-          float sc;
-          const float ss = convert_half(q[0], st.q, false, 32 * m + row, half, sc);
-          if (half == 0) st.of_o[32 * m + row] = p.scale * (p.normalize ? rsqrtf(fmaf(NORM_EPS * sc, sc, ss)) : inverse_power(sc));
+      for (int c = 0; c < D; c += 16) {
+        float2 a[8], b[8];
+        tmem_ld16x2(tm + TM_QS + c, tm + TM_PU + c, a, b);
+        uint32_t x[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) q[0][e] = q[1][e];
+        for (int e = 0; e < 8; ++e) {
+          a[e] = fma2(b[e], both(fu), mul2(a[e], both(fs)));
+          x[e] = pack_bf16x2(a[e].x, a[e].y);
         }
-        if (n + 1 < part.chunks) fetch(part.begin + (n + 1) * CHUNK);
-        settle();
-        bar_arrive(BAR_SCORES, 2 * OUT_THREADS);
+        if (t < part.len) {
+          uint4* to = reinterpret_cast<uint4*>(op + size_t(t) * p.ldo + c);
+          to[0] = make_uint4(x[0], x[1], x[2], x[3]);
+          to[1] = make_uint4(x[4], x[5], x[6], x[7]);
+        }
       }
-      if (n > 0) rows(op, n - 1);
+      tc_fence_before_sync();
+      if (n + 1 < part.chunks) bar_arrive(BAR_TAKEN, STATE + OUT_THREADS);
     }
-    const int first = part.begin + part.chunks * CHUNK, t = first - CHUNK + 32 * w + lane;
+    const int first = part.begin + part.chunks * CHUNK, t = first - CHUNK + row;
     if (part.chunks > 0 && t >= part.len && t < p.T) zero_row(op, t);
-    for (int i = first + 32 * w + lane; i < p.T; i += OUT_THREADS) zero_row(op, i);
+    for (int i = first + row; i < p.T; i += OUT_THREADS) zero_row(op, i);
   }
   __device__ __forceinline__ void zero_row(__nv_bfloat16* op, int t) const {
 #pragma unroll 1
