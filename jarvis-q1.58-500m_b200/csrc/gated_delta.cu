@@ -25,7 +25,13 @@ struct DeltaParams {
   int B, T, H, per_key;                     // per_key: value heads that share a key head
   float scale;
   int normalize;
+  int segments, seg_chunks;                 // pieces of a sequence, 64 tokens times seg_chunks each
+  int what;                                 // of this launch: ALL segments (with outputs), the PIECES of all but the last, the LAST segment's state
+  float* pieces;                            // [B][H][2 segments - 1][64][64]: what segment s adds (from segment s + 1 on: the state before it), then what
+                                            // it multiplies the state by, last the state before segment 0
 };
+enum { ALL, PIECES, LAST };
+__host__ __device__ __forceinline__ size_t piece_at(int segments, int bh, int i) { return (size_t(bh) * (2 * segments - 1) + i) * D * D; }
 
 __device__ __forceinline__ int sequence_length(const DeltaParams& p, int b) {
   return p.lengths == nullptr ? p.T : min(max(__ldg(p.lengths + b), 0), p.T);
@@ -161,6 +167,7 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 // is one term, 2^-12 of a value where the output's own rounding is 2^-9.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int CHUNK = 64;
+constexpr int CHUNK_TOKENS = 24;          // from so many tokens on
 constexpr int TILE = CHUNK * D * 2;        // bytes of 64 rows of 128, the 16-byte units of row r at unit ^ (r & 7): the 128-byte swizzle
 constexpr int STAGES = 3;
 constexpr int STATE = 128, GROUP = 128;    // threads of the state's group, of a preparing one
@@ -739,12 +746,13 @@ struct Follow : Common {
 
   // The loops over a thread's 32 columns stay loops: the roles of this kernel share the instruction caches, and unrolled (77 KB in all) every one of
   // them waited for its instructions (a chunk took 9600 cycles on 128 SMs).
-  __device__ __forceinline__ void run(const float* from, float* to) const {
+  // from `from` (null: 0) through the part's chunks to `to`; `factor`: from the identity, with v as 0, which gives what the part multiplies a state by
+  __device__ __forceinline__ void run(const float* from, float* to, bool factor) const {
     const int row = 32 * (w & 1) + lane, half = w >> 1;          // a key (S) or a token (X, U), and which 32 values of it
     const uint32_t cols = tm + TM_CHAIN + 32 * half;
     const __nv_bfloat16* vp = p.v + size_t(part.b) * p.T * p.ldv + size_t(part.h) * D + 32 * half;
     uint4 v[4];
-    if (part.chunks > 0) fetch_half(v, vp + size_t(part.begin + row) * p.ldv, part.begin + row < part.len);
+    if (part.chunks > 0) fetch_half(v, vp + size_t(part.begin + row) * p.ldv, !factor && part.begin + row < part.len);
     // the state before the first chunk is added to none as if it were a product
     float m = 0.f;
     float2 S[16] = {};
@@ -755,6 +763,9 @@ struct Follow : Common {
       if (from != nullptr)
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = make_float2(from[(32 * half + 2 * (c + e)) * D + row], from[(32 * half + 2 * (c + e) + 1) * D + row]);
+      else if (factor)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = make_float2(32 * half + 2 * (c + e) == row, 32 * half + 2 * (c + e) + 1 == row);
       tmem_st16(cols + 2 * c, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = fmaxf(m, fmaxf(fabsf(x[e].x), fabsf(x[e].y)));
@@ -835,7 +846,7 @@ struct Follow : Common {
       }
       if (n + 1 < part.chunks) {
         const int t = part.begin + (n + 1) * CHUNK + row;
-        fetch_half(v, vp + size_t(t) * p.ldv, t < part.len);
+        fetch_half(v, vp + size_t(t) * p.ldv, !factor && t < part.len);
       }
       wait(sm.bar_u, n);
 #pragma unroll 1
@@ -913,9 +924,9 @@ struct Outputs : Common {
       tc_fence_before_sync();
       if (n + 1 < part.chunks) bar_arrive(BAR_TAKEN, STATE + OUT_THREADS);
     }
-    const int first = part.begin + part.chunks * CHUNK, t = first - CHUNK + row;
-    if (part.chunks > 0 && t >= part.len && t < p.T) zero_row(op, t);
-    for (int i = first + row; i < p.T; i += OUT_THREADS) zero_row(op, i);
+    const int last = part.begin + part.chunks * CHUNK, t = last - CHUNK + row, end = min(p.T, part.begin + p.seg_chunks * CHUNK);
+    if (part.chunks > 0 && t >= part.len && t < end) zero_row(op, t);
+    for (int i = last + row; i < end; i += OUT_THREADS) zero_row(op, i);
   }
   __device__ __forceinline__ void zero_row(__nv_bfloat16* op, int t) const {
 #pragma unroll 1
@@ -950,18 +961,31 @@ __global__ void __launch_bounds__(3 * GROUP + (OUT ? 2 * OUT_THREADS : 0), 1) de
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  // A CTA a segment; of the pieces one for the first segment, which starts from the state that is given, two for each of the others
+  const int ctas = p.what == PIECES ? 2 * p.segments - 3 : p.what == LAST ? 1 : p.segments, bh = blockIdx.x / ctas, j = blockIdx.x % ctas;
+  const bool factor = p.what == PIECES && j > 0 && (j & 1) == 0;
+  const int segment = p.what == PIECES ? (j + 1) >> 1 : p.what == LAST ? p.segments - 1 : j;
   Part part;
-  part.b = blockIdx.x / p.H;
-  part.h = blockIdx.x % p.H;
-  part.begin = 0;
+  part.b = bh / p.H;
+  part.h = bh % p.H;
+  part.begin = segment * p.seg_chunks * CHUNK;
   pdl_wait();
   pdl_trigger();
-  part.len = sequence_length(p, part.b);
-  part.chunks = (part.len + CHUNK - 1) / CHUNK;
-  const size_t state = size_t(blockIdx.x) * D * D;
+  part.len = min(sequence_length(p, part.b), part.begin + p.seg_chunks * CHUNK);
+  part.chunks = part.len > part.begin ? (part.len - part.begin + CHUNK - 1) / CHUNK : 0;
+  const float* from = p.s_in == nullptr ? nullptr : p.s_in + size_t(bh) * D * D;
+  float* to = p.s_out == nullptr ? nullptr : p.s_out + size_t(bh) * D * D;
+  if (p.what == PIECES) {
+    if (segment > 0) from = nullptr;
+    to = p.pieces + piece_at(p.segments, bh, (factor ? p.segments - 1 : 0) + segment);
+  } else if (p.segments > 1) {
+    if (segment > 0) from = p.pieces + piece_at(p.segments, bh, segment - 1);
+    else if (p.s_in == p.s_out && p.s_in != nullptr) from = p.pieces + piece_at(p.segments, bh, 2 * p.segments - 2);
+    if (segment + 1 < p.segments) to = nullptr;
+  }
   const Common common{p, sm, part, w, lane, sm.tmem + (uint32_t(w) << 21), status};
   if (warp < 4) {
-    Follow<OUT>{common}.run(p.s_in == nullptr ? nullptr : p.s_in + state, p.s_out == nullptr ? nullptr : p.s_out + state);
+    Follow<OUT>{common}.run(from, to, factor);
   } else if (warp < 12) {
     Prepare<OUT>{common, (warp >> 2) - 1}.run();
   } else if (OUT) {
@@ -976,16 +1000,69 @@ __global__ void __launch_bounds__(3 * GROUP + (OUT ? 2 * OUT_THREADS : 0), 1) de
   }
 }
 
+// The state before every segment from what the segments add and multiply by: S_(s+1) = S_s M_s + N_s.  Eight value rows a CTA.
+__global__ void __launch_bounds__(128) delta_join_kernel(DeltaParams p) {
+  __shared__ __align__(16) float rows[2][8][D];
+  const int bh = blockIdx.x >> 3, r = threadIdx.x >> 4, c = (threadIdx.x & 15) * 4, v = (blockIdx.x & 7) * 8 + r;
+  pdl_wait();
+  pdl_trigger();
+  if (p.s_in == p.s_out && p.s_in != nullptr)        // the last segment may write it before the first one has read it
+    *reinterpret_cast<float4*>(p.pieces + piece_at(p.segments, bh, 2 * p.segments - 2) + v * D + c) =
+        *reinterpret_cast<const float4*>(p.s_in + size_t(bh) * D * D + v * D + c);
+  *reinterpret_cast<float4*>(&rows[0][r][c]) = *reinterpret_cast<const float4*>(p.pieces + piece_at(p.segments, bh, 0) + v * D + c);
+  for (int s = 1; s + 1 < p.segments; ++s) {
+    float4* n = reinterpret_cast<float4*>(p.pieces + piece_at(p.segments, bh, s) + v * D + c);
+    const float* m = p.pieces + piece_at(p.segments, bh, p.segments - 1 + s) + c;
+    float4 sum = *n;
+    __syncthreads();
+    const float* row = rows[(s + 1) & 1][r];
+#pragma unroll 16
+    for (int k = 0; k < D; ++k) {
+      const float4 x = *reinterpret_cast<const float4*>(m + k * D);
+      const float f = row[k];
+      sum.x = fmaf(f, x.x, sum.x);
+      sum.y = fmaf(f, x.y, sum.y);
+      sum.z = fmaf(f, x.z, sum.z);
+      sum.w = fmaf(f, x.w, sum.w);
+    }
+    *reinterpret_cast<float4*>(&rows[s & 1][r][c]) = sum;
+    *n = sum;
+  }
+}
+
+// Segments of a sequence where sequences and heads alone leave SMs idle.  In chunks' time, about 3 us: a pass over the tokens costs its chunks on as many
+// waves of CTAs as it has (1 CTA an SM), the pieces' pass has 2 n - 3 CTAs a head for the outputs' n; filling the pipeline and joining
+// come to about 6 (measured; the smaller sum wins, segments only by a tenth).
+int segments_of(int B, int T, int H) {
+  const long long sms = sm_count(), heads = (long long)B * H, chunks = (T + CHUNK - 1) / CHUNK;
+  auto waves = [&](long long ctas) { return (ctas + sms - 1) / sms; };
+  const double whole = double(waves(heads) * chunks);
+  double least = 0.9 * whole;
+  int best = 1;
+  for (int n = 3; n <= 32 && heads * n <= 2 * sms; ++n) {
+    const long long part = (chunks + n - 1) / n;
+    if ((chunks + part - 1) / part != n) continue;             // the last ones would be empty
+    const double cost = double(part) * double(waves(heads * (2 * n - 3)) + waves(heads * n)) + 6.0 + 0.25 * n;
+    if (cost < least) { least = cost; best = n; }
+  }
+  return best;
+}
+
 }  // namespace
 
-size_t gated_delta_scratch_bytes(int B, int T, int H) { return 0; }
+size_t gated_delta_scratch_bytes(int B, int T, int H) {
+  if (B < 1 || H < 1 || T < CHUNK_TOKENS) return 0;
+  const int n = segments_of(B, T, H);
+  return n == 1 ? 0 : piece_at(n, B * H, 0) * sizeof(float);
+}
 
 int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream) {
   JB_REQUIRE(d != nullptr, "gated_delta: null pointer");
   const int B = d->B, T = d->T, H = d->H, KH = d->key_heads;
   JB_REQUIRE(B >= 0 && T >= 0 && H >= 1 && KH >= 1 && H % KH == 0, "gated_delta: bad shape (B=%d, T=%d, H=%d, key heads=%d)", B, T, H, KH);
   JB_REQUIRE(d->head_dim == D, "gated_delta: head_dim must be 64 (got %d)", d->head_dim);
-  JB_REQUIRE((long long)B * H <= 0x1fffffff && (long long)B * T <= 0x7fffffff, "gated_delta: too many heads or tokens");
+  JB_REQUIRE((long long)B * H <= 0x1fffffff && (long long)B * T <= 0x7fffffff && T <= 1 << 30,
+             "gated_delta: too many heads or tokens");
   if (B == 0) return JB200_OK;
   JB_REQUIRE(d->o != nullptr || d->s_out != nullptr, "gated_delta: neither an output nor a final state is asked for");
   JB_REQUIRE(T == 0 || (d->q && d->k && d->v && d->log_decay && d->beta), "gated_delta: null pointer");
@@ -1003,14 +1080,31 @@ int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream)
   p.o = static_cast<__nv_bfloat16*>(d->o);
   p.B = B; p.T = T; p.H = H; p.per_key = H / KH;
   p.scale = d->scale; p.normalize = d->flags & JB200_DELTA_NORMALIZE;
-  if (T >= 24) {
-    if (p.o != nullptr) {
-      JB_MAX_SMEM(delta_chunk_kernel<true>, CHUNK_SMEM);
-      launch_dep(delta_chunk_kernel<true>, B * H, 3 * GROUP + 2 * OUT_THREADS, CHUNK_SMEM, stream, p, device_status_ptr());
-    } else {
-      JB_MAX_SMEM(delta_chunk_kernel<false>, CHUNK_SMEM);
-      launch_dep(delta_chunk_kernel<false>, B * H, 3 * GROUP, CHUNK_SMEM, stream, p, device_status_ptr());
+  p.segments = 1;
+  p.what = ALL;
+  p.seg_chunks = (T + CHUNK - 1) / CHUNK;
+  p.pieces = static_cast<float*>(scratch);
+  if (T >= CHUNK_TOKENS) {
+    JB_MAX_SMEM(delta_chunk_kernel<true>, CHUNK_SMEM);
+    JB_MAX_SMEM(delta_chunk_kernel<false>, CHUNK_SMEM);
+    if (scratch != nullptr) {
+      const int n = segments_of(B, T, H);
+      JB_REQUIRE(aligned16(scratch), "gated_delta: scratch must be 16-byte aligned");
+      if (n > 1) {
+        p.segments = n;
+        p.seg_chunks = (p.seg_chunks + n - 1) / n;
+        p.what = PIECES;
+        launch_dep(delta_chunk_kernel<false>, B * H * (2 * n - 3), STATE + 2 * GROUP, CHUNK_SMEM, stream, p, device_status_ptr());
+        JB_LAUNCH_CHECK("delta_chunk_kernel");
+        launch_dep(delta_join_kernel, B * H * 8, 128, 0, stream, p);
+        JB_LAUNCH_CHECK("delta_join_kernel");
+        p.what = p.o != nullptr ? ALL : LAST;
+      }
     }
+    if (p.o != nullptr)
+      launch_dep(delta_chunk_kernel<true>, B * H * p.segments, STATE + 2 * GROUP + 2 * OUT_THREADS, CHUNK_SMEM, stream, p, device_status_ptr());
+    else
+      launch_dep(delta_chunk_kernel<false>, B * H, STATE + 2 * GROUP, CHUNK_SMEM, stream, p, device_status_ptr());
     JB_LAUNCH_CHECK("delta_chunk_kernel");
     return JB200_OK;
   }

@@ -787,24 +787,40 @@ def sample(logits: torch.Tensor, u: torch.Tensor | None = None, *, temperature: 
 # --------------------------------------------------------------------------- gated delta rule, norms around a block, draws
 def _forward_only(what: str, *tensors):
     """These operators have no gradients: a graph that runs through one would lose its part without a word."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what}: a tensor requires a gradient, and none is formed here (call it under torch.no_grad() or detach)")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what}: a tensor requires a gradient, and none is formed here (call it under torch.no_grad() or detach)")
 
 
-def _row_view(t: torch.Tensor, rows: int, columns: int, dtype, what: str) -> torch.Tensor:
-    """A 2-D CUDA view (rows, columns) with unit inner stride, e.g. columns of a fused projection."""
+def _view(t: torch.Tensor, dev: int, shape, dtype, what: str, name: str) -> int:
+    """Checks a 2-D CUDA view with unit inner stride, e.g. columns of a fused projection, on device `dev`; -> elements from row to row."""
+    if t.dtype is dtype and t.get_device() == dev and t.shape == shape:
+        if shape[0] > 1 and shape[1] > 1:
+            ld, inner = t.stride()
+            if inner == 1:
+                return ld
+        elif shape[1] <= 1:
+            return t.stride(0) if shape[0] > 1 else 1
+        elif t.stride(1) == 1:
+            return shape[1]                      # the stride of one row says nothing
     if not t.is_cuda:
-        raise RuntimeError(f"{what}: expected a CUDA tensor (this path has no CPU fallback)")
-    if t.dtype != dtype:
-        raise RuntimeError(f"{what}: expected dtype {dtype}, got {t.dtype}")
-    if t.dim() != 2 or tuple(t.shape) != (rows, columns) or (columns > 1 and t.stride(1) != 1):
-        raise RuntimeError(f"{what}: expected ({rows}, {columns}) rows with unit inner stride, got {tuple(t.shape)} with strides {tuple(t.stride())}")
-    return t
+        raise RuntimeError(f"{what}.{name}: expected a CUDA tensor (this path has no CPU fallback)")
+    if t.get_device() != dev:
+        raise RuntimeError(f"{what}: tensors on cuda:{dev} and {t.device}")
+    if t.dtype is not dtype:
+        raise RuntimeError(f"{what}.{name}: expected dtype {dtype}, got {t.dtype}")
+    raise RuntimeError(f"{what}.{name}: expected {shape} rows with unit inner stride, got {tuple(t.shape)} with strides {tuple(t.stride())}")
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    """Elements from row to row; of a tensor of at most one row, whose stride says nothing, its width."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+def _whole(t: torch.Tensor, dev: int, dtype, count: int, what: str, name: str, meaning: str) -> int:
+    """Checks a contiguous tensor of `count` values on device `dev`; -> its address.  `meaning`: what an error says of the count."""
+    if t.dtype is dtype and t.get_device() == dev and t.numel() == count and t.is_contiguous():
+        return t.data_ptr()
+    _need(t, dtype, f"{what}.{name}")
+    if t.get_device() != dev:
+        raise RuntimeError(f"{what}: tensors on cuda:{dev} and {t.device}")
+    raise RuntimeError(f"{what}.{name}: {meaning}, got {tuple(t.shape)} for {count}")
 
 
 def _touch(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -815,6 +831,13 @@ def _touch(a: torch.Tensor, b: torch.Tensor) -> bool:
     return span[0][0] < span[1][1] and span[1][0] < span[0][1]
 
 
+def _apart(what: str, name: str, t: torch.Tensor, *others):
+    """What is written to must not be read as anything else."""
+    for o in others:
+        if o is not None and _touch(t, o):
+            raise RuntimeError(f"{what}: {name} overlaps another argument")
+
+
 def gated_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, beta: torch.Tensor, B: int, T: int, H: int, *,
                      key_heads: int | None = None, scale: float | None = None, normalize: bool = True, lengths: torch.Tensor | None = None,
                      state_in: torch.Tensor | None = None, want_state: bool = False, state_out: torch.Tensor | None = None,
@@ -823,89 +846,96 @@ def gated_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     S_t = a_t S_{t-1} (I - b_t k k^T) + b_t v k^T with a = exp(log_decay), o_t = scale S_t q_t.
     q, k: bf16 2-D views (B*T, key_heads*64), v: bf16 (B*T, H*64), each with a row stride of its own (e.g. column slices of a fused
     projection; 16-byte aligned, strides multiples of 8); value head h takes key head h // (H // key_heads).  log_decay (<= 0), beta: f32 (B*T, H), column
-    slices allowed.  normalize: k and q are divided by their norms, sqrt(|.|^2 + 1e-6).  scale: 1/8 unless given.  lengths: int32 (B,), for padded
-    batches: rows behind a sequence's length are not read, their output is 0, the state is that after its last row.
+    slices allowed.  normalize: k and q are divided by their norms, sqrt(|.|^2 + 1e-6); without it keep beta |k|^2 <= 2.  scale: 1/8 unless given.
+    lengths: int32 (B,), for padded batches: rows behind a sequence's length are not read, their output is 0, the state is that after its last row.
     Returns (o bf16 (B*T, H*64) or None, state f32 (B, H, 64 values, 64 keys) or None).  state_out may be state_in itself."""
     lib = _lib.load()
     what = "gated_delta_scan"
     KH = H if key_heads is None else key_heads
     if B < 0 or T < 0 or H < 1 or KH < 1 or H % KH:
         raise RuntimeError(f"{what}: bad shape (B={B}, T={T}, H={H}, key_heads={KH})")
-    N, bf16, f32 = B * T, torch.bfloat16, torch.float32
-    _row_view(q, N, KH * 64, bf16, what + ".q")
-    _row_view(k, N, KH * 64, bf16, what + ".k")
-    _row_view(v, N, H * 64, bf16, what + ".v")
-    _row_view(log_decay, N, H, f32, what + ".log_decay")
-    _row_view(beta, N, H, f32, what + ".beta")
-    if _row_stride(log_decay) != _row_stride(beta):
+    N, bf16, f32, dev = B * T, torch.bfloat16, torch.float32, q.get_device()
+    ldq = _view(q, dev, (N, KH * 64), bf16, what, "q")
+    ldk = _view(k, dev, (N, KH * 64), bf16, what, "k")
+    ldv = _view(v, dev, (N, H * 64), bf16, what, "v")
+    ldg = _view(log_decay, dev, (N, H), f32, what, "log_decay")
+    if _view(beta, dev, (N, H), f32, what, "beta") != ldg:
         raise RuntimeError(f"{what}: log_decay and beta must share their row stride")
-    if lengths is not None and _need(lengths, torch.int32, what + ".lengths").numel() != B:
-        raise RuntimeError(f"{what}: one length per sequence is needed")
-    _forward_only(what, q, k, v, log_decay, beta, state_in)
-    _together(what, q, k, v, log_decay, beta, lengths, state_in, state_out, out)
+    if not q.is_cuda:
+        raise RuntimeError(f"{what}.q: expected a CUDA tensor (this path has no CPU fallback)")
+    _forward_only(what, q, k, v, log_decay, beta, state_in, state_out, out)
     if _elsewhere(q):
-        with torch.cuda.device(q.device):
+        with torch.cuda.device(dev):
             return gated_delta_scan(q, k, v, log_decay, beta, B, T, H, key_heads=key_heads, scale=scale, normalize=normalize, lengths=lengths,
                                     state_in=state_in, want_state=want_state, state_out=state_out, out=out, want_out=want_out)
-    dev = q.device
+    lens = None if lengths is None else _whole(lengths, dev, torch.int32, B, what, "lengths", "one length per sequence is needed")
+    states = B * H * 4096
     for name, t in (("state_in", state_in), ("state_out", state_out)):
-        if t is not None and tuple(_need(t, f32, f"{what}.{name}").shape) != (B, H, 64, 64):
-            raise RuntimeError(f"{what}: {name} must be (B, H, 64, 64)")
-    if state_out is None and want_state:
-        state_out = torch.empty((B, H, 64, 64), dtype=f32, device=dev)
-    elif state_out is not None and state_in is not None and state_out.data_ptr() != state_in.data_ptr() and _overlap(state_out, state_in):
-        raise RuntimeError(f"{what}: state_out overlaps state_in without being it")
+        if t is not None and t.shape != (B, H, 64, 64):
+            raise RuntimeError(f"{what}: {name} must be (B, H, 64, 64), got {tuple(t.shape)}")
+    s_in = None if state_in is None else _whole(state_in, dev, f32, states, what, "state_in", "state_in must be (B, H, 64, 64)")
+    if state_out is not None:
+        s_out = _whole(state_out, dev, f32, states, what, "state_out", "state_out must be (B, H, 64, 64)")
+        if s_out != s_in and state_in is not None and _overlap(state_out, state_in):
+            raise RuntimeError(f"{what}: state_out overlaps state_in without being it")
+        _apart(what, "state_out", state_out, q, k, v, log_decay, beta, lengths, out)
+    elif want_state:
+        state_out = torch.empty((B, H, 64, 64), dtype=f32, device=q.device)
+        s_out = state_out.data_ptr()
+    else:
+        s_out = None
     if not want_out:
         if out is not None:
             raise RuntimeError(f"{what}: out is given and want_out is False")
-        if state_out is None:
+        if s_out is None:
             raise RuntimeError(f"{what}: neither an output nor a state is asked for")
-    elif out is None:
-        out = torch.empty((N, H * 64), dtype=bf16, device=dev)
+        o, ldo = None, 0
     else:
-        _row_view(out, N, H * 64, bf16, what + ".out")
-        if out.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{what}: out requires a gradient")
-        if any(t is not None and _touch(out, t) for t in (q, k, v, log_decay, beta, lengths, state_in, state_out)):
-            raise RuntimeError(f"{what}: out overlaps another argument")
-    if state_out is not None and any(t is not None and _touch(state_out, t) for t in (q, k, v, log_decay, beta, lengths)):
-        raise RuntimeError(f"{what}: state_out overlaps another argument")
-    if B == 0:
-        return out, state_out
-    d = _lib.Delta(B, T, H, KH, 64, _lib.DELTA_NORMALIZE if normalize else 0, _ptr(q), _ptr(k), _ptr(v), _row_stride(q), _row_stride(k), _row_stride(v),
-                   _ptr(log_decay), _ptr(beta), _row_stride(beta), _ptr(lengths), 0.125 if scale is None else float(scale), _ptr(state_in), _ptr(out),
-                   0 if out is None else _row_stride(out), _ptr(state_out))
-    nbytes = lib.jb200_gated_delta_scratch_bytes(B, T, H)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _lib.check(lib.jb200_gated_delta(ctypes.byref(d), _ptr(scratch), _stream()), "jb200_gated_delta")
+        if out is None:
+            out = torch.empty((N, H * 64), dtype=bf16, device=q.device)
+            ldo = H * 64
+        else:
+            ldo = _view(out, dev, (N, H * 64), bf16, what, "out")
+            _apart(what, "out", out, q, k, v, log_decay, beta, lengths, state_in)
+        o = out.data_ptr()
+    if B:
+        d = _lib.Delta(B, T, H, KH, 64, _lib.DELTA_NORMALIZE if normalize else 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), ldq, ldk, ldv,
+                       log_decay.data_ptr(), beta.data_ptr(), ldg, lens, 0.125 if scale is None else scale, s_in, o, ldo, s_out)
+        nbytes = lib.jb200_gated_delta_scratch_bytes(B, T, H) if T > 1 else 0
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
+        rc = lib.jb200_gated_delta(ctypes.byref(d), scratch, _stream())
+        if rc:
+            _lib.check(rc, "jb200_gated_delta")
     return out, state_out
 
 
-def _norm_arguments(what, y, gate):
-    """Rows of y and gate as 2-D views: leading dimensions must fold into one row stride."""
-    if y.dim() < 1 or (gate is not None and gate.shape != y.shape):
-        raise RuntimeError(f"{what}: y {tuple(y.shape)} and gate {tuple(gate.shape) if gate is not None else None} do not belong together")
-    width = y.shape[-1]
-    if width < 1:
-        raise RuntimeError(f"{what}: rows without columns")
-    views = []
-    for name, t in (("y", y), ("gate", gate)):
-        if t is None:
-            views.append(None)
-            continue
+def _norm_rows(t: torch.Tensor, width: int, dev: int, shape, dtype, what: str, name: str):
+    """Rows of one stride of a (..., width) tensor -> (address, elements from row to row)."""
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape:
         if not t.is_cuda:
             raise RuntimeError(f"{what}.{name}: expected a CUDA tensor (this path has no CPU fallback)")
-        _dt(t)
-        if t.dtype != y.dtype:
-            raise RuntimeError(f"{what}: gate must have y's dtype ({y.dtype}), got {t.dtype}")
+        if t.get_device() != dev:
+            raise RuntimeError(f"{what}: tensors on cuda:{dev} and {t.device}")
+        raise RuntimeError(f"{what}: y {tuple(shape)} ({dtype}) and {name} {tuple(t.shape)} ({t.dtype}) do not belong together (shape, dtype)")
+    if t.is_contiguous():
+        return t.data_ptr(), width
+    rows = t if t.dim() == 2 else None
+    if rows is None:
         try:
-            t = t.view(-1, width) if t.numel() else t.reshape(0, width)
+            rows = t.view(-1, width)
         except RuntimeError:
             raise RuntimeError(f"{what}.{name}: rows of one stride are needed, got {tuple(t.shape)} with strides {tuple(t.stride())}") from None
-        if width > 1 and t.stride(1) != 1:
-            raise RuntimeError(f"{what}.{name}: rows must have unit inner stride, got {tuple(t.stride())}")
-        views.append(t)
-    return views
+    if width > 1 and rows.stride(1) != 1:
+        raise RuntimeError(f"{what}.{name}: rows must have unit inner stride, got {tuple(t.stride())}")
+    return rows.data_ptr(), rows.stride(0) if rows.shape[0] > 1 else width
+
+
+def _norm_width(y: torch.Tensor, what: str) -> int:
+    if y.dim() < 1 or y.shape[-1] < 1:
+        raise RuntimeError(f"{what}: rows without columns, {tuple(y.shape)}")
+    if not y.is_cuda:
+        raise RuntimeError(f"{what}.y: expected a CUDA tensor (this path has no CPU fallback)")
+    return y.shape[-1]
 
 
 def gated_norm(y: torch.Tensor, weight: torch.Tensor, gate: torch.Tensor | None = None, *, group: int | None = None, eps: float = 1e-6,
@@ -915,20 +945,20 @@ def gated_norm(y: torch.Tensor, weight: torch.Tensor, gate: torch.Tensor | None 
     rows of one stride; weight f32.  After RMSNorm.forward (jarvis_engine/jarvis_model.py:25-26)."""
     lib = _lib.load()
     what = "gated_norm"
-    rows, g = _norm_arguments(what, y, gate)
-    _need(weight, torch.float32, what + ".weight")
-    N, width = rows.shape
+    width = _norm_width(y, what)
+    dev, dt = y.get_device(), _dt(y)
     group = width if group is None else int(group)
-    if weight.numel() != group:
-        raise RuntimeError(f"{what}: groups of {group} columns and weight {tuple(weight.shape)} do not belong together")
+    a, ldy = _norm_rows(y, width, dev, y.shape, y.dtype, what, "y")
+    g, ldg = (None, 0) if gate is None else _norm_rows(gate, width, dev, y.shape, y.dtype, what, "gate")
+    w = _whole(weight, dev, torch.float32, group, what, "weight", "groups and weight do not belong together")
     _forward_only(what, y, weight, gate)
-    _together(what, y, weight, gate)
     if _elsewhere(y):
-        with torch.cuda.device(y.device):
+        with torch.cuda.device(dev):
             return gated_norm(y, weight, gate, group=group, eps=eps, out_dtype=out_dtype)
     out = torch.empty(y.shape, dtype=out_dtype, device=y.device)
-    _lib.check(lib.jb200_gated_norm(_ptr(rows), _dt(rows), _row_stride(rows), _ptr(weight), _ptr(g), 0 if g is None else _row_stride(g), group, eps,
-                                    _ptr(out), _dt(out), N, width, _stream()), "jb200_gated_norm")
+    rc = lib.jb200_gated_norm(a, dt, ldy, w, g, ldg, group, eps, out.data_ptr(), _dt(out), y.numel() // width, width, _stream())
+    if rc:
+        _lib.check(rc, "jb200_gated_norm")
     return out
 
 
@@ -939,32 +969,32 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, w_after: torch.Tensor, w_bef
     w_before, scale: f32 (C,).  out: where x' goes, x itself for an update in place; a new tensor unless given.  Returns (x', xn)."""
     lib = _lib.load()
     what = "residual_norm"
-    rows, g = _norm_arguments(what, y, gate)
-    _need(x, torch.float32, what + ".x")
-    N, width = rows.shape
+    width = _norm_width(y, what)
+    dev, dt, f32 = y.get_device(), _dt(y), torch.float32
     if x.shape != y.shape:
         raise RuntimeError(f"{what}: x {tuple(x.shape)} and y {tuple(y.shape)} must have one shape")
-    for name, t in (("w_after", w_after), ("w_before", w_before), ("scale", scale)):
-        if t is not None and _need(t, torch.float32, f"{what}.{name}").numel() != width:
-            raise RuntimeError(f"{what}: {name} {tuple(t.shape)} does not fit rows of {width}")
+    n = y.numel()
+    px = _whole(x, dev, f32, n, what, "x", "wrong size")
+    a, ldy = _norm_rows(y, width, dev, y.shape, y.dtype, what, "y")
+    g, ldg = (None, 0) if gate is None else _norm_rows(gate, width, dev, y.shape, y.dtype, what, "gate")
+    wa, wb = _whole(w_after, dev, f32, width, what, "w_after", "does not fit the rows"), _whole(w_before, dev, f32, width, what, "w_before", "does not fit the rows")
+    sc = None if scale is None else _whole(scale, dev, f32, width, what, "scale", "does not fit the rows")
     _forward_only(what, x, y, w_after, w_before, gate, scale, out)
-    _together(what, x, y, w_after, w_before, gate, scale, out)
-    if _elsewhere(x):
-        with torch.cuda.device(x.device):
+    if _elsewhere(y):
+        with torch.cuda.device(dev):
             return residual_norm(x, y, w_after, w_before, gate=gate, scale=scale, eps=eps, out=out, out_dtype=out_dtype)
     if out is None:
-        out = torch.empty_like(x)
+        out = torch.empty(x.shape, dtype=f32, device=x.device)
     else:
-        _need(out, torch.float32, what + ".out")
         if out.shape != x.shape:
             raise RuntimeError(f"{what}: out {tuple(out.shape)} must have x's shape {tuple(x.shape)}")
-        if out.data_ptr() != x.data_ptr() and _touch(out, x):
+        if _whole(out, dev, f32, n, what, "out", "wrong size") != px and _touch(out, x):
             raise RuntimeError(f"{what}: out overlaps x without being it")
-        if any(t is not None and _touch(out, t) for t in (rows, g, w_after, w_before, scale)):
-            raise RuntimeError(f"{what}: out overlaps another argument")
+        _apart(what, "out", out, y, gate, w_after, w_before, scale)
     xn = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    _lib.check(lib.jb200_residual_norm(_ptr(x), _ptr(rows), _dt(rows), _row_stride(rows), _ptr(w_after), _ptr(g), 0 if g is None else _row_stride(g),
-                                       _ptr(scale), _ptr(w_before), eps, _ptr(out), _ptr(xn), _dt(xn), N, width, _stream()), "jb200_residual_norm")
+    rc = lib.jb200_residual_norm(px, a, dt, ldy, wa, g, ldg, sc, wb, eps, out.data_ptr(), xn.data_ptr(), _dt(xn), n // width, width, _stream())
+    if rc:
+        _lib.check(rc, "jb200_residual_norm")
     return out, xn
 
 
@@ -983,28 +1013,32 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, *, temperature=0.7, top_k
     if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise RuntimeError(f"{what}: logits must be (B, V) with contiguous rows")
     B, V = logits.shape
-    s = _lib.Sampling(_ptr(logits), _row_stride(logits), _dt(logits), V)
-    if _need(u, torch.float32, what + ".u").numel() != B:
-        raise RuntimeError(f"{what}: u must hold one number per row")
-    s.u = _ptr(u)
-    given = [logits, u]
-    for name, value, dtype, off in (("temperature", temperature, torch.float32, 0.0), ("top_k", top_k, torch.int32, 0),
-                                    ("top_p", top_p, torch.float32, 0.0), ("min_p", min_p, torch.float32, 0.0)):
-        if torch.is_tensor(value):
-            if _need(value, dtype, f"{what}.{name}").numel() != B:
-                raise RuntimeError(f"{what}: {name} must be one value or hold one per row")
-            setattr(s, name, _ptr(value))
-            given.append(value)
-        else:
-            value = off if value is None else value
-            setattr(s, name + "_all", min(max(int(value), 0), 2 ** 31 - 1) if dtype is torch.int32 else float(value))
-    _together(what, *given)
-    if B > 1 and logits.stride(0) < V:
-        raise RuntimeError(f"{what}: rows of logits overlap (stride {logits.stride(0)}, {V} columns)")
+    dev, ld, f32 = logits.get_device(), logits.stride(0) if logits.shape[0] > 1 else logits.shape[1], torch.float32
+    if ld < V:
+        raise RuntimeError(f"{what}: rows of logits overlap (stride {ld}, {V} columns)")
+    s = _lib.Sampling(logits.data_ptr(), ld, _dt(logits), V, _whole(u, dev, f32, B, what, "u", "one number per row is needed"))
+    if torch.is_tensor(temperature):
+        s.temperature = _whole(temperature, dev, f32, B, what, "temperature", "one value or one per row")
+    else:
+        s.temperature_all = 0.0 if temperature is None else temperature
+    if torch.is_tensor(top_k):
+        s.top_k = _whole(top_k, dev, torch.int32, B, what, "top_k", "one value or one per row")
+    elif top_k is not None:
+        s.top_k_all = min(max(int(top_k), 0), 2 ** 31 - 1)
+    if torch.is_tensor(top_p):
+        s.top_p = _whole(top_p, dev, f32, B, what, "top_p", "one value or one per row")
+    elif top_p is not None:
+        s.top_p_all = top_p
+    if torch.is_tensor(min_p):
+        s.min_p = _whole(min_p, dev, f32, B, what, "min_p", "one value or one per row")
+    elif min_p is not None:
+        s.min_p_all = min_p
     if _elsewhere(logits):
-        with torch.cuda.device(logits.device):
+        with torch.cuda.device(dev):
             return sample_rows(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, want_prob=want_prob)
     out = torch.empty((B, 1), dtype=torch.int64, device=logits.device)
-    prob = torch.empty((B,), dtype=torch.float32, device=logits.device) if want_prob else None
-    _lib.check(lib.jb200_sample_rows(ctypes.byref(s), B, _ptr(out), _ptr(prob), _stream()), "jb200_sample_rows")
+    prob = torch.empty((B,), dtype=f32, device=logits.device) if want_prob else None
+    rc = lib.jb200_sample_rows(ctypes.byref(s), B, out.data_ptr(), None if prob is None else prob.data_ptr(), _stream())
+    if rc:
+        _lib.check(rc, "jb200_sample_rows")
     return (out, prob) if want_prob else out
