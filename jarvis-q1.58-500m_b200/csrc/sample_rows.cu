@@ -8,11 +8,14 @@
 //   min-p:  w_i >= min_p
 //   draw:   the first i whose running sum over what is left exceeds u times the whole
 //
-// All of them ask "which token covers position z of the running sum", once with every weight 1 (top-k).  Weights are taken in f64 and held as
-// integers of 2^-45 of the largest one's, so that sums do not depend on the order of the atomics that form them, and a token that the exact
-// sums choose is missed only where u lies within some 1e-12 of a border.  A CTA has a row.  A histogram of counts and sums over 2048 bins of
-// 1/32 of an e-fold finds the bin that covers z; its tokens (some hundred) are ranked by comparison with one another.  A bin of more than
-// 256 tokens is first cut by the bits of their keys, 512 parts a time.
+// All of them ask "which token covers position z of the running sum", top-k with every weight 1.  Weights are taken in f64 and held as integers of
+// 2^-45 of the largest one's, so that sums do not depend on the order of the atomics that form them, and a token that the exact sums choose is
+// missed only where u lies within some 1e-12 of a border.  A cluster of CTAs has a row, a slice each, with as many CTAs as keep the SMs busy.  A
+// histogram of the sums (for top-k of the counts, too) over 2048 bins of 1/32 of an e-fold finds the bin that covers z; its tokens (some hundred) are ranked
+// by comparison with one another.  A bin of more than 256 tokens is first cut by the bits of their keys, 512 parts a time.  Every CTA
+// counts and lists its slice in its own memory; the first one reads the others' and searches, the others read what it found.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "launchers.h"
 
@@ -27,6 +30,7 @@ constexpr int BINS = 2048;              // 1/32 of an e-fold each; the last: eve
 constexpr float BINS_A_FOLD = 32.f;
 constexpr int FINE = 512;
 constexpr int LIST = 256;
+constexpr int TABLE = 64;               // 2^-(j / 64)
 
 struct Sampling {
   const void* logits;
@@ -59,6 +63,8 @@ struct Smem {
   u64 above, weight;                              // the sum over keys above, the weight of one of the ties
   int bin, id;
   u64 sum;
+  uint32_t from, to;                              // keys in question
+  double table[TABLE];
 };
 
 // order-preserving map float -> uint32; NaN is treated as -inf, -0 as 0
@@ -74,16 +80,16 @@ __device__ __forceinline__ float widen(T x) { return x; }
 template <>
 __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// f(id, value) for every element of the row, 16 bytes a load where they are aligned
-template <typename T, typename F>
-__device__ __forceinline__ void every(const T* row, int V, F&& f) {
+// f(id, value) for every element of this CTA's slice of the row, 16 bytes a load where they are aligned
+template <typename T, int CTAS, typename F>
+__device__ __forceinline__ void every(const T* row, int V, int rank, F&& f) {
   constexpr int PER = 16 / sizeof(T);
   const int head = min(V, int((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / int(sizeof(T)));
   const int vectors = (V - head) / PER, tail = head + vectors * PER;
   const uint4* body = reinterpret_cast<const uint4*>(row + head);
-  if (int(threadIdx.x) < head) f(int(threadIdx.x), widen(row[threadIdx.x]));
-#pragma unroll 2
-  for (int i = threadIdx.x; i < vectors; i += THREADS) {
+  if (rank == 0 && int(threadIdx.x) < head) f(int(threadIdx.x), widen(row[threadIdx.x]));
+#pragma unroll 4
+  for (int i = rank * THREADS + threadIdx.x; i < vectors; i += CTAS * THREADS) {
     const uint4 x = __ldg(body + i);
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
     const int id = head + i * PER;
@@ -97,20 +103,46 @@ __device__ __forceinline__ void every(const T* row, int V, F&& f) {
       }
     }
   }
-  if (tail + int(threadIdx.x) < V) f(tail + int(threadIdx.x), widen(row[tail + threadIdx.x]));
+  if (rank == CTAS - 1 && tail + int(threadIdx.x) < V) f(tail + int(threadIdx.x), widen(row[tail + threadIdx.x]));
+}
+
+// All CTAs of the row, with what they wrote
+template <int CTAS>
+__device__ __forceinline__ void meet() {
+  if constexpr (CTAS == 1) __syncthreads();
+  else cooperative_groups::this_cluster().sync();
+}
+
+// x as f64 (a subnormal x as some other number of 1e-38: no weight shows it); the conversion instruction runs at an eighth of this one's rate
+__device__ __forceinline__ double to_f64(float x) {
+  const uint32_t b = __float_as_uint(x), m = b & 0x7fffffffu;
+  return __hiloint2double(int((b & 0x80000000u) | ((m >> 3) + 0x38000000u)), int(m << 29));
 }
 
 struct Row {
   float top, fold;                      // the largest logit; bins an e-fold of the row's temperature
-  double rate;                          // 1 / temperature
-  double unit;                          // 2^shift
+  double top64, rate;                   // 64 log2(e) / temperature
+  int shift;
+  const double* table;
 
   __device__ __forceinline__ int bin(float x) const {
     const float d = x == top ? 0.f : (top - x) * fold;
     return d < float(BINS - 1) ? int(d) : BINS - 1;            // NaN and infinities are the last bin's
   }
-  __device__ __forceinline__ double ratio(float x) const { return x == top ? 1.0 : exp((double(x) - double(top)) * rate); }
-  __device__ __forceinline__ u64 weight(float x) const { return __double2ull_rn(ratio(x) * unit); }
+  // 2^shift exp((x - top) / temperature) as a double, of an x of any bin but the last: 2^-(n / 64) from the table, the rest from its series (the fifth
+  // term is below 2^-44)
+  __device__ __forceinline__ double scaled(float x) const {
+    if (x == top) return __hiloint2double((1023 + shift) << 20, 0);
+    constexpr double C1 = -0.6931471805599453 / 64, C2 = C1 * C1 / 2, C3 = C1 * C1 * C1 / 6, C4 = C1 * C1 * C1 * C1 / 24, MAGIC = 6755399441055744.0;
+    const double t = (top64 - to_f64(x)) * rate, m = t + MAGIC, r = t - (m - MAGIC);
+    const int n = __double2loint(m);
+    const double w = fma(r, fma(r, fma(r, fma(r, C4, C3), C2), C1), 1.0) * table[n & (TABLE - 1)];
+    const int hi = __double2hiint(w) + ((shift - (n >> 6)) << 20);
+    return __hiloint2double(hi, __double2loint(w));
+  }
+  __device__ __forceinline__ u64 weight(float x) const {       // to the nearest integer: below 2^52 that is what the sum with 2^52 leaves
+    return bin(x) == BINS - 1 ? 0 : __double_as_longlong(scaled(x) + 4503599627370496.0) & 0xfffffffffffffull;
+  }
 };
 
 __device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, u64 w) {
@@ -176,64 +208,135 @@ __device__ int covering(const uint32_t* count, const uint32_t* lo, const uint32_
   return bin;
 }
 
-// The key that covers position z of the running sum (of the running count): sm.key, .above, .weight, .ties; draw: also sm.id, the token.
-template <typename T, bool BY_COUNT>
-__device__ void search(const T* row, int V, const Row& r, Smem& sm, u64 z, bool draw) {
+// CTA c's memory, to be read
+template <int CTAS>
+__device__ __forceinline__ Smem& of_cta(Smem& sm, int c) {
+  if constexpr (CTAS == 1) return sm;
+  else return *cooperative_groups::this_cluster().map_shared_rank(&sm, c);
+}
+
+// The first CTA's bins: the sums over all CTAs
+template <int CTAS, int N_BINS, typename C, typename L, typename H>
+__device__ __forceinline__ void join(Smem& sm, C&& count, L&& lo, H&& hi, bool counts) {
+  if constexpr (CTAS > 1) {
+    for (int i = threadIdx.x; i < N_BINS; i += THREADS) {
+      u64 sum = 0;
+      uint32_t n = 0;
+#pragma unroll
+      for (int c = 0; c < CTAS; ++c) {
+        Smem& other = of_cta<CTAS>(sm, c);
+        sum += (u64(hi(other)[i]) << 32) + lo(other)[i];
+        if (counts) n += count(other)[i];
+      }
+      lo(sm)[i] = uint32_t(sum);
+      hi(sm)[i] = uint32_t(sum >> 32);
+      count(sm)[i] = n;
+    }
+    __syncthreads();
+  }
+}
+
+// The key that covers position z of the running sum (of the running count): the first CTA's .key, .above, .weight, .ties; draw: also its .id, the token.
+// z is the first CTA's to know.
+template <typename T, int CTAS, bool BY_COUNT>
+__device__ void search(const T* row, int V, int rank, const Row& r, Smem& sm, u64 z, bool draw) {
   const int tid = threadIdx.x;
-  const int bin = covering<BINS, BY_COUNT>(sm.count, sm.lo, sm.hi, sm, z);
-  u64 above = (u64(sm.hi[bin]) << 32) + sm.lo[bin];
-  uint32_t cabove = sm.count[bin];
-  uint32_t from = 0, to = 0xffffffffu;              // keys in question, beside the bin
+  const Smem& first = of_cta<CTAS>(sm, 0);
+  u64 above = 0;
+  uint32_t cabove = 0;
+  if (rank == 0) {
+    const int bin = covering<BINS, BY_COUNT>(sm.count, sm.lo, sm.hi, sm, z);
+    above = (u64(sm.hi[bin]) << 32) + sm.lo[bin];
+    cabove = sm.count[bin];
+    if (tid == 0) { sm.from = 0; sm.to = 0xffffffffu; sm.bin = bin; }
+  }
   for (;;) {
     if (tid == 0) { sm.n = 0; sm.key_min = 0xffffffffu; sm.key_max = 0; }
-    __syncthreads();
-    every(row, V, [&](int id, float x) {
+    meet<CTAS>();
+    const int bin = first.bin;
+    const uint32_t low = first.from, high = first.to;
+    every<T, CTAS>(row, V, rank, [&](int id, float x) {
       if (r.bin(x) != bin) return;
       const uint32_t key = key_of(x);
-      if (key < from || key > to) return;
+      if (key < low || key > high) return;
       const uint32_t slot = atomicAdd(&sm.n, 1u);
       if (slot < LIST) { sm.list[slot].key = key; sm.list[slot].id = id; }
       atomicMin(&sm.key_min, key);
       atomicMax(&sm.key_max, key);
     });
-    __syncthreads();
-    const uint32_t n = sm.n;
-    from = sm.key_min;
-    to = sm.key_max;
-    if (n <= LIST) break;
-    if (from == to) {                               // one key of many tokens
-      const u64 w = r.weight(value_of(to));
-      __syncthreads();
-      if (tid == 0) { sm.key = to; sm.ties = n; sm.above = above; sm.weight = w; }
-      if (draw) {                                   // its tokens in order of ids: every thread counts those of a piece of the row
-        const int piece = (V + THREADS - 1) / THREADS, a = min(V, tid * piece), b = min(V, a + piece);
-        uint32_t mine = 0;
-        for (int i = a; i < b; ++i) mine += key_of(widen(row[i])) == to;
-        uint32_t incl = mine;
+    meet<CTAS>();
+    uint32_t n = 0, from = 0xffffffffu, to = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
-          if ((tid & 31) >= o) incl += x;
+    for (int c = 0; c < CTAS; ++c) {
+      const Smem& other = of_cta<CTAS>(sm, c);
+      n += other.n;
+      from = min(from, other.key_min);
+      to = max(to, other.key_max);
+    }
+    if (n <= LIST) {
+      if (rank == 0) {                              // the tokens of all slices, ranked by comparison
+        Item mine;
+        if (tid < int(n)) {
+          int c = 0, at = tid;
+          if constexpr (CTAS > 1)
+            for (; at >= int(of_cta<CTAS>(sm, c).n); ++c) at -= int(of_cta<CTAS>(sm, c).n);
+          mine = of_cta<CTAS>(sm, c).list[at];
+          mine.w = r.weight(value_of(mine.key));
         }
-        if ((tid & 31) == 31) sm.warp_count[tid >> 5] = incl;
         __syncthreads();
-        uint32_t before = incl - mine;
-        for (int i = 0; i < (tid >> 5); ++i) before += sm.warp_count[i];
-        const uint32_t want = uint32_t((z - above) / w);
-        if (want >= before && want < before + mine) {
-          uint32_t left = want - before;
-          for (int i = a; i < b; ++i)
-            if (key_of(widen(row[i])) == to && left-- == 0) { sm.id = i; break; }
+        if (tid < int(n)) sm.list[tid] = mine;
+        __syncthreads();
+        if (tid < int(n)) {
+          u64 over = 0;
+          uint32_t higher = 0, ties = 0, place = 0;
+          for (int j = 0; j < int(n); ++j) {
+            const Item it = sm.list[j];
+            if (it.key > mine.key) { over += it.w; ++higher; }
+            else if (it.key == mine.key) { ++ties; place += it.id < mine.id; }
+          }
+          const u64 start = BY_COUNT ? cabove + higher : above + over;
+          const u64 size = BY_COUNT ? ties : mine.w * ties;
+          if (start <= z && z - start < size) {
+            if (place == 0) { sm.key = mine.key; sm.ties = ties; sm.above = above + over; sm.weight = mine.w; }
+            if (draw && uint32_t((z - start) / mine.w) == place) sm.id = mine.id;
+          }
         }
       }
-      __syncthreads();
-      return;
+      break;
+    }
+    if (from == to) {                               // one key of many tokens
+      if (rank == 0) {
+        const u64 w = r.weight(value_of(to));
+        if (tid == 0) { sm.key = to; sm.ties = n; sm.above = above; sm.weight = w; }
+        if (draw) {                                 // its tokens in order of ids: every thread counts those of a piece of the row
+          const int piece = (V + THREADS - 1) / THREADS, a = min(V, tid * piece), b = min(V, a + piece);
+          uint32_t mine = 0;
+          for (int i = a; i < b; ++i) mine += key_of(widen(row[i])) == to;
+          uint32_t incl = mine;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
+            if ((tid & 31) >= o) incl += x;
+          }
+          if ((tid & 31) == 31) sm.warp_count[tid >> 5] = incl;
+          __syncthreads();
+          uint32_t before = incl - mine;
+          for (int i = 0; i < (tid >> 5); ++i) before += sm.warp_count[i];
+          const uint32_t want = uint32_t((z - above) / w);
+          if (want >= before && want < before + mine) {
+            uint32_t left = want - before;
+            for (int i = a; i < b; ++i)
+              if (key_of(widen(row[i])) == to && left-- == 0) { sm.id = i; break; }
+          }
+        }
+      }
+      break;
     }
     int cut = 0;
     while (((to - from) >> cut) >= FINE) ++cut;
     for (int i = tid; i < FINE; i += THREADS) sm.fcount[i] = sm.flo[i] = sm.fhi[i] = 0;
     __syncthreads();
-    every(row, V, [&](int id, float x) {
+    every<T, CTAS>(row, V, rank, [&](int id, float x) {
       if (r.bin(x) != bin) return;
       const uint32_t key = key_of(x);
       if (key < from || key > to) return;
@@ -241,40 +344,22 @@ __device__ void search(const T* row, int V, const Row& r, Smem& sm, u64 z, bool 
       atomicAdd(&sm.fcount[at], 1u);
       add64(&sm.flo[at], &sm.fhi[at], r.weight(x));
     });
-    __syncthreads();
-    running_sums<FINE>(sm.fcount, sm.flo, sm.fhi, sm, above, cabove);
-    const int at = covering<FINE, BY_COUNT>(sm.fcount, sm.flo, sm.fhi, sm, z);
-    above = (u64(sm.fhi[at]) << 32) + sm.flo[at];
-    cabove = sm.fcount[at];
-    const uint32_t high = to - (uint32_t(at) << cut), size = (1u << cut) - 1u;
-    from = high - from > size ? high - size : from;
-    to = high;
-    __syncthreads();
-  }
-  const int n = int(sm.n);
-  Item mine;
-  if (tid < n) {
-    mine = sm.list[tid];
-    mine.w = r.weight(value_of(mine.key));
-    sm.list[tid].w = mine.w;
-  }
-  __syncthreads();
-  if (tid < n) {
-    u64 over = 0;
-    uint32_t higher = 0, ties = 0, rank = 0;
-    for (int j = 0; j < n; ++j) {
-      const Item it = sm.list[j];
-      if (it.key > mine.key) { over += it.w; ++higher; }
-      else if (it.key == mine.key) { ++ties; rank += it.id < mine.id; }
-    }
-    const u64 first = BY_COUNT ? cabove + higher : above + over;
-    const u64 size = BY_COUNT ? ties : mine.w * ties;
-    if (first <= z && z - first < size) {
-      if (rank == 0) { sm.key = mine.key; sm.ties = ties; sm.above = above + over; sm.weight = mine.w; }
-      if (draw && uint32_t((z - first) / mine.w) == rank) sm.id = mine.id;
+    meet<CTAS>();
+    if (rank == 0) {
+      join<CTAS, FINE>(sm, [](Smem& x) { return x.fcount; }, [](Smem& x) { return x.flo; }, [](Smem& x) { return x.fhi; }, true);
+      running_sums<FINE>(sm.fcount, sm.flo, sm.fhi, sm, above, cabove);
+      const int at = covering<FINE, BY_COUNT>(sm.fcount, sm.flo, sm.fhi, sm, z);
+      above = (u64(sm.fhi[at]) << 32) + sm.flo[at];
+      cabove = sm.fcount[at];
+      if (tid == 0) {
+        const uint32_t top = to - (uint32_t(at) << cut), size = (1u << cut) - 1u;
+        sm.from = top - from > size ? top - size : from;
+        sm.to = top;
+        sm.bin = bin;
+      }
     }
   }
-  __syncthreads();
+  meet<CTAS>();                                     // everybody has read what this search used
 }
 
 __device__ __forceinline__ u64 share(double part, u64 whole) {
@@ -283,15 +368,16 @@ __device__ __forceinline__ u64 share(double part, u64 whole) {
   return min(z < 1.8e19 ? __double2ull_rd(z) : ~0ull, whole - 1);
 }
 
-template <typename T>
+template <typename T, int CTAS>
 __global__ void __launch_bounds__(THREADS) sample_rows_kernel(Sampling p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
-  const int tid = threadIdx.x, V = p.V;
-  const size_t at = blockIdx.x;
-  if (tid == 0) sm.best = 0;
+  const int tid = threadIdx.x, V = p.V, rank = CTAS == 1 ? 0 : int(blockIdx.x % CTAS);
+  const size_t at = blockIdx.x / CTAS;
+  if (tid == 0) { sm.best = 0; sm.sum = 0; }
   for (int i = tid; i < BINS; i += THREADS) sm.count[i] = sm.lo[i] = sm.hi[i] = 0;
-  __syncthreads();
+  if (tid < TABLE) sm.table[tid] = exp2(-double(tid) / TABLE);
+  meet<CTAS>();
   pdl_wait();
   pdl_trigger();
   const T* row = static_cast<const T*>(p.logits) + at * p.ld;
@@ -300,74 +386,98 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(Sampling p) {
   const int top_k = p.top_k != nullptr ? p.top_k[at] : p.top_k_all;
 
   u64 best = 0;
-  every(row, V, [&](int id, float x) { best = max(best, (u64(key_of(x)) << 32) | uint32_t(~id)); });
+  every<T, CTAS>(row, V, rank, [&](int id, float x) { best = max(best, (u64(key_of(x)) << 32) | uint32_t(~id)); });
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   if ((tid & 31) == 0) atomicMax(&sm.best, best);
-  __syncthreads();
-  best = sm.best;
+  meet<CTAS>();
+#pragma unroll
+  for (int c = 0; c < CTAS; ++c) best = max(best, of_cta<CTAS>(sm, c).best);
   Row r;
   r.top = value_of(uint32_t(best >> 32));
   const bool nothing = r.top == -INFINITY;
   if (!(temperature > 0.f) || nothing) {              // the largest, lowest id among equals; no logit above -inf: token 0 with probability 0
-    if (tid == 0) {
+    if (rank == 0 && tid == 0) {
       p.token[at] = nothing ? 0 : int64_t(~uint32_t(best));
       if (p.prob != nullptr) p.prob[at] = nothing ? 0.f : 1.f;
     }
+    meet<CTAS>();                                     // a CTA's memory is there until everybody has read it
     return;
   }
-  r.rate = 1.0 / fmax(double(temperature), 1e-5);
-  r.fold = float(r.rate) * BINS_A_FOLD;
-  r.unit = double(1ull << p.shift);
+  const double rate = 1.0 / fmax(double(temperature), 1e-5);
+  r.fold = float(rate) * BINS_A_FOLD;
+  r.top64 = to_f64(r.top);
+  r.rate = rate * (64 * 1.4426950408889634);
+  r.shift = p.shift;
+  r.table = sm.table;
+  const bool count = top_k > 0 && top_k < V;
 
-  every(row, V, [&](int id, float x) {
+  every<T, CTAS>(row, V, rank, [&](int id, float x) {
     const int b = r.bin(x);
-    atomicAdd(&sm.count[b], 1u);
+    if (count) atomicAdd(&sm.count[b], 1u);
     if (b < BINS - 1) {
-      const u64 w = r.weight(x);
+      const u64 w = __double_as_longlong(r.scaled(x) + 4503599627370496.0) & 0xfffffffffffffull;
       if (w) add64(&sm.lo[b], &sm.hi[b], w);
     }
   });
-  __syncthreads();
-  // the last bin's weights are 0, so that the sum before it is the whole
-  running_sums<BINS>(sm.count, sm.lo, sm.hi, sm, 0, 0);
-  u64 whole = (u64(sm.hi[BINS - 1]) << 32) + sm.lo[BINS - 1];
-  if (top_k > 0 && top_k < V) {
-    search<T, true>(row, V, r, sm, u64(top_k - 1), false);
-    whole = sm.above + sm.weight * sm.ties;
-    __syncthreads();
+  meet<CTAS>();
+  u64 whole = 0, left = 0;
+  if (rank == 0) {
+    join<CTAS, BINS>(sm, [](Smem& x) { return x.count; }, [](Smem& x) { return x.lo; }, [](Smem& x) { return x.hi; }, count);
+    // the last bin's weights are 0, so that the sum before it is the whole
+    running_sums<BINS>(sm.count, sm.lo, sm.hi, sm, 0, 0);
+    whole = (u64(sm.hi[BINS - 1]) << 32) + sm.lo[BINS - 1];
   }
-  u64 left = whole;
+  if (count) {
+    search<T, CTAS, true>(row, V, rank, r, sm, u64(top_k - 1), false);
+    whole = sm.above + sm.weight * sm.ties;
+  }
+  left = whole;
   if (top_p > 0.f && top_p < 1.f) {
     const u64 z = share(double(top_p), whole);
-    search<T, false>(row, V, r, sm, z, false);
-    left = sm.above + ((z - sm.above) / sm.weight + 1) * sm.weight;
-    __syncthreads();
+    search<T, CTAS, false>(row, V, rank, r, sm, z, false);
+    if (rank == 0) left = sm.above + ((z - sm.above) / sm.weight + 1) * sm.weight;
   }
   if (min_p > 0.f) {
     // bins well above the border are in, those well below out; weights decide in the three around it (the bins' borders are rounded)
-    const double d = -log(double(min_p)) * double(BINS_A_FOLD);
-    const int mid = d < double(BINS - 3) ? max(int(d), 0) : BINS - 3, first = max(mid - 1, 0), last = mid + 1;
-    if (tid == 0) sm.sum = (u64(sm.hi[first]) << 32) + sm.lo[first];
-    __syncthreads();
+    const double d = -log(double(min_p)) * double(BINS_A_FOLD), least = double(min_p) * double(1ull << p.shift);
+    const int mid = d < double(BINS - 3) ? max(int(d), 0) : BINS - 3, low = max(mid - 1, 0), high = mid + 1;
     u64 mine = 0;
-    every(row, V, [&](int id, float x) {
+    every<T, CTAS>(row, V, rank, [&](int id, float x) {
       const int b = r.bin(x);
-      if (b >= first && b <= last) {
-        const double w = r.ratio(x);
-        if (w >= double(min_p)) mine += __double2ull_rn(w * r.unit);
+      if (b >= low && b <= high) {
+        const double w = r.scaled(x);
+        if (w >= least) mine += __double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
       }
     });
     if (mine) atomicAdd(&sm.sum, mine);
-    __syncthreads();
-    left = max(min(left, sm.sum), u64(1) << p.shift);           // min_p beyond 1 leaves the largest
-    __syncthreads();
+    meet<CTAS>();
+    if (rank == 0) {
+      u64 sum = (u64(sm.hi[low]) << 32) + sm.lo[low];
+#pragma unroll
+      for (int c = 0; c < CTAS; ++c) sum += of_cta<CTAS>(sm, c).sum;
+      left = max(min(left, sum), u64(1) << p.shift);           // min_p beyond 1 leaves the largest
+    }
   }
-  const double u = double(p.u[at]);
-  search<T, false>(row, V, r, sm, share(u, left), true);
-  if (tid == 0) {
+  search<T, CTAS, false>(row, V, rank, r, sm, rank == 0 ? share(double(p.u[at]), left) : 0, true);
+  if (rank == 0 && tid == 0) {
     p.token[at] = sm.id;
-    if (p.prob != nullptr) p.prob[at] = float(r.ratio(value_of(sm.key)) * r.unit / double(left));
+    if (p.prob != nullptr) p.prob[at] = float(r.scaled(value_of(sm.key)) / double(left));
   }
+}
+
+template <typename T>
+void launch_rows(const Sampling& p, int n_rows, cudaStream_t stream) {
+  // CTAs a row: as many as two a SM leave room for, slices of 4096 tokens or more
+  const int most = 2 * sm_count() / n_rows, wide = p.V / 4096;
+  auto start = [&](auto kernel, int ctas) {
+    if (ctas == 1) launch_dep(kernel, n_rows, THREADS, sizeof(Smem), stream, p);
+    else launch_dep_cluster(kernel, n_rows * ctas, THREADS, sizeof(Smem), ctas, stream, p);
+  };
+  const int ctas = most < wide ? most : wide;
+  if (ctas >= 8) start(sample_rows_kernel<T, 8>, 8);
+  else if (ctas >= 4) start(sample_rows_kernel<T, 4>, 4);
+  else if (ctas >= 2) start(sample_rows_kernel<T, 2>, 2);
+  else start(sample_rows_kernel<T, 1>, 1);
 }
 
 }  // namespace
@@ -380,6 +490,7 @@ int launch_sample_rows(const jb200_sampling* s, int n_rows, int64_t* token, floa
   if (n_rows == 0) return JB200_OK;
   JB_REQUIRE(s->logits && s->u && token, "sample_rows: null pointer");
   Sampling p;
+  static_assert(sizeof(Smem) <= 48 * 1024, "no larger than a launch may ask for without more ado");
   p.logits = s->logits; p.ld = size_t(s->ld); p.V = s->V;
   int bits = 0;
   while ((1 << bits) < s->V) ++bits;
@@ -387,13 +498,8 @@ int launch_sample_rows(const jb200_sampling* s, int n_rows, int64_t* token, floa
   p.u = s->u; p.temperature = s->temperature; p.top_k = s->top_k; p.top_p = s->top_p; p.min_p = s->min_p;
   p.temperature_all = s->temperature_all; p.top_k_all = s->top_k_all; p.top_p_all = s->top_p_all; p.min_p_all = s->min_p_all;
   p.token = token; p.prob = prob;
-  if (s->logits_dtype == 0) {
-    JB_MAX_SMEM(sample_rows_kernel<float>, sizeof(Smem));
-    launch_dep(sample_rows_kernel<float>, n_rows, THREADS, sizeof(Smem), stream, p);
-  } else {
-    JB_MAX_SMEM(sample_rows_kernel<__nv_bfloat16>, sizeof(Smem));
-    launch_dep(sample_rows_kernel<__nv_bfloat16>, n_rows, THREADS, sizeof(Smem), stream, p);
-  }
+  if (s->logits_dtype == 0) launch_rows<float>(p, n_rows, stream);
+  else launch_rows<__nv_bfloat16>(p, n_rows, stream);
   JB_LAUNCH_CHECK("sample_rows_kernel");
   return JB200_OK;
 }
