@@ -25,7 +25,7 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int THREADS = 1024;
+constexpr int THREADS = 512;
 constexpr int BINS = 2048;              // 1/32 of an e-fold each; the last: everything 64 e-folds or more below the largest, whose weight is 0
 constexpr float BINS_A_FOLD = 32.f;
 constexpr int FINE = 512;
@@ -409,38 +409,57 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(Sampling p) {
   r.rate = rate * (64 * 1.4426950408889634);
   r.shift = p.shift;
   r.table = sm.table;
-  const bool count = top_k > 0 && top_k < V;
-
+  const bool count = top_k > 0 && top_k < V, nucleus = top_p > 0.f && top_p < 1.f;
+  // min-p: bins well above the border are in, those well below out; weights decide in the three around it (the bins' borders are rounded)
+  int low = 0, high = BINS - 2;
+  if (min_p > 0.f) {
+    const double d = -log(double(min_p)) * double(BINS_A_FOLD);
+    const int mid = d < double(BINS - 3) ? max(int(d), 0) : BINS - 3;
+    low = max(mid - 1, 0);
+    high = mid + 1;
+  }
+  u64 whole = 0, left = 0;
+  int last = nucleus ? BINS - 2 : high;               // bins from here on have no say: only a nucleus needs the sum over what min-p cuts
+  if (count) {
+    // the k-th largest by counts alone, so that nobody takes weights of what lies below it
+    every<T, CTAS>(row, V, rank, [&](int id, float x) { atomicAdd(&sm.count[r.bin(x)], 1u); });
+    meet<CTAS>();
+    if (rank == 0) {
+      join<CTAS, BINS>(sm, [](Smem& x) { return x.count; }, [](Smem& x) { return x.lo; }, [](Smem& x) { return x.hi; }, true);
+      running_sums<BINS>(sm.count, sm.lo, sm.hi, sm, 0, 0);
+    }
+    search<T, CTAS, true>(row, V, rank, r, sm, u64(top_k - 1), false);
+    last = min(last, of_cta<CTAS>(sm, 0).bin);
+    meet<CTAS>();
+    for (int i = tid; i < BINS; i += THREADS) sm.lo[i] = sm.hi[i] = 0;
+    __syncthreads();
+  }
   every<T, CTAS>(row, V, rank, [&](int id, float x) {
     const int b = r.bin(x);
-    if (count) atomicAdd(&sm.count[b], 1u);
-    if (b < BINS - 1) {
+    if (b <= last) {
       const u64 w = __double_as_longlong(r.scaled(x) + 4503599627370496.0) & 0xfffffffffffffull;
       if (w) add64(&sm.lo[b], &sm.hi[b], w);
     }
   });
   meet<CTAS>();
-  u64 whole = 0, left = 0;
   if (rank == 0) {
-    join<CTAS, BINS>(sm, [](Smem& x) { return x.count; }, [](Smem& x) { return x.lo; }, [](Smem& x) { return x.hi; }, count);
+    join<CTAS, BINS>(sm, [](Smem& x) { return x.count; }, [](Smem& x) { return x.lo; }, [](Smem& x) { return x.hi; }, false);
     // the last bin's weights are 0, so that the sum before it is the whole
     running_sums<BINS>(sm.count, sm.lo, sm.hi, sm, 0, 0);
     whole = (u64(sm.hi[BINS - 1]) << 32) + sm.lo[BINS - 1];
-  }
-  if (count) {
-    search<T, CTAS, true>(row, V, rank, r, sm, u64(top_k - 1), false);
-    whole = sm.above + sm.weight * sm.ties;
+    if (count) {                                      // of the k-th's bin what is not below it
+      const int bin = sm.bin;
+      whole = (u64(sm.hi[bin]) << 32) + sm.lo[bin] + sm.above + sm.weight * sm.ties;
+    }
   }
   left = whole;
-  if (top_p > 0.f && top_p < 1.f) {
+  if (nucleus) {
     const u64 z = share(double(top_p), whole);
     search<T, CTAS, false>(row, V, rank, r, sm, z, false);
     if (rank == 0) left = sm.above + ((z - sm.above) / sm.weight + 1) * sm.weight;
   }
   if (min_p > 0.f) {
-    // bins well above the border are in, those well below out; weights decide in the three around it (the bins' borders are rounded)
-    const double d = -log(double(min_p)) * double(BINS_A_FOLD), least = double(min_p) * double(1ull << p.shift);
-    const int mid = d < double(BINS - 3) ? max(int(d), 0) : BINS - 3, low = max(mid - 1, 0), high = mid + 1;
+    const double least = double(min_p) * double(1ull << p.shift);
     u64 mine = 0;
     every<T, CTAS>(row, V, rank, [&](int id, float x) {
       const int b = r.bin(x);
