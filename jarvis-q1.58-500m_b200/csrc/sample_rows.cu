@@ -10,10 +10,11 @@
 //
 // All of them ask "which token covers position z of the running sum", top-k with every weight 1.  Weights are taken in f64 and held as integers of
 // 2^-45 of the largest one's, so that sums do not depend on the order of the atomics that form them, and a token that the exact sums choose is
-// missed only where u lies within some 1e-12 of a border.  A cluster of CTAs has a row, a slice each, with as many CTAs as keep the SMs busy.  A
-// histogram of the sums (for top-k of the counts, too) over 2048 bins of 1/32 of an e-fold finds the bin that covers z; its tokens (some hundred) are ranked
-// by comparison with one another.  A bin of more than 256 tokens is first cut by the bits of their keys, 512 parts a time.  Every CTA
-// counts and lists its slice in its own memory; the first one reads the others' and searches, the others read what it found.
+// missed only where u lies within some 1e-12 of a border.  A cluster of CTAs has a row, a slice each (in shared memory where it fits), with as many CTAs as
+// keep the SMs busy.  A histogram of the sums (for top-k of the counts) over 2048 bins of 1/32 of an e-fold finds the bin that covers z.  The
+// tokens of a bin, up to 256, are ranked by comparison with one another; where there are more they are first cut into 512 parts of their order, logit
+// then id, until there are not.  Every CTA counts and lists its slice in its own memory; the first one reads the others' and searches, the others
+// read what it found.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -35,7 +36,7 @@ constexpr int TABLE = 64;               // 2^-(j / 64)
 struct Sampling {
   const void* logits;
   size_t ld;
-  int V, shift;                         // weights are multiples of 2^-shift
+  int V, ids, shift, staged;            // bits of an id; weights are multiples of 2^-shift; slices are kept in shared memory
   const float *u, *temperature, *top_p, *min_p;
   const int32_t* top_k;
   float temperature_all, top_p_all, min_p_all;
@@ -45,8 +46,7 @@ struct Sampling {
 };
 
 struct Item {
-  uint32_t key;
-  int id;
+  u64 place;                            // what the order goes by, larger first: the logit's key, then the id from the end
   u64 w;
 };
 
@@ -57,13 +57,11 @@ struct Smem {
   u64 warp_sum[THREADS / 32];
   uint32_t warp_count[THREADS / 32];
   u64 best;                                       // (key, ~id) of the largest
-  uint32_t n, key_min, key_max;
-  // what a search leaves
-  uint32_t key, ties;
-  u64 above, weight;                              // the sum over keys above, the weight of one of the ties
-  int bin, id;
+  uint32_t n;
+  int bin, cut;                                   // what is searched next: of this bin the places from..to; cut: in parts of 2^cut of them, < 0: one by one
+  u64 from, to;
+  u64 place, above, weight;                       // what a search leaves: the token that covers z, the sum before it, its weight
   u64 sum;
-  uint32_t from, to;                              // keys in question
   double table[TABLE];
 };
 
@@ -80,31 +78,46 @@ __device__ __forceinline__ float widen(T x) { return x; }
 template <>
 __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// f(id, value) for every element of this CTA's slice of the row, 16 bytes a load where they are aligned
-template <typename T, int CTAS, typename F>
-__device__ __forceinline__ void every(const T* row, int V, int rank, F&& f) {
-  constexpr int PER = 16 / sizeof(T);
-  const int head = min(V, int((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / int(sizeof(T)));
-  const int vectors = (V - head) / PER, tail = head + vectors * PER;
-  const uint4* body = reinterpret_cast<const uint4*>(row + head);
-  if (rank == 0 && int(threadIdx.x) < head) f(int(threadIdx.x), widen(row[threadIdx.x]));
-#pragma unroll 4
-  for (int i = rank * THREADS + threadIdx.x; i < vectors; i += CTAS * THREADS) {
-    const uint4 x = __ldg(body + i);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    const int id = head + i * PER;
+// A CTA's slice of a row: vectors of 16 bytes, every CTAS-th 512 of them, and the elements before and behind them that are not aligned
+template <typename T, int CTAS>
+struct Slice {
+  static constexpr int PER = 16 / sizeof(T);
+  const T* row;
+  uint4* stage;                         // null: read again
+  int V, rank, head, vectors;
+
+  __device__ __forceinline__ Slice(const T* row, int V, int rank, uint4* stage) : row(row), stage(stage), V(V), rank(rank) {
+    head = min(V, int((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / int(sizeof(T)));
+    vectors = (V - head) / PER;
+  }
+  // f(id, value) for every element; FIRST: from memory and into the stage
+  template <bool FIRST = false, typename F>
+  __device__ __forceinline__ void every(F&& f) const {
+    const int tail = head + vectors * PER;
+    const uint4* body = reinterpret_cast<const uint4*>(row + head);
+    if (rank == 0 && int(threadIdx.x) < head) f(int(threadIdx.x), widen(row[threadIdx.x]));
+    uint4* staged = stage + threadIdx.x;
+#pragma unroll 2
+    for (int i = rank * THREADS + threadIdx.x; i < vectors; i += CTAS * THREADS, staged += THREADS) {
+      uint4 x;
+      if (FIRST || stage == nullptr) x = __ldg(body + i);
+      else x = *staged;
+      if (FIRST && stage != nullptr) *staged = x;
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      const int id = head + i * PER;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (sizeof(T) == 2) {
-        f(id + 2 * j, bf16_lo(w[j]));
-        f(id + 2 * j + 1, bf16_hi(w[j]));
-      } else {
-        f(id + j, __uint_as_float(w[j]));
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 2) {
+          f(id + 2 * j, bf16_lo(w[j]));
+          f(id + 2 * j + 1, bf16_hi(w[j]));
+        } else {
+          f(id + j, __uint_as_float(w[j]));
+        }
       }
     }
+    if (rank == CTAS - 1 && tail + int(threadIdx.x) < V) f(tail + int(threadIdx.x), widen(row[tail + threadIdx.x]));
   }
-  if (rank == CTAS - 1 && tail + int(threadIdx.x) < V) f(tail + int(threadIdx.x), widen(row[tail + threadIdx.x]));
-}
+};
 
 // All CTAs of the row, with what they wrote
 template <int CTAS>
@@ -117,6 +130,17 @@ __device__ __forceinline__ void meet() {
 __device__ __forceinline__ double to_f64(float x) {
   const uint32_t b = __float_as_uint(x), m = b & 0x7fffffffu;
   return __hiloint2double(int((b & 0x80000000u) | ((m >> 3) + 0x38000000u)), int(m << 29));
+}
+
+// Place in the order of a row: `ids` bits of the id from the end behind the logit's key, of which bf16 has 16 bits
+template <typename T>
+__device__ __forceinline__ u64 place_of(uint32_t key, int id, int ids) { return (u64(sizeof(T) == 2 ? key >> 16 : key) << ids) + ((1u << ids) - 1u - uint32_t(id)); }
+template <typename T>
+__device__ __forceinline__ int id_at(u64 place, int ids) { return int((1u << ids) - 1u - (uint32_t(place) & ((1u << ids) - 1u))); }
+template <typename T>
+__device__ __forceinline__ uint32_t key_at(u64 place, int ids) {
+  const uint32_t key = uint32_t(place >> ids);
+  return sizeof(T) == 4 ? key : key & 0x8000u ? key << 16 : key << 16 | 0xffffu;
 }
 
 struct Row {
@@ -151,9 +175,9 @@ __device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, u64 w) {
   if (up) atomicAdd(hi, up);
 }
 
-// Running sums before each of PER N-thread bins in place; the first N threads hold PER neighbouring ones.
+// Running sums before each bin in place, neighbouring ones with a thread; returns the count of all.
 template <int N_BINS>
-__device__ void running_sums(uint32_t* count, uint32_t* lo, uint32_t* hi, Smem& sm, u64 sum0, uint32_t count0) {
+__device__ uint32_t running_sums(uint32_t* count, uint32_t* lo, uint32_t* hi, Smem& sm, u64 sum0, uint32_t count0) {
   constexpr int PER = N_BINS >= THREADS ? N_BINS / THREADS : 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool on = tid * PER < N_BINS;
@@ -177,8 +201,11 @@ __device__ void running_sums(uint32_t* count, uint32_t* lo, uint32_t* hi, Smem& 
   if (lane == 31) { sm.warp_sum[warp] = incl; sm.warp_count[warp] = cincl; }
   __syncthreads();
   u64 before = sum0 + incl - mine;
-  uint32_t cbefore = count0 + cincl - cnt;
-  for (int i = 0; i < warp; ++i) { before += sm.warp_sum[i]; cbefore += sm.warp_count[i]; }
+  uint32_t cbefore = count0 + cincl - cnt, all = count0;
+  for (int i = 0; i < THREADS / 32; ++i) {
+    if (i < warp) { before += sm.warp_sum[i]; cbefore += sm.warp_count[i]; }
+    all += sm.warp_count[i];
+  }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     if (on) {
@@ -190,6 +217,7 @@ __device__ void running_sums(uint32_t* count, uint32_t* lo, uint32_t* hi, Smem& 
     cbefore += c[i];
   }
   __syncthreads();
+  return all;
 }
 
 // The bin that covers position z: the last whose sum before it is not beyond z among those that hold anything of it.
@@ -236,130 +264,121 @@ __device__ __forceinline__ void join(Smem& sm, C&& count, L&& lo, H&& hi, bool c
   }
 }
 
-// The key that covers position z of the running sum (of the running count): the first CTA's .key, .above, .weight, .ties; draw: also its .id, the token.
-// z is the first CTA's to know.
+// The token that covers position z of the running sum (of the running count), in the first CTA's .place, .above and .weight.  z is the first CTA's to
+// know.  least: keys below it are not in the sums.
 template <typename T, int CTAS, bool BY_COUNT>
-__device__ void search(const T* row, int V, int rank, const Row& r, Smem& sm, u64 z, bool draw) {
-  const int tid = threadIdx.x;
+__device__ void search(const Slice<T, CTAS>& slice, int ids, const Row& r, Smem& sm, u64 z, uint32_t least) {
+  const int tid = threadIdx.x, rank = slice.rank;
   const Smem& first = of_cta<CTAS>(sm, 0);
   u64 above = 0;
   uint32_t cabove = 0;
+  // how the places from..to of n tokens are searched
+  auto next = [&](u64 from, u64 to, double n) {
+    int cut = -1;
+    if (n > double(LIST)) {
+      cut = 0;
+      while (((to - from) >> cut) >= FINE) ++cut;
+    }
+    sm.from = from;
+    sm.to = to;
+    sm.cut = cut;
+  };
   if (rank == 0) {
     const int bin = covering<BINS, BY_COUNT>(sm.count, sm.lo, sm.hi, sm, z);
     above = (u64(sm.hi[bin]) << 32) + sm.lo[bin];
     cabove = sm.count[bin];
-    if (tid == 0) { sm.from = 0; sm.to = 0xffffffffu; sm.bin = bin; }
+    if (tid == 0) {
+      // the bin's logits lie within a rounding of its borders; it has at most as many tokens as go into its sum at its lowest weight
+      const double top = double(r.top), fold = double(r.fold);
+      const float x_hi = bin == 0 ? r.top : __double2float_ru(top - bin / fold * (1 - 1e-6));
+      const float x_lo = bin == BINS - 1 ? -INFINITY : __double2float_rd(top - (bin + 1) / fold * (1 + 1e-6));
+      double n;
+      if (BY_COUNT) {
+        n = bin == BINS - 1 ? 1e9 : double(sm.count[bin + 1] - cabove);
+      } else if (bin == BINS - 1) {                   // nothing lies there
+        n = 0.0;
+      } else {
+        const double sum = double((u64(sm.hi[bin + 1]) << 32) + sm.lo[bin + 1] - above);
+        n = sum / fmax(exp(-double(bin + 1) / double(BINS_A_FOLD)) * double(1ull << r.shift) * 0.99 - 1.0, 1.0);
+      }
+      sm.bin = bin;
+      next(place_of<T>(key_of(x_lo), (1 << ids) - 1, ids), place_of<T>(key_of(x_hi), 0, ids), n);
+    }
   }
   for (;;) {
-    if (tid == 0) { sm.n = 0; sm.key_min = 0xffffffffu; sm.key_max = 0; }
+    if (tid == 0) sm.n = 0;
     meet<CTAS>();
-    const int bin = first.bin;
-    const uint32_t low = first.from, high = first.to;
-    every<T, CTAS>(row, V, rank, [&](int id, float x) {
+    const int bin = first.bin, cut = first.cut;
+    const u64 from = first.from, to = first.to;
+    if (cut >= 0) {
+      for (int i = tid; i < FINE; i += THREADS) sm.fcount[i] = sm.flo[i] = sm.fhi[i] = 0;
+      __syncthreads();
+    }
+    slice.every([&](int id, float x) {
       if (r.bin(x) != bin) return;
       const uint32_t key = key_of(x);
-      if (key < low || key > high) return;
-      const uint32_t slot = atomicAdd(&sm.n, 1u);
-      if (slot < LIST) { sm.list[slot].key = key; sm.list[slot].id = id; }
-      atomicMin(&sm.key_min, key);
-      atomicMax(&sm.key_max, key);
+      if (key < least) return;
+      const u64 place = place_of<T>(key, id, ids);
+      if (place < from || place > to) return;
+      if (cut >= 0) {
+        const uint32_t at = uint32_t((to - place) >> cut);
+        atomicAdd(&sm.fcount[at], 1u);
+        if (!BY_COUNT) add64(&sm.flo[at], &sm.fhi[at], r.weight(x));
+      } else {
+        const uint32_t slot = atomicAdd(&sm.n, 1u);
+        if (slot < LIST) sm.list[slot].place = place;
+      }
     });
     meet<CTAS>();
-    uint32_t n = 0, from = 0xffffffffu, to = 0;
+    if (cut < 0) {
+      uint32_t n = 0;
 #pragma unroll
-    for (int c = 0; c < CTAS; ++c) {
-      const Smem& other = of_cta<CTAS>(sm, c);
-      n += other.n;
-      from = min(from, other.key_min);
-      to = max(to, other.key_max);
-    }
-    if (n <= LIST) {
-      if (rank == 0) {                              // the tokens of all slices, ranked by comparison
-        Item mine;
-        if (tid < int(n)) {
-          int c = 0, at = tid;
-          if constexpr (CTAS > 1)
-            for (; at >= int(of_cta<CTAS>(sm, c).n); ++c) at -= int(of_cta<CTAS>(sm, c).n);
-          mine = of_cta<CTAS>(sm, c).list[at];
-          mine.w = r.weight(value_of(mine.key));
-        }
-        __syncthreads();
-        if (tid < int(n)) sm.list[tid] = mine;
-        __syncthreads();
-        if (tid < int(n)) {
-          u64 over = 0;
-          uint32_t higher = 0, ties = 0, place = 0;
-          for (int j = 0; j < int(n); ++j) {
-            const Item it = sm.list[j];
-            if (it.key > mine.key) { over += it.w; ++higher; }
-            else if (it.key == mine.key) { ++ties; place += it.id < mine.id; }
+      for (int c = 0; c < CTAS; ++c) n += of_cta<CTAS>(sm, c).n;
+      if (n <= LIST) {
+        if (rank == 0) {                              // the tokens of all slices, ranked by comparison
+          Item mine;
+          if (tid < int(n)) {
+            int c = 0, at = tid;
+            if constexpr (CTAS > 1)
+              for (; at >= int(of_cta<CTAS>(sm, c).n); ++c) at -= int(of_cta<CTAS>(sm, c).n);
+            mine.place = of_cta<CTAS>(sm, c).list[at].place;
+            mine.w = r.weight(value_of(key_at<T>(mine.place, ids)));
           }
-          const u64 start = BY_COUNT ? cabove + higher : above + over;
-          const u64 size = BY_COUNT ? ties : mine.w * ties;
-          if (start <= z && z - start < size) {
-            if (place == 0) { sm.key = mine.key; sm.ties = ties; sm.above = above + over; sm.weight = mine.w; }
-            if (draw && uint32_t((z - start) / mine.w) == place) sm.id = mine.id;
-          }
-        }
-      }
-      break;
-    }
-    if (from == to) {                               // one key of many tokens
-      if (rank == 0) {
-        const u64 w = r.weight(value_of(to));
-        if (tid == 0) { sm.key = to; sm.ties = n; sm.above = above; sm.weight = w; }
-        if (draw) {                                 // its tokens in order of ids: every thread counts those of a piece of the row
-          const int piece = (V + THREADS - 1) / THREADS, a = min(V, tid * piece), b = min(V, a + piece);
-          uint32_t mine = 0;
-          for (int i = a; i < b; ++i) mine += key_of(widen(row[i])) == to;
-          uint32_t incl = mine;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
-            if ((tid & 31) >= o) incl += x;
-          }
-          if ((tid & 31) == 31) sm.warp_count[tid >> 5] = incl;
           __syncthreads();
-          uint32_t before = incl - mine;
-          for (int i = 0; i < (tid >> 5); ++i) before += sm.warp_count[i];
-          const uint32_t want = uint32_t((z - above) / w);
-          if (want >= before && want < before + mine) {
-            uint32_t left = want - before;
-            for (int i = a; i < b; ++i)
-              if (key_of(widen(row[i])) == to && left-- == 0) { sm.id = i; break; }
+          if (tid < int(n)) sm.list[tid] = mine;
+          __syncthreads();
+          if (tid < int(n)) {
+            u64 over = 0;
+            uint32_t higher = 0;
+#pragma unroll 4
+            for (int j = 0; j < int(n); ++j) {
+              const Item it = sm.list[j];
+              if (it.place > mine.place) { over += it.w; ++higher; }
+            }
+            const u64 start = BY_COUNT ? cabove + higher : above + over;
+            if (start <= z && z - start < (BY_COUNT ? 1 : mine.w)) { sm.place = mine.place; sm.above = above + over; sm.weight = mine.w; }
           }
         }
+        break;
       }
-      break;
+      if (rank == 0 && tid == 0) next(from, to, double(n));          // more than were to be expected
+      continue;
     }
-    int cut = 0;
-    while (((to - from) >> cut) >= FINE) ++cut;
-    for (int i = tid; i < FINE; i += THREADS) sm.fcount[i] = sm.flo[i] = sm.fhi[i] = 0;
-    __syncthreads();
-    every<T, CTAS>(row, V, rank, [&](int id, float x) {
-      if (r.bin(x) != bin) return;
-      const uint32_t key = key_of(x);
-      if (key < from || key > to) return;
-      const uint32_t at = (to - key) >> cut;
-      atomicAdd(&sm.fcount[at], 1u);
-      add64(&sm.flo[at], &sm.fhi[at], r.weight(x));
-    });
-    meet<CTAS>();
     if (rank == 0) {
       join<CTAS, FINE>(sm, [](Smem& x) { return x.fcount; }, [](Smem& x) { return x.flo; }, [](Smem& x) { return x.fhi; }, true);
-      running_sums<FINE>(sm.fcount, sm.flo, sm.fhi, sm, above, cabove);
+      const uint32_t all = running_sums<FINE>(sm.fcount, sm.flo, sm.fhi, sm, above, cabove);
       const int at = covering<FINE, BY_COUNT>(sm.fcount, sm.flo, sm.fhi, sm, z);
       above = (u64(sm.fhi[at]) << 32) + sm.flo[at];
+      const uint32_t n = (at + 1 == FINE ? all : sm.fcount[at + 1]) - sm.fcount[at];
       cabove = sm.fcount[at];
       if (tid == 0) {
-        const uint32_t top = to - (uint32_t(at) << cut), size = (1u << cut) - 1u;
-        sm.from = top - from > size ? top - size : from;
-        sm.to = top;
+        const u64 top = to - (u64(at) << cut), size = (u64(1) << cut) - 1;
         sm.bin = bin;
+        next(top - from > size ? top - size : from, top, double(n));
       }
     }
   }
-  meet<CTAS>();                                     // everybody has read what this search used
+  meet<CTAS>();                                       // everybody has read what this search used
 }
 
 __device__ __forceinline__ u64 share(double part, u64 whole) {
@@ -369,7 +388,7 @@ __device__ __forceinline__ u64 share(double part, u64 whole) {
 }
 
 template <typename T, int CTAS>
-__global__ void __launch_bounds__(THREADS) sample_rows_kernel(Sampling p) {
+__global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, V = p.V, rank = CTAS == 1 ? 0 : int(blockIdx.x % CTAS);
@@ -385,8 +404,9 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(Sampling p) {
   const float top_p = p.top_p != nullptr ? p.top_p[at] : p.top_p_all, min_p = p.min_p != nullptr ? p.min_p[at] : p.min_p_all;
   const int top_k = p.top_k != nullptr ? p.top_k[at] : p.top_k_all;
 
+  const Slice<T, CTAS> slice(row, V, rank, p.staged ? reinterpret_cast<uint4*>(smem_raw + (sizeof(Smem) + 15) / 16 * 16) : nullptr);
   u64 best = 0;
-  every<T, CTAS>(row, V, rank, [&](int id, float x) { best = max(best, (u64(key_of(x)) << 32) | uint32_t(~id)); });
+  slice.template every<true>([&](int id, float x) { best = max(best, (u64(key_of(x)) << 32) | uint32_t(~id)); });
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   if ((tid & 31) == 0) atomicMax(&sm.best, best);
   meet<CTAS>();
@@ -418,54 +438,51 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(Sampling p) {
     low = max(mid - 1, 0);
     high = mid + 1;
   }
-  u64 whole = 0, left = 0;
   int last = nucleus ? BINS - 2 : high;               // bins from here on have no say: only a nucleus needs the sum over what min-p cuts
+  uint32_t least = 0;
   if (count) {
     // the k-th largest by counts alone, so that nobody takes weights of what lies below it
-    every<T, CTAS>(row, V, rank, [&](int id, float x) { atomicAdd(&sm.count[r.bin(x)], 1u); });
+    slice.every([&](int id, float x) { atomicAdd(&sm.count[r.bin(x)], 1u); });
     meet<CTAS>();
     if (rank == 0) {
       join<CTAS, BINS>(sm, [](Smem& x) { return x.count; }, [](Smem& x) { return x.lo; }, [](Smem& x) { return x.hi; }, true);
       running_sums<BINS>(sm.count, sm.lo, sm.hi, sm, 0, 0);
     }
-    search<T, CTAS, true>(row, V, rank, r, sm, u64(top_k - 1), false);
-    last = min(last, of_cta<CTAS>(sm, 0).bin);
+    search<T, CTAS, true>(slice, p.ids, r, sm, u64(top_k - 1), 0);
+    least = key_at<T>(of_cta<CTAS>(sm, 0).place, p.ids);
+    if (sizeof(T) == 2) least &= 0xffff0000u;
+    last = min(last, r.bin(value_of(key_at<T>(of_cta<CTAS>(sm, 0).place, p.ids))));
     meet<CTAS>();
     for (int i = tid; i < BINS; i += THREADS) sm.lo[i] = sm.hi[i] = 0;
     __syncthreads();
   }
-  every<T, CTAS>(row, V, rank, [&](int id, float x) {
+  slice.every([&](int id, float x) {
     const int b = r.bin(x);
-    if (b <= last) {
+    if (b <= last && b < BINS - 1 && key_of(x) >= least) {
       const u64 w = __double_as_longlong(r.scaled(x) + 4503599627370496.0) & 0xfffffffffffffull;
       if (w) add64(&sm.lo[b], &sm.hi[b], w);
     }
   });
   meet<CTAS>();
+  u64 left = 0;
   if (rank == 0) {
     join<CTAS, BINS>(sm, [](Smem& x) { return x.count; }, [](Smem& x) { return x.lo; }, [](Smem& x) { return x.hi; }, false);
     // the last bin's weights are 0, so that the sum before it is the whole
     running_sums<BINS>(sm.count, sm.lo, sm.hi, sm, 0, 0);
-    whole = (u64(sm.hi[BINS - 1]) << 32) + sm.lo[BINS - 1];
-    if (count) {                                      // of the k-th's bin what is not below it
-      const int bin = sm.bin;
-      whole = (u64(sm.hi[bin]) << 32) + sm.lo[bin] + sm.above + sm.weight * sm.ties;
-    }
+    left = (u64(sm.hi[BINS - 1]) << 32) + sm.lo[BINS - 1];
   }
-  left = whole;
   if (nucleus) {
-    const u64 z = share(double(top_p), whole);
-    search<T, CTAS, false>(row, V, rank, r, sm, z, false);
-    if (rank == 0) left = sm.above + ((z - sm.above) / sm.weight + 1) * sm.weight;
+    search<T, CTAS, false>(slice, p.ids, r, sm, share(double(top_p), left), least);
+    if (rank == 0) left = sm.above + sm.weight;
   }
   if (min_p > 0.f) {
-    const double least = double(min_p) * double(1ull << p.shift);
+    const double border = double(min_p) * double(1ull << p.shift);
     u64 mine = 0;
-    every<T, CTAS>(row, V, rank, [&](int id, float x) {
+    slice.every([&](int id, float x) {
       const int b = r.bin(x);
-      if (b >= low && b <= high) {
+      if (b >= low && b <= high && key_of(x) >= least) {
         const double w = r.scaled(x);
-        if (w >= least) mine += __double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
+        if (w >= border) mine += __double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
       }
     });
     if (mine) atomicAdd(&sm.sum, mine);
@@ -477,26 +494,31 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(Sampling p) {
       left = max(min(left, sum), u64(1) << p.shift);           // min_p beyond 1 leaves the largest
     }
   }
-  search<T, CTAS, false>(row, V, rank, r, sm, rank == 0 ? share(double(p.u[at]), left) : 0, true);
+  search<T, CTAS, false>(slice, p.ids, r, sm, rank == 0 ? share(double(p.u[at]), left) : 0, least);
   if (rank == 0 && tid == 0) {
-    p.token[at] = sm.id;
-    if (p.prob != nullptr) p.prob[at] = float(r.scaled(value_of(sm.key)) / double(left));
+    p.token[at] = id_at<T>(sm.place, p.ids);
+    if (p.prob != nullptr) p.prob[at] = float(r.scaled(value_of(key_at<T>(sm.place, p.ids))) / double(left));
   }
 }
 
+template <typename T, int CTAS>
+int launch_rows_by(Sampling p, int n_rows, cudaStream_t stream) {
+  // a slice of up to 64 KB is kept: two CTAs a SM
+  constexpr size_t base = (sizeof(Smem) + 15) / 16 * 16, most = 64 * 1024;
+  const size_t slice = size_t((p.V / int(16 / sizeof(T)) + CTAS * THREADS - 1) / (CTAS * THREADS)) * THREADS * 16;
+  p.staged = slice <= most;
+  JB_MAX_SMEM((sample_rows_kernel<T, CTAS>), base + most);
+  if constexpr (CTAS == 1) launch_dep(sample_rows_kernel<T, 1>, n_rows, THREADS, base + (p.staged ? slice : 0), stream, p);
+  else launch_dep_cluster(sample_rows_kernel<T, CTAS>, n_rows * CTAS, THREADS, base + (p.staged ? slice : 0), CTAS, stream, p);
+  return JB200_OK;
+}
+
+// CTAs a row: as many as two a SM leave room for, slices of 4096 tokens or more
 template <typename T>
-void launch_rows(const Sampling& p, int n_rows, cudaStream_t stream) {
-  // CTAs a row: as many as two a SM leave room for, slices of 4096 tokens or more
-  const int most = 2 * sm_count() / n_rows, wide = p.V / 4096;
-  auto start = [&](auto kernel, int ctas) {
-    if (ctas == 1) launch_dep(kernel, n_rows, THREADS, sizeof(Smem), stream, p);
-    else launch_dep_cluster(kernel, n_rows * ctas, THREADS, sizeof(Smem), ctas, stream, p);
-  };
-  const int ctas = most < wide ? most : wide;
-  if (ctas >= 8) start(sample_rows_kernel<T, 8>, 8);
-  else if (ctas >= 4) start(sample_rows_kernel<T, 4>, 4);
-  else if (ctas >= 2) start(sample_rows_kernel<T, 2>, 2);
-  else start(sample_rows_kernel<T, 1>, 1);
+int launch_rows(const Sampling& p, int n_rows, cudaStream_t stream) {
+  const int most = 2 * sm_count() / n_rows, wide = p.V / 4096, ctas = most < wide ? most : wide;
+  return ctas >= 8 ? launch_rows_by<T, 8>(p, n_rows, stream) : ctas >= 4 ? launch_rows_by<T, 4>(p, n_rows, stream)
+       : ctas >= 2 ? launch_rows_by<T, 2>(p, n_rows, stream) : launch_rows_by<T, 1>(p, n_rows, stream);
 }
 
 }  // namespace
@@ -509,16 +531,16 @@ int launch_sample_rows(const jb200_sampling* s, int n_rows, int64_t* token, floa
   if (n_rows == 0) return JB200_OK;
   JB_REQUIRE(s->logits && s->u && token, "sample_rows: null pointer");
   Sampling p;
-  static_assert(sizeof(Smem) <= 48 * 1024, "no larger than a launch may ask for without more ado");
   p.logits = s->logits; p.ld = size_t(s->ld); p.V = s->V;
   int bits = 0;
   while ((1 << bits) < s->V) ++bits;
+  p.ids = bits > 0 ? bits : 1;
   p.shift = 63 - bits < 45 ? 63 - bits : 45;        // V weights of at most 2^shift fit 63 bits
   p.u = s->u; p.temperature = s->temperature; p.top_k = s->top_k; p.top_p = s->top_p; p.min_p = s->min_p;
   p.temperature_all = s->temperature_all; p.top_k_all = s->top_k_all; p.top_p_all = s->top_p_all; p.min_p_all = s->min_p_all;
   p.token = token; p.prob = prob;
-  if (s->logits_dtype == 0) launch_rows<float>(p, n_rows, stream);
-  else launch_rows<__nv_bfloat16>(p, n_rows, stream);
+  const int rc = s->logits_dtype == 0 ? launch_rows<float>(p, n_rows, stream) : launch_rows<__nv_bfloat16>(p, n_rows, stream);
+  if (rc != JB200_OK) return rc;
   JB_LAUNCH_CHECK("sample_rows_kernel");
   return JB200_OK;
 }
