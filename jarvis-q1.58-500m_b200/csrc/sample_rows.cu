@@ -13,7 +13,7 @@
 // missed only where u lies within some 1e-12 of a border.  A cluster of CTAs has a row, a slice each (in shared memory where it fits), with as many CTAs as
 // keep the SMs busy.  A histogram of the sums (for top-k of the counts) over 2048 bins of 1/32 of an e-fold finds the bin that covers z.  The
 // tokens of a bin, up to 256, are ranked by comparison with one another; where there are more they are first cut into 512 parts of their order, logit
-// then id, until there are not.  Every CTA counts and lists its slice in its own memory; the first one reads the others' and searches, the others
+// then id, until there are not.  The few tokens near the largest, where most answers lie, are listed as the sums are taken.  Every CTA counts and lists its slice in its own memory; the first one reads the others' and searches, the others
 // read what it found.
 #include <cooperative_groups.h>
 
@@ -31,6 +31,7 @@ constexpr int BINS = 2048;              // 1/32 of an e-fold each; the last: eve
 constexpr float BINS_A_FOLD = 32.f;
 constexpr int FINE = 512;
 constexpr int LIST = 256;
+constexpr int NEAR = 224, NEAR_LIST = 512;   // bins whose tokens are listed at once (7 e-folds), as long as there are no more than that in a slice
 constexpr int TABLE = 64;               // 2^-(j / 64)
 
 struct Sampling {
@@ -54,10 +55,11 @@ struct Smem {
   uint32_t count[BINS], lo[BINS], hi[BINS];       // then, as running sums before every bin: count, (lo, hi)
   uint32_t fcount[FINE], flo[FINE], fhi[FINE];
   Item list[LIST];
+  u64 near[NEAR_LIST];
   u64 warp_sum[THREADS / 32];
   uint32_t warp_count[THREADS / 32];
   u64 best;                                       // (key, ~id) of the largest
-  uint32_t n;
+  uint32_t n, n_near;
   int bin, cut;                                   // what is searched next: of this bin the places from..to; cut: in parts of 2^cut of them, < 0: one by one
   u64 from, to;
   u64 place, above, weight;                       // what a search leaves: the token that covers z, the sum before it, its weight
@@ -265,17 +267,17 @@ __device__ __forceinline__ void join(Smem& sm, C&& count, L&& lo, H&& hi, bool c
 }
 
 // The token that covers position z of the running sum (of the running count), in the first CTA's .place, .above and .weight.  z is the first CTA's to
-// know.  least: keys below it are not in the sums.
+// know.  least: keys below it are not in the sums; near: bins below it are in the lists of what is near the largest.
 template <typename T, int CTAS, bool BY_COUNT>
-__device__ void search(const Slice<T, CTAS>& slice, int ids, const Row& r, Smem& sm, u64 z, uint32_t least) {
+__device__ void search(const Slice<T, CTAS>& slice, int ids, const Row& r, Smem& sm, u64 z, uint32_t least, int near) {
   const int tid = threadIdx.x, rank = slice.rank;
   const Smem& first = of_cta<CTAS>(sm, 0);
   u64 above = 0;
   uint32_t cabove = 0;
   // how the places from..to of n tokens are searched
-  auto next = [&](u64 from, u64 to, double n) {
+  auto next = [&](u64 from, u64 to, float n) {
     int cut = -1;
-    if (n > double(LIST)) {
+    if (n > float(LIST)) {
       cut = 0;
       while (((to - from) >> cut) >= FINE) ++cut;
     }
@@ -288,18 +290,18 @@ __device__ void search(const Slice<T, CTAS>& slice, int ids, const Row& r, Smem&
     above = (u64(sm.hi[bin]) << 32) + sm.lo[bin];
     cabove = sm.count[bin];
     if (tid == 0) {
-      // the bin's logits lie within a rounding of its borders; it has at most as many tokens as go into its sum at its lowest weight
-      const double top = double(r.top), fold = double(r.fold);
-      const float x_hi = bin == 0 ? r.top : __double2float_ru(top - bin / fold * (1 - 1e-6));
-      const float x_lo = bin == BINS - 1 ? -INFINITY : __double2float_rd(top - (bin + 1) / fold * (1 + 1e-6));
-      double n;
+      // the bin's logits lie within roundings of its borders; it has at most as many tokens as go into its sum at its lowest weight
+      const float lo = float(bin) / r.fold, hi = float(bin + 1) / r.fold;
+      const float x_hi = bin == 0 ? r.top : r.top - lo + 2e-6f * (fabsf(r.top) + lo);
+      const float x_lo = bin == BINS - 1 ? -INFINITY : r.top - hi - 2e-6f * (fabsf(r.top) + hi);
+      float n;
       if (BY_COUNT) {
-        n = bin == BINS - 1 ? 1e9 : double(sm.count[bin + 1] - cabove);
+        n = bin == BINS - 1 ? 1e9f : float(sm.count[bin + 1] - cabove);
       } else if (bin == BINS - 1) {                   // nothing lies there
-        n = 0.0;
+        n = 0.f;
       } else {
-        const double sum = double((u64(sm.hi[bin + 1]) << 32) + sm.lo[bin + 1] - above);
-        n = sum / fmax(exp(-double(bin + 1) / double(BINS_A_FOLD)) * double(1ull << r.shift) * 0.99 - 1.0, 1.0);
+        const float sum = float((u64(sm.hi[bin + 1]) << 32) + sm.lo[bin + 1] - above);
+        n = sum / fmaxf(__expf(-float(bin + 1) / BINS_A_FOLD) * float(1ull << r.shift) * 0.99f - 1.f, 1.f);
       }
       sm.bin = bin;
       next(place_of<T>(key_of(x_lo), (1 << ids) - 1, ids), place_of<T>(key_of(x_hi), 0, ids), n);
@@ -314,11 +316,7 @@ __device__ void search(const Slice<T, CTAS>& slice, int ids, const Row& r, Smem&
       for (int i = tid; i < FINE; i += THREADS) sm.fcount[i] = sm.flo[i] = sm.fhi[i] = 0;
       __syncthreads();
     }
-    slice.every([&](int id, float x) {
-      if (r.bin(x) != bin) return;
-      const uint32_t key = key_of(x);
-      if (key < least) return;
-      const u64 place = place_of<T>(key, id, ids);
+    auto take = [&](u64 place, float x) {
       if (place < from || place > to) return;
       if (cut >= 0) {
         const uint32_t at = uint32_t((to - place) >> cut);
@@ -328,7 +326,19 @@ __device__ void search(const Slice<T, CTAS>& slice, int ids, const Row& r, Smem&
         const uint32_t slot = atomicAdd(&sm.n, 1u);
         if (slot < LIST) sm.list[slot].place = place;
       }
-    });
+    };
+    if (bin < near) {
+      for (int i = tid; i < int(sm.n_near); i += THREADS) {
+        const float x = value_of(key_at<T>(sm.near[i], ids));
+        if (r.bin(x) == bin) take(sm.near[i], x);
+      }
+    } else {
+      slice.every([&](int id, float x) {
+        if (r.bin(x) != bin) return;
+        const uint32_t key = key_of(x);
+        if (key >= least) take(place_of<T>(key, id, ids), x);
+      });
+    }
     meet<CTAS>();
     if (cut < 0) {
       uint32_t n = 0;
@@ -347,21 +357,31 @@ __device__ void search(const Slice<T, CTAS>& slice, int ids, const Row& r, Smem&
           __syncthreads();
           if (tid < int(n)) sm.list[tid] = mine;
           __syncthreads();
-          if (tid < int(n)) {
-            u64 over = 0;
-            uint32_t higher = 0;
-#pragma unroll 4
-            for (int j = 0; j < int(n); ++j) {
+          // a power of two of neighbouring threads an element, each with its part of the others
+          int helpers = 1;
+          while (helpers < 32 && 2 * helpers * int(n) <= THREADS) helpers *= 2;
+          const int me = tid / helpers;
+          u64 over = 0;
+          uint32_t higher = 0;
+          if (me < int(n)) {
+            mine = sm.list[me];
+            for (int j = tid & (helpers - 1); j < int(n); j += helpers) {
               const Item it = sm.list[j];
               if (it.place > mine.place) { over += it.w; ++higher; }
             }
+          }
+          for (int o = 1; o < helpers; o *= 2) {
+            over += __shfl_xor_sync(0xffffffffu, over, o);
+            higher += __shfl_xor_sync(0xffffffffu, higher, o);
+          }
+          if (me < int(n) && (tid & (helpers - 1)) == 0) {
             const u64 start = BY_COUNT ? cabove + higher : above + over;
             if (start <= z && z - start < (BY_COUNT ? 1 : mine.w)) { sm.place = mine.place; sm.above = above + over; sm.weight = mine.w; }
           }
         }
         break;
       }
-      if (rank == 0 && tid == 0) next(from, to, double(n));          // more than were to be expected
+      if (rank == 0 && tid == 0) next(from, to, float(n));          // more than were to be expected
       continue;
     }
     if (rank == 0) {
@@ -374,7 +394,7 @@ __device__ void search(const Slice<T, CTAS>& slice, int ids, const Row& r, Smem&
       if (tid == 0) {
         const u64 top = to - (u64(at) << cut), size = (u64(1) << cut) - 1;
         sm.bin = bin;
-        next(top - from > size ? top - size : from, top, double(n));
+        next(top - from > size ? top - size : from, top, float(n));
       }
     }
   }
@@ -393,7 +413,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, V = p.V, rank = CTAS == 1 ? 0 : int(blockIdx.x % CTAS);
   const size_t at = blockIdx.x / CTAS;
-  if (tid == 0) { sm.best = 0; sm.sum = 0; }
+  if (tid == 0) { sm.best = 0; sm.sum = 0; sm.n_near = 0; }
   for (int i = tid; i < BINS; i += THREADS) sm.count[i] = sm.lo[i] = sm.hi[i] = 0;
   if (tid < TABLE) sm.table[tid] = exp2(-double(tid) / TABLE);
   meet<CTAS>();
@@ -433,8 +453,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
   // min-p: bins well above the border are in, those well below out; weights decide in the three around it (the bins' borders are rounded)
   int low = 0, high = BINS - 2;
   if (min_p > 0.f) {
-    const double d = -log(double(min_p)) * double(BINS_A_FOLD);
-    const int mid = d < double(BINS - 3) ? max(int(d), 0) : BINS - 3;
+    const float d = -logf(min_p) * BINS_A_FOLD;
+    const int mid = d < float(BINS - 3) ? max(int(d), 0) : BINS - 3;
     low = max(mid - 1, 0);
     high = mid + 1;
   }
@@ -448,7 +468,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
       join<CTAS, BINS>(sm, [](Smem& x) { return x.count; }, [](Smem& x) { return x.lo; }, [](Smem& x) { return x.hi; }, true);
       running_sums<BINS>(sm.count, sm.lo, sm.hi, sm, 0, 0);
     }
-    search<T, CTAS, true>(slice, p.ids, r, sm, u64(top_k - 1), 0);
+    search<T, CTAS, true>(slice, p.ids, r, sm, u64(top_k - 1), 0, 0);
     least = key_at<T>(of_cta<CTAS>(sm, 0).place, p.ids);
     if (sizeof(T) == 2) least &= 0xffff0000u;
     last = min(last, r.bin(value_of(key_at<T>(of_cta<CTAS>(sm, 0).place, p.ids))));
@@ -456,14 +476,28 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
     for (int i = tid; i < BINS; i += THREADS) sm.lo[i] = sm.hi[i] = 0;
     __syncthreads();
   }
+  const double border = double(min_p) * double(1ull << p.shift);
+  u64 bordering = 0;
   slice.every([&](int id, float x) {
     const int b = r.bin(x);
-    if (b <= last && b < BINS - 1 && key_of(x) >= least) {
-      const u64 w = __double_as_longlong(r.scaled(x) + 4503599627370496.0) & 0xfffffffffffffull;
-      if (w) add64(&sm.lo[b], &sm.hi[b], w);
+    if (b > last || b == BINS - 1) return;
+    const uint32_t key = key_of(x);
+    if (key < least) return;
+    const double scaled = r.scaled(x);
+    const u64 w = __double_as_longlong(scaled + 4503599627370496.0) & 0xfffffffffffffull;
+    if (b >= low && b <= high && scaled >= border) bordering += w;
+    if (w) add64(&sm.lo[b], &sm.hi[b], w);
+    if (b < NEAR && *static_cast<volatile uint32_t*>(&sm.n_near) <= NEAR_LIST) {
+      const uint32_t slot = atomicAdd(&sm.n_near, 1u);
+      if (slot < NEAR_LIST) sm.near[slot] = place_of<T>(key, id, p.ids);
     }
   });
+  if (min_p > 0.f && bordering) atomicAdd(&sm.sum, bordering);
   meet<CTAS>();
+  int near = NEAR;
+#pragma unroll
+  for (int c = 0; c < CTAS; ++c)
+    if (of_cta<CTAS>(sm, c).n_near > NEAR_LIST) near = 0;
   u64 left = 0;
   if (rank == 0) {
     join<CTAS, BINS>(sm, [](Smem& x) { return x.count; }, [](Smem& x) { return x.lo; }, [](Smem& x) { return x.hi; }, false);
@@ -472,29 +506,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
     left = (u64(sm.hi[BINS - 1]) << 32) + sm.lo[BINS - 1];
   }
   if (nucleus) {
-    search<T, CTAS, false>(slice, p.ids, r, sm, share(double(top_p), left), least);
+    search<T, CTAS, false>(slice, p.ids, r, sm, share(double(top_p), left), least, near);
     if (rank == 0) left = sm.above + sm.weight;
   }
-  if (min_p > 0.f) {
-    const double border = double(min_p) * double(1ull << p.shift);
-    u64 mine = 0;
-    slice.every([&](int id, float x) {
-      const int b = r.bin(x);
-      if (b >= low && b <= high && key_of(x) >= least) {
-        const double w = r.scaled(x);
-        if (w >= border) mine += __double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
-      }
-    });
-    if (mine) atomicAdd(&sm.sum, mine);
-    meet<CTAS>();
-    if (rank == 0) {
-      u64 sum = (u64(sm.hi[low]) << 32) + sm.lo[low];
+  if (min_p > 0.f && rank == 0) {
+    u64 sum = (u64(sm.hi[low]) << 32) + sm.lo[low];
 #pragma unroll
-      for (int c = 0; c < CTAS; ++c) sum += of_cta<CTAS>(sm, c).sum;
-      left = max(min(left, sum), u64(1) << p.shift);           // min_p beyond 1 leaves the largest
-    }
+    for (int c = 0; c < CTAS; ++c) sum += of_cta<CTAS>(sm, c).sum;
+    left = max(min(left, sum), u64(1) << p.shift);             // min_p beyond 1 leaves the largest
   }
-  search<T, CTAS, false>(slice, p.ids, r, sm, rank == 0 ? share(double(p.u[at]), left) : 0, least);
+  search<T, CTAS, false>(slice, p.ids, r, sm, rank == 0 ? share(double(p.u[at]), left) : 0, least, near);
   if (rank == 0 && tid == 0) {
     p.token[at] = id_at<T>(sm.place, p.ids);
     if (p.prob != nullptr) p.prob[at] = float(r.scaled(value_of(key_at<T>(sm.place, p.ids))) / double(left));
