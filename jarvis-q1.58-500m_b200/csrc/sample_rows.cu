@@ -10,11 +10,15 @@
 //
 // All of them ask "which token covers position z of the running sum", top-k with every weight 1.  Weights are taken in f64 and held as integers of
 // 2^-45 of the largest one's, so that sums do not depend on the order of the atomics that form them, and a token that the exact sums choose is
-// missed only where u lies within some 1e-12 of a border.  A cluster of CTAs has a row, a slice each (in shared memory where it fits), with as many CTAs as
-// keep the SMs busy.  A histogram of the sums (for top-k of the counts) over 2048 bins of 1/32 of an e-fold finds the bin that covers z.  The
-// tokens of a bin, up to 256, are ranked by comparison with one another; where there are more they are first cut into 512 parts of their order, logit
-// then id, until there are not.  The few tokens near the largest, where most answers lie, are listed as the sums are taken.  Every CTA counts and lists its slice in its own memory; the first one reads the others' and searches, the others
-// read what it found.
+// missed only where u lies within some 1e-12 of a border.  A cluster of CTAs has a row, a slice each (in shared memory where it fits), with as many
+// CTAs as keep the SMs busy.  A histogram of the sums (for top-k of the counts) over 2048 bins of 1/32 of an e-fold finds the bin that covers z.
+// The tokens of a bin, up to 256, are ranked by comparison with one another; where there are more they are first cut into 512 parts of their order,
+// logit then id, until there are not.  The few tokens near the largest, where most answers lie, are listed as the sums are taken.  Every CTA counts
+// and lists its slice in its own memory; the first one reads the others' and searches, the others read what it found.
+//
+// Bounds: a row alone, the chain of passes, barriers and searches (50257 tokens, nucleus: 27 us, of which the weights 6 and each search 4); many rows,
+// reading them once and again from L2 (256 rows of 50257 f32, min-p: 28 us, the first reading alone 7.8); with a nucleus over everything, the 11
+// f64 operations and the atomics of every token's weight (64 rows of bf16, every setting of its own: 44 us).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -51,6 +55,13 @@ struct Item {
   u64 w;
 };
 
+// What the first CTA wants of all: the tokens of a bin with places from..to, in parts of 2^cut places (LISTED: the tokens themselves; DONE: nothing more)
+struct Command {
+  int bin, cut;
+  u64 from, to;
+};
+constexpr int LISTED = -1, DONE = -2;
+
 struct Smem {
   uint32_t count[BINS], lo[BINS], hi[BINS];       // then, as running sums before every bin: count, (lo, hi)
   uint32_t fcount[FINE], flo[FINE], fhi[FINE];
@@ -58,10 +69,10 @@ struct Smem {
   u64 near[NEAR_LIST];
   u64 warp_sum[THREADS / 32];
   uint32_t warp_count[THREADS / 32];
-  u64 best;                                       // (key, ~id) of the largest
+  uint32_t best, best_id;                         // the largest: key, ~id
   uint32_t n, n_near;
-  int bin, cut;                                   // what is searched next: of this bin the places from..to; cut: in parts of 2^cut of them, < 0: one by one
-  u64 from, to;
+  Command command[2];                             // taken in turn, so that one can be written while the other is read
+  int bin;
   u64 place, above, weight;                       // what a search leaves: the token that covers z, the sum before it, its weight
   u64 sum;
   double table[TABLE];
@@ -80,7 +91,7 @@ __device__ __forceinline__ float widen(T x) { return x; }
 template <>
 __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// A CTA's slice of a row: vectors of 16 bytes, every CTAS-th 512 of them, and the elements before and behind them that are not aligned
+// A CTA's slice of a row: vectors of 16 bytes, every CTAS-th THREADS of them, and the elements before and behind them that are not aligned
 template <typename T, int CTAS>
 struct Slice {
   static constexpr int PER = 16 / sizeof(T);
@@ -92,32 +103,57 @@ struct Slice {
     head = min(V, int((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / int(sizeof(T)));
     vectors = (V - head) / PER;
   }
-  // f(id, value) for every element; FIRST: from memory and into the stage
-  template <bool FIRST = false, typename F>
-  __device__ __forceinline__ void every(F&& f) const {
+  static __device__ __forceinline__ float largest(const uint4& x) {       // NaN only where all are
+    if constexpr (sizeof(T) == 2) {
+      const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(&x);
+      const __nv_bfloat162 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+      return fmaxf(__low2float(m), __high2float(m));
+    } else {
+      return fmaxf(fmaxf(__uint_as_float(x.x), __uint_as_float(x.y)), fmaxf(__uint_as_float(x.z), __uint_as_float(x.w)));
+    }
+  }
+  // the largest of this thread's elements, which go into the stage on the way
+  __device__ __forceinline__ float peak() const {
     const int tail = head + vectors * PER;
     const uint4* body = reinterpret_cast<const uint4*>(row + head);
-    if (rank == 0 && int(threadIdx.x) < head) f(int(threadIdx.x), widen(row[threadIdx.x]));
+    float top = -INFINITY;
     uint4* staged = stage + threadIdx.x;
-#pragma unroll 2
+#pragma unroll 4
     for (int i = rank * THREADS + threadIdx.x; i < vectors; i += CTAS * THREADS, staged += THREADS) {
-      uint4 x;
-      if (FIRST || stage == nullptr) x = __ldg(body + i);
-      else x = *staged;
-      if (FIRST && stage != nullptr) *staged = x;
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      const uint4 x = __ldg(body + i);
+      if (stage != nullptr) *staged = x;
+      top = fmaxf(top, largest(x));
+    }
+    if (rank == 0 && int(threadIdx.x) < head) top = fmaxf(top, widen(row[threadIdx.x]));
+    if (rank == CTAS - 1 && tail + int(threadIdx.x) < V) top = fmaxf(top, widen(row[tail + threadIdx.x]));
+    return top;
+  }
+  // f(id, values, n) for four neighbours at a time, so that their chains of arithmetic overlap, without those that are all below `lowest`.  Elements
+  // that are not aligned come one by one (n 1), with -infinities behind them.  Not unrolled further: a CTA runs most instructions for the first time,
+  // and fetching them is what a row alone waits for (50257 tokens, nucleus: 27 us; two vectors a turn: 49).
+  template <typename F>
+  __device__ __forceinline__ void fours(float lowest, F&& f) const {
+    const int tail = head + vectors * PER;
+    const uint4* body = reinterpret_cast<const uint4*>(row + head);
+    auto four = [&](int id, int n, float a, float b, float c, float d) {
+      if (fmaxf(fmaxf(a, b), fmaxf(c, d)) < lowest) return;
+      const float x[4] = {a, b, c, d};
+      f(id, x, n);
+    };
+    const uint4* staged = stage + threadIdx.x;
+#pragma unroll 1
+    for (int i = rank * THREADS + threadIdx.x; i < vectors; i += CTAS * THREADS, staged += THREADS) {
+      const uint4 x = stage == nullptr ? __ldg(body + i) : *staged;
       const int id = head + i * PER;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(T) == 2) {
-          f(id + 2 * j, bf16_lo(w[j]));
-          f(id + 2 * j + 1, bf16_hi(w[j]));
-        } else {
-          f(id + j, __uint_as_float(w[j]));
-        }
+      if constexpr (sizeof(T) == 2) {
+        four(id, 4, bf16_lo(x.x), bf16_hi(x.x), bf16_lo(x.y), bf16_hi(x.y));
+        four(id + 4, 4, bf16_lo(x.z), bf16_hi(x.z), bf16_lo(x.w), bf16_hi(x.w));
+      } else {
+        four(id, 4, __uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
       }
     }
-    if (rank == CTAS - 1 && tail + int(threadIdx.x) < V) f(tail + int(threadIdx.x), widen(row[tail + threadIdx.x]));
+    if (rank == 0 && int(threadIdx.x) < head) four(int(threadIdx.x), 1, widen(row[threadIdx.x]), -INFINITY, -INFINITY, -INFINITY);
+    if (rank == CTAS - 1 && tail + int(threadIdx.x) < V) four(tail + int(threadIdx.x), 1, widen(row[tail + threadIdx.x]), -INFINITY, -INFINITY, -INFINITY);
   }
 };
 
@@ -125,7 +161,13 @@ struct Slice {
 template <int CTAS>
 __device__ __forceinline__ void meet() {
   if constexpr (CTAS == 1) __syncthreads();
-  else cooperative_groups::this_cluster().sync();
+  else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// This CTA's memory; functions that are called rather than inlined ask for it, so that the compiler knows that it is shared memory
+__device__ __forceinline__ Smem& own_smem() {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  return *reinterpret_cast<Smem*>(smem_raw);
 }
 
 // x as f64 (a subnormal x as some other number of 1e-38: no weight shows it); the conversion instruction runs at an eighth of this one's rate
@@ -155,6 +197,12 @@ struct Row {
     const float d = x == top ? 0.f : (top - x) * fold;
     return d < float(BINS - 1) ? int(d) : BINS - 1;            // NaN and infinities are the last bin's
   }
+  // a value that none of the bins up to b goes below; an infinite largest has bin 0 for itself, and all others have the last
+  __device__ __forceinline__ float below(int b) const {
+    if (top == INFINITY && b < BINS - 1) return top;
+    const float hi = float(b + 1) / fold;
+    return b >= BINS - 1 ? -INFINITY : top - hi - 2e-6f * (fabsf(top) + hi);
+  }
   // 2^shift exp((x - top) / temperature) as a double, of an x of any bin but the last: 2^-(n / 64) from the table, the rest from its series (the fifth
   // term is below 2^-44)
   __device__ __forceinline__ double scaled(float x) const {
@@ -179,7 +227,11 @@ __device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, u64 w) {
 
 // Running sums before each bin in place, neighbouring ones with a thread; returns the count of all.
 template <int N_BINS>
-__device__ uint32_t running_sums(uint32_t* count, uint32_t* lo, uint32_t* hi, Smem& sm, u64 sum0, uint32_t count0) {
+__device__ __forceinline__ uint32_t running_sums(u64 sum0, uint32_t count0) {
+  Smem& sm = own_smem();
+  uint32_t* const count = N_BINS == BINS ? sm.count : sm.fcount;
+  uint32_t* const lo = N_BINS == BINS ? sm.lo : sm.flo;
+  uint32_t* const hi = N_BINS == BINS ? sm.hi : sm.fhi;
   constexpr int PER = N_BINS >= THREADS ? N_BINS / THREADS : 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool on = tid * PER < N_BINS;
@@ -204,9 +256,12 @@ __device__ uint32_t running_sums(uint32_t* count, uint32_t* lo, uint32_t* hi, Sm
   __syncthreads();
   u64 before = sum0 + incl - mine;
   uint32_t cbefore = count0 + cincl - cnt, all = count0;
-  for (int i = 0; i < THREADS / 32; ++i) {
-    if (i < warp) { before += sm.warp_sum[i]; cbefore += sm.warp_count[i]; }
-    all += sm.warp_count[i];
+  for (int i = 0; i < THREADS / 32; i += 4) {
+#pragma unroll
+    for (int j = i; j < i + 4; ++j) {
+      if (j < warp) { before += sm.warp_sum[j]; cbefore += sm.warp_count[j]; }
+      all += sm.warp_count[j];
+    }
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -223,13 +278,17 @@ __device__ uint32_t running_sums(uint32_t* count, uint32_t* lo, uint32_t* hi, Sm
 }
 
 // The bin that covers position z: the last whose sum before it is not beyond z among those that hold anything of it.
-template <int N_BINS, bool BY_COUNT>
-__device__ int covering(const uint32_t* count, const uint32_t* lo, const uint32_t* hi, Smem& sm, u64 z) {
+template <int N_BINS>
+__device__ __forceinline__ int covering(bool by_count, u64 z) {
+  Smem& sm = own_smem();
+  const uint32_t* const count = N_BINS == BINS ? sm.count : sm.fcount;
+  const uint32_t* const lo = N_BINS == BINS ? sm.lo : sm.flo;
+  const uint32_t* const hi = N_BINS == BINS ? sm.hi : sm.fhi;
   if (threadIdx.x == 0) sm.bin = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < N_BINS; i += THREADS) {
-    const u64 a = BY_COUNT ? count[i] : (u64(hi[i]) << 32) + lo[i];
-    const u64 b = i + 1 == N_BINS ? ~0ull : BY_COUNT ? count[i + 1] : (u64(hi[i + 1]) << 32) + lo[i + 1];
+    const u64 a = by_count ? count[i] : (u64(hi[i]) << 32) + lo[i];
+    const u64 b = i + 1 == N_BINS ? ~0ull : by_count ? count[i + 1] : (u64(hi[i + 1]) << 32) + lo[i + 1];
     if (a <= z && z < b) sm.bin = i;
   }
   __syncthreads();
@@ -245,57 +304,97 @@ __device__ __forceinline__ Smem& of_cta(Smem& sm, int c) {
   else return *cooperative_groups::this_cluster().map_shared_rank(&sm, c);
 }
 
-// The first CTA's bins: the sums over all CTAs
-template <int CTAS, int N_BINS, typename C, typename L, typename H>
-__device__ __forceinline__ void join(Smem& sm, C&& count, L&& lo, H&& hi, bool counts) {
+// The sums over all CTAs, in the first one's memory: a part of the bins to a CTA.  Behind a meeting, and before one.
+template <int CTAS>
+__device__ __forceinline__ void join_counts(Smem& sm, int rank) {
   if constexpr (CTAS > 1) {
-    for (int i = threadIdx.x; i < N_BINS; i += THREADS) {
+    for (int i = rank * (BINS / CTAS) + threadIdx.x; i < (rank + 1) * (BINS / CTAS); i += THREADS) {
+      uint32_t n = 0;
+#pragma unroll
+      for (int c = 0; c < CTAS; ++c) n += of_cta<CTAS>(sm, c).count[i];
+      of_cta<CTAS>(sm, 0).count[i] = n;
+    }
+    meet<CTAS>();
+  }
+}
+template <int CTAS>
+__device__ __forceinline__ void join_sums(Smem& sm, int rank) {
+  if constexpr (CTAS > 1) {
+    for (int i = rank * (BINS / CTAS) + threadIdx.x; i < (rank + 1) * (BINS / CTAS); i += THREADS) {
+      u64 sum = 0;
+#pragma unroll
+      for (int c = 0; c < CTAS; ++c) sum += (u64(of_cta<CTAS>(sm, c).hi[i]) << 32) + of_cta<CTAS>(sm, c).lo[i];
+      of_cta<CTAS>(sm, 0).lo[i] = uint32_t(sum);
+      of_cta<CTAS>(sm, 0).hi[i] = uint32_t(sum >> 32);
+    }
+    meet<CTAS>();
+  }
+}
+// The same of the parts of a bin, by the first CTA alone
+template <int CTAS>
+__device__ __forceinline__ void join_parts(Smem& sm) {
+  if constexpr (CTAS > 1) {
+    for (int i = threadIdx.x; i < FINE; i += THREADS) {
       u64 sum = 0;
       uint32_t n = 0;
 #pragma unroll
       for (int c = 0; c < CTAS; ++c) {
         Smem& other = of_cta<CTAS>(sm, c);
-        sum += (u64(hi(other)[i]) << 32) + lo(other)[i];
-        if (counts) n += count(other)[i];
+        sum += (u64(other.fhi[i]) << 32) + other.flo[i];
+        n += other.fcount[i];
       }
-      lo(sm)[i] = uint32_t(sum);
-      hi(sm)[i] = uint32_t(sum >> 32);
-      count(sm)[i] = n;
+      sm.flo[i] = uint32_t(sum);
+      sm.fhi[i] = uint32_t(sum >> 32);
+      sm.fcount[i] = n;
     }
     __syncthreads();
   }
 }
 
+// A token of the bin that is searched.  A call, since few tokens are of it.
+template <typename T>
+__device__ __forceinline__ void take(const Command now, const Row r, bool by_count, u64 place, float x) {
+  Smem& sm = own_smem();
+  if (place < now.from || place > now.to) return;
+  if (now.cut >= 0) {
+    const uint32_t at = uint32_t((now.to - place) >> now.cut);
+    atomicAdd(&sm.fcount[at], 1u);
+    if (!by_count) add64(&sm.flo[at], &sm.fhi[at], r.weight(x));
+  } else {
+    const uint32_t slot = atomicAdd(&sm.n, 1u);
+    if (slot < LIST) sm.list[slot].place = place;
+  }
+}
+
 // The token that covers position z of the running sum (of the running count), in the first CTA's .place, .above and .weight.  z is the first CTA's to
 // know.  least: keys below it are not in the sums; near: bins below it are in the lists of what is near the largest.
-template <typename T, int CTAS, bool BY_COUNT>
-__device__ void search(const Slice<T, CTAS>& slice, int ids, const Row& r, Smem& sm, u64 z, uint32_t least, int near) {
+// `turn`: which of the commands is next.
+template <typename T, int CTAS>
+__device__ __forceinline__ void search(const Slice<T, CTAS> slice, int ids, const Row r, bool by_count, u64 z, uint32_t least, int near, int& turn) {
+  Smem& sm = own_smem();
   const int tid = threadIdx.x, rank = slice.rank;
-  const Smem& first = of_cta<CTAS>(sm, 0);
   u64 above = 0;
   uint32_t cabove = 0;
   // how the places from..to of n tokens are searched
-  auto next = [&](u64 from, u64 to, float n) {
-    int cut = -1;
-    if (n > float(LIST)) {
-      cut = 0;
-      while (((to - from) >> cut) >= FINE) ++cut;
-    }
-    sm.from = from;
-    sm.to = to;
-    sm.cut = cut;
+  auto next = [&](int bin, u64 from, u64 to, float n) {
+    int cut = LISTED;
+    if (n > float(LIST)) cut = 64 - __clzll((long long)((to - from) / FINE));
+    sm.command[turn].bin = bin;
+    sm.command[turn].cut = cut;
+    sm.command[turn].from = from;
+    sm.command[turn].to = to;
   };
   if (rank == 0) {
-    const int bin = covering<BINS, BY_COUNT>(sm.count, sm.lo, sm.hi, sm, z);
+    const int bin = covering<BINS>(by_count, z);
     above = (u64(sm.hi[bin]) << 32) + sm.lo[bin];
     cabove = sm.count[bin];
     if (tid == 0) {
       // the bin's logits lie within roundings of its borders; it has at most as many tokens as go into its sum at its lowest weight
-      const float lo = float(bin) / r.fold, hi = float(bin + 1) / r.fold;
+      const float lo = float(bin) / r.fold;
       const float x_hi = bin == 0 ? r.top : r.top - lo + 2e-6f * (fabsf(r.top) + lo);
-      const float x_lo = bin == BINS - 1 ? -INFINITY : r.top - hi - 2e-6f * (fabsf(r.top) + hi);
+      const float x_lo = r.below(bin);
       float n;
-      if (BY_COUNT) {
+      if (by_count) {
         n = bin == BINS - 1 ? 1e9f : float(sm.count[bin + 1] - cabove);
       } else if (bin == BINS - 1) {                   // nothing lies there
         n = 0.f;
@@ -303,102 +402,103 @@ __device__ void search(const Slice<T, CTAS>& slice, int ids, const Row& r, Smem&
         const float sum = float((u64(sm.hi[bin + 1]) << 32) + sm.lo[bin + 1] - above);
         n = sum / fmaxf(__expf(-float(bin + 1) / BINS_A_FOLD) * float(1ull << r.shift) * 0.99f - 1.f, 1.f);
       }
-      sm.bin = bin;
-      next(place_of<T>(key_of(x_lo), (1 << ids) - 1, ids), place_of<T>(key_of(x_hi), 0, ids), n);
+      next(bin, place_of<T>(key_of(x_lo), (1 << ids) - 1, ids), place_of<T>(key_of(x_hi), 0, ids), n);
     }
+    __syncthreads();
   }
+  bool alone = rank == 0 && sm.command[turn].bin < near;      // what is listed the first CTA reads by itself; the others wait until it is done
   for (;;) {
+    if (!alone) meet<CTAS>();
+    const Command now = of_cta<CTAS>(sm, 0).command[turn];
+    if (now.cut == DONE) break;
+    if (!alone) turn ^= 1;
     if (tid == 0) sm.n = 0;
-    meet<CTAS>();
-    const int bin = first.bin, cut = first.cut;
-    const u64 from = first.from, to = first.to;
-    if (cut >= 0) {
+    if (now.cut >= 0)
       for (int i = tid; i < FINE; i += THREADS) sm.fcount[i] = sm.flo[i] = sm.fhi[i] = 0;
+    __syncthreads();
+    if (alone) {                                      // a CTA's list to as many threads
+      const Smem& other = of_cta<CTAS>(sm, tid / (THREADS / CTAS));
+      const int n = int(other.n_near);
+      for (int i = tid % (THREADS / CTAS); i < n; i += THREADS / CTAS) {
+        const u64 place = other.near[i];
+        const float x = value_of(key_at<T>(place, ids));
+        if (r.bin(x) == now.bin) take<T>(now, r, by_count, place, x);
+      }
       __syncthreads();
-    }
-    auto take = [&](u64 place, float x) {
-      if (place < from || place > to) return;
-      if (cut >= 0) {
-        const uint32_t at = uint32_t((to - place) >> cut);
-        atomicAdd(&sm.fcount[at], 1u);
-        if (!BY_COUNT) add64(&sm.flo[at], &sm.fhi[at], r.weight(x));
-      } else {
-        const uint32_t slot = atomicAdd(&sm.n, 1u);
-        if (slot < LIST) sm.list[slot].place = place;
-      }
-    };
-    if (bin < near) {
-      for (int i = tid; i < int(sm.n_near); i += THREADS) {
-        const float x = value_of(key_at<T>(sm.near[i], ids));
-        if (r.bin(x) == bin) take(sm.near[i], x);
-      }
     } else {
-      slice.every([&](int id, float x) {
-        if (r.bin(x) != bin) return;
-        const uint32_t key = key_of(x);
-        if (key >= least) take(place_of<T>(key, id, ids), x);
-      });
-    }
-    meet<CTAS>();
-    if (cut < 0) {
-      uint32_t n = 0;
+      const float lowest = value_of(max(least, sizeof(T) == 2 ? uint32_t(now.from >> ids) << 16 : uint32_t(now.from >> ids)));
+      slice.fours(lowest == lowest ? lowest : -INFINITY, [&](int id, const float (&x)[4], int n) {
 #pragma unroll
-      for (int c = 0; c < CTAS; ++c) n += of_cta<CTAS>(sm, c).n;
-      if (n <= LIST) {
-        if (rank == 0) {                              // the tokens of all slices, ranked by comparison
-          Item mine;
-          if (tid < int(n)) {
-            int c = 0, at = tid;
-            if constexpr (CTAS > 1)
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t key = key_of(x[j]);
+          if (j < n && r.bin(x[j]) == now.bin && key >= least) take<T>(now, r, by_count, place_of<T>(key, id + j, ids), x[j]);
+        }
+      });
+      meet<CTAS>();
+    }
+    if (rank != 0) continue;
+    if (now.cut < 0) {
+      uint32_t n = 0;
+      if (alone) {
+        n = sm.n;
+      } else {
+#pragma unroll
+        for (int c = 0; c < CTAS; ++c) n += of_cta<CTAS>(sm, c).n;
+      }
+      if (n > LIST) {                                 // more than were to be expected
+        if (tid == 0) next(now.bin, now.from, now.to, float(n));
+      } else {                                        // the tokens of all slices, ranked by comparison
+        Item mine;
+        if (tid < int(n)) {
+          int c = 0, at = tid;
+          if constexpr (CTAS > 1)
+            if (!alone)
               for (; at >= int(of_cta<CTAS>(sm, c).n); ++c) at -= int(of_cta<CTAS>(sm, c).n);
-            mine.place = of_cta<CTAS>(sm, c).list[at].place;
-            mine.w = r.weight(value_of(key_at<T>(mine.place, ids)));
-          }
-          __syncthreads();
-          if (tid < int(n)) sm.list[tid] = mine;
-          __syncthreads();
-          // a power of two of neighbouring threads an element, each with its part of the others
-          int helpers = 1;
-          while (helpers < 32 && 2 * helpers * int(n) <= THREADS) helpers *= 2;
-          const int me = tid / helpers;
-          u64 over = 0;
-          uint32_t higher = 0;
-          if (me < int(n)) {
-            mine = sm.list[me];
-            for (int j = tid & (helpers - 1); j < int(n); j += helpers) {
-              const Item it = sm.list[j];
-              if (it.place > mine.place) { over += it.w; ++higher; }
-            }
-          }
-          for (int o = 1; o < helpers; o *= 2) {
-            over += __shfl_xor_sync(0xffffffffu, over, o);
-            higher += __shfl_xor_sync(0xffffffffu, higher, o);
-          }
-          if (me < int(n) && (tid & (helpers - 1)) == 0) {
-            const u64 start = BY_COUNT ? cabove + higher : above + over;
-            if (start <= z && z - start < (BY_COUNT ? 1 : mine.w)) { sm.place = mine.place; sm.above = above + over; sm.weight = mine.w; }
+          mine.place = of_cta<CTAS>(sm, c).list[at].place;
+          mine.w = r.weight(value_of(key_at<T>(mine.place, ids)));
+        }
+        __syncthreads();
+        if (tid < int(n)) sm.list[tid] = mine;
+        __syncthreads();
+        // a power of two of neighbouring threads an element, each with its part of the others
+        int helpers = 1;
+        while (helpers < 32 && 2 * helpers * int(n) <= THREADS) helpers *= 2;
+        const int me = tid / helpers;
+        u64 over = 0;
+        uint32_t higher = 0;
+        if (me < int(n)) {
+          mine = sm.list[me];
+          for (int j = tid & (helpers - 1); j < int(n); j += helpers) {
+            const Item it = sm.list[j];
+            if (it.place > mine.place) { over += it.w; ++higher; }
           }
         }
-        break;
+        for (int o = 1; o < helpers; o *= 2) {
+          over += __shfl_xor_sync(0xffffffffu, over, o);
+          higher += __shfl_xor_sync(0xffffffffu, higher, o);
+        }
+        if (me < int(n) && (tid & (helpers - 1)) == 0) {
+          const u64 start = by_count ? cabove + higher : above + over;
+          if (start <= z && z - start < (by_count ? 1 : mine.w)) { sm.place = mine.place; sm.above = above + over; sm.weight = mine.w; }
+        }
+        if (tid == 0) sm.command[turn].cut = DONE;
+        alone = false;                                // to the others
       }
-      if (rank == 0 && tid == 0) next(from, to, float(n));          // more than were to be expected
-      continue;
-    }
-    if (rank == 0) {
-      join<CTAS, FINE>(sm, [](Smem& x) { return x.fcount; }, [](Smem& x) { return x.flo; }, [](Smem& x) { return x.fhi; }, true);
-      const uint32_t all = running_sums<FINE>(sm.fcount, sm.flo, sm.fhi, sm, above, cabove);
-      const int at = covering<FINE, BY_COUNT>(sm.fcount, sm.flo, sm.fhi, sm, z);
+    } else {
+      if (!alone) join_parts<CTAS>(sm);
+      const uint32_t all = running_sums<FINE>(above, cabove);
+      const int at = covering<FINE>(by_count, z);
       above = (u64(sm.fhi[at]) << 32) + sm.flo[at];
       const uint32_t n = (at + 1 == FINE ? all : sm.fcount[at + 1]) - sm.fcount[at];
       cabove = sm.fcount[at];
       if (tid == 0) {
-        const u64 top = to - (u64(at) << cut), size = (u64(1) << cut) - 1;
-        sm.bin = bin;
-        next(top - from > size ? top - size : from, top, float(n));
+        const u64 top = now.to - (u64(at) << now.cut), size = (u64(1) << now.cut) - 1;
+        next(now.bin, top - now.from > size ? top - size : now.from, top, float(n));
       }
     }
+    __syncthreads();                                  // the command is there, and what it was found by has been read
   }
-  meet<CTAS>();                                       // everybody has read what this search used
+  turn ^= 1;
 }
 
 __device__ __forceinline__ u64 share(double part, u64 whole) {
@@ -410,10 +510,10 @@ __device__ __forceinline__ u64 share(double part, u64 whole) {
 template <typename T, int CTAS>
 __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  Smem& sm = own_smem();
   const int tid = threadIdx.x, V = p.V, rank = CTAS == 1 ? 0 : int(blockIdx.x % CTAS);
   const size_t at = blockIdx.x / CTAS;
-  if (tid == 0) { sm.best = 0; sm.sum = 0; sm.n_near = 0; }
+  if (tid == 0) { sm.best = 0; sm.best_id = 0; sm.sum = 0; sm.n_near = 0; }
   for (int i = tid; i < BINS; i += THREADS) sm.count[i] = sm.lo[i] = sm.hi[i] = 0;
   if (tid < TABLE) sm.table[tid] = exp2(-double(tid) / TABLE);
   meet<CTAS>();
@@ -425,22 +525,32 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
   const int top_k = p.top_k != nullptr ? p.top_k[at] : p.top_k_all;
 
   const Slice<T, CTAS> slice(row, V, rank, p.staged ? reinterpret_cast<uint4*>(smem_raw + (sizeof(Smem) + 15) / 16 * 16) : nullptr);
-  u64 best = 0;
-  slice.template every<true>([&](int id, float x) { best = max(best, (u64(key_of(x)) << 32) | uint32_t(~id)); });
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  uint32_t best = key_of(slice.peak());
+  best = __reduce_max_sync(0xffffffffu, best);
   if ((tid & 31) == 0) atomicMax(&sm.best, best);
   meet<CTAS>();
 #pragma unroll
   for (int c = 0; c < CTAS; ++c) best = max(best, of_cta<CTAS>(sm, c).best);
   Row r;
-  r.top = value_of(uint32_t(best >> 32));
+  r.top = value_of(best);
   const bool nothing = r.top == -INFINITY;
   if (!(temperature > 0.f) || nothing) {              // the largest, lowest id among equals; no logit above -inf: token 0 with probability 0
+    if (!nothing) {
+      slice.fours(r.top, [&](int id, const float (&x)[4], int n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (x[j] == r.top) atomicMax(&sm.best_id, ~uint32_t(id + j));
+      });
+      meet<CTAS>();
+    }
     if (rank == 0 && tid == 0) {
-      p.token[at] = nothing ? 0 : int64_t(~uint32_t(best));
+      uint32_t id = nothing ? ~0u : 0u;
+#pragma unroll
+      for (int c = 0; c < CTAS; ++c) id = max(id, of_cta<CTAS>(sm, c).best_id);
+      p.token[at] = int64_t(~id);
       if (p.prob != nullptr) p.prob[at] = nothing ? 0.f : 1.f;
     }
-    meet<CTAS>();                                     // a CTA's memory is there until everybody has read it
+    meet<CTAS>();                                     // as at the end
     return;
   }
   const double rate = 1.0 / fmax(double(temperature), 1e-5);
@@ -460,36 +570,49 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
   }
   int last = nucleus ? BINS - 2 : high;               // bins from here on have no say: only a nucleus needs the sum over what min-p cuts
   uint32_t least = 0;
+  int turn = 0;
   if (count) {
     // the k-th largest by counts alone, so that nobody takes weights of what lies below it
-    slice.every([&](int id, float x) { atomicAdd(&sm.count[r.bin(x)], 1u); });
+    slice.fours(-INFINITY, [&](int, const float (&x)[4], int n) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < n) atomicAdd(&sm.count[r.bin(x[j])], 1u);
+    });
     meet<CTAS>();
-    if (rank == 0) {
-      join<CTAS, BINS>(sm, [](Smem& x) { return x.count; }, [](Smem& x) { return x.lo; }, [](Smem& x) { return x.hi; }, true);
-      running_sums<BINS>(sm.count, sm.lo, sm.hi, sm, 0, 0);
-    }
-    search<T, CTAS, true>(slice, p.ids, r, sm, u64(top_k - 1), 0, 0);
+    join_counts<CTAS>(sm, rank);
+    if (rank == 0) running_sums<BINS>(0, 0);
+    search<T, CTAS>(slice, p.ids, r, true, u64(top_k - 1), 0, 0, turn);
     least = key_at<T>(of_cta<CTAS>(sm, 0).place, p.ids);
     if (sizeof(T) == 2) least &= 0xffff0000u;
     last = min(last, r.bin(value_of(key_at<T>(of_cta<CTAS>(sm, 0).place, p.ids))));
-    meet<CTAS>();
     for (int i = tid; i < BINS; i += THREADS) sm.lo[i] = sm.hi[i] = 0;
     __syncthreads();
   }
   const double border = double(min_p) * double(1ull << p.shift);
   u64 bordering = 0;
-  slice.every([&](int id, float x) {
-    const int b = r.bin(x);
-    if (b > last || b == BINS - 1) return;
-    const uint32_t key = key_of(x);
-    if (key < least) return;
-    const double scaled = r.scaled(x);
-    const u64 w = __double_as_longlong(scaled + 4503599627370496.0) & 0xfffffffffffffull;
-    if (b >= low && b <= high && scaled >= border) bordering += w;
-    if (w) add64(&sm.lo[b], &sm.hi[b], w);
-    if (b < NEAR && *static_cast<volatile uint32_t*>(&sm.n_near) <= NEAR_LIST) {
-      const uint32_t slot = atomicAdd(&sm.n_near, 1u);
-      if (slot < NEAR_LIST) sm.near[slot] = place_of<T>(key, id, p.ids);
+  slice.fours(fmaxf(r.below(min(last, BINS - 2)), count ? value_of(least) : -INFINITY), [&](int id, const float (&x)[4], int) {
+    u64 w[4];
+    int b[4];
+    uint32_t before[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      b[j] = r.bin(x[j]);
+      const bool in = b[j] <= last && b[j] < BINS - 1 && key_of(x[j]) >= least;
+      const double scaled = r.scaled(x[j]);
+      w[j] = in ? __double_as_longlong(scaled + 4503599627370496.0) & 0xfffffffffffffull : 0;
+      if (in && b[j] >= low && b[j] <= high && scaled >= border) bordering += w[j];
+      if (!in) b[j] = BINS - 1;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) before[j] = w[j] ? atomicAdd(&sm.lo[b[j]], uint32_t(w[j])) : 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t up = uint32_t(w[j] >> 32) + (before[j] + uint32_t(w[j]) < before[j] ? 1u : 0u);
+      if (up) atomicAdd(&sm.hi[b[j]], up);
+      if (b[j] < NEAR && *static_cast<volatile uint32_t*>(&sm.n_near) <= NEAR_LIST) {
+        const uint32_t slot = atomicAdd(&sm.n_near, 1u);
+        if (slot < NEAR_LIST) sm.near[slot] = place_of<T>(key_of(x[j]), id + j, p.ids);
+      }
     }
   });
   if (min_p > 0.f && bordering) atomicAdd(&sm.sum, bordering);
@@ -499,14 +622,14 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
   for (int c = 0; c < CTAS; ++c)
     if (of_cta<CTAS>(sm, c).n_near > NEAR_LIST) near = 0;
   u64 left = 0;
+  join_sums<CTAS>(sm, rank);
   if (rank == 0) {
-    join<CTAS, BINS>(sm, [](Smem& x) { return x.count; }, [](Smem& x) { return x.lo; }, [](Smem& x) { return x.hi; }, false);
     // the last bin's weights are 0, so that the sum before it is the whole
-    running_sums<BINS>(sm.count, sm.lo, sm.hi, sm, 0, 0);
+    running_sums<BINS>(0, 0);
     left = (u64(sm.hi[BINS - 1]) << 32) + sm.lo[BINS - 1];
   }
   if (nucleus) {
-    search<T, CTAS, false>(slice, p.ids, r, sm, share(double(top_p), left), least, near);
+    search<T, CTAS>(slice, p.ids, r, false, share(double(top_p), left), least, near, turn);
     if (rank == 0) left = sm.above + sm.weight;
   }
   if (min_p > 0.f && rank == 0) {
@@ -515,11 +638,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
     for (int c = 0; c < CTAS; ++c) sum += of_cta<CTAS>(sm, c).sum;
     left = max(min(left, sum), u64(1) << p.shift);             // min_p beyond 1 leaves the largest
   }
-  search<T, CTAS, false>(slice, p.ids, r, sm, rank == 0 ? share(double(p.u[at]), left) : 0, least, near);
+  search<T, CTAS>(slice, p.ids, r, false, rank == 0 ? share(double(p.u[at]), left) : 0, least, near, turn);
   if (rank == 0 && tid == 0) {
     p.token[at] = id_at<T>(sm.place, p.ids);
     if (p.prob != nullptr) p.prob[at] = float(r.scaled(value_of(key_at<T>(sm.place, p.ids))) / double(left));
   }
+  meet<CTAS>();                                       // a CTA's memory is there until everybody has read it
 }
 
 template <typename T, int CTAS>
@@ -534,7 +658,8 @@ int launch_rows_by(Sampling p, int n_rows, cudaStream_t stream) {
   return JB200_OK;
 }
 
-// CTAs a row: as many as two a SM leave room for, slices of 4096 tokens or more
+// CTAs a row: as many as two a SM leave room for (64 rows of 50257 bf16, every setting of its own: 47 us; with one a SM 57), slices of 4096 tokens
+// or more
 template <typename T>
 int launch_rows(const Sampling& p, int n_rows, cudaStream_t stream) {
   const int most = 2 * sm_count() / n_rows, wide = p.V / 4096, ctas = most < wide ? most : wide;
