@@ -3,6 +3,10 @@
 //   residual_norm:  x' = x + scale * (y / rms(y) * w_after [* silu(gate)]),  xn = x' / rms(x') * w_before
 // after jarvis_engine/jarvis_model.py:25-26 (RMSNorm) and :428-436 (the residual sums around it).  One pass over memory: rows stay in
 // registers between the sums and the products; sums are f32, each result is rounded once.
+//
+// Bound by memory: 16384 rows of 1024 of residual_norm move 201 MB in 36 us, 5.6 TB/s.  The head norm of as many rows with a gate moves 100 MB in 20 us;
+// 3 of them are the gate's exponentials and reciprocals (without: 17), and more vectors a thread, fewer threads or one reciprocal for two elements
+// take longer.  Few rows take the launch and one chain of two reads, two sums and a write.
 #include "common.cuh"
 #include "launchers.h"
 
@@ -45,7 +49,7 @@ __global__ void __launch_bounds__(256) group_norm_kernel(const TY* __restrict__ 
   const long long padded = (vectors + 31) / 32 * 32;                    // whole warps: the sums go over lanes
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < padded; i += gridDim.x * 256ll) {
     const bool on = i < vectors;
-    const long long row = on ? i / vectors_a_row : 0;
+    const long long row = !on ? 0 : vectors <= 0xffffffffll ? uint32_t(i) / uint32_t(vectors_a_row) : i / vectors_a_row;
     const int col = on ? int(i - row * vectors_a_row) * 8 : 0;
     float v[8] = {}, g[8], ww[8];
     if (on) load8(y + row * ldy + col, v);
@@ -79,24 +83,22 @@ struct RowNorm {
   float eps;
 };
 
-// TPR threads a row, V vectors of eight columns a thread.  32: a warp a row, eight rows a CTA; more: a CTA a row.
-template <typename TY, typename TO, int TPR, int V>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) row_norm_kernel(RowNorm p) {
-  __shared__ float part[2][32];
-  const int t = threadIdx.x % TPR;
-  const long long row = TPR == 32 ? blockIdx.x * 8ll + threadIdx.x / 32 : blockIdx.x;
+// A CTA a row, V vectors of eight columns a thread.  128 threads up to 1024 columns: a warp a row, eight rows a CTA, reads four times as much at once
+// but took 16384 rows of 1024 in 52 us instead of 39, 2048 in 19 instead of 12.
+template <typename TY, typename TO, int THREADS, int V>
+__global__ void __launch_bounds__(THREADS) row_norm_kernel(RowNorm p) {
+  __shared__ float part[2][THREADS / 32];
+  const int t = threadIdx.x;
+  const long long row = blockIdx.x;
   pdl_wait();
   pdl_trigger();
-  if (row >= p.n_rows) return;                                          // whole warps, or the whole CTA
   auto row_sum = [&](float s, float* slots) {
     s = warp_sum(s);
-    if constexpr (TPR > 32) {
-      if ((t & 31) == 0) slots[t >> 5] = s;
-      __syncthreads();
-      s = 0.f;
+    if ((t & 31) == 0) slots[t >> 5] = s;
+    __syncthreads();
+    s = 0.f;
 #pragma unroll
-      for (int i = 0; i < TPR / 32; ++i) s += slots[i];
-    }
+    for (int i = 0; i < THREADS / 32; ++i) s += slots[i];
     return s;
   };
   const TY* y = static_cast<const TY*>(p.y) + row * p.ldy;
@@ -106,7 +108,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) row_norm_kernel(RowNorm
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = (i * TPR + t) * 8;
+    const int c = (i * THREADS + t) * 8;
     if (c < p.C) {
       load8(y + c, v[i]);
       if (p.x != nullptr) load8(p.x + row * p.C + c, x[i]);
@@ -117,7 +119,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) row_norm_kernel(RowNorm
   float s2 = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = (i * TPR + t) * 8;
+    const int c = (i * THREADS + t) * 8;
     if (c < p.C) {
       float w[8];
       load8(p.w_after + c, w);
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) row_norm_kernel(RowNorm
   const float r2 = rsqrtf(row_sum(s2, part[1]) / float(p.C) + p.eps);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = (i * TPR + t) * 8;
+    const int c = (i * THREADS + t) * 8;
     if (c < p.C) {
       float w[8];
       load8(p.w_before + c, w);
@@ -163,12 +165,8 @@ constexpr int MAX_C = 8192;
 
 template <typename TY, typename TO>
 void launch_rows(const RowNorm& p, cudaStream_t stream) {
-  if (p.C > 1024)
-    launch_dep(row_norm_kernel<TY, TO, 256, 4>, p.n_rows, 256, 0, stream, p);
-  else if (p.n_rows < 4 * sm_count())
-    launch_dep(row_norm_kernel<TY, TO, 128, 1>, p.n_rows, 128, 0, stream, p);
-  else
-    launch_dep(row_norm_kernel<TY, TO, 32, 4>, (p.n_rows + 7) / 8, 256, 0, stream, p);
+  if (p.C > 1024) launch_dep(row_norm_kernel<TY, TO, 256, 4>, p.n_rows, 256, 0, stream, p);
+  else launch_dep(row_norm_kernel<TY, TO, 128, 1>, p.n_rows, 128, 0, stream, p);
 }
 
 int check_norm(const char* what, const void* y, int y_dtype, long long ldy, const float* w, const void* gate, long long ldg, const void* out,
