@@ -155,9 +155,13 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 //   warps 14, 15       P
 // The products are tcgen05.mma, 128 rows at a time: a chunk has 64, so that the operand is there twice (K twice in memory; a second reading
 // of T^T and K, MN-major) and all four of a group's warps find 64 rows in their lanes; for P it is [K; Q], of Q and P as operands the
-// upper half is what happens to follow, in lanes that nobody reads.  Both terms of S, X and U (below) are one operand of 128 columns: the product reads its other operand
-// once for both, and what bounds these small products is reading (6 KB in 48 cycles, 8 KB in 64, for 32 and 64 of mathematics).  T's blocks come from
-// mma.sync: products of 16 x 16.
+// upper half is what happens to follow, in lanes that nobody reads.  Both terms of S, X and U (below) are one operand of 128 columns: the product
+// reads its other operand once for both, and what bounds these small products is reading (6 KB in 48 cycles, 8 KB in 64, for 32 and 64 of
+// mathematics).  T's blocks come from mma.sync: products of 16 x 16.
+//
+// Bound by that chain, some 5900 cycles a chunk on every SM that has a head (8 sequences of 2048 tokens, 16 heads: 107 us, where reading and writing
+// takes 21).  With mma.sync alone a chunk took 10800, with these warps' parts but all products unrolled 9600: 77 KB of code, which the SMs fetch
+// again and again.
 //
 // Precision: the state is f32 and stays it.  What it is multiplied by and into is f16 in two terms, x = hi + lo (22 bits), at a power of two
 // that brings a bound of its size to 2^15, so that f16's subnormals lie 2^-39 below: |X|, |U| <= 16 max|S| + 130 max|b v| and
@@ -167,7 +171,6 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 // is one term, 2^-12 of a value where the output's own rounding is 2^-9.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int CHUNK = 64;
-constexpr int CHUNK_TOKENS = 24;          // from so many tokens on
 constexpr int TILE = CHUNK * D * 2;        // bytes of 64 rows of 128, the 16-byte units of row r at unit ^ (r & 7): the 128-byte swizzle
 constexpr int STAGES = 3;
 constexpr int STATE = 128, GROUP = 128;    // threads of the state's group, of a preparing one
@@ -237,7 +240,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const float2 (&x)[8]) {
                : "memory");
 }
 // The CTA's barriers.  Ready and free of a stage: the preparing group arrives and waits, the others wait and arrive.
-enum { BAR_GROUP = 1 /* + group */, BAR_STATE = 3, BAR_READY = 4 /* + stage */, BAR_FREE = 7 /* + stage */, BAR_TAKEN = 10, BAR_GIVEN = 11, BAR_PAIR = 12 /* + group */, BAR_SCORES = 14 };
+enum {
+  BAR_GROUP = 1 /* + group */, BAR_STATE = 3, BAR_READY = 4 /* + stage */, BAR_FREE = 7 /* + stage */, BAR_TAKEN = 10, BAR_GIVEN = 11,
+  BAR_PAIR = 12 /* + group */, BAR_SCORES = 14
+};
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
@@ -363,8 +369,8 @@ __device__ __forceinline__ void fetch_half(uint4 (&x)[4], const __nv_bfloat16* a
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = on ? load_now(static_cast<const void*>(at + 8 * i)) : make_uint4(0, 0, 0, 0);
 }
-// ... and to f16 in a tile (`twice`: and in the next one), times the power of two s that brings the row's norm into [1, 2); returns the sum of squares after that.  A sum of
-// squares beyond f32's range makes the row NaN, one below it makes it 0.
+// ... and to f16 in a tile (`twice`: and in the next one), times the power of two s that brings the row's norm into [1, 2); returns the sum of
+// squares after that.  A sum of squares beyond f32's range makes the row NaN, one below it makes it 0.
 __device__ __forceinline__ float convert_half(const uint4 (&x)[4], uint8_t* tile, bool twice, int row, int half, float& s) {
   float ss = 0.f, other = 0.f;
 #pragma unroll
@@ -1000,21 +1006,39 @@ __global__ void __launch_bounds__(3 * GROUP + (OUT ? 2 * OUT_THREADS : 0), 1) de
   }
 }
 
-// The state before every segment from what the segments add and multiply by: S_(s+1) = S_s M_s + N_s.  Eight value rows a CTA.
+// The state before every segment from what the segments add and multiply by: S_(s+1) = S_s M_s + N_s.  Eight value rows a CTA.  A chain of products
+// of 8 x 64 x 64, each of them short: the next three M are on their way into shared memory meanwhile (read where they are needed, a segment took 4 us).
+constexpr int JOIN_STAGES = 4;
+constexpr int JOIN_SMEM = JOIN_STAGES * D * D * 4;
 __global__ void __launch_bounds__(128) delta_join_kernel(DeltaParams p) {
+  extern __shared__ __align__(16) float join_m[];
   __shared__ __align__(16) float rows[2][8][D];
   const int bh = blockIdx.x >> 3, r = threadIdx.x >> 4, c = (threadIdx.x & 15) * 4, v = (blockIdx.x & 7) * 8 + r;
   pdl_wait();
   pdl_trigger();
+  auto fetch = [&](int s) {
+    if (s + 1 < p.segments) {
+      const float* m = p.pieces + piece_at(p.segments, bh, p.segments - 1 + s);
+      const uint32_t to = smem_u32(join_m + (s % JOIN_STAGES) * D * D);
+#pragma unroll
+      for (int i = 0; i < D * D / 4 / 128; ++i) copy_async_16(to + (i * 128 + threadIdx.x) * 16, m + (i * 128 + threadIdx.x) * 4);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto added = [&](int s) { return reinterpret_cast<float4*>(p.pieces + piece_at(p.segments, bh, s) + v * D + c); };
+  for (int s = 1; s < JOIN_STAGES; ++s) fetch(s);
   if (p.s_in == p.s_out && p.s_in != nullptr)        // the last segment may write it before the first one has read it
     *reinterpret_cast<float4*>(p.pieces + piece_at(p.segments, bh, 2 * p.segments - 2) + v * D + c) =
         *reinterpret_cast<const float4*>(p.s_in + size_t(bh) * D * D + v * D + c);
-  *reinterpret_cast<float4*>(&rows[0][r][c]) = *reinterpret_cast<const float4*>(p.pieces + piece_at(p.segments, bh, 0) + v * D + c);
+  *reinterpret_cast<float4*>(&rows[0][r][c]) = *added(0);
+  float4 next = *added(1);                           // three segments or more
   for (int s = 1; s + 1 < p.segments; ++s) {
-    float4* n = reinterpret_cast<float4*>(p.pieces + piece_at(p.segments, bh, s) + v * D + c);
-    const float* m = p.pieces + piece_at(p.segments, bh, p.segments - 1 + s) + c;
-    float4 sum = *n;
-    __syncthreads();
+    float4 sum = next;
+    if (s + 2 < p.segments) next = *added(s + 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(JOIN_STAGES - 2) : "memory");
+    __syncthreads();                                 // everybody's part of M_s is there, and nobody reads M_(s-1)
+    fetch(s + JOIN_STAGES - 1);
+    const float* m = join_m + (s % JOIN_STAGES) * D * D + c;
     const float* row = rows[(s + 1) & 1][r];
 #pragma unroll 16
     for (int k = 0; k < D; ++k) {
@@ -1026,13 +1050,19 @@ __global__ void __launch_bounds__(128) delta_join_kernel(DeltaParams p) {
       sum.w = fmaf(f, x.w, sum.w);
     }
     *reinterpret_cast<float4*>(&rows[s & 1][r][c]) = sum;
-    *n = sum;
+    *added(s) = sum;
   }
 }
 
-// Segments of a sequence where sequences and heads alone leave SMs idle.  In chunks' time, about 3 us: a pass over the tokens costs its chunks on as many
-// waves of CTAs as it has (1 CTA an SM), the pieces' pass has 2 n - 3 CTAs a head for the outputs' n; filling the pipeline and joining
-// come to about 6 (measured; the smaller sum wins, segments only by a tenth).
+// In chunks from so many tokens on.  A chunk's pass takes as long for one token as for 64, a token's step the longer the more heads there are.  us
+// token by token / in chunks: 16 heads, 8 tokens 11.4 / 12.8, 16 tokens 16.4 / 12.7; 256 heads, 8 tokens 16.0 / 20.9, 16 tokens 24.1 / 21.5;
+// 1024 heads, 16 tokens 46 / 61, 24 tokens 63.5 / 61.7.
+int chunk_tokens(int heads) { return heads < 2 * sm_count() ? 12 : 24; }
+
+// Segments of a sequence where sequences and heads alone leave SMs idle.  In chunks' time, about 3 us: a pass over the tokens costs its chunks, and one
+// to fill the pipeline, on as many waves of CTAs as it has (1 CTA an SM); the pieces' pass has 2 n - 3 CTAs a head for the outputs' n; the join takes 1
+// and a quarter a segment.  The smaller sum wins, segments only by a tenth.  16 heads, us whole / in segments: 512 tokens 35 / 32 (not taken), 1024
+// 60 / 42, 4096 209 / 86, 16384 797 / 261; 2 sequences of 2048 110 / 80; with 4 sequences of 2048 there is nothing to gain.
 int segments_of(int B, int T, int H) {
   const long long sms = sm_count(), heads = (long long)B * H, chunks = (T + CHUNK - 1) / CHUNK;
   auto waves = [&](long long ctas) { return (ctas + sms - 1) / sms; };
@@ -1042,7 +1072,7 @@ int segments_of(int B, int T, int H) {
   for (int n = 3; n <= 32 && heads * n <= 2 * sms; ++n) {
     const long long part = (chunks + n - 1) / n;
     if ((chunks + part - 1) / part != n) continue;             // the last ones would be empty
-    const double cost = double(part) * double(waves(heads * (2 * n - 3)) + waves(heads * n)) + 6.0 + 0.25 * n;
+    const double cost = (double(part) + 1.0) * double(waves(heads * (2 * n - 3)) + waves(heads * n)) + 1.0 + 0.25 * n;
     if (cost < least) { least = cost; best = n; }
   }
   return best;
@@ -1051,7 +1081,7 @@ int segments_of(int B, int T, int H) {
 }  // namespace
 
 size_t gated_delta_scratch_bytes(int B, int T, int H) {
-  if (B < 1 || H < 1 || T < CHUNK_TOKENS) return 0;
+  if (B < 1 || H < 1 || T < 1) return 0;
   const int n = segments_of(B, T, H);
   return n == 1 ? 0 : piece_at(n, B * H, 0) * sizeof(float);
 }
@@ -1084,7 +1114,7 @@ int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream)
   p.what = ALL;
   p.seg_chunks = (T + CHUNK - 1) / CHUNK;
   p.pieces = static_cast<float*>(scratch);
-  if (T >= CHUNK_TOKENS) {
+  if (T >= chunk_tokens(B * H)) {
     JB_MAX_SMEM(delta_chunk_kernel<true>, CHUNK_SMEM);
     JB_MAX_SMEM(delta_chunk_kernel<false>, CHUNK_SMEM);
     if (scratch != nullptr) {
@@ -1096,7 +1126,8 @@ int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream)
         p.what = PIECES;
         launch_dep(delta_chunk_kernel<false>, B * H * (2 * n - 3), STATE + 2 * GROUP, CHUNK_SMEM, stream, p, device_status_ptr());
         JB_LAUNCH_CHECK("delta_chunk_kernel");
-        launch_dep(delta_join_kernel, B * H * 8, 128, 0, stream, p);
+        JB_MAX_SMEM(delta_join_kernel, JOIN_SMEM);
+        launch_dep(delta_join_kernel, B * H * 8, 128, JOIN_SMEM, stream, p);
         JB_LAUNCH_CHECK("delta_join_kernel");
         p.what = p.o != nullptr ? ALL : LAST;
       }
@@ -1108,6 +1139,7 @@ int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream)
     JB_LAUNCH_CHECK("delta_chunk_kernel");
     return JB200_OK;
   }
+  // rows a lane: one for few heads (16: 6.5 us for a token, with four 8.0; 256: 8.2 and 8.6), four for many (304: 8.3, with one 9.8; 4096: 28 and 42)
   if (B * H < 2 * sm_count())
     launch_dep(delta_step_kernel<1>, B * H * 4, 128, 0, stream, p);
   else
