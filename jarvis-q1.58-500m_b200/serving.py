@@ -21,21 +21,26 @@ take part in it; their state is reset on release so that it stays finite.
 from __future__ import annotations
 
 import collections
+import math
 import time
 from typing import Dict, List, Optional
 
 import torch
 
+TOP_K_OF_ALL = 1024          # what one sampling kernel for all rows takes
+
 
 class Request:
-    """Same fields as the reference's Request (exp_batching_continuous.py:131-139)."""
+    """Same fields as the reference's Request (exp_batching_continuous.py:131-139); `sampling`: settings of this request's own, any of
+    temperature, top_k, top_p and min_p (what it leaves out is the engine's)."""
 
-    def __init__(self, req_id: int, prompt_tokens: List[int], max_new_tokens: int):
+    def __init__(self, req_id: int, prompt_tokens: List[int], max_new_tokens: int, sampling: Optional[Dict[str, float]] = None):
         if len(prompt_tokens) == 0:
             raise ValueError("Request: the prompt must hold at least one token")
         self.req_id = req_id
         self.prompt_tokens = list(prompt_tokens)
         self.max_new_tokens = max_new_tokens
+        self.sampling = None if sampling is None else dict(sampling)
         self.generated_tokens: List[int] = []
         self.is_finished = False
         self.arrival_time = time.time()
@@ -46,8 +51,8 @@ class Request:
 class ContinuousBatchingScheduler:
     """Slot policy of exp_batching_continuous.py:141-177 over an engine with
     `admit(slot, prompt_tokens, max_new_tokens)`, `release(slot)` and `step(active_slots) -> {slot: token}`.
-    A request the engine refuses (ValueError from `admit`: its positions would run past the engine's limit)
-    is retired at once, unfinished, with the message in `req.error`; the slot goes to the next request."""
+    A request the engine refuses (ValueError from `admit`: its positions would run past the engine's limit, or
+    it has sampling settings, passed as `sampling`, that the engine does not take) is retired at once, unfinished, with the message in `req.error`; the slot goes to the next request."""
 
     def __init__(self, engine, max_batch_size: int = 8, eos_token: Optional[int] = None):
         self.engine = engine
@@ -67,7 +72,8 @@ class ContinuousBatchingScheduler:
             while slot not in self.active_slots and self.waiting_queue:
                 req = self.waiting_queue.popleft()
                 try:
-                    self.engine.admit(slot, req.prompt_tokens, req.max_new_tokens)
+                    own = {} if req.sampling is None else {"sampling": req.sampling}
+                    self.engine.admit(slot, req.prompt_tokens, req.max_new_tokens, **own)
                 except ValueError as exc:
                     req.error = str(exc)
                     req.finish_time = time.time()
@@ -99,22 +105,55 @@ class ContinuousBatchingScheduler:
         return it
 
 
+SAMPLING = ("temperature", "top_k", "top_p", "min_p")
+
+
+def check_sampling(settings: Dict[str, float]) -> Dict[str, float]:
+    """Settings of a draw, with None as what leaves that cut out; ValueError for anything that is none."""
+    unknown = sorted(set(settings) - set(SAMPLING))
+    if unknown:
+        raise ValueError(f"sampling settings are {', '.join(SAMPLING)}, not {', '.join(unknown)}")
+    out = {}
+    for name, value in settings.items():
+        try:
+            v = 0.0 if value is None else float(value)
+        except (TypeError, ValueError):
+            raise ValueError(f"{name} must be a number, got {value!r}") from None
+        if not math.isfinite(v):
+            raise ValueError(f"{name} must be finite, got {value}")
+        if name == "top_k" and (v != int(v) or not 0 <= v < 2 ** 31):
+            raise ValueError(f"top_k must be an int, 0 or None for the whole vocabulary, got {value}")
+        if name in ("top_p", "min_p") and not 0.0 <= v <= 1.0:
+            raise ValueError(f"{name} must lie in [0, 1], got {value}")
+        out[name] = int(v) if name == "top_k" else v
+    return out
+
+
 class CudaDecodeEngine:
     """Per-slot recurrent state + one CUDA-graphed batched step + the sampling kernel.
 
     temperature <= 0 selects argmax.  `seed` fixes the uniform numbers fed to the sampling kernel.
+    With `per_request` a request may bring settings of its own, and every slot draws by its own (`ops.sample_rows`); so do engines with
+    a min_p, or with a top_k that is not 1..1024 (0, None: the whole vocabulary, e.g. for a nucleus of it).  Others draw by `ops.sample`.
     `record=True` keeps, per iteration, the step's inputs and logits (for tests and debugging)."""
 
     def __init__(self, model, max_batch_size: int = 8, max_position: int = 4096, temperature: float = 0.7,
                  top_k: int = 50, top_p: float = 0.9, seed: int = 0, pad_token: int = 0, use_cuda_graph: bool = True,
-                 record: bool = False):
+                 record: bool = False, min_p: float = 0.0, per_request: bool = False):
         from . import ops
         from .modules import DecodeSession
         self._ops = ops
         self.model = model
         self.B = max_batch_size
         self.max_position = max_position
-        self.temperature, self.top_k, self.top_p = temperature, top_k, top_p
+        self.temperature, self.top_k, self.top_p, self.min_p = temperature, top_k, top_p, min_p
+        self.per_request = per_request
+        greedy = temperature is None or temperature <= 0.0
+        self.rows = None
+        if per_request or not greedy and (min_p or not top_k or not 1 <= top_k <= TOP_K_OF_ALL):
+            self.defaults = check_sampling(dict(zip(SAMPLING, (temperature, top_k, top_p, min_p))))
+            self.rows = {name: torch.full((self.B,), v, dtype=torch.int32 if name == "top_k" else torch.float32,
+                                          device=model.tok_emb.weight.device) for name, v in self.defaults.items()}
         self.pad_token = pad_token
         dev = model.tok_emb.weight.device
         self.device = dev
@@ -144,13 +183,21 @@ class CudaDecodeEngine:
         self.session.positions[slot] = 0
         self.next_token[slot, 0] = self.pad_token
 
-    def admit(self, slot: int, prompt_tokens: List[int], max_new_tokens: int = 0):
+    def admit(self, slot: int, prompt_tokens: List[int], max_new_tokens: int = 0, sampling: Optional[Dict[str, float]] = None):
         """Prefill prompt[:-1] into the slot's state; the step of this iteration consumes prompt[-1].
         The RoPE table captured in the step's graph has `max_position` rows and the kernels clamp positions
-        to it silently, so a request whose last generated token would sit beyond the table is refused here."""
+        to it silently, so a request whose last generated token would sit beyond the table is refused here.
+        `sampling`: settings of the request's own (temperature, top_k, top_p, min_p), with `per_request`."""
         if len(prompt_tokens) + max(int(max_new_tokens), 0) > self.max_position:
             raise ValueError(f"prompt of {len(prompt_tokens)} tokens + {max_new_tokens} new tokens exceeds "
                              f"max_position={self.max_position}")
+        if sampling is not None:
+            if not self.per_request:
+                raise ValueError("a request with sampling settings of its own needs an engine with per_request=True")
+            sampling = check_sampling(sampling)
+        if self.per_request:
+            for name, value in {**self.defaults, **(sampling or {})}.items():
+                self.rows[name][slot] = value
         if len(prompt_tokens) == 1:
             self._zero_slot(slot)           # longer prompts overwrite every tensor of the slot below
         if len(prompt_tokens) > 1:
@@ -181,7 +228,11 @@ class CudaDecodeEngine:
         rows = logits[:, 0, :]
         greedy = self.temperature is None or self.temperature <= 0.0
         u = None if greedy else torch.rand((self.B,), dtype=torch.float32, device=self.device, generator=self.gen)
-        tok = ops.sample(rows, u, temperature=0.0 if greedy else self.temperature, top_k=self.top_k, top_p=self.top_p)
+        if self.rows is not None:
+            u = torch.rand((self.B,), dtype=torch.float32, device=self.device, generator=self.gen) if u is None else u
+            tok = ops.sample_rows(rows, u, **self.rows)
+        else:
+            tok = ops.sample(rows, u, temperature=0.0 if greedy else self.temperature, top_k=self.top_k, top_p=self.top_p)
         if self.record is not None:
             self.record[-1]["logits"] = rows.float().clone()
             self.record[-1]["tokens"] = tok.clone()

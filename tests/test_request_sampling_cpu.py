@@ -1,0 +1,58 @@
+"""Sampling settings of requests: what they may be, and their way through the scheduler."""
+import math
+
+import pytest
+
+from jarvis_b200 import serving
+
+
+class _Engine:
+    def __init__(self):
+        self.calls = []
+
+    def admit(self, slot, prompt_tokens, max_new_tokens=0, **own):
+        if "sampling" in own:
+            serving.check_sampling(own["sampling"])
+        self.calls.append((slot, tuple(prompt_tokens), own))
+
+    def release(self, slot):
+        pass
+
+    def step(self, active_slots):
+        return {s: 7 for s in active_slots}
+
+
+def test_settings_reach_the_engine_with_the_requests_that_have_them():
+    eng = _Engine()
+    sched = serving.ContinuousBatchingScheduler(eng, max_batch_size=2)
+    mine = {"temperature": 0.5, "min_p": 0.1}
+    sched.add_request(serving.Request(0, [1], 2))
+    sched.add_request(serving.Request(1, [2], 2, sampling=mine))
+    mine["temperature"] = 9.0                                    # the caller's dict is the caller's
+    sched.add_request(serving.Request(2, [3], 2, sampling={"top_p": 1.5}))
+    sched.run()
+    assert eng.calls == [(0, (1,), {}), (1, (2,), {"sampling": {"temperature": 0.5, "min_p": 0.1}})]
+    by_id = {r.req_id: r for r in sched.completed}
+    assert "top_p" in by_id[2].error and not by_id[2].is_finished and by_id[1].is_finished
+
+
+def test_settings_that_are_none():
+    check = serving.check_sampling
+    assert check({}) == {}
+    assert check({"temperature": None, "top_k": None, "top_p": None, "min_p": None}) == {"temperature": 0.0, "top_k": 0, "top_p": 0.0, "min_p": 0.0}
+    assert check({"temperature": 1, "top_k": 40.0, "top_p": 1}) == {"temperature": 1.0, "top_k": 40, "top_p": 1.0}
+    for bad, text in (({"typical_p": 0.5}, "typical_p"), ({"temperature": math.nan}, "finite"), ({"temperature": math.inf}, "finite"), ({"top_k": -1}, "top_k"),
+                      ({"top_k": 2.5}, "top_k"), ({"top_k": 2 ** 31}, "top_k"), ({"top_p": -0.1}, "top_p"), ({"top_p": 1.1}, "top_p"), ({"min_p": 2}, "min_p"),
+                      ({"top_p": "0.9x"}, "number"), ({"top_k": [1]}, "number")):
+        with pytest.raises(ValueError, match=text):
+            check(bad)
+
+
+def test_an_engine_for_all_refuses_a_requests_own_before_it_touches_the_slot():
+    eng = serving.CudaDecodeEngine.__new__(serving.CudaDecodeEngine)
+    eng.max_position, eng.per_request = 64, False
+    with pytest.raises(ValueError, match="per_request"):
+        eng.admit(0, [1, 2], max_new_tokens=4, sampling={"temperature": 1.0})
+    eng.per_request = True
+    with pytest.raises(ValueError, match="min_p"):
+        eng.admit(0, [1, 2], max_new_tokens=4, sampling={"min_p": -1.0})
