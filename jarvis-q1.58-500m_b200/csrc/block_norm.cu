@@ -4,9 +4,9 @@
 // after jarvis_engine/jarvis_model.py:25-26 (RMSNorm) and :428-436 (the residual sums around it).  One pass over memory: rows stay in
 // registers between the sums and the products; sums are f32, each result is rounded once.
 //
-// Bound by memory: 16384 rows of 1024 of residual_norm move 201 MB in 36 us, 5.6 TB/s.  The head norm of as many rows with a gate moves 100 MB in 20 us;
-// 3 of them are the gate's exponentials and reciprocals (without: 17), and more vectors a thread, fewer threads or one reciprocal for two elements
-// take longer.  Few rows take the launch and one chain of two reads, two sums and a write.
+// Bound by memory: 16384 rows of 1024 of residual_norm move 201 MB in 36 us, 5.6 TB/s.  The head norm of as many rows with a gate moves 100 MB in
+// 18.5 us, next to its instructions (with exponentials and quotients that mind subnormals, and a division for every vector's row, 21.3); a second
+// vector a thread, or one read ahead, took longer.  Few rows take the launch and one chain of two reads, two sums and a write.
 #include "common.cuh"
 #include "launchers.h"
 
@@ -36,8 +36,14 @@ __device__ __forceinline__ float sumsq8(const float (&v)[8]) {
   for (int j = 0; j < 8; ++j) s = fmaf(v[j], v[j], s);
   return s;
 }
-// x / (1 + e^-x); e^-x beyond the range gives 0 as it should
-__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+// x / (1 + e^-x); e^-x beyond the range gives 0 as it should, and subnormal ones are 0 beside 1.  The flushing forms, since the others spend more on
+// subnormals than on the rest, and instructions bound the head norm.
+__device__ __forceinline__ float silu(float x) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.44269504f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return x * r;
+}
 
 // Groups of 8 to 256 columns, a power of two: group / 8 neighbouring lanes hold one, wherever rows end.
 template <typename TY, typename TO>
@@ -46,19 +52,27 @@ __global__ void __launch_bounds__(256) group_norm_kernel(const TY* __restrict__ 
   pdl_wait();
   pdl_trigger();
   const int lanes = group >> 3;
+  const float share = 1.f / float(group);                               // exact
+  const bool dense = ldy == size_t(vectors_a_row) * 8 && (gate == nullptr || ldg == ldy);   // then nothing asks for the row
   const long long padded = (vectors + 31) / 32 * 32;                    // whole warps: the sums go over lanes
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < padded; i += gridDim.x * 256ll) {
     const bool on = i < vectors;
-    const long long row = !on ? 0 : vectors <= 0xffffffffll ? uint32_t(i) / uint32_t(vectors_a_row) : i / vectors_a_row;
-    const int col = on ? int(i - row * vectors_a_row) * 8 : 0;
+    size_t at_y = size_t(i) * 8, at_g = at_y;
+    const int col = int(at_y) & (group - 1);                            // rows are whole groups
+    if (!dense) {
+      const long long row = vectors <= 0xffffffffll ? uint32_t(i) / uint32_t(vectors_a_row) : i / vectors_a_row;
+      const size_t in_row = at_y - size_t(row) * vectors_a_row * 8;
+      at_y = row * ldy + in_row;
+      at_g = row * ldg + in_row;
+    }
     float v[8] = {}, g[8], ww[8];
-    if (on) load8(y + row * ldy + col, v);
-    if (on && gate != nullptr) load8(gate + row * ldg + col, g);
+    if (on) load8(y + at_y, v);
+    if (on && gate != nullptr) load8(gate + at_g, g);
     float s = sumsq8(v);
     for (int o = 1; o < lanes; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (!on) continue;
-    const float r = rsqrtf(s / float(group) + eps);
-    load8(w + (col & (group - 1)), ww);
+    const float r = rsqrtf(fmaf(s, share, eps));
+    load8(w + col, ww);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = v[j] * r * ww[j];
     if (gate != nullptr)
@@ -205,7 +219,7 @@ int launch_gated_norm(const void* y, int y_dtype, long long ldy, const float* w,
     by_types(y_dtype, out_dtype, [&](auto ty, auto to) {
       using TY = decltype(ty);
       using TO = decltype(to);
-      launch_dep(group_norm_kernel<TY, TO>, unsigned(blocks < 16ll * sm_count() ? blocks : 16ll * sm_count()), 256, 0, stream, static_cast<const TY*>(y),
+      launch_dep(group_norm_kernel<TY, TO>, unsigned(blocks < 8ll * sm_count() ? blocks : 8ll * sm_count()), 256, 0, stream, static_cast<const TY*>(y),
                  size_t(ldy), w, static_cast<const TY*>(gate), size_t(ldg), static_cast<TO*>(out), C / 8, vectors, group, eps);
     });
     JB_LAUNCH_CHECK("group_norm_kernel");
