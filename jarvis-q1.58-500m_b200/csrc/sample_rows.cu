@@ -13,12 +13,13 @@
 // missed only where u lies within some 1e-12 of a border.  A cluster of CTAs has a row, a slice each (in shared memory where it fits), with as many
 // CTAs as keep the SMs busy.  A histogram of the sums (for top-k of the counts) over 2048 bins of 1/32 of an e-fold finds the bin that covers z.
 // The tokens of a bin, up to 256, are ranked by comparison with one another; where there are more they are first cut into 512 parts of their order,
-// logit then id, until there are not.  The few tokens near the largest, where most answers lie, are listed as the sums are taken.  Every CTA counts
-// and lists its slice in its own memory; the first one reads the others' and searches, the others read what it found.
+// logit then id, until there are not.  What top-k or min-p leaves is listed before it is weighed, and where they leave everything the few tokens near the
+// largest are as the sums are taken: most answers are then found without the slices.  Every CTA counts and lists its slice in its own memory; the
+// first one reads the others' and searches, the others read what it found.
 //
-// Bounds: a row alone, the chain of passes, barriers and searches (50257 tokens, nucleus: 27 us, of which the weights 6 and each search 4); many rows,
-// reading them once and again from L2 (256 rows of 50257 f32, min-p: 28 us, the first reading alone 7.8); with a nucleus over everything, the 11
-// f64 operations and the atomics of every token's weight (64 rows of bf16, every setting of its own: 44 us).
+// Bounds: a row alone, the chain of passes, barriers and searches (50257 tokens, nucleus: 25 us, of which the weights 6 and each search 4); many rows,
+// reading them once and again from L2 (256 rows of 50257 f32, min-p: 23 us, the first reading alone 7.8); with a nucleus over everything, the 11
+// f64 operations and the atomics of every token's weight (64 rows of bf16, every setting of its own: 43 us).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -35,7 +36,7 @@ constexpr int BINS = 2048;              // 1/32 of an e-fold each; the last: eve
 constexpr float BINS_A_FOLD = 32.f;
 constexpr int FINE = 512;
 constexpr int LIST = 256;
-constexpr int NEAR = 224, NEAR_LIST = 512;   // bins whose tokens are listed at once (7 e-folds), as long as there are no more than that in a slice
+constexpr int NEAR = 224, NEAR_LIST = 1024;  // bins whose tokens are listed at once (7 e-folds), as long as there are no more than that in a slice
 constexpr int TABLE = 64;               // 2^-(j / 64)
 
 struct Sampling {
@@ -71,6 +72,7 @@ struct Smem {
   uint32_t warp_count[THREADS / 32];
   uint32_t best, best_id;                         // the largest: key, ~id
   uint32_t n, n_near;
+  int listed;                                     // tokens of the bins below this are in `near`
   Command command[2];                             // taken in turn, so that one can be written while the other is read
   int bin;
   u64 place, above, weight;                       // what a search leaves: the token that covers z, the sum before it, its weight
@@ -308,6 +310,7 @@ __device__ __forceinline__ Smem& of_cta(Smem& sm, int c) {
 template <int CTAS>
 __device__ __forceinline__ void join_counts(Smem& sm, int rank) {
   if constexpr (CTAS > 1) {
+#pragma unroll 1
     for (int i = rank * (BINS / CTAS) + threadIdx.x; i < (rank + 1) * (BINS / CTAS); i += THREADS) {
       uint32_t n = 0;
 #pragma unroll
@@ -320,6 +323,7 @@ __device__ __forceinline__ void join_counts(Smem& sm, int rank) {
 template <int CTAS>
 __device__ __forceinline__ void join_sums(Smem& sm, int rank) {
   if constexpr (CTAS > 1) {
+#pragma unroll 1
     for (int i = rank * (BINS / CTAS) + threadIdx.x; i < (rank + 1) * (BINS / CTAS); i += THREADS) {
       u64 sum = 0;
 #pragma unroll
@@ -334,6 +338,7 @@ __device__ __forceinline__ void join_sums(Smem& sm, int rank) {
 template <int CTAS>
 __device__ __forceinline__ void join_parts(Smem& sm) {
   if constexpr (CTAS > 1) {
+#pragma unroll 1
     for (int i = threadIdx.x; i < FINE; i += THREADS) {
       u64 sum = 0;
       uint32_t n = 0;
@@ -414,6 +419,7 @@ __device__ __forceinline__ void search(const Slice<T, CTAS> slice, int ids, cons
     if (!alone) turn ^= 1;
     if (tid == 0) sm.n = 0;
     if (now.cut >= 0)
+#pragma unroll 1
       for (int i = tid; i < FINE; i += THREADS) sm.fcount[i] = sm.flo[i] = sm.fhi[i] = 0;
     __syncthreads();
     if (alone) {                                      // a CTA's list to as many threads
@@ -427,7 +433,12 @@ __device__ __forceinline__ void search(const Slice<T, CTAS> slice, int ids, cons
       __syncthreads();
     } else {
       const float lowest = value_of(max(least, sizeof(T) == 2 ? uint32_t(now.from >> ids) << 16 : uint32_t(now.from >> ids)));
+      const float highest = value_of(key_at<T>(now.to, ids));          // infinity's bf16 place has NaN here, which nothing exceeds
       slice.fours(lowest == lowest ? lowest : -INFINITY, [&](int id, const float (&x)[4], int n) {
+        bool some = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) some |= !(x[j] < lowest) && !(x[j] > highest);
+        if (!some) return;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t key = key_of(x[j]);
@@ -473,6 +484,7 @@ __device__ __forceinline__ void search(const Slice<T, CTAS> slice, int ids, cons
             if (it.place > mine.place) { over += it.w; ++higher; }
           }
         }
+#pragma unroll 1
         for (int o = 1; o < helpers; o *= 2) {
           over += __shfl_xor_sync(0xffffffffu, over, o);
           higher += __shfl_xor_sync(0xffffffffu, higher, o);
@@ -514,6 +526,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
   const int tid = threadIdx.x, V = p.V, rank = CTAS == 1 ? 0 : int(blockIdx.x % CTAS);
   const size_t at = blockIdx.x / CTAS;
   if (tid == 0) { sm.best = 0; sm.best_id = 0; sm.sum = 0; sm.n_near = 0; }
+#pragma unroll 1
   for (int i = tid; i < BINS; i += THREADS) sm.count[i] = sm.lo[i] = sm.hi[i] = 0;
   if (tid < TABLE) sm.table[tid] = exp2(-double(tid) / TABLE);
   meet<CTAS>();
@@ -585,42 +598,78 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
     least = key_at<T>(of_cta<CTAS>(sm, 0).place, p.ids);
     if (sizeof(T) == 2) least &= 0xffff0000u;
     last = min(last, r.bin(value_of(key_at<T>(of_cta<CTAS>(sm, 0).place, p.ids))));
+#pragma unroll 1
     for (int i = tid; i < BINS; i += THREADS) sm.lo[i] = sm.hi[i] = 0;
     __syncthreads();
   }
   const double border = double(min_p) * double(1ull << p.shift);
+  const float lowest = fmaxf(r.below(min(last, BINS - 2)), count ? value_of(least) : -INFINITY);
   u64 bordering = 0;
-  slice.fours(fmaxf(r.below(min(last, BINS - 2)), count ? value_of(least) : -INFINITY), [&](int id, const float (&x)[4], int) {
-    u64 w[4];
-    int b[4];
-    uint32_t before[4];
+  // a token's weight into its bin (one that has no say: BINS - 1) and, near the border of min-p, into what min-p leaves
+  auto weigh = [&](float x, int& b) {
+    b = r.bin(x);
+    const bool in = b <= last && b < BINS - 1 && key_of(x) >= least;
+    const double scaled = r.scaled(x);
+    const u64 w = in ? __double_as_longlong(scaled + 4503599627370496.0) & 0xfffffffffffffull : 0;
+    if (in && b >= low && b <= high && scaled >= border) bordering += w;
+    if (!in) b = BINS - 1;
+    return w;
+  };
+  // Where a filter leaves few, they are listed first, since in a warp some lane nearly always has one: a thread then has one of them.
+  bool all = count ? top_k <= NEAR_LIST / 2 * CTAS : min_p > 0.f && !nucleus;
+  if (all) {
+    slice.fours(lowest, [&](int id, const float (&x)[4], int n) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      b[j] = r.bin(x[j]);
-      const bool in = b[j] <= last && b[j] < BINS - 1 && key_of(x[j]) >= least;
-      const double scaled = r.scaled(x[j]);
-      w[j] = in ? __double_as_longlong(scaled + 4503599627370496.0) & 0xfffffffffffffull : 0;
-      if (in && b[j] >= low && b[j] <= high && scaled >= border) bordering += w[j];
-      if (!in) b[j] = BINS - 1;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) before[j] = w[j] ? atomicAdd(&sm.lo[b[j]], uint32_t(w[j])) : 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t up = uint32_t(w[j] >> 32) + (before[j] + uint32_t(w[j]) < before[j] ? 1u : 0u);
-      if (up) atomicAdd(&sm.hi[b[j]], up);
-      if (b[j] < NEAR && *static_cast<volatile uint32_t*>(&sm.n_near) <= NEAR_LIST) {
-        const uint32_t slot = atomicAdd(&sm.n_near, 1u);
-        if (slot < NEAR_LIST) sm.near[slot] = place_of<T>(key_of(x[j]), id + j, p.ids);
+      for (int j = 0; j < 4; ++j) {
+        if (j < n && x[j] >= lowest && *static_cast<volatile uint32_t*>(&sm.n_near) <= NEAR_LIST) {
+          const uint32_t slot = atomicAdd(&sm.n_near, 1u);
+          if (slot < NEAR_LIST) sm.near[slot] = place_of<T>(key_of(x[j]), id + j, p.ids);
+        }
       }
+    });
+    __syncthreads();
+    const int n = int(sm.n_near);
+    all = n <= NEAR_LIST;
+    if (all) {
+      for (int i = tid; i < n; i += THREADS) {
+        int b;
+        const u64 w = weigh(value_of(key_at<T>(sm.near[i], p.ids)), b);
+        if (w) add64(&sm.lo[b], &sm.hi[b], w);
+        else sm.near[i] = 0;                          // below every token's place: in no range that is searched
+      }
+    } else {
+      __syncthreads();
+      if (tid == 0) sm.n_near = 0;
+      __syncthreads();
     }
-  });
-  if (min_p > 0.f && bordering) atomicAdd(&sm.sum, bordering);
-  meet<CTAS>();
-  int near = NEAR;
+  }
+  if (!all) {
+    slice.fours(lowest, [&](int id, const float (&x)[4], int) {
+      u64 w[4];
+      int b[4];
+      uint32_t before[4];
 #pragma unroll
-  for (int c = 0; c < CTAS; ++c)
-    if (of_cta<CTAS>(sm, c).n_near > NEAR_LIST) near = 0;
+      for (int j = 0; j < 4; ++j) w[j] = weigh(x[j], b[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) before[j] = w[j] ? atomicAdd(&sm.lo[b[j]], uint32_t(w[j])) : 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t up = uint32_t(w[j] >> 32) + (before[j] + uint32_t(w[j]) < before[j] ? 1u : 0u);
+        if (up) atomicAdd(&sm.hi[b[j]], up);
+        if (b[j] < NEAR && *static_cast<volatile uint32_t*>(&sm.n_near) <= NEAR_LIST) {
+          const uint32_t slot = atomicAdd(&sm.n_near, 1u);
+          if (slot < NEAR_LIST) sm.near[slot] = place_of<T>(key_of(x[j]), id + j, p.ids);
+        }
+      }
+    });
+  }
+  if (min_p > 0.f && bordering) atomicAdd(&sm.sum, bordering);
+  __syncthreads();
+  if (tid == 0) sm.listed = all ? BINS : sm.n_near <= NEAR_LIST ? NEAR : 0;
+  meet<CTAS>();
+  int near = BINS;
+#pragma unroll
+  for (int c = 0; c < CTAS; ++c) near = min(near, of_cta<CTAS>(sm, c).listed);
   u64 left = 0;
   join_sums<CTAS>(sm, rank);
   if (rank == 0) {
@@ -628,17 +677,22 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
     running_sums<BINS>(0, 0);
     left = (u64(sm.hi[BINS - 1]) << 32) + sm.lo[BINS - 1];
   }
-  if (nucleus) {
-    search<T, CTAS>(slice, p.ids, r, false, share(double(top_p), left), least, near, turn);
-    if (rank == 0) left = sm.above + sm.weight;
-  }
-  if (min_p > 0.f && rank == 0) {
-    u64 sum = (u64(sm.hi[low]) << 32) + sm.lo[low];
+  // the nucleus, then the draw: one call, since a second copy of the search would be fetched anew
+  for (bool draw = !nucleus;; draw = true) {
+    u64 z = share(double(top_p), left);
+    if (draw && rank == 0) {
+      if (min_p > 0.f) {
+        u64 sum = (u64(sm.hi[low]) << 32) + sm.lo[low];
 #pragma unroll
-    for (int c = 0; c < CTAS; ++c) sum += of_cta<CTAS>(sm, c).sum;
-    left = max(min(left, sum), u64(1) << p.shift);             // min_p beyond 1 leaves the largest
+        for (int c = 0; c < CTAS; ++c) sum += of_cta<CTAS>(sm, c).sum;
+        left = max(min(left, sum), u64(1) << p.shift);         // min_p beyond 1 leaves the largest
+      }
+      z = share(double(p.u[at]), left);
+    }
+    search<T, CTAS>(slice, p.ids, r, false, z, least, near, turn);
+    if (draw) break;
+    left = sm.above + sm.weight;
   }
-  search<T, CTAS>(slice, p.ids, r, false, rank == 0 ? share(double(p.u[at]), left) : 0, least, near, turn);
   if (rank == 0 && tid == 0) {
     p.token[at] = id_at<T>(sm.place, p.ids);
     if (p.prob != nullptr) p.prob[at] = float(r.scaled(value_of(key_at<T>(sm.place, p.ids))) / double(left));
@@ -658,7 +712,7 @@ int launch_rows_by(Sampling p, int n_rows, cudaStream_t stream) {
   return JB200_OK;
 }
 
-// CTAs a row: as many as two a SM leave room for (64 rows of 50257 bf16, every setting of its own: 47 us; with one a SM 57), slices of 4096 tokens
+// CTAs a row: as many as two a SM leave room for (64 rows of 50257 bf16, every setting of its own: 43 us; with one a SM some 50), slices of 4096 tokens
 // or more
 template <typename T>
 int launch_rows(const Sampling& p, int n_rows, cudaStream_t stream) {

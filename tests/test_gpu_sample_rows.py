@@ -213,3 +213,23 @@ def test_no_rows_and_refusals():
                        (lambda: ops.sample_rows(x[:1].expand(4, 100), u), "overlap")):
         with pytest.raises(RuntimeError, match=text):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,V", [(300, 6007), (2, 50257)])
+@pytest.mark.parametrize("few", [1, 1000, 1023, 1024, 1025, 3000])
+def test_what_a_filter_leaves_fits_a_list_or_not(few, B, V, dtype):
+    """`few` neighbouring tokens, so that one slice has them all, stand out by more than min-p (or top-k) leaves: around the length of its list."""
+    x = _logits(B, V, dtype, seed=few, size=0.5) - 20.0
+    x[:, 7:7 + few] = (_logits(B, few, dtype, seed=1, size=0.25).float() + 4.0).to(dtype)
+    one, rows = [1.0] * 4, [x[:4].contiguous(), x[-4:].contiguous()] if B > 4 else [x]
+    for r in rows:
+        n = r.shape[0]
+        for k, p, m in ((0, 1.0, 0.02), (few, 1.0, 0.0), (few, 0.7, 0.05), (0, 0.9, 0.02), (min(few + 30, V), 1.0, 1e-5)):
+            _check(r, one[:n], [k] * n, [p] * n, [m] * n, seed=few)
+    # as many rows as make one CTA of each: the same tokens as a few at a time
+    u = torch.rand(B, generator=torch.Generator().manual_seed(few)).cuda()
+    for kw in (dict(min_p=0.02), dict(top_k=few), dict(top_k=few, top_p=0.7, min_p=0.05)):
+        together = ops.sample_rows(x, u, temperature=1.0, **kw)
+        apart = torch.cat([ops.sample_rows(x[i:i + 4], u[i:i + 4].contiguous(), temperature=1.0, **kw) for i in range(0, B, 4)])
+        assert torch.equal(together, apart)
