@@ -180,7 +180,9 @@ __device__ __forceinline__ double to_f64(float x) {
 
 // Place in the order of a row: `ids` bits of the id from the end behind the logit's key, of which bf16 has 16 bits
 template <typename T>
-__device__ __forceinline__ u64 place_of(uint32_t key, int id, int ids) { return (u64(sizeof(T) == 2 ? key >> 16 : key) << ids) + ((1u << ids) - 1u - uint32_t(id)); }
+__device__ __forceinline__ u64 place_of(uint32_t key, int id, int ids) {
+  return (u64(sizeof(T) == 2 ? key >> 16 : key) << ids) + ((1u << ids) - 1u - uint32_t(id));
+}
 template <typename T>
 __device__ __forceinline__ int id_at(u64 place, int ids) { return int((1u << ids) - 1u - (uint32_t(place) & ((1u << ids) - 1u))); }
 template <typename T>
@@ -712,8 +714,8 @@ int launch_rows_by(Sampling p, int n_rows, cudaStream_t stream) {
   return JB200_OK;
 }
 
-// CTAs a row: as many as two a SM leave room for (64 rows of 50257 bf16, every setting of its own: 43 us; with one a SM some 50), slices of 4096 tokens
-// or more
+// CTAs a row: as many as two a SM leave room for (64 rows of 50257 bf16, every setting of its own: with their launch 53 us; with one a SM 57), slices of 4096 tokens or
+// more
 template <typename T>
 int launch_rows(const Sampling& p, int n_rows, cudaStream_t stream) {
   const int most = 2 * sm_count() / n_rows, wide = p.V / 4096, ctas = most < wide ? most : wide;
