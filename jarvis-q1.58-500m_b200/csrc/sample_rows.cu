@@ -714,8 +714,8 @@ int launch_rows_by(Sampling p, int n_rows, cudaStream_t stream) {
   return JB200_OK;
 }
 
-// CTAs a row: as many as two a SM leave room for (64 rows of 50257 bf16, every setting of its own: with their launch 53 us; with one a SM 57), slices of 4096 tokens or
-// more
+// CTAs a row: as many as two a SM leave room for (64 rows of 50257 bf16, every setting of its own, with their launch: 53 us; with one a SM 57), slices of
+// 4096 tokens or more
 template <typename T>
 int launch_rows(const Sampling& p, int n_rows, cudaStream_t stream) {
   const int most = 2 * sm_count() / n_rows, wide = p.V / 4096, ctas = most < wide ? most : wide;
