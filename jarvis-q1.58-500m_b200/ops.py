@@ -848,7 +848,8 @@ def gated_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     projection; 16-byte aligned, strides multiples of 8); value head h takes key head h // (H // key_heads).  log_decay (<= 0), beta: f32 (B*T, H), column
     slices allowed.  normalize: k and q are divided by their norms, sqrt(|.|^2 + 1e-6); without it keep beta |k|^2 <= 2.  scale: 1/8 unless given.
     lengths: int32 (B,), for padded batches: rows behind a sequence's length are not read, their output is 0, the state is that after its last row.
-    Returns (o bf16 (B*T, H*64) or None, state f32 (B, H, 64 values, 64 keys) or None).  state_out may be state_in itself."""
+    Returns (o bf16 (B*T, H*64) or None, state f32 (B, H, 64 values, 64 keys) or None).  state_out may be state_in itself; out and state_out must
+    otherwise lie outside of every argument, from its first to its last element (other columns of one buffer are inside)."""
     lib = _lib.load()
     what = "gated_delta_scan"
     KH = H if key_heads is None else key_heads

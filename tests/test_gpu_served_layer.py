@@ -164,3 +164,33 @@ def test_an_engine_with_a_nucleus_of_the_whole_vocabulary():
             for rec in sched.engine.record:
                 w = ((rec["logits"] - rec["logits"].amax(dim=1, keepdim=True)) / 0.9).exp()
                 assert (w.gather(1, rec["tokens"]) >= 0.1 * (1 - 2.0 ** -18)).all()
+
+
+def test_rows_further_apart_than_32_bits_count():
+    """Views with 2^20 elements from row to row, 2500 rows: the bits of contiguous copies."""
+    B, T, H, far = 1, 2500, 2, 1 << 20
+    buf = torch.zeros(B * T, far, dtype=BF16, device="cuda")
+    q, k, v, g, b, s = delta._problem(B, T, H, H, seed=4)
+    wide = [buf[:, i * 128:(i + 1) * 128] for i in range(3)]
+    for view, t in zip(wide, (q, k, v)):
+        view.copy_(t)
+    out = torch.empty(B * T, far, dtype=BF16, device="cuda")[:, 64:192]
+    with pytest.raises(RuntimeError, match="overlaps"):          # other columns of an argument's buffer count as the argument
+        ops.gated_delta_scan(*wide, g, b, B, T, H, out=buf[:, 512:640])
+    near = ops.gated_delta_scan(q, k, v, g, b, B, T, H, state_in=s, want_state=True)
+    got = ops.gated_delta_scan(*wide, g, b, B, T, H, state_in=s, want_state=True, out=out)
+    assert torch.equal(got[0], near[0]) and torch.equal(got[1], near[1])
+    w = 1 + 0.2 * torch.randn(64, generator=torch.Generator().manual_seed(1)).cuda()
+    assert torch.equal(ops.gated_norm(wide[0], w, wide[1], group=64), ops.gated_norm(q, w, k, group=64))
+    w2, x = w.repeat(2), torch.randn(B * T, 128, generator=torch.Generator().manual_seed(2)).cuda()
+    for a, b_ in zip(ops.residual_norm(x, wide[0], w2, w2, gate=wide[1]), ops.residual_norm(x, q, w2, w2, gate=k)):
+        assert torch.equal(a, b_)
+    rows = buf[:, 1:1004]                                        # not aligned either
+    rows.copy_(draws._logits(B * T, 1003, BF16, seed=6))
+    u = torch.rand(B * T, device="cuda")
+    for kw in (dict(top_p=0.9), dict(top_k=20, min_p=0.05), dict(temperature=0.0)):
+        assert torch.equal(ops.sample_rows(rows, u, **kw), ops.sample_rows(rows.contiguous(), u, **kw))
+    # a vocabulary of 2^24, the largest
+    logits = draws._logits(1, 1 << 24, BF16, seed=8)
+    draws._check(logits, [1.0], [0], [0.9], [0.0])
+    draws._check(logits, [0.7], [3000], [1.0], [0.0])
