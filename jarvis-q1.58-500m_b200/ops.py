@@ -785,6 +785,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor | None = None, *, temperature: 
 
 
 # --------------------------------------------------------------------------- gated delta rule, norms around a block, draws
+# Results are allocated after an argument of their shape where there is one (empty_like: a third of the host time of empty with its keywords).
 def _forward_only(what: str, *tensors):
     """These operators have no gradients: a graph that runs through one would lose its part without a word."""
     if torch.is_grad_enabled():
@@ -881,7 +882,7 @@ def gated_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
             raise RuntimeError(f"{what}: state_out overlaps state_in without being it")
         _apart(what, "state_out", state_out, q, k, v, log_decay, beta, lengths, out)
     elif want_state:
-        state_out = torch.empty((B, H, 64, 64), dtype=f32, device=q.device)
+        state_out = torch.empty((B, H, 64, 64), dtype=f32, device=q.device) if state_in is None else torch.empty_like(state_in)
         s_out = state_out.data_ptr()
     else:
         s_out = None
@@ -893,7 +894,7 @@ def gated_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
         o, ldo = None, 0
     else:
         if out is None:
-            out = torch.empty((N, H * 64), dtype=bf16, device=q.device)
+            out = torch.empty_like(v) if v.is_contiguous() else torch.empty((N, H * 64), dtype=bf16, device=q.device)
             ldo = H * 64
         else:
             ldo = _view(out, dev, (N, H * 64), bf16, what, "out")
@@ -956,7 +957,7 @@ def gated_norm(y: torch.Tensor, weight: torch.Tensor, gate: torch.Tensor | None 
     if _elsewhere(y):
         with torch.cuda.device(dev):
             return gated_norm(y, weight, gate, group=group, eps=eps, out_dtype=out_dtype)
-    out = torch.empty(y.shape, dtype=out_dtype, device=y.device)
+    out = torch.empty_like(y, dtype=out_dtype) if y.is_contiguous() else torch.empty(y.shape, dtype=out_dtype, device=y.device)
     rc = lib.jb200_gated_norm(a, dt, ldy, w, g, ldg, group, eps, out.data_ptr(), _dt(out), y.numel() // width, width, _stream())
     if rc:
         _lib.check(rc, "jb200_gated_norm")
@@ -985,14 +986,14 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, w_after: torch.Tensor, w_bef
         with torch.cuda.device(dev):
             return residual_norm(x, y, w_after, w_before, gate=gate, scale=scale, eps=eps, out=out, out_dtype=out_dtype)
     if out is None:
-        out = torch.empty(x.shape, dtype=f32, device=x.device)
+        out = torch.empty_like(x)
     else:
         if out.shape != x.shape:
             raise RuntimeError(f"{what}: out {tuple(out.shape)} must have x's shape {tuple(x.shape)}")
         if _whole(out, dev, f32, n, what, "out", "wrong size") != px and _touch(out, x):
             raise RuntimeError(f"{what}: out overlaps x without being it")
         _apart(what, "out", out, y, gate, w_after, w_before, scale)
-    xn = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    xn = torch.empty_like(x, dtype=out_dtype)
     rc = lib.jb200_residual_norm(px, a, dt, ldy, wa, g, ldg, sc, wb, eps, out.data_ptr(), xn.data_ptr(), _dt(xn), n // width, width, _stream())
     if rc:
         _lib.check(rc, "jb200_residual_norm")
@@ -1037,8 +1038,8 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, *, temperature=0.7, top_k
     if _elsewhere(logits):
         with torch.cuda.device(dev):
             return sample_rows(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, want_prob=want_prob)
-    out = torch.empty((B, 1), dtype=torch.int64, device=logits.device)
-    prob = torch.empty((B,), dtype=f32, device=logits.device) if want_prob else None
+    out = torch.empty_like(u, dtype=torch.int64).view(B, 1)
+    prob = torch.empty_like(u).view(B) if want_prob else None
     rc = lib.jb200_sample_rows(ctypes.byref(s), B, out.data_ptr(), None if prob is None else prob.data_ptr(), _stream())
     if rc:
         _lib.check(rc, "jb200_sample_rows")
