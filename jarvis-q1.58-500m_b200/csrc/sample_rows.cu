@@ -11,7 +11,7 @@
 // All of them ask "which token covers position z of the running sum", top-k with every weight 1.  Weights are taken in f64 and held as integers of
 // 2^-45 of the largest one's, so that sums do not depend on the order of the atomics that form them, and a token that the exact sums choose is
 // missed only where u lies within some 1e-12 of a border.  A cluster of CTAs has a row, a slice each (in shared memory where it fits), with as many
-// CTAs as keep the SMs busy.  A histogram of the sums (for top-k of the counts) over 2048 bins of 1/32 of an e-fold finds the bin that covers z.
+// CTAs as keep the SMs busy.  A histogram of the sums (for top-k of the counts) over 2048 bins of 1/64 of an e-fold finds the bin that covers z.
 // The tokens of a bin, up to 256, are ranked by comparison with one another; where there are more they are first cut into 512 parts of their order,
 // logit then id, until there are not.  What top-k or min-p leaves is listed before it is weighed, and where they leave everything the few tokens near the
 // largest are as the sums are taken: most answers are then found without the slices.  Every CTA counts and lists its slice in its own memory; the
@@ -32,11 +32,11 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int THREADS = 512;
-constexpr int BINS = 2048;              // 1/32 of an e-fold each; the last: everything 64 e-folds or more below the largest, whose weight is 0
-constexpr float BINS_A_FOLD = 32.f;
+constexpr int BINS = 2048;              // 1/64 of an e-fold each; the last: all that is some 32 e-folds (2^46) below the largest, whose weight is 0
+constexpr float BINS_A_FOLD = 64.f;
 constexpr int FINE = 512;
 constexpr int LIST = 256;
-constexpr int NEAR = 224, NEAR_LIST = 1024;  // bins whose tokens are listed at once (7 e-folds), as long as there are no more than that in a slice
+constexpr int NEAR = 448, NEAR_LIST = 1024;  // bins whose tokens are listed at once (7 e-folds), as long as there are no more than that in a slice
 constexpr int TABLE = 64;               // 2^-(j / 64)
 
 struct Sampling {
