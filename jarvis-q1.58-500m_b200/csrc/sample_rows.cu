@@ -19,7 +19,7 @@
 //
 // Bounds: a row alone, the chain of passes, barriers and searches (50257 tokens, nucleus: 25 us, of which the weights 6 and each search 4); many rows,
 // reading them once and again from L2 (256 rows of 50257 f32, min-p: 23 us, the first reading alone 7.8); with a nucleus over everything, the 11
-// f64 operations and the atomics of every token's weight (64 rows of bf16, every setting of its own: 43 us).
+// f64 operations and the atomics of every token's weight (64 rows of bf16, every setting of its own: 41 us; 256 rows of f32 107).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -166,7 +166,7 @@ __device__ __forceinline__ void meet() {
   else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// This CTA's memory; functions that are called rather than inlined ask for it, so that the compiler knows that it is shared memory
+// This CTA's memory
 __device__ __forceinline__ Smem& own_smem() {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   return *reinterpret_cast<Smem*>(smem_raw);
@@ -374,8 +374,7 @@ __device__ __forceinline__ void take(const Command now, const Row r, bool by_cou
 }
 
 // The token that covers position z of the running sum (of the running count), in the first CTA's .place, .above and .weight.  z is the first CTA's to
-// know.  least: keys below it are not in the sums; near: bins below it are in the lists of what is near the largest.
-// `turn`: which of the commands is next.
+// know.  least: keys below it are not in the sums; near: tokens of the bins below it are in the CTAs' lists; turn: which of the commands is next.
 template <typename T, int CTAS>
 __device__ __forceinline__ void search(const Slice<T, CTAS> slice, int ids, const Row r, bool by_count, u64 z, uint32_t least, int near, int& turn) {
   Smem& sm = own_smem();
