@@ -703,7 +703,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
 
 template <typename T, int CTAS>
 int launch_rows_by(Sampling p, int n_rows, cudaStream_t stream) {
-  // a slice of up to 64 KB is kept: two CTAs a SM
+  // a slice of up to 64 KB is kept, so that two CTAs fit a SM (one row of 16384 tokens 20.6 to 25.3 us, read again from L2 21.0 to 26.6)
   constexpr size_t base = (sizeof(Smem) + 15) / 16 * 16, most = 64 * 1024;
   const size_t slice = size_t((p.V / int(16 / sizeof(T)) + CTAS * THREADS - 1) / (CTAS * THREADS)) * THREADS * 16;
   p.staged = slice <= most;
@@ -713,8 +713,9 @@ int launch_rows_by(Sampling p, int n_rows, cudaStream_t stream) {
   return JB200_OK;
 }
 
-// CTAs a row: as many as two a SM leave room for (64 rows of 50257 bf16, every setting of its own, with their launch: 53 us; with one a SM 57), slices of
-// 4096 tokens or more
+// CTAs a row: as many as two a SM leave room for, slices of 4096 tokens or more.  us with the launch, 50257 bf16: 64 rows with every setting of their
+// own 46, with one CTA a SM 51, with four 61 to 65; one row in eight slices 26, in four 31.  One row of 16384 in four slices 21, whole 25; of 8192 in two
+// 20, whole 19; of 4096 in two 20.5, whole 16.
 template <typename T>
 int launch_rows(const Sampling& p, int n_rows, cudaStream_t stream) {
   const int most = 2 * sm_count() / n_rows, wide = p.V / 4096, ctas = most < wide ? most : wide;
