@@ -89,3 +89,75 @@ def test_host_tensors_raise():
             call()
     with pytest.raises(RuntimeError, match="bad shape"):
         ops.gated_delta_scan(rows, rows, rows, g, g, 2, 2, 2, key_heads=3)
+
+
+class _OnCard(torch.Tensor):
+    """A host tensor that says it is on the card `card`."""
+    card = 0
+    is_cuda = property(lambda self: True)
+
+    def get_device(self):
+        return self.card
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        with torch._C.DisableTorchFunctionSubclass():
+            return func(*args, **(kwargs or {}))
+
+
+def _on(card, *shape, dtype=F32):
+    t = torch.zeros(*shape, dtype=dtype).as_subclass(_OnCard)
+    t.card = card
+    return t
+
+
+def test_launches_on_the_tensors_card(monkeypatch):
+    current, seen = [0], []
+
+    class Card:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Lib:
+        def __getattr__(self, name):
+            if name.endswith("_scratch_bytes"):
+                return lambda *a: 0
+            return lambda *a: seen.append((name, current[0])) or 0
+
+    monkeypatch.setattr(ops._lib, "load", lambda: Lib())
+    monkeypatch.setattr(ops, "_raw_device", lambda: current[0])
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops.torch.cuda, "device", Card)
+
+    def calls(card, other):
+        rows, g, x = _on(card, 4, 128, dtype=BF16), _on(card, 4, 2), _on(card, 4, 128)
+        return (lambda: ops.gated_delta_scan(rows, rows, rows, g, _on(other, 4, 2), 2, 2, 2), lambda: ops.gated_norm(rows, _on(other, 64), rows, group=64),
+                lambda: ops.residual_norm(x, rows, _on(other, 128), _on(card, 128)), lambda: ops.sample_rows(x, _on(other, 4), top_p=_on(card, 4)))
+
+    names = ["jb200_gated_delta", "jb200_gated_norm", "jb200_residual_norm", "jb200_sample_rows"]
+    for card in (1, 0):
+        for call in calls(card, card):
+            call()
+        assert seen == [(n, card) for n in names] and current == [0]
+        seen.clear()
+    for call in calls(0, 1) + calls(1, 0):
+        with pytest.raises(RuntimeError, match="tensors on cuda"):
+            call()
+    assert not seen
+
+
+def test_tensors_that_require_a_gradient_are_refused(monkeypatch):
+    monkeypatch.setattr(ops, "_raw_device", lambda: 0)
+    rows, g, x, w = _on(0, 4, 128, dtype=BF16), _on(0, 4, 2), _on(0, 4, 128), _on(0, 128)
+    w.requires_grad_(True)
+    x.requires_grad_(True)
+    for call in (lambda: ops.gated_norm(rows, w), lambda: ops.residual_norm(x, rows, _on(0, 128), _on(0, 128)),
+                 lambda: ops.gated_delta_scan(rows, rows, rows, g, g, 2, 2, 2, state_in=_on(0, 2, 2, 64, 64).requires_grad_(True))):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
