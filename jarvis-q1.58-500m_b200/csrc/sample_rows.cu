@@ -13,9 +13,9 @@
 // missed only where u lies within some 1e-12 of a border.  A cluster of CTAs has a row, a slice each (in shared memory where it fits), with as many
 // CTAs as keep the SMs busy.  A histogram of the sums (for top-k of the counts) over 2048 bins of 1/64 of an e-fold finds the bin that covers z.
 // The tokens of a bin, up to 256, are ranked by comparison with one another; where there are more they are first cut into 512 parts of their order,
-// logit then id, until there are not.  What top-k or min-p leaves is listed before it is weighed, and where they leave everything the few tokens near the
-// largest are as the sums are taken: most answers are then found without the slices.  Every CTA counts and lists its slice in its own memory; the
-// first one reads the others' and searches, the others read what it found.
+// logit then id, until there are not.  What top-k or min-p leaves is listed before it is weighed (and up to 256 ranked at once); where they leave
+// everything, the few tokens near the largest are as the sums are taken: most answers are then found without the slices.  Every CTA counts and lists
+// its slice in its own memory; the first one reads the others' and searches, the others read what it found.
 //
 // Bounds: a row alone, the chain of passes, barriers and searches (50257 tokens, nucleus: 25 us, of which the weights 6 and each search 4); many rows,
 // reading them once and again from L2 (256 rows of 50257 f32, min-p: 23 us, the first reading alone 7.8); with a nucleus over everything, the 11
@@ -68,11 +68,11 @@ struct Smem {
   uint32_t fcount[FINE], flo[FINE], fhi[FINE];
   Item list[LIST];
   u64 near[NEAR_LIST];
-  u64 warp_sum[THREADS / 32];
+  u64 warp_sum[THREADS / 32], warp_ok[THREADS / 32];
   uint32_t warp_count[THREADS / 32];
   uint32_t best, best_id;                         // the largest: key, ~id
   uint32_t n, n_near;
-  int listed;                                     // tokens of the bins below this are in `near`
+  int listed, kept;                               // tokens of the bins below this are in `near`; how many a filter left
   Command command[2];                             // taken in turn, so that one can be written while the other is read
   int bin;
   u64 place, above, weight;                       // what a search leaves: the token that covers z, the sum before it, its weight
@@ -373,6 +373,31 @@ __device__ __forceinline__ void take(const Command now, const Row r, bool by_cou
   }
 }
 
+// Of the list's n tokens one for a power of two of neighbouring threads, each with its part of the others: the weights and the number of those before
+// it.  True for one thread of each.
+__device__ __forceinline__ bool ranked(int n, Item& mine, u64& over, uint32_t& higher) {
+  Smem& sm = own_smem();
+  const int tid = threadIdx.x;
+  int helpers = 1;
+  while (helpers < 32 && 2 * helpers * n <= THREADS) helpers *= 2;
+  const int me = tid / helpers;
+  over = 0;
+  higher = 0;
+  if (me < n) {
+    mine = sm.list[me];
+    for (int j = tid & (helpers - 1); j < n; j += helpers) {
+      const Item it = sm.list[j];
+      if (it.place > mine.place) { over += it.w; ++higher; }
+    }
+  }
+#pragma unroll 1
+  for (int o = 1; o < helpers; o *= 2) {
+    over += __shfl_xor_sync(0xffffffffu, over, o);
+    higher += __shfl_xor_sync(0xffffffffu, higher, o);
+  }
+  return me < n && (tid & (helpers - 1)) == 0;
+}
+
 // The token that covers position z of the running sum (of the running count), in the first CTA's .place, .above and .weight.  z is the first CTA's to
 // know.  least: keys below it are not in the sums; near: tokens of the bins below it are in the CTAs' lists; turn: which of the commands is next.
 template <typename T, int CTAS>
@@ -472,25 +497,10 @@ __device__ __forceinline__ void search(const Slice<T, CTAS> slice, int ids, cons
         __syncthreads();
         if (tid < int(n)) sm.list[tid] = mine;
         __syncthreads();
-        // a power of two of neighbouring threads an element, each with its part of the others
-        int helpers = 1;
-        while (helpers < 32 && 2 * helpers * int(n) <= THREADS) helpers *= 2;
-        const int me = tid / helpers;
-        u64 over = 0;
-        uint32_t higher = 0;
-        if (me < int(n)) {
-          mine = sm.list[me];
-          for (int j = tid & (helpers - 1); j < int(n); j += helpers) {
-            const Item it = sm.list[j];
-            if (it.place > mine.place) { over += it.w; ++higher; }
-          }
-        }
-#pragma unroll 1
-        for (int o = 1; o < helpers; o *= 2) {
-          over += __shfl_xor_sync(0xffffffffu, over, o);
-          higher += __shfl_xor_sync(0xffffffffu, higher, o);
-        }
-        if (me < int(n) && (tid & (helpers - 1)) == 0) {
+        u64 over;
+        uint32_t higher;
+        const bool speaks = ranked(int(n), mine, over, higher);
+        if (speaks) {
           const u64 start = by_count ? cabove + higher : above + over;
           if (start <= z && z - start < (by_count ? 1 : mine.w)) { sm.place = mine.place; sm.above = above + over; sm.weight = mine.w; }
         }
@@ -518,6 +528,60 @@ __device__ __forceinline__ u64 share(double part, u64 whole) {
   const double z = part * double(whole);
   if (!(z > 0.0)) return 0;
   return min(z < 1.8e19 ? __double2ull_rd(z) : ~0ull, whole - 1);
+}
+
+// The draw from `n` listed tokens of all CTAs, at most LIST, by the first one, without any bins (one row of 50257, min-p: 12 us instead of 16).  A call,
+// so that rows of which much is left do not carry its registers (inlined, rows with a nucleus took a tenth longer).
+template <typename T, int CTAS>
+__device__ __noinline__ void draw_of_few(const Sampling p, size_t at, const Row r, int n, int last, int low, int high, uint32_t least, float top_p,
+                                         float min_p) {
+  Smem& sm = own_smem();
+  const int tid = threadIdx.x;
+  const double border = double(min_p) * double(1ull << r.shift);
+  Item mine;
+  u64 in = 0, ok = 0;                                 // what top-k leaves of the whole, and min-p
+  if (tid < n) {
+    int c = 0, i = tid;
+    if constexpr (CTAS > 1)
+      for (; i >= of_cta<CTAS>(sm, c).kept; ++c) i -= of_cta<CTAS>(sm, c).kept;
+    mine.place = of_cta<CTAS>(sm, c).near[i];
+    const float x = value_of(key_at<T>(mine.place, p.ids));
+    const int b = r.bin(x);
+    if (b <= last && key_of(x) >= least) in = r.weight(x);
+    if (b < low || (b <= high && r.scaled(x) >= border)) ok = in;
+    mine.w = in;
+    sm.list[tid] = mine;
+  }
+  for (int o = 16; o > 0; o >>= 1) {
+    in += __shfl_xor_sync(0xffffffffu, in, o);
+    ok += __shfl_xor_sync(0xffffffffu, ok, o);
+  }
+  if ((tid & 31) == 0) {
+    sm.warp_sum[tid >> 5] = in;
+    sm.warp_ok[tid >> 5] = ok;
+  }
+  __syncthreads();
+  in = ok = 0;
+#pragma unroll 1
+  for (int i = 0; i < THREADS / 32; ++i) {
+    in += sm.warp_sum[i];
+    ok += sm.warp_ok[i];
+  }
+  u64 over;
+  uint32_t higher;
+  const bool speaks = ranked(n, mine, over, higher);
+  if (top_p > 0.f && top_p < 1.f) {
+    const u64 z = share(double(top_p), in);
+    if (speaks && over <= z && z - over < mine.w) sm.above = over + mine.w;
+    __syncthreads();
+    in = sm.above;
+  }
+  if (min_p > 0.f) in = max(min(in, ok), u64(1) << r.shift);
+  const u64 z = share(double(p.u[at]), in);
+  if (speaks && over <= z && z - over < mine.w) {
+    p.token[at] = id_at<T>(mine.place, p.ids);
+    if (p.prob != nullptr) p.prob[at] = float(r.scaled(value_of(key_at<T>(mine.place, p.ids))) / double(in));
+  }
 }
 
 template <typename T, int CTAS>
@@ -631,6 +695,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
     __syncthreads();
     const int n = int(sm.n_near);
     all = n <= NEAR_LIST;
+    if (tid == 0) sm.kept = n;
+    meet<CTAS>();
+    int whole = 0;
+#pragma unroll
+    for (int c = 0; c < CTAS; ++c) whole += of_cta<CTAS>(sm, c).kept;
+    if (whole <= LIST) {                              // so few in all: ranked at once, without any bins
+      if (rank == 0) draw_of_few<T, CTAS>(p, at, r, whole, last, low, high, least, top_p, min_p);
+      meet<CTAS>();                                   // as at the end
+      return;
+    }
     if (all) {
       for (int i = tid; i < n; i += THREADS) {
         int b;
