@@ -18,7 +18,7 @@
 // its slice in its own memory; the first one reads the others' and searches, the others read what it found.
 //
 // Bounds: a row alone, the chain of passes, barriers and searches (50257 tokens, nucleus: 25 us, of which the weights 6 and each search 4); many rows,
-// reading them once and again from L2 (256 rows of 50257 f32, min-p: 23 us, the first reading alone 7.8); with a nucleus over everything, the 11
+// reading them once and again from L2 (256 rows of 50257 f32, min-p: 20 us, the first reading alone 7.8); with a nucleus over everything, the 11
 // f64 operations and the atomics of every token's weight (64 rows of bf16, every setting of its own: 41 us; 256 rows of f32 107).
 #include <cooperative_groups.h>
 
