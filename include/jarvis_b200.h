@@ -173,7 +173,9 @@ int jb200_ternary_linear_grouped(const void* x, int M, int K, const uint8_t* pac
  * sequence are not read, their output is 0, and the state is the one after the last row before them.  s_in NULL: zeros.  s_out NULL: not wanted;
  * may be s_in itself, else the two must not overlap; o must overlap no input.  o NULL: the state alone.  scratch:
  * jb200_gated_delta_scratch_bytes (0: may be NULL), 16-byte aligned; NULL where bytes are wanted: sequences are not cut into pieces.
- * An infinity or NaN in a row reaches the rows of its chunk of 64 tokens, in that value row (from k, q and the gates: in that head), and what follows. */
+ * Value rows (a column of v, of o; a row of S) are independent of one another: an infinity or NaN in v or in the state stays in its value row and
+ * reaches the rows of its chunk of 64 tokens and what follows (from k, q and the gates: in that head).  Of a chunk's largest |beta v| in a value row
+ * that row's outputs of earlier tokens of the chunk are off by up to 2^-32 of it. */
 #define JB200_DELTA_NORMALIZE 1
 typedef struct jb200_delta {
   int B, T, H, key_heads, head_dim, flags;

@@ -159,15 +159,18 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 // reads its other operand once for both, and what bounds these small products is reading (6 KB in 48 cycles, 8 KB in 64, for 32 and 64 of
 // mathematics).  T's blocks come from mma.sync: products of 16 x 16.
 //
-// Bound by that chain, some 5900 cycles a chunk on every SM that has a head (8 sequences of 2048 tokens, 16 heads: 107 us, where reading and writing
-// takes 21).  With mma.sync alone a chunk took 10800, with these warps' parts but all products unrolled 9600: 77 KB of code, which the SMs fetch
+// Bound by that chain, some 6400 cycles a chunk on every SM that has a head (8 sequences of 2048 tokens, 16 heads: 116 us, where reading and writing
+// takes 21; with one power of two for all value rows, which is wrong beside an outlier, 5900 and 107).  With mma.sync alone a chunk took 10800, with these warps' parts but all products unrolled 9600: 77 KB of code, which the SMs fetch
 // again and again.
 //
 // Precision: the state is f32 and stays it.  What it is multiplied by and into is f16 in two terms, x = hi + lo (22 bits), at a power of two
-// that brings a bound of its size to 2^15, so that f16's subnormals lie 2^-39 below: |X|, |U| <= 16 max|S| + 130 max|b v| and
-// max|S'| <= 8 e^Gc max|S| + 64 max|b v|, since a (I - b k k^T) with b |k|^2 <= 2 enlarges nothing (rows have 64 entries, a chunk 64 tokens).
-// The bounds need no exchange between warps where the chain would wait for it; typical values lie 2^4 to 2^8 below them.  K and Q come as bf16 and fit one
-// term, with a power of two per row; their norms are factors of rows and columns.  T X is hi hi + hi lo + lo hi.  What only the output sees (Q S^T, P U)
+// that brings a bound of its size to 2^15, so that f16's subnormals lie 2^-39 below.  Value rows of S are independent of one another, and so is each
+// one's power: a value row is a column of every product here, so that an infinity, or values far larger than the others, stay in theirs.  With N a
+// bound of a value row's norm, a chunk's S, X and U are at most 2 N + 130 max|b v| there and N' = e^Gc N + 64 max|b v|, since a (I - b k k^T)
+// with b |k|^2 <= 2 enlarges nothing (a chunk has 64 tokens); every eighth chunk N is at most 8 max|S| as well (a row has 64 entries).  max|b v| comes
+// from the preparing groups, and the next chunk's powers are made while T X is formed.  Typical values lie 2^5 to 2^12 below the bound, and 2^15 below
+// it two terms still have an f32's 24 bits.  A row's largest |b v| of a chunk counts for the chunk's earlier tokens too: outputs there are off by up to
+// 2^-32 of it.  K and Q come as bf16 and fit one term, with a power of two per row; their norms are factors of rows and columns.  T X is hi hi + hi lo + lo hi.  What only the output sees (Q S^T, P U)
 // is one term, 2^-12 of a value where the output's own rounding is 2^-9.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int CHUNK = 64;
@@ -184,6 +187,7 @@ struct alignas(1024) Stage {
   float2 g[CHUNK];                                     // G in two terms
   float rk[CHUNK], nk[CHUNK], beta[CHUNK];
   float of_v[CHUNK], of_y[CHUNK], of_u[CHUNK], of_s[CHUNK], of_o[CHUNK];
+  alignas(16) uint32_t most_v[D / 2][4];               // the largest |b v| of a value row, two rows' as bf16, of every warp that looked
   float whole;
 };
 struct Solve {                                         // of a preparing group
@@ -196,8 +200,7 @@ struct alignas(1024) ChunkSmem {
   uint8_t x_hi[TILE], x_lo[TILE];                      // X, then e^(Gc - G) U, [token][value]
   uint8_t u[TILE];                                     // U, one term
   Solve solve[2];
-  float most_s[2][4], most_v[2][4];                    // of every warp of the state
-  float2 inverse[2];                                   // of the powers of S and of X and U
+  float power[2][D], inverse[2][D];                    // a value row's power of two, by turns: a chunk's is in use when the next one's is made
   unsigned long long bar_y, bar_u, bar_s, bar_o, bar_a[2], bar_p, bar_k[STAGES];
   uint32_t tmem, abort_flag;
 };
@@ -295,17 +298,18 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 // A power of two s with s m in [2^14, 2^15) and its inverse; of m = 0, infinities and what is too small any that are finite
 __device__ __forceinline__ void power_scale(float m, float& s, float& inv) {
-  const int e = max(int(__float_as_uint(m) >> 23), 17);
+  const int e = max(int(__float_as_uint(m) >> 23), 17);         // 255 at most: m is none below 0
   s = __uint_as_float(uint32_t(254 + 14 - e) << 23);
   inv = __uint_as_float(uint32_t(e - 14) << 23);
 }
-// The larger sizes of two pairs of f16
-__device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {
-  const __half2 m = __hmax2(__habs2(*reinterpret_cast<const __half2*>(&a)), __habs2(*reinterpret_cast<const __half2*>(&b)));
-  return *reinterpret_cast<const uint32_t*>(&m);
+// Of four pairs of sizes a lane (bf16 or f16: they compare as integers, NaN above all) the largest over the lanes that differ in bits 4 and 3, pair
+// (lane >> 3) & 3 for each
+__device__ __forceinline__ uint32_t most_of_four(const uint32_t (&m)[4], int lane) {
+  const bool up = lane & 16, up8 = lane & 8;
+  const uint32_t a = __vmaxu2(up ? m[2] : m[0], __shfl_xor_sync(0xffffffffu, up ? m[0] : m[2], 16));
+  const uint32_t b = __vmaxu2(up ? m[3] : m[1], __shfl_xor_sync(0xffffffffu, up ? m[1] : m[3], 16));
+  return __vmaxu2(up8 ? b : a, __shfl_xor_sync(0xffffffffu, up8 ? a : b, 8));
 }
-__device__ __forceinline__ float f16_lo(uint32_t x) { return __low2float(*reinterpret_cast<const __half2*>(&x)); }
-__device__ __forceinline__ float f16_hi(uint32_t x) { return __high2float(*reinterpret_cast<const __half2*>(&x)); }
 __device__ __forceinline__ float inverse_power(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }      // of a power of two
 __device__ __forceinline__ uint32_t unit_at(int row, int unit) { return uint32_t(row * 128 + ((unit ^ (row & 7)) << 4)); }
 
@@ -352,10 +356,23 @@ struct Part {
   int b, h, begin, len, chunks;
 };
 
-// 16 bytes that are asked for here and not where they are used (an ordinary read-only load may be moved there, behind barriers and all)
-__device__ __forceinline__ uint4 load_now(const void* p) {
+// 16 bytes that are asked for here and not where they are used (an ordinary read-only load may be moved there, behind barriers and all), or zeros: in the same
+// registers, since a choice behind the load would wait for it here
+__device__ __forceinline__ uint4 load_now(const void* p, bool on) {
   uint4 x;
-  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p) : "memory");
+  asm volatile(
+      "{\n\t"
+      ".reg .pred on;\n\t"
+      "setp.ne.b32 on, %5, 0;\n\t"
+      "mov.b32 %0, 0;\n\t"
+      "mov.b32 %1, 0;\n\t"
+      "mov.b32 %2, 0;\n\t"
+      "mov.b32 %3, 0;\n\t"
+      "@on ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n\t"
+      "}"
+      : "=&r"(x.x), "=&r"(x.y), "=&r"(x.z), "=&r"(x.w)
+      : "l"(p), "r"(int(on))
+      : "memory");
   return x;
 }
 __device__ __forceinline__ float load_now(const float* p) {
@@ -367,7 +384,7 @@ __device__ __forceinline__ float load_now(const float* p) {
 // Half a row of a bf16 matrix a thread: from memory ...
 __device__ __forceinline__ void fetch_half(uint4 (&x)[4], const __nv_bfloat16* at, bool on) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = on ? load_now(static_cast<const void*>(at + 8 * i)) : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < 4; ++i) x[i] = load_now(at + 8 * i, on);
 }
 // ... and to f16 in a tile (`twice`: and in the next one), times the power of two s that brings the row's norm into [1, 2); returns the sum of
 // squares after that.  A sum of squares beyond f32's range makes the row NaN, one below it makes it 0.
@@ -422,6 +439,15 @@ struct Common {
       x[2 * e + 1] = v.y;
     }
   }
+  // 16 factors of value rows, two by two
+  __device__ __forceinline__ static void factors(const float* at, float2 (&f)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float4 x = reinterpret_cast<const float4*>(at)[e];
+      f[2 * e] = make_float2(x.x, x.y);
+      f[2 * e + 1] = make_float2(x.z, x.w);
+    }
+  }
   static __device__ __noinline__ void wait_on(uint32_t bar, uint32_t parity, uint32_t* abort_flag, unsigned int* status) {
     (void)mbar_wait(bar, parity, abort_flag, status, JB200_STATUS_ATTN_MMA);
   }
@@ -436,6 +462,7 @@ struct Common {
 template <bool OUT>
 struct Prepare : Common {
   int group;
+  bool factor;                               // v counts as 0
 
   // Running sums of log2 a, in f64 for differences of late tokens: of two tokens a lane
   struct Gates {
@@ -616,7 +643,8 @@ struct Prepare : Common {
     const __nv_bfloat16* kp = p.k + first * p.ldk + size_t(part.h / p.per_key) * D;
     const __nv_bfloat16* qp = p.q + first * p.ldq + size_t(part.h / p.per_key) * D;
     Solve& so = sm.solve[group];
-    const int row = 16 * w + (lane >> 1), half = lane & 1;
+    const int tid = 32 * w + lane, row = tid >> 1, half = tid & 1;
+    const __nv_bfloat16* vp = p.v + first * p.ldv + size_t(part.h) * D + 8 * (tid & 7);
     uint4 k[4], q[4];
     float g0 = 0.f, g1 = 0.f, b0 = 0.f, b1 = 0.f;
     auto fetch = [&](int t0) {
@@ -637,6 +665,12 @@ struct Prepare : Common {
       Stage& st = sm.stage[s];
       Gates x;
       if (w == 3) x = gates(g0, g1);
+      uint4 v[4];                                // 16 bytes of four tokens, asked for here, so that they come while the stage gets free
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + 16 * i + (tid >> 3);
+        v[i] = load_now(vp + size_t(t) * p.ldv, !factor && t < part.len);
+      }
       if (n >= STAGES) bar_sync(BAR_FREE + s, GROUP + STATE + (OUT ? OUT_THREADS : 0));
       if (w == 3) {
         *reinterpret_cast<float2*>(st.beta + 2 * lane) = make_float2(b0, b1);
@@ -680,8 +714,23 @@ struct Prepare : Common {
         st.of_y[i] = beta * n1 * n1 * st.of_s[i] * r;
         st.of_u[i] *= r;
       }
+      {                                          // rounded twice: less than the 130 for 129 of the bound
+        uint32_t m[4] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = 16 * i + (tid >> 3);
+          const __nv_bfloat162 f = __float2bfloat162_rn(st.beta[t] * st.nk[t]);
+          const uint32_t in[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&in[j]), f);
+            *reinterpret_cast<__nv_bfloat162*>(&m[j]) = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&m[j]), __habs2(y));
+          }
+        }
+        st.most_v[4 * (tid & 7) + ((lane >> 3) & 3)][w] = most_of_four(m, lane);
+      }
       bar_sync(BAR_GROUP + group, GROUP);
-      if (OUT && lane == 0) mbar_arrive(smem_u32(&sm.bar_k[s]));
+      if (lane == 0) mbar_arrive(smem_u32(&sm.bar_k[s]));
       wait(sm.bar_a[group], n >> 1);
       rows_of_a(st, so);
       bar_sync(BAR_GROUP + group, GROUP);
@@ -732,86 +781,106 @@ struct Scores : Common {
 // ---- the group of the state ------------------------------------------------------------------------------------------
 template <bool OUT>
 struct Follow : Common {
-  // 16 values of a row in two terms, from unit `unit` on; most: the largest sizes among the hi terms
-  __device__ __forceinline__ static void put(const float2 (&x)[8], uint8_t* hi_tile, uint8_t* lo_tile, int row, int unit, uint32_t& most) {
+  // 16 values of a row in two terms, from unit `unit` on
+  __device__ __forceinline__ static void put(const float2 (&x)[8], uint8_t* hi_tile, uint8_t* lo_tile, int row, int unit) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        split(x[4 * u + e], hi[e], lo[e]);
-        most = max_f16x2(most, hi[e]);
-      }
+      for (int e = 0; e < 4; ++e) split(x[4 * u + e], hi[e], lo[e]);
       const uint32_t at = unit_at(row, unit + u);
       *reinterpret_cast<uint4*>(hi_tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       *reinterpret_cast<uint4*>(lo_tile + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
   }
-  __device__ __forceinline__ static float most(const float (&m)[4]) { return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])); }
-  __device__ __forceinline__ static float warp_most(float m) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))); }
+  // The largest |S| of value row 32 (w & 1) + lane, times the row's power, by a warp for 32 of them: of its tile's upper terms
+  __device__ __forceinline__ float largest_s() const {
+    const int unit = 4 * (w & 1) + (lane & 3), at = (lane >> 3) | (lane & 4);      // the two rows that eight lanes read differ in the swizzle
+    uint32_t m[4] = {};
+#pragma unroll
+    for (int i = 0; i < D; i += 8) {
+      const uint4 x = *reinterpret_cast<const uint4*>(sm.s_hi + unit_at(i + at, unit));
+      const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m[j] = __vmaxu2(m[j], in[j] & 0x7fff7fffu);
+    }
+    uint32_t most = most_of_four(m, lane);
+    most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 4));
+    const int pair = lane >> 1;
+    most = __shfl_sync(0xffffffffu, most, pair >> 2 | (pair & 3) << 3);
+    const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&most));
+    return (lane & 1 ? two.y : two.x) + 5.9604645e-8f;           // 2^-24: more than upper terms leave out
+  }
 
-  // The loops over a thread's 32 columns stay loops: the roles of this kernel share the instruction caches, and unrolled (77 KB in all) every one of
-  // them waited for its instructions (a chunk took 9600 cycles on 128 SMs).
+  // Loops over a thread's 32 columns stay loops where registers allow: the roles of this kernel share the instruction caches, and with all products unrolled
+  // (77 KB in all) every one of them waited for its instructions (a chunk took 9600 cycles on 128 SMs).  The one over X is open, since V, moved down
+  // between its turns, would be waited for where it is asked for.
   // from `from` (null: 0) through the part's chunks to `to`; `factor`: from the identity, with v as 0, which gives what the part multiplies a state by
   __device__ __forceinline__ void run(const float* from, float* to, bool factor) const {
     const int row = 32 * (w & 1) + lane, half = w >> 1;          // a key (S) or a token (X, U), and which 32 values of it
     const uint32_t cols = tm + TM_CHAIN + 32 * half;
     const __nv_bfloat16* vp = p.v + size_t(part.b) * p.T * p.ldv + size_t(part.h) * D + 32 * half;
     uint4 v[4];
-    if (part.chunks > 0) fetch_half(v, vp + size_t(part.begin + row) * p.ldv, !factor && part.begin + row < part.len);
-    // the state before the first chunk is added to none as if it were a product
-    float m = 0.f;
-    float2 S[16] = {};
+    float2 S[16];
 #pragma unroll
-    for (int c = 0; c < 16; c += 8) {
-      float2 x[8] = {};
-      tmem_st16(cols + 64 + 2 * c, x);
-      if (from != nullptr)
+    for (int e = 0; e < 16; ++e) {
+      const int i = 32 * half + 2 * e;
+      S[e] = from != nullptr ? make_float2(from[i * D + row], from[(i + 1) * D + row]) : make_float2(factor && i == row, factor && i + 1 == row);
+    }
+    const float2 none[8] = {};                                   // the product before the first chunk
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = make_float2(from[(32 * half + 2 * (c + e)) * D + row], from[(32 * half + 2 * (c + e) + 1) * D + row]);
-      else if (factor)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = make_float2(32 * half + 2 * (c + e) == row, 32 * half + 2 * (c + e) + 1 == row);
-      tmem_st16(cols + 2 * c, x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, fmaxf(fabsf(x[e].x), fabsf(x[e].y)));
+    for (int c = 0; c < 128; c += 64) {
+      tmem_st16(cols + c, none);
+      tmem_st16(cols + c + 16, none);
     }
     tmem_st_wait();
-    m = warp_most(m);
-    if (lane == 0) sm.most_s[1][w] = m;
+    auto values = [&](int n) {                                   // of a chunk
+      const int t = part.begin + n * CHUNK + row;
+      fetch_half(v, vp + size_t(t) * p.ldv, !factor && t < part.len);
+    };
+    // two of the warps that issue no products have a value row a thread, whose powers they give
+    const int v_row = threadIdx.x - 64;
+    float bound = 0.f, most_v = 0.f, whole = 1.f;
+    if (w >= 2) {
+      float m = factor ? 1.f : 0.f;
+      if (from != nullptr)
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) {
+          const float4 x = reinterpret_cast<const float4*>(from + v_row * D)[i];
+          m = fmaxf(fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+        }
+      bound = 8.f * m;
+      sm.power[0][v_row] = sm.inverse[1][v_row] = 1.f;           // where there are no chunks; of that product
+    }
+    auto powers = [&](int n) {                                   // of a chunk
+      wait(sm.bar_k[n % STAGES], n / STAGES);                    // V has been looked at
+      const uint4 of = *reinterpret_cast<const uint4*>(sm.stage[n % STAGES].most_v[v_row >> 1]);
+      const uint32_t pair = __vmaxu2(__vmaxu2(of.x, of.y), __vmaxu2(of.z, of.w));
+      most_v = v_row & 1 ? bf16_hi(pair) : bf16_lo(pair);
+      power_scale(fmaf(2.f, bound, 130.f * most_v), sm.power[n & 1][v_row], sm.inverse[n & 1][v_row]);
+    };
+    if (part.chunks > 0) {
+      values(0);
+      if (w >= 2) powers(0);
+    }
     bar_sync(BAR_STATE, STATE);
-    float bound = most(sm.most_s[1]), ix = 1.f, whole = 0.f;
     for (int n = 0;; ++n) {
-      float ps, is, px;
-      power_scale(bound, ps, is);
-      uint32_t m2 = 0;                           // of the hi terms, f16
 #pragma unroll
       for (int c = 0; c < 16; c += 8) {
-        float2 x[8], y[8];
+        float2 x[8], y[8], f[8];
+        factors(sm.inverse[(n + 1) & 1] + 32 * half + 2 * c, f);
         tmem_ld16x2(cols + 2 * c, cols + 64 + 2 * c, x, y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          S[c + e] = fma2(add2(x[e], y[e]), both(ix), mul2(S[c + e], both(whole)));
-          x[e] = mul2(S[c + e], both(ps));
-        }
-        put(x, sm.s_hi, sm.s_lo, row, 4 * half + (c >> 2), m2);
+        for (int e = 0; e < 8; ++e) S[c + e] = fma2(add2(x[e], y[e]), f[e], mul2(S[c + e], both(whole)));
+        factors(sm.power[n & 1] + 32 * half + 2 * c, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = mul2(S[c + e], f[e]);
+        put(x, sm.s_hi, sm.s_lo, row, 4 * half + (c >> 2));
       }
       if (n == part.chunks) break;
       const int s = n % STAGES;
       Stage& st = sm.stage[s];
       bar_sync(BAR_READY + s, GROUP + STATE + (OUT ? OUT_THREADS : 0));
-      const float m = warp_most(fmaxf(f16_lo(m2), f16_hi(m2))) * is;
-      m2 = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t m4 = 0x7fff7fffu;
-        m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(v[i].x & m4, v[i].y & m4), __vmaxu2(v[i].z & m4, v[i].w & m4)));
-      }
-      const float fv = st.of_v[row], mv = warp_most(fabsf(fv) * fmaxf(bf16_lo(m2), bf16_hi(m2)));
-      if (lane == 0) {
-        sm.most_s[n & 1][w] = m;
-        sm.most_v[n & 1][w] = mv;
-      }
       settle();
       if (OUT && n > 0) bar_sync(BAR_TAKEN, STATE + OUT_THREADS);
       else bar_sync(BAR_STATE, STATE);
@@ -822,25 +891,20 @@ struct Follow : Common {
         if (OUT) product<64, 0, 1>(sm.tmem + TM_QS, operand(st.q), operand(sm.s_hi), false);
         __syncwarp();
       }
-      const float ms = most(sm.most_s[n & 1]), mb = most(sm.most_v[n & 1]);
-      power_scale(fmaxf(fmaf(16.f, ms, 130.f * mb), bound * 7.8886091e-31f), px, ix);      // 2^-100: the powers' quotient stays in range
       whole = st.whole;
-      bound = fmaf(8.f * whole, ms, 64.f * mb);
-      const float fx = fv * px, fy = st.of_y[row] * (is * px), fu = st.of_u[row];
-      if (OUT && threadIdx.x == 0) sm.inverse[n & 1] = make_float2(is, ix);
-      uint32_t unused = 0;
+      const float fv = st.of_v[row], fy = st.of_y[row], fu = st.of_u[row];
       wait(sm.bar_y, n);
-#pragma unroll 1
+#pragma unroll
       for (int c = 0; c < 32; c += 16) {
-        float2 x[8], y[8];
+        float2 x[8], y[8], f[8];
+        factors(sm.power[n & 1] + 32 * half + c, f);
         tmem_ld16x2(cols + c, cols + 64 + c, x, y);
-        const uint32_t in[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
-        v[0] = v[2];
-        v[1] = v[3];
+        const uint4 a = v[c >> 3], b = v[(c >> 3) + 1];
+        const uint32_t in[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          x[e] = fma2(add2(x[e], y[e]), both(-fy), mul2(make_float2(bf16_lo(in[e]), bf16_hi(in[e])), both(fx)));
-        put(x, sm.x_hi, sm.x_lo, row, 4 * half + (c >> 3), unused);
+          x[e] = fma2(add2(x[e], y[e]), both(-fy), mul2(mul2(make_float2(bf16_lo(in[e]), bf16_hi(in[e])), both(fv)), f[e]));
+        put(x, sm.x_hi, sm.x_lo, row, 4 * half + (c >> 3));
       }
       settle();
       bar_sync(BAR_STATE, STATE);
@@ -851,8 +915,12 @@ struct Follow : Common {
         commit(sm.bar_u);
       }
       if (n + 1 < part.chunks) {
-        const int t = part.begin + (n + 1) * CHUNK + row;
-        fetch_half(v, vp + size_t(t) * p.ldv, !factor && t < part.len);
+        values(n + 1);
+        if (w >= 2) {
+          if ((n & 7) == 7) bound = fminf(bound, 8.1f * largest_s() * sm.inverse[n & 1][v_row]);
+          bound = fmaf(whole, bound, 64.5f * most_v);
+          powers(n + 1);
+        }
       }
       wait(sm.bar_u, n);
 #pragma unroll 1
@@ -870,7 +938,7 @@ struct Follow : Common {
           *reinterpret_cast<uint4*>(sm.u + unit_at(row, 4 * half + (c >> 3))) = make_uint4(one[0], one[1], one[2], one[3]);
           *reinterpret_cast<uint4*>(sm.u + unit_at(row, 4 * half + (c >> 3) + 1)) = make_uint4(one[4], one[5], one[6], one[7]);
         }
-        put(x, sm.x_hi, sm.x_lo, row, 4 * half + (c >> 3), unused);
+        put(x, sm.x_hi, sm.x_lo, row, 4 * half + (c >> 3));
       }
       settle();
       bar_sync(BAR_STATE, STATE);
@@ -907,18 +975,18 @@ struct Outputs : Common {
       const int s = n % STAGES, t = part.begin + n * CHUNK + row;
       const Stage& st = sm.stage[s];
       bar_sync(BAR_GIVEN, STATE + OUT_THREADS);
-      const float2 inverse = sm.inverse[n & 1];
-      const float fs = st.of_s[row] * inverse.x, fu = st.of_o[row] * inverse.y;
+      const float fs = st.of_s[row], fu = st.of_o[row];
       wait(sm.bar_o, n);
       if (n + STAGES < part.chunks) bar_arrive(BAR_FREE + s, GROUP + STATE + OUT_THREADS);
 #pragma unroll 1
       for (int c = 0; c < D; c += 16) {
-        float2 a[8], b[8];
+        float2 a[8], b[8], f[8];
+        factors(sm.inverse[n & 1] + c, f);
         tmem_ld16x2(tm + TM_QS + c, tm + TM_PU + c, a, b);
         uint32_t x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          a[e] = fma2(b[e], both(fu), mul2(a[e], both(fs)));
+          a[e] = mul2(fma2(b[e], both(fu), mul2(a[e], both(fs))), f[e]);
           x[e] = pack_bf16x2(a[e].x, a[e].y);
         }
         if (t < part.len) {
@@ -993,7 +1061,7 @@ __global__ void __launch_bounds__(3 * GROUP + (OUT ? 2 * OUT_THREADS : 0), 1) de
   if (warp < 4) {
     Follow<OUT>{common}.run(from, to, factor);
   } else if (warp < 12) {
-    Prepare<OUT>{common, (warp >> 2) - 1}.run();
+    Prepare<OUT>{common, (warp >> 2) - 1, factor}.run();
   } else if (OUT) {
     if (warp < 14) Outputs{common}.run();
     else Scores{common}.run();
