@@ -904,8 +904,9 @@ def gated_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
         d = _lib.Delta(B, T, H, KH, 64, _lib.DELTA_NORMALIZE if normalize else 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), ldq, ldk, ldv,
                        log_decay.data_ptr(), beta.data_ptr(), ldg, lens, 0.125 if scale is None else scale, s_in, o, ldo, s_out)
         nbytes = lib.jb200_gated_delta_scratch_bytes(B, T, H) if T > 1 else 0
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
-        rc = lib.jb200_gated_delta(ctypes.byref(d), scratch, _stream())
+        # held until the call has launched everything: freed before, another thread's launches on this stream could take its memory between ours
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        rc = lib.jb200_gated_delta(ctypes.byref(d), _ptr(scratch), _stream())
         if rc:
             _lib.check(rc, "jb200_gated_delta")
     return out, state_out
