@@ -110,17 +110,17 @@ SAMPLING = ("temperature", "top_k", "top_p", "min_p")
 
 def check_sampling(settings: Dict[str, float]) -> Dict[str, float]:
     """Settings of a draw, with None as what leaves that cut out; ValueError for anything that is none."""
-    unknown = sorted(set(settings) - set(SAMPLING))
+    unknown = sorted(str(name) for name in settings if name not in SAMPLING)
     if unknown:
         raise ValueError(f"sampling settings are {', '.join(SAMPLING)}, not {', '.join(unknown)}")
     out = {}
     for name, value in settings.items():
         try:
             v = 0.0 if value is None else float(value)
-        except (TypeError, ValueError):
-            raise ValueError(f"{name} must be a number, got {value!r}") from None
-        if not math.isfinite(v):
-            raise ValueError(f"{name} must be finite, got {value}")
+        except (TypeError, ValueError, OverflowError, RuntimeError):         # RuntimeError: a tensor of several numbers
+            raise ValueError(f"{name} must be one number, got {type(value).__name__}") from None
+        if not math.isfinite(v) or abs(v) > torch.finfo(torch.float32).max:  # slots hold f32
+            raise ValueError(f"{name} must be finite in 32 bits, got {v}")
         if name == "top_k" and (v != int(v) or not 0 <= v < 2 ** 31):
             raise ValueError(f"top_k must be an int, 0 or None for the whole vocabulary, got {value}")
         if name in ("top_p", "min_p") and not 0.0 <= v <= 1.0:

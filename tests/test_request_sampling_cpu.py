@@ -56,3 +56,23 @@ def test_an_engine_for_all_refuses_a_requests_own_before_it_touches_the_slot():
     eng.per_request = True
     with pytest.raises(ValueError, match="min_p"):
         eng.admit(0, [1, 2], max_new_tokens=4, sampling={"min_p": -1.0})
+
+
+def test_numbers_that_32_bits_do_not_hold_are_refused():
+    import torch
+    check = serving.check_sampling
+    for bad, text in (({"temperature": 1e39}, "finite"), ({"temperature": -1e39}, "finite"), ({"temperature": 10 ** 400}, "number"), ({"top_k": 10 ** 400}, "number"),
+                      ({"top_p": torch.zeros(2)}, "number"), ({"min_p": 1j}, "number"), ({1: 2, "x": 3}, "not 1, x")):
+        with pytest.raises(ValueError, match=text):
+            check(bad)
+    assert check({"temperature": torch.finfo(torch.float32).max})["temperature"] == torch.finfo(torch.float32).max
+
+
+def test_a_request_with_such_settings_does_not_end_the_others():
+    sched = serving.ContinuousBatchingScheduler(_Engine(), max_batch_size=2)
+    for i, own in enumerate((None, {"temperature": 1e39}, {"top_k": 10 ** 400}, {7: 1.0}, {"top_k": 5})):
+        sched.add_request(serving.Request(i, [1], 3, sampling=own))
+    sched.run()
+    by_id = {r.req_id: r for r in sched.completed}
+    assert [by_id[i].error is not None for i in range(5)] == [False, True, True, True, False]
+    assert all(by_id[i].is_finished and len(by_id[i].generated_tokens) == 3 for i in (0, 4))
