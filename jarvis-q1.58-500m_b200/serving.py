@@ -154,6 +154,8 @@ class CudaDecodeEngine:
             self.defaults = check_sampling(dict(zip(SAMPLING, (temperature, top_k, top_p, min_p))))
             self.rows = {name: torch.full((self.B,), v, dtype=torch.int32 if name == "top_k" else torch.float32,
                                           device=model.tok_emb.weight.device) for name, v in self.defaults.items()}
+            if per_request:
+                self.rows["temperature"].zero_()        # idle slots: see release
         self.pad_token = pad_token
         dev = model.tok_emb.weight.device
         self.device = dev
@@ -216,6 +218,8 @@ class CudaDecodeEngine:
     def release(self, slot: int):
         self._zero_slot(slot)
         self.active[slot] = 0
+        if self.per_request:
+            self.rows["temperature"][slot] = 0.0        # an idle slot's draw counts for nothing: the largest logit, which needs no filter
 
     def step(self, active_slots: List[int]) -> Dict[int, int]:
         """One token for every slot (idle ones run the pad token); returns {slot: token} for the active ones."""

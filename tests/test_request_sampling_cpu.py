@@ -76,3 +76,21 @@ def test_a_request_with_such_settings_does_not_end_the_others():
     by_id = {r.req_id: r for r in sched.completed}
     assert [by_id[i].error is not None for i in range(5)] == [False, True, True, True, False]
     assert all(by_id[i].is_finished and len(by_id[i].generated_tokens) == 3 for i in (0, 4))
+
+
+def test_a_released_slot_no_longer_draws_by_the_requests_settings():
+    import types
+
+    import torch
+    eng = serving.CudaDecodeEngine.__new__(serving.CudaDecodeEngine)
+    eng.max_position, eng.per_request, eng.pad_token = 64, True, 0
+    eng.defaults = serving.check_sampling(dict(temperature=0.7, top_k=50, top_p=0.9, min_p=None))
+    eng.rows = {n: torch.zeros(2, dtype=torch.int32 if n == "top_k" else torch.float32) for n in serving.SAMPLING}
+    eng.session = types.SimpleNamespace(state={"h": [torch.zeros(2, 4)], "S": [torch.zeros(2, 1, 2, 2)]}, positions=torch.zeros(2, dtype=torch.int32))
+    eng.next_token, eng.active = torch.zeros(2, 1, dtype=torch.int64), torch.zeros(2, dtype=torch.int32)
+    eng.admit(1, [5], 3, sampling={"top_k": 0, "top_p": 0.95})
+    assert eng.rows["temperature"].tolist() == [0.0, pytest.approx(0.7)] and eng.rows["top_k"].tolist() == [0, 0] and eng.active.tolist() == [0, 1]
+    eng.release(1)
+    assert eng.rows["temperature"].tolist() == [0.0, 0.0] and eng.active.tolist() == [0, 0]
+    eng.admit(1, [6], 3)                                          # the engine's own again
+    assert eng.rows["temperature"][1] == pytest.approx(0.7) and eng.rows["top_k"][1] == 50 and eng.rows["top_p"][1] == pytest.approx(0.9)
