@@ -23,9 +23,9 @@ sums.
 from __future__ import annotations
 
 import torch
-from torch.autograd import forward_ad
 
 from . import ops
+from .ops import _no_tangents
 
 
 def _bf16(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -40,15 +40,6 @@ def _trains(weight: torch.Tensor):
     """Marks a weight that is about to get a gradient: updates may leave no trace on it, so nobody keeps a copy (modules._in_training)."""
     if weight.requires_grad:
         weight._jb_trained = True
-
-
-def _no_tangents(what: str, *tensors):
-    """Dual tensors do not require gradients: their tangents would go missing where nothing else does."""
-    if getattr(forward_ad, "_current_level", 0) < 0:       # outside every dual_level there are none
-        return
-    for t in tensors:
-        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-            raise RuntimeError(f"{what}: a tensor carries a tangent, and there is no forward-mode derivative")
 
 
 def _rows(t: torch.Tensor, lead, dtypes, what: str, columns: int | None = None) -> torch.Tensor:

@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import ATTN_QK_PREPARED, EPI_BF16, EPI_F32, EPI_GELU_BF16, EPI_RESID_F32  # noqa: F401
@@ -786,8 +787,18 @@ def sample(logits: torch.Tensor, u: torch.Tensor | None = None, *, temperature: 
 
 # --------------------------------------------------------------------------- gated delta rule, norms around a block, draws
 # Results are allocated after an argument of their shape where there is one (empty_like: a third of the host time of empty with its keywords).
+def _no_tangents(what: str, *tensors):
+    """Dual tensors do not require gradients: their tangents would go missing where nothing else does."""
+    if getattr(forward_ad, "_current_level", 0) < 0:       # outside every dual_level there are none
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what}: a tensor carries a tangent, and there is no forward-mode derivative")
+
+
 def _forward_only(what: str, *tensors):
-    """These operators have no gradients: a graph that runs through one would lose its part without a word."""
+    """These operators have no derivatives: a graph that runs through one would lose its part without a word."""
+    _no_tangents(what, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -1008,7 +1019,7 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, *, temperature=0.7, top_k
     k-th largest, top_p drops a token when the sum of w before it exceeds top_p of what top_k left (never the first), min_p keeps w >= min_p, and the
     token is the first whose running sum over the rest exceeds u (f32 (B,), uniform in [0, 1)) times its whole.  Cf. sample_next_token
     (jarvis_engine/evaluate_jarvis.py:158-185).  NaN logits are -inf; a row without any logit above -inf gives token 0, probability 0.
-    -> int64 (B, 1) [, f32 (B,) probability of the token among what is left]."""
+    -> int64 (B, 1) [, f32 (B,) probability of the token among what is left, without a derivative: refused where one is wanted]."""
     lib = _lib.load()
     what = "sample_rows"
     if not logits.is_cuda:
@@ -1036,6 +1047,8 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, *, temperature=0.7, top_k
         s.min_p = _whole(min_p, dev, f32, B, what, "min_p", "one value or one per row")
     elif min_p is not None:
         s.min_p_all = min_p
+    if want_prob:                                # the token itself has no derivative
+        _forward_only(what, logits, *(t for t in (temperature, top_p, min_p) if torch.is_tensor(t)))
     if _elsewhere(logits):
         with torch.cuda.device(dev):
             return sample_rows(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, want_prob=want_prob)

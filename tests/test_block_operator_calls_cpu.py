@@ -50,3 +50,46 @@ def test_scratch_lives_until_everything_is_launched(library, monkeypatch):
     library.jb200_gated_delta = lambda d, scratch, stream: held.append([ref() is not None and at == scratch for ref, at in tensors]) or 0
     ops.gated_delta_scan(*_delta_args())
     assert held == [[True]]
+
+
+def _calls():
+    """name -> (a call with one of its tensors, the tensors that it may be)"""
+    rows, g, x, w = _on(0, 4, 128, dtype=BF16), _on(0, 4, 2), _on(0, 4, 128), _on(0, 128)
+    state = _on(0, 2, 2, 64, 64)
+    return {
+        "scan, q": (lambda t: ops.gated_delta_scan(t, rows, rows, g, g, 2, 2, 2), rows),
+        "scan, log_decay": (lambda t: ops.gated_delta_scan(rows, rows, rows, t, g, 2, 2, 2), g),
+        "scan, state": (lambda t: ops.gated_delta_scan(rows, rows, rows, g, g, 2, 2, 2, state_in=t), state),
+        "norm, y": (lambda t: ops.gated_norm(t, w), x),
+        "norm, weight": (lambda t: ops.gated_norm(x, t), w),
+        "norm, gate": (lambda t: ops.gated_norm(x, w, t), x),
+        "residual, x": (lambda t: ops.residual_norm(t, x, w, w), x),
+        "residual, scale": (lambda t: ops.residual_norm(x, x, w, w, scale=t), w),
+        "draw, logits": (lambda t: ops.sample_rows(t, _on(0, 4), want_prob=True), x),
+        "draw, temperature": (lambda t: ops.sample_rows(x, _on(0, 4), temperature=t, want_prob=True), _on(0, 4)),
+        "draw, min_p": (lambda t: ops.sample_rows(x, _on(0, 4), min_p=t, want_prob=True), _on(0, 4)),
+    }
+
+
+@pytest.mark.parametrize("name", list(_calls()))
+def test_derivatives_are_refused_not_dropped(library, name):
+    call, t = _calls()[name]
+    call(t)
+    assert len(library.seen) == 1
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(t.as_subclass(torch.Tensor), torch.ones(t.shape, dtype=t.dtype)).as_subclass(type(t))
+        assert torch.autograd.forward_ad.unpack_dual(dual).tangent is not None
+        for grad in (True, False):                                # no_grad does not end forward mode
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="tangent"):
+                call(dual)
+    wanted = t.clone().as_subclass(type(t)).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="gradient"):
+        call(wanted)
+    with torch.no_grad():
+        call(wanted)
+    assert len(library.seen) == 2
+
+
+def test_a_draw_without_its_probability_takes_logits_that_require_a_gradient(library):
+    ops.sample_rows(_on(0, 4, 128).requires_grad_(True), _on(0, 4))
+    assert [n for n, _ in library.seen] == ["jb200_sample_rows"]
