@@ -13,6 +13,7 @@ namespace {
 
 constexpr int D = 64;
 constexpr float NORM_EPS = 1e-6f;
+constexpr float SMALLER = 6.7762636e-21f, LARGER = 1.2379401e27f;      // 2^-67, 2^90: bring squares that are too large or too small for f32 into it
 
 struct DeltaParams {
   const __nv_bfloat16 *q, *k, *v;
@@ -107,13 +108,23 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
     float k[8], q[8];
     unpack8(now.k0, now.k1, k);
     unpack8(now.q0, now.q1, q);
-    float kk = 0.f, qq = 0.f, kq = 0.f;
+    float kk, qq, kq, eps_k = NORM_EPS, eps_q = NORM_EPS;
+    for (bool again = false;; again = true) {
+      kk = qq = kq = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { kk = fmaf(k[j], k[j], kk); qq = fmaf(q[j], q[j], qq); kq = fmaf(k[j], q[j], kq); }
-    kk = sum8(kk);
-    qq = sum8(qq);
-    kq = sum8(kq);
-    const float rk = p.normalize ? rsqrtf(kk + NORM_EPS) : 1.f, rq = (p.normalize ? rsqrtf(qq + NORM_EPS) : 1.f) * p.scale;
+      for (int j = 0; j < 8; ++j) { kk = fmaf(k[j], k[j], kk); qq = fmaf(q[j], q[j], qq); kq = fmaf(k[j], q[j], kq); }
+      kk = sum8(kk);
+      qq = sum8(qq);
+      kq = sum8(kq);
+      if (again || !p.normalize || !(fmaxf(kk, qq) == INFINITY)) break;
+      // squares that leave f32, the same in all lanes: once more of smaller rows, beside which NORM_EPS is nothing
+      const float fk = kk == INFINITY ? SMALLER : 1.f, fq = qq == INFINITY ? SMALLER : 1.f;
+      eps_k *= fk;
+      eps_q *= fq;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { k[j] *= fk; q[j] *= fq; }
+    }
+    const float rk = p.normalize ? rsqrtf(kk + eps_k) : 1.f, rq = (p.normalize ? rsqrtf(qq + eps_q) : 1.f) * p.scale;
     const float a = expf(now.g);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
@@ -159,7 +170,7 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 // reads its other operand once for both, and what bounds these small products is reading (6 KB in 48 cycles, 8 KB in 64, for 32 and 64 of
 // mathematics).  T's blocks come from mma.sync: products of 16 x 16.
 //
-// Bound by that chain, some 6400 cycles a chunk on every SM that has a head (8 sequences of 2048 tokens, 16 heads: 116 us, where reading and writing
+// Bound by that chain, some 6200 cycles a chunk on every SM that has a head (8 sequences of 2048 tokens, 16 heads: 113 us, where reading and writing
 // takes 21; with one power of two for all value rows, which is wrong beside an outlier, 5900 and 107).  With mma.sync alone a chunk took 10800, with these warps' parts but all products unrolled 9600: 77 KB of code, which the SMs fetch
 // again and again.
 //
@@ -386,20 +397,36 @@ __device__ __forceinline__ void fetch_half(uint4 (&x)[4], const __nv_bfloat16* a
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = load_now(at + 8 * i, on);
 }
-// ... and to f16 in a tile (`twice`: and in the next one), times the power of two s that brings the row's norm into [1, 2); returns the sum of
-// squares after that.  A sum of squares beyond f32's range makes the row NaN, one below it makes it 0.
+// ... and to f16 in a tile (`twice`: and in the next one), times the power of two s that brings the row's norm into [1, 2), or near it where s or its
+// inverse would leave f32 (2^126); returns the sum of squares after that.
 __device__ __forceinline__ float convert_half(const uint4 (&x)[4], uint8_t* tile, bool twice, int row, int half, float& s) {
-  float ss = 0.f, other = 0.f;
+  float ss;
+  auto squares = [&](float size) {                       // of the row times `size`; the power of two for their root
+    float other = 0.f;
+    ss = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { ss = fmaf(bf16_lo(in[j]), bf16_lo(in[j]), ss); other = fmaf(bf16_hi(in[j]), bf16_hi(in[j]), other); }
+      for (int j = 0; j < 4; ++j) {
+        const float a = bf16_lo(in[j]) * size, b = bf16_hi(in[j]) * size;
+        ss = fmaf(a, a, ss);
+        other = fmaf(b, b, other);
+      }
+    }
+    ss += other;
+    ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+    const int e = (int(__float_as_uint(ss) >> 23) - 127) >> 1;                   // ss in [4^e, 4^(e + 1))
+    return __uint_as_float(uint32_t(127 - e) << 23);
+  };
+  float t = squares(1.f);
+  s = t;
+  constexpr float LEAST = 8.2718061e-25f;                // 2^-80: below, squares of its addends may be subnormal
+  if (__builtin_expect(__any_sync(0xffffffffu, ss == INFINITY || ss < LEAST), 0)) {
+    const float size = ss == INFINITY ? SMALLER : ss < LEAST ? LARGER : 1.f;
+    t = fminf(fmaxf(squares(size), 1.17549435e-38f / size), 8.5070592e37f / size);
+    s = t * size;
   }
-  ss += other;
-  ss += __shfl_xor_sync(0xffffffffu, ss, 1);
-  const int e = (int(__float_as_uint(ss) >> 23) - 127) >> 1;                     // ss in [4^e, 4^(e + 1))
-  s = __uint_as_float(uint32_t(127 - e) << 23);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
@@ -410,7 +437,7 @@ __device__ __forceinline__ float convert_half(const uint4 (&x)[4], uint8_t* tile
     *reinterpret_cast<uint4*>(to) = make_uint4(out[0], out[1], out[2], out[3]);
     if (twice) *reinterpret_cast<uint4*>(to + TILE) = make_uint4(out[0], out[1], out[2], out[3]);
   }
-  return ss * s * s;
+  return ss * t * t;
 }
 
 struct Common {
@@ -685,12 +712,13 @@ struct Prepare : Common {
         const float ss = convert_half(k, m == 0 ? st.k_again : st.q, m == 0, row, half, sc);
         if (half == 0) {
           // k = n (k16 r) with |k16 r| = 1, or of the normalised key n = 1 and k16 r its value
-          const float r = p.normalize ? rsqrtf(fmaf(NORM_EPS * sc, sc, ss)) : ss > 0.f ? rsqrtf(ss) : 0.f;
+          const float inv = inverse_power(sc);
+          const float r = !p.normalize ? ss > 0.f ? rsqrtf(ss) : 0.f : sc > 1e12f ? inv * 1e3f : rsqrtf(fmaf(NORM_EPS * sc, sc, ss));
           if (m == 0) {
             st.rk[row] = r;
-            st.nk[row] = p.normalize ? 1.f : ss * r * inverse_power(sc);
+            st.nk[row] = p.normalize ? 1.f : ss * r * inv;
           } else {
-            st.of_o[row] = p.scale * (p.normalize ? r : inverse_power(sc));
+            st.of_o[row] = p.scale * (p.normalize ? r : inv);
           }
         }
         if (OUT) {

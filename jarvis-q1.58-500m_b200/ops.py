@@ -858,7 +858,7 @@ def gated_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     S_t = a_t S_{t-1} (I - b_t k k^T) + b_t v k^T with a = exp(log_decay), o_t = scale S_t q_t.
     q, k: bf16 2-D views (B*T, key_heads*64), v: bf16 (B*T, H*64), each with a row stride of its own (e.g. column slices of a fused
     projection; 16-byte aligned, strides multiples of 8); value head h takes key head h // (H // key_heads).  log_decay (<= 0), beta: f32 (B*T, H), column
-    slices allowed.  normalize: k and q are divided by their norms, sqrt(|.|^2 + 1e-6); without it keep beta |k|^2 <= 2.  scale: 1/8 unless given.
+    slices allowed.  normalize: k and q are divided by their norms, sqrt(|.|^2 + 1e-6).  Keep 0 <= beta |k|^2 <= 2 (normalised: beta <= 2).  scale: 1/8 unless given.
     lengths: int32 (B,), for padded batches: rows behind a sequence's length are not read, their output is 0, the state is that after its last row.
     Returns (o bf16 (B*T, H*64) or None, state f32 (B, H, 64 values, 64 keys) or None).  state_out may be state_in itself; out and state_out must
     otherwise lie outside of every argument, from its first to its last element (other columns of one buffer are inside)."""

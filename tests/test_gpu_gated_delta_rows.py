@@ -107,3 +107,30 @@ def test_rows_do_not_know_of_one_another():
     s2 = torch.where(keep[:, None], s, s * 1e-15)
     o2, S2 = _scan((q, k, v2, g, b, s2), B, T, H)
     assert torch.equal(S[:, :, keep], S2[:, :, keep]) and torch.equal(o[:, keep.repeat(H)], o2[:, keep.repeat(H)])
+
+
+@pytest.mark.parametrize("B,T", FORMS)
+def test_keys_and_queries_whose_squares_leave_f32(B, T):
+    """Sums of squares from nothing to 2^250: normalised rows are what they are at any size that bf16 holds."""
+    H = 2
+    q, k, v, g, b, s = _problem(B, T, H, H, seed=16)
+    size = torch.logspace(-30, 37, B * T, device="cuda")[torch.randperm(B * T, generator=torch.Generator().manual_seed(T)).cuda()][:, None]
+    if T == 1:
+        size = torch.tensor([[1e37], [1e22]], device="cuda")
+    k, q = (k.float() * size).to(BF16), (q.float() * size.flip(0)).to(BF16)
+    assert torch.isfinite(k).all() and torch.isfinite(q).all() and (k.float().view(B * T, H, D).square().sum(-1) == math.inf).any()
+    p = (q, k, v, g, b, s)
+    _check(_scan(p, B, T, H), _definition(*p, B, T, H, H))
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("B,T", [(2, 10), (2, 190)])
+@pytest.mark.parametrize("size", [1e-25, 1e25, 1e36])
+def test_queries_of_any_size_taken_as_they_are(B, T, size):
+    H = 2
+    q, k, v, g, b, s = _problem(B, T, H, H, seed=17)
+    k = torch.nn.functional.normalize(k.float().view(-1, D), dim=1).to(BF16).view(B * T, H * D)
+    q = (q.float() * size).to(BF16)
+    p = (q, k, v, g, b, s)
+    wo, wS, tol, off = _definition(*p, B, T, H, H, normalize=False, scale=0.125 / size)
+    _check(_scan(p, B, T, H, normalize=False, scale=0.125 / size), (wo, wS, 2 * tol, 2 * off))      # |k|^2 of up to 1 + 2^-7 for the 1 of the derivation
