@@ -911,7 +911,7 @@ def gated_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
             ldo = _view(out, dev, (N, H * 64), bf16, what, "out")
             _apart(what, "out", out, q, k, v, log_decay, beta, lengths, state_in)
         o = out.data_ptr()
-    if B:
+    if B and (T or s_out is not None):           # without tokens and a state nothing is there to be written
         d = _lib.Delta(B, T, H, KH, 64, _lib.DELTA_NORMALIZE if normalize else 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), ldq, ldk, ldv,
                        log_decay.data_ptr(), beta.data_ptr(), ldg, lens, 0.125 if scale is None else scale, s_in, o, ldo, s_out)
         nbytes = lib.jb200_gated_delta_scratch_bytes(B, T, H) if T > 1 else 0

@@ -93,3 +93,13 @@ def test_derivatives_are_refused_not_dropped(library, name):
 def test_a_draw_without_its_probability_takes_logits_that_require_a_gradient(library):
     ops.sample_rows(_on(0, 4, 128).requires_grad_(True), _on(0, 4))
     assert [n for n, _ in library.seen] == ["jb200_sample_rows"]
+
+
+def test_no_tokens_and_no_state_is_an_empty_output(monkeypatch):
+    """The library itself, which has no address of an empty output to tell it from none."""
+    monkeypatch.setattr(ops, "_raw_device", lambda: 0)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    rows, g = _on(0, 0, 128, dtype=BF16), _on(0, 0, 2)
+    for B, T in ((3, 0), (0, 5), (0, 0)):
+        o, state = ops.gated_delta_scan(rows, rows, rows, g, g, B, T, 2)
+        assert o.shape == (0, 128) and o.dtype is BF16 and state is None
