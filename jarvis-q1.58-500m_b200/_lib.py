@@ -52,7 +52,7 @@ class Delta(C.Structure):
     _fields_ = [(n, _I) for n in ("B", "T", "H", "key_heads", "head_dim", "flags")] + [("q", _P), ("k", _P), ("v", _P)] + \
                [(n, C.c_longlong) for n in ("ldq", "ldk", "ldv")] + \
                [("log_decay", _P), ("beta", _P), ("ldg", C.c_longlong), ("lengths", _P), ("scale", _F), ("s_in", _P), ("o", _P),
-                ("ldo", C.c_longlong), ("s_out", _P)]
+                ("ldo", C.c_longlong), ("s_out", _P), ("ldb", C.c_longlong)]
 
 
 class Sampling(C.Structure):

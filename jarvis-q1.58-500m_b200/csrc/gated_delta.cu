@@ -17,8 +17,8 @@ constexpr float SMALLER = 6.7762636e-21f, LARGER = 1.2379401e27f;      // 2^-67,
 
 struct DeltaParams {
   const __nv_bfloat16 *q, *k, *v;
-  size_t ldq, ldk, ldv, ldo, ldg;           // elements
-  const float *log_decay, *beta;            // [B T][ldg]
+  size_t ldq, ldk, ldv, ldo, ldg, ldb;      // elements
+  const float *log_decay, *beta;            // [B T][ldg], [B T][ldb]
   const int32_t* lengths;                   // [B] or null
   const float* s_in;                        // [B][H][64][64] or null
   float* s_out;                             // or null
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
   const __nv_bfloat16* qp = p.q + first * p.ldq + size_t(h / p.per_key) * D + 4 * l;
   const __nv_bfloat16* vp = p.v + first * p.ldv + size_t(h) * D + row0;
   const float* gp = p.log_decay + first * p.ldg + h;
-  const float* bp = p.beta + first * p.ldg + h;
+  const float* bp = p.beta + first * p.ldb + h;
   Token next;
   float v_next[ROWS];
   auto fetch = [&](int t) {
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
     next.q0 = *reinterpret_cast<const uint2*>(qp + size_t(t) * p.ldq);
     next.q1 = *reinterpret_cast<const uint2*>(qp + size_t(t) * p.ldq + 32);
     next.g = gp[size_t(t) * p.ldg];
-    next.beta = bp[size_t(t) * p.ldg];
+    next.beta = bp[size_t(t) * p.ldb];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) v_next[r] = __bfloat162float(vp[size_t(t) * p.ldv + 16 * r]);
   };
@@ -681,9 +681,9 @@ struct Prepare : Common {
       if (w == 3) {
         const int t = t0 + 2 * lane;
         g0 = t < part.len ? load_now(p.log_decay + (first + t) * p.ldg + part.h) : 0.f;
-        b0 = t < part.len ? load_now(p.beta + (first + t) * p.ldg + part.h) : 0.f;
+        b0 = t < part.len ? load_now(p.beta + (first + t) * p.ldb + part.h) : 0.f;
         g1 = t + 1 < part.len ? load_now(p.log_decay + (first + t + 1) * p.ldg + part.h) : 0.f;
-        b1 = t + 1 < part.len ? load_now(p.beta + (first + t + 1) * p.ldg + part.h) : 0.f;
+        b1 = t + 1 < part.len ? load_now(p.beta + (first + t + 1) * p.ldb + part.h) : 0.f;
       }
     };
     if (group < part.chunks) fetch(part.begin + group * CHUNK);
@@ -1192,7 +1192,7 @@ int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream)
   if (B == 0) return JB200_OK;
   JB_REQUIRE(d->o != nullptr || d->s_out != nullptr, "gated_delta: neither an output nor a final state is asked for");
   JB_REQUIRE(T == 0 || (d->q && d->k && d->v && d->log_decay && d->beta), "gated_delta: null pointer");
-  JB_REQUIRE(d->ldq >= KH * D && d->ldk >= KH * D && d->ldv >= H * D && d->ldg >= H && (d->o == nullptr || d->ldo >= H * D),
+  JB_REQUIRE(d->ldq >= KH * D && d->ldk >= KH * D && d->ldv >= H * D && d->ldg >= H && (d->ldb == 0 || d->ldb >= H) && (d->o == nullptr || d->ldo >= H * D),
              "gated_delta: row strides are smaller than the rows");
   JB_REQUIRE(aligned16(d->q) && aligned16(d->k) && aligned16(d->v) && aligned16(d->o) && aligned16(d->s_in) && aligned16(d->s_out) &&
                  d->ldq % 8 == 0 && d->ldk % 8 == 0 && d->ldv % 8 == 0 && (d->o == nullptr || d->ldo % 8 == 0),
@@ -1201,7 +1201,7 @@ int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream)
   p.q = static_cast<const __nv_bfloat16*>(d->q);
   p.k = static_cast<const __nv_bfloat16*>(d->k);
   p.v = static_cast<const __nv_bfloat16*>(d->v);
-  p.ldq = d->ldq; p.ldk = d->ldk; p.ldv = d->ldv; p.ldo = d->ldo; p.ldg = d->ldg;
+  p.ldq = d->ldq; p.ldk = d->ldk; p.ldv = d->ldv; p.ldo = d->ldo; p.ldg = d->ldg; p.ldb = d->ldb != 0 ? d->ldb : d->ldg;
   p.log_decay = d->log_decay; p.beta = d->beta; p.lengths = d->lengths; p.s_in = d->s_in; p.s_out = d->s_out;
   p.o = static_cast<__nv_bfloat16*>(d->o);
   p.B = B; p.T = T; p.H = H; p.per_key = H / KH;

@@ -857,8 +857,8 @@ def gated_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     """The gated delta rule over sequences of T tokens, T = 1 being a decode step:
     S_t = a_t S_{t-1} (I - b_t k k^T) + b_t v k^T with a = exp(log_decay), o_t = scale S_t q_t.
     q, k: bf16 2-D views (B*T, key_heads*64), v: bf16 (B*T, H*64), each with a row stride of its own (e.g. column slices of a fused
-    projection; 16-byte aligned, strides multiples of 8); value head h takes key head h // (H // key_heads).  log_decay (<= 0), beta: f32 (B*T, H), column
-    slices allowed.  normalize: k and q are divided by their norms, sqrt(|.|^2 + 1e-6).  Keep 0 <= beta |k|^2 <= 2 (normalised: beta <= 2).  scale: 1/8 unless given.
+    projection; 16-byte aligned, strides multiples of 8); value head h takes key head h // (H // key_heads).  log_decay (<= 0), beta: f32 (B*T, H), each
+    with a row stride of its own.  normalize: k and q are divided by their norms, sqrt(|.|^2 + 1e-6).  Keep 0 <= beta |k|^2 <= 2 (normalised: beta <= 2).  scale: 1/8 unless given.
     lengths: int32 (B,), for padded batches: rows behind a sequence's length are not read, their output is 0, the state is that after its last row.
     Returns (o bf16 (B*T, H*64) or None, state f32 (B, H, 64 values, 64 keys) or None).  state_out may be state_in itself; out and state_out must
     otherwise lie outside of every argument, from its first to its last element (other columns of one buffer are inside)."""
@@ -872,8 +872,7 @@ def gated_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     ldk = _view(k, dev, (N, KH * 64), bf16, what, "k")
     ldv = _view(v, dev, (N, H * 64), bf16, what, "v")
     ldg = _view(log_decay, dev, (N, H), f32, what, "log_decay")
-    if _view(beta, dev, (N, H), f32, what, "beta") != ldg:
-        raise RuntimeError(f"{what}: log_decay and beta must share their row stride")
+    ldb = _view(beta, dev, (N, H), f32, what, "beta")
     if not q.is_cuda:
         raise RuntimeError(f"{what}.q: expected a CUDA tensor (this path has no CPU fallback)")
     _forward_only(what, q, k, v, log_decay, beta, state_in, state_out, out)
@@ -913,7 +912,7 @@ def gated_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
         o = out.data_ptr()
     if B and (T or s_out is not None):           # without tokens and a state nothing is there to be written
         d = _lib.Delta(B, T, H, KH, 64, _lib.DELTA_NORMALIZE if normalize else 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), ldq, ldk, ldv,
-                       log_decay.data_ptr(), beta.data_ptr(), ldg, lens, 0.125 if scale is None else scale, s_in, o, ldo, s_out)
+                       log_decay.data_ptr(), beta.data_ptr(), ldg, lens, 0.125 if scale is None else scale, s_in, o, ldo, s_out, ldb)
         nbytes = lib.jb200_gated_delta_scratch_bytes(B, T, H) if T > 1 else 0
         # held until the call has launched everything: freed before, another thread's launches on this stream could take its memory between ours
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None

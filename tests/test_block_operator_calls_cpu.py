@@ -103,3 +103,23 @@ def test_no_tokens_and_no_state_is_an_empty_output(monkeypatch):
     for B, T in ((3, 0), (0, 5), (0, 0)):
         o, state = ops.gated_delta_scan(rows, rows, rows, g, g, B, T, 2)
         assert o.shape == (0, 128) and o.dtype is BF16 and state is None
+
+
+def test_gates_have_row_strides_of_their_own(library):
+    rows, both, beta = _on(0, 4, 128, dtype=BF16), _on(0, 4, 4), _on(0, 4, 2)
+    seen = []
+    library.jb200_gated_delta = lambda d, *a: seen.append((d._obj.ldg, d._obj.ldb)) or 0
+    sliced = both[:, :2].as_subclass(type(both))
+    ops.gated_delta_scan(rows, rows, rows, sliced, beta, 2, 2, 2)
+    ops.gated_delta_scan(rows, rows, rows, beta, sliced, 2, 2, 2)
+    ops.gated_delta_scan(rows, rows, rows, sliced, sliced, 2, 2, 2)
+    assert seen == [(4, 2), (2, 4), (4, 4)]
+
+
+@pytest.mark.parametrize("ldb,text", [(3, "row strides"), (-4, "row strides")])
+def test_a_stride_of_beta_that_does_not_hold_a_row_is_refused(ldb, text):
+    import ctypes
+
+    from jarvis_b200 import _lib
+    from tests.test_block_operators_cpu import _delta
+    assert _lib.load().jb200_gated_delta(ctypes.byref(_delta(ldb=ldb)), None, None) == _lib.ERR_ARG and text in _lib.last_error()

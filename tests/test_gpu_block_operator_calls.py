@@ -38,3 +38,16 @@ def test_two_threads_on_one_stream():
     for got, want in zip(results, alone):
         assert len(got) == 40 and all(torch.equal(a, b) for g in got for a, b in zip(g, want))
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("T", [1, 9, 200, 1500])
+def test_gates_with_row_strides_of_their_own(T):
+    """A slice of one projection beside a tensor of its own: the bits of two contiguous ones."""
+    B, H = 1, 3
+    q, k, v, g, b, s = delta._problem(B, T, H, H, seed=31)
+    wide = torch.full((B * T, 2 * H + 1), float("nan"), device="cuda")
+    wide[:, :H], wide[:, H:2 * H] = g, b
+    want = ops.gated_delta_scan(q, k, v, g, b, B, T, H, state_in=s, want_state=True)
+    for log_decay, beta in ((wide[:, :H], b), (g, wide[:, H:2 * H]), (wide[:, :H], wide[:, H:2 * H])):
+        got = ops.gated_delta_scan(q, k, v, log_decay, beta, B, T, H, state_in=s, want_state=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
