@@ -194,6 +194,8 @@ typedef struct jb200_delta {
 } jb200_delta;
 size_t jb200_gated_delta_scratch_bytes(int B, int T, int H);
 int jb200_gated_delta(const jb200_delta* d, void* scratch, void* stream);
+/* How a sequence is cut on a device with `sms` SMs: pieces, chunks of 64 tokens of each; out2 may be NULL.  Returns the scratch's bytes. */
+size_t jb200_host_delta_plan(int B, int T, int H, int sms, int32_t* out2);
 
 /* ---- block glue --------------------------------------------------------------------- */
 

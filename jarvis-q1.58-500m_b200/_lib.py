@@ -110,6 +110,7 @@ PROTOTYPES = {
     "jb200_rmsnorm_backward_scratch_bytes": (_Z, [_I] * 2),
     "jb200_rmsnorm_backward": (_I, [_P, _I, _P, _F, _P, _I, _I, _I, _P, _P, _P, _P]),
     "jb200_gated_delta_scratch_bytes": (_Z, [_I] * 3),
+    "jb200_host_delta_plan": (_Z, [_I] * 4 + [C.POINTER(C.c_int32)]),
     "jb200_gated_delta": (_I, [C.POINTER(Delta), _P, _P]),
     "jb200_gated_norm": (_I, [_P, _I, C.c_longlong, _P, _P, C.c_longlong, _I, _F, _P, _I, _I, _I, _P]),
     "jb200_residual_norm": (_I, [_P, _P, _I, C.c_longlong, _P, _P, C.c_longlong, _P, _P, _F, _P, _P, _I, _I, _I, _P]),

@@ -501,6 +501,7 @@ int jb200_rmsnorm_backward(const void* x, int x_dtype, const float* w, float eps
 }
 
 size_t jb200_gated_delta_scratch_bytes(int B, int T, int H) { return gated_delta_scratch_bytes(B, T, H); }
+size_t jb200_host_delta_plan(int B, int T, int H, int sms, int32_t* out2) { return delta_plan_host(B, T, H, sms, out2); }
 int jb200_gated_delta(const jb200_delta* d, void* scratch, void* stream) {
   return launch_gated_delta(d, scratch, static_cast<cudaStream_t>(stream));
 }

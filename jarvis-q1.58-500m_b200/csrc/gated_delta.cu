@@ -1159,8 +1159,8 @@ int chunk_tokens(int heads) { return heads < 2 * sm_count() ? 12 : 24; }
 // to fill the pipeline, on as many waves of CTAs as it has (1 CTA an SM); the pieces' pass has 2 n - 3 CTAs a head for the outputs' n; the join takes 1
 // and a quarter a segment.  The smaller sum wins, segments only by a tenth.  16 heads, us whole / in segments: 512 tokens 35 / 32 (not taken), 1024
 // 60 / 42, 4096 209 / 86, 16384 797 / 261; 2 sequences of 2048 110 / 80; with 4 sequences of 2048 there is nothing to gain.
-int segments_of(int B, int T, int H) {
-  const long long sms = sm_count(), heads = (long long)B * H, chunks = (T + CHUNK - 1) / CHUNK;
+int segments_of(int B, int T, int H, long long sms) {
+  const long long heads = (long long)B * H, chunks = (T + CHUNK - 1) / CHUNK;
   auto waves = [&](long long ctas) { return (ctas + sms - 1) / sms; };
   const double whole = double(waves(heads) * chunks);
   double least = 0.9 * whole;
@@ -1176,11 +1176,17 @@ int segments_of(int B, int T, int H) {
 
 }  // namespace
 
-size_t gated_delta_scratch_bytes(int B, int T, int H) {
-  if (B < 1 || H < 1 || T < 1) return 0;
-  const int n = segments_of(B, T, H);
+size_t delta_plan_host(int B, int T, int H, int sms, int32_t* out2) {
+  const bool any = B >= 1 && H >= 1 && T >= 1;
+  const int n = any ? segments_of(B, T, H, sms) : 1, chunks = any ? (T + CHUNK - 1) / CHUNK : 0;
+  if (out2 != nullptr) {
+    out2[0] = n;
+    out2[1] = (chunks + n - 1) / n;
+  }
   return n == 1 ? 0 : piece_at(n, B * H, 0) * sizeof(float);
 }
+
+size_t gated_delta_scratch_bytes(int B, int T, int H) { return delta_plan_host(B, T, H, sm_count(), nullptr); }
 
 int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream) {
   JB_REQUIRE(d != nullptr, "gated_delta: null pointer");
@@ -1214,7 +1220,7 @@ int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream)
     JB_MAX_SMEM(delta_chunk_kernel<true>, CHUNK_SMEM);
     JB_MAX_SMEM(delta_chunk_kernel<false>, CHUNK_SMEM);
     if (scratch != nullptr) {
-      const int n = segments_of(B, T, H);
+      const int n = segments_of(B, T, H, sm_count());
       JB_REQUIRE(aligned16(scratch), "gated_delta: scratch must be 16-byte aligned");
       if (n > 1) {
         p.segments = n;

@@ -194,6 +194,7 @@ int launch_sample(const void* logits, int logits_dtype, int ld, int n_rows, int 
                   float top_p, const float* u, int64_t* out_token, float* out_prob, cudaStream_t stream);
 
 size_t gated_delta_scratch_bytes(int B, int T, int H);
+size_t delta_plan_host(int B, int T, int H, int sms, int32_t* out2);
 int launch_gated_delta(const jb200_delta* d, void* scratch, cudaStream_t stream);
 int launch_gated_norm(const void* y, int y_dtype, long long ldy, const float* w, const void* gate, long long ldg, int group, float eps, void* out,
                       int out_dtype, int n_rows, int C, cudaStream_t stream);

@@ -123,3 +123,34 @@ def test_a_stride_of_beta_that_does_not_hold_a_row_is_refused(ldb, text):
     from jarvis_b200 import _lib
     from tests.test_block_operators_cpu import _delta
     assert _lib.load().jb200_gated_delta(ctypes.byref(_delta(ldb=ldb)), None, None) == _lib.ERR_ARG and text in _lib.last_error()
+
+
+def _plan(B, T, H, sms=148):
+    import ctypes
+
+    from jarvis_b200 import _lib
+    out = (ctypes.c_int32 * 2)()
+    nbytes = _lib.load().jb200_host_delta_plan(B, T, H, sms, out)
+    return out[0], out[1], nbytes
+
+
+@pytest.mark.parametrize("B,T,H,pieces,chunks", [(1, 16384, 16, 6, 43), (2, 2048, 16, 3, 11), (1, 512, 16, 1, 8), (8, 2048, 16, 1, 32), (4, 2048, 16, 1, 32),
+                                                 (1, 64, 16, 1, 1), (3, 777, 16, 1, 13), (0, 100, 16, 1, 0), (2, 0, 16, 1, 0)])
+def test_pieces_of_a_sequence(B, T, H, pieces, chunks):
+    """Worked out by hand from the rule's costs: (chunks + 1) (waves of 2 n - 3 CTAs a head + waves of n) + 1 + n / 4 against nine tenths of the chunks."""
+    assert _plan(B, T, H)[:2] == (pieces, chunks)
+
+
+@pytest.mark.parametrize("sms", [148, 132, 20])
+def test_pieces_hold_a_sequence_and_none_is_empty(sms):
+    cut = 0
+    for B, H in ((1, 1), (1, 3), (1, 16), (2, 16), (3, 16), (5, 3), (64, 16)):
+        for T in (*range(1, 4100, 61), 5000, 8191, 8192, 16384, 65536, 1 << 20, 1 << 30):
+            n, chunks, nbytes = _plan(B, T, H, sms)
+            whole = -(-T // 64)
+            assert n == 1 or (3 <= n <= 32 and B * H * n <= 2 * sms)
+            assert (n - 1) * chunks < whole <= n * chunks
+            assert nbytes == (0 if n == 1 else (2 * n - 1) * B * H * 64 * 64 * 4)
+            cut += n > 1
+    assert cut > 100 or sms == 20
+    assert _plan(64, 1 << 20, 16, sms)[0] == 1
