@@ -1151,14 +1151,14 @@ __global__ void __launch_bounds__(128) delta_join_kernel(DeltaParams p) {
 }
 
 // In chunks from so many tokens on.  A chunk's pass takes as long for one token as for 64, a token's step the longer the more heads there are.  us
-// token by token / in chunks: 16 heads, 8 tokens 11.4 / 12.8, 16 tokens 16.4 / 12.7; 256 heads, 8 tokens 16.0 / 20.9, 16 tokens 24.1 / 21.5;
-// 1024 heads, 16 tokens 46 / 61, 24 tokens 63.5 / 61.7.
-int chunk_tokens(int heads) { return heads < 2 * sm_count() ? 12 : 24; }
+// from cold token by token / in chunks: 16 heads, 8 tokens 12.3 / 12.3, 16 tokens 18.5 / 12.3; 256 heads, 8 tokens 16.4 / 22.5, 16 tokens 24.6 / 22.5;
+// 304 heads, 24 tokens 30.7 / 30.8, 32 tokens 38.9 / 31.2; 1024 heads, 24 tokens 63.5 / 69.6, 32 tokens 79.9 / 71.7.
+int chunk_tokens(int heads) { return heads < 2 * sm_count() ? 12 : 28; }
 
 // Segments of a sequence where sequences and heads alone leave SMs idle.  In chunks' time, about 3 us: a pass over the tokens costs its chunks, and one
 // to fill the pipeline, on as many waves of CTAs as it has (1 CTA an SM); the pieces' pass has 2 n - 3 CTAs a head for the outputs' n; the join takes 1
-// and a quarter a segment.  The smaller sum wins, segments only by a tenth.  16 heads, us whole / in segments: 512 tokens 35 / 32 (not taken), 1024
-// 60 / 42, 4096 209 / 86, 16384 797 / 261; 2 sequences of 2048 110 / 80; with 4 sequences of 2048 there is nothing to gain.
+// and a quarter a segment.  The smaller sum wins, segments only by a tenth.  16 heads, us whole / in segments: 512 tokens 37 / 33 (not taken), 1024
+// 63 / 43, 4096 217 / 89, 16384 839 / 269; 2 sequences of 2048 115 / 83; with 4 sequences of 2048 there is nothing to gain.
 int segments_of(int B, int T, int H, long long sms) {
   const long long heads = (long long)B * H, chunks = (T + CHUNK - 1) / CHUNK;
   auto waves = [&](long long ctas) { return (ctas + sms - 1) / sms; };
