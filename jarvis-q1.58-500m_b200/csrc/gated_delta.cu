@@ -680,10 +680,11 @@ struct Prepare : Common {
       if (OUT) fetch_half(q, qp + size_t(at) * p.ldq + 32 * half, at < part.len);
       if (w == 3) {
         const int t = t0 + 2 * lane;
-        g0 = t < part.len ? load_now(p.log_decay + (first + t) * p.ldg + part.h) : 0.f;
-        b0 = t < part.len ? load_now(p.beta + (first + t) * p.ldb + part.h) : 0.f;
-        g1 = t + 1 < part.len ? load_now(p.log_decay + (first + t + 1) * p.ldg + part.h) : 0.f;
-        b1 = t + 1 < part.len ? load_now(p.beta + (first + t + 1) * p.ldb + part.h) : 0.f;
+        const float *gp = p.log_decay + (first + t) * p.ldg + part.h, *bp = p.beta + (first + t) * p.ldb + part.h;
+        g0 = t < part.len ? load_now(gp) : 0.f;
+        b0 = t < part.len ? load_now(bp) : 0.f;
+        g1 = t + 1 < part.len ? load_now(gp + p.ldg) : 0.f;
+        b1 = t + 1 < part.len ? load_now(bp + p.ldb) : 0.f;
       }
     };
     if (group < part.chunks) fetch(part.begin + group * CHUNK);
