@@ -569,8 +569,9 @@ int jb200_sample(const void* logits, int logits_dtype, int ld, int n_rows, int V
  * and the token is the first whose running sum over what is left exceeds u times the whole, u in [0, 1).  temperature <= 0 (or NaN): the
  * largest logit, the lowest id among equals.  Logits: f32 (logits_dtype 0) or bf16 (1), row stride ld >= V elements; NaN is -inf.  A row without any
  * logit above -inf gives token 0 with probability 0.  temperature, top_k, top_p, min_p: [n_rows], or NULL and one value for all rows.
- * prob (optional, f32 [n_rows]): the token's probability among what is left.  Weights are f64, rounded to 2^-45 of the largest (of
- * 2^-(63 - log2 V) beyond 2^18 tokens); the same inputs give the same token in every call. */
+ * prob (optional, f32 [n_rows]): the token's probability among what is left.  Weights are f64, rounded to multiples of 2^-45 of the largest (of
+ * 2^-(63 - log2 V) beyond 2^18 tokens), which moves a border of the running sum by up to V / 2 of them; the same inputs give the same token in
+ * every call. */
 typedef struct jb200_sampling {
   const void* logits;
   long long ld;

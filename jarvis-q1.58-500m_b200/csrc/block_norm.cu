@@ -4,7 +4,7 @@
 // after jarvis_engine/jarvis_model.py:25-26 (RMSNorm) and :428-436 (the residual sums around it).  One pass over memory: rows stay in
 // registers between the sums and the products; sums are f32, each result is rounded once.
 //
-// Bound by memory: 16384 rows of 1024 of residual_norm move 201 MB in 36 us, 5.6 TB/s.  The head norm of as many rows with a gate moves 100 MB in
+// Bound by memory: 16384 rows of 1024 of residual_norm move 201 MB in 37 us, 5.4 TB/s.  The head norm of as many rows with a gate moves 100 MB in
 // 18.5 us, next to its instructions (with exponentials and quotients that mind subnormals, and a division for every vector's row, 21.3); a second
 // vector a thread, or one read ahead, took longer.  Few rows take the launch and one chain of two reads, two sums and a write.
 #include "common.cuh"
@@ -98,7 +98,8 @@ struct RowNorm {
 };
 
 // A CTA a row, V vectors of eight columns a thread.  128 threads up to 1024 columns: a warp a row, eight rows a CTA, reads four times as much at once
-// but took 16384 rows of 1024 in 52 us instead of 39, 2048 in 19 instead of 12.
+// but took 16384 rows of 1024 a third longer and 2048 half again as long.  Above 1024 columns most of a thread's four vectors are idle up to 2048
+// (16384 rows of 1032, bf16, without a gate: 68 us, where 8192 of 2048 take 36 and 2048 of 8192 take 19).
 template <typename TY, typename TO, int THREADS, int V>
 __global__ void __launch_bounds__(THREADS) row_norm_kernel(RowNorm p) {
   __shared__ float part[2][THREADS / 32];

@@ -9,17 +9,20 @@
 //   draw:   the first i whose running sum over what is left exceeds u times the whole
 //
 // All of them ask "which token covers position z of the running sum", top-k with every weight 1.  Weights are taken in f64 and held as integers of
-// 2^-45 of the largest one's, so that sums do not depend on the order of the atomics that form them, and a token that the exact sums choose is
-// missed only where u lies within some 1e-12 of a border.  A cluster of CTAs has a row, a slice each (in shared memory where it fits), with as many
-// CTAs as keep the SMs busy.  A histogram of the sums (for top-k of the counts) over 2048 bins of 1/64 of an e-fold finds the bin that covers z.
-// The tokens of a bin, up to 256, are ranked by comparison with one another; where there are more they are first cut into 512 parts of their order,
+// 2^-45 of the largest one's (of 2^-(63 - log2 V) beyond 2^18 tokens), so that sums do not depend on the order of the atomics that form them.  Each is
+// off by up to half a step, and what is below that is none: a border of the running sum lies up to V / 2 steps off, 7e-10 of the largest weight for 50257
+// tokens, 1.5e-5 for 2^24, and a token that the exact sums choose is missed only where u is that near to one.  A cluster of CTAs has a row, a slice
+// each (in shared memory where it fits), with as many CTAs as keep the SMs busy.  A histogram of the sums (for top-k of the counts) over 2048 bins of
+// 1/64 of an e-fold finds the bin that covers z.  The tokens of a bin, up to 256, are ranked by comparison with one another; where there are more they are first cut into 512 parts of their order,
 // logit then id, until there are not.  What top-k or min-p leaves is listed before it is weighed (and up to 256 ranked at once); where they leave
 // everything, the few tokens near the largest are as the sums are taken: most answers are then found without the slices.  Every CTA counts and lists
-// its slice in its own memory; the first one reads the others' and searches, the others read what it found.
+// its slice in its own memory by atomics.  Behind a meeting each adds up a part of the bins over all CTAs and stores it in the first one's memory
+// (plain stores, another meeting follows); the first one searches, the others read what it found.
 //
-// Bounds: a row alone, the chain of passes, barriers and searches (50257 tokens, nucleus: 25 us, of which the weights 6 and each search 4); many rows,
-// reading them once and again from L2 (256 rows of 50257 f32, min-p: 20 us, the first reading alone 7.8); with a nucleus over everything, the 11
-// f64 operations and the atomics of every token's weight (64 rows of bf16, every setting of its own: 41 us; 256 rows of f32 107).
+// Bounds: a row alone, the chain of passes, barriers and searches (50257 tokens, nucleus: 18 to 27 us, by where the answer lies); many rows, reading
+// them once and again from L2 (256 rows of 50257 f32, min-p: 20 us, the first reading alone 7.8); with a nucleus or the temperature alone over
+// everything, the 11 f64 operations and the atomics of every token's weight (256 rows of f32: 103 and 86 us; 64 rows of bf16, every setting of its own:
+// 37 to 40).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -132,7 +135,7 @@ struct Slice {
   }
   // f(id, values, n) for four neighbours at a time, so that their chains of arithmetic overlap, without those that are all below `lowest`.  Elements
   // that are not aligned come one by one (n 1), with -infinities behind them.  Not unrolled further: a CTA runs most instructions for the first time,
-  // and fetching them is what a row alone waits for (50257 tokens, nucleus: 27 us; two vectors a turn: 49).
+  // and fetching them is what a row alone waits for (50257 tokens, nucleus: two vectors a turn took 49 us where one took 27).
   template <typename F>
   __device__ __forceinline__ void fours(float lowest, F&& f) const {
     const int tail = head + vectors * PER;
@@ -358,7 +361,7 @@ __device__ __forceinline__ void join_parts(Smem& sm) {
   }
 }
 
-// A token of the bin that is searched.  A call, since few tokens are of it.
+// A token of the bin that is searched: few are, but a call (its stack is in cold memory) made a row alone 40 us instead of 27.
 template <typename T>
 __device__ __forceinline__ void take(const Command now, const Row r, bool by_count, u64 place, float x) {
   Smem& sm = own_smem();
@@ -459,7 +462,7 @@ __device__ __forceinline__ void search(const Slice<T, CTAS> slice, int ids, cons
       __syncthreads();
     } else {
       const float lowest = value_of(max(least, sizeof(T) == 2 ? uint32_t(now.from >> ids) << 16 : uint32_t(now.from >> ids)));
-      const float highest = value_of(key_at<T>(now.to, ids));          // infinity's bf16 place has NaN here, which nothing exceeds
+      const float highest = value_of(key_at<T>(now.to, ids));          // a place of infinity has infinity here, which nothing exceeds
       slice.fours(lowest == lowest ? lowest : -INFINITY, [&](int id, const float (&x)[4], int n) {
         bool some = false;
 #pragma unroll
@@ -777,7 +780,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_rows_kernel(Sampling p) {
 
 template <typename T, int CTAS>
 int launch_rows_by(Sampling p, int n_rows, cudaStream_t stream) {
-  // a slice of up to 64 KB is kept, so that two CTAs fit a SM (one row of 16384 tokens 20.6 to 25.3 us, read again from L2 21.0 to 26.6)
+  // a slice of up to 64 KB is kept, so that two CTAs fit a SM (one row of 16384 tokens 20.6 to 25.6 us, read again from L2 20.5 to 26.3; of 50257 24.3 to
+  // 36.6 and 24.6 to 36.9)
   constexpr size_t base = (sizeof(Smem) + 15) / 16 * 16, most = 64 * 1024;
   const size_t slice = size_t((p.V / int(16 / sizeof(T)) + CTAS * THREADS - 1) / (CTAS * THREADS)) * THREADS * 16;
   p.staged = slice <= most;
@@ -787,9 +791,9 @@ int launch_rows_by(Sampling p, int n_rows, cudaStream_t stream) {
   return JB200_OK;
 }
 
-// CTAs a row: as many as two a SM leave room for, slices of 4096 tokens or more.  us with the launch, 50257 bf16: 64 rows with every setting of their
-// own 46, with one CTA a SM 51, with four 61 to 65; one row in eight slices 26, in four 31.  One row of 16384 in four slices 21, whole 25; of 8192 in two
-// 20, whole 19; of 4096 in two 20.5, whole 16.
+// CTAs a row: as many as two a SM leave room for, slices of 4096 tokens or more.  us with the launch from cold, bf16: 64 rows of 50257 with every setting
+// of their own 46, with one CTA a SM 54, with four 58 to 64; one row of 50257 (nucleus, by seed) in eight slices 24 to 37, in four 30 to 41, whole 47 to 68;
+// of 16384 in four 21 to 26, whole 25 to 31; of 8192 in two 21 to 25, whole 19 to 21; of 4096 in two 21, whole 16.
 template <typename T>
 int launch_rows(const Sampling& p, int n_rows, cudaStream_t stream) {
   const int most = 2 * sm_count() / n_rows, wide = p.V / 4096, ctas = most < wide ? most : wide;
