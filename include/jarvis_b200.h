@@ -169,14 +169,16 @@ int jb200_ternary_linear_grouped(const void* x, int M, int K, const uint8_t* pac
  * per (sequence, head), S f32 [64 values][64 keys] as in jb200_attn_scan.  q, k: bf16 rows [B T] of key_heads heads of 64; value head h takes
  * key head h / (H / key_heads).  v, o: bf16 rows of H heads.  log_decay (0 or below; -inf forgets all that was), beta: f32 rows of H.  ld*: row
  * strides in elements, multiples of 8 (ldg of log_decay, ldb of beta: any; ldb 0: as ldg).  JB200_DELTA_NORMALIZE: k and q, of any finite size, are
- * divided by sqrt(|.|^2 + 1e-6).  The caller sees to 0 <= beta |k|^2 <= 2 (normalised: beta <= 2), beyond which the rule itself diverges.
+ * divided by sqrt(|.|^2 + 1e-6).  The caller sees to 0 <= beta |k|^2 <= 2 (normalised: beta <= 2; else a rounding of k to bf16 more),
+ * beyond which the rule itself diverges.
  * lengths: int32 [B] or NULL; rows t >= lengths[b] (clamped to 0..T) of a sequence are not read, their output is 0, and the state is the one after
  * the last row before them.  s_in NULL: zeros.  s_out NULL: not wanted; may be s_in itself, else the two must not overlap; o must overlap no
  * input.  o NULL: the state alone.  scratch:
  * jb200_gated_delta_scratch_bytes (0: may be NULL), 16-byte aligned; NULL where bytes are wanted: sequences are not cut into pieces.
  * Value rows (a column of v, of o; a row of S) are independent of one another: an infinity or NaN in v or in the state stays in its value row and
  * reaches the rows of its chunk of 64 tokens and what follows (from k, q and the gates: in that head).  Of a chunk's largest |beta v| in a value row
- * that row's outputs of earlier tokens of the chunk are off by up to 2^-32 of it. */
+ * that row's outputs of earlier tokens of the chunk are off by up to 2^-32 of it.  The state is good to some 2^-20 of the largest that its value row has
+ * been; in chunks to 1e-4 only where beta |k|^2 is near 2 and a chunk's keys are all but the same (the chunk's system is ill-conditioned there). */
 #define JB200_DELTA_NORMALIZE 1
 typedef struct jb200_delta {
   int B, T, H, key_heads, head_dim, flags;

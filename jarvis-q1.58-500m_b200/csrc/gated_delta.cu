@@ -178,10 +178,11 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 // that brings a bound of its size to 2^15, so that f16's subnormals lie 2^-39 below.  Value rows of S are independent of one another, and so is each
 // one's power: a value row is a column of every product here, so that an infinity, or values far larger than the others, stay in theirs.  With N a
 // bound of a value row's norm, a chunk's S, X and U are at most 2 N + 130 max|b v| there and N' = e^Gc N + 64 max|b v|, since a (I - b k k^T)
-// with b |k|^2 <= 2 enlarges nothing (a chunk has 64 tokens); every eighth chunk N is at most 8 max|S| as well (a row has 64 entries).  max|b v| comes
-// from the preparing groups, and the next chunk's powers are made while T X is formed.  Typical values lie 2^5 to 2^12 below the bound, and 2^15 below
-// it two terms still have an f32's 24 bits.  A row's largest |b v| of a chunk counts for the chunk's earlier tokens too: outputs there are off by up to
-// 2^-32 of it.  K and Q come as bf16 and fit one term, with a power of two per row; their norms are factors of rows and columns.  T X is hi hi + hi lo + lo hi.  What only the output sees (Q S^T, P U)
+// with b |k|^2 <= 2 enlarges nothing (a chunk has 64 tokens); every fourth chunk N is at most 8 max|S| as well (a row has 64 entries).  Keys of norm 1
+// that bf16 has rounded up to 1 + 2^-8 make that 2.0078, which may enlarge a row by 1.0078^64 = 1.65 in a chunk: N' has that much room.  max|b v|
+// comes from the preparing groups, and the next chunk's powers are made while T X is formed.  Typical values lie 2^5 to 2^11 below the bound, and 2^15
+// below it two terms still have an f32's 24 bits.  A row's largest |b v| of a chunk counts for the chunk's earlier tokens too: outputs there are off by
+// up to 2^-32 of it.  K and Q come as bf16 and fit one term, with a power of two per row; their norms are factors of rows and columns.  T X is hi hi + hi lo + lo hi.  What only the output sees (Q S^T, P U)
 // is one term, 2^-12 of a value where the output's own rounding is 2^-9.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int CHUNK = 64;
@@ -946,8 +947,8 @@ struct Follow : Common {
       if (n + 1 < part.chunks) {
         values(n + 1);
         if (w >= 2) {
-          if ((n & 7) == 7) bound = fminf(bound, 8.1f * largest_s() * sm.inverse[n & 1][v_row]);
-          bound = fmaf(whole, bound, 64.5f * most_v);
+          if ((n & 3) == 3) bound = fminf(bound, 8.1f * largest_s() * sm.inverse[n & 1][v_row]);
+          bound = fmaf(1.65f * whole, bound, 64.5f * most_v);
           powers(n + 1);
         }
       }
