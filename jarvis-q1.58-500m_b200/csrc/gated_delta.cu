@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 // reads its other operand once for both, and what bounds these small products is reading (6 KB in 48 cycles, 8 KB in 64, for 32 and 64 of
 // mathematics).  T's blocks come from mma.sync: products of 16 x 16.
 //
-// Bound by that chain, some 6200 cycles a chunk on every SM that has a head (8 sequences of 2048 tokens, 16 heads: 113 us, where reading and writing
+// Bound by that chain, some 6200 cycles a chunk on every SM that has a head (8 sequences of 2048 tokens, 16 heads: 114 us, where reading and writing
 // takes 21; with one power of two for all value rows, which is wrong beside an outlier, 5900 and 107).  With mma.sync alone a chunk took 10800, with these warps' parts but all products unrolled 9600: 77 KB of code, which the SMs fetch
 // again and again.
 //
