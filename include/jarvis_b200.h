@@ -177,8 +177,9 @@ int jb200_ternary_linear_grouped(const void* x, int M, int K, const uint8_t* pac
  * jb200_gated_delta_scratch_bytes (0: may be NULL), 16-byte aligned; NULL where bytes are wanted: sequences are not cut into pieces.
  * Value rows (a column of v, of o; a row of S) are independent of one another: an infinity or NaN in v or in the state stays in its value row and
  * reaches the rows of its chunk of 64 tokens and what follows (from k, q and the gates: in that head).  Of a chunk's largest |beta v| in a value row
- * that row's outputs of earlier tokens of the chunk are off by up to 2^-32 of it.  The state is good to some 2^-20 of the largest that its value row has
- * been; to 1e-4 only where beta |k|^2 is near 2 and keys are all but the same (a chunk's system is ill-conditioned there). */
+ * that row's outputs of earlier tokens of the chunk are off by up to 2^-25 scale |q| of it (normalised, at a scale of 1/8: 2^-28).  The state is good
+ * to some 2^-20 of the largest that its value row has been; to 1e-4 only where beta |k|^2 is near 2 and keys are all but the same (a chunk's system
+ * is ill-conditioned there). */
 #define JB200_DELTA_NORMALIZE 1
 typedef struct jb200_delta {
   int B, T, H, key_heads, head_dim, flags;

@@ -181,9 +181,10 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 // with b |k|^2 <= 2 enlarges nothing (a chunk has 64 tokens); every fourth chunk N is at most 8 max|S| as well (a row has 64 entries).  Keys of norm 1
 // that bf16 has rounded up to 1 + 2^-8 make that 2.0078, which may enlarge a row by 1.0078^64 = 1.65 in a chunk: N' has that much room.  max|b v|
 // comes from the preparing groups, and the next chunk's powers are made while T X is formed.  Typical values lie 2^5 to 2^11 below the bound, and 2^15
-// below it two terms still have an f32's 24 bits.  A row's largest |b v| of a chunk counts for the chunk's earlier tokens too: outputs there are off by
-// up to 2^-32 of it.  K and Q come as bf16 and fit one term, with a power of two per row; their norms are factors of rows and columns.  T X is hi hi + hi lo + lo hi.  What only the output sees (Q S^T, P U)
-// is one term, 2^-12 of a value where the output's own rounding is 2^-9.
+// below it two terms still have an f32's 24 bits.  A row's largest |b v| of a chunk counts for the chunk's earlier tokens too: 2^-39 of the bound an
+// element of S, X and U, outputs there are off by up to 2^-25 scale |q| of it.  K and Q come as bf16 and fit one term, with a power of two per row;
+// their norms are factors of rows and columns.  T X is hi hi + hi lo + lo hi.  What only the output sees (Q S^T, P U) is one term, 2^-12 of a value
+// where the output's own rounding is 2^-9.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int CHUNK = 64;
 constexpr int TILE = CHUNK * D * 2;        // bytes of 64 rows of 128, the 16-byte units of row r at unit ^ (r & 7): the 128-byte swizzle

@@ -7,7 +7,8 @@ three operands: 3 2^-29 of the 24 2^-24 that a token is allowed.
 Those bounds know what came before a token.  A chunk of 64 tokens has one power of two a value row, by the largest b v_i of all of them, so that what comes
 later in the chunk counts as well (`_of_the_chunk`): with X = max (2 N + 130 |b v_i|) brought into [2^14, 2^15), f16's subnormal step 2^-24 rounds an
 element of X and of U by at most 2^-25 / 2^14 X = 2^-39 X.  An error e of every b v_i moves the state's row by at most 64 e (nothing enlarges it), and
-so the output by scale |q| 64 e; one of every u_i by at most as much.  Together scale |q| 128 2^-39 X = scale |q| 2^-32 X, of which 2 N is covered above.
+so the output by scale |q| 64 e; one of every u_i by at most as much, and one of every element of S by scale |q| 8 e.  Together scale |q| 136 2^-39 X, of which
+2 N is covered above.
 """
 import math
 
@@ -25,7 +26,7 @@ def _of_the_chunk(v, b, B, T, H, scale=0.125):
     """What outputs may be off by because of later tokens of their chunk; |q| is 1."""
     bv = (b.to(F64).view(B, T, H, 1) * v.to(F64).view(B, T, H, D)).abs()
     most = torch.cat([c.amax(1, keepdim=True).expand_as(c) for c in bv.split(64, 1)], 1)
-    return (2.0 ** -32 * 130 * scale * most).view(B * T, H * D)
+    return (136 * 2.0 ** -39 * 130 * scale * most).view(B * T, H * D)
 
 
 FORMS = [(2, 1), (2, 10), (2, 64), (2, 190), (3, 777), (1, 1500)]            # token by token, a chunk, chunks, segments
