@@ -171,8 +171,8 @@ __global__ void __launch_bounds__(128) delta_step_kernel(DeltaParams p) {
 // mathematics).  T's blocks come from mma.sync: products of 16 x 16.
 //
 // Bound by that chain, some 6200 cycles a chunk on every SM that has a head (8 sequences of 2048 tokens, 16 heads: 114 us, where reading and writing
-// takes 21; with one power of two for all value rows, which is wrong beside an outlier, 5900 and 107).  With mma.sync alone a chunk took 10800, with these warps' parts but all products unrolled 9600: 77 KB of code, which the SMs fetch
-// again and again.
+// takes 21; with one power of two for all value rows, which is wrong beside an outlier, 5900 and 107).  With mma.sync alone a chunk took 10800, with
+// these warps' parts but all products unrolled 9600: 77 KB of code, which the SMs fetch again and again.
 //
 // Precision: the state is f32 and stays it.  What it is multiplied by and into is f16 in two terms, x = hi + lo (22 bits), at a power of two
 // that brings a bound of its size to 2^15, so that f16's subnormals lie 2^-39 below.  Value rows of S are independent of one another, and so is each

@@ -157,3 +157,31 @@ def test_unit_keys_that_bf16_has_rounded_up(T, H):
     assert torch.isfinite(o).all() and torch.isfinite(S).all()
     if T == 10:
         _check((o, S), (wo, wS, 2 * tol, 2 * off))
+
+
+@pytest.mark.parametrize("B,T", [(2, 10), (2, 190), (1, 1500)])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("where", ["q", "k", "log_decay", "beta"])
+def test_infinities_and_nan_of_keys_and_gates_stay_in_their_head(B, T, bad, where):
+    """The bits of everything else: other heads, other sequences, chunks (tokens, without chunks) before; of a query all but its token's output."""
+    H, at = 3, T // 2
+    q, k, v, g, b, s = _problem(B, T, H, H, seed=18)
+    o, S = _scan((q, k, v, g, b, s), B, T, H)
+    if where in "qk":
+        (q if where == "q" else k)[at, D + 7] = bad                   # sequence 0, head 1
+    else:
+        (g if where == "log_decay" else b)[at, 1] = bad
+    o2, S2 = _scan((q, k, v, g, b, s), B, T, H)
+    same = torch.ones(B * T, H, dtype=torch.bool, device="cuda")
+    if where == "q":
+        assert not torch.isfinite(o2[at, D:2 * D]).any()
+        same[at, 1] = False
+    else:
+        assert not torch.isfinite(S2[0, 1]).any() and not torch.isfinite(o2[T - 1, D:2 * D]).any()
+        same[at // 64 * 64 if T > 24 else at:T, 1] = False
+    same = same.repeat_interleave(D, 1)
+    assert torch.equal(torch.where(same, o, 0.0), torch.where(same, o2, 0.0))
+    others = torch.ones(B, H, dtype=torch.bool, device="cuda")
+    others[0, 1] = where == "q"
+    assert torch.equal(S[others], S2[others])
+    assert _lib.device_status() == 0
