@@ -798,7 +798,8 @@ def _no_tangents(what: str, *tensors):
 
 def _forward_only(what: str, *tensors):
     """These operators have no derivatives: a graph that runs through one would lose its part without a word."""
-    _no_tangents(what, *tensors)
+    if getattr(forward_ad, "_current_level", 0) >= 0:     # as in there, without the call: a single token's host time counts
+        _no_tangents(what, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
